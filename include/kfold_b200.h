@@ -516,6 +516,27 @@ KFB_API int kfb_layernorm(const void* x, void* y, const float* weight, const flo
                   long long x_row_stride, long long y_row_stride, float eps, int in_dtype, int out_dtype, void* stream);
 
 /*
+ * Training: the gradient of LayerNorm, and dropout (the reference trains through torch's autograd; no entry point of its own).
+ *
+ *   kfb_layernorm_bwd: from dy (rows, c) of dy_dtype and x (rows, c) of x_dtype, both contiguous, c <= 1024,
+ *     dx (rows, c) of x_dtype and, where the pointers are not NULL, dweight and dbias fp32 [c]: the sums over all rows, added in an order
+ *     that depends on the sizes alone.  weight: fp32 [c] or NULL (no scale); the offset does not enter.  KFB_BF16 or KFB_FP32 each.
+ *     workspace: kfb_layernorm_bwd_workspace_bytes(c) bytes, or NULL where neither dweight nor dbias is wanted.  rows == 0 gives zeros.
+ *   kfb_dropout: out = (residual +) (kept ? scale x : 0), in fp32; scale = 1 / (1 - p) for a share p of dropped elements.  x (outer, shared, inner) of x_dtype, residual
+ *     (or NULL) and out of out_dtype: bf16 -> bf16, bf16 -> fp32 or fp32 -> fp32; out may be x (of its type) or residual.  The mask
+ *     [outer][inner] is shared along `shared` (1: every element by itself) and never stored: element e takes word e % 4 of
+ *     Philox-4x32-10 at counter (e / 4, offset) and key seed, and is dropped when it is below drop_below = p 2^32 (0 ... 2^32).  rng: NULL, or two int64 in
+ *     device memory (seed, offset) that take the place of the arguments when the kernel runs (a captured graph can then draw a new mask at
+ *     every replay).  The gradient of x is the same call on the gradient of out without residual; the residual's is that gradient itself.
+ */
+KFB_API size_t kfb_layernorm_bwd_workspace_bytes(int c);
+KFB_API int kfb_layernorm_bwd(const void* dy, const void* x, const float* weight, void* dx, float* dweight, float* dbias, void* workspace,
+                              size_t workspace_bytes, long long rows, int c, float eps, int dy_dtype, int x_dtype, void* stream);
+KFB_API int kfb_dropout(const void* x, const void* residual, void* out, long long outer, long long shared, long long inner,
+                        long long drop_below, float scale, const long long* rng, long long seed, long long offset, int x_dtype, int out_dtype,
+                        void* stream);
+
+/*
  * Plain bf16 GEMM on the tcgen05 path: D[b, m, n] = sum_k A[b, m, k] * B[b, n, k]  (+ bias[n]).
  * The building block every projection and the triangle contraction run on; exported
  * so that it can be checked in isolation.  lda / ldb / ldd are row strides, the

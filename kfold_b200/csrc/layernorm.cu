@@ -4,6 +4,7 @@
 #include "layernorm.cuh"
 
 #include "gemm.cuh"  // part_a
+#include "vec_io.cuh"
 
 #include <type_traits>
 
@@ -298,9 +299,67 @@ static int dispatch_g(cudaStream_t stream, const void* x, void* y, const float* 
   return KFB_ERR_UNSUPPORTED;
 }
 
+// Rows that the kernels above, which move pairs of channels, do not take: an odd width or row stride, or a tensor that starts between two
+// pairs.  A warp per row, a channel per lane and access; the same two passes.
+template <typename TI, typename TO, int P>
+__global__ void __launch_bounds__(256) layernorm_single_kernel(const TI* x, TO* y, const float* w, const float* b, long long rows, int c,
+                                                               long long xs, long long ys, float eps) {
+  grid_dependency_enter();
+  const int lane = threadIdx.x & 31;
+  const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
+  for (long long row = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); row < rows; row += warps) {
+    float v[P], s = 0.f, q = 0.f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      v[p] = p * 32 + lane < c ? load1(x + row * xs + p * 32 + lane) : 0.f;
+      s += v[p];
+    }
+    const float mean = warp_sum(s) / static_cast<float>(c);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      v[p] = p * 32 + lane < c ? v[p] - mean : 0.f;
+      q = fmaf(v[p], v[p], q);
+    }
+    const float rstd = rsqrtf(warp_sum(q) / static_cast<float>(c) + eps);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int ch = p * 32 + lane;
+      v[p] = fmaf(v[p] * rstd, w != nullptr && ch < c ? w[ch] : 1.0f, b != nullptr && ch < c ? b[ch] : 0.0f);
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int ch = p * 32 + lane;
+      if (ch < c) store_vec<1>(y + row * ys + ch, &v[p]);
+    }
+  }
+}
+
+template <typename TI, typename TO>
+static int launch_single(cudaStream_t stream, const void* x, void* y, const float* w, const float* b, long long rows, int c, long long xs,
+                         long long ys, float eps) {
+  if (c > 1024) {
+    set_error("layernorm: channel count %d above 1024 is not supported", c);
+    return KFB_ERR_UNSUPPORTED;
+  }
+  const long long want = (rows + 7) / 8, most = static_cast<long long>(sm_count()) * 16;
+  auto kernel = c <= 256 ? layernorm_single_kernel<TI, TO, 8> : layernorm_single_kernel<TI, TO, 32>;
+  LaunchScope scope(stream, "layernorm_single");
+  return launch_kernel(stream, kernel, static_cast<unsigned>(want < most ? want : most), 256, 0, static_cast<const TI*>(x), static_cast<TO*>(y), w,
+                       b, rows, c, xs, ys, eps);
+}
+
 int launch_layernorm(cudaStream_t stream, const void* x, void* y, const float* w, const float* b, long long rows, int c,
                      long long xs, long long ys, float eps, int in_dtype, int out_dtype, RowPerm perm) {
-  KFB_CHECK_ARG(rows >= 0 && c > 0 && c % 2 == 0, "layernorm: rows %lld, channels %d (must be even)", rows, c);
+  const uintptr_t pair_x = in_dtype == KFB_BF16 ? 4 : 8, pair_y = out_dtype == KFB_BF16 ? 4 : 8;
+  if (rows > 0 && c > 0 && perm.rows == 0 &&
+      (c % 2 != 0 || xs % 2 != 0 || ys % 2 != 0 || reinterpret_cast<uintptr_t>(x) % pair_x != 0 || reinterpret_cast<uintptr_t>(y) % pair_y != 0 ||
+       ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(b)) & 7) != 0)) {
+    if (in_dtype == KFB_BF16 && out_dtype == KFB_BF16) return launch_single<__nv_bfloat16, __nv_bfloat16>(stream, x, y, w, b, rows, c, xs, ys, eps);
+    if (in_dtype == KFB_FP32 && out_dtype == KFB_BF16) return launch_single<float, __nv_bfloat16>(stream, x, y, w, b, rows, c, xs, ys, eps);
+    if (in_dtype == KFB_FP32 && out_dtype == KFB_FP32) return launch_single<float, float>(stream, x, y, w, b, rows, c, xs, ys, eps);
+    if (in_dtype == KFB_BF16 && out_dtype == KFB_FP32) return launch_single<__nv_bfloat16, float>(stream, x, y, w, b, rows, c, xs, ys, eps);
+  }
+  KFB_CHECK_ARG(rows >= 0 && c > 0 && (c % 2 == 0 || rows == 0), "layernorm: rows %lld, channels %d (must be even)", rows, c);
   KFB_CHECK_ARG(perm.rows == 0 || (perm.n % perm.rows == 0 && rows == static_cast<long long>(perm.rows) * perm.n),
                 "layernorm: exchange order needs a (%d, %d) shard, got %lld rows", perm.rows, perm.n, rows);
   KFB_CHECK_ARG(xs % 2 == 0 && ys % 2 == 0, "layernorm: row strides must be even");

@@ -1,0 +1,271 @@
+// The gradient of LayerNorm.  With m, r the row's mean and 1 / sqrt(var + eps), z = (x - m) r and g = w dy:
+//   dx = r (g - mean(g) - z mean(g z)),   dw = sum over rows of dy z,   db = sum over rows of dy.
+//
+// What bounds it: x and dy in, dx out, and nothing else is large, so HBM.  The statistics are taken again from the row, which is in registers
+// anyway, instead of being saved by the forward pass (8 bytes a row and two more tensors for the caller to keep).
+// Split: a row is held by 8, 16 or 32 lanes, in 16-byte pieces where the width allows; a warp has enough rows in flight to cover the memory's
+// latency, keeps its lanes' shares of dw and db in registers from row to row, and a block leaves one row of partial sums.  A second kernel adds
+// those in the blocks' order, so that the result does not hang on which block was first: no atomics.
+#include <cuda_bf16.h>
+
+#include <mutex>
+#include <type_traits>
+
+#include "ops_common.cuh"
+#include "vec_io.cuh"
+
+namespace kfb {
+namespace {
+
+constexpr int kWarps = 8;
+
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int m = LANES / 2; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
+
+// LANES lanes hold a row, P pieces of V channels each; R rows in flight for each group of lanes.  EXACT: c == LANES * V * P.  PARAMS: dw, db wanted.
+template <typename TX, typename TD, int V, int LANES, int P, int R, bool EXACT, bool PARAMS>
+__global__ void __launch_bounds__(32 * kWarps) layernorm_grad_kernel(const TD* dy, const TX* x, const float* w, TX* dx, float* partial, long long rows,
+                                                                     int c, float eps) {
+  constexpr int N = P * V, kGroups = 32 / LANES, kRows = kGroups * R;
+  grid_dependency_enter();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LANES;
+  const float inv_c = 1.0f / static_cast<float>(c);
+  auto channel = [&](int p) { return (p * LANES + sub) * V; };
+  auto inside = [&](int p) { return EXACT || channel(p) < c; };
+  float wv[N], aw[PARAMS ? N : 1], ab[PARAMS ? N : 1];
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+#pragma unroll
+    for (int i = 0; i < V; ++i) wv[p * V + i] = w != nullptr && inside(p) ? w[channel(p) + i] : 1.0f;
+#pragma unroll
+  for (int i = 0; i < (PARAMS ? N : 1); ++i) aw[i] = ab[i] = 0.f;
+
+  const long long warps = static_cast<long long>(gridDim.x) * kWarps;
+  for (long long base = (static_cast<long long>(blockIdx.x) * kWarps + warp) * kRows; base < rows; base += warps * kRows) {
+    float xv[R][N], dv[R][N];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long row = base + r * kGroups + lane / LANES;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        if (row < rows && inside(p)) {
+          load_vec<V>(x + row * c + channel(p), &xv[r][p * V]);
+          load_vec<V>(dy + row * c + channel(p), &dv[r][p * V]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) xv[r][p * V + i] = dv[r][p * V + i] = 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long row = base + r * kGroups + lane / LANES;
+      float s = 0.f, sg = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        s += xv[r][i];
+        sg = fmaf(dv[r][i], wv[i], sg);
+      }
+      const float mean = lanes_sum<LANES>(s) * inv_c;
+      sg = lanes_sum<LANES>(sg) * inv_c;
+      float q = 0.f, sz = 0.f;
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = p * V; i < p * V + V; ++i) {
+          xv[r][i] = inside(p) ? xv[r][i] - mean : 0.f;
+          q = fmaf(xv[r][i], xv[r][i], q);
+          sz = fmaf(dv[r][i] * wv[i], xv[r][i], sz);
+        }
+      const float rstd = rsqrtf(lanes_sum<LANES>(q) * inv_c + eps);
+      sz = lanes_sum<LANES>(sz) * inv_c * rstd;
+      if (row < rows) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          float o[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float z = xv[r][p * V + i] * rstd, d = dv[r][p * V + i];
+            o[i] = rstd * (fmaf(d, wv[p * V + i], -sg) - z * sz);
+            if constexpr (PARAMS) {
+              aw[p * V + i] = fmaf(d, z, aw[p * V + i]);
+              ab[p * V + i] += d;
+            }
+          }
+          if (inside(p)) store_vec<V>(dx + row * c + channel(p), o);
+        }
+      }
+    }
+  }
+
+  if constexpr (PARAMS) {
+    __shared__ float s_sum[kWarps][LANES * N];
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float(&a)[N] = which ? ab : aw;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int m = LANES; m < 32; m <<= 1) a[i] += __shfl_xor_sync(0xffffffffu, a[i], m);
+      }
+      if (lane < LANES) {
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int i = 0; i < V; ++i) s_sum[warp][channel(p) + i] = a[p * V + i];
+      }
+      __syncthreads();
+      for (int ch = threadIdx.x; ch < c; ch += 32 * kWarps) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) t += s_sum[k][ch];
+        partial[(static_cast<long long>(blockIdx.x) * 2 + which) * c + ch] = t;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// dw and db (either may be null) from the blocks' partial sums, in the order of the blocks.  A block takes 32 channels of the 2 c.
+__global__ void __launch_bounds__(1024) layernorm_grad_sum_kernel(const float* partial, float* dw, float* db, int blocks, int c) {
+  __shared__ float s[32][33];
+  grid_dependency_enter();
+  const int col = blockIdx.x * 32 + threadIdx.x % 32, part = threadIdx.x / 32;
+  float t = 0.f;
+  if (col < 2 * c) {
+#pragma unroll 4
+    for (int b = part; b < blocks; b += 32) t += partial[static_cast<long long>(b) * 2 * c + col];
+  }
+  s[part][threadIdx.x % 32] = t;
+  __syncthreads();
+  if (part == 0 && col < 2 * c) {
+    t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) t += s[k][threadIdx.x];
+    if (col < c) {
+      if (dw != nullptr) dw[col] = t;
+    } else if (db != nullptr) {
+      db[col - c] = t;
+    }
+  }
+}
+
+constexpr int kBlocksPerSm = 8;      // at most: the workspace's partial sums are sized by it
+constexpr int kMostSms = 160;
+
+struct Args {
+  cudaStream_t stream;
+  const void *dy, *x;
+  const float* w;
+  void* dx;
+  float *dw, *db, *partial;
+  long long rows;
+  int c;
+  float eps;
+};
+
+template <typename TX, typename TD, int V, int LANES, int P, bool EXACT, bool PARAMS>
+int launch_params(const Args& a) {
+  constexpr int N = V * P, R = N <= 8 ? 2 : 1;
+  auto kernel = layernorm_grad_kernel<TX, TD, V, LANES, P, R, EXACT, PARAMS>;
+  static std::once_flag once;
+  static int held = 1;
+  std::call_once(once, [&] {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, 32 * kWarps, 0) != cudaSuccess) cudaGetLastError();
+    held = held < 1 ? 1 : held > kBlocksPerSm ? kBlocksPerSm : held;
+  });
+  const int sms = sm_count() < kMostSms ? sm_count() : kMostSms;
+  const long long step = static_cast<long long>(kWarps) * (32 / LANES) * R, want = (a.rows + step - 1) / step;
+  const int blocks = static_cast<int>(want < static_cast<long long>(sms) * held ? want : static_cast<long long>(sms) * held);
+  {
+    LaunchScope scope(a.stream, "layernorm_grad");
+    KFB_TRY(launch_kernel(a.stream, kernel, blocks, 32 * kWarps, 0, static_cast<const TD*>(a.dy), static_cast<const TX*>(a.x), a.w,
+                          static_cast<TX*>(a.dx), a.partial, a.rows, a.c, a.eps));
+  }
+  if (PARAMS) {
+    LaunchScope scope(a.stream, "layernorm_grad_sum");
+    KFB_TRY(launch_kernel(a.stream, layernorm_grad_sum_kernel, cdiv(2 * a.c, 32), 1024, 0, const_cast<const float*>(a.partial), a.dw, a.db, blocks,
+                          a.c));
+  }
+  return KFB_OK;
+}
+
+template <typename TX, typename TD, int V, int LANES, int P, bool EXACT>
+int launch(const Args& a) {
+  return a.dw != nullptr || a.db != nullptr ? launch_params<TX, TD, V, LANES, P, EXACT, true>(a) : launch_params<TX, TD, V, LANES, P, EXACT, false>(a);
+}
+
+template <typename TX, typename TD>
+int dispatch(const Args& a) {
+  constexpr bool kHalf = std::is_same<TX, __nv_bfloat16>::value && std::is_same<TD, __nv_bfloat16>::value;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.dx);
+  if ((at & 15) == 0) {
+    if constexpr (kHalf) {
+      switch (a.c) {
+        case 64: return launch<TX, TD, 8, 8, 1, true>(a);
+        case 128: return launch<TX, TD, 8, 16, 1, true>(a);
+        case 256: return launch<TX, TD, 8, 32, 1, true>(a);
+        case 384: return launch<TX, TD, 8, 16, 3, true>(a);
+        case 768: return launch<TX, TD, 8, 32, 3, true>(a);
+      }
+    } else {
+      switch (a.c) {
+        case 64: return launch<TX, TD, 4, 16, 1, true>(a);
+        case 128: return launch<TX, TD, 4, 32, 1, true>(a);
+        case 256: return launch<TX, TD, 4, 32, 2, true>(a);
+        case 384: return launch<TX, TD, 4, 32, 3, true>(a);
+        case 768: return launch<TX, TD, 4, 32, 6, true>(a);
+      }
+    }
+    if (a.c % 4 == 0) {
+      if (a.c <= 256) return launch<TX, TD, 4, 32, 2, false>(a);
+      if (a.c <= 512) return launch<TX, TD, 4, 32, 4, false>(a);
+      return launch<TX, TD, 4, 32, 8, false>(a);
+    }
+  }
+  if (a.c <= 256) return launch<TX, TD, 1, 32, 8, false>(a);
+  return launch<TX, TD, 1, 32, 32, false>(a);
+}
+
+}  // namespace
+}  // namespace kfb
+
+using namespace kfb;
+
+extern "C" {
+
+KFB_API size_t kfb_layernorm_bwd_workspace_bytes(int c) {
+  return align_up(static_cast<size_t>(kMostSms) * kBlocksPerSm * 2 * (c > 0 ? c : 0) * sizeof(float), 256);
+}
+
+KFB_API int kfb_layernorm_bwd(const void* dy, const void* x, const float* weight, void* dx, float* dweight, float* dbias, void* workspace,
+                              size_t workspace_bytes, long long rows, int c, float eps, int dy_dtype, int x_dtype, void* stream) {
+  KFB_CHECK_ARG(rows >= 0 && c > 0, "layernorm_bwd: rows %lld, channels %d", rows, c);
+  if (c > 1024) {
+    set_error("layernorm_bwd: channel count %d above 1024 is not supported", c);
+    return KFB_ERR_UNSUPPORTED;
+  }
+  const bool params = dweight != nullptr || dbias != nullptr;
+  KFB_CHECK_ARG((dy_dtype == KFB_BF16 || dy_dtype == KFB_FP32) && (x_dtype == KFB_BF16 || x_dtype == KFB_FP32), "layernorm_bwd: bad dtype %d / %d",
+                dy_dtype, x_dtype);
+  cudaStream_t s = as_stream(stream);
+  if (rows == 0) {
+    if (dweight != nullptr) KFB_CUDA(cudaMemsetAsync(dweight, 0, static_cast<size_t>(c) * 4, s));
+    if (dbias != nullptr) KFB_CUDA(cudaMemsetAsync(dbias, 0, static_cast<size_t>(c) * 4, s));
+    return KFB_OK;
+  }
+  KFB_CHECK_ARG(dy != nullptr && x != nullptr && dx != nullptr, "layernorm_bwd: null tensor");
+  KFB_CHECK_ARG(!params || (workspace != nullptr && workspace_bytes >= kfb_layernorm_bwd_workspace_bytes(c)),
+                "layernorm_bwd: workspace %zu < %zu bytes", workspace_bytes, kfb_layernorm_bwd_workspace_bytes(c));
+  KFB_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "layernorm_bwd: workspace must be 256-byte aligned");
+  const Args a = {s, dy, x, weight, dx, dweight, dbias, static_cast<float*>(workspace), rows, c, eps};
+  if (x_dtype == KFB_BF16)
+    return dy_dtype == KFB_BF16 ? dispatch<__nv_bfloat16, __nv_bfloat16>(a) : dispatch<__nv_bfloat16, float>(a);
+  return dy_dtype == KFB_BF16 ? dispatch<float, __nv_bfloat16>(a) : dispatch<float, float>(a);
+}
+
+}  // extern "C"

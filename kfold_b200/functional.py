@@ -7,6 +7,7 @@ and the extension must be built.
 """
 from __future__ import annotations
 
+import math
 
 import torch
 
@@ -104,6 +105,81 @@ def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype=None)
         L.check(L.lib().kfb_layernorm(L.ptr(x2), L.ptr(out), L.ptr(w), L.ptr(b), x2.shape[0], c, x2.stride(0), c, eps,
                                       L.dtype_code(x2.dtype), L.dtype_code(out.dtype), L.stream_ptr()))
     return out.view(*x.shape[:-1], c)
+
+
+def _same_device(name: str, *ts: torch.Tensor | None) -> None:
+    """A kernel follows every pointer on one GPU: refuse a mixture."""
+    devices = {t.device for t in ts if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"{name}: tensors on {', '.join(sorted(map(str, devices)))}")
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-5, need_weight: bool = True,
+                        need_bias: bool = True):
+    """Gradient of ``layer_norm(x, weight, bias, eps)``: (dx, dweight, dbias) from dy, of y's shape, bfloat16 or float32.
+
+    dx is of x's dtype, dweight and dbias float32 (None without a weight or where not asked for).  Any width up to 1024.  The row's
+    statistics are taken from x again, nothing has to be kept from the forward pass; sums over the rows have a fixed order."""
+    _require_cuda(dy, x, weight)
+    _same_device("layer_norm_backward", dy, x, weight)
+    c = x.shape[-1]
+    if dy.shape != x.shape or (weight is not None and tuple(weight.shape) != (c,)):
+        raise ValueError(f"layer_norm_backward: dy {tuple(dy.shape)}, weight {None if weight is None else tuple(weight.shape)} for x {tuple(x.shape)}")
+    need_weight = need_weight and weight is not None
+    x2, d2 = x.reshape(-1, c).contiguous(), dy.reshape(-1, c).contiguous()
+    w = None if weight is None else weight.detach().float().contiguous()
+    dx = torch.empty_like(x2)
+    dw = torch.empty(c, dtype=torch.float32, device=x.device) if need_weight else None
+    db = torch.empty(c, dtype=torch.float32, device=x.device) if need_bias else None
+    lib = L.lib()
+    with L.on_device(x.device):
+        ws = _workspace(x.device, lib.kfb_layernorm_bwd_workspace_bytes(c)) if need_weight or need_bias else None
+        L.check(lib.kfb_layernorm_bwd(L.ptr(d2), L.ptr(x2), L.ptr(w), L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), 0 if ws is None else ws.numel(),
+                                      x2.shape[0], c, eps, L.dtype_code(d2.dtype), L.dtype_code(x2.dtype), L.stream_ptr()))
+    return dx.view(x.shape), dw, db
+
+
+def _signed64(v: int) -> int:
+    return v - (1 << 64) if v >= 1 << 63 else v
+
+
+def dropout(x: torch.Tensor, p: float, rng, shared_dim: int | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """(residual +) dropout(x): an element is dropped with probability p, the others are multiplied by 1 / (1 - p).
+
+    ``rng`` is (seed, offset), two integers below 2^64, or an int64 CUDA tensor of the two that the kernel reads when it runs (for
+    captured graphs).  The mask is a function of them and of the element's number alone (Philox-4x32-10: element e of the row-major mask
+    takes word e % 4 of block e // 4 and is dropped below p 2^32) and is never stored: the gradient of x is ``dropout(dout, p, rng,
+    shared_dim)`` with the same ``rng``, the residual's is dout.  ``shared_dim``: the mask has extent one along this dim of x, as row-wise
+    (-3) and column-wise (-2) dropout of a pair tensor have it.  ``residual``, of x's shape, gives the result its dtype (float32 also for a
+    bfloat16 x)."""
+    _require_cuda(x, residual)
+    _same_device("dropout", x, residual, rng if isinstance(rng, torch.Tensor) else None)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout: p = {p}")
+    if residual is not None and (residual.shape != x.shape or (residual.dtype != x.dtype and residual.dtype != torch.float32)):
+        raise ValueError(f"dropout: residual {residual.dtype} {tuple(residual.shape)} for x {x.dtype} {tuple(x.shape)}")
+    state, seed, offset = None, 0, 0
+    if isinstance(rng, torch.Tensor):
+        if not rng.is_cuda or rng.dtype != torch.int64 or tuple(rng.shape) != (2,) or not rng.is_contiguous():
+            raise ValueError("dropout: rng is a pair of integers or a contiguous int64 CUDA tensor of two")
+        state = rng
+    else:
+        seed, offset = (int(v) for v in rng)
+        if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
+            raise ValueError(f"dropout: seed {seed} and offset {offset} are not in [0, 2^64)")
+    outer, shared, inner = 1, 1, x.numel()
+    if shared_dim is not None:
+        if not -x.dim() <= shared_dim < x.dim():
+            raise ValueError(f"dropout: dim {shared_dim} of x {tuple(x.shape)}")
+        d = shared_dim % x.dim()
+        outer, shared, inner = math.prod(x.shape[:d]), x.shape[d], math.prod(x.shape[d + 1:])
+    xc, rc = x.contiguous(), None if residual is None else residual.contiguous()
+    out = torch.empty(x.shape, dtype=x.dtype if residual is None else residual.dtype, device=x.device)
+    scale = 1.0 / (1.0 - p) if p < 1.0 else 0.0
+    with L.on_device(x.device):
+        L.check(L.lib().kfb_dropout(L.ptr(xc), L.ptr(rc), L.ptr(out), outer, shared, inner, int(p * 4294967296.0 + 0.5), scale, L.ptr(state),
+                                    _signed64(seed), _signed64(offset), L.dtype_code(x.dtype), L.dtype_code(out.dtype), L.stream_ptr()))
+    return out
 
 
 def triangle_multiplication(x: torch.Tensor, mask: torch.Tensor, packed: dict, direction: str, eps: float = 1e-5,

@@ -1,0 +1,54 @@
+"""What the training operators refuse, and the generator the dropout's mask comes from (no GPU)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import plain_training as P
+from kfold_b200 import functional as F
+
+
+@pytest.fixture(scope="module")
+def library():
+    from kfold_b200 import _lib, build
+    build.build()
+    return _lib.lib()
+
+
+@pytest.mark.parametrize("block, offset, seed, words", [
+    (0, 0, 0, (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+    (2 ** 64 - 1, 2 ** 64 - 1, 2 ** 64 - 1, (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+    (0x85A308D3243F6A88, 0x0370734413198A2E, 0x299F31D0A4093822, (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1)),
+])
+def test_generator_gives_the_published_words(block, offset, seed, words):
+    """The known answers that the method's authors publish."""
+    assert tuple(P.philox(np.array([block], dtype=np.uint64), offset, seed)[0].tolist()) == words
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 8)
+    for call in (lambda: F.layer_norm_backward(x, x, None), lambda: F.dropout(x, 0.1, (1, 2))):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+def test_layernorm_bwd_refuses_before_any_cuda_call(library):
+    vp, some = ctypes.c_void_p, 256
+    need = library.kfb_layernorm_bwd_workspace_bytes(64)
+    call = lambda dy=some, x=some, dx=some, dw=some, ws=some, size=need, rows=3, c=64, dt=0: library.kfb_layernorm_bwd(
+        vp(dy), vp(x), None, vp(dx), vp(dw), None, vp(ws), size, rows, c, 1e-5, dt, 0, None)
+    assert call(dy=None) == call(x=None) == call(dx=None) == 1
+    assert call(rows=-1) == call(c=0) == call(dt=2) == call(dt=7) == 1
+    assert call(ws=None) == call(size=need - 1) == call(ws=some + 8) == 1
+    assert b"aligned" in library.kfb_last_error()
+    assert call(c=1025, size=1 << 30) == 2
+
+
+def test_dropout_refuses_before_any_cuda_call(library):
+    vp, some = ctypes.c_void_p, 256
+    call = lambda x=some, out=some, n=8, below=1 << 30, xt=0, ot=0: library.kfb_dropout(vp(x), None, vp(out), 1, 1, n, below, 1.5, None, 1, 2, xt, ot, None)
+    assert call(x=None) == call(out=None) == call(n=-1) == 1
+    assert call(below=-1) == call(below=(1 << 32) + 1) == 1
+    assert call(xt=1, ot=0) == call(xt=2) == call(ot=5) == 1
+    assert call(n=0) == 0

@@ -529,6 +529,21 @@ KFB_API int kfb_layernorm(const void* x, void* y, const float* weight, const flo
  *     device memory (seed, offset) that take the place of the arguments when the kernel runs (a captured graph can then draw a new mask at
  *     every replay).  The gradient of x is the same call on the gradient of out without residual; the residual's is that gradient itself.
  */
+/*
+ * Gated feed-forward y = (silu(x Wa^T) * (x Wb^T)) Wo^T, [Wa; Wb] = w_in, and its gradient: SwiGLU and output projection of
+ * Transition.forward (src/kfold/model/layers/folding/transition.py:48-68) in training, on the plain (not packed) parameters.
+ *   x, out, dy, dx (rows, c), w_in, dw_in (2 hidden, c), w_out, dw_out (c, hidden), row-major, 16-byte aligned; c and hidden multiples of 8.
+ *   dtype KFB_BF16: all bf16, products with fp32 accumulation, only the operands h, da, db are rounded in between; KFB_FP32_PRECISE: all
+ *   fp32 at fp32 accuracy.  grad_dtype: of dw_in and dw_out, KFB_BF16 or KFB_FP32 (always fp32 in the fp32-accurate mode).  dx, dw_in and
+ *   dw_out may each be NULL (not wanted); rows == 0 gives zero gradients of the weights.  The sums over rows have an order that depends on
+ *   the sizes alone.  workspace: kfb_feed_forward_workspace_bytes(..., backward) bytes; it stops growing at some ten thousand rows.
+ */
+KFB_API size_t kfb_feed_forward_workspace_bytes(long long rows, int c, int hidden, int dtype, int backward);
+KFB_API int kfb_feed_forward_fwd(const void* x, const void* w_in, const void* w_out, void* out, void* workspace, size_t workspace_bytes,
+                                 long long rows, int c, int hidden, int dtype, void* stream);
+KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in, const void* w_out, void* dx, void* dw_in, void* dw_out,
+                                 void* workspace, size_t workspace_bytes, long long rows, int c, int hidden, int dtype, int grad_dtype,
+                                 void* stream);
 KFB_API size_t kfb_layernorm_bwd_workspace_bytes(int c);
 KFB_API int kfb_layernorm_bwd(const void* dy, const void* x, const float* weight, void* dx, float* dweight, float* dbias, void* workspace,
                               size_t workspace_bytes, long long rows, int c, float eps, int dy_dtype, int x_dtype, void* stream);

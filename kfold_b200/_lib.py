@@ -129,12 +129,15 @@ _SIGNATURES = {
                            c_int, c_int, c_void_p],
     "kfb_atom_stack_fwd": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_ll, c_void_p, c_int, c_int,
                            c_void_p, ctypes.c_size_t] + [c_int] * 6 + [c_float, c_void_p],
+    "kfb_feed_forward_fwd": [c_void_p] * 5 + [ctypes.c_size_t, c_ll, c_int, c_int, c_int, c_void_p],
+    "kfb_feed_forward_bwd": [c_void_p] * 8 + [ctypes.c_size_t, c_ll, c_int, c_int, c_int, c_int, c_void_p],
     "kfb_layernorm_bwd": [c_void_p] * 7 + [ctypes.c_size_t, c_ll, c_int, c_float, c_int, c_int, c_void_p],
     "kfb_dropout": [c_void_p, c_void_p, c_void_p, c_ll, c_ll, c_ll, c_ll, c_float, c_void_p, c_ll, c_ll, c_int, c_int, c_void_p],
     "kfb_transition_fwd_static": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_int, c_int,
                                   c_float, c_int, c_void_p],
 }
 _SIZE_FUNCS = {
+    "kfb_feed_forward_workspace_bytes": [c_ll, c_int, c_int, c_int, c_int],
     "kfb_layernorm_bwd_workspace_bytes": [c_int],
     "kfb_triatt_workspace_bytes_precise": [c_int, c_int, c_int, c_int],
     "kfb_apb_workspace_bytes_precise": [c_int, c_int, c_int],

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 #include "../../include/kfold_b200.h"
 
 namespace kfb {
@@ -117,6 +119,18 @@ inline int clusters_held(void (*kernel)(KArgs...), unsigned cluster, int threads
     return held;
   cudaGetLastError();
   return 0;
+}
+
+// Allows a kernel its shared memory on the current device, once per device.
+template <auto kernel>
+inline int allow_smem(int bytes) {
+  static std::once_flag once[64];
+  int dev = 0;
+  KFB_CUDA(cudaGetDevice(&dev));
+  cudaError_t err = cudaSuccess;
+  std::call_once(once[dev & 63], [&] { err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+  KFB_CUDA(err);
+  return KFB_OK;
 }
 
 #ifdef __CUDACC__

@@ -1,0 +1,292 @@
+// D[m][n] = sum_k A(m, k) B(n, k) for operands stored along k or across it (see matmul.cuh).
+//
+// A CTA computes one 128 x 128 tile of one piece of k: a thread fetches 64-wide blocks of both operands with TMA into a ring, a thread issues
+// the products, four warps bring the accumulator from tensor memory to global memory.  Two CTAs share an SM, so that one's start and end lie
+// under the other's products.  An operand stored across k ([k][i]) is fetched as two boxes of 64 k by 64 i and read MN-major as it lies: the
+// gradients of weights contract over rows, and nothing is transposed for them.
+// fp32-accurate mode: three parts an operand, six products, x0 w0 in an accumulator of its own (the tensor core cuts off relative to the
+// accumulator at every step: the five small ones keep their small error apart).
+#include "matmul.cuh"
+
+#include "gemm.cuh"   // split3, epi_store_chunk
+#include "ops_common.cuh"
+#include "ptx.cuh"
+
+namespace kfb {
+namespace {
+
+constexpr int kTile = 128, kK = 64;
+constexpr int kOperand = kTile * kK * 2;           // bytes of a block of one operand
+constexpr int kStage = 2 * kOperand;
+constexpr int kThreads = 192;                      // TMA, products, four warps of rows
+
+struct MmParams {
+  int m, n, m_tiles, n_tiles;
+  int blocks, per_split;                           // of 64 along k: all, of a piece
+  EpiSeg out;
+  long long plane_d;
+  int accumulate;
+};
+
+template <int PARTS>
+constexpr int stages() { return PARTS == 3 ? 6 : 3; }
+template <int PARTS>
+constexpr int smem_bytes() { return stages<PARTS>() * kStage + 1024 + 256; }
+
+__device__ __forceinline__ uint64_t by_k_desc(uint32_t addr) {
+  // 128-byte swizzled rows of 64 i, one per k: eight of them (a swizzle atom) 1024 bytes apart, the next 64 i half an operand further
+  return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | (static_cast<uint64_t>((kOperand / 2) >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+template <bool A_BY_K, bool B_BY_K, int PARTS>
+__global__ void __launch_bounds__(kThreads, PARTS == 3 ? 1 : 2)
+matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const MmParams p) {
+  constexpr int kStages = stages<PARTS>();
+  constexpr uint32_t kCols = PARTS == 3 ? 256 : 128;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * kStage);
+  uint64_t* empty = full + kStages;
+  uint64_t* done = empty + kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int m_tile = blockIdx.x % p.m_tiles, n_tile = blockIdx.x / p.m_tiles, split = blockIdx.y;
+  const int first = split * p.per_split, last = min(first + p.per_split, p.blocks);
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tmap(&tm_a);
+    ptx::prefetch_tmap(&tm_b);
+    for (int i = 0; i < kStages; ++i) {
+      ptx::mbar_init(&full[i], 1);
+      ptx::mbar_init(&empty[i], 1);
+    }
+    ptx::mbar_init(done, 1);
+    ptx::fence_barrier_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(tmem_slot, kCols);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_enter();
+
+  if (warp == 0) {
+    if (ptx::elect_one()) {
+      int st = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int kb = first; ok && kb < last; ++kb)
+        for (int part = 0; part < PARTS; ++part) {
+          ok = ptx::mbar_wait(&empty[st], ph ^ 1, 501);
+          if (!ok) break;
+          ptx::mbar_expect_tx(&full[st], kStage);
+          uint8_t *a = ring + st * kStage, *b = a + kOperand;
+          if (A_BY_K) {
+            ptx::tma_load_3d(a, &tm_a, &full[st], m_tile * kTile, kb * kK, part);
+            ptx::tma_load_3d(a + kOperand / 2, &tm_a, &full[st], m_tile * kTile + 64, kb * kK, part);
+          } else {
+            ptx::tma_load_3d(a, &tm_a, &full[st], kb * kK, m_tile * kTile, part);
+          }
+          if (B_BY_K) {
+            ptx::tma_load_3d(b, &tm_b, &full[st], n_tile * kTile, kb * kK, part);
+            ptx::tma_load_3d(b + kOperand / 2, &tm_b, &full[st], n_tile * kTile + 64, kb * kK, part);
+          } else {
+            ptx::tma_load_3d(b, &tm_b, &full[st], kb * kK, n_tile * kTile, part);
+          }
+          if (++st == kStages) { st = 0; ph ^= 1u; }
+        }
+    }
+  } else if (warp == 1) {
+    if (ptx::elect_one()) {
+      constexpr uint32_t idesc = ptx::make_idesc(kTile, kTile, 1) | (A_BY_K ? 1u << 15 : 0u) | (B_BY_K ? 1u << 16 : 0u);
+      constexpr uint32_t a_step = A_BY_K ? 2048 >> 4 : 2, b_step = B_BY_K ? 2048 >> 4 : 2;     // of 16 k
+      int st = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int kb = first; ok && kb < last; ++kb) {
+        uint64_t ad[PARTS], bd[PARTS];
+        int used[PARTS];
+        auto product = [&](int i, int j, uint32_t d, bool fresh) {
+#pragma unroll
+          for (int k = 0; k < kK / 16; ++k) ptx::mma_f16_ss(d, ad[i] + k * a_step, bd[j] + k * b_step, idesc, fresh && k == 0 ? 0u : 1u);
+        };
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+          ok = ok && ptx::mbar_wait(&full[st], ph, 502);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          const uint32_t at = ptx::smem_u32(ring + st * kStage);
+          ad[i] = A_BY_K ? by_k_desc(at) : ptx::make_kmajor_desc<128>(at);
+          bd[i] = B_BY_K ? by_k_desc(at + kOperand) : ptx::make_kmajor_desc<128>(at + kOperand);
+          used[i] = st;
+          if (++st == kStages) { st = 0; ph ^= 1u; }
+          if (i == 0) {
+            product(0, 0, tmem, kb == first);
+          } else {
+            product(0, i, tmem + 128, kb == first && i == 1);
+            product(i, 0, tmem + 128, false);
+            if (i == 1) product(1, 1, tmem + 128, false);
+          }
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) ptx::tc_commit(&empty[used[i]]);
+      }
+      if (ok) ptx::tc_commit(done);
+    }
+  } else {
+    const int quad = warp & 3, row = m_tile * kTile + quad * 32 + lane;
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const bool ok = __all_sync(0xffffffffu, ptx::mbar_wait(done, 0, 503)) != 0;
+    ptx::tc_fence_after_sync();
+    if (ok) {
+      const long long row_off = static_cast<long long>(row) * p.out.s_n + split * p.plane_d;
+#pragma unroll 1
+      for (int c = 0; c < kTile; c += 32) {
+        const int col = n_tile * kTile + c;
+        if (col >= p.n) break;
+        uint32_t raw[32];
+        float v[32];
+        ptx::tmem_ld_32x32b_x32(t_row + c, raw);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
+        if (PARTS == 3) {
+          ptx::tmem_ld_32x32b_x32(t_row + 128 + c, raw);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(raw[i]);
+        }
+        if (p.accumulate && row < p.m) {
+          const float* d = static_cast<const float*>(p.out.dst) + row_off + col;
+          if (p.out.vec && col + 32 <= p.n) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 t = *reinterpret_cast<const float4*>(d + i);
+              v[i] += t.x;
+              v[i + 1] += t.y;
+              v[i + 2] += t.z;
+              v[i + 3] += t.w;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (col + i < p.n) v[i] += d[i];
+          }
+        }
+        epi_store_chunk(p.out, row_off, col, v, row < p.m);
+      }
+    }
+    ptx::tc_fence_before_sync();
+  }
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc(tmem, kCols);
+  }
+}
+
+int operand_map(CUtensorMap* map, const MatOperand& o, int extent, long long k, int parts) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(o.by_k ? extent : k), static_cast<uint64_t>(o.by_k ? k : extent), static_cast<uint64_t>(parts)};
+  const uint64_t str[2] = {static_cast<uint64_t>(o.ld) * 2, static_cast<uint64_t>(parts > 1 ? o.plane : o.ld) * 2};
+  const uint32_t box[3] = {64, o.by_k ? 64u : static_cast<uint32_t>(kTile), 1};
+  return make_tmap(map, o.ptr, 2, 3, dims, str, box, 128);
+}
+
+template <bool A_BY_K, bool B_BY_K, int PARTS>
+int launch(cudaStream_t stream, const MatmulArgs& a, const MmParams& p) {
+  CUtensorMap ta, tb;
+  KFB_TRY(operand_map(&ta, a.a, a.m, a.k, PARTS));
+  KFB_TRY(operand_map(&tb, a.b, a.n, a.k, PARTS));
+  constexpr auto kernel = matmul_kernel<A_BY_K, B_BY_K, PARTS>;
+  KFB_TRY(allow_smem<kernel>(smem_bytes<PARTS>()));
+  LaunchScope scope(stream, a.tag);
+  return launch_kernel(stream, kernel, dim3(p.m_tiles * p.n_tiles, a.splits), kThreads, smem_bytes<PARTS>(), ta, tb, p);
+}
+template <int PARTS>
+int launch_majors(cudaStream_t stream, const MatmulArgs& a, const MmParams& p) {
+  if (a.a.by_k) return a.b.by_k ? launch<true, true, PARTS>(stream, a, p) : launch<true, false, PARTS>(stream, a, p);
+  return a.b.by_k ? launch<false, true, PARTS>(stream, a, p) : launch<false, false, PARTS>(stream, a, p);
+}
+
+// out[i .. i + 3] of the planes' sums
+template <typename TO>
+__global__ void __launch_bounds__(256) sum_planes_kernel(const float* planes, long long plane, int splits, TO* out, long long n) {
+  grid_dependency_enter();
+  const long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int k = 0; k < splits; ++k) {
+    const float4 t = *reinterpret_cast<const float4*>(planes + k * plane + i);
+    s.x += t.x;
+    s.y += t.y;
+    s.z += t.z;
+    s.w += t.w;
+  }
+  if constexpr (sizeof(TO) == 2) *reinterpret_cast<uint2*>(out + i) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+  else *reinterpret_cast<float4*>(out + i) = s;
+}
+
+__global__ void __launch_bounds__(256) split_planes_kernel(const float* x, __nv_bfloat16* parts, long long plane, long long n) {
+  grid_dependency_enter();
+  const long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const float4 v = *reinterpret_cast<const float4*>(x + i);
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  __nv_bfloat16 q[3][4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) split3(f[k], q[0][k], q[1][k], q[2][k]);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2*>(parts + k * plane + i) = *reinterpret_cast<const uint2*>(q[k]);
+}
+
+}  // namespace
+
+int matmul_splits(int m, int n, long long k, int most) {
+  const long long tiles = static_cast<long long>(cdiv(m, kTile)) * cdiv(n, kTile), blocks = (k + kK - 1) / kK;
+  long long want = 2ll * sm_count() / tiles;
+  if (want > most) want = most;
+  if (want > blocks) want = blocks;
+  if (want < 1) want = 1;
+  const long long per = (blocks + want - 1) / want;
+  return static_cast<int>((blocks + per - 1) / per);
+}
+
+int launch_matmul(cudaStream_t stream, const MatmulArgs& a) {
+  KFB_CHECK_ARG(a.m > 0 && a.n > 0 && a.k > 0 && a.k < (1ll << 31) && a.splits >= 1, "matmul: m %d n %d k %lld, %d pieces", a.m, a.n, a.k, a.splits);
+  KFB_CHECK_ARG(a.out_fp32 || (a.splits == 1 && !a.accumulate), "matmul: pieces and sums need an fp32 result");
+  MmParams p = {};
+  p.m = a.m;
+  p.n = a.n;
+  p.m_tiles = cdiv(a.m, kTile);
+  p.n_tiles = cdiv(a.n, kTile);
+  p.blocks = static_cast<int>((a.k + kK - 1) / kK);
+  p.per_split = cdiv(p.blocks, a.splits);
+  KFB_CHECK_ARG(cdiv(p.blocks, p.per_split) == a.splits, "matmul: an empty piece of k (%d blocks in %d)", p.blocks, a.splits);
+  p.out = row_major_seg(a.d, a.n, a.ld_d, 0, 0, a.out_fp32);
+  if (a.splits > 1 && a.plane_d % 4 != 0) p.out.vec = 0;
+  p.plane_d = a.plane_d;
+  p.accumulate = a.accumulate;
+  return a.precise ? launch_majors<3>(stream, a, p) : launch_majors<1>(stream, a, p);
+}
+
+int launch_sum_planes(cudaStream_t stream, const float* planes, long long plane, int splits, void* out, int out_fp32, long long n) {
+  KFB_CHECK_ARG(n % 4 == 0 && plane % 4 == 0, "sum_planes: %lld elements, planes %lld apart (multiples of 4)", n, plane);
+  const unsigned blocks = static_cast<unsigned>((n / 4 + 255) / 256);
+  LaunchScope scope(stream, "sum_planes");
+  if (out_fp32) return launch_kernel(stream, sum_planes_kernel<float>, blocks, 256, 0, planes, plane, splits, static_cast<float*>(out), n);
+  return launch_kernel(stream, sum_planes_kernel<__nv_bfloat16>, blocks, 256, 0, planes, plane, splits, static_cast<__nv_bfloat16*>(out), n);
+}
+
+int launch_split_planes(cudaStream_t stream, const float* x, __nv_bfloat16* parts, long long plane, long long n) {
+  KFB_CHECK_ARG(n % 4 == 0 && plane % 4 == 0, "split_planes: %lld elements, planes %lld apart (multiples of 4)", n, plane);
+  LaunchScope scope(stream, "split_planes");
+  return launch_kernel(stream, split_planes_kernel, static_cast<unsigned>((n / 4 + 255) / 256), 256, 0, x, parts, plane, n);
+}
+
+}  // namespace kfb

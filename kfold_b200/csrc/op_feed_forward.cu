@@ -1,0 +1,228 @@
+// Gated feed-forward and its gradient (training; the inference path has it inside kfb_transition_fwd):
+//   [a, b] = x [Wa; Wb]^T,  h = silu(a) b,  y = h Wo^T
+//   dh = dy Wo,  da = dh b silu'(a),  db = dh silu(a),  dx = [da, db] [Wa; Wb],  d[Wa; Wb] = [da, db]^T x,  dWo = dy^T h
+// with s = sigmoid(a), silu(a) = a s, silu'(a) = s + silu(a) (1 - s).
+//
+// a and b are not kept from the forward pass: computing them again is 4 of the backward pass's 16 operations per row, channel and hidden channel,
+// keeping them 8 bytes per row and hidden channel.  a, b and dh stay float32; h, da and db are rounded to bf16 once, as operands.
+// Rows are taken in pieces, so that the workspace does not grow with them; the weights' gradients are summed over pieces of rows in float32
+// planes and added up at the end, in an order that depends on the sizes alone.
+#include "gemm.cuh"   // sigmoidf_exact, split3
+#include "matmul.cuh"
+#include "ops_common.cuh"
+
+namespace kfb {
+namespace {
+
+constexpr int kMostRows = 16384;      // of a piece
+constexpr int kMostPlanes = 64;
+
+// h and, with dh, [da, db] from u = [a, b] (rows, 2 hidden) and dh (rows, hidden); four hidden channels a thread.  PARTS == 3: the results as three
+// bf16 parts each, planes rows * hidden and rows * 2 hidden apart.
+template <int PARTS>
+__device__ __forceinline__ void store_parts(__nv_bfloat16* d, long long plane, const float (&v)[4]) {
+  if constexpr (PARTS == 1) {
+    *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+  } else {
+    __nv_bfloat16 q[3][4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) split3(v[k], q[0][k], q[1][k], q[2][k]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2*>(d + k * plane) = *reinterpret_cast<const uint2*>(q[k]);
+  }
+}
+
+template <int PARTS>
+__global__ void __launch_bounds__(256) ffn_hidden_kernel(const float* u, const float* dh, __nv_bfloat16* h, __nv_bfloat16* dab, long long rows,
+                                                         int hidden) {
+  grid_dependency_enter();
+  const long long per_row = hidden / 4, n = rows * per_row;
+  for (long long t = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; t < n; t += static_cast<long long>(gridDim.x) * 256) {
+    const long long row = t / per_row;
+    const int j = static_cast<int>(t - row * per_row) * 4;
+    const float4 a4 = *reinterpret_cast<const float4*>(u + row * 2 * hidden + j), b4 = *reinterpret_cast<const float4*>(u + row * 2 * hidden + hidden + j);
+    const float4 g4 = dh != nullptr ? *reinterpret_cast<const float4*>(dh + row * hidden + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w}, g[4] = {g4.x, g4.y, g4.z, g4.w};
+    float hv[4], da[4], db[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float s = sigmoidf_exact(a[i]), silu = a[i] * s;
+      hv[i] = silu * b[i];
+      da[i] = g[i] * b[i] * fmaf(silu, 1.0f - s, s);
+      db[i] = g[i] * silu;
+    }
+    store_parts<PARTS>(h + row * hidden + j, rows * hidden, hv);
+    if (dh != nullptr) {
+      store_parts<PARTS>(dab + row * 2 * hidden + j, rows * 2 * hidden, da);
+      store_parts<PARTS>(dab + row * 2 * hidden + hidden + j, rows * 2 * hidden, db);
+    }
+  }
+}
+
+struct FfnWs {
+  __nv_bfloat16 *x3, *dy3, *wi3, *wo3;      // fp32-accurate mode: the operands' parts
+  float *u, *dh;
+  __nv_bfloat16 *h, *dab;
+  float *pl_in, *pl_out;
+};
+// Pieces that the rows of a weight's gradient are summed in.
+int planes_in(long long rows, int c, int hidden) { return matmul_splits(2 * hidden, c, rows < kMostRows ? rows : kMostRows, kMostPlanes); }
+int planes_out(long long rows, int c, int hidden) { return matmul_splits(c, hidden, rows < kMostRows ? rows : kMostRows, kMostPlanes); }
+
+size_t carve(FfnWs& w, void* base, long long rows, int c, int hidden, int precise, int backward) {
+  Carver cv(base);
+  const size_t r = static_cast<size_t>(rows < kMostRows ? rows : kMostRows), parts = precise ? 3 : 1, cc = c, hh = hidden;
+  w = {};
+  if (precise) {
+    w.x3 = cv.take<__nv_bfloat16>(3 * r * cc);
+    w.wi3 = cv.take<__nv_bfloat16>(3 * 2 * hh * cc);
+    w.wo3 = cv.take<__nv_bfloat16>(3 * hh * cc);
+    if (backward) w.dy3 = cv.take<__nv_bfloat16>(3 * r * cc);
+  }
+  w.u = cv.take<float>(r * 2 * hh);
+  w.h = cv.take<__nv_bfloat16>(parts * r * hh);
+  if (backward) {
+    w.dh = cv.take<float>(r * hh);
+    w.dab = cv.take<__nv_bfloat16>(parts * r * 2 * hh);
+    w.pl_in = cv.take<float>(planes_in(rows, c, hidden) * 2 * hh * cc);
+    w.pl_out = cv.take<float>(planes_out(rows, c, hidden) * hh * cc);
+  }
+  return cv.off;
+}
+
+int launch_hidden(cudaStream_t stream, const FfnWs& w, bool backward, long long rows, int hidden, int precise) {
+  const long long want = (rows * (hidden / 4) + 255) / 256, most = static_cast<long long>(sm_count()) * 16;
+  LaunchScope scope(stream, "feed_forward_hidden");
+  return launch_kernel(stream, precise ? ffn_hidden_kernel<3> : ffn_hidden_kernel<1>, static_cast<unsigned>(want < most ? want : most), 256, 0,
+                       const_cast<const float*>(w.u), backward ? const_cast<const float*>(w.dh) : nullptr, w.h, w.dab, rows, hidden);
+}
+
+int check(const char* name, const void* workspace, size_t workspace_bytes, size_t need, long long rows, int c, int hidden, int dtype,
+          uintptr_t tensors) {
+  KFB_CHECK_ARG(dtype == KFB_BF16 || dtype == KFB_FP32_PRECISE, "%s: bad dtype %d", name, dtype);
+  KFB_CHECK_ARG(rows >= 0 && rows < (1ll << 31), "%s: rows %lld", name, rows);
+  KFB_CHECK_ARG(c > 0 && c % 8 == 0 && hidden > 0 && hidden % 8 == 0 && c <= 65536 && hidden <= 65536, "%s: c=%d, hidden=%d (multiples of 8)", name, c,
+                hidden);
+  KFB_CHECK_ARG((tensors & 15) == 0, "%s: tensors must be 16-byte aligned", name);
+  KFB_CHECK_ARG(workspace != nullptr && workspace_bytes >= need, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
+  KFB_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "%s: workspace must be 256-byte aligned", name);
+  return KFB_OK;
+}
+uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+}  // namespace
+}  // namespace kfb
+
+using namespace kfb;
+
+extern "C" {
+
+KFB_API size_t kfb_feed_forward_workspace_bytes(long long rows, int c, int hidden, int dtype, int backward) {
+  if (rows < 1 || c < 1 || hidden < 1) return 0;
+  FfnWs w;
+  return carve(w, nullptr, rows, c, hidden, dtype == KFB_FP32_PRECISE, backward);
+}
+
+KFB_API int kfb_feed_forward_fwd(const void* x, const void* w_in, const void* w_out, void* out, void* workspace, size_t workspace_bytes,
+                                 long long rows, int c, int hidden, int dtype, void* stream) {
+  if (rows == 0) return KFB_OK;
+  KFB_CHECK_ARG(x && w_in && w_out && out, "feed_forward: null tensor");
+  KFB_TRY(check("feed_forward", workspace, workspace_bytes, kfb_feed_forward_workspace_bytes(rows, c, hidden, dtype, 0), rows, c, hidden, dtype,
+                bits(x) | bits(w_in) | bits(w_out) | bits(out)));
+  cudaStream_t s = as_stream(stream);
+  const int precise = dtype == KFB_FP32_PRECISE;
+  const size_t size = precise ? 4 : 2;
+  FfnWs w;
+  carve(w, workspace, rows, c, hidden, precise, 0);
+  const long long wi_n = 2ll * hidden * c, wo_n = static_cast<long long>(hidden) * c;
+  if (precise) {
+    KFB_TRY(launch_split_planes(s, static_cast<const float*>(w_in), w.wi3, wi_n, wi_n));
+    KFB_TRY(launch_split_planes(s, static_cast<const float*>(w_out), w.wo3, wo_n, wo_n));
+  }
+  const void *wi = precise ? w.wi3 : w_in, *wo = precise ? w.wo3 : w_out;
+  for (long long r0 = 0; r0 < rows; r0 += kMostRows) {
+    const long long r = rows - r0 < kMostRows ? rows - r0 : kMostRows;
+    const int m = static_cast<int>(r);
+    const void* xr = static_cast<const char*>(x) + r0 * c * size;
+    if (precise) {
+      KFB_TRY(launch_split_planes(s, static_cast<const float*>(xr), w.x3, r * c, r * c));
+      xr = w.x3;
+    }
+    MatmulArgs in = {{xr, c, 0, r * c}, {wi, c, 0, wi_n}, m, 2 * hidden, c, w.u, 2ll * hidden, 1, 1, 0, 0, precise, "feed_forward_in"};
+    KFB_TRY(launch_matmul(s, in));
+    KFB_TRY(launch_hidden(s, w, false, r, hidden, precise));
+    MatmulArgs out_p = {{w.h, hidden, 0, r * hidden}, {wo, hidden, 0, wo_n}, m, c, hidden, static_cast<char*>(out) + r0 * c * size, c, precise, 1, 0, 0,
+                        precise, "feed_forward_out"};
+    KFB_TRY(launch_matmul(s, out_p));
+  }
+  return KFB_OK;
+}
+
+KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in, const void* w_out, void* dx, void* dw_in, void* dw_out,
+                                 void* workspace, size_t workspace_bytes, long long rows, int c, int hidden, int dtype, int grad_dtype,
+                                 void* stream) {
+  cudaStream_t s = as_stream(stream);
+  const long long wi_n = 2ll * hidden * c, wo_n = static_cast<long long>(hidden) * c;
+  const int precise = dtype == KFB_FP32_PRECISE;
+  const size_t size = precise ? 4 : 2;
+  KFB_CHECK_ARG(grad_dtype == KFB_FP32 || (grad_dtype == KFB_BF16 && !precise), "feed_forward_bwd: bad dtype %d of the weights' gradients", grad_dtype);
+  if (rows == 0) {
+    const size_t g = grad_dtype == KFB_FP32 ? 4 : 2;
+    KFB_CHECK_ARG(c > 0 && hidden > 0, "feed_forward_bwd: c=%d, hidden=%d", c, hidden);
+    if (dw_in != nullptr) KFB_CUDA(cudaMemsetAsync(dw_in, 0, wi_n * g, s));
+    if (dw_out != nullptr) KFB_CUDA(cudaMemsetAsync(dw_out, 0, wo_n * g, s));
+    return KFB_OK;
+  }
+  KFB_CHECK_ARG(dy && x && w_in && w_out, "feed_forward_bwd: null tensor");
+  KFB_TRY(check("feed_forward_bwd", workspace, workspace_bytes, kfb_feed_forward_workspace_bytes(rows, c, hidden, dtype, 1), rows, c, hidden, dtype,
+                bits(dy) | bits(x) | bits(w_in) | bits(w_out) | bits(dx) | bits(dw_in) | bits(dw_out)));
+  FfnWs w;
+  carve(w, workspace, rows, c, hidden, precise, 1);
+  if (precise) {
+    KFB_TRY(launch_split_planes(s, static_cast<const float*>(w_in), w.wi3, wi_n, wi_n));
+    KFB_TRY(launch_split_planes(s, static_cast<const float*>(w_out), w.wo3, wo_n, wo_n));
+  }
+  const void *wi = precise ? w.wi3 : w_in, *wo = precise ? w.wo3 : w_out;
+  const int most_in = planes_in(rows, c, hidden), most_out = planes_out(rows, c, hidden);
+  for (long long r0 = 0; r0 < rows; r0 += kMostRows) {
+    const long long r = rows - r0 < kMostRows ? rows - r0 : kMostRows;
+    const int m = static_cast<int>(r);
+    const void *xr = static_cast<const char*>(x) + r0 * c * size, *dr = static_cast<const char*>(dy) + r0 * c * size;
+    if (precise) {
+      KFB_TRY(launch_split_planes(s, static_cast<const float*>(xr), w.x3, r * c, r * c));
+      KFB_TRY(launch_split_planes(s, static_cast<const float*>(dr), w.dy3, r * c, r * c));
+      xr = w.x3;
+      dr = w.dy3;
+    }
+    const MatOperand mx = {xr, c, 0, r * c}, md = {dr, c, 0, r * c}, mh = {w.h, hidden, 0, r * hidden}, mg = {w.dab, 2ll * hidden, 0, r * 2 * hidden};
+    auto across = [](MatOperand o) {
+      o.by_k = 1;
+      return o;
+    };
+    MatmulArgs in = {mx, {wi, c, 0, wi_n}, m, 2 * hidden, c, w.u, 2ll * hidden, 1, 1, 0, 0, precise, "feed_forward_in"};
+    KFB_TRY(launch_matmul(s, in));
+    MatmulArgs dh = {md, {wo, hidden, 1, wo_n}, m, hidden, c, w.dh, hidden, 1, 1, 0, 0, precise, "feed_forward_dh"};
+    KFB_TRY(launch_matmul(s, dh));
+    KFB_TRY(launch_hidden(s, w, true, r, hidden, precise));
+    if (dx != nullptr) {
+      MatmulArgs g = {mg, {wi, c, 1, wi_n}, m, c, 2 * hidden, static_cast<char*>(dx) + r0 * c * size, c, precise, 1, 0, 0, precise, "feed_forward_dx"};
+      KFB_TRY(launch_matmul(s, g));
+    }
+    const int add = r0 > 0;
+    if (dw_in != nullptr) {
+      const int splits = matmul_splits(2 * hidden, c, r, most_in);
+      MatmulArgs g = {across(mg), across(mx), 2 * hidden, c, r, w.pl_in, c, 1, splits, wi_n, add, precise, "feed_forward_dw"};
+      KFB_TRY(launch_matmul(s, g));
+    }
+    if (dw_out != nullptr) {
+      const int splits = matmul_splits(c, hidden, r, most_out);
+      MatmulArgs g = {across(md), across(mh), c, hidden, r, w.pl_out, hidden, 1, splits, wo_n, add, precise, "feed_forward_dw"};
+      KFB_TRY(launch_matmul(s, g));
+    }
+  }
+  if (dw_in != nullptr) KFB_TRY(launch_sum_planes(s, w.pl_in, wi_n, most_in, dw_in, grad_dtype == KFB_FP32, wi_n));
+  if (dw_out != nullptr) KFB_TRY(launch_sum_planes(s, w.pl_out, wo_n, most_out, dw_out, grad_dtype == KFB_FP32, wo_n));
+  return KFB_OK;
+}
+
+}  // extern "C"

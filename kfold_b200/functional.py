@@ -139,6 +139,62 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
     return dx.view(x.shape), dw, db
 
 
+def _feed_forward_operands(name: str, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, dy: torch.Tensor | None = None):
+    """(hidden channels, kernel's dtype code, rows of x, of dy, weights in x's dtype), all as the kernels read them."""
+    _require_cuda(x, w_in, w_out, dy)
+    _same_device(name, x, w_in, w_out, dy)
+    c = x.shape[-1] if x.dim() else 0
+    hidden = w_out.shape[1] if w_out.dim() == 2 else 0
+    if tuple(w_out.shape) != (c, hidden) or tuple(w_in.shape) != (2 * hidden, c) or c % 8 or hidden % 8 or not c or not hidden:
+        raise ValueError(f"{name}: w_in {tuple(w_in.shape)}, w_out {tuple(w_out.shape)} for x {tuple(x.shape)} (channels multiples of 8)")
+    if x.dtype not in (torch.bfloat16, torch.float32) or (dy is not None and (dy.dtype != x.dtype or dy.shape != x.shape)):
+        raise ValueError(f"{name}: x {x.dtype} {tuple(x.shape)}" + ("" if dy is None else f", dy {dy.dtype} {tuple(dy.shape)}"))
+    if any(w.dtype not in (x.dtype, torch.float32) for w in (w_in, w_out)) or w_in.dtype != w_out.dtype:
+        raise ValueError(f"{name}: weights {w_in.dtype} and {w_out.dtype} for x {x.dtype}")
+    code = L.KFB_BF16 if x.dtype == torch.bfloat16 else L.KFB_FP32_PRECISE
+    return hidden, code, _aligned_rows(x, c), None if dy is None else _aligned_rows(dy, c), _aligned_rows(w_in, c, x.dtype), _aligned_rows(w_out, hidden, x.dtype)
+
+
+def _aligned_rows(t: torch.Tensor, c: int, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """`t` as dense rows of c that start on a 16-byte boundary."""
+    t = t.detach().reshape(-1, c)
+    if dtype is not None:
+        t = t.to(dtype)
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor) -> torch.Tensor:
+    """y = (silu(x Wa^T) * (x Wb^T)) Wo^T with [Wa; Wb] = w_in (2 hidden, C), Wo = w_out (C, hidden): SwiGLU and output projection of a
+    Transition (model/layers/folding/transition.py:48-68) on its plain parameters, for training.
+
+    x (..., C) bfloat16 (tensor-core arithmetic, float32 sums) or float32 (the fp32-accurate mode); the weights of x's dtype, or float32
+    parameters that are rounded to it here.  C and hidden multiples of 8."""
+    hidden, code, x2, _, wi, wo = _feed_forward_operands("gated_feed_forward", x, w_in, w_out)
+    out = torch.empty_like(x2)
+    lib = L.lib()
+    with L.on_device(x.device):
+        ws = _workspace(x.device, lib.kfb_feed_forward_workspace_bytes(*x2.shape, hidden, code, 0), MOST_KEPT_BYTES)
+        L.check(lib.kfb_feed_forward_fwd(L.ptr(x2), L.ptr(wi), L.ptr(wo), L.ptr(out), L.ptr(ws), ws.numel(), *x2.shape, hidden, code, L.stream_ptr()))
+    return out.view(x.shape)
+
+
+def gated_feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, need_x: bool = True,
+                                need_w_in: bool = True, need_w_out: bool = True):
+    """Gradient of ``gated_feed_forward``: (dx, dw_in, dw_out) from dy, of x's shape and dtype; None where not asked for.  The weights'
+    gradients have the weights' dtype (float32 sums either way).  The hidden channels are computed again, nothing has to be kept."""
+    hidden, code, x2, d2, wi, wo = _feed_forward_operands("gated_feed_forward_backward", x, w_in, w_out, dy)
+    dx = torch.empty_like(x2) if need_x else None
+    dwi = torch.empty(w_in.shape, dtype=w_in.dtype, device=x.device) if need_w_in else None
+    dwo = torch.empty(w_out.shape, dtype=w_out.dtype, device=x.device) if need_w_out else None
+    lib = L.lib()
+    with L.on_device(x.device):
+        ws = _workspace(x.device, lib.kfb_feed_forward_workspace_bytes(*x2.shape, hidden, code, 1), MOST_KEPT_BYTES)
+        L.check(lib.kfb_feed_forward_bwd(L.ptr(d2), L.ptr(x2), L.ptr(wi), L.ptr(wo), L.ptr(dx), L.ptr(dwi), L.ptr(dwo), L.ptr(ws), ws.numel(),
+                                         *x2.shape, hidden, code, L.dtype_code(w_in.dtype), L.stream_ptr()))
+    return None if dx is None else dx.view(x.shape), dwi, dwo
+
+
 def _signed64(v: int) -> int:
     return v - (1 << 64) if v >= 1 << 63 else v
 

@@ -57,16 +57,33 @@ def kept(shape, shared_dim, p, rng):
 
 
 def feed_forward(x, w_in, w_out):
-    a, b = (x.double() @ w_in.double().t()).chunk(2, -1)
-    return (a * torch.sigmoid(a) * b) @ w_out.double().t()
+    return feed_forward_pass(x, w_in, w_out)[0]
 
 
 def feed_forward_gradient(dy, x, w_in, w_out):
     """(dx, dw_in, dw_out)."""
-    x, dy, wi, wo = x.double(), dy.double(), w_in.double(), w_out.double()
-    x, dy = x.reshape(-1, x.shape[-1]), dy.reshape(-1, dy.shape[-1])
+    return feed_forward_pass(x, w_in, w_out, dy)[1:4]
+
+
+def feed_forward_pass(x, w_in, w_out, dy=None, operand=0.0, gate=0.0, sums=0.0):
+    """(y, dx, dw_in, dw_out) and, for each, what the roundings in between can move it by at the very worst: h, da and db are off by
+    `operand` of themselves, by what an error of `gate` in sigmoid(a) makes of them, and by what a, b and dh bring, sums that are off by `sums` of
+    their terms' magnitudes (|silu'| < 1.1, |silu''| <= 0.5)."""
+    shape, c = x.shape, x.shape[-1]
+    x, wi, wo = x.double().reshape(-1, c), w_in.double(), w_out.double()
     a, b = (x @ wi.t()).chunk(2, -1)
     s = torch.sigmoid(a)
-    dh = dy @ wo
-    dab = torch.cat((dh * b * s * (1 + a * (1 - s)), dh * a * s), -1)
-    return dab @ wi, dab.t() @ x, dy.t() @ (a * s * b)
+    h = a * s * b
+    da0, db0 = (sums * (x.abs() @ wi.abs().t())).chunk(2, -1)
+    dh_off = operand * h.abs() + gate * (a * b).abs() + 1.1 * b.abs() * da0 + (a * s).abs() * db0
+    out, room = [(h @ wo.t()).reshape(shape)], [(dh_off @ wo.abs().t()).reshape(shape)]
+    if dy is not None:
+        dy = dy.double().reshape(-1, c)
+        g = dy @ wo
+        dab = torch.cat((g * b * s * (1 + a * (1 - s)), g * a * s), -1)
+        off = operand * dab.abs() + gate * torch.cat(((g * b).abs() * (1 + a.abs()), (g * a).abs()), -1)
+        dg = sums * (dy.abs() @ wo.abs())
+        off = off + torch.cat((1.1 * b.abs() * dg + 1.1 * g.abs() * db0 + 0.5 * (g * b).abs() * da0, (a * s).abs() * dg + 1.1 * g.abs() * da0), -1)
+        out += [(dab @ wi).reshape(shape), dab.t() @ x, dy.t() @ h]
+        room += [(off @ wi.abs()).reshape(shape), off.t() @ x.abs(), dy.abs().t() @ dh_off]
+    return (*out, *room) if dy is not None else (out[0], room[0])

@@ -52,3 +52,35 @@ def test_dropout_refuses_before_any_cuda_call(library):
     assert call(below=-1) == call(below=(1 << 32) + 1) == 1
     assert call(xt=1, ot=0) == call(xt=2) == call(ot=5) == 1
     assert call(n=0) == 0
+
+
+def test_feed_forward_refuses_before_any_cuda_call(library):
+    vp, some, big = ctypes.c_void_p, 256, 1 << 40
+    fwd = lambda x=some, wi=some, out=some, ws=some, size=big, rows=3, c=64, h=128, dt=0: library.kfb_feed_forward_fwd(
+        vp(x), vp(wi), vp(some), vp(out), vp(ws), size, rows, c, h, dt, None)
+    bwd = lambda dy=some, wi=some, dx=some, ws=some, size=big, rows=3, c=64, h=128, dt=0, gt=0: library.kfb_feed_forward_bwd(
+        vp(dy), vp(some), vp(wi), vp(some), vp(dx), vp(some), vp(some), vp(ws), size, rows, c, h, dt, gt, None)
+    for call in (fwd, bwd):
+        assert call(wi=None) == call(ws=None) == call(size=16) == call(ws=some + 16) == 1
+        assert call(rows=-1) == call(rows=1 << 31) == call(c=0) == call(c=60) == call(h=100) == call(h=-8) == call(dt=1) == call(dt=9) == 1
+        assert call(wi=some + 8) == 1
+        assert b"16-byte" in library.kfb_last_error()
+    assert fwd(x=None) == fwd(out=None) == bwd(dy=None) == bwd(gt=2) == bwd(dt=2, gt=0) == 1
+    assert fwd(rows=0) == 0
+
+
+def test_feed_forward_workspace_stops_growing(library):
+    need = library.kfb_feed_forward_workspace_bytes
+    for c in (128, 256, 384):
+        for dt in (0, 2):
+            for backward in (0, 1):
+                sizes = [need(r, c, 4 * c, dt, backward) for r in (1, 1000, 1 << 17, 1 << 20, (1 << 31) - 1)]
+                assert sizes == sorted(sizes) and sizes[-1] == sizes[-2] == sizes[-3] and sizes[0] > 0
+    assert need(0, 128, 512, 0, 0) == need(5, 0, 512, 0, 0) == 0
+
+
+def test_feed_forward_refuses_cpu_tensors():
+    x, wi, wo = torch.zeros(4, 8), torch.zeros(32, 8), torch.zeros(8, 16)
+    for call in (lambda: F.gated_feed_forward(x, wi, wo), lambda: F.gated_feed_forward_backward(x, x, wi, wo)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()

@@ -20,9 +20,44 @@ namespace {
 
 constexpr int kThreads = 256;
 
+struct Words {
+  uint32_t w[4];
+};
+
+// Seed and offset of a launch, the seed as the ten rounds' keys.  STATE: read from device memory when the kernel runs; otherwise the keys are launch
+// parameters, operands that cost no instruction.
+struct Keys {
+  uint32_t k[20];
+};
+__host__ __device__ __forceinline__ void round_keys(unsigned long long seed, Keys& d) {
+  uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
+#pragma unroll
+  for (int i = 0; i < 10; ++i) {
+    d.k[2 * i] = k0;
+    d.k[2 * i + 1] = k1;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+}
+
+__device__ __forceinline__ Words philox(unsigned long long block, unsigned long long offset, const Keys& keys) {
+  uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32);
+  uint32_t c2 = static_cast<uint32_t>(offset), c3 = static_cast<uint32_t>(offset >> 32);
+#pragma unroll
+  for (int i = 0; i < 10; ++i) {
+    const unsigned long long a = static_cast<unsigned long long>(0xD2511F53u) * c0, b = static_cast<unsigned long long>(0xCD9E8D57u) * c2;
+    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ keys.k[2 * i];
+    c1 = static_cast<uint32_t>(b);
+    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ keys.k[2 * i + 1];
+    c3 = static_cast<uint32_t>(a);
+  }
+  return {{c0, c1, c2, c3}};
+}
+
 struct DropParams {
   const long long* rng;             // (seed, offset) in device memory, or null: the two below
-  unsigned long long seed, offset;
+  Keys keys;
+  unsigned long long offset;
   uint32_t cut;                     // kept: word > cut
   int keep_all;                     // nothing is dropped
   float scale;
@@ -30,82 +65,109 @@ struct DropParams {
   long long chunks, chunk;          // `shared` positions in `chunks` pieces of `chunk`
 };
 
-struct Words {
-  uint32_t w[4];
+// V elements of x as they lie in memory, and the mask as words to and them with: an element that is dropped becomes a zero whatever it was, an
+// infinity or NaN too, at one instruction for two bf16 elements.
+template <typename TX, int V>
+struct Piece {
+  static constexpr int kWords = V * sizeof(TX) < 4 ? 1 : V * static_cast<int>(sizeof(TX)) / 4;
+  uint32_t w[kWords];
 };
-
-__device__ __forceinline__ Words philox(unsigned long long block, unsigned long long offset, unsigned long long seed) {
-  uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32);
-  uint32_t c2 = static_cast<uint32_t>(offset), c3 = static_cast<uint32_t>(offset >> 32);
-  uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
+template <typename TX, int V>
+__device__ __forceinline__ void load_piece(const TX* p, Piece<TX, V>& d) {
+  constexpr int kBytes = V * static_cast<int>(sizeof(TX));
+  if constexpr (kBytes >= 16) {
 #pragma unroll
-  for (int i = 0; i < 10; ++i) {
-    const unsigned long long a = static_cast<unsigned long long>(0xD2511F53u) * c0, b = static_cast<unsigned long long>(0xCD9E8D57u) * c2;
-    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
-    c1 = static_cast<uint32_t>(b);
-    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
-    c3 = static_cast<uint32_t>(a);
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
+    for (int i = 0; i < kBytes / 16; ++i) {
+      const uint4 t = reinterpret_cast<const uint4*>(p)[i];
+      d.w[4 * i] = t.x;
+      d.w[4 * i + 1] = t.y;
+      d.w[4 * i + 2] = t.z;
+      d.w[4 * i + 3] = t.w;
+    }
+  } else if constexpr (kBytes == 8) {
+    const uint2 t = *reinterpret_cast<const uint2*>(p);
+    d.w[0] = t.x;
+    d.w[1] = t.y;
+  } else if constexpr (kBytes == 4) {
+    d.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    d.w[0] = *reinterpret_cast<const unsigned short*>(p);
   }
-  return {{c0, c1, c2, c3}};
+}
+template <typename TX, int V>
+__device__ __forceinline__ void values(const Piece<TX, V>& d, float (&v)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if constexpr (sizeof(TX) == 4) v[i] = __uint_as_float(d.w[i]);
+    else v[i] = __uint_as_float(i & 1 ? d.w[i / 2] & 0xffff0000u : d.w[i / 2] << 16);
+  }
 }
 
-// Bit i: element e + i of the mask is kept, i < V.
-template <int V>
-__device__ __forceinline__ uint32_t kept_bits(const DropParams& p, unsigned long long seed, unsigned long long offset, long long e) {
-  uint32_t bits = 0;
+// The mask of elements e ... e + V - 1 (e a multiple of 4 unless V is 1).
+template <typename TX, int V>
+__device__ __forceinline__ void kept(const DropParams& p, const Keys& keys, unsigned long long offset, long long e, Piece<TX, V>& m) {
+#pragma unroll
+  for (int i = 0; i < Piece<TX, V>::kWords; ++i) m.w[i] = 0;
   if constexpr (V == 1) {
-    const Words r = philox(static_cast<unsigned long long>(e) >> 2, offset, seed);
+    const Words r = philox(static_cast<unsigned long long>(e) >> 2, offset, keys);
     const int at = static_cast<int>(e & 3);
     const uint32_t w = at == 0 ? r.w[0] : at == 1 ? r.w[1] : at == 2 ? r.w[2] : r.w[3];
-    bits = (w > p.cut) | p.keep_all;
+    m.w[0] = (w > p.cut) | p.keep_all ? 0xffffffffu : 0u;
   } else {
 #pragma unroll
     for (int b = 0; b < V / 4; ++b) {
-      const Words r = philox((static_cast<unsigned long long>(e) >> 2) + b, offset, seed);
+      const Words r = philox((static_cast<unsigned long long>(e) >> 2) + b, offset, keys);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) bits |= static_cast<uint32_t>((r.w[i] > p.cut) | p.keep_all) << (4 * b + i);
+      for (int i = 0; i < 4; ++i) {
+        const int k = 4 * b + i;
+        if constexpr (sizeof(TX) == 4) m.w[k] = r.w[i] > p.cut ? 0xffffffffu : 0u;
+        else m.w[k / 2] |= r.w[i] > p.cut ? (k & 1 ? 0xffff0000u : 0xffffu) : 0u;
+      }
+    }
+    if (p.keep_all) {
+#pragma unroll
+      for (int i = 0; i < Piece<TX, V>::kWords; ++i) m.w[i] = 0xffffffffu;
     }
   }
-  return bits;
 }
 
-// U pieces of V elements, their loads before the first store: out may be x or resid, so the compiler keeps the order it is given.
-template <int V, int U, typename TX, typename TR, typename Bits>
-__device__ __forceinline__ void apply(const TX* x, const TR* resid, TR* out, const long long (&at)[U], const bool (&live)[U], float scale, Bits bits) {
-  float v[U][V], r[U][V];
+// U pieces, their loads before the first store: out may be x or resid, so the compiler keeps the order it is given.  mask(u): the piece's.
+template <int V, int U, bool RESID, typename TX, typename TR, typename Mask>
+__device__ __forceinline__ void apply(const TX* x, const TR* resid, TR* out, const long long (&at)[U], const bool (&live)[U], float scale, Mask mask) {
+  Piece<TX, V> v[U];
+  Piece<TR, V> r[U];
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (live[u]) {
-      load_vec<V>(x + at[u], v[u]);
-      if (resid != nullptr) load_vec<V>(resid + at[u], r[u]);
+      load_piece<TX, V>(x + at[u], v[u]);
+      if (RESID) load_piece<TR, V>(resid + at[u], r[u]);
     }
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (live[u]) {
-      const uint32_t kept = bits(u);
+      const Piece<TX, V> m = mask(u);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float t = (kept >> i & 1) ? v[u][i] * scale : 0.f;      // (a select: an infinity or NaN that is dropped leaves no trace)
-        v[u][i] = resid != nullptr ? r[u][i] + t : t;
-      }
-      store_vec<V>(out + at[u], v[u]);
+      for (int i = 0; i < Piece<TX, V>::kWords; ++i) v[u].w[i] &= m.w[i];
+      float f[V], add[V];
+      values<TX, V>(v[u], f);
+      if (RESID) values<TR, V>(r[u], add);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = RESID ? fmaf(f[i], scale, add[i]) : f[i] * scale;
+      store_vec<V>(out + at[u], f);
     }
 }
 
-__device__ __forceinline__ void stream_of(const DropParams& p, unsigned long long& seed, unsigned long long& offset) {
-  seed = p.rng != nullptr ? static_cast<unsigned long long>(p.rng[0]) : p.seed;
-  offset = p.rng != nullptr ? static_cast<unsigned long long>(p.rng[1]) : p.offset;
-}
+constexpr int kBlocksPerSm = 4;
 
 // Every element by itself: `inner` of them, a multiple of V.
-template <typename TX, typename TR, int V>
-__global__ void __launch_bounds__(kThreads) dropout_kernel(const TX* x, const TR* resid, TR* out, const DropParams p) {
+template <typename TX, typename TR, int V, bool RESID, bool STATE>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) dropout_kernel(const TX* x, const TR* resid, TR* out, const DropParams p) {
   constexpr int U = 2;
   grid_dependency_enter();
-  unsigned long long seed, offset;
-  stream_of(p, seed, offset);
+  Keys own;
+  if (STATE) round_keys(static_cast<unsigned long long>(p.rng[0]), own);
+  const Keys& keys = STATE ? own : p.keys;
+  const unsigned long long offset = STATE ? static_cast<unsigned long long>(p.rng[1]) : p.offset;
   constexpr long long kBlock = static_cast<long long>(kThreads) * U * V;
   for (long long base = blockIdx.x * kBlock; base < p.inner; base += gridDim.x * kBlock) {
     long long at[U];
@@ -115,54 +177,77 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const TX* x, const TR
       at[u] = base + (u * kThreads + static_cast<int>(threadIdx.x)) * V;
       live[u] = at[u] < p.inner;
     }
-    apply<V, U>(x, resid, out, at, live, p.scale, [&](int u) { return kept_bits<V>(p, seed, offset, at[u]); });
+    apply<V, U, RESID>(x, resid, out, at, live, p.scale, [&](int u) {
+      Piece<TX, V> m;
+      kept<TX, V>(p, keys, offset, at[u], m);
+      return m;
+    });
   }
 }
 
 // A shared mask: a thread has V elements of it and the positions of its piece of the shared axis.
-template <typename TX, typename TR, int V>
-__global__ void __launch_bounds__(kThreads) dropout_shared_kernel(const TX* x, const TR* resid, TR* out, const DropParams p) {
-  constexpr int U = 4;
+template <typename TX, typename TR, int V, bool RESID, bool STATE>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) dropout_shared_kernel(const TX* x, const TR* resid, TR* out, const DropParams p) {
+  constexpr int U = RESID ? 3 : 4;
   grid_dependency_enter();
-  unsigned long long seed, offset;
-  stream_of(p, seed, offset);
+  Keys own;
+  if (STATE) round_keys(static_cast<unsigned long long>(p.rng[0]), own);
+  const Keys& keys = STATE ? own : p.keys;
+  const unsigned long long offset = STATE ? static_cast<unsigned long long>(p.rng[1]) : p.offset;
   const long long pieces = p.inner / V, total = p.outer * p.chunks * pieces;
   for (long long t = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; t < total; t += static_cast<long long>(gridDim.x) * kThreads) {
     const long long i = t % pieces * V, rest = t / pieces, o = rest / p.chunks, s0 = rest % p.chunks * p.chunk;
-    const long long s1 = s0 + p.chunk < p.shared ? s0 + p.chunk : p.shared;
-    const uint32_t kept = kept_bits<V>(p, seed, offset, o * p.inner + i);
-    for (long long s = s0; s < s1; s += U) {
+    // (a piece of the shared axis is short, or the threads are many: either way below 2^31 for what a GPU can hold)
+    int left = static_cast<int>(s0 + p.chunk < p.shared ? p.chunk : p.shared - s0);
+    Piece<TX, V> m;
+    kept<TX, V>(p, keys, offset, o * p.inner + i, m);
+    const long long first = (o * p.shared + s0) * p.inner + i;
+    const TX* xs = x + first;
+    const TR* rs = RESID ? resid + first : nullptr;
+    TR* os = out + first;
+    for (; left > 0; left -= U) {
       long long at[U];
       bool live[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        at[u] = (o * p.shared + s + u) * p.inner + i;
-        live[u] = s + u < s1;
+        at[u] = u * p.inner;
+        live[u] = u < left;
       }
-      apply<V, U>(x, resid, out, at, live, p.scale, [&](int) { return kept; });
+      apply<V, U, RESID>(xs, rs, os, at, live, p.scale, [&](int) { return m; });
+      xs += U * p.inner;
+      if (RESID) rs += U * p.inner;
+      os += U * p.inner;
     }
   }
 }
 
-template <typename TX, typename TR, int V>
-int launch(cudaStream_t stream, const void* x, const void* resid, void* out, DropParams p) {
+template <typename TX, typename TR, int V, bool RESID, bool STATE>
+int launch_state(cudaStream_t stream, const void* x, const void* resid, void* out, DropParams p) {
   const long long sms = sm_count();
   LaunchScope scope(stream, "dropout");
   if (p.shared == 1) {
     p.inner *= p.outer;
     const long long blocks = (p.inner + 2ll * V * kThreads - 1) / (2ll * V * kThreads);
-    return launch_kernel(stream, dropout_kernel<TX, TR, V>, static_cast<unsigned>(blocks < sms * 64 ? blocks : sms * 64), kThreads, 0,
+    return launch_kernel(stream, dropout_kernel<TX, TR, V, RESID, STATE>, static_cast<unsigned>(blocks < sms * 64 ? blocks : sms * 64), kThreads, 0,
                          static_cast<const TX*>(x), static_cast<const TR*>(resid), static_cast<TR*>(out), p);
   }
-  // pieces of the shared axis: as long as the device stays full (8 blocks of 256 threads an SM)
-  const long long items = p.outer * (p.inner / V), full = sms * 8 * kThreads;
-  long long chunks = items >= full ? 1 : (full + items - 1) / items;
+  // pieces of the shared axis: as many as fill the device once
+  const long long items = p.outer * (p.inner / V), full = sms * kBlocksPerSm * kThreads;
+  long long chunks = items >= full ? 1 : full / items;
   if (chunks > p.shared) chunks = p.shared;
   p.chunk = (p.shared + chunks - 1) / chunks;
   p.chunks = (p.shared + p.chunk - 1) / p.chunk;
   const long long blocks = (items * p.chunks + kThreads - 1) / kThreads;
-  return launch_kernel(stream, dropout_shared_kernel<TX, TR, V>, static_cast<unsigned>(blocks < sms * 64 ? blocks : sms * 64), kThreads, 0,
+  return launch_kernel(stream, dropout_shared_kernel<TX, TR, V, RESID, STATE>, static_cast<unsigned>(blocks < sms * 64 ? blocks : sms * 64), kThreads, 0,
                        static_cast<const TX*>(x), static_cast<const TR*>(resid), static_cast<TR*>(out), p);
+}
+template <typename TX, typename TR, int V, bool RESID>
+int launch_resid(cudaStream_t stream, const void* x, const void* resid, void* out, const DropParams& p) {
+  return p.rng != nullptr ? launch_state<TX, TR, V, RESID, true>(stream, x, resid, out, p) : launch_state<TX, TR, V, RESID, false>(stream, x, resid, out, p);
+}
+template <typename TX, typename TR, int V>
+int launch(cudaStream_t stream, const void* x, const void* resid, void* out, const DropParams& p) {
+  return resid != nullptr ? launch_resid<TX, TR, V, true>(stream, x, resid, out, p) : launch_resid<TX, TR, V, false>(stream, x, resid, out, p);
 }
 
 template <typename TX, typename TR>
@@ -191,7 +276,7 @@ extern "C" KFB_API int kfb_dropout(const void* x, const void* residual, void* ou
   KFB_CHECK_ARG(x != nullptr && out != nullptr, "dropout: null tensor");
   DropParams d = {};
   d.rng = rng;
-  d.seed = static_cast<unsigned long long>(seed);
+  round_keys(static_cast<unsigned long long>(seed), d.keys);
   d.offset = static_cast<unsigned long long>(offset);
   d.keep_all = drop_below == 0;
   d.cut = drop_below == 0 ? 0u : static_cast<uint32_t>(drop_below - 1);

@@ -91,27 +91,49 @@ def _pad_pair(x: torch.Tensor, mask: torch.Tensor, precise: bool = True, mult: i
     return xp, mp, n
 
 
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _dense_like(x: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """A dense tensor of x's shape, of `dtype` or x's.  (empty_like costs the host 1.4 us where empty with its arguments costs 3.3.)"""
+    if x.is_contiguous() and (dtype is None or dtype == x.dtype):
+        return torch.empty_like(x)
+    return torch.empty(x.shape, dtype=dtype or x.dtype, device=x.device)
+
+
+def _affine(t: torch.Tensor | None) -> torch.Tensor | None:
+    """A LayerNorm's scale or offset as the kernels read it: float32, dense."""
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().float().contiguous()
+
+
 def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype=None) -> torch.Tensor:
     """LayerNorm over the last dim (model/primitives/normalization.py:61-91)."""
     _require_cuda(x)
     c = x.shape[-1]
-    x2 = x.reshape(-1, c)
-    if x2.stride(-1) != 1:
-        x2 = x2.contiguous()
-    out = torch.empty(x2.shape, dtype=out_dtype or x.dtype, device=x.device)
-    w = None if weight is None else weight.detach().float().contiguous()
-    b = None if bias is None else bias.detach().float().contiguous()
+    if x.is_contiguous():
+        x2, rows, pitch = x, x.numel() // c if c else 0, c
+    else:
+        x2 = x.reshape(-1, c)
+        if x2.stride(-1) != 1:
+            x2 = x2.contiguous()
+        rows, pitch = x2.shape[0], x2.stride(0)
+    out = _dense_like(x, out_dtype)
+    w, b = _affine(weight), _affine(bias)
     with L.on_device(x.device):
-        L.check(L.lib().kfb_layernorm(L.ptr(x2), L.ptr(out), L.ptr(w), L.ptr(b), x2.shape[0], c, x2.stride(0), c, eps,
-                                      L.dtype_code(x2.dtype), L.dtype_code(out.dtype), L.stream_ptr()))
-    return out.view(*x.shape[:-1], c)
+        L.check(L.lib().kfb_layernorm(L.ptr(x2), L.ptr(out), L.ptr(w), L.ptr(b), rows, c, pitch, c, eps, L.dtype_code(x.dtype),
+                                      L.dtype_code(out.dtype), L.stream_ptr()))
+    return out
 
 
-def _same_device(name: str, *ts: torch.Tensor | None) -> None:
+def _same_device(name: str, x: torch.Tensor, *ts: torch.Tensor | None) -> None:
     """A kernel follows every pointer on one GPU: refuse a mixture."""
-    devices = {t.device for t in ts if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"{name}: tensors on {', '.join(sorted(map(str, devices)))}")
+    at = x.get_device()
+    for t in ts:
+        if t is not None and t.get_device() != at:
+            raise ValueError(f"{name}: tensors on {x.device} and {t.device}")
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-5, need_weight: bool = True,
@@ -123,44 +145,43 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
     _require_cuda(dy, x, weight)
     _same_device("layer_norm_backward", dy, x, weight)
     c = x.shape[-1]
-    if dy.shape != x.shape or (weight is not None and tuple(weight.shape) != (c,)):
+    if dy.shape != x.shape or (weight is not None and weight.shape != (c,)):
         raise ValueError(f"layer_norm_backward: dy {tuple(dy.shape)}, weight {None if weight is None else tuple(weight.shape)} for x {tuple(x.shape)}")
     need_weight = need_weight and weight is not None
-    x2, d2 = x.reshape(-1, c).contiguous(), dy.reshape(-1, c).contiguous()
-    w = None if weight is None else weight.detach().float().contiguous()
-    dx = torch.empty_like(x2)
+    xc, dc, w = _dense(x), _dense(dy), _affine(weight)
+    dx = _dense_like(x)
     dw = torch.empty(c, dtype=torch.float32, device=x.device) if need_weight else None
     db = torch.empty(c, dtype=torch.float32, device=x.device) if need_bias else None
     lib = L.lib()
     with L.on_device(x.device):
         ws = _workspace(x.device, lib.kfb_layernorm_bwd_workspace_bytes(c)) if need_weight or need_bias else None
-        L.check(lib.kfb_layernorm_bwd(L.ptr(d2), L.ptr(x2), L.ptr(w), L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), 0 if ws is None else ws.numel(),
-                                      x2.shape[0], c, eps, L.dtype_code(d2.dtype), L.dtype_code(x2.dtype), L.stream_ptr()))
-    return dx.view(x.shape), dw, db
+        L.check(lib.kfb_layernorm_bwd(L.ptr(dc), L.ptr(xc), L.ptr(w), L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), 0 if ws is None else ws.numel(),
+                                      x.numel() // c if c else 0, c, eps, L.dtype_code(dy.dtype), L.dtype_code(x.dtype), L.stream_ptr()))
+    return dx, dw, db
 
 
 def _feed_forward_operands(name: str, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, dy: torch.Tensor | None = None):
-    """(hidden channels, kernel's dtype code, rows of x, of dy, weights in x's dtype), all as the kernels read them."""
+    """(rows, channels, hidden channels, kernel's dtype code; x, dy and the weights as the kernels read them)."""
     _require_cuda(x, w_in, w_out, dy)
     _same_device(name, x, w_in, w_out, dy)
     c = x.shape[-1] if x.dim() else 0
     hidden = w_out.shape[1] if w_out.dim() == 2 else 0
-    if tuple(w_out.shape) != (c, hidden) or tuple(w_in.shape) != (2 * hidden, c) or c % 8 or hidden % 8 or not c or not hidden:
+    if w_out.shape != (c, hidden) or w_in.shape != (2 * hidden, c) or c % 8 or hidden % 8 or not c or not hidden:
         raise ValueError(f"{name}: w_in {tuple(w_in.shape)}, w_out {tuple(w_out.shape)} for x {tuple(x.shape)} (channels multiples of 8)")
-    if x.dtype not in (torch.bfloat16, torch.float32) or (dy is not None and (dy.dtype != x.dtype or dy.shape != x.shape)):
-        raise ValueError(f"{name}: x {x.dtype} {tuple(x.shape)}" + ("" if dy is None else f", dy {dy.dtype} {tuple(dy.shape)}"))
-    if any(w.dtype not in (x.dtype, torch.float32) for w in (w_in, w_out)) or w_in.dtype != w_out.dtype:
-        raise ValueError(f"{name}: weights {w_in.dtype} and {w_out.dtype} for x {x.dtype}")
-    code = L.KFB_BF16 if x.dtype == torch.bfloat16 else L.KFB_FP32_PRECISE
-    return hidden, code, _aligned_rows(x, c), None if dy is None else _aligned_rows(dy, c), _aligned_rows(w_in, c, x.dtype), _aligned_rows(w_out, hidden, x.dtype)
+    dt = x.dtype
+    if dt not in (torch.bfloat16, torch.float32) or (dy is not None and (dy.dtype != dt or dy.shape != x.shape)):
+        raise ValueError(f"{name}: x {dt} {tuple(x.shape)}" + ("" if dy is None else f", dy {dy.dtype} {tuple(dy.shape)}"))
+    if w_in.dtype != w_out.dtype or w_in.dtype not in (dt, torch.float32):
+        raise ValueError(f"{name}: weights {w_in.dtype} and {w_out.dtype} for x {dt}")
+    code = L.KFB_BF16 if dt == torch.bfloat16 else L.KFB_FP32_PRECISE
+    return x.numel() // c, c, hidden, code, _operand(x, dt), None if dy is None else _operand(dy, dt), _operand(w_in, dt), _operand(w_out, dt)
 
 
-def _aligned_rows(t: torch.Tensor, c: int, dtype: torch.dtype | None = None) -> torch.Tensor:
-    """`t` as dense rows of c that start on a 16-byte boundary."""
-    t = t.detach().reshape(-1, c)
-    if dtype is not None:
-        t = t.to(dtype)
-    t = t.contiguous()
+def _operand(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """`t` dense, of `dtype`, starting on a 16-byte boundary."""
+    if t.dtype != dtype:
+        t = t.detach().to(dtype)
+    t = _dense(t)
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -170,29 +191,29 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor)
 
     x (..., C) bfloat16 (tensor-core arithmetic, float32 sums) or float32 (the fp32-accurate mode); the weights of x's dtype, or float32
     parameters that are rounded to it here.  C and hidden multiples of 8."""
-    hidden, code, x2, _, wi, wo = _feed_forward_operands("gated_feed_forward", x, w_in, w_out)
-    out = torch.empty_like(x2)
+    rows, c, hidden, code, xc, _, wi, wo = _feed_forward_operands("gated_feed_forward", x, w_in, w_out)
+    out = _dense_like(x)
     lib = L.lib()
     with L.on_device(x.device):
-        ws = _workspace(x.device, lib.kfb_feed_forward_workspace_bytes(*x2.shape, hidden, code, 0), MOST_KEPT_BYTES)
-        L.check(lib.kfb_feed_forward_fwd(L.ptr(x2), L.ptr(wi), L.ptr(wo), L.ptr(out), L.ptr(ws), ws.numel(), *x2.shape, hidden, code, L.stream_ptr()))
-    return out.view(x.shape)
+        ws = _workspace(x.device, lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, code, 0), MOST_KEPT_BYTES)
+        L.check(lib.kfb_feed_forward_fwd(L.ptr(xc), L.ptr(wi), L.ptr(wo), L.ptr(out), L.ptr(ws), ws.numel(), rows, c, hidden, code, L.stream_ptr()))
+    return out
 
 
 def gated_feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, need_x: bool = True,
                                 need_w_in: bool = True, need_w_out: bool = True):
     """Gradient of ``gated_feed_forward``: (dx, dw_in, dw_out) from dy, of x's shape and dtype; None where not asked for.  The weights'
     gradients have the weights' dtype (float32 sums either way).  The hidden channels are computed again, nothing has to be kept."""
-    hidden, code, x2, d2, wi, wo = _feed_forward_operands("gated_feed_forward_backward", x, w_in, w_out, dy)
-    dx = torch.empty_like(x2) if need_x else None
-    dwi = torch.empty(w_in.shape, dtype=w_in.dtype, device=x.device) if need_w_in else None
-    dwo = torch.empty(w_out.shape, dtype=w_out.dtype, device=x.device) if need_w_out else None
+    rows, c, hidden, code, xc, dc, wi, wo = _feed_forward_operands("gated_feed_forward_backward", x, w_in, w_out, dy)
+    dx = _dense_like(x) if need_x else None
+    dwi = _dense_like(w_in) if need_w_in else None
+    dwo = _dense_like(w_out) if need_w_out else None
     lib = L.lib()
     with L.on_device(x.device):
-        ws = _workspace(x.device, lib.kfb_feed_forward_workspace_bytes(*x2.shape, hidden, code, 1), MOST_KEPT_BYTES)
-        L.check(lib.kfb_feed_forward_bwd(L.ptr(d2), L.ptr(x2), L.ptr(wi), L.ptr(wo), L.ptr(dx), L.ptr(dwi), L.ptr(dwo), L.ptr(ws), ws.numel(),
-                                         *x2.shape, hidden, code, L.dtype_code(w_in.dtype), L.stream_ptr()))
-    return None if dx is None else dx.view(x.shape), dwi, dwo
+        ws = _workspace(x.device, lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, code, 1), MOST_KEPT_BYTES)
+        L.check(lib.kfb_feed_forward_bwd(L.ptr(dc), L.ptr(xc), L.ptr(wi), L.ptr(wo), L.ptr(dx), L.ptr(dwi), L.ptr(dwo), L.ptr(ws), ws.numel(), rows, c,
+                                         hidden, code, L.dtype_code(w_in.dtype), L.stream_ptr()))
+    return dx, dwi, dwo
 
 
 def _signed64(v: int) -> int:
@@ -216,11 +237,11 @@ def dropout(x: torch.Tensor, p: float, rng, shared_dim: int | None = None, resid
         raise ValueError(f"dropout: residual {residual.dtype} {tuple(residual.shape)} for x {x.dtype} {tuple(x.shape)}")
     state, seed, offset = None, 0, 0
     if isinstance(rng, torch.Tensor):
-        if not rng.is_cuda or rng.dtype != torch.int64 or tuple(rng.shape) != (2,) or not rng.is_contiguous():
+        if not rng.is_cuda or rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
             raise ValueError("dropout: rng is a pair of integers or a contiguous int64 CUDA tensor of two")
         state = rng
     else:
-        seed, offset = (int(v) for v in rng)
+        seed, offset = int(rng[0]), int(rng[1])
         if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
             raise ValueError(f"dropout: seed {seed} and offset {offset} are not in [0, 2^64)")
     outer, shared, inner = 1, 1, x.numel()
@@ -229,8 +250,8 @@ def dropout(x: torch.Tensor, p: float, rng, shared_dim: int | None = None, resid
             raise ValueError(f"dropout: dim {shared_dim} of x {tuple(x.shape)}")
         d = shared_dim % x.dim()
         outer, shared, inner = math.prod(x.shape[:d]), x.shape[d], math.prod(x.shape[d + 1:])
-    xc, rc = x.contiguous(), None if residual is None else residual.contiguous()
-    out = torch.empty(x.shape, dtype=x.dtype if residual is None else residual.dtype, device=x.device)
+    xc, rc = _dense(x), None if residual is None else _dense(residual)
+    out = _dense_like(x if residual is None else residual)
     scale = 1.0 / (1.0 - p) if p < 1.0 else 0.0
     with L.on_device(x.device):
         L.check(L.lib().kfb_dropout(L.ptr(xc), L.ptr(rc), L.ptr(out), outer, shared, inner, int(p * 4294967296.0 + 0.5), scale, L.ptr(state),

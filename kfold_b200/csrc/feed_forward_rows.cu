@@ -1,0 +1,415 @@
+// The gradient of the gated feed-forward with respect to its rows, in one kernel:
+//   a, b = x Wa^T, x Wb^T,  dh = dy Wo,  da = dh b silu'(a),  db = dh silu(a),  dx = da Wa + db Wb
+// for 128 or 256 channels, bf16; h, da and db are stored only where the weights' gradients want them (SPILL).
+//
+// What bounds it.  Five products of rows x channels x hidden channels; as separate launches da and db alone are 4 bytes per row and hidden channel
+// written and read, and the memory takes writes at 4 TB/s only (measured, where a copy moves 6.5).  Here they go from one product to the next through
+// tensor memory.
+//
+// Split.  A CTA pair takes 256 rows, 128 in each CTA, and walks the hidden channels in chunks of 64:
+//   S  = [x [Wa; Wb]^T | dy Wo]   192 columns                              (CTA 0 loads the chunk's rows of Wa, CTA 1 those of Wb, each half of Wo's)
+//   P  = [da | db] as bf16        64 columns of tensor memory
+//   dX += P [Wa; Wb]              C columns, Wa and Wb read across k       (each CTA loads its half of the channels)
+// S and dX have a thread each that issues them.  dX of a chunk runs while sixteen warps bring the next chunk's S into registers: one S buffer is enough,
+// and with P and dX it fills the tensor memory at 256 channels.  x and dy stay in shared memory for a tile; the next tile's come into L2 meanwhile, and
+// into the buffers as its slots fall free.
+#include <mutex>
+
+#include "feed_forward_hidden.cuh"
+#include "gemm.cuh"   // tanh_fast, pack_bf16x2
+#include "ptx.cuh"
+
+namespace kfb {
+namespace {
+
+constexpr int kRows = 128, kChunk = 64;
+constexpr int kBox = kRows * 128;                    // [128 rows][64 bf16], 128-byte swizzle
+constexpr int kRowSlot = 2 * kBox, kRowSlots = 4;    // a 64-wide block of x and of dy
+constexpr int kW1 = 64 * 128, kWo = 64 * 64;         // a CTA's [64 hidden][64 k] of Wa or Wb, and [64 k][32 hidden] of Wo (64-byte swizzle)
+constexpr int kWSlot = kW1 + kWo, kWSlots = 5;
+constexpr int kVSlots = 2;                           // of the [64 hidden][C / 2] that dX takes of Wa or Wb
+constexpr int kEpiWarp = 4, kEpiWarps = 16;          // four warps for each 32 rows, 16 hidden channels each
+constexpr int kThreads = 32 * (kEpiWarp + kEpiWarps);
+template <int C>
+struct Cfg {
+  static constexpr int kVSlot = 64 * (C / 2) * 2;
+  static constexpr int kSmem = kRowSlots * kRowSlot + kWSlots * kWSlot + kVSlots * kVSlot + 512 + 1024;
+  static_assert(kSmem <= 232448, "shared memory");
+};
+
+struct RowsParams {
+  int rows, chunks, hidden, tiles;
+  __nv_bfloat16 *dx, *h, *dab;                       // rows 32-byte aligned
+};
+
+__device__ __forceinline__ uint64_t wo_desc(uint32_t addr) {   // [k][32 hidden] rows of 64 bytes, eight of them (a swizzle atom) 512 bytes apart
+  return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | (1ull << 16) | (static_cast<uint64_t>(512 >> 4) << 32) | (1ull << 46) | (4ull << 61);
+}
+__device__ __forceinline__ uint64_t v_desc(uint32_t addr) {    // [64 k][64 channels] boxes of 128-byte rows, the next 64 channels a box further
+  return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | (static_cast<uint64_t>(8192 >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+template <int C, bool SPILL>
+__global__ void __launch_bounds__(kThreads, 1)
+ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_w1,
+                     const __grid_constant__ CUtensorMap tm_wo, const RowsParams p) {
+  constexpr int kK = C / 64, kVSlot = Cfg<C>::kVSlot;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* s_rows = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* s_w = s_rows + kRowSlots * kRowSlot;
+  uint8_t* s_v = s_w + kWSlots * kWSlot;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + kVSlots * kVSlot);
+  uint64_t* w_full = bars;                        // in the leader: both CTAs' copies
+  uint64_t* w_free = w_full + kWSlots;
+  uint64_t* v_full = w_free + kWSlots;            // in the leader
+  uint64_t* v_free = v_full + kVSlots;
+  uint64_t* r_full = v_free + kVSlots;            // in the leader
+  uint64_t* r_free = r_full + kRowSlots;
+  uint64_t* s_full = r_free + kRowSlots;
+  uint64_t* s_free = s_full + 1;                  // in the leader: the element-wise warps of both CTAs
+  uint64_t* p_full = s_free + 1;                  // in the leader, likewise
+  uint64_t* p_free = p_full + 1;
+  uint64_t* o_full = p_free + 1;
+  uint64_t* o_free = o_full + 1;                  // in the leader, likewise
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(ptx::cluster_ctarank());
+  const int tile0 = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
+  const int my_tiles = (p.tiles - tile0 + tile_step - 1) / tile_step;      // (the grid has no pair without a tile)
+  const int total = my_tiles * p.chunks;
+  auto row0_of = [&](int it) { return (2 * (tile0 + it * tile_step) + rank) * kRows; };
+
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tmap(&tm_x);
+    ptx::prefetch_tmap(&tm_w1);
+    for (int i = 0; i < kWSlots; ++i) {
+      ptx::mbar_init(&w_full[i], 1);
+      ptx::mbar_init(&w_free[i], 1);
+    }
+    for (int i = 0; i < kVSlots; ++i) {
+      ptx::mbar_init(&v_full[i], 1);
+      ptx::mbar_init(&v_free[i], 1);
+    }
+    for (int i = 0; i < kRowSlots; ++i) {
+      ptx::mbar_init(&r_full[i], 1);
+      ptx::mbar_init(&r_free[i], 1);
+    }
+    ptx::mbar_init(s_full, 1);
+    ptx::mbar_init(s_free, 2 * kEpiWarps);
+    ptx::mbar_init(p_full, 2 * kEpiWarps);
+    ptx::mbar_init(p_free, 1);
+    ptx::mbar_init(o_full, 1);
+    ptx::mbar_init(o_free, 2 * kEpiWarps);
+    ptx::fence_barrier_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(tmem_slot, 512);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::tc_fence_before_sync();
+  __syncwarp();
+  ptx::cluster_sync();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot, tmem_s = tmem + C, tmem_p = tmem_s + 192;      // dX first
+  grid_dependency_enter();
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- weights, in the order of the products
+    if (ptx::elect_one()) {
+      int st = 0, v = 0;
+      uint32_t ph = 0, v_ph = 0;
+      bool ok = true;
+      int c1 = 0, c2 = 0;
+      for (int i = 0; ok && i <= total; ++i) {
+        if (i < total) {
+          for (int kb = 0; kb < kK; ++kb) {
+            ok = ptx::mbar_wait(&w_free[st], ph ^ 1, 541);
+            if (!ok) break;
+            if (rank == 0) ptx::mbar_expect_tx(&w_full[st], 2 * kWSlot);
+            const uint32_t bar = ptx::leader_addr(&w_full[st]);
+            ptx::tma_load_4d_pair(s_w + st * kWSlot, &tm_w1, bar, kb * 64, rank * p.hidden + c1 * kChunk, 0, 0);
+            ptx::tma_load_4d_pair(s_w + st * kWSlot + kW1, &tm_wo, bar, c1 * kChunk + rank * 32, kb * 64, 0, 0);
+            if (++st == kWSlots) { st = 0; ph ^= 1u; }
+          }
+          if (++c1 == p.chunks) c1 = 0;
+        }
+        if (i > 0) {
+          for (int which = 0; ok && which < 2; ++which) {
+            ok = ptx::mbar_wait(&v_free[v], v_ph ^ 1, 542);
+            if (!ok) break;
+            if (rank == 0) ptx::mbar_expect_tx(&v_full[v], 2 * kVSlot);
+            const uint32_t bar = ptx::leader_addr(&v_full[v]);
+#pragma unroll
+            for (int q = 0; q < C / 128; ++q)
+              ptx::tma_load_4d_pair(s_v + v * kVSlot + q * 8192, &tm_w1, bar, rank * (C / 2) + q * 64, which * p.hidden + c2 * kChunk, 0, 0);
+            if (++v == kVSlots) { v = 0; v_ph ^= 1u; }
+          }
+          if (++c2 == p.chunks) c2 = 0;
+        }
+      }
+      // the last products' arrivals at this CTA's barriers, before it may exit
+      for (int i = 0; ok && i < kWSlots; ++i) {
+        ok = ptx::mbar_wait(&w_free[st], ph ^ 1, 543);
+        if (++st == kWSlots) { st = 0; ph ^= 1u; }
+      }
+      for (int i = 0; ok && i < kVSlots; ++i) {
+        ok = ptx::mbar_wait(&v_free[v], v_ph ^ 1, 544);
+        if (++v == kVSlots) { v = 0; v_ph ^= 1u; }
+      }
+    }
+  } else if (warp == 2) {
+    // ---------------------------------------------------------------- rows
+    if (ptx::elect_one()) {
+      int st = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int it = 0; ok && it < my_tiles; ++it) {
+        for (int kb = 0; kb < kK; ++kb) {
+          ok = ptx::mbar_wait(&r_free[st], ph ^ 1, 545);
+          if (!ok) break;
+          if (rank == 0) ptx::mbar_expect_tx(&r_full[st], 2 * kRowSlot);
+          const uint32_t bar = ptx::leader_addr(&r_full[st]);
+          ptx::tma_load_4d_pair(s_rows + st * kRowSlot, &tm_x, bar, kb * 64, row0_of(it), 0, 0);
+          ptx::tma_load_4d_pair(s_rows + st * kRowSlot + kBox, &tm_dy, bar, kb * 64, row0_of(it), 0, 0);
+          if (++st == kRowSlots) { st = 0; ph ^= 1u; }
+        }
+        if (it + 1 < my_tiles)
+          for (int kb = 0; kb < kK; ++kb) {
+            ptx::tma_prefetch_4d(&tm_x, kb * 64, row0_of(it + 1), 0, 0);
+            ptx::tma_prefetch_4d(&tm_dy, kb * 64, row0_of(it + 1), 0, 0);
+          }
+      }
+      for (int i = 0; ok && i < kRowSlots; ++i) {
+        ok = ptx::mbar_wait(&r_free[st], ph ^ 1, 546);
+        if (++st == kRowSlots) { st = 0; ph ^= 1u; }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- S
+    if (rank == 0 && ptx::elect_one()) {
+      constexpr uint32_t idesc_s = ptx::make_idesc(2 * kRows, 2 * kChunk, 1), idesc_g = ptx::make_idesc(2 * kRows, kChunk, 1) | (1u << 16);
+      const uint64_t row_desc = ptx::make_kmajor_desc<128>(ptx::smem_u32(s_rows));
+      const uint64_t w1_desc = ptx::make_kmajor_desc<128>(ptx::smem_u32(s_w)), g_desc = wo_desc(ptx::smem_u32(s_w) + kW1);
+      int st = 0, rs0 = 0, c = 0;
+      uint32_t ph = 0, r_ph = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < total; ++i) {
+        ok = ptx::mbar_wait(s_free, (i & 1) ^ 1, 547);
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+#pragma unroll
+        for (int kb = 0; kb < kK; ++kb) {
+          const int rs = rs0 + kb;                  // (kRowSlots is a multiple of kK)
+          if (c == 0) ok = ptx::mbar_wait(&r_full[rs], r_ph, 548);
+          ok = ok && ptx::mbar_wait(&w_full[st], ph, 549);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          const uint64_t xd = row_desc + rs * (kRowSlot >> 4), wd = w1_desc + st * (kWSlot >> 4), gd = g_desc + st * (kWSlot >> 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) ptx::mma_f16_ss_pair(tmem_s, xd + k * 2, wd + k * 2, idesc_s, kb > 0 || k > 0 ? 1u : 0u);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            ptx::mma_f16_ss_pair(tmem_s + 128, xd + (kBox >> 4) + k * 2, gd + k * (1024 >> 4), idesc_g, kb > 0 || k > 0 ? 1u : 0u);
+          ptx::tc_commit_pair(&w_free[st]);
+          if (c == p.chunks - 1) ptx::tc_commit_pair(&r_free[rs]);
+          if (++st == kWSlots) { st = 0; ph ^= 1u; }
+        }
+        if (!ok) break;
+        ptx::tc_commit_pair(s_full);
+        if (++c == p.chunks) {
+          c = 0;
+          rs0 += kK;
+          if (rs0 == kRowSlots) { rs0 = 0; r_ph ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == 3) {
+    // ---------------------------------------------------------------- dX
+    if (rank == 0 && ptx::elect_one()) {
+      constexpr uint32_t idesc = ptx::make_idesc(2 * kRows, C, 1) | (1u << 16);
+      const uint64_t vd0 = v_desc(ptx::smem_u32(s_v));
+      int v = 0, c = 0, it = 0;
+      uint32_t v_ph = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < total; ++i) {
+        if (c == 0) ok = ptx::mbar_wait(o_free, (it & 1) ^ 1, 550);
+        ok = ok && ptx::mbar_wait(p_full, i & 1, 551);
+        for (int which = 0; ok && which < 2; ++which) {
+          ok = ptx::mbar_wait(&v_full[v], v_ph, 552);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          const uint64_t vd = vd0 + v * (kVSlot >> 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            ptx::mma_f16_ts_pair(tmem, tmem_p + which * 32 + k * 8, vd + k * (2048 >> 4), idesc, c > 0 || which > 0 || k > 0 ? 1u : 0u);
+          ptx::tc_commit_pair(&v_free[v]);
+          if (++v == kVSlots) { v = 0; v_ph ^= 1u; }
+        }
+        if (!ok) break;
+        ptx::tc_commit_pair(p_free);
+        if (++c == p.chunks) {
+          ptx::tc_commit_pair(o_full);
+          c = 0;
+          ++it;
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- da, db (and h); dx
+    const int part = (warp - kEpiWarp) >> 2, quad = warp & 3;
+    const uint32_t t_quad = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t t_s = tmem_s + t_quad + part * 16, t_p = tmem_p + t_quad + part * 8, t_o = tmem + t_quad;
+    bool ok = true;
+    // the finished tile's dx: a quarter of the channels a warp
+    auto finish = [&](int it) {
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(o_full, it & 1, 553)) != 0;
+      if (!ok) return;
+      ptx::tc_fence_after_sync();
+      const int row = row0_of(it) + quad * 32 + lane;
+      __nv_bfloat16* out = p.dx + static_cast<long long>(row) * C + part * (C / 4);
+#pragma unroll
+      for (int q = 0; q < C / 4; q += 32) {
+        uint32_t o[32];
+        ptx::tmem_ld_32x32b_x32(t_o + part * (C / 4) + q, o);
+        ptx::tmem_ld_wait();
+        if (q + 32 == C / 4) {
+          ptx::tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive_cluster(ptx::leader_addr(o_free));
+        }
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
+        if (row < p.rows) {
+          st_global_v8(out + q, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+          st_global_v8(out + q + 16, w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]);
+        }
+      }
+    };
+    int c = 0, it = 0;
+    for (int i = 0; ok && i < total; ++i) {
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(s_full, i & 1, 554)) != 0;
+      if (!ok) break;
+      ptx::tc_fence_after_sync();
+      uint32_t a[16], b[16], g[16];
+      ptx::tmem_ld_32x32b_x16(t_s, a);
+      ptx::tmem_ld_32x32b_x16(t_s + 64, b);
+      ptx::tmem_ld_32x32b_x16(t_s + 128, g);
+      ptx::tmem_ld_wait();
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::leader_addr(s_free));
+      uint32_t hw[8], aw[8], bw[8];
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        // pairs: s = tanh(a / 2) / 2 + 1 / 2, silu = a s, silu' = s + silu (1 - s)
+        const uint64_t half2 = ptx::pack2(0.5f, 0.5f), one2 = ptx::pack2(1.0f, 1.0f), minus2 = ptx::pack2(-1.0f, -1.0f);
+        const uint64_t av = ptx::pack2(a[j], a[j + 1]), bv = ptx::pack2(b[j], b[j + 1]), gv = ptx::pack2(g[j], g[j + 1]);
+        const float2 ah = ptx::unpack2(ptx::mul2(av, half2));
+        const uint64_t sv = ptx::fma2(ptx::pack2(tanh_fast(ah.x), tanh_fast(ah.y)), half2, half2);
+        const uint64_t silu = ptx::mul2(av, sv);
+        const uint64_t slope = ptx::fma2(silu, ptx::fma2(sv, minus2, one2), sv);
+        aw[j >> 1] = pack_bf16x2(ptx::mul2(ptx::mul2(gv, bv), slope));
+        bw[j >> 1] = pack_bf16x2(ptx::mul2(gv, silu));
+        if (SPILL) hw[j >> 1] = pack_bf16x2(ptx::mul2(silu, bv));
+      }
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(p_free, (i & 1) ^ 1, 555)) != 0;
+      if (!ok) break;
+      ptx::tc_fence_after_sync();
+      ptx::tmem_st_32x32b_x8(t_p, aw);
+      ptx::tmem_st_32x32b_x8(t_p + 32, bw);
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::leader_addr(p_full));
+      if (SPILL) {
+        // a whole 32-byte sector of each array a thread; the four warps of these rows fill their lines together
+        const int row = row0_of(it) + quad * 32 + lane, at = c * kChunk + part * 16;
+        if (row < p.rows) {
+          __nv_bfloat16* g_row = p.dab + 2ll * row * p.hidden + at;
+          st_global_v8(p.h + static_cast<long long>(row) * p.hidden + at, hw[0], hw[1], hw[2], hw[3], hw[4], hw[5], hw[6], hw[7]);
+          st_global_v8(g_row, aw[0], aw[1], aw[2], aw[3], aw[4], aw[5], aw[6], aw[7]);
+          st_global_v8(g_row + p.hidden, bw[0], bw[1], bw[2], bw[3], bw[4], bw[5], bw[6], bw[7]);
+        }
+      }
+      // (behind the next tile's first chunk: its S then runs under dX of the last)
+      if (c == 0 && it > 0) finish(it - 1);
+      if (++c == p.chunks) {
+        c = 0;
+        ++it;
+      }
+    }
+    if (ok) finish(my_tiles - 1);
+  }
+
+  ptx::tc_fence_before_sync();
+  __syncwarp();
+  ptx::cluster_sync();      // neither CTA leaves while the other may still read its operands or reach its barriers
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+template <int C, bool SPILL>
+int pairs_held() {
+  static std::once_flag once[64];
+  static int held[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  std::call_once(once[dev & 63], [&] { held[dev & 63] = clusters_held(ffn_rows_pair_kernel<C, SPILL>, 2, kThreads, Cfg<C>::kSmem); });
+  return held[dev & 63];
+}
+
+int matrix_map(CUtensorMap* m, const void* ptr, long long rows, long long cols, uint32_t box_rows, uint32_t box_cols) {
+  const uint64_t dims[4] = {(uint64_t)cols, (uint64_t)rows, 1, 1};
+  const uint64_t str[3] = {(uint64_t)cols * 2, (uint64_t)cols * 2 * rows, (uint64_t)cols * 2 * rows};
+  const uint32_t box[4] = {box_cols, box_rows, 1, 1};
+  return make_tmap(m, ptr, 2, 4, dims, str, box, static_cast<int>(box_cols) * 2);
+}
+
+template <int C, bool SPILL>
+int launch(cudaStream_t stream, const void* x, const void* dy, const void* w_in, const void* w_out, void* dx, void* h, void* dab, int rows,
+           int hidden) {
+  CUtensorMap tx, td, t1, to;
+  KFB_TRY(matrix_map(&tx, x, rows, C, kRows, 64));
+  KFB_TRY(matrix_map(&td, dy, rows, C, kRows, 64));
+  KFB_TRY(matrix_map(&t1, w_in, 2ll * hidden, C, kChunk, 64));
+  KFB_TRY(matrix_map(&to, w_out, C, hidden, 64, 32));
+  const int held = pairs_held<C, SPILL>();
+  KFB_CHECK_ARG(held > 0, "feed_forward: the device holds no pair of this kernel");
+  RowsParams p = {};
+  p.rows = rows;
+  p.chunks = hidden / kChunk;
+  p.hidden = hidden;
+  p.tiles = cdiv(rows, 2 * kRows);
+  p.dx = static_cast<__nv_bfloat16*>(dx);
+  p.h = static_cast<__nv_bfloat16*>(h);
+  p.dab = static_cast<__nv_bfloat16*>(dab);
+  LaunchScope scope(stream, SPILL ? "feed_forward_rows_grad_kept" : "feed_forward_rows_grad");
+  return launch_kernel_clustered(stream, ffn_rows_pair_kernel<C, SPILL>, 2, 2 * (p.tiles < held ? p.tiles : held), kThreads, Cfg<C>::kSmem, tx, td, t1,
+                                 to, p);
+}
+
+}  // namespace
+
+bool ffn_rows_ok(int c, int hidden) {
+  return (c == 128 || c == 256) && hidden % 64 == 0 && (c == 128 ? pairs_held<128, false>() > 0 && pairs_held<128, true>() > 0
+                                                               : pairs_held<256, false>() > 0 && pairs_held<256, true>() > 0);
+}
+
+int launch_ffn_rows(cudaStream_t stream, const void* x, const void* dy, const void* w_in, const void* w_out, void* dx, void* h, void* dab, int rows,
+                    int c, int hidden) {
+  if (c == 128)
+    return h != nullptr ? launch<128, true>(stream, x, dy, w_in, w_out, dx, h, dab, rows, hidden)
+                        : launch<128, false>(stream, x, dy, w_in, w_out, dx, h, dab, rows, hidden);
+  return h != nullptr ? launch<256, true>(stream, x, dy, w_in, w_out, dx, h, dab, rows, hidden)
+                      : launch<256, false>(stream, x, dy, w_in, w_out, dx, h, dab, rows, hidden);
+}
+
+}  // namespace kfb

@@ -7,6 +7,7 @@
 // keeping them 8 bytes per row and hidden channel.  a, b and dh stay float32; h, da and db are rounded to bf16 once, as operands.
 // Rows are taken in pieces, so that the workspace does not grow with them; the weights' gradients are summed over pieces of rows in float32
 // planes and added up at the end, in an order that depends on the sizes alone.
+#include "feed_forward_hidden.cuh"
 #include "gemm.cuh"   // sigmoidf_exact, split3
 #include "matmul.cuh"
 #include "ops_common.cuh"
@@ -14,8 +15,15 @@
 namespace kfb {
 namespace {
 
-constexpr int kMostRows = 16384;      // of a piece
 constexpr int kMostPlanes = 64;
+
+// Rows of a piece: as many as keep what a row needs between its products below a gigabyte.  (Smaller ones, whose hidden channels would stay in L2, are no
+// faster: writes into L2 are no faster than writes through it, and every piece starts and ends its launches.)
+long long piece_rows(long long rows, int c, int hidden, int precise, int backward, bool one) {
+  const long long per_row = precise ? 12ll * c + (backward ? 30ll : 14ll) * hidden : one ? (backward ? 6ll : 2ll) * hidden : (backward ? 18ll : 10ll) * hidden;
+  const long long most = ((1ll << 30) / per_row + 255) / 256 * 256;
+  return rows < most ? rows : most;
+}
 
 // h and, with dh, [da, db] from u = [a, b] (rows, 2 hidden) and dh (rows, hidden); four hidden channels a thread.  PARTS == 3: the results as three
 // bf16 parts each, planes rows * hidden and rows * 2 hidden apart.
@@ -61,17 +69,21 @@ __global__ void __launch_bounds__(256) ffn_hidden_kernel(const float* u, const f
 
 struct FfnWs {
   __nv_bfloat16 *x3, *dy3, *wi3, *wo3;      // fp32-accurate mode: the operands' parts
-  float *u, *dh;
-  __nv_bfloat16 *h, *dab;
+  float *u, *dh;                            // where no kernel keeps them in tensor memory
+  __nv_bfloat16 *h, *dab, *wi_t;
   float *pl_in, *pl_out;
 };
+// Whether h, da and db come from the one kernel (feed_forward_hidden.cu).
+bool one_kernel(int c, int hidden, int precise) { return !precise && ffn_hidden_ok(c, hidden); }
 // Pieces that the rows of a weight's gradient are summed in.
-int planes_in(long long rows, int c, int hidden) { return matmul_splits(2 * hidden, c, rows < kMostRows ? rows : kMostRows, kMostPlanes); }
-int planes_out(long long rows, int c, int hidden) { return matmul_splits(c, hidden, rows < kMostRows ? rows : kMostRows, kMostPlanes); }
+int planes_in(long long piece, int c, int hidden) { return matmul_splits(2 * hidden, c, piece, kMostPlanes); }
+int planes_out(long long piece, int c, int hidden) { return matmul_splits(c, hidden, piece, kMostPlanes); }
 
 size_t carve(FfnWs& w, void* base, long long rows, int c, int hidden, int precise, int backward) {
   Carver cv(base);
-  const size_t r = static_cast<size_t>(rows < kMostRows ? rows : kMostRows), parts = precise ? 3 : 1, cc = c, hh = hidden;
+  const bool one = one_kernel(c, hidden, precise);
+  const long long piece = piece_rows(rows, c, hidden, precise, backward, one);
+  const size_t r = static_cast<size_t>(piece), parts = precise ? 3 : 1, cc = c, hh = hidden;
   w = {};
   if (precise) {
     w.x3 = cv.take<__nv_bfloat16>(3 * r * cc);
@@ -79,13 +91,14 @@ size_t carve(FfnWs& w, void* base, long long rows, int c, int hidden, int precis
     w.wo3 = cv.take<__nv_bfloat16>(3 * hh * cc);
     if (backward) w.dy3 = cv.take<__nv_bfloat16>(3 * r * cc);
   }
-  w.u = cv.take<float>(r * 2 * hh);
+  if (!one) w.u = cv.take<float>(r * 2 * hh);
   w.h = cv.take<__nv_bfloat16>(parts * r * hh);
   if (backward) {
-    w.dh = cv.take<float>(r * hh);
+    if (!one) w.dh = cv.take<float>(r * hh);
+    if (!precise) w.wi_t = cv.take<__nv_bfloat16>(2 * hh * cc);
     w.dab = cv.take<__nv_bfloat16>(parts * r * 2 * hh);
-    w.pl_in = cv.take<float>(planes_in(rows, c, hidden) * 2 * hh * cc);
-    w.pl_out = cv.take<float>(planes_out(rows, c, hidden) * hh * cc);
+    w.pl_in = cv.take<float>(planes_in(piece, c, hidden) * 2 * hh * cc);
+    w.pl_out = cv.take<float>(planes_out(piece, c, hidden) * hh * cc);
   }
   return cv.off;
 }
@@ -95,6 +108,39 @@ int launch_hidden(cudaStream_t stream, const FfnWs& w, bool backward, long long 
   LaunchScope scope(stream, "feed_forward_hidden");
   return launch_kernel(stream, precise ? ffn_hidden_kernel<3> : ffn_hidden_kernel<1>, static_cast<unsigned>(want < most ? want : most), 256, 0,
                        const_cast<const float*>(w.u), backward ? const_cast<const float*>(w.dh) : nullptr, w.h, w.dab, rows, hidden);
+}
+
+// t[j][i] = w[i][j], 32 x 32 a block
+__global__ void __launch_bounds__(256) transpose_kernel(const __nv_bfloat16* w, __nv_bfloat16* t, int rows, int cols) {
+  __shared__ __nv_bfloat16 s[32][34];
+  grid_dependency_enter();
+  const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32, i = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int k = i; k < 32; k += 8)
+    if (r0 + k < rows && c0 + lane < cols) s[k][lane] = w[static_cast<long long>(r0 + k) * cols + c0 + lane];
+  __syncthreads();
+#pragma unroll
+  for (int k = i; k < 32; k += 8)
+    if (c0 + k < cols && r0 + lane < rows) t[static_cast<long long>(c0 + k) * rows + r0 + lane] = s[lane][k];
+}
+int launch_transpose(cudaStream_t stream, const void* w, __nv_bfloat16* t, int rows, int cols) {
+  LaunchScope scope(stream, "feed_forward_transpose");
+  return launch_kernel(stream, transpose_kernel, dim3(cdiv(cols, 32), cdiv(rows, 32)), 256, 0, static_cast<const __nv_bfloat16*>(w), t, rows, cols);
+}
+
+// out = a b^T, a (m, k), b (n, k): the library's own product for operands along k
+int product(cudaStream_t stream, const void* a, const void* b, void* out, long long m, int n, int k, const char* tag) {
+  GemmParams p = {};
+  p.n_extent = static_cast<int>(m);
+  p.o_extent = 1;
+  p.batch = 1;
+  p.n_cols = n;
+  p.k_extent = k;
+  p.nseg = 1;
+  p.seg[0] = row_major_seg(out, n, n, 0, 0, 0);
+  GemmOperandA oa = {a, k, 0, 0};
+  GemmOperandB ob = {b, k, 0};
+  return launch_gemm_bf16(stream, oa, ob, p, 0, tag);
 }
 
 int check(const char* name, const void* workspace, size_t workspace_bytes, size_t need, long long rows, int c, int hidden, int dtype,
@@ -140,10 +186,17 @@ KFB_API int kfb_feed_forward_fwd(const void* x, const void* w_in, const void* w_
     KFB_TRY(launch_split_planes(s, static_cast<const float*>(w_out), w.wo3, wo_n, wo_n));
   }
   const void *wi = precise ? w.wi3 : w_in, *wo = precise ? w.wo3 : w_out;
-  for (long long r0 = 0; r0 < rows; r0 += kMostRows) {
-    const long long r = rows - r0 < kMostRows ? rows - r0 : kMostRows;
+  const bool one = one_kernel(c, hidden, precise);
+  const long long piece = piece_rows(rows, c, hidden, precise, 0, one);
+  for (long long r0 = 0; r0 < rows; r0 += piece) {
+    const long long r = rows - r0 < piece ? rows - r0 : piece;
     const int m = static_cast<int>(r);
     const void* xr = static_cast<const char*>(x) + r0 * c * size;
+    if (one) {
+      KFB_TRY(launch_ffn_hidden(s, xr, nullptr, wi, wo, w.h, nullptr, m, c, hidden));
+      KFB_TRY(product(s, w.h, wo, static_cast<char*>(out) + r0 * c * size, r, c, hidden, "feed_forward_out"));
+      continue;
+    }
     if (precise) {
       KFB_TRY(launch_split_planes(s, static_cast<const float*>(xr), w.x3, r * c, r * c));
       xr = w.x3;
@@ -183,9 +236,12 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
     KFB_TRY(launch_split_planes(s, static_cast<const float*>(w_out), w.wo3, wo_n, wo_n));
   }
   const void *wi = precise ? w.wi3 : w_in, *wo = precise ? w.wo3 : w_out;
-  const int most_in = planes_in(rows, c, hidden), most_out = planes_out(rows, c, hidden);
-  for (long long r0 = 0; r0 < rows; r0 += kMostRows) {
-    const long long r = rows - r0 < kMostRows ? rows - r0 : kMostRows;
+  const bool one = one_kernel(c, hidden, precise);
+  const long long piece = piece_rows(rows, c, hidden, precise, 1, one);
+  const int most_in = planes_in(piece, c, hidden), most_out = planes_out(piece, c, hidden);
+  if (!precise && dx != nullptr) KFB_TRY(launch_transpose(s, w_in, w.wi_t, 2 * hidden, c));
+  for (long long r0 = 0; r0 < rows; r0 += piece) {
+    const long long r = rows - r0 < piece ? rows - r0 : piece;
     const int m = static_cast<int>(r);
     const void *xr = static_cast<const char*>(x) + r0 * c * size, *dr = static_cast<const char*>(dy) + r0 * c * size;
     if (precise) {
@@ -199,12 +255,22 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
       o.by_k = 1;
       return o;
     };
-    MatmulArgs in = {mx, {wi, c, 0, wi_n}, m, 2 * hidden, c, w.u, 2ll * hidden, 1, 1, 0, 0, precise, "feed_forward_in"};
-    KFB_TRY(launch_matmul(s, in));
-    MatmulArgs dh = {md, {wo, hidden, 1, wo_n}, m, hidden, c, w.dh, hidden, 1, 1, 0, 0, precise, "feed_forward_dh"};
-    KFB_TRY(launch_matmul(s, dh));
-    KFB_TRY(launch_hidden(s, w, true, r, hidden, precise));
-    if (dx != nullptr) {
+    const bool rows_too = one && dx != nullptr && ffn_rows_ok(c, hidden) && m >= 64 * sm_count();
+    void* dxr = static_cast<char*>(dx) + r0 * c * size;
+    if (rows_too) {
+      KFB_TRY(launch_ffn_rows(s, xr, dr, wi, wo, dxr, w.h, w.dab, m, c, hidden));
+    } else if (one) {
+      KFB_TRY(launch_ffn_hidden(s, xr, dr, wi, wo, w.h, w.dab, m, c, hidden));
+    } else {
+      MatmulArgs in = {mx, {wi, c, 0, wi_n}, m, 2 * hidden, c, w.u, 2ll * hidden, 1, 1, 0, 0, precise, "feed_forward_in"};
+      KFB_TRY(launch_matmul(s, in));
+      MatmulArgs dh = {md, {wo, hidden, 1, wo_n}, m, hidden, c, w.dh, hidden, 1, 1, 0, 0, precise, "feed_forward_dh"};
+      KFB_TRY(launch_matmul(s, dh));
+      KFB_TRY(launch_hidden(s, w, true, r, hidden, precise));
+    }
+    if (dx != nullptr && !precise && !rows_too) {
+      KFB_TRY(product(s, w.dab, w.wi_t, dxr, r, c, 2 * hidden, "feed_forward_dx"));
+    } else if (dx != nullptr && precise) {
       MatmulArgs g = {mg, {wi, c, 1, wi_n}, m, c, 2 * hidden, static_cast<char*>(dx) + r0 * c * size, c, precise, 1, 0, 0, precise, "feed_forward_dx"};
       KFB_TRY(launch_matmul(s, g));
     }

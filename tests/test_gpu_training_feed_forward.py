@@ -83,6 +83,12 @@ def test_many_rows(rows, c, hidden):
     _check(*_case(rows, c, hidden, seed=5))
 
 
+@pytest.mark.parametrize("rows, c, hidden, dtype", [(30001, 64, 8192, BF), (47000, 128, 8192, BF), (23000, 256, 8192, BF), (9000, 72, 8192, BF), (5000, 8, 8192, F32)])
+def test_rows_in_several_pieces(rows, c, hidden, dtype):
+    """More rows than a workspace holds at once, the last piece a short one."""
+    _check(*_case(rows, c, hidden, dtype=dtype, seed=3))
+
+
 @pytest.mark.parametrize("rows, c, hidden", [(1, 128, 512), (200, 128, 512), (129, 256, 1024), (65, 72, 136), (777, 384, 1536), (17000, 64, 64)])
 def test_float32(rows, c, hidden):
     _check(*_case(rows, c, hidden, dtype=F32, seed=9))

@@ -74,7 +74,7 @@ def test_feed_forward_workspace_stops_growing(library):
     for c in (128, 256, 384):
         for dt in (0, 2):
             for backward in (0, 1):
-                sizes = [need(r, c, 4 * c, dt, backward) for r in (1, 1000, 1 << 17, 1 << 20, (1 << 31) - 1)]
+                sizes = [need(r, c, 4 * c, dt, backward) for r in (1, 1000, 1 << 20, 1 << 22, (1 << 31) - 1)]
                 assert sizes == sorted(sizes) and sizes[-1] == sizes[-2] == sizes[-3] and sizes[0] > 0
     assert need(0, 128, 512, 0, 0) == need(5, 0, 512, 0, 0) == 0
 

@@ -342,7 +342,7 @@ static int launch_single(cudaStream_t stream, const void* x, void* y, const floa
     return KFB_ERR_UNSUPPORTED;
   }
   const long long want = (rows + 7) / 8, most = static_cast<long long>(sm_count()) * 16;
-  auto kernel = c <= 256 ? layernorm_single_kernel<TI, TO, 8> : layernorm_single_kernel<TI, TO, 32>;
+  auto kernel = c <= 256 ? layernorm_single_kernel<TI, TO, 8> : c <= 512 ? layernorm_single_kernel<TI, TO, 16> : layernorm_single_kernel<TI, TO, 32>;
   LaunchScope scope(stream, "layernorm_single");
   return launch_kernel(stream, kernel, static_cast<unsigned>(want < most ? want : most), 256, 0, static_cast<const TI*>(x), static_cast<TO*>(y), w,
                        b, rows, c, xs, ys, eps);

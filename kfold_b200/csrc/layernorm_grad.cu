@@ -19,12 +19,39 @@ namespace {
 
 constexpr int kWarps = 8;
 
-template <int LANES>
-__device__ __forceinline__ float lanes_sum(float v) {
+// V elements as they lie in memory: what is on its way takes no more registers than its bytes.
+template <typename T, int V>
+struct Raw {
+  static constexpr int kBytes = V * static_cast<int>(sizeof(T)), kWords = kBytes < 4 ? 1 : kBytes / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* p, bool there) {
+    if constexpr (kBytes % 16 == 0) {
 #pragma unroll
-  for (int m = LANES / 2; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-  return v;
-}
+      for (int i = 0; i < kBytes / 16; ++i) {
+        const uint4 t = there ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0, 0, 0, 0);
+        w[4 * i] = t.x;
+        w[4 * i + 1] = t.y;
+        w[4 * i + 2] = t.z;
+        w[4 * i + 3] = t.w;
+      }
+    } else if constexpr (kBytes == 8) {
+      const uint2 t = there ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
+      w[0] = t.x;
+      w[1] = t.y;
+    } else if constexpr (kBytes == 4) {
+      w[0] = there ? *reinterpret_cast<const uint32_t*>(p) : 0u;
+    } else {
+      w[0] = there ? *reinterpret_cast<const unsigned short*>(p) : 0u;
+    }
+  }
+  __device__ __forceinline__ void values(float* v) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
+      else v[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+  }
+};
 
 // LANES lanes hold a row, P pieces of V channels each; R rows in flight for each group of lanes.  EXACT: c == LANES * V * P.  PARAMS: dw, db wanted.
 template <typename TX, typename TD, int V, int LANES, int P, int R, bool EXACT, bool PARAMS>
@@ -44,60 +71,90 @@ __global__ void __launch_bounds__(32 * kWarps) layernorm_grad_kernel(const TD* d
 #pragma unroll
   for (int i = 0; i < (PARAMS ? N : 1); ++i) aw[i] = ab[i] = 0.f;
 
-  const long long warps = static_cast<long long>(gridDim.x) * kWarps;
-  for (long long base = (static_cast<long long>(blockIdx.x) * kWarps + warp) * kRows; base < rows; base += warps * kRows) {
-    float xv[R][N], dv[R][N];
+  // The next rows' pieces are on their way while these are worked on.  (They have to be asked for before this step's stores: behind one, a load waits.)
+  const long long step = static_cast<long long>(gridDim.x) * kWarps * kRows;
+  Raw<TX, V> x_raw[R][P];
+  Raw<TD, V> d_raw[R][P];
+  auto fetch = [&](long long base) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const long long row = base + r * kGroups + lane / LANES;
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        if (row < rows && inside(p)) {
-          load_vec<V>(x + row * c + channel(p), &xv[r][p * V]);
-          load_vec<V>(dy + row * c + channel(p), &dv[r][p * V]);
-        } else {
+        const bool there = row < rows && inside(p);
+        x_raw[r][p].load(x + row * c + channel(p), there);
+        d_raw[r][p].load(dy + row * c + channel(p), there);
+      }
+    }
+  };
+  long long base = (static_cast<long long>(blockIdx.x) * kWarps + warp) * kRows;
+  if (base < rows) fetch(base);
+  for (; base < rows; base += step) {
+    float xv[R][N], dv[R][N], mean[R], sg[R], q[R], sz[R];
 #pragma unroll
-          for (int i = 0; i < V; ++i) xv[r][p * V + i] = dv[r][p * V + i] = 0.f;
-        }
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        x_raw[r][p].values(&xv[r][p * V]);
+        d_raw[r][p].values(&dv[r][p * V]);
+      }
+    if (base + step < rows) fetch(base + step);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mean[r] = sg[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        mean[r] += xv[r][i];
+        sg[r] = fmaf(dv[r][i], wv[i], sg[r]);
       }
     }
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const long long row = base + r * kGroups + lane / LANES;
-      float s = 0.f, sg = 0.f;
+    for (int m = LANES / 2; m > 0; m >>= 1)
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        s += xv[r][i];
-        sg = fmaf(dv[r][i], wv[i], sg);
+      for (int r = 0; r < R; ++r) {
+        mean[r] += __shfl_xor_sync(0xffffffffu, mean[r], m);
+        sg[r] += __shfl_xor_sync(0xffffffffu, sg[r], m);
       }
-      const float mean = lanes_sum<LANES>(s) * inv_c;
-      sg = lanes_sum<LANES>(sg) * inv_c;
-      float q = 0.f, sz = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mean[r] *= inv_c;
+      q[r] = sz[r] = 0.f;
 #pragma unroll
       for (int p = 0; p < P; ++p)
 #pragma unroll
         for (int i = p * V; i < p * V + V; ++i) {
-          xv[r][i] = inside(p) ? xv[r][i] - mean : 0.f;
-          q = fmaf(xv[r][i], xv[r][i], q);
-          sz = fmaf(dv[r][i] * wv[i], xv[r][i], sz);
+          xv[r][i] = inside(p) ? xv[r][i] - mean[r] : 0.f;
+          q[r] = fmaf(xv[r][i], xv[r][i], q[r]);
+          sz[r] = fmaf(dv[r][i] * wv[i], xv[r][i], sz[r]);
         }
-      const float rstd = rsqrtf(lanes_sum<LANES>(q) * inv_c + eps);
-      sz = lanes_sum<LANES>(sz) * inv_c * rstd;
-      if (row < rows) {
+    }
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-          float o[V];
+    for (int m = LANES / 2; m > 0; m >>= 1)
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float z = xv[r][p * V + i] * rstd, d = dv[r][p * V + i];
-            o[i] = rstd * (fmaf(d, wv[p * V + i], -sg) - z * sz);
-            if constexpr (PARAMS) {
-              aw[p * V + i] = fmaf(d, z, aw[p * V + i]);
-              ab[p * V + i] += d;
-            }
+      for (int r = 0; r < R; ++r) {
+        q[r] += __shfl_xor_sync(0xffffffffu, q[r], m);
+        sz[r] += __shfl_xor_sync(0xffffffffu, sz[r], m);
+      }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long row = base + r * kGroups + lane / LANES;
+      if (row >= rows) continue;
+      const float rstd = rsqrtf(q[r] * inv_c + eps);
+      sz[r] *= inv_c * rstd;
+      sg[r] *= inv_c;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float z = xv[r][p * V + i] * rstd, d = dv[r][p * V + i];
+          o[i] = rstd * (fmaf(d, wv[p * V + i], -sg[r]) - z * sz[r]);
+          if constexpr (PARAMS) {
+            aw[p * V + i] = fmaf(d, z, aw[p * V + i]);
+            ab[p * V + i] += d;
           }
-          if (inside(p)) store_vec<V>(dx + row * c + channel(p), o);
         }
+        if (inside(p)) store_vec<V>(dx + row * c + channel(p), o);
       }
     }
   }
@@ -228,6 +285,7 @@ int dispatch(const Args& a) {
     }
   }
   if (a.c <= 256) return launch<TX, TD, 1, 32, 8, false>(a);
+  if (a.c <= 512) return launch<TX, TD, 1, 32, 16, false>(a);
   return launch<TX, TD, 1, 32, 32, false>(a);
 }
 

@@ -11,6 +11,7 @@
 #include "gemm.cuh"   // sigmoidf_exact, split3
 #include "matmul.cuh"
 #include "ops_common.cuh"
+#include "transition_pair.cuh"
 
 namespace kfb {
 namespace {
@@ -178,6 +179,8 @@ KFB_API int kfb_feed_forward_fwd(const void* x, const void* w_in, const void* w_
   cudaStream_t s = as_stream(stream);
   const int precise = dtype == KFB_FP32_PRECISE;
   const size_t size = precise ? 4 : 2;
+  if (!precise && feed_forward_pair_ok(rows, c, hidden) && transition_pair_is_faster(rows, c, hidden))
+    return launch_feed_forward_pair(s, x, w_in, w_out, out, rows, c, hidden);
   FfnWs w;
   carve(w, workspace, rows, c, hidden, precise, 0);
   const long long wi_n = 2ll * hidden * c, wo_n = static_cast<long long>(hidden) * c;
@@ -239,7 +242,7 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
   const bool one = one_kernel(c, hidden, precise);
   const long long piece = piece_rows(rows, c, hidden, precise, 1, one);
   const int most_in = planes_in(piece, c, hidden), most_out = planes_out(piece, c, hidden);
-  if (!precise && dx != nullptr) KFB_TRY(launch_transpose(s, w_in, w.wi_t, 2 * hidden, c));
+  bool transposed = false;
   for (long long r0 = 0; r0 < rows; r0 += piece) {
     const long long r = rows - r0 < piece ? rows - r0 : piece;
     const int m = static_cast<int>(r);
@@ -269,6 +272,8 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
       KFB_TRY(launch_hidden(s, w, true, r, hidden, precise));
     }
     if (dx != nullptr && !precise && !rows_too) {
+      if (!transposed) KFB_TRY(launch_transpose(s, w_in, w.wi_t, 2 * hidden, c));
+      transposed = true;
       KFB_TRY(product(s, w.dab, w.wi_t, dxr, r, c, 2 * hidden, "feed_forward_dx"));
     } else if (dx != nullptr && precise) {
       MatmulArgs g = {mg, {wi, c, 1, wi_n}, m, c, 2 * hidden, static_cast<char*>(dx) + r0 * c * size, c, precise, 1, 0, 0, precise, "feed_forward_dx"};

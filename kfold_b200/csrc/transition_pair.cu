@@ -63,7 +63,9 @@ struct PairTransParams {
   float eps;
 };
 
-template <int C>
+// RAW: the gated feed-forward alone, on parameters as a module holds them: rows are multiplied as they come, the value rows of w1 lie before its gate
+// rows and are not halved.
+template <int C, bool RAW>
 __global__ void __launch_bounds__(kThreads, 1)
 transition_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w1, const __grid_constant__ CUtensorMap tm_w2,
                        const __grid_constant__ CUtensorMap tm_r, const __grid_constant__ CUtensorMap tm_out, const PairTransParams p) {
@@ -151,7 +153,7 @@ transition_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
           grid_dependency_launch();
         }
         if (i < total) {
-          const int row = (c1 >> 1) * 256 + 128 * rank + (c1 & 1) * kChunk;
+          const int row = RAW ? rank * p.chunks * kChunk + c1 * kChunk : (c1 >> 1) * 256 + 128 * rank + (c1 & 1) * kChunk;
           for (int u = 0; u < K::kUnits; ++u) {
             ok = ptx::mbar_wait(&empty[slot], par ^ 1, 401);
             if (!ok) break;
@@ -278,7 +280,13 @@ transition_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         uint32_t w[8];
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-          w[j >> 1] = pack_bf16x2(ptx::mul2(glu_half2(v[j], v[j + 1], v[j], v[j + 1]), ptx::pack2(g[j], g[j + 1])));
+          if constexpr (RAW) {
+            const float2 a = ptx::unpack2(ptx::mul2(ptx::pack2(v[j], v[j + 1]), ptx::pack2(0.5f, 0.5f)));
+            w[j >> 1] = pack_bf16x2(ptx::mul2(ptx::fma2(ptx::pack2(a.x, a.y), ptx::pack2(tanh_fast(a.x), tanh_fast(a.y)), ptx::pack2(a.x, a.y)),
+                                              ptx::pack2(g[j], g[j + 1])));
+          } else {
+            w[j >> 1] = pack_bf16x2(ptx::mul2(glu_half2(v[j], v[j + 1], v[j], v[j + 1]), ptx::pack2(g[j], g[j + 1])));
+          }
         }
         ptx::tmem_st_32x32b_x8(t + c / 2, w);
       };
@@ -309,7 +317,7 @@ transition_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + col0;
     grid_dependency_wait();
     uint64_t lw[4], lb[4];
-    rows_affine<C>(p.ln_w, p.ln_b, lane, lw, lb);
+    if constexpr (!RAW) rows_affine<C>(p.ln_w, p.ln_b, lane, lw, lb);
     bool ok = true;
     int ab = 0, ob = 0;                          // buffers of the next tile and of the last, and their phases
     uint32_t a_par = 0, o_par = 0;
@@ -317,7 +325,7 @@ transition_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       if (it < my_tiles) {
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(&rows_in[ab], a_par, 408)) != 0;
         if (!ok) break;
-        rows_layernorm<C>(s_a + ab * K::kABytes, part * (kRows / kRowWarps), kRows / kRowWarps, lane, lw, lb, p.eps);
+        if constexpr (!RAW) rows_layernorm<C>(s_a + ab * K::kABytes, part * (kRows / kRowWarps), kRows / kRowWarps, lane, lw, lb, p.eps);
         ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&a_norm[ab]);
@@ -404,7 +412,7 @@ transition_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
 }
 
 // Pairs of CTAs that the current device holds at once (0: none), asked once per device.
-template <int C>
+template <int C, bool RAW = false>
 int pairs_held() {
   static std::once_flag once[64];
   static int held[64];
@@ -413,12 +421,12 @@ int pairs_held() {
     cudaGetLastError();
     return 0;
   }
-  std::call_once(once[dev & 63], [&] { held[dev & 63] = clusters_held(transition_pair_kernel<C>, 2, kThreads, Cfg<C>::kSmem); });
+  std::call_once(once[dev & 63], [&] { held[dev & 63] = clusters_held(transition_pair_kernel<C, RAW>, 2, kThreads, Cfg<C>::kSmem); });
   return held[dev & 63];
 }
 int pairs_held(int c) { return c == 128 ? pairs_held<128>() : pairs_held<256>(); }
 
-template <int C>
+template <int C, bool RAW>
 int launch(cudaStream_t stream, const void* x, const float* ln_w, const float* ln_b, const void* w_swiglu, const void* w_out, void* out,
            const void* resid, long long rows, int hidden, float eps, int w_static) {
   auto rows_map = [&](CUtensorMap* m, const void* ptr, long long n, int c, uint32_t box_rows) {
@@ -433,7 +441,7 @@ int launch(cudaStream_t stream, const void* x, const float* ln_w, const float* l
   KFB_TRY(rows_map(&t2, w_out, C, hidden, C / 2));
   KFB_TRY(rows_map(&tr, resid != nullptr ? resid : x, rows, C, kRows));
   KFB_TRY(rows_map(&to, out, rows, C, kRows));
-  const int held = pairs_held<C>();
+  const int held = pairs_held<C, RAW>();
   KFB_CHECK_ARG(held > 0, "transition: the device holds no pair of this kernel");
   PairTransParams p;
   p.ln_w = ln_w;
@@ -444,8 +452,8 @@ int launch(cudaStream_t stream, const void* x, const float* ln_w, const float* l
   p.has_resid = resid != nullptr;
   p.w_static = w_static;
   p.eps = eps;
-  LaunchScope scope(stream, "transition_pair");
-  return launch_kernel_clustered(stream, transition_pair_kernel<C>, 2, 2 * (p.tiles < held ? p.tiles : held), kThreads, Cfg<C>::kSmem, tx, t1, t2,
+  LaunchScope scope(stream, RAW ? "feed_forward_pair" : "transition_pair");
+  return launch_kernel_clustered(stream, transition_pair_kernel<C, RAW>, 2, 2 * (p.tiles < held ? p.tiles : held), kThreads, Cfg<C>::kSmem, tx, t1, t2,
                                  tr, to, p);
 }
 
@@ -476,8 +484,18 @@ bool transition_pair_is_faster(long long rows, int c, int hidden) {
 
 int launch_transition_pair(cudaStream_t stream, const void* x, const float* ln_w, const float* ln_b, const void* w_swiglu, const void* w_out,
                            void* out, const void* resid, long long rows, int c, int hidden, float eps, int w_static) {
-  return c == 128 ? launch<128>(stream, x, ln_w, ln_b, w_swiglu, w_out, out, resid, rows, hidden, eps, w_static)
-                  : launch<256>(stream, x, ln_w, ln_b, w_swiglu, w_out, out, resid, rows, hidden, eps, w_static);
+  return c == 128 ? launch<128, false>(stream, x, ln_w, ln_b, w_swiglu, w_out, out, resid, rows, hidden, eps, w_static)
+                  : launch<256, false>(stream, x, ln_w, ln_b, w_swiglu, w_out, out, resid, rows, hidden, eps, w_static);
+}
+
+bool feed_forward_pair_ok(long long rows, int c, int hidden) {
+  if ((c != 128 && c != 256) || hidden % 128 != 0 || rows > (1ll << 30)) return false;
+  return (c == 128 ? pairs_held<128, true>() : pairs_held<256, true>()) > 0;
+}
+
+int launch_feed_forward_pair(cudaStream_t stream, const void* x, const void* w_in, const void* w_out, void* out, long long rows, int c, int hidden) {
+  return c == 128 ? launch<128, true>(stream, x, nullptr, nullptr, w_in, w_out, out, nullptr, rows, hidden, 0.f, 0)
+                  : launch<256, true>(stream, x, nullptr, nullptr, w_in, w_out, out, nullptr, rows, hidden, 0.f, 0);
 }
 
 }  // namespace kfb

@@ -14,4 +14,10 @@ bool transition_pair_is_faster(long long rows, int c, int hidden);
 int launch_transition_pair(cudaStream_t stream, const void* x, const float* ln_w, const float* ln_b, const void* w_swiglu, const void* w_out,
                            void* out, const void* resid, long long rows, int c, int hidden, float eps, int w_static);
 
+
+// The same kernel without LayerNorm and residual, on the parameters as a module holds them (w_in: value rows, then gate rows): the gated feed-forward.
+// Tensors 16-byte aligned.
+bool feed_forward_pair_ok(long long rows, int c, int hidden);
+int launch_feed_forward_pair(cudaStream_t stream, const void* x, const void* w_in, const void* w_out, void* out, long long rows, int c, int hidden);
+
 }  // namespace kfb

@@ -76,6 +76,8 @@ struct FfnWs {
 };
 // Whether h, da and db come from the one kernel (feed_forward_hidden.cu).
 bool one_kernel(int c, int hidden, int precise) { return !precise && ffn_hidden_ok(c, hidden); }
+// Whether both gradients come from x and dy alone, nothing kept in between (feed_forward_rows.cu, feed_forward_weights.cu).
+bool nothing_kept(int c, int hidden, int precise) { return !precise && ffn_weights_ok(c, hidden) && ffn_rows_ok(c, hidden); }
 // Pieces that the rows of a weight's gradient are summed in.
 int planes_in(long long piece, int c, int hidden) { return matmul_splits(2 * hidden, c, piece, kMostPlanes); }
 int planes_out(long long piece, int c, int hidden) { return matmul_splits(c, hidden, piece, kMostPlanes); }
@@ -86,6 +88,12 @@ size_t carve(FfnWs& w, void* base, long long rows, int c, int hidden, int precis
   const long long piece = piece_rows(rows, c, hidden, precise, backward, one);
   const size_t r = static_cast<size_t>(piece), parts = precise ? 3 : 1, cc = c, hh = hidden;
   w = {};
+  if (backward && nothing_kept(c, hidden, precise)) {
+    const size_t planes = ffn_weights_planes(rows, hidden);
+    w.pl_in = cv.take<float>(planes * 2 * hh * cc);
+    w.pl_out = cv.take<float>(planes * hh * cc);
+    return cv.off;
+  }
   if (precise) {
     w.x3 = cv.take<__nv_bfloat16>(3 * r * cc);
     w.wi3 = cv.take<__nv_bfloat16>(3 * 2 * hh * cc);
@@ -234,6 +242,15 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
                 bits(dy) | bits(x) | bits(w_in) | bits(w_out) | bits(dx) | bits(dw_in) | bits(dw_out)));
   FfnWs w;
   carve(w, workspace, rows, c, hidden, precise, 1);
+  if (nothing_kept(c, hidden, precise)) {
+    const int r = static_cast<int>(rows), planes = ffn_weights_planes(rows, hidden);
+    if (dx != nullptr) KFB_TRY(launch_ffn_rows(s, x, dy, w_in, w_out, dx, nullptr, nullptr, r, c, hidden));
+    if (dw_in == nullptr && dw_out == nullptr) return KFB_OK;
+    KFB_TRY(launch_ffn_weights(s, x, dy, w_in, w_out, dw_in != nullptr ? w.pl_in : nullptr, dw_out != nullptr ? w.pl_out : nullptr, r, hidden));
+    if (dw_in != nullptr) KFB_TRY(launch_sum_planes(s, w.pl_in, wi_n, planes, dw_in, grad_dtype == KFB_FP32, wi_n));
+    if (dw_out != nullptr) KFB_TRY(launch_sum_planes(s, w.pl_out, wo_n, planes, dw_out, grad_dtype == KFB_FP32, wo_n));
+    return KFB_OK;
+  }
   if (precise) {
     KFB_TRY(launch_split_planes(s, static_cast<const float*>(w_in), w.wi3, wi_n, wi_n));
     KFB_TRY(launch_split_planes(s, static_cast<const float*>(w_out), w.wo3, wo_n, wo_n));

@@ -8,10 +8,10 @@
 //
 // Split.  A CTA pair takes 256 rows, 128 in each CTA, and walks the hidden channels in chunks of 64:
 //   S  = [x [Wa; Wb]^T | dy Wo]   192 columns                              (CTA 0 loads the chunk's rows of Wa, CTA 1 those of Wb, each half of Wo's)
-//   P  = [da | db] as bf16        64 columns of tensor memory
+//   P  = da, db as bf16           64 columns of tensor memory, 16 hidden channels of da and db in turn
 //   dX += P [Wa; Wb]              C columns, Wa and Wb read across k       (each CTA loads its half of the channels)
-// S and dX have a thread each that issues them.  dX of a chunk runs while sixteen warps bring the next chunk's S into registers: one S buffer is enough,
-// and with P and dX it fills the tensor memory at 256 channels.  x and dy stay in shared memory for a tile; the next tile's come into L2 meanwhile, and
+// S and dX have a thread each that issues them, in the order S(i + 1), dX(i): dX runs while sixteen warps bring S into registers, so that one S buffer is
+// enough; with P and dX it fills the tensor memory at 256 channels.  x and dy stay in shared memory for a tile; the next tile's come into L2 meanwhile, and
 // into the buffers as its slots fall free.
 #include <mutex>
 
@@ -26,20 +26,20 @@ constexpr int kRows = 128, kChunk = 64;
 constexpr int kBox = kRows * 128;                    // [128 rows][64 bf16], 128-byte swizzle
 constexpr int kRowSlot = 2 * kBox, kRowSlots = 4;    // a 64-wide block of x and of dy
 constexpr int kW1 = 64 * 128, kWo = 64 * 64;         // a CTA's [64 hidden][64 k] of Wa or Wb, and [64 k][32 hidden] of Wo (64-byte swizzle)
-constexpr int kWSlot = kW1 + kWo, kWSlots = 5;
-constexpr int kVSlots = 2;                           // of the [64 hidden][C / 2] that dX takes of Wa or Wb
+constexpr int kWSlot = kW1 + kWo, kWSlots = 4;
+constexpr int kOut = 32 * 128;                       // [32 rows][64 channels] bf16 on its way out, 128-byte swizzle
 constexpr int kEpiWarp = 4, kEpiWarps = 16;          // four warps for each 32 rows, 16 hidden channels each
 constexpr int kThreads = 32 * (kEpiWarp + kEpiWarps);
 template <int C>
 struct Cfg {
   static constexpr int kVSlot = 64 * (C / 2) * 2;
-  static constexpr int kSmem = kRowSlots * kRowSlot + kWSlots * kWSlot + kVSlots * kVSlot + 512 + 1024;
+  static constexpr int kVSlots = C == 128 ? 4 : 2;   // of the [64 hidden][C / 2] that dX takes of Wa or Wb
+  static constexpr int kSmem = kRowSlots * kRowSlot + kWSlots * kWSlot + kVSlots * kVSlot + 4 * kOut + 512 + 1024;
   static_assert(kSmem <= 232448, "shared memory");
 };
 
 struct RowsParams {
   int rows, chunks, hidden, tiles;
-  __nv_bfloat16 *dx, *h, *dab;                       // rows 32-byte aligned
 };
 
 __device__ __forceinline__ uint64_t wo_desc(uint32_t addr) {   // [k][32 hidden] rows of 64 bytes, eight of them (a swizzle atom) 512 bytes apart
@@ -50,16 +50,21 @@ __device__ __forceinline__ uint64_t v_desc(uint32_t addr) {    // [64 k][64 chan
          (1ull << 46) | (2ull << 61);
 }
 
+// The four warps that share 32 rows.
+__device__ __forceinline__ void quad_sync(int quad) { asm volatile("bar.sync %0, 128;" ::"r"(quad + 1) : "memory"); }
+
 template <int C, bool SPILL>
 __global__ void __launch_bounds__(kThreads, 1)
 ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_w1,
-                     const __grid_constant__ CUtensorMap tm_wo, const RowsParams p) {
-  constexpr int kK = C / 64, kVSlot = Cfg<C>::kVSlot;
+                     const __grid_constant__ CUtensorMap tm_wo, const __grid_constant__ CUtensorMap tm_dx, const __grid_constant__ CUtensorMap tm_h,
+                     const __grid_constant__ CUtensorMap tm_dab, const RowsParams p) {
+  constexpr int kK = C / 64, kVSlot = Cfg<C>::kVSlot, kVSlots = Cfg<C>::kVSlots;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* s_rows = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_w = s_rows + kRowSlots * kRowSlot;
   uint8_t* s_v = s_w + kWSlots * kWSlot;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + kVSlots * kVSlot);
+  uint8_t* s_out = s_v + kVSlots * kVSlot;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_out + 4 * kOut);
   uint64_t* w_full = bars;                        // in the leader: both CTAs' copies
   uint64_t* w_free = w_full + kWSlots;
   uint64_t* v_full = w_free + kWSlots;            // in the leader
@@ -68,7 +73,8 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
   uint64_t* r_free = r_full + kRowSlots;
   uint64_t* s_full = r_free + kRowSlots;
   uint64_t* s_free = s_full + 1;                  // in the leader: the element-wise warps of both CTAs
-  uint64_t* p_full = s_free + 1;                  // in the leader, likewise
+  uint64_t* s_issued = s_free + 1;                // in the leader: dX of the chunk before may follow
+  uint64_t* p_full = s_issued + 1;                // in the leader: the element-wise warps of both CTAs
   uint64_t* p_free = p_full + 1;
   uint64_t* o_full = p_free + 1;
   uint64_t* o_free = o_full + 1;                  // in the leader, likewise
@@ -98,6 +104,7 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     }
     ptx::mbar_init(s_full, 1);
     ptx::mbar_init(s_free, 2 * kEpiWarps);
+    ptx::mbar_init(s_issued, 1);
     ptx::mbar_init(p_full, 2 * kEpiWarps);
     ptx::mbar_init(p_free, 1);
     ptx::mbar_init(o_full, 1);
@@ -218,6 +225,7 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         }
         if (!ok) break;
         ptx::tc_commit_pair(s_full);
+        ptx::mbar_arrive(s_issued);
         if (++c == p.chunks) {
           c = 0;
           rs0 += kK;
@@ -235,6 +243,8 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
       bool ok = true;
       for (int i = 0; ok && i < total; ++i) {
         if (c == 0) ok = ptx::mbar_wait(o_free, (it & 1) ^ 1, 550);
+        // (behind the next chunk's S, not before or within it: the tensor core then has dX to do while that S is read)
+        if (i + 1 < total) ok = ok && ptx::mbar_wait(s_issued, (i + 1) & 1, 556);
         ok = ok && ptx::mbar_wait(p_full, i & 1, 551);
         for (int which = 0; ok && which < 2; ++which) {
           ok = ptx::mbar_wait(&v_full[v], v_ph, 552);
@@ -243,7 +253,7 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
           const uint64_t vd = vd0 + v * (kVSlot >> 4);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            ptx::mma_f16_ts_pair(tmem, tmem_p + which * 32 + k * 8, vd + k * (2048 >> 4), idesc, c > 0 || which > 0 || k > 0 ? 1u : 0u);
+            ptx::mma_f16_ts_pair(tmem, tmem_p + which * 8 + k * 16, vd + k * (2048 >> 4), idesc, c > 0 || which > 0 || k > 0 ? 1u : 0u);
           ptx::tc_commit_pair(&v_free[v]);
           if (++v == kVSlots) { v = 0; v_ph ^= 1u; }
         }
@@ -260,38 +270,56 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     // ---------------------------------------------------------------- da, db (and h); dx
     const int part = (warp - kEpiWarp) >> 2, quad = warp & 3;
     const uint32_t t_quad = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t t_s = tmem_s + t_quad + part * 16, t_p = tmem_p + t_quad + part * 8, t_o = tmem + t_quad;
+    const uint32_t t_s = tmem_s + t_quad + part * 16, t_p = tmem_p + t_quad + part * 16, t_o = tmem + t_quad;
     bool ok = true;
-    // the finished tile's dx: a quarter of the channels a warp
-    auto finish = [&](int it) {
-      ok = __all_sync(0xffffffffu, ptx::mbar_wait(o_full, it & 1, 553)) != 0;
-      if (!ok) return;
-      ptx::tc_fence_after_sync();
-      const int row = row0_of(it) + quad * 32 + lane;
-      __nv_bfloat16* out = p.dx + static_cast<long long>(row) * C + part * (C / 4);
-#pragma unroll
-      for (int q = 0; q < C / 4; q += 32) {
-        uint32_t o[32];
-        ptx::tmem_ld_32x32b_x32(t_o + part * (C / 4) + q, o);
-        ptx::tmem_ld_wait();
-        if (q + 32 == C / 4) {
-          ptx::tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive_cluster(ptx::leader_addr(o_free));
-        }
-        uint32_t w[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
-        if (row < p.rows) {
-          st_global_v8(out + q, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
-          st_global_v8(out + q + 16, w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]);
-        }
+    // 16 channels of a row from each of the four warps, as one box by the copy engine: stores from registers are 32-byte sectors of 32 lines each, which left
+    // an SM at 10 bytes a cycle and held the warps up.  (Where a wait gave up the warps keep meeting here, and leave memory alone.)
+    uint8_t* box = s_out + quad * kOut;
+    // 16-byte cells of a row's 128 bytes, swizzled: cell j of row r lies at j ^ (r % 8)
+    uint4 *cell0 = reinterpret_cast<uint4*>(box + lane * 128 + (((2 * part) ^ (lane & 7)) << 4));
+    uint4 *cell1 = reinterpret_cast<uint4*>(box + lane * 128 + (((2 * part + 1) ^ (lane & 7)) << 4));
+    const bool sender = part == 0 && lane == 0;
+    auto send = [&](const CUtensorMap* map, const uint32_t (&w)[8], int col, int row) {
+      if (sender) ptx::tma_store_wait_read();      // the box that left last
+      quad_sync(quad);
+      *cell0 = make_uint4(w[0], w[1], w[2], w[3]);
+      *cell1 = make_uint4(w[4], w[5], w[6], w[7]);
+      ptx::fence_proxy_async_smem();
+      quad_sync(quad);
+      if (sender && ok && row < p.rows) {
+        ptx::tma_store_4d(map, box, col, row, 0, 0);
+        ptx::tma_store_commit();
       }
     };
-    int c = 0, it = 0;
-    for (int i = 0; ok && i < total; ++i) {
-      ok = __all_sync(0xffffffffu, ptx::mbar_wait(s_full, i & 1, 554)) != 0;
-      if (!ok) break;
+    // the finished tile's dx
+    auto finish = [&](int it) {
+      ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(o_full, it & 1, 553)) != 0;
+      ptx::tc_fence_after_sync();
+      uint32_t w[C / 64][8];
+#pragma unroll
+      for (int q = 0; q < C / 64; ++q) {
+        uint32_t o[16];
+        ptx::tmem_ld_32x32b_x16(t_o + q * 64 + part * 16, o);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[q][j] = pack_bf16x2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
+      }
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::leader_addr(o_free));
+#pragma unroll
+      for (int q = 0; q < C / 64; ++q) send(&tm_dx, w[q], q * 64, row0_of(it) + quad * 32);
+    };
+    // da (at = 0) or db (8) of the last chunk, which P still holds
+    auto keep = [&](int at, int col, int row) {
+      uint32_t w[8];
+      ptx::tmem_ld_32x32b_x8(t_p + at, w);
+      ptx::tmem_ld_wait();
+      send(&tm_dab, w, col, row);
+    };
+    int c = 0, it = 0, last_col = 0, last_row = 0;
+    for (int i = 0; i < total; ++i) {
+      ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(s_full, i & 1, 554)) != 0;
       ptx::tc_fence_after_sync();
       uint32_t a[16], b[16], g[16];
       ptx::tmem_ld_32x32b_x16(t_s, a);
@@ -302,37 +330,38 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive_cluster(ptx::leader_addr(s_free));
       uint32_t hw[8], aw[8], bw[8];
+      auto pairs = [&](int j0) {
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        // pairs: s = tanh(a / 2) / 2 + 1 / 2, silu = a s, silu' = s + silu (1 - s)
-        const uint64_t half2 = ptx::pack2(0.5f, 0.5f), one2 = ptx::pack2(1.0f, 1.0f), minus2 = ptx::pack2(-1.0f, -1.0f);
-        const uint64_t av = ptx::pack2(a[j], a[j + 1]), bv = ptx::pack2(b[j], b[j + 1]), gv = ptx::pack2(g[j], g[j + 1]);
-        const float2 ah = ptx::unpack2(ptx::mul2(av, half2));
-        const uint64_t sv = ptx::fma2(ptx::pack2(tanh_fast(ah.x), tanh_fast(ah.y)), half2, half2);
-        const uint64_t silu = ptx::mul2(av, sv);
-        const uint64_t slope = ptx::fma2(silu, ptx::fma2(sv, minus2, one2), sv);
-        aw[j >> 1] = pack_bf16x2(ptx::mul2(ptx::mul2(gv, bv), slope));
-        bw[j >> 1] = pack_bf16x2(ptx::mul2(gv, silu));
-        if (SPILL) hw[j >> 1] = pack_bf16x2(ptx::mul2(silu, bv));
-      }
-      ok = __all_sync(0xffffffffu, ptx::mbar_wait(p_free, (i & 1) ^ 1, 555)) != 0;
-      if (!ok) break;
+        for (int j = j0; j < j0 + 8; j += 2) {
+          // s = tanh(a / 2) / 2 + 1 / 2, silu = a s, silu' = s + silu (1 - s)
+          const uint64_t half2 = ptx::pack2(0.5f, 0.5f), one2 = ptx::pack2(1.0f, 1.0f), minus2 = ptx::pack2(-1.0f, -1.0f);
+          const uint64_t av = ptx::pack2(a[j], a[j + 1]), bv = ptx::pack2(b[j], b[j + 1]), gv = ptx::pack2(g[j], g[j + 1]);
+          const float2 ah = ptx::unpack2(ptx::mul2(av, half2));
+          const uint64_t sv = ptx::fma2(ptx::pack2(tanh_fast(ah.x), tanh_fast(ah.y)), half2, half2);
+          const uint64_t silu = ptx::mul2(av, sv);
+          const uint64_t slope = ptx::fma2(silu, ptx::fma2(sv, minus2, one2), sv);
+          aw[j >> 1] = pack_bf16x2(ptx::mul2(ptx::mul2(gv, bv), slope));
+          bw[j >> 1] = pack_bf16x2(ptx::mul2(gv, silu));
+          if (SPILL) hw[j >> 1] = pack_bf16x2(ptx::mul2(silu, bv));
+        }
+      };
+      // (the last chunk's da and db leave between the halves of this one's arithmetic: a box takes some 500 cycles to go)
+      if (SPILL && i > 0) keep(0, last_col, last_row);
+      pairs(0);
+      if (SPILL && i > 0) keep(8, p.hidden + last_col, last_row);
+      pairs(8);
+      ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(p_free, (i & 1) ^ 1, 555)) != 0;
       ptx::tc_fence_after_sync();
       ptx::tmem_st_32x32b_x8(t_p, aw);
-      ptx::tmem_st_32x32b_x8(t_p + 32, bw);
+      ptx::tmem_st_32x32b_x8(t_p + 8, bw);
       ptx::tmem_st_wait();
       ptx::tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive_cluster(ptx::leader_addr(p_full));
       if (SPILL) {
-        // a whole 32-byte sector of each array a thread; the four warps of these rows fill their lines together
-        const int row = row0_of(it) + quad * 32 + lane, at = c * kChunk + part * 16;
-        if (row < p.rows) {
-          __nv_bfloat16* g_row = p.dab + 2ll * row * p.hidden + at;
-          st_global_v8(p.h + static_cast<long long>(row) * p.hidden + at, hw[0], hw[1], hw[2], hw[3], hw[4], hw[5], hw[6], hw[7]);
-          st_global_v8(g_row, aw[0], aw[1], aw[2], aw[3], aw[4], aw[5], aw[6], aw[7]);
-          st_global_v8(g_row + p.hidden, bw[0], bw[1], bw[2], bw[3], bw[4], bw[5], bw[6], bw[7]);
-        }
+        last_col = c * kChunk;
+        last_row = row0_of(it) + quad * 32;
+        send(&tm_h, hw, last_col, last_row);
       }
       // (behind the next tile's first chunk: its S then runs under dX of the last)
       if (c == 0 && it > 0) finish(it - 1);
@@ -341,7 +370,12 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         ++it;
       }
     }
-    if (ok) finish(my_tiles - 1);
+    if (SPILL) {
+      keep(0, last_col, last_row);
+      keep(8, p.hidden + last_col, last_row);
+    }
+    finish(my_tiles - 1);
+    if (sender) ptx::tma_store_wait_all();
   }
 
   ptx::tc_fence_before_sync();
@@ -376,11 +410,17 @@ int matrix_map(CUtensorMap* m, const void* ptr, long long rows, long long cols, 
 template <int C, bool SPILL>
 int launch(cudaStream_t stream, const void* x, const void* dy, const void* w_in, const void* w_out, void* dx, void* h, void* dab, int rows,
            int hidden) {
-  CUtensorMap tx, td, t1, to;
+  CUtensorMap tx, td, t1, to, tdx, th, tg;
   KFB_TRY(matrix_map(&tx, x, rows, C, kRows, 64));
   KFB_TRY(matrix_map(&td, dy, rows, C, kRows, 64));
   KFB_TRY(matrix_map(&t1, w_in, 2ll * hidden, C, kChunk, 64));
   KFB_TRY(matrix_map(&to, w_out, C, hidden, 64, 32));
+  KFB_TRY(matrix_map(&tdx, dx, rows, C, 32, 64));
+  th = tg = tdx;
+  if (SPILL) {
+    KFB_TRY(matrix_map(&th, h, rows, hidden, 32, 64));
+    KFB_TRY(matrix_map(&tg, dab, rows, 2ll * hidden, 32, 64));
+  }
   const int held = pairs_held<C, SPILL>();
   KFB_CHECK_ARG(held > 0, "feed_forward: the device holds no pair of this kernel");
   RowsParams p = {};
@@ -388,26 +428,24 @@ int launch(cudaStream_t stream, const void* x, const void* dy, const void* w_in,
   p.chunks = hidden / kChunk;
   p.hidden = hidden;
   p.tiles = cdiv(rows, 2 * kRows);
-  p.dx = static_cast<__nv_bfloat16*>(dx);
-  p.h = static_cast<__nv_bfloat16*>(h);
-  p.dab = static_cast<__nv_bfloat16*>(dab);
   LaunchScope scope(stream, SPILL ? "feed_forward_rows_grad_kept" : "feed_forward_rows_grad");
   return launch_kernel_clustered(stream, ffn_rows_pair_kernel<C, SPILL>, 2, 2 * (p.tiles < held ? p.tiles : held), kThreads, Cfg<C>::kSmem, tx, td, t1,
-                                 to, p);
+                                 to, tdx, th, tg, p);
 }
 
 }  // namespace
 
 bool ffn_rows_ok(int c, int hidden) {
-  return (c == 128 || c == 256) && hidden % 64 == 0 && (c == 128 ? pairs_held<128, false>() > 0 && pairs_held<128, true>() > 0
-                                                               : pairs_held<256, false>() > 0 && pairs_held<256, true>() > 0);
+  if (hidden % kChunk != 0) return false;
+  return c == 128 ? pairs_held<128, false>() > 0 : c == 256 && pairs_held<256, false>() > 0 && pairs_held<256, true>() > 0;
 }
 
 int launch_ffn_rows(cudaStream_t stream, const void* x, const void* dy, const void* w_in, const void* w_out, void* dx, void* h, void* dab, int rows,
                     int c, int hidden) {
-  if (c == 128)
-    return h != nullptr ? launch<128, true>(stream, x, dy, w_in, w_out, dx, h, dab, rows, hidden)
-                        : launch<128, false>(stream, x, dy, w_in, w_out, dx, h, dab, rows, hidden);
+  if (c == 128) {
+    KFB_CHECK_ARG(h == nullptr, "feed_forward: 128 channels keep nothing");
+    return launch<128, false>(stream, x, dy, w_in, w_out, dx, h, dab, rows, hidden);
+  }
   return h != nullptr ? launch<256, true>(stream, x, dy, w_in, w_out, dx, h, dab, rows, hidden)
                       : launch<256, false>(stream, x, dy, w_in, w_out, dx, h, dab, rows, hidden);
 }

@@ -162,16 +162,6 @@ ffn_weights_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
               ptx::mma_f16_ss(tmem + kS, rows_k + x1 * (kSlot >> 4) + (k >> 2) * (kBox >> 4) + (k & 3) * 2, w_ab + (k >> 2) * (kBox >> 4) + (k & 3) * 2, id_ab,
                               k > 0 ? 1u : 0u);
           }
-          if (i >= 0) {
-            if (i == 0) ok = ptx::mbar_wait(o_free, (unit & 1) ^ 1, 566);
-            ok = ok && ptx::mbar_wait(p_full, g & 1, 567);
-            if (!ok) break;
-            ptx::tc_fence_after_sync();
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              ptx::mma_f16_ss(tmem + kSumAb, rows_x + x0 * (kSlot >> 4) + k * (2048 >> 4), p_ab + k * (2048 >> 4), id_dab, i > 0 || k > 0 ? 1u : 0u);
-            ptx::tc_commit(&r_free[x0]);
-          }
           if (i + 1 < n) {
             ok = ptx::mbar_wait(&r_full[x1 + 1], ((g + 1) >> 1) & 1, 568);
             if (!ok) break;
@@ -182,6 +172,16 @@ ffn_weights_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                               k > 0 ? 1u : 0u);
             ptx::tc_commit(s_full);
             if (i + 2 == n) ptx::tc_commit(w_free);
+          }
+          if (i >= 0) {
+            if (i == 0) ok = ptx::mbar_wait(o_free, (unit & 1) ^ 1, 566);
+            ok = ok && ptx::mbar_wait(p_full, g & 1, 567);
+            if (!ok) break;
+            ptx::tc_fence_after_sync();
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              ptx::mma_f16_ss(tmem + kSumAb, rows_x + x0 * (kSlot >> 4) + k * (2048 >> 4), p_ab + k * (2048 >> 4), id_dab, i > 0 || k > 0 ? 1u : 0u);
+            ptx::tc_commit(&r_free[x0]);
           }
           if (i >= 0) {
 #pragma unroll

@@ -278,7 +278,8 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
     const bool rows_too = one && dx != nullptr && ffn_rows_ok(c, hidden) && m >= 64 * sm_count();
     void* dxr = static_cast<char*>(dx) + r0 * c * size;
     if (rows_too) {
-      KFB_TRY(launch_ffn_rows(s, xr, dr, wi, wo, dxr, w.h, w.dab, m, c, hidden));
+      const bool keep = dw_in != nullptr || dw_out != nullptr;
+      KFB_TRY(launch_ffn_rows(s, xr, dr, wi, wo, dxr, keep ? w.h : nullptr, keep ? w.dab : nullptr, m, c, hidden));
     } else if (one) {
       KFB_TRY(launch_ffn_hidden(s, xr, dr, wi, wo, w.h, w.dab, m, c, hidden));
     } else {

@@ -25,4 +25,11 @@ int ffn_weights_planes(long long rows, int hidden);
 int launch_ffn_weights(cudaStream_t stream, const void* x, const void* dy, const void* w_in, const void* w_out, float* dw_in, float* dw_out, int rows,
                        int hidden);
 
+// ... and from what was kept (feed_forward_sums.cu): 256 channels, hidden a multiple of 64.  `splits` planes (ffn_sums_planes; fewer where there are fewer
+// blocks of 64 rows) are written, or added to.
+bool ffn_sums_ok(int c, int hidden);
+int ffn_sums_planes(long long rows, int hidden);
+int launch_ffn_sums(cudaStream_t stream, const void* dab, const void* x, const void* h, const void* dy, float* dw_in, float* dw_out, int splits, int add,
+                    int rows, int hidden);
+
 }  // namespace kfb

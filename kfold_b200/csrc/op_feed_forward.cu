@@ -79,8 +79,13 @@ bool one_kernel(int c, int hidden, int precise) { return !precise && ffn_hidden_
 // Whether both gradients come from x and dy alone, nothing kept in between (feed_forward_rows.cu, feed_forward_weights.cu).
 bool nothing_kept(int c, int hidden, int precise) { return !precise && ffn_weights_ok(c, hidden) && ffn_rows_ok(c, hidden); }
 // Pieces that the rows of a weight's gradient are summed in.
-int planes_in(long long piece, int c, int hidden) { return matmul_splits(2 * hidden, c, piece, kMostPlanes); }
-int planes_out(long long piece, int c, int hidden) { return matmul_splits(c, hidden, piece, kMostPlanes); }
+bool sums_kernel(int c, int hidden, int precise) { return one_kernel(c, hidden, precise) && ffn_sums_ok(c, hidden); }
+int planes_in(long long piece, int c, int hidden, int precise) {
+  return sums_kernel(c, hidden, precise) ? ffn_sums_planes(piece, hidden) : matmul_splits(2 * hidden, c, piece, kMostPlanes);
+}
+int planes_out(long long piece, int c, int hidden, int precise) {
+  return sums_kernel(c, hidden, precise) ? ffn_sums_planes(piece, hidden) : matmul_splits(c, hidden, piece, kMostPlanes);
+}
 
 size_t carve(FfnWs& w, void* base, long long rows, int c, int hidden, int precise, int backward) {
   Carver cv(base);
@@ -106,8 +111,8 @@ size_t carve(FfnWs& w, void* base, long long rows, int c, int hidden, int precis
     if (!one) w.dh = cv.take<float>(r * hh);
     if (!precise) w.wi_t = cv.take<__nv_bfloat16>(2 * hh * cc);
     w.dab = cv.take<__nv_bfloat16>(parts * r * 2 * hh);
-    w.pl_in = cv.take<float>(planes_in(piece, c, hidden) * 2 * hh * cc);
-    w.pl_out = cv.take<float>(planes_out(piece, c, hidden) * hh * cc);
+    w.pl_in = cv.take<float>(planes_in(piece, c, hidden, precise) * 2 * hh * cc);
+    w.pl_out = cv.take<float>(planes_out(piece, c, hidden, precise) * hh * cc);
   }
   return cv.off;
 }
@@ -258,7 +263,7 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
   const void *wi = precise ? w.wi3 : w_in, *wo = precise ? w.wo3 : w_out;
   const bool one = one_kernel(c, hidden, precise);
   const long long piece = piece_rows(rows, c, hidden, precise, 1, one);
-  const int most_in = planes_in(piece, c, hidden), most_out = planes_out(piece, c, hidden);
+  const int most_in = planes_in(piece, c, hidden, precise), most_out = planes_out(piece, c, hidden, precise);
   bool transposed = false;
   for (long long r0 = 0; r0 < rows; r0 += piece) {
     const long long r = rows - r0 < piece ? rows - r0 : piece;
@@ -298,6 +303,11 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
       KFB_TRY(launch_matmul(s, g));
     }
     const int add = r0 > 0;
+    if (sums_kernel(c, hidden, precise)) {
+      if (dw_in != nullptr || dw_out != nullptr)
+        KFB_TRY(launch_ffn_sums(s, w.dab, xr, w.h, dr, dw_in != nullptr ? w.pl_in : nullptr, dw_out != nullptr ? w.pl_out : nullptr, most_in, add, m, hidden));
+      continue;
+    }
     if (dw_in != nullptr) {
       const int splits = matmul_splits(2 * hidden, c, r, most_in);
       MatmulArgs g = {across(mg), across(mx), 2 * hidden, c, r, w.pl_in, c, 1, splits, wi_n, add, precise, "feed_forward_dw"};

@@ -26,14 +26,18 @@ constexpr int kRows = 128, kChunk = 64;
 constexpr int kBox = kRows * 128;                    // [128 rows][64 bf16], 128-byte swizzle
 constexpr int kRowSlot = 2 * kBox, kRowSlots = 4;    // a 64-wide block of x and of dy
 constexpr int kW1 = 64 * 128, kWo = 64 * 64;         // a CTA's [64 hidden][64 k] of Wa or Wb, and [64 k][32 hidden] of Wo (64-byte swizzle)
-constexpr int kWSlot = kW1 + kWo, kWSlots = 4;
+constexpr int kWBlock = kW1 + kWo;
 constexpr int kOut = 32 * 128;                       // [32 rows][64 channels] bf16 on its way out, 128-byte swizzle
 constexpr int kEpiWarp = 4, kEpiWarps = 16;          // four warps for each 32 rows, 16 hidden channels each
 constexpr int kThreads = 32 * (kEpiWarp + kEpiWarps);
 template <int C>
 struct Cfg {
-  static constexpr int kVSlot = 64 * (C / 2) * 2;
-  static constexpr int kVSlots = C == 128 ? 4 : 2;   // of the [64 hidden][C / 2] that dX takes of Wa or Wb
+  // (every wait and every commit costs the thread that issues the products some 100 cycles: few and large slots)
+  static constexpr int kWSlot = 2 * kWBlock, kWSlots = 2;        // 128 k of a chunk's S
+  static constexpr int kVSlot = 2 * 64 * (C / 2) * 2, kVSlots = C == 128 ? 2 : 1;   // the [2 x 64 hidden][C / 2] that dX takes of Wa and Wb
+  // 128 channels: a tile's x and dy are brought into tensor memory too (128 columns).  A product whose left operand comes from shared memory takes some 40
+  // cycles longer: 93 for 128 columns where it is 63 from tensor memory, 67 for 64 where it is 37 (pairs, 256 rows x 16).
+  static constexpr bool kTmemRows = C == 128;
   static constexpr int kSmem = kRowSlots * kRowSlot + kWSlots * kWSlot + kVSlots * kVSlot + 4 * kOut + 512 + 1024;
   static_assert(kSmem <= 232448, "shared memory");
 };
@@ -50,6 +54,13 @@ __device__ __forceinline__ uint64_t v_desc(uint32_t addr) {    // [64 k][64 chan
          (1ull << 46) | (2ull << 61);
 }
 
+// The wait of a thread that issues products: most of what it waits for is there, or about to be, and a suspended thread is slow to come back.
+__device__ __forceinline__ bool hot_wait(uint64_t* bar, uint32_t parity, int code) {
+  for (int i = 0; i < 64; ++i)
+    if (ptx::mbar_test(bar, parity)) return true;
+  return ptx::mbar_wait(bar, parity, code);
+}
+
 // The four warps that share 32 rows.
 __device__ __forceinline__ void quad_sync(int quad) { asm volatile("bar.sync %0, 128;" ::"r"(quad + 1) : "memory"); }
 
@@ -58,7 +69,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_w1,
                      const __grid_constant__ CUtensorMap tm_wo, const __grid_constant__ CUtensorMap tm_dx, const __grid_constant__ CUtensorMap tm_h,
                      const __grid_constant__ CUtensorMap tm_dab, const RowsParams p) {
-  constexpr int kK = C / 64, kVSlot = Cfg<C>::kVSlot, kVSlots = Cfg<C>::kVSlots;
+  constexpr int kK = C / 64, kWSlot = Cfg<C>::kWSlot, kWSlots = Cfg<C>::kWSlots, kVSlot = Cfg<C>::kVSlot, kVSlots = Cfg<C>::kVSlots;
+  constexpr bool kTmemRows = Cfg<C>::kTmemRows;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* s_rows = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_w = s_rows + kRowSlots * kRowSlot;
@@ -69,7 +81,7 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
   uint64_t* w_free = w_full + kWSlots;
   uint64_t* v_full = w_free + kWSlots;            // in the leader
   uint64_t* v_free = v_full + kVSlots;
-  uint64_t* r_full = v_free + kVSlots;            // in the leader
+  uint64_t* r_full = v_free + kVSlots;            // in the leader (kTmemRows: of this CTA's rows)
   uint64_t* r_free = r_full + kRowSlots;
   uint64_t* s_full = r_free + kRowSlots;
   uint64_t* s_free = s_full + 1;                  // in the leader: the element-wise warps of both CTAs
@@ -78,7 +90,8 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
   uint64_t* p_free = p_full + 1;
   uint64_t* o_full = p_free + 1;
   uint64_t* o_free = o_full + 1;                  // in the leader, likewise
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 1);
+  uint64_t* xy_full = o_free + 1;                 // in the leader: x and dy of both CTAs' rows are in tensor memory
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(xy_full + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(ptx::cluster_ctarank());
@@ -100,8 +113,9 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     }
     for (int i = 0; i < kRowSlots; ++i) {
       ptx::mbar_init(&r_full[i], 1);
-      ptx::mbar_init(&r_free[i], 1);
+      ptx::mbar_init(&r_free[i], kTmemRows ? kEpiWarps / 2 : 1);
     }
+    ptx::mbar_init(xy_full, 2 * kEpiWarps);
     ptx::mbar_init(s_full, 1);
     ptx::mbar_init(s_free, 2 * kEpiWarps);
     ptx::mbar_init(s_issued, 1);
@@ -119,7 +133,7 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
   __syncwarp();
   ptx::cluster_sync();
   ptx::tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot, tmem_s = tmem + C, tmem_p = tmem_s + 192;      // dX first
+  const uint32_t tmem = *tmem_slot, tmem_s = tmem + C, tmem_p = tmem_s + 192, tmem_xy = tmem_p + 64;      // dX first
   grid_dependency_enter();
 
   if (warp == 0) {
@@ -131,28 +145,33 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
       int c1 = 0, c2 = 0;
       for (int i = 0; ok && i <= total; ++i) {
         if (i < total) {
-          for (int kb = 0; kb < kK; ++kb) {
+          for (int kb = 0; kb < kK; kb += 2) {
             ok = ptx::mbar_wait(&w_free[st], ph ^ 1, 541);
             if (!ok) break;
             if (rank == 0) ptx::mbar_expect_tx(&w_full[st], 2 * kWSlot);
             const uint32_t bar = ptx::leader_addr(&w_full[st]);
-            ptx::tma_load_4d_pair(s_w + st * kWSlot, &tm_w1, bar, kb * 64, rank * p.hidden + c1 * kChunk, 0, 0);
-            ptx::tma_load_4d_pair(s_w + st * kWSlot + kW1, &tm_wo, bar, c1 * kChunk + rank * 32, kb * 64, 0, 0);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint8_t* d = s_w + st * kWSlot + q * kWBlock;
+              ptx::tma_load_4d_pair(d, &tm_w1, bar, (kb + q) * 64, rank * p.hidden + c1 * kChunk, 0, 0);
+              ptx::tma_load_4d_pair(d + kW1, &tm_wo, bar, c1 * kChunk + rank * 32, (kb + q) * 64, 0, 0);
+            }
             if (++st == kWSlots) { st = 0; ph ^= 1u; }
           }
           if (++c1 == p.chunks) c1 = 0;
         }
         if (i > 0) {
-          for (int which = 0; ok && which < 2; ++which) {
-            ok = ptx::mbar_wait(&v_free[v], v_ph ^ 1, 542);
-            if (!ok) break;
-            if (rank == 0) ptx::mbar_expect_tx(&v_full[v], 2 * kVSlot);
-            const uint32_t bar = ptx::leader_addr(&v_full[v]);
+          ok = ok && ptx::mbar_wait(&v_free[v], v_ph ^ 1, 542);
+          if (!ok) break;
+          if (rank == 0) ptx::mbar_expect_tx(&v_full[v], 2 * kVSlot);
+          const uint32_t bar = ptx::leader_addr(&v_full[v]);
+#pragma unroll
+          for (int which = 0; which < 2; ++which)
 #pragma unroll
             for (int q = 0; q < C / 128; ++q)
-              ptx::tma_load_4d_pair(s_v + v * kVSlot + q * 8192, &tm_w1, bar, rank * (C / 2) + q * 64, which * p.hidden + c2 * kChunk, 0, 0);
-            if (++v == kVSlots) { v = 0; v_ph ^= 1u; }
-          }
+              ptx::tma_load_4d_pair(s_v + v * kVSlot + which * (kVSlot / 2) + q * 8192, &tm_w1, bar, rank * (C / 2) + q * 64,
+                                    which * p.hidden + c2 * kChunk, 0, 0);
+          if (++v == kVSlots) { v = 0; v_ph ^= 1u; }
           if (++c2 == p.chunks) c2 = 0;
         }
       }
@@ -176,10 +195,16 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         for (int kb = 0; kb < kK; ++kb) {
           ok = ptx::mbar_wait(&r_free[st], ph ^ 1, 545);
           if (!ok) break;
-          if (rank == 0) ptx::mbar_expect_tx(&r_full[st], 2 * kRowSlot);
-          const uint32_t bar = ptx::leader_addr(&r_full[st]);
-          ptx::tma_load_4d_pair(s_rows + st * kRowSlot, &tm_x, bar, kb * 64, row0_of(it), 0, 0);
-          ptx::tma_load_4d_pair(s_rows + st * kRowSlot + kBox, &tm_dy, bar, kb * 64, row0_of(it), 0, 0);
+          if constexpr (kTmemRows) {
+            ptx::mbar_expect_tx(&r_full[st], kRowSlot);
+            ptx::tma_load_4d(s_rows + st * kRowSlot, &tm_x, &r_full[st], kb * 64, row0_of(it), 0, 0);
+            ptx::tma_load_4d(s_rows + st * kRowSlot + kBox, &tm_dy, &r_full[st], kb * 64, row0_of(it), 0, 0);
+          } else {
+            if (rank == 0) ptx::mbar_expect_tx(&r_full[st], 2 * kRowSlot);
+            const uint32_t bar = ptx::leader_addr(&r_full[st]);
+            ptx::tma_load_4d_pair(s_rows + st * kRowSlot, &tm_x, bar, kb * 64, row0_of(it), 0, 0);
+            ptx::tma_load_4d_pair(s_rows + st * kRowSlot + kBox, &tm_dy, bar, kb * 64, row0_of(it), 0, 0);
+          }
           if (++st == kRowSlots) { st = 0; ph ^= 1u; }
         }
         if (it + 1 < my_tiles)
@@ -199,35 +224,46 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
       constexpr uint32_t idesc_s = ptx::make_idesc(2 * kRows, 2 * kChunk, 1), idesc_g = ptx::make_idesc(2 * kRows, kChunk, 1) | (1u << 16);
       const uint64_t row_desc = ptx::make_kmajor_desc<128>(ptx::smem_u32(s_rows));
       const uint64_t w1_desc = ptx::make_kmajor_desc<128>(ptx::smem_u32(s_w)), g_desc = wo_desc(ptx::smem_u32(s_w) + kW1);
-      int st = 0, rs0 = 0, c = 0;
+      int st = 0, rs0 = 0, c = 0, it = 0;
       uint32_t ph = 0, r_ph = 0;
       bool ok = true;
       for (int i = 0; ok && i < total; ++i) {
-        ok = ptx::mbar_wait(s_free, (i & 1) ^ 1, 547);
+        ok = hot_wait(s_free, (i & 1) ^ 1, 547);
+        if (kTmemRows && c == 0) ok = ok && hot_wait(xy_full, it & 1, 557);
         if (!ok) break;
         ptx::tc_fence_after_sync();
 #pragma unroll
         for (int kb = 0; kb < kK; ++kb) {
           const int rs = rs0 + kb;                  // (kRowSlots is a multiple of kK)
-          if (c == 0) ok = ptx::mbar_wait(&r_full[rs], r_ph, 548);
-          ok = ok && ptx::mbar_wait(&w_full[st], ph, 549);
+          if (!kTmemRows && c == 0) ok = hot_wait(&r_full[rs], r_ph, 548);
+          if ((kb & 1) == 0) ok = ok && hot_wait(&w_full[st], ph, 549);
           if (!ok) break;
           ptx::tc_fence_after_sync();
-          const uint64_t xd = row_desc + rs * (kRowSlot >> 4), wd = w1_desc + st * (kWSlot >> 4), gd = g_desc + st * (kWSlot >> 4);
+          const uint32_t w_at = st * (kWSlot >> 4) + (kb & 1) * (kWBlock >> 4);
+          const uint64_t xd = row_desc + rs * (kRowSlot >> 4), wd = w1_desc + w_at, gd = g_desc + w_at;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) ptx::mma_f16_ss_pair(tmem_s, xd + k * 2, wd + k * 2, idesc_s, kb > 0 || k > 0 ? 1u : 0u);
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (kTmemRows) ptx::mma_f16_ts_pair(tmem_s, tmem_xy + kb * 32 + k * 8, wd + k * 2, idesc_s, kb > 0 || k > 0 ? 1u : 0u);
+            else ptx::mma_f16_ss_pair(tmem_s, xd + k * 2, wd + k * 2, idesc_s, kb > 0 || k > 0 ? 1u : 0u);
+          }
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            ptx::mma_f16_ss_pair(tmem_s + 128, xd + (kBox >> 4) + k * 2, gd + k * (1024 >> 4), idesc_g, kb > 0 || k > 0 ? 1u : 0u);
-          ptx::tc_commit_pair(&w_free[st]);
-          if (c == p.chunks - 1) ptx::tc_commit_pair(&r_free[rs]);
-          if (++st == kWSlots) { st = 0; ph ^= 1u; }
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (kTmemRows)
+              ptx::mma_f16_ts_pair(tmem_s + 128, tmem_xy + 64 + kb * 32 + k * 8, gd + k * (1024 >> 4), idesc_g, kb > 0 || k > 0 ? 1u : 0u);
+            else ptx::mma_f16_ss_pair(tmem_s + 128, xd + (kBox >> 4) + k * 2, gd + k * (1024 >> 4), idesc_g, kb > 0 || k > 0 ? 1u : 0u);
+          }
+          if (!kTmemRows && c == p.chunks - 1) ptx::tc_commit_pair(&r_free[rs]);
+          if (kb & 1) {
+            ptx::tc_commit_pair(&w_free[st]);
+            if (++st == kWSlots) { st = 0; ph ^= 1u; }
+          }
         }
         if (!ok) break;
         ptx::tc_commit_pair(s_full);
         ptx::mbar_arrive(s_issued);
         if (++c == p.chunks) {
           c = 0;
+          ++it;
           rs0 += kK;
           if (rs0 == kRowSlots) { rs0 = 0; r_ph ^= 1u; }
         }
@@ -242,22 +278,20 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
       uint32_t v_ph = 0;
       bool ok = true;
       for (int i = 0; ok && i < total; ++i) {
-        if (c == 0) ok = ptx::mbar_wait(o_free, (it & 1) ^ 1, 550);
+        if (c == 0) ok = hot_wait(o_free, (it & 1) ^ 1, 550);
         // (behind the next chunk's S, not before or within it: the tensor core then has dX to do while that S is read)
-        if (i + 1 < total) ok = ok && ptx::mbar_wait(s_issued, (i + 1) & 1, 556);
-        ok = ok && ptx::mbar_wait(p_full, i & 1, 551);
-        for (int which = 0; ok && which < 2; ++which) {
-          ok = ptx::mbar_wait(&v_full[v], v_ph, 552);
-          if (!ok) break;
-          ptx::tc_fence_after_sync();
-          const uint64_t vd = vd0 + v * (kVSlot >> 4);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            ptx::mma_f16_ts_pair(tmem, tmem_p + which * 8 + k * 16, vd + k * (2048 >> 4), idesc, c > 0 || which > 0 || k > 0 ? 1u : 0u);
-          ptx::tc_commit_pair(&v_free[v]);
-          if (++v == kVSlots) { v = 0; v_ph ^= 1u; }
-        }
+        if (i + 1 < total) ok = ok && hot_wait(s_issued, (i + 1) & 1, 556);
+        ok = ok && hot_wait(p_full, i & 1, 551);
+        ok = ok && hot_wait(&v_full[v], v_ph, 552);
         if (!ok) break;
+        ptx::tc_fence_after_sync();
+        const uint64_t vd = vd0 + v * (kVSlot >> 4);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          ptx::mma_f16_ts_pair(tmem, tmem_p + (k >> 2) * 8 + (k & 3) * 16, vd + (k >> 2) * (kVSlot >> 5) + (k & 3) * (2048 >> 4), idesc,
+                               c > 0 || k > 0 ? 1u : 0u);
+        ptx::tc_commit_pair(&v_free[v]);
+        if (++v == kVSlots) { v = 0; v_ph ^= 1u; }
         ptx::tc_commit_pair(p_free);
         if (++c == p.chunks) {
           ptx::tc_commit_pair(o_full);
@@ -317,6 +351,32 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
       ptx::tmem_ld_wait();
       send(&tm_dab, w, col, row);
     };
+    // a tile's x and dy into tensor memory: a block of 64 channels of one of them a warp
+    auto take = [&](int it) {
+      const int slot = (2 * it + (part & 1)) & 3;
+      ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(&r_full[slot], (it >> 1) & 1, 558)) != 0;
+      const int r = quad * 32 + lane;
+      const uint8_t* src = s_rows + slot * kRowSlot + (part >> 1) * kBox + r * 128;
+      uint32_t w[2][16];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint4 v = *reinterpret_cast<const uint4*>(src + ((j ^ (r & 7)) << 4));
+        w[j >> 2][4 * (j & 3)] = v.x;
+        w[j >> 2][4 * (j & 3) + 1] = v.y;
+        w[j >> 2][4 * (j & 3) + 2] = v.z;
+        w[j >> 2][4 * (j & 3) + 3] = v.w;
+      }
+      ptx::tmem_st_32x32b_x16(tmem_xy + t_quad + (part >> 1) * 64 + (part & 1) * 32, w[0]);
+      ptx::tmem_st_32x32b_x16(tmem_xy + t_quad + (part >> 1) * 64 + (part & 1) * 32 + 16, w[1]);
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        ptx::mbar_arrive(&r_free[slot]);
+        ptx::mbar_arrive_cluster(ptx::leader_addr(xy_full));
+      }
+    };
+    if constexpr (kTmemRows) take(0);
     int c = 0, it = 0, last_col = 0, last_row = 0;
     for (int i = 0; i < total; ++i) {
       ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(s_full, i & 1, 554)) != 0;
@@ -329,6 +389,8 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
       ptx::tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive_cluster(ptx::leader_addr(s_free));
+      // (the tile's last S is complete: the next tile's rows may take its operands' place)
+      if (kTmemRows && c == p.chunks - 1 && it + 1 < my_tiles) take(it + 1);
       uint32_t hw[8], aw[8], bw[8];
       auto pairs = [&](int j0) {
 #pragma unroll

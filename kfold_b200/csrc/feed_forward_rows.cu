@@ -85,8 +85,8 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
   uint64_t* r_free = r_full + kRowSlots;
   uint64_t* s_full = r_free + kRowSlots;
   uint64_t* s_free = s_full + 1;                  // in the leader: the element-wise warps of both CTAs
-  uint64_t* s_issued = s_free + 1;                // in the leader: dX of the chunk before may follow
-  uint64_t* p_full = s_issued + 1;                // in the leader: the element-wise warps of both CTAs
+  uint64_t* s_issued = s_free + 1;                // [2] in the leader: dX of the chunk before may follow (S may be two chunks ahead of it)
+  uint64_t* p_full = s_issued + 2;                // in the leader: the element-wise warps of both CTAs
   uint64_t* p_free = p_full + 1;
   uint64_t* o_full = p_free + 1;
   uint64_t* o_free = o_full + 1;                  // in the leader, likewise
@@ -118,7 +118,8 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     ptx::mbar_init(xy_full, 2 * kEpiWarps);
     ptx::mbar_init(s_full, 1);
     ptx::mbar_init(s_free, 2 * kEpiWarps);
-    ptx::mbar_init(s_issued, 1);
+    ptx::mbar_init(&s_issued[0], 1);
+    ptx::mbar_init(&s_issued[1], 1);
     ptx::mbar_init(p_full, 2 * kEpiWarps);
     ptx::mbar_init(p_free, 1);
     ptx::mbar_init(o_full, 1);
@@ -260,7 +261,7 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         }
         if (!ok) break;
         ptx::tc_commit_pair(s_full);
-        ptx::mbar_arrive(s_issued);
+        ptx::mbar_arrive(&s_issued[i & 1]);
         if (++c == p.chunks) {
           c = 0;
           ++it;
@@ -280,7 +281,7 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
       for (int i = 0; ok && i < total; ++i) {
         if (c == 0) ok = hot_wait(o_free, (it & 1) ^ 1, 550);
         // (behind the next chunk's S, not before or within it: the tensor core then has dX to do while that S is read)
-        if (i + 1 < total) ok = ok && hot_wait(s_issued, (i + 1) & 1, 556);
+        if (i + 1 < total) ok = ok && hot_wait(&s_issued[(i + 1) & 1], ((i + 1) >> 1) & 1, 556);
         ok = ok && hot_wait(p_full, i & 1, 551);
         ok = ok && hot_wait(&v_full[v], v_ph, 552);
         if (!ok) break;

@@ -136,6 +136,13 @@ def _same_device(name: str, x: torch.Tensor, *ts: torch.Tensor | None) -> None:
             raise ValueError(f"{name}: tensors on {x.device} and {t.device}")
 
 
+def _call_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+    """Scratch for a training call.  One that is being captured gets memory of its graph's own: two graphs may then be replayed at once."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return _workspace(device, nbytes, MOST_KEPT_BYTES)
+
+
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-5, need_weight: bool = True,
                         need_bias: bool = True):
     """Gradient of ``layer_norm(x, weight, bias, eps)``: (dx, dweight, dbias) from dy, of y's shape, bfloat16 or float32.
@@ -154,7 +161,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
     db = torch.empty(c, dtype=torch.float32, device=x.device) if need_bias else None
     lib = L.lib()
     with L.on_device(x.device):
-        ws = _workspace(x.device, lib.kfb_layernorm_bwd_workspace_bytes(c)) if need_weight or need_bias else None
+        ws = _call_workspace(x.device, lib.kfb_layernorm_bwd_workspace_bytes(c)) if need_weight or need_bias else None
         L.check(lib.kfb_layernorm_bwd(L.ptr(dc), L.ptr(xc), L.ptr(w), L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), 0 if ws is None else ws.numel(),
                                       x.numel() // c if c else 0, c, eps, L.dtype_code(dy.dtype), L.dtype_code(x.dtype), L.stream_ptr()))
     return dx, dw, db
@@ -195,7 +202,7 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor)
     out = _dense_like(x)
     lib = L.lib()
     with L.on_device(x.device):
-        ws = _workspace(x.device, lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, code, 0), MOST_KEPT_BYTES)
+        ws = _call_workspace(x.device, lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, code, 0))
         L.check(lib.kfb_feed_forward_fwd(L.ptr(xc), L.ptr(wi), L.ptr(wo), L.ptr(out), L.ptr(ws), ws.numel(), rows, c, hidden, code, L.stream_ptr()))
     return out
 
@@ -210,7 +217,7 @@ def gated_feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.T
     dwo = _dense_like(w_out) if need_w_out else None
     lib = L.lib()
     with L.on_device(x.device):
-        ws = _workspace(x.device, lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, code, 1), MOST_KEPT_BYTES)
+        ws = _call_workspace(x.device, lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, code, 1))
         L.check(lib.kfb_feed_forward_bwd(L.ptr(dc), L.ptr(xc), L.ptr(wi), L.ptr(wo), L.ptr(dx), L.ptr(dwi), L.ptr(dwo), L.ptr(ws), ws.numel(), rows, c,
                                          hidden, code, L.dtype_code(w_in.dtype), L.stream_ptr()))
     return dx, dwi, dwo

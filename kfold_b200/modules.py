@@ -14,7 +14,8 @@ modules they stand in for, with the CUDA kernels behind them:
 
 Conventions copied from the reference's Triton backend
 (model/primitives/triangle_multiplication.py:94-145): inference only (``RuntimeError``
-when autograd is recording or the input is not on a CUDA device), compute dtype =
+when autograd is recording or the input is not on a CUDA device; LayerNorm, Transition and
+Dropout are trained too and record their gradients), compute dtype =
 autocast dtype if autocast is on else the input dtype, result returned in the input
 dtype, weights packed once per module and re-packed when a parameter's storage or
 version changes.
@@ -24,13 +25,14 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from . import autograd as A
 from . import functional as F
 from . import _lib as L
 from . import packing
 from .plans import NativeCall, ParamState, StandsFor, Unshared, handed_out
 
 __all__ = [
-    "LayerNorm", "LinearNoBias", "Linear",
+    "LayerNorm", "LinearNoBias", "Linear", "Dropout",
     "TriangleMultiplicationOutgoing", "TriangleMultiplicationIncoming",
     "TriangleAttentionStartingNode", "TriangleAttentionEndingNode",
     "Transition", "AdaLN", "SelfAttentionPairBias", "ConditionedTransitionBlock", "CachedGlobalTransformerBlock",
@@ -42,7 +44,7 @@ __all__ = [
 # parameter holders (names match the reference so that state dicts are interchangeable)
 # --------------------------------------------------------------------------------------------
 class LayerNorm(nn.Module):
-    """LayerNorm with fp32 statistics (model/primitives/normalization.py:24-91)."""
+    """LayerNorm with fp32 statistics (model/primitives/normalization.py:24-91); differentiable."""
 
     def __init__(self, normalized_shape: int, create_scale: bool = True, create_offset: bool = True, eps: float = 1e-5):
         super().__init__()
@@ -53,6 +55,8 @@ class LayerNorm(nn.Module):
 
     @torch.compiler.disable
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if torch.is_grad_enabled():
+            return A.layer_norm(x, self.weight, self.bias, self.eps)
         _check_inference(x)
         return F.layer_norm(x, self.weight, self.bias, self.eps)
 
@@ -72,6 +76,34 @@ class Linear(nn.Module):
 class LinearNoBias(Linear):
     def __init__(self, in_features: int, out_features: int):
         super().__init__(in_features, out_features, bias=False)
+
+
+class Dropout(nn.Module):
+    """Dropout whose mask is never stored, along with the residual sum: ``x -> (residual +) dropout(x)``; in evaluation (residual +) x.
+
+    ``shared_dim``: the mask has extent one along this dim of x (row-wise -3 and column-wise -2 dropout of a pair tensor).  Each call draws a
+    seed from torch's default CPU generator, so ``torch.manual_seed`` and activation checkpointing reproduce it.  In a CUDA graph pass
+    ``rng``, an int64 CUDA tensor (seed, offset) that is moved on between replays (``rng[1] += 1``)."""
+
+    def __init__(self, p: float, shared_dim: int | None = None):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"Dropout: p = {p}")
+        self.p, self.shared_dim = p, shared_dim
+
+    def extra_repr(self) -> str:
+        return f"p={self.p}" + ("" if self.shared_dim is None else f", shared_dim={self.shared_dim}")
+
+    @torch.compiler.disable
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, rng: torch.Tensor | None = None) -> torch.Tensor:
+        p = self.p if self.training else 0.0
+        if p == 0.0 and residual is None:
+            return x
+        if rng is None:
+            if p and x.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("Dropout: a captured call needs `rng`, or every replay would draw the same mask")
+            rng = (int(torch.randint(0, 2 ** 63 - 1, ())), 0) if p else (0, 0)
+        return (A if torch.is_grad_enabled() else F).dropout(x, p, rng, shared_dim=self.shared_dim, residual=residual)
 
 
 class _SwiGLU(nn.Module):
@@ -228,13 +260,26 @@ class Transition(_PackedMixin, nn.Module):
 
     @torch.compiler.disable
     def forward(self, x: torch.Tensor, residual: bool = False) -> torch.Tensor:
-        _check_inference(x)
         cd = compute_dtype(x)
         precise = _is_precise(cd, "Transition")
+        if torch.is_grad_enabled():
+            return self._training(x, cd, residual)
+        _check_inference(x)
         pk = self._packed(x.device, cd, lambda sd, dev: packing.pack_transition(sd, dev, precise=precise))
         with torch.autocast(x.device.type, enabled=False):
             out = F.transition(x.float() if precise else x, pk, eps=self.layernorm.eps, residual=residual)
         return out.to(x.dtype)
+
+    def _training(self, x: torch.Tensor, cd: torch.dtype, residual: bool) -> torch.Tensor:
+        """While autograd records: the parameters as they are, gradients for all of them and x."""
+        if not x.is_cuda:
+            raise RuntimeError("The kfold_b200 kernel backend requires CUDA tensors.")
+        with torch.autocast(x.device.type, enabled=False):
+            xn = A.layer_norm(x, self.layernorm.weight, self.layernorm.bias, self.layernorm.eps, out_dtype=cd)
+            y = A.gated_feed_forward(xn, self.swiglu.linear.weight, self.linear_out.weight)
+            if not residual:
+                return y.to(x.dtype)
+            return A.dropout(y if x.dtype == torch.float32 else y.to(x.dtype), 0.0, (0, 0), residual=x)
 
 
 class AdaLN(_PackedMixin, nn.Module):

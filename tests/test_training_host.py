@@ -84,3 +84,20 @@ def test_feed_forward_refuses_cpu_tensors():
     for call in (lambda: F.gated_feed_forward(x, wi, wo), lambda: F.gated_feed_forward_backward(x, x, wi, wo)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_modules_refuse_cpu_tensors_while_recording():
+    from kfold_b200 import modules as M
+    x = torch.zeros(3, 64)
+    for call in (lambda: M.LayerNorm(64)(x), lambda: M.Transition(64, 2)(x), lambda: M.Dropout(0.5)(x)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+    with pytest.raises(ValueError):
+        M.Dropout(1.5)
+    assert M.Dropout(0.5).eval()(x) is x and M.Dropout(0.0)(x) is x
+
+
+def test_transition_keeps_its_parameters_names():
+    from kfold_b200 import modules as M
+    assert sorted(M.Transition(64, 2).state_dict()) == ["layernorm.bias", "layernorm.weight", "linear_out.weight", "swiglu.linear.weight"]
+    assert not M.Dropout(0.1).state_dict()

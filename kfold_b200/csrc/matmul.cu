@@ -1,6 +1,6 @@
 // D[m][n] = sum_k A(m, k) B(n, k) for operands stored along k or across it (see matmul.cuh).
 //
-// A CTA computes one 128 x 128 tile of one piece of k: a thread fetches 64-wide blocks of both operands with TMA into a ring, a thread issues
+// A CTA computes one 128 x 128 tile of one piece of k of one of up to three products: a thread fetches 64-wide blocks of both operands with TMA into a ring, a thread issues
 // the products, four warps bring the accumulator from tensor memory to global memory.  Two CTAs share an SM, so that one's start and end lie
 // under the other's products.  An operand stored across k ([k][i]) is fetched as two boxes of 64 k by 64 i and read MN-major as it lies: the
 // gradients of weights contract over rows, and nothing is transposed for them.
@@ -21,11 +21,17 @@ constexpr int kStage = 2 * kOperand;
 constexpr int kThreads = 192;                      // TMA, products, four warps of rows
 
 struct MmParams {
-  int m, n, m_tiles, n_tiles;
+  int m, n, m_tiles, n_tiles, splits;
   int blocks, per_split;                           // of 64 along k: all, of a piece
+  int a_by_k, b_by_k;
   EpiSeg out;
   long long plane_d;
   int accumulate;
+};
+struct MmBatch {
+  CUtensorMap a[kMostMatmuls], b[kMostMatmuls];
+  MmParams p[kMostMatmuls];
+  int end[kMostMatmuls];                           // blocks of the grid up to and with each product
 };
 
 template <int PARTS>
@@ -39,9 +45,8 @@ __device__ __forceinline__ uint64_t by_k_desc(uint32_t addr) {
          (1ull << 46) | (2ull << 61);
 }
 
-template <bool A_BY_K, bool B_BY_K, int PARTS>
-__global__ void __launch_bounds__(kThreads, PARTS == 3 ? 1 : 2)
-matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const MmParams p) {
+template <int PARTS>
+__global__ void __launch_bounds__(kThreads, PARTS == 3 ? 1 : 2) matmul_kernel(const __grid_constant__ MmBatch batch) {
   constexpr int kStages = stages<PARTS>();
   constexpr uint32_t kCols = PARTS == 3 ? 256 : 128;
   extern __shared__ uint8_t smem_raw[];
@@ -52,7 +57,16 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m_tile = blockIdx.x % p.m_tiles, n_tile = blockIdx.x / p.m_tiles, split = blockIdx.y;
+  int which = 0, block = blockIdx.x;
+#pragma unroll
+  for (int i = 0; i + 1 < kMostMatmuls; ++i)
+    if (static_cast<int>(blockIdx.x) >= batch.end[i]) {
+      which = i + 1;
+      block = blockIdx.x - batch.end[i];
+    }
+  const MmParams& p = batch.p[which];
+  const CUtensorMap &tm_a = batch.a[which], &tm_b = batch.b[which];
+  const int m_tile = block % p.m_tiles, n_tile = block / p.m_tiles % p.n_tiles, split = block / (p.m_tiles * p.n_tiles);
   const int first = split * p.per_split, last = min(first + p.per_split, p.blocks);
   if (threadIdx.x == 0) {
     ptx::prefetch_tmap(&tm_a);
@@ -85,13 +99,13 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           if (!ok) break;
           ptx::mbar_expect_tx(&full[st], kStage);
           uint8_t *a = ring + st * kStage, *b = a + kOperand;
-          if (A_BY_K) {
+          if (p.a_by_k) {
             ptx::tma_load_3d(a, &tm_a, &full[st], m_tile * kTile, kb * kK, part);
             ptx::tma_load_3d(a + kOperand / 2, &tm_a, &full[st], m_tile * kTile + 64, kb * kK, part);
           } else {
             ptx::tma_load_3d(a, &tm_a, &full[st], kb * kK, m_tile * kTile, part);
           }
-          if (B_BY_K) {
+          if (p.b_by_k) {
             ptx::tma_load_3d(b, &tm_b, &full[st], n_tile * kTile, kb * kK, part);
             ptx::tma_load_3d(b + kOperand / 2, &tm_b, &full[st], n_tile * kTile + 64, kb * kK, part);
           } else {
@@ -102,8 +116,8 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     }
   } else if (warp == 1) {
     if (ptx::elect_one()) {
-      constexpr uint32_t idesc = ptx::make_idesc(kTile, kTile, 1) | (A_BY_K ? 1u << 15 : 0u) | (B_BY_K ? 1u << 16 : 0u);
-      constexpr uint32_t a_step = A_BY_K ? 2048 >> 4 : 2, b_step = B_BY_K ? 2048 >> 4 : 2;     // of 16 k
+      const uint32_t idesc = ptx::make_idesc(kTile, kTile, 1) | (p.a_by_k ? 1u << 15 : 0u) | (p.b_by_k ? 1u << 16 : 0u);
+      const uint32_t a_step = p.a_by_k ? 2048 >> 4 : 2, b_step = p.b_by_k ? 2048 >> 4 : 2;     // of 16 k
       int st = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -120,8 +134,8 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           if (!ok) break;
           ptx::tc_fence_after_sync();
           const uint32_t at = ptx::smem_u32(ring + st * kStage);
-          ad[i] = A_BY_K ? by_k_desc(at) : ptx::make_kmajor_desc<128>(at);
-          bd[i] = B_BY_K ? by_k_desc(at + kOperand) : ptx::make_kmajor_desc<128>(at + kOperand);
+          ad[i] = p.a_by_k ? by_k_desc(at) : ptx::make_kmajor_desc<128>(at);
+          bd[i] = p.b_by_k ? by_k_desc(at + kOperand) : ptx::make_kmajor_desc<128>(at + kOperand);
           used[i] = st;
           if (++st == kStages) { st = 0; ph ^= 1u; }
           if (i == 0) {
@@ -197,39 +211,34 @@ int operand_map(CUtensorMap* map, const MatOperand& o, int extent, long long k, 
   return make_tmap(map, o.ptr, 2, 3, dims, str, box, 128);
 }
 
-template <bool A_BY_K, bool B_BY_K, int PARTS>
-int launch(cudaStream_t stream, const MatmulArgs& a, const MmParams& p) {
-  CUtensorMap ta, tb;
-  KFB_TRY(operand_map(&ta, a.a, a.m, a.k, PARTS));
-  KFB_TRY(operand_map(&tb, a.b, a.n, a.k, PARTS));
-  constexpr auto kernel = matmul_kernel<A_BY_K, B_BY_K, PARTS>;
-  KFB_TRY(allow_smem<kernel>(smem_bytes<PARTS>()));
-  LaunchScope scope(stream, a.tag);
-  return launch_kernel(stream, kernel, dim3(p.m_tiles * p.n_tiles, a.splits), kThreads, smem_bytes<PARTS>(), ta, tb, p);
-}
-template <int PARTS>
-int launch_majors(cudaStream_t stream, const MatmulArgs& a, const MmParams& p) {
-  if (a.a.by_k) return a.b.by_k ? launch<true, true, PARTS>(stream, a, p) : launch<true, false, PARTS>(stream, a, p);
-  return a.b.by_k ? launch<false, true, PARTS>(stream, a, p) : launch<false, false, PARTS>(stream, a, p);
-}
-
-// out[i .. i + 3] of the planes' sums
-template <typename TO>
-__global__ void __launch_bounds__(256) sum_planes_kernel(const float* planes, long long plane, int splits, TO* out, long long n) {
+struct SumBatch {
+  PlaneSum s[kMostMatmuls];
+  unsigned end[kMostMatmuls];                      // blocks of the grid up to and with each sum
+};
+__global__ void __launch_bounds__(256) sum_planes_kernel(const SumBatch batch) {
   grid_dependency_enter();
-  const long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 4;
-  if (i >= n) return;
+  int which = 0;
+  unsigned block = blockIdx.x;
+#pragma unroll
+  for (int i = 0; i + 1 < kMostMatmuls; ++i)
+    if (blockIdx.x >= batch.end[i]) {
+      which = i + 1;
+      block = blockIdx.x - batch.end[i];
+    }
+  const PlaneSum& q = batch.s[which];
+  const long long i = (static_cast<long long>(block) * 256 + threadIdx.x) * 4;
+  if (i >= q.n) return;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-  for (int k = 0; k < splits; ++k) {
-    const float4 t = *reinterpret_cast<const float4*>(planes + k * plane + i);
+  for (int k = 0; k < q.splits; ++k) {
+    const float4 t = *reinterpret_cast<const float4*>(q.planes + k * q.plane + i);
     s.x += t.x;
     s.y += t.y;
     s.z += t.z;
     s.w += t.w;
   }
-  if constexpr (sizeof(TO) == 2) *reinterpret_cast<uint2*>(out + i) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
-  else *reinterpret_cast<float4*>(out + i) = s;
+  if (q.out_fp32) *reinterpret_cast<float4*>(static_cast<float*>(q.out) + i) = s;
+  else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(q.out) + i) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
 }
 
 __global__ void __launch_bounds__(256) split_planes_kernel(const float* x, __nv_bfloat16* parts, long long plane, long long n) {
@@ -250,37 +259,69 @@ __global__ void __launch_bounds__(256) split_planes_kernel(const float* x, __nv_
 int matmul_splits(int m, int n, long long k, int most) {
   const long long tiles = static_cast<long long>(cdiv(m, kTile)) * cdiv(n, kTile), blocks = (k + kK - 1) / kK;
   long long want = 2ll * sm_count() / tiles;
+  // (a piece of less than six blocks is start and end only: 331 rows of 384 channels and 1 536 hidden ones are fastest in one piece)
+  if (want > blocks / 6) want = blocks / 6;
   if (want > most) want = most;
-  if (want > blocks) want = blocks;
   if (want < 1) want = 1;
   const long long per = (blocks + want - 1) / want;
   return static_cast<int>((blocks + per - 1) / per);
 }
 
-int launch_matmul(cudaStream_t stream, const MatmulArgs& a) {
-  KFB_CHECK_ARG(a.m > 0 && a.n > 0 && a.k > 0 && a.k < (1ll << 31) && a.splits >= 1, "matmul: m %d n %d k %lld, %d pieces", a.m, a.n, a.k, a.splits);
-  KFB_CHECK_ARG(a.out_fp32 || (a.splits == 1 && !a.accumulate), "matmul: pieces and sums need an fp32 result");
-  MmParams p = {};
-  p.m = a.m;
-  p.n = a.n;
-  p.m_tiles = cdiv(a.m, kTile);
-  p.n_tiles = cdiv(a.n, kTile);
-  p.blocks = static_cast<int>((a.k + kK - 1) / kK);
-  p.per_split = cdiv(p.blocks, a.splits);
-  KFB_CHECK_ARG(cdiv(p.blocks, p.per_split) == a.splits, "matmul: an empty piece of k (%d blocks in %d)", p.blocks, a.splits);
-  p.out = row_major_seg(a.d, a.n, a.ld_d, 0, 0, a.out_fp32);
-  if (a.splits > 1 && a.plane_d % 4 != 0) p.out.vec = 0;
-  p.plane_d = a.plane_d;
-  p.accumulate = a.accumulate;
-  return a.precise ? launch_majors<3>(stream, a, p) : launch_majors<1>(stream, a, p);
+int launch_matmuls(cudaStream_t stream, const MatmulArgs* list, int count, const char* tag) {
+  KFB_CHECK_ARG(count >= 1 && count <= kMostMatmuls, "matmul: %d products", count);
+  MmBatch batch = {};
+  int blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    const MatmulArgs& a = list[i];
+    KFB_CHECK_ARG(a.m > 0 && a.n > 0 && a.k > 0 && a.k < (1ll << 31) && a.splits >= 1, "matmul: m %d n %d k %lld, %d pieces", a.m, a.n, a.k, a.splits);
+    KFB_CHECK_ARG(a.out_fp32 || (a.splits == 1 && !a.accumulate), "matmul: pieces and sums need an fp32 result");
+    KFB_CHECK_ARG(a.precise == list[0].precise, "matmul: products of both modes in one launch");
+    MmParams& p = batch.p[i];
+    p.m = a.m;
+    p.n = a.n;
+    p.m_tiles = cdiv(a.m, kTile);
+    p.n_tiles = cdiv(a.n, kTile);
+    p.splits = a.splits;
+    p.blocks = static_cast<int>((a.k + kK - 1) / kK);
+    p.per_split = cdiv(p.blocks, a.splits);
+    KFB_CHECK_ARG(cdiv(p.blocks, p.per_split) == a.splits, "matmul: an empty piece of k (%d blocks in %d)", p.blocks, a.splits);
+    p.a_by_k = a.a.by_k;
+    p.b_by_k = a.b.by_k;
+    p.out = row_major_seg(a.d, a.n, a.ld_d, 0, 0, a.out_fp32);
+    if (a.splits > 1 && a.plane_d % 4 != 0) p.out.vec = 0;
+    p.plane_d = a.plane_d;
+    p.accumulate = a.accumulate;
+    KFB_TRY(operand_map(&batch.a[i], a.a, a.m, a.k, a.precise ? 3 : 1));
+    KFB_TRY(operand_map(&batch.b[i], a.b, a.n, a.k, a.precise ? 3 : 1));
+    const long long add = static_cast<long long>(p.m_tiles) * p.n_tiles * p.splits;
+    KFB_CHECK_ARG(add + blocks < (1ll << 31), "matmul: %lld tiles", add);
+    blocks += static_cast<int>(add);
+    batch.end[i] = blocks;
+  }
+  for (int i = count; i < kMostMatmuls; ++i) batch.end[i] = blocks;
+  LaunchScope scope(stream, tag);
+  if (list[0].precise) {
+    KFB_TRY(allow_smem<matmul_kernel<3>>(smem_bytes<3>()));
+    return launch_kernel(stream, matmul_kernel<3>, blocks, kThreads, smem_bytes<3>(), batch);
+  }
+  KFB_TRY(allow_smem<matmul_kernel<1>>(smem_bytes<1>()));
+  return launch_kernel(stream, matmul_kernel<1>, blocks, kThreads, smem_bytes<1>(), batch);
 }
 
-int launch_sum_planes(cudaStream_t stream, const float* planes, long long plane, int splits, void* out, int out_fp32, long long n) {
-  KFB_CHECK_ARG(n % 4 == 0 && plane % 4 == 0, "sum_planes: %lld elements, planes %lld apart (multiples of 4)", n, plane);
-  const unsigned blocks = static_cast<unsigned>((n / 4 + 255) / 256);
+int launch_sum_planes(cudaStream_t stream, const PlaneSum* list, int count) {
+  KFB_CHECK_ARG(count >= 1 && count <= kMostMatmuls, "sum_planes: %d sums", count);
+  SumBatch batch = {};
+  unsigned blocks = 0;
+  for (int i = 0; i < kMostMatmuls; ++i) {
+    if (i < count) {
+      KFB_CHECK_ARG(list[i].n % 4 == 0 && list[i].plane % 4 == 0, "sum_planes: %lld elements, planes %lld apart (multiples of 4)", list[i].n, list[i].plane);
+      batch.s[i] = list[i];
+      blocks += static_cast<unsigned>((list[i].n / 4 + 255) / 256);
+    }
+    batch.end[i] = blocks;
+  }
   LaunchScope scope(stream, "sum_planes");
-  if (out_fp32) return launch_kernel(stream, sum_planes_kernel<float>, blocks, 256, 0, planes, plane, splits, static_cast<float*>(out), n);
-  return launch_kernel(stream, sum_planes_kernel<__nv_bfloat16>, blocks, 256, 0, planes, plane, splits, static_cast<__nv_bfloat16*>(out), n);
+  return launch_kernel(stream, sum_planes_kernel, blocks, 256, 0, batch);
 }
 
 int launch_split_planes(cudaStream_t stream, const float* x, __nv_bfloat16* parts, long long plane, long long n) {

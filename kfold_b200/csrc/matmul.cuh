@@ -28,15 +28,25 @@ struct MatmulArgs {
   long long plane_d;
   int accumulate;        // fp32 D only: add to what D holds
   int precise;           // operands are three bf16 parts each
-  const char* tag;
 };
-int launch_matmul(cudaStream_t stream, const MatmulArgs& p);
+static constexpr int kMostMatmuls = 3;
+// Up to kMostMatmuls products in one launch, all of them precise or none.
+int launch_matmuls(cudaStream_t stream, const MatmulArgs* list, int count, const char* tag);
+inline int launch_matmul(cudaStream_t stream, const MatmulArgs& p, const char* tag) { return launch_matmuls(stream, &p, 1, tag); }
 
 // How many pieces (at most `most`) k is best cut into so that the tiles of an m x n product fill the device, none of them empty.
 int matmul_splits(int m, int n, long long k, int most);
 
-// out[i] = sum over s of planes[s * plane + i], i < n, in the order of s; bf16 or fp32.
-int launch_sum_planes(cudaStream_t stream, const float* planes, long long plane, int splits, void* out, int out_fp32, long long n);
+// out[i] = sum over s of planes[s * plane + i], i < n, in the order of s; bf16 or fp32.  Up to kMostMatmuls of them in one launch.
+struct PlaneSum {
+  const float* planes;
+  long long plane;
+  int splits;
+  void* out;
+  int out_fp32;
+  long long n;           // a multiple of 4, as plane is
+};
+int launch_sum_planes(cudaStream_t stream, const PlaneSum* list, int count);
 
 // Three bf16 parts of n floats (a multiple of 4): parts[q * plane + i], x = x0 + x1 + x2.
 int launch_split_planes(cudaStream_t stream, const float* x, __nv_bfloat16* parts, long long plane, long long n);

@@ -72,7 +72,7 @@ struct FfnWs {
   __nv_bfloat16 *x3, *dy3, *wi3, *wo3;      // fp32-accurate mode: the operands' parts
   float *u, *dh;                            // where no kernel keeps them in tensor memory
   __nv_bfloat16 *h, *dab, *wi_t;
-  float *pl_in, *pl_out;
+  float *pl_in, *pl_out, *pl_dx;
 };
 // Whether h, da and db come from the one kernel (feed_forward_hidden.cu).
 bool one_kernel(int c, int hidden, int precise) { return !precise && ffn_hidden_ok(c, hidden); }
@@ -85,6 +85,11 @@ int planes_in(long long piece, int c, int hidden, int precise) {
 }
 int planes_out(long long piece, int c, int hidden, int precise) {
   return sums_kernel(c, hidden, precise) ? ffn_sums_planes(piece, hidden) : matmul_splits(c, hidden, piece, kMostPlanes);
+}
+
+// Pieces of the hidden channels of dx = [da, db] [Wa; Wb] where the rows come in one piece and their tiles do not fill the device (1 elsewhere).
+int planes_dx(long long rows, long long piece, int c, int hidden) {
+  return rows > piece ? 1 : matmul_splits(static_cast<int>(rows), c, 2ll * hidden, 16);
 }
 
 size_t carve(FfnWs& w, void* base, long long rows, int c, int hidden, int precise, int backward) {
@@ -113,6 +118,8 @@ size_t carve(FfnWs& w, void* base, long long rows, int c, int hidden, int precis
     w.dab = cv.take<__nv_bfloat16>(parts * r * 2 * hh);
     w.pl_in = cv.take<float>(planes_in(piece, c, hidden, precise) * 2 * hh * cc);
     w.pl_out = cv.take<float>(planes_out(piece, c, hidden, precise) * hh * cc);
+    const int dx_planes = planes_dx(rows, piece, c, hidden);
+    if (dx_planes > 1) w.pl_dx = cv.take<float>(dx_planes * r * cc);
   }
   return cv.off;
 }
@@ -217,12 +224,12 @@ KFB_API int kfb_feed_forward_fwd(const void* x, const void* w_in, const void* w_
       KFB_TRY(launch_split_planes(s, static_cast<const float*>(xr), w.x3, r * c, r * c));
       xr = w.x3;
     }
-    MatmulArgs in = {{xr, c, 0, r * c}, {wi, c, 0, wi_n}, m, 2 * hidden, c, w.u, 2ll * hidden, 1, 1, 0, 0, precise, "feed_forward_in"};
-    KFB_TRY(launch_matmul(s, in));
+    MatmulArgs in = {{xr, c, 0, r * c}, {wi, c, 0, wi_n}, m, 2 * hidden, c, w.u, 2ll * hidden, 1, 1, 0, 0, precise};
+    KFB_TRY(launch_matmul(s, in, "feed_forward_in"));
     KFB_TRY(launch_hidden(s, w, false, r, hidden, precise));
     MatmulArgs out_p = {{w.h, hidden, 0, r * hidden}, {wo, hidden, 0, wo_n}, m, c, hidden, static_cast<char*>(out) + r0 * c * size, c, precise, 1, 0, 0,
-                        precise, "feed_forward_out"};
-    KFB_TRY(launch_matmul(s, out_p));
+                        precise};
+    KFB_TRY(launch_matmul(s, out_p, "feed_forward_out"));
   }
   return KFB_OK;
 }
@@ -252,8 +259,11 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
     if (dx != nullptr) KFB_TRY(launch_ffn_rows(s, x, dy, w_in, w_out, dx, nullptr, nullptr, r, c, hidden));
     if (dw_in == nullptr && dw_out == nullptr) return KFB_OK;
     KFB_TRY(launch_ffn_weights(s, x, dy, w_in, w_out, dw_in != nullptr ? w.pl_in : nullptr, dw_out != nullptr ? w.pl_out : nullptr, r, hidden));
-    if (dw_in != nullptr) KFB_TRY(launch_sum_planes(s, w.pl_in, wi_n, planes, dw_in, grad_dtype == KFB_FP32, wi_n));
-    if (dw_out != nullptr) KFB_TRY(launch_sum_planes(s, w.pl_out, wo_n, planes, dw_out, grad_dtype == KFB_FP32, wo_n));
+    PlaneSum sums[2];
+    int n = 0;
+    if (dw_in != nullptr) sums[n++] = {w.pl_in, wi_n, planes, dw_in, grad_dtype == KFB_FP32, wi_n};
+    if (dw_out != nullptr) sums[n++] = {w.pl_out, wo_n, planes, dw_out, grad_dtype == KFB_FP32, wo_n};
+    KFB_TRY(launch_sum_planes(s, sums, n));
     return KFB_OK;
   }
   if (precise) {
@@ -264,10 +274,17 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
   const bool one = one_kernel(c, hidden, precise);
   const long long piece = piece_rows(rows, c, hidden, precise, 1, one);
   const int most_in = planes_in(piece, c, hidden, precise), most_out = planes_out(piece, c, hidden, precise);
+  const int grad_fp32 = grad_dtype == KFB_FP32;
+  const bool single = rows <= piece, sums_by_pair = sums_kernel(c, hidden, precise);
+  // dx of few rows: by the same launch as the weights' gradients, its hidden channels in pieces; of many: by the library's own product for operands along k
+  const int dx_planes = planes_dx(rows, piece, c, hidden);
+  const bool dx_here = precise || (single && static_cast<long long>(cdiv(static_cast<int>(rows), 128)) * cdiv(c, 128) < 2 * sm_count());
+  PlaneSum sums[3];
+  int n_sums = 0;
   bool transposed = false;
   for (long long r0 = 0; r0 < rows; r0 += piece) {
     const long long r = rows - r0 < piece ? rows - r0 : piece;
-    const int m = static_cast<int>(r);
+    const int m = static_cast<int>(r), add = r0 > 0;
     const void *xr = static_cast<const char*>(x) + r0 * c * size, *dr = static_cast<const char*>(dy) + r0 * c * size;
     if (precise) {
       KFB_TRY(launch_split_planes(s, static_cast<const float*>(xr), w.x3, r * c, r * c));
@@ -288,40 +305,46 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
     } else if (one) {
       KFB_TRY(launch_ffn_hidden(s, xr, dr, wi, wo, w.h, w.dab, m, c, hidden));
     } else {
-      MatmulArgs in = {mx, {wi, c, 0, wi_n}, m, 2 * hidden, c, w.u, 2ll * hidden, 1, 1, 0, 0, precise, "feed_forward_in"};
-      KFB_TRY(launch_matmul(s, in));
-      MatmulArgs dh = {md, {wo, hidden, 1, wo_n}, m, hidden, c, w.dh, hidden, 1, 1, 0, 0, precise, "feed_forward_dh"};
-      KFB_TRY(launch_matmul(s, dh));
+      const MatmulArgs both[2] = {{mx, {wi, c, 0, wi_n}, m, 2 * hidden, c, w.u, 2ll * hidden, 1, 1, 0, 0, precise},
+                                  {md, {wo, hidden, 1, wo_n}, m, hidden, c, w.dh, hidden, 1, 1, 0, 0, precise}};
+      KFB_TRY(launch_matmuls(s, both, 2, "feed_forward_in"));
       KFB_TRY(launch_hidden(s, w, true, r, hidden, precise));
     }
-    if (dx != nullptr && !precise && !rows_too) {
-      if (!transposed) KFB_TRY(launch_transpose(s, w_in, w.wi_t, 2 * hidden, c));
-      transposed = true;
-      KFB_TRY(product(s, w.dab, w.wi_t, dxr, r, c, 2 * hidden, "feed_forward_dx"));
-    } else if (dx != nullptr && precise) {
-      MatmulArgs g = {mg, {wi, c, 1, wi_n}, m, c, 2 * hidden, static_cast<char*>(dx) + r0 * c * size, c, precise, 1, 0, 0, precise, "feed_forward_dx"};
-      KFB_TRY(launch_matmul(s, g));
+    MatmulArgs list[3];
+    int n = 0;
+    if (dx != nullptr && !rows_too) {
+      if (dx_here) {
+        if (dx_planes > 1) {
+          list[n++] = {mg, {wi, c, 1, wi_n}, m, c, 2ll * hidden, w.pl_dx, c, 1, dx_planes, r * c, 0, precise};
+          sums[n_sums++] = {w.pl_dx, r * c, dx_planes, dxr, precise, r * c};
+        } else {
+          list[n++] = {mg, {wi, c, 1, wi_n}, m, c, 2ll * hidden, dxr, c, precise, 1, 0, 0, precise};
+        }
+      } else {
+        if (!transposed) KFB_TRY(launch_transpose(s, w_in, w.wi_t, 2 * hidden, c));
+        transposed = true;
+        KFB_TRY(product(s, w.dab, w.wi_t, dxr, r, c, 2 * hidden, "feed_forward_dx"));
+      }
     }
-    const int add = r0 > 0;
-    if (sums_kernel(c, hidden, precise)) {
+    if (sums_by_pair) {
       if (dw_in != nullptr || dw_out != nullptr)
         KFB_TRY(launch_ffn_sums(s, w.dab, xr, w.h, dr, dw_in != nullptr ? w.pl_in : nullptr, dw_out != nullptr ? w.pl_out : nullptr, most_in, add, m, hidden));
-      continue;
+    } else {
+      // (one piece of the rows, of the contraction too: straight into the gradient)
+      if (dw_in != nullptr) {
+        if (single && most_in == 1) list[n++] = {across(mg), across(mx), 2 * hidden, c, r, dw_in, c, grad_fp32, 1, 0, 0, precise};
+        else list[n++] = {across(mg), across(mx), 2 * hidden, c, r, w.pl_in, c, 1, matmul_splits(2 * hidden, c, r, most_in), wi_n, add, precise};
+      }
+      if (dw_out != nullptr) {
+        if (single && most_out == 1) list[n++] = {across(md), across(mh), c, hidden, r, dw_out, hidden, grad_fp32, 1, 0, 0, precise};
+        else list[n++] = {across(md), across(mh), c, hidden, r, w.pl_out, hidden, 1, matmul_splits(c, hidden, r, most_out), wo_n, add, precise};
+      }
     }
-    if (dw_in != nullptr) {
-      const int splits = matmul_splits(2 * hidden, c, r, most_in);
-      MatmulArgs g = {across(mg), across(mx), 2 * hidden, c, r, w.pl_in, c, 1, splits, wi_n, add, precise, "feed_forward_dw"};
-      KFB_TRY(launch_matmul(s, g));
-    }
-    if (dw_out != nullptr) {
-      const int splits = matmul_splits(c, hidden, r, most_out);
-      MatmulArgs g = {across(md), across(mh), c, hidden, r, w.pl_out, hidden, 1, splits, wo_n, add, precise, "feed_forward_dw"};
-      KFB_TRY(launch_matmul(s, g));
-    }
+    if (n > 0) KFB_TRY(launch_matmuls(s, list, n, "feed_forward_products"));
   }
-  if (dw_in != nullptr) KFB_TRY(launch_sum_planes(s, w.pl_in, wi_n, most_in, dw_in, grad_dtype == KFB_FP32, wi_n));
-  if (dw_out != nullptr) KFB_TRY(launch_sum_planes(s, w.pl_out, wo_n, most_out, dw_out, grad_dtype == KFB_FP32, wo_n));
-  return KFB_OK;
+  if (dw_in != nullptr && (sums_by_pair || !single || most_in > 1)) sums[n_sums++] = {w.pl_in, wi_n, most_in, dw_in, grad_fp32, wi_n};
+  if (dw_out != nullptr && (sums_by_pair || !single || most_out > 1)) sums[n_sums++] = {w.pl_out, wo_n, most_out, dw_out, grad_fp32, wo_n};
+  return n_sums > 0 ? launch_sum_planes(s, sums, n_sums) : KFB_OK;
 }
 
 }  // extern "C"

@@ -12,6 +12,7 @@
 #include <type_traits>
 
 #include "ops_common.cuh"
+#include "ptx.cuh"
 #include "vec_io.cuh"
 
 namespace kfb {
@@ -53,10 +54,20 @@ struct Raw {
   }
 };
 
-// LANES lanes hold a row, P pieces of V channels each; R rows in flight for each group of lanes.  EXACT: c == LANES * V * P.  PARAMS: dw, db wanted.
-template <typename TX, typename TD, int V, int LANES, int P, int R, bool EXACT, bool PARAMS>
-__global__ void __launch_bounds__(32 * kWarps) layernorm_grad_kernel(const TD* dy, const TX* x, const float* w, TX* dx, float* partial, long long rows,
-                                                                     int c, float eps) {
+enum Params : int { kNone = 0, kPartial = 1, kCluster = 2 };   // dw, db: not wanted; a row of partial sums a block; the whole grid is one cluster
+
+// A float of the shared memory of the cluster's CTA `rank`, at the place of this CTA's `p`.
+__device__ __forceinline__ float peer_float(const float* p, unsigned rank) {
+  float v;
+  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(ptx::smem_u32(p)), "r"(rank) : "memory");
+  return v;
+}
+
+// LANES lanes hold a row, P pieces of V channels each; R rows in flight for each group of lanes.  EXACT: c == LANES * V * P.
+template <typename TX, typename TD, int V, int LANES, int P, int R, bool EXACT, int MODE>
+__global__ void __launch_bounds__(32 * kWarps) layernorm_grad_kernel(const TD* dy, const TX* x, const float* w, TX* dx, float* partial, float* dw,
+                                                                     float* db, long long rows, int c, float eps) {
+  constexpr bool PARAMS = MODE != kNone;
   constexpr int N = P * V, kGroups = 32 / LANES, kRows = kGroups * R;
   grid_dependency_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LANES;
@@ -161,6 +172,7 @@ __global__ void __launch_bounds__(32 * kWarps) layernorm_grad_kernel(const TD* d
 
   if constexpr (PARAMS) {
     __shared__ float s_sum[kWarps][LANES * N];
+    __shared__ float s_total[MODE == kCluster ? 2 * LANES * N : 1];
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       float(&a)[N] = which ? ab : aw;
@@ -180,9 +192,21 @@ __global__ void __launch_bounds__(32 * kWarps) layernorm_grad_kernel(const TD* d
         float t = 0.f;
 #pragma unroll
         for (int k = 0; k < kWarps; ++k) t += s_sum[k][ch];
-        partial[(static_cast<long long>(blockIdx.x) * 2 + which) * c + ch] = t;
+        if constexpr (MODE == kCluster) s_total[which * c + ch] = t;
+        else partial[(static_cast<long long>(blockIdx.x) * 2 + which) * c + ch] = t;
       }
       __syncthreads();
+    }
+    if constexpr (MODE == kCluster) {
+      // the blocks' sums, in their order, from one another's shared memory: few rows then take one launch
+      ptx::cluster_sync();
+      for (int i = blockIdx.x * 32 * kWarps + threadIdx.x; i < 2 * c; i += gridDim.x * 32 * kWarps) {
+        float t = 0.f;
+        for (unsigned b = 0; b < gridDim.x; ++b) t += peer_float(&s_total[i], b);
+        float* d = i < c ? dw : db;
+        if (d != nullptr) d[i < c ? i : i - c] = t;
+      }
+      ptx::cluster_sync();
     }
   }
 }
@@ -213,6 +237,7 @@ __global__ void __launch_bounds__(1024) layernorm_grad_sum_kernel(const float* p
 
 constexpr int kBlocksPerSm = 8;      // at most: the workspace's partial sums are sized by it
 constexpr int kMostSms = 160;
+constexpr int kMostCluster = 8;      // blocks of a cluster.  Up to four steps of each of them they are faster than many blocks and a second launch
 
 struct Args {
   cudaStream_t stream;
@@ -225,25 +250,31 @@ struct Args {
   float eps;
 };
 
-template <typename TX, typename TD, int V, int LANES, int P, bool EXACT, bool PARAMS>
-int launch_params(const Args& a) {
+template <typename TX, typename TD, int V, int LANES, int P, bool EXACT, int MODE>
+int launch_mode(const Args& a) {
   constexpr int N = V * P, R = N <= 8 ? 2 : 1;
-  auto kernel = layernorm_grad_kernel<TX, TD, V, LANES, P, R, EXACT, PARAMS>;
-  static std::once_flag once;
-  static int held = 1;
-  std::call_once(once, [&] {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, 32 * kWarps, 0) != cudaSuccess) cudaGetLastError();
-    held = held < 1 ? 1 : held > kBlocksPerSm ? kBlocksPerSm : held;
-  });
-  const int sms = sm_count() < kMostSms ? sm_count() : kMostSms;
+  auto kernel = layernorm_grad_kernel<TX, TD, V, LANES, P, R, EXACT, MODE>;
   const long long step = static_cast<long long>(kWarps) * (32 / LANES) * R, want = (a.rows + step - 1) / step;
-  const int blocks = static_cast<int>(want < static_cast<long long>(sms) * held ? want : static_cast<long long>(sms) * held);
+  if constexpr (MODE == kPartial) {
+    if (want <= 4 * kMostCluster) return launch_mode<TX, TD, V, LANES, P, EXACT, kCluster>(a);
+  }
+  int blocks = static_cast<int>(want < kMostCluster ? want : kMostCluster);
+  if constexpr (MODE != kCluster) {
+    static std::once_flag once;
+    static int held = 1;
+    std::call_once(once, [&] {
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, 32 * kWarps, 0) != cudaSuccess) cudaGetLastError();
+      held = held < 1 ? 1 : held > kBlocksPerSm ? kBlocksPerSm : held;
+    });
+    const long long sms = sm_count() < kMostSms ? sm_count() : kMostSms;
+    blocks = static_cast<int>(want < sms * held ? want : sms * held);
+  }
   {
     LaunchScope scope(a.stream, "layernorm_grad");
-    KFB_TRY(launch_kernel(a.stream, kernel, blocks, 32 * kWarps, 0, static_cast<const TD*>(a.dy), static_cast<const TX*>(a.x), a.w,
-                          static_cast<TX*>(a.dx), a.partial, a.rows, a.c, a.eps));
+    KFB_TRY(launch_kernel_clustered(a.stream, kernel, MODE == kCluster ? blocks : 1, blocks, 32 * kWarps, 0, static_cast<const TD*>(a.dy),
+                                    static_cast<const TX*>(a.x), a.w, static_cast<TX*>(a.dx), a.partial, a.dw, a.db, a.rows, a.c, a.eps));
   }
-  if (PARAMS) {
+  if (MODE == kPartial) {
     LaunchScope scope(a.stream, "layernorm_grad_sum");
     KFB_TRY(launch_kernel(a.stream, layernorm_grad_sum_kernel, cdiv(2 * a.c, 32), 1024, 0, const_cast<const float*>(a.partial), a.dw, a.db, blocks,
                           a.c));
@@ -253,7 +284,7 @@ int launch_params(const Args& a) {
 
 template <typename TX, typename TD, int V, int LANES, int P, bool EXACT>
 int launch(const Args& a) {
-  return a.dw != nullptr || a.db != nullptr ? launch_params<TX, TD, V, LANES, P, EXACT, true>(a) : launch_params<TX, TD, V, LANES, P, EXACT, false>(a);
+  return a.dw != nullptr || a.db != nullptr ? launch_mode<TX, TD, V, LANES, P, EXACT, kPartial>(a) : launch_mode<TX, TD, V, LANES, P, EXACT, kNone>(a);
 }
 
 template <typename TX, typename TD>

@@ -24,40 +24,61 @@ struct Words {
   uint32_t w[4];
 };
 
-// Seed and offset of a launch, the seed as the ten rounds' keys.  STATE: read from device memory when the kernel runs; otherwise the keys are launch
-// parameters, operands that cost no instruction.
-struct Keys {
-  uint32_t k[20];
+// What a launch's words have in common: the seed as the ten rounds' keys, and the products of the first two rounds that hang on the offset alone (the
+// second one's on the block's upper half too, which is zero up to 2^34 elements).  STATE: read from device memory when the kernel runs; otherwise
+// launch parameters, operands that cost no instruction.
+constexpr uint32_t kM0 = 0xD2511F53u, kM1 = 0xCD9E8D57u;
+struct Stream {
+  uint32_t key[20];
+  uint32_t offset_hi, b1_hi, b1_lo;      // 64-bit product of the first round with the offset's lower half
+  uint32_t a2_hi, a2_lo;                 // of the second round, for an upper half of zero
 };
-__host__ __device__ __forceinline__ void round_keys(unsigned long long seed, Keys& d) {
+__host__ __device__ __forceinline__ void make_stream(unsigned long long seed, unsigned long long offset, Stream& d) {
   uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
-    d.k[2 * i] = k0;
-    d.k[2 * i + 1] = k1;
+    d.key[2 * i] = k0;
+    d.key[2 * i + 1] = k1;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
+  const unsigned long long b1 = static_cast<unsigned long long>(kM1) * static_cast<uint32_t>(offset);
+  d.offset_hi = static_cast<uint32_t>(offset >> 32);
+  d.b1_hi = static_cast<uint32_t>(b1 >> 32);
+  d.b1_lo = static_cast<uint32_t>(b1);
+  const unsigned long long a2 = static_cast<unsigned long long>(kM0) * (d.b1_hi ^ d.key[0]);
+  d.a2_hi = static_cast<uint32_t>(a2 >> 32);
+  d.a2_lo = static_cast<uint32_t>(a2);
 }
 
-__device__ __forceinline__ Words philox(unsigned long long block, unsigned long long offset, const Keys& keys) {
-  uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32);
-  uint32_t c2 = static_cast<uint32_t>(offset), c3 = static_cast<uint32_t>(offset >> 32);
+__device__ __forceinline__ Words philox(unsigned long long block, const Stream& s) {
+  const uint32_t upper = static_cast<uint32_t>(block >> 32);
+  // the first two rounds
+  const unsigned long long a1 = static_cast<unsigned long long>(kM0) * static_cast<uint32_t>(block);
+  const uint32_t d2 = static_cast<uint32_t>(a1 >> 32) ^ s.offset_hi ^ s.key[1], d3 = static_cast<uint32_t>(a1);
+  uint32_t a2_hi = s.a2_hi, a2_lo = s.a2_lo;
+  if (upper != 0) {
+    const unsigned long long a2 = static_cast<unsigned long long>(kM0) * (s.b1_hi ^ upper ^ s.key[0]);
+    a2_hi = static_cast<uint32_t>(a2 >> 32);
+    a2_lo = static_cast<uint32_t>(a2);
+  }
+  const unsigned long long b2 = static_cast<unsigned long long>(kM1) * d2;
+  uint32_t c0 = static_cast<uint32_t>(b2 >> 32) ^ s.b1_lo ^ s.key[2], c1 = static_cast<uint32_t>(b2);
+  uint32_t c2 = a2_hi ^ d3 ^ s.key[3], c3 = a2_lo;
 #pragma unroll
-  for (int i = 0; i < 10; ++i) {
-    const unsigned long long a = static_cast<unsigned long long>(0xD2511F53u) * c0, b = static_cast<unsigned long long>(0xCD9E8D57u) * c2;
-    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ keys.k[2 * i];
+  for (int i = 2; i < 10; ++i) {
+    const unsigned long long a = static_cast<unsigned long long>(kM0) * c0, b = static_cast<unsigned long long>(kM1) * c2;
+    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ s.key[2 * i];
     c1 = static_cast<uint32_t>(b);
-    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ keys.k[2 * i + 1];
+    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ s.key[2 * i + 1];
     c3 = static_cast<uint32_t>(a);
   }
   return {{c0, c1, c2, c3}};
 }
 
 struct DropParams {
-  const long long* rng;             // (seed, offset) in device memory, or null: the two below
-  Keys keys;
-  unsigned long long offset;
+  const long long* rng;             // (seed, offset) in device memory, or null: `stream` is made of them
+  Stream stream;
   uint32_t cut;                     // kept: word > cut
   int keep_all;                     // nothing is dropped
   float scale;
@@ -105,18 +126,18 @@ __device__ __forceinline__ void values(const Piece<TX, V>& d, float (&v)[V]) {
 
 // The mask of elements e ... e + V - 1 (e a multiple of 4 unless V is 1).
 template <typename TX, int V>
-__device__ __forceinline__ void kept(const DropParams& p, const Keys& keys, unsigned long long offset, long long e, Piece<TX, V>& m) {
+__device__ __forceinline__ void kept(const DropParams& p, const Stream& stream, long long e, Piece<TX, V>& m) {
 #pragma unroll
   for (int i = 0; i < Piece<TX, V>::kWords; ++i) m.w[i] = 0;
   if constexpr (V == 1) {
-    const Words r = philox(static_cast<unsigned long long>(e) >> 2, offset, keys);
+    const Words r = philox(static_cast<unsigned long long>(e) >> 2, stream);
     const int at = static_cast<int>(e & 3);
     const uint32_t w = at == 0 ? r.w[0] : at == 1 ? r.w[1] : at == 2 ? r.w[2] : r.w[3];
     m.w[0] = (w > p.cut) | p.keep_all ? 0xffffffffu : 0u;
   } else {
 #pragma unroll
     for (int b = 0; b < V / 4; ++b) {
-      const Words r = philox((static_cast<unsigned long long>(e) >> 2) + b, offset, keys);
+      const Words r = philox((static_cast<unsigned long long>(e) >> 2) + b, stream);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int k = 4 * b + i;
@@ -164,10 +185,9 @@ template <typename TX, typename TR, int V, bool RESID, bool STATE>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm) dropout_kernel(const TX* x, const TR* resid, TR* out, const DropParams p) {
   constexpr int U = 2;
   grid_dependency_enter();
-  Keys own;
-  if (STATE) round_keys(static_cast<unsigned long long>(p.rng[0]), own);
-  const Keys& keys = STATE ? own : p.keys;
-  const unsigned long long offset = STATE ? static_cast<unsigned long long>(p.rng[1]) : p.offset;
+  Stream own;
+  if (STATE) make_stream(static_cast<unsigned long long>(p.rng[0]), static_cast<unsigned long long>(p.rng[1]), own);
+  const Stream& stream = STATE ? own : p.stream;
   constexpr long long kBlock = static_cast<long long>(kThreads) * U * V;
   for (long long base = blockIdx.x * kBlock; base < p.inner; base += gridDim.x * kBlock) {
     long long at[U];
@@ -179,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) dropout_kernel(const T
     }
     apply<V, U, RESID>(x, resid, out, at, live, p.scale, [&](int u) {
       Piece<TX, V> m;
-      kept<TX, V>(p, keys, offset, at[u], m);
+      kept<TX, V>(p, stream, at[u], m);
       return m;
     });
   }
@@ -190,17 +210,16 @@ template <typename TX, typename TR, int V, bool RESID, bool STATE>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm) dropout_shared_kernel(const TX* x, const TR* resid, TR* out, const DropParams p) {
   constexpr int U = RESID ? 3 : 4;
   grid_dependency_enter();
-  Keys own;
-  if (STATE) round_keys(static_cast<unsigned long long>(p.rng[0]), own);
-  const Keys& keys = STATE ? own : p.keys;
-  const unsigned long long offset = STATE ? static_cast<unsigned long long>(p.rng[1]) : p.offset;
+  Stream own;
+  if (STATE) make_stream(static_cast<unsigned long long>(p.rng[0]), static_cast<unsigned long long>(p.rng[1]), own);
+  const Stream& stream = STATE ? own : p.stream;
   const long long pieces = p.inner / V, total = p.outer * p.chunks * pieces;
   for (long long t = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; t < total; t += static_cast<long long>(gridDim.x) * kThreads) {
     const long long i = t % pieces * V, rest = t / pieces, o = rest / p.chunks, s0 = rest % p.chunks * p.chunk;
     // (a piece of the shared axis is short, or the threads are many: either way below 2^31 for what a GPU can hold)
     int left = static_cast<int>(s0 + p.chunk < p.shared ? p.chunk : p.shared - s0);
     Piece<TX, V> m;
-    kept<TX, V>(p, keys, offset, o * p.inner + i, m);
+    kept<TX, V>(p, stream, o * p.inner + i, m);
     const long long first = (o * p.shared + s0) * p.inner + i;
     const TX* xs = x + first;
     const TR* rs = RESID ? resid + first : nullptr;
@@ -276,8 +295,7 @@ extern "C" KFB_API int kfb_dropout(const void* x, const void* residual, void* ou
   KFB_CHECK_ARG(x != nullptr && out != nullptr, "dropout: null tensor");
   DropParams d = {};
   d.rng = rng;
-  round_keys(static_cast<unsigned long long>(seed), d.keys);
-  d.offset = static_cast<unsigned long long>(offset);
+  make_stream(static_cast<unsigned long long>(seed), static_cast<unsigned long long>(offset), d.stream);
   d.keep_all = drop_below == 0;
   d.cut = drop_below == 0 ? 0u : static_cast<uint32_t>(drop_below - 1);
   d.scale = scale;

@@ -166,15 +166,15 @@ ffn_hidden_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         const int rs0 = rs;
         const uint32_t r_ph0 = r_ph;
         for (int c = 0; ok && c < n; ++c) {
-          ok = ptx::mbar_wait_cluster(&s_free[s], s_ph, 525);
+          ok = ptx::mbar_wait_hot(&s_free[s], s_ph, 525);
           if (!ok) break;
           ptx::tc_fence_after_sync();
           const uint32_t d = tmem + s * kS;
           if (p.resident) { rs = rs0; r_ph = r_ph0; }
           const bool fresh_rows = !p.resident || c == 0, last_rows = !p.resident || c == n - 1;
           for (int kb = 0; kb < p.k_blocks; ++kb) {
-            if (fresh_rows) ok = ptx::mbar_wait(&r_full[rs], r_ph, 526);
-            ok = ok && ptx::mbar_wait(&w_full[st], ph, 527);
+            if (fresh_rows) ok = ptx::mbar_wait_hot(&r_full[rs], r_ph, 526);
+            ok = ok && ptx::mbar_wait_hot(&w_full[st], ph, 527);
             if (!ok) break;
             ptx::tc_fence_after_sync();
             const uint64_t xd = row_desc + rs * (kRowSlot >> 4), wd = w1_desc + st * (kWSlot >> 4), gd = g_desc + st * (kWSlot >> 4);

@@ -54,13 +54,6 @@ __device__ __forceinline__ uint64_t v_desc(uint32_t addr) {    // [64 k][64 chan
          (1ull << 46) | (2ull << 61);
 }
 
-// The wait of a thread that issues products: most of what it waits for is there, or about to be, and a suspended thread is slow to come back.
-__device__ __forceinline__ bool hot_wait(uint64_t* bar, uint32_t parity, int code) {
-  for (int i = 0; i < 64; ++i)
-    if (ptx::mbar_test(bar, parity)) return true;
-  return ptx::mbar_wait(bar, parity, code);
-}
-
 // The four warps that share 32 rows.
 __device__ __forceinline__ void quad_sync(int quad) { asm volatile("bar.sync %0, 128;" ::"r"(quad + 1) : "memory"); }
 
@@ -229,15 +222,15 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
       uint32_t ph = 0, r_ph = 0;
       bool ok = true;
       for (int i = 0; ok && i < total; ++i) {
-        ok = hot_wait(s_free, (i & 1) ^ 1, 547);
-        if (kTmemRows && c == 0) ok = ok && hot_wait(xy_full, it & 1, 557);
+        ok = ptx::mbar_wait_hot(s_free, (i & 1) ^ 1, 547);
+        if (kTmemRows && c == 0) ok = ok && ptx::mbar_wait_hot(xy_full, it & 1, 557);
         if (!ok) break;
         ptx::tc_fence_after_sync();
 #pragma unroll
         for (int kb = 0; kb < kK; ++kb) {
           const int rs = rs0 + kb;                  // (kRowSlots is a multiple of kK)
-          if (!kTmemRows && c == 0) ok = hot_wait(&r_full[rs], r_ph, 548);
-          if ((kb & 1) == 0) ok = ok && hot_wait(&w_full[st], ph, 549);
+          if (!kTmemRows && c == 0) ok = ptx::mbar_wait_hot(&r_full[rs], r_ph, 548);
+          if ((kb & 1) == 0) ok = ok && ptx::mbar_wait_hot(&w_full[st], ph, 549);
           if (!ok) break;
           ptx::tc_fence_after_sync();
           const uint32_t w_at = st * (kWSlot >> 4) + (kb & 1) * (kWBlock >> 4);
@@ -279,11 +272,11 @@ ffn_rows_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
       uint32_t v_ph = 0;
       bool ok = true;
       for (int i = 0; ok && i < total; ++i) {
-        if (c == 0) ok = hot_wait(o_free, (it & 1) ^ 1, 550);
+        if (c == 0) ok = ptx::mbar_wait_hot(o_free, (it & 1) ^ 1, 550);
         // (behind the next chunk's S, not before or within it: the tensor core then has dX to do while that S is read)
-        if (i + 1 < total) ok = ok && hot_wait(&s_issued[(i + 1) & 1], ((i + 1) >> 1) & 1, 556);
-        ok = ok && hot_wait(p_full, i & 1, 551);
-        ok = ok && hot_wait(&v_full[v], v_ph, 552);
+        if (i + 1 < total) ok = ok && ptx::mbar_wait_hot(&s_issued[(i + 1) & 1], ((i + 1) >> 1) & 1, 556);
+        ok = ok && ptx::mbar_wait_hot(p_full, i & 1, 551);
+        ok = ok && ptx::mbar_wait_hot(&v_full[v], v_ph, 552);
         if (!ok) break;
         ptx::tc_fence_after_sync();
         const uint64_t vd = vd0 + v * (kVSlot >> 4);

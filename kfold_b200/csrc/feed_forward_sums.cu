@@ -105,7 +105,7 @@ ffn_sums_pair_kernel(const __grid_constant__ CUtensorMap tm_dab, const __grid_co
       uint32_t ph = 0;
       bool ok = true;
       for (int b = b0; b < b1; ++b) {
-        ok = ptx::mbar_wait(&full[st], ph, 583);
+        ok = ptx::mbar_wait_hot(&full[st], ph, 583);
         if (!ok) break;
         ptx::tc_fence_after_sync();
         const uint64_t a = d0 + st * (kStage >> 4), bd = a + (2 * kAPart >> 4);

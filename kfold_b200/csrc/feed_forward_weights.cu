@@ -11,8 +11,9 @@
 //   S   = [x [Wa; Wb]^T | dy Wo]      rows x 192
 //   P   = da, db, h as bf16           in shared memory: sixteen warps, one S buffer
 //   sums += x^T [da | db], dy^T h     channels x 192, every operand read across k as it lies: the tiles of x and dy serve both products
-// One thread issues  ab(i + 1), dab(i), dh(i + 1), dWo(i): the next tile's products run under the element-wise part, and a buffer of x or dy has 768 cycles of
-// products between its last use and the next tile's first (three tiles are alive, two fit).
+// One thread issues  S(i + 1), sums(i):  S runs under the element-wise part.  (With x^T and dy^T in tensor memory, 8 x 8 blocks transposed on their way by four
+// more warps, the sums' products would be a third shorter; but the copy competes with S for shared memory, 1 500 cycles a tile, and the sums wait for it:
+// 119 us where this is 106, 147 456 rows of 512 hidden channels.)  Bound by shared memory: 336 KB a tile, 2 600 cycles, and 2 990 for the products as they are.
 #include <mutex>
 
 #include "feed_forward_hidden.cuh"
@@ -149,12 +150,12 @@ ffn_weights_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
       for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x, ++unit) {
         int t0;
         const int n = tiles_of(u, t0);
-        ok = ptx::mbar_wait(w_full, unit & 1, 563);
+        ok = ptx::mbar_wait_hot(w_full, unit & 1, 563);
         for (int i = -1; ok && i < n; ++i) {
           const int g = round + i;                            // tile i of this unit, and the next one's slots
           const int x1 = 2 * ((g + 1) & 1), x0 = 2 * (g & 1);
           if (i + 1 < n) {
-            ok = ptx::mbar_wait(s_free, (g & 1), 564) && ptx::mbar_wait(&r_full[x1], ((g + 1) >> 1) & 1, 565);
+            ok = ptx::mbar_wait_hot(s_free, (g & 1), 564) && ptx::mbar_wait_hot(&r_full[x1], ((g + 1) >> 1) & 1, 565);
             if (!ok) break;
             ptx::tc_fence_after_sync();
 #pragma unroll
@@ -163,7 +164,7 @@ ffn_weights_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                               k > 0 ? 1u : 0u);
           }
           if (i + 1 < n) {
-            ok = ptx::mbar_wait(&r_full[x1 + 1], ((g + 1) >> 1) & 1, 568);
+            ok = ptx::mbar_wait_hot(&r_full[x1 + 1], ((g + 1) >> 1) & 1, 568);
             if (!ok) break;
             ptx::tc_fence_after_sync();
 #pragma unroll
@@ -174,8 +175,8 @@ ffn_weights_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
             if (i + 2 == n) ptx::tc_commit(w_free);
           }
           if (i >= 0) {
-            if (i == 0) ok = ptx::mbar_wait(o_free, (unit & 1) ^ 1, 566);
-            ok = ok && ptx::mbar_wait(p_full, g & 1, 567);
+            if (i == 0) ok = ptx::mbar_wait_hot(o_free, (unit & 1) ^ 1, 566);
+            ok = ok && ptx::mbar_wait_hot(p_full, g & 1, 567);
             if (!ok) break;
             ptx::tc_fence_after_sync();
 #pragma unroll

@@ -128,6 +128,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int co
   return true;
 }
 
+// The wait of a thread that issues products: most of what it waits for is there, or about to be, and a suspended thread is slow to come back (a wait for a
+// barrier that has flipped costs it some 90 cycles this way, 230 to 400 otherwise; clock stamps).
+__device__ __forceinline__ bool mbar_wait_hot(uint64_t* bar, uint32_t parity, int code) {
+  for (int i = 0; i < 64; ++i)
+    if (mbar_test(bar, parity)) return true;
+  return mbar_wait(bar, parity, code);
+}
+
 // ---------------------------------------------------------------- TMA (tiled bulk tensor copies, one CTA, no cluster broadcast)
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");

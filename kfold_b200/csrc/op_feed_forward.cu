@@ -76,15 +76,22 @@ struct FfnWs {
 };
 // Whether h, da and db come from the one kernel (feed_forward_hidden.cu).
 bool one_kernel(int c, int hidden, int precise) { return !precise && ffn_hidden_ok(c, hidden); }
-// Whether both gradients come from x and dy alone, nothing kept in between (feed_forward_rows.cu, feed_forward_weights.cu).
-bool nothing_kept(int c, int hidden, int precise) { return !precise && ffn_weights_ok(c, hidden) && ffn_rows_ok(c, hidden); }
+// Whether both gradients come from x and dy alone, nothing kept in between (feed_forward_rows.cu, feed_forward_weights.cu).  Few rows do not fill their
+// tiles of 256 rows: the kernel that spreads the hidden channels over the device, and one launch of all products, are faster (128 channels, 512 hidden, forward
+// and gradient in graph replays: 256 rows 23 us where these take 30, 6 000 36 and 38, 9 000 46 and 40).
+bool nothing_kept(long long rows, int c, int hidden, int precise) {
+  return rows >= 48ll * sm_count() && !precise && ffn_weights_ok(c, hidden) && ffn_rows_ok(c, hidden);
+}
 // Pieces that the rows of a weight's gradient are summed in.
-bool sums_kernel(int c, int hidden, int precise) { return one_kernel(c, hidden, precise) && ffn_sums_ok(c, hidden); }
+// (256 channels: the pairs' sums from as many rows on as dx comes with the hidden channels; 1 000 rows 34 us by the one launch of products, 48 by these, 9 600
+// 95 and 91, 20 000 171 and 159.)
+bool many_rows(long long rows) { return rows >= 64ll * sm_count(); }
+bool sums_kernel(long long piece, int c, int hidden, int precise) { return many_rows(piece) && one_kernel(c, hidden, precise) && ffn_sums_ok(c, hidden); }
 int planes_in(long long piece, int c, int hidden, int precise) {
-  return sums_kernel(c, hidden, precise) ? ffn_sums_planes(piece, hidden) : matmul_splits(2 * hidden, c, piece, kMostPlanes);
+  return sums_kernel(piece, c, hidden, precise) ? ffn_sums_planes(piece, hidden) : matmul_splits(2 * hidden, c, piece, kMostPlanes);
 }
 int planes_out(long long piece, int c, int hidden, int precise) {
-  return sums_kernel(c, hidden, precise) ? ffn_sums_planes(piece, hidden) : matmul_splits(c, hidden, piece, kMostPlanes);
+  return sums_kernel(piece, c, hidden, precise) ? ffn_sums_planes(piece, hidden) : matmul_splits(c, hidden, piece, kMostPlanes);
 }
 
 // Pieces of the hidden channels of dx = [da, db] [Wa; Wb] where the rows come in one piece and their tiles do not fill the device (1 elsewhere).
@@ -98,7 +105,7 @@ size_t carve(FfnWs& w, void* base, long long rows, int c, int hidden, int precis
   const long long piece = piece_rows(rows, c, hidden, precise, backward, one);
   const size_t r = static_cast<size_t>(piece), parts = precise ? 3 : 1, cc = c, hh = hidden;
   w = {};
-  if (backward && nothing_kept(c, hidden, precise)) {
+  if (backward && nothing_kept(rows, c, hidden, precise)) {
     const size_t planes = ffn_weights_planes(rows, hidden);
     w.pl_in = cv.take<float>(planes * 2 * hh * cc);
     w.pl_out = cv.take<float>(planes * hh * cc);
@@ -254,7 +261,7 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
                 bits(dy) | bits(x) | bits(w_in) | bits(w_out) | bits(dx) | bits(dw_in) | bits(dw_out)));
   FfnWs w;
   carve(w, workspace, rows, c, hidden, precise, 1);
-  if (nothing_kept(c, hidden, precise)) {
+  if (nothing_kept(rows, c, hidden, precise)) {
     const int r = static_cast<int>(rows), planes = ffn_weights_planes(rows, hidden);
     if (dx != nullptr) KFB_TRY(launch_ffn_rows(s, x, dy, w_in, w_out, dx, nullptr, nullptr, r, c, hidden));
     if (dw_in == nullptr && dw_out == nullptr) return KFB_OK;
@@ -275,7 +282,7 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
   const long long piece = piece_rows(rows, c, hidden, precise, 1, one);
   const int most_in = planes_in(piece, c, hidden, precise), most_out = planes_out(piece, c, hidden, precise);
   const int grad_fp32 = grad_dtype == KFB_FP32;
-  const bool single = rows <= piece, sums_by_pair = sums_kernel(c, hidden, precise);
+  const bool single = rows <= piece, sums_by_pair = sums_kernel(piece, c, hidden, precise);
   // dx of few rows: by the same launch as the weights' gradients, its hidden channels in pieces; of many: by the library's own product for operands along k
   const int dx_planes = planes_dx(rows, piece, c, hidden);
   const bool dx_here = precise || (single && static_cast<long long>(cdiv(static_cast<int>(rows), 128)) * cdiv(c, 128) < 2 * sm_count());
@@ -297,7 +304,7 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
       o.by_k = 1;
       return o;
     };
-    const bool rows_too = one && dx != nullptr && ffn_rows_ok(c, hidden) && m >= 64 * sm_count();
+    const bool rows_too = one && dx != nullptr && ffn_rows_ok(c, hidden) && c == 256 && many_rows(m);
     void* dxr = static_cast<char*>(dx) + r0 * c * size;
     if (rows_too) {
       const bool keep = dw_in != nullptr || dw_out != nullptr;

@@ -83,6 +83,47 @@ def test_many_rows(rows, c, hidden):
     _check(*_case(rows, c, hidden, seed=5))
 
 
+@pytest.mark.parametrize("rows", [7103, 7104, 7105, 7167, 7169, 7231, 7295, 7297, 9471, 9472, 9473, 9535, 9537, 9599, 9601, 18943, 18945, 19072, 19201, 37889])
+@pytest.mark.parametrize("c, hidden", [(128, 128), (256, 128)])
+def test_rows_around_the_tiles_of_many(rows, c, hidden):
+    """From 7 104 rows (128 channels) and 9 472 (256) on other kernels take them: tiles that end inside a tile, a warp, a pair; one, two and more a CTA."""
+    _check(*_case(rows, c, hidden, seed=rows))
+
+
+@pytest.mark.parametrize("c, hidden", [(128, 8), (128, 64), (128, 192), (128, 448), (128, 1024), (128, 2048), (256, 64), (256, 192), (256, 448), (256, 576), (256, 2048)])
+def test_widths_with_many_rows(c, hidden):
+    """One chunk of hidden channels, odd numbers of them, more than the device has multiprocessors for."""
+    _check(*_case(19333, c, hidden, seed=hidden))
+
+
+@pytest.mark.parametrize("c", [128, 256])
+def test_only_some_gradients_of_many_rows(c):
+    x, w_in, w_out, dy = _case(10001, c, 256)
+    want = F.gated_feed_forward_backward(dy, x, w_in, w_out)
+    for need in ((True, False, False), (False, True, False), (False, False, True), (False, True, True), (True, False, True), (False, False, False)):
+        got = F.gated_feed_forward_backward(dy, x, w_in, w_out, *need)
+        for g, w, n in zip(got, want, need):
+            assert (g is None) == (not n) and (g is None or torch.equal(g, w))
+
+
+@pytest.mark.parametrize("c", [128, 256])
+def test_rows_behind_the_last_of_many_are_left_alone(c):
+    rows, hidden = 9601, 192
+    x, w_in, w_out, dy = _case(rows, c, hidden)
+    out, dx = (torch.full((rows + 300, c), 7.0, dtype=BF, device=DEV) for _ in range(2))
+    dwi, dwo = torch.empty_like(w_in), torch.empty_like(w_out)
+    lib = L.lib()
+    need = [lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, 0, b) for b in (0, 1)]
+    ws = torch.full((max(need) + 4096,), 0xA5, dtype=torch.uint8, device=DEV)
+    L.check(lib.kfb_feed_forward_fwd(L.ptr(x), L.ptr(w_in), L.ptr(w_out), L.ptr(out), L.ptr(ws), need[0], rows, c, hidden, 0, L.stream_ptr()))
+    L.check(lib.kfb_feed_forward_bwd(L.ptr(dy), L.ptr(x), L.ptr(w_in), L.ptr(w_out), L.ptr(dx), L.ptr(dwi), L.ptr(dwo), L.ptr(ws), need[1], rows, c,
+                                     hidden, 0, 0, L.stream_ptr()))
+    assert (out[rows:] == 7).all() and (dx[rows:] == 7).all() and (ws[max(need):] == 0xA5).all()
+    want = _plain(x, w_in, w_out, dy)
+    _near(out[:rows], want[0], want[4], BF, "y")
+    _near(dx[:rows], want[1], want[5], BF, "dx")
+
+
 @pytest.mark.parametrize("rows, c, hidden, dtype", [(30001, 64, 8192, BF), (47000, 128, 8192, BF), (23000, 256, 8192, BF), (9000, 72, 8192, BF), (5000, 8, 8192, F32)])
 def test_rows_in_several_pieces(rows, c, hidden, dtype):
     """More rows than a workspace holds at once, the last piece a short one."""

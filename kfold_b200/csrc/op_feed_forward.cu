@@ -18,6 +18,9 @@ namespace {
 
 constexpr int kMostPlanes = 64;
 
+// The widths that the sizes below are computed for without leaving their range.
+bool widths_ok(int c, int hidden) { return c > 0 && c % 8 == 0 && hidden > 0 && hidden % 8 == 0 && c <= 65536 && hidden <= 65536; }
+
 // Rows of a piece: as many as keep what a row needs between its products below a gigabyte.  (Smaller ones, whose hidden channels would stay in L2, are no
 // faster: writes into L2 are no faster than writes through it, and every piece starts and ends its launches.)
 long long piece_rows(long long rows, int c, int hidden, int precise, int backward, bool one) {
@@ -175,8 +178,7 @@ int check(const char* name, const void* workspace, size_t workspace_bytes, size_
           uintptr_t tensors) {
   KFB_CHECK_ARG(dtype == KFB_BF16 || dtype == KFB_FP32_PRECISE, "%s: bad dtype %d", name, dtype);
   KFB_CHECK_ARG(rows >= 0 && rows < (1ll << 31), "%s: rows %lld", name, rows);
-  KFB_CHECK_ARG(c > 0 && c % 8 == 0 && hidden > 0 && hidden % 8 == 0 && c <= 65536 && hidden <= 65536, "%s: c=%d, hidden=%d (multiples of 8)", name, c,
-                hidden);
+  KFB_CHECK_ARG(widths_ok(c, hidden), "%s: c=%d, hidden=%d (multiples of 8 up to 65 536)", name, c, hidden);
   KFB_CHECK_ARG((tensors & 15) == 0, "%s: tensors must be 16-byte aligned", name);
   KFB_CHECK_ARG(workspace != nullptr && workspace_bytes >= need, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
   KFB_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "%s: workspace must be 256-byte aligned", name);
@@ -192,7 +194,7 @@ using namespace kfb;
 extern "C" {
 
 KFB_API size_t kfb_feed_forward_workspace_bytes(long long rows, int c, int hidden, int dtype, int backward) {
-  if (rows < 1 || c < 1 || hidden < 1) return 0;
+  if (rows < 1 || !widths_ok(c, hidden)) return 0;
   FfnWs w;
   return carve(w, nullptr, rows, c, hidden, dtype == KFB_FP32_PRECISE, backward);
 }
@@ -251,7 +253,7 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
   KFB_CHECK_ARG(grad_dtype == KFB_FP32 || (grad_dtype == KFB_BF16 && !precise), "feed_forward_bwd: bad dtype %d of the weights' gradients", grad_dtype);
   if (rows == 0) {
     const size_t g = grad_dtype == KFB_FP32 ? 4 : 2;
-    KFB_CHECK_ARG(c > 0 && hidden > 0, "feed_forward_bwd: c=%d, hidden=%d", c, hidden);
+    KFB_CHECK_ARG(widths_ok(c, hidden), "feed_forward_bwd: c=%d, hidden=%d (multiples of 8 up to 65 536)", c, hidden);
     if (dw_in != nullptr) KFB_CUDA(cudaMemsetAsync(dw_in, 0, wi_n * g, s));
     if (dw_out != nullptr) KFB_CUDA(cudaMemsetAsync(dw_out, 0, wo_n * g, s));
     return KFB_OK;

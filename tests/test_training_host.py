@@ -79,6 +79,19 @@ def test_feed_forward_workspace_stops_growing(library):
     assert need(0, 128, 512, 0, 0) == need(5, 0, 512, 0, 0) == 0
 
 
+@pytest.mark.parametrize("c, hidden", [(8, 2 ** 31 - 8), (2 ** 31 - 8, 8), (2 ** 31 - 8, 2 ** 31 - 8), (65544, 8), (8, 65544), (12, 8), (8, -8)])
+def test_feed_forward_refuses_widths_out_of_range(library, c, hidden):
+    vp, some, big = ctypes.c_void_p, 256, 1 << 60
+    for dt in (0, 2):
+        for rows in (1, 1000, (1 << 31) - 1):
+            assert library.kfb_feed_forward_workspace_bytes(rows, c, hidden, dt, 0) == library.kfb_feed_forward_workspace_bytes(rows, c, hidden, dt, 1) == 0
+            assert library.kfb_feed_forward_fwd(vp(some), vp(some), vp(some), vp(some), vp(some), big, rows, c, hidden, dt, None) == 1
+            assert library.kfb_feed_forward_bwd(vp(some), vp(some), vp(some), vp(some), vp(some), vp(some), vp(some), vp(some), big, rows, c, hidden, dt, 1,
+                                                None) == 1
+            assert b"multiples of 8" in library.kfb_last_error()
+    assert library.kfb_feed_forward_bwd(None, None, None, None, None, vp(some), vp(some), None, 0, 0, c, hidden, 0, 0, None) == 1
+
+
 def test_feed_forward_refuses_cpu_tensors():
     x, wi, wo = torch.zeros(4, 8), torch.zeros(32, 8), torch.zeros(8, 16)
     for call in (lambda: F.gated_feed_forward(x, wi, wo), lambda: F.gated_feed_forward_backward(x, x, wi, wo)):

@@ -111,8 +111,12 @@ def _affine(t: torch.Tensor | None) -> torch.Tensor | None:
 
 def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype=None) -> torch.Tensor:
     """LayerNorm over the last dim (model/primitives/normalization.py:61-91)."""
-    _require_cuda(x)
+    _require_cuda(x, weight, bias)
+    _same_device("layer_norm", x, weight, bias)
     c = x.shape[-1]
+    for t in (weight, bias):
+        if t is not None and t.numel() != c:
+            raise ValueError(f"layer_norm: weight or bias {tuple(t.shape)} for x {tuple(x.shape)}")
     if x.is_contiguous():
         x2, rows, pitch = x, x.numel() // c if c else 0, c
     else:

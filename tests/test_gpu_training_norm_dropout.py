@@ -132,6 +132,18 @@ def test_norm_refusals():
         F.layer_norm_backward(_randn(1, 2, 1025), _randn(1, 2, 1025), None)
 
 
+@pytest.mark.parametrize("which", ["weight", "bias"])
+def test_norm_refuses_parameters_of_another_width_or_device(which):
+    x, w = _randn(1, 4, 64), _randn(2, 64)
+    norm = lambda t: F.layer_norm(x, **{"weight": w, "bias": w, which: t})
+    for t in (_randn(3, 32), _randn(3, 65), _randn(3, 1)):
+        with pytest.raises(ValueError, match="layer_norm"):
+            norm(t)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        norm(w.cpu())
+    norm(w.view(1, 64))
+
+
 # ------------------------------------------------------------------------------------------------ dropout
 RNG = (0x0123456789ABCDEF, (1 << 63) + 12345)
 

@@ -8,6 +8,7 @@ and the extension must be built.
 from __future__ import annotations
 
 import math
+from threading import get_ident
 
 import torch
 
@@ -20,11 +21,12 @@ _workspaces: dict = {}
 MOST_KEPT_BYTES = 1 << 30
 
 
-def _workspace(device: torch.device, nbytes: int, most_kept: int | None = None) -> torch.Tensor:
-    """At least `nbytes` of scratch for a call on the current stream, kept for the next call on it unless more than `most_kept`."""
+def _workspace(device: torch.device, nbytes: int, most_kept: int | None = None, holder: int = 0) -> torch.Tensor:
+    """At least `nbytes` of scratch for a call on the current stream, kept for the next call on it (of the same `holder`) unless more than
+    `most_kept`."""
     if most_kept is not None and nbytes > most_kept:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index, L.raw_stream(device.index))
+    key = (device.index, L.raw_stream(device.index), holder)
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = None
@@ -141,10 +143,12 @@ def _same_device(name: str, x: torch.Tensor, *ts: torch.Tensor | None) -> None:
 
 
 def _call_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Scratch for a training call.  One that is being captured gets memory of its graph's own: two graphs may then be replayed at once."""
+    """Scratch for a training call.  One that is being captured gets memory of its graph's own: two graphs may then be replayed at once.
+    Each host thread has its own too (autograd calls from threads that it starts): two that feed one stream put the launches of their calls
+    between one another's."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return _workspace(device, nbytes, MOST_KEPT_BYTES)
+    return _workspace(device, nbytes, MOST_KEPT_BYTES, get_ident())
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-5, need_weight: bool = True,

@@ -5,6 +5,8 @@ Tolerances: bf16 stores the normalised rows, the feed-forward's output, their gr
 root mean square each, and the feed-forward's own 4e-3 (see its tests) for y and again for its gradients: sqrt(5 * 2.3^2 + 2 * 4^2) e-3 = 7.6e-3
 of the root mean square of each result at most.  Float32 parameters' gradients add up bf16 products: the same.  Float32 compute: 4e-5.
 """
+import threading
+
 import pytest
 import torch
 
@@ -231,3 +233,31 @@ def test_cpu_tensors_are_refused_while_recording():
         M.Transition(64, 2)(torch.zeros(3, 64))
     with pytest.raises(RuntimeError, match="CUDA"):
         M.LayerNorm(64)(torch.zeros(3, 64))
+
+
+def test_host_threads_that_share_a_stream():
+    """Their calls' launches mix on the stream; each thread has scratch memory of its own."""
+    c, hidden, n = 256, 1024, 1500
+    w_in, w_out = _randn(1, 2 * hidden, c, dtype=BF, scale=c ** -0.5), _randn(2, c, hidden, dtype=BF, scale=hidden ** -0.5)
+    ln = 1 + 0.1 * _randn(3, c)
+    data = [(_randn(10 + i, n, c, dtype=BF), _randn(20 + i, n, c, dtype=BF, scale=0.1)) for i in range(4)]
+    step = lambda x, dy: (F.gated_feed_forward(x, w_in, w_out), *F.gated_feed_forward_backward(dy, x, w_in, w_out), *F.layer_norm_backward(dy, x, ln))
+    want = [step(*d) for d in data]
+    torch.cuda.synchronize()
+    start, wrong, places = threading.Barrier(len(data)), [], []
+
+    def run(i):
+        start.wait()
+        places.append(F._call_workspace(data[i][0].device, 1 << 16).data_ptr())
+        for _ in range(40):
+            got = step(*data[i])
+            torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(data))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and len(set(places)) == len(data)

@@ -63,7 +63,7 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor)
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, rng, shared_dim):
-        if isinstance(rng, torch.Tensor):      # the caller may move it on before the backward pass
+        if isinstance(rng, torch.Tensor) and p:      # the caller may move it on before the backward pass
             rng = rng.clone()
             ctx.save_for_backward(rng)
             ctx.rng = None
@@ -77,8 +77,11 @@ class _Dropout(torch.autograd.Function):
     def backward(ctx, dy):
         dx = None
         if ctx.needs_input_grad[0]:
-            rng = ctx.saved_tensors[0] if ctx.rng is None else ctx.rng
-            dx = F.dropout(dy, ctx.p, rng, ctx.shared_dim).to(ctx.dtype)
+            if ctx.p:
+                dy_kept = F.dropout(dy, ctx.p, ctx.saved_tensors[0] if ctx.rng is None else ctx.rng, ctx.shared_dim)
+            else:
+                dy_kept = dy
+            dx = dy_kept.to(ctx.dtype)
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
 
 

@@ -83,6 +83,11 @@ def test_many_rows(rows, c, hidden):
     _check(*_case(rows, c, hidden, seed=5))
 
 
+@pytest.mark.parametrize("rows, c, hidden", [(7200, 128, 16384), (9600, 256, 16384), (1, 64, 65536), (3, 65536, 8), (200, 4096, 64)])
+def test_largest_widths(rows, c, hidden):
+    _check(*_case(rows, c, hidden))
+
+
 @pytest.mark.parametrize("rows", [7103, 7104, 7105, 7167, 7169, 7231, 7295, 7297, 9471, 9472, 9473, 9535, 9537, 9599, 9601, 18943, 18945, 19072, 19201, 37889])
 @pytest.mark.parametrize("c, hidden", [(128, 128), (256, 128)])
 def test_rows_around_the_tiles_of_many(rows, c, hidden):

@@ -261,3 +261,17 @@ def test_host_threads_that_share_a_stream():
     for t in threads:
         t.join()
     assert not wrong and len(set(places)) == len(data)
+
+
+@pytest.mark.parametrize("rng", [(1, 2), None], ids=["numbers", "device memory"])
+@pytest.mark.parametrize("dtypes", [(BF, BF), (F32, F32), (BF, F32)], ids=lambda d: "+".join(str(t)[6:] for t in d))
+def test_residual_sum_without_dropout(dtypes, rng):
+    """p = 0 adds, and its gradient goes to both sides as it is."""
+    x, res = (_randn(1 + i, 5, 64, dtype=t).requires_grad_() for i, t in enumerate(dtypes))
+    out = A.dropout(x, 0.0, torch.tensor([1, 2], device=DEV) if rng is None else rng, residual=res)
+    dy = _randn(3, 5, 64, dtype=dtypes[1])
+    out.backward(dy)
+    assert torch.equal(out, (x.float() + res.float()).to(dtypes[1]))
+    assert torch.equal(x.grad, dy.to(dtypes[0])) and torch.equal(res.grad, dy)
+    x.grad += 1                                            # neither gradient is the other's memory
+    assert torch.equal(res.grad, dy)

@@ -275,3 +275,38 @@ def test_residual_sum_without_dropout(dtypes, rng):
     assert torch.equal(x.grad, dy.to(dtypes[0])) and torch.equal(res.grad, dy)
     x.grad += 1                                            # neither gradient is the other's memory
     assert torch.equal(res.grad, dy)
+
+
+def test_captured_step_of_modules():
+    """Forward and backward pass of LayerNorm, Transition and Dropout in one graph: every replay gives the gradients of its inputs and its mask.
+    (No eager graph of the same parameters is alive while the step is captured: its accumulation nodes belong to another stream.)"""
+    c, p = 128, 0.25
+    mod, drop, norm = _transition(c), M.Dropout(p), M.LayerNorm(c).to(DEV)
+    params = [*mod.parameters(), *norm.parameters()]
+    z, dy = torch.zeros(3, 50, c, dtype=BF, device=DEV, requires_grad=True), torch.zeros(3, 50, c, dtype=BF, device=DEV)
+    rng = torch.tensor([9, 0], device=DEV)
+
+    def step(z, dy, rng):
+        out = norm(drop(mod(z), residual=z, rng=rng))
+        return (out.detach(), *torch.autograd.grad(out, [z, *params], dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(z, dy, rng)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(z, dy, rng)
+        rng[1] += 1
+    rng[1] = 0
+    for i in range(3):
+        with torch.no_grad():
+            z.copy_(_randn(30 + i, *z.shape))
+            dy.copy_(_randn(40 + i, *z.shape, scale=0.1))
+        graph.replay()
+        want = step(z.detach().clone().requires_grad_(), dy, torch.tensor([9, i], device=DEV))
+        assert int(rng[1]) == i + 1
+        for got, ref in zip(outs, want):
+            assert torch.equal(got, ref)

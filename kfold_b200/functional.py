@@ -113,8 +113,7 @@ def _affine(t: torch.Tensor | None) -> torch.Tensor | None:
 
 def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype=None) -> torch.Tensor:
     """LayerNorm over the last dim (model/primitives/normalization.py:61-91)."""
-    _require_cuda(x, weight, bias)
-    _same_device("layer_norm", x, weight, bias)
+    _one_gpu("layer_norm", x, weight, bias)
     c = x.shape[-1]
     for t in (weight, bias):
         if t is not None and t.numel() != c:
@@ -129,17 +128,19 @@ def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype=None)
     out = _dense_like(x, out_dtype)
     w, b = _affine(weight), _affine(bias)
     with L.on_device(x.device):
-        L.check(L.lib().kfb_layernorm(L.ptr(x2), L.ptr(out), L.ptr(w), L.ptr(b), rows, c, pitch, c, eps, L.dtype_code(x.dtype),
-                                      L.dtype_code(out.dtype), L.stream_ptr()))
+        L.check(L.lib().kfb_layernorm(x2.data_ptr(), out.data_ptr(), L.ptr(w), L.ptr(b), rows, c, pitch, c, eps, L.dtype_code(x.dtype),
+                                      L.dtype_code(out.dtype), L.raw_stream(x.get_device())))
     return out
 
 
-def _same_device(name: str, x: torch.Tensor, *ts: torch.Tensor | None) -> None:
+def _one_gpu(name: str, x: torch.Tensor, *ts: torch.Tensor | None) -> None:
     """A kernel follows every pointer on one GPU: refuse a mixture."""
     at = x.get_device()
     for t in ts:
         if t is not None and t.get_device() != at:
+            _require_cuda(x, t)
             raise ValueError(f"{name}: tensors on {x.device} and {t.device}")
+    _require_cuda(x)
 
 
 def _call_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
@@ -157,28 +158,28 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
 
     dx is of x's dtype, dweight and dbias float32 (None without a weight or where not asked for).  Any width up to 1024.  The row's
     statistics are taken from x again, nothing has to be kept from the forward pass; sums over the rows have a fixed order."""
-    _require_cuda(dy, x, weight)
-    _same_device("layer_norm_backward", dy, x, weight)
+    _one_gpu("layer_norm_backward", x, dy, weight)
     c = x.shape[-1]
     if dy.shape != x.shape or (weight is not None and weight.shape != (c,)):
         raise ValueError(f"layer_norm_backward: dy {tuple(dy.shape)}, weight {None if weight is None else tuple(weight.shape)} for x {tuple(x.shape)}")
     need_weight = need_weight and weight is not None
     xc, dc, w = _dense(x), _dense(dy), _affine(weight)
     dx = _dense_like(x)
-    dw = torch.empty(c, dtype=torch.float32, device=x.device) if need_weight else None
-    db = torch.empty(c, dtype=torch.float32, device=x.device) if need_bias else None
+    param = lambda: torch.empty(c, dtype=torch.float32, device=x.device) if w is None else torch.empty_like(w)
+    dw = param() if need_weight else None
+    db = param() if need_bias else None
     lib = L.lib()
     with L.on_device(x.device):
         ws = _call_workspace(x.device, lib.kfb_layernorm_bwd_workspace_bytes(c)) if need_weight or need_bias else None
-        L.check(lib.kfb_layernorm_bwd(L.ptr(dc), L.ptr(xc), L.ptr(w), L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), 0 if ws is None else ws.numel(),
-                                      x.numel() // c if c else 0, c, eps, L.dtype_code(dy.dtype), L.dtype_code(x.dtype), L.stream_ptr()))
+        L.check(lib.kfb_layernorm_bwd(dc.data_ptr(), xc.data_ptr(), L.ptr(w), dx.data_ptr(), L.ptr(dw), L.ptr(db), L.ptr(ws),
+                                      0 if ws is None else ws.numel(), x.numel() // c if c else 0, c, eps, L.dtype_code(dy.dtype),
+                                      L.dtype_code(x.dtype), L.raw_stream(x.get_device())))
     return dx, dw, db
 
 
 def _feed_forward_operands(name: str, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, dy: torch.Tensor | None = None):
     """(rows, channels, hidden channels, kernel's dtype code; x, dy and the weights as the kernels read them)."""
-    _require_cuda(x, w_in, w_out, dy)
-    _same_device(name, x, w_in, w_out, dy)
+    _one_gpu(name, x, w_in, w_out, dy)
     c = x.shape[-1] if x.dim() else 0
     hidden = w_out.shape[1] if w_out.dim() == 2 else 0
     if w_out.shape != (c, hidden) or w_in.shape != (2 * hidden, c) or c % 8 or hidden % 8 or not c or not hidden:
@@ -211,7 +212,8 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor)
     lib = L.lib()
     with L.on_device(x.device):
         ws = _call_workspace(x.device, lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, code, 0))
-        L.check(lib.kfb_feed_forward_fwd(L.ptr(xc), L.ptr(wi), L.ptr(wo), L.ptr(out), L.ptr(ws), ws.numel(), rows, c, hidden, code, L.stream_ptr()))
+        L.check(lib.kfb_feed_forward_fwd(xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(), rows, c, hidden, code,
+                                         L.raw_stream(x.get_device())))
     return out
 
 
@@ -226,8 +228,8 @@ def gated_feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.T
     lib = L.lib()
     with L.on_device(x.device):
         ws = _call_workspace(x.device, lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, code, 1))
-        L.check(lib.kfb_feed_forward_bwd(L.ptr(dc), L.ptr(xc), L.ptr(wi), L.ptr(wo), L.ptr(dx), L.ptr(dwi), L.ptr(dwo), L.ptr(ws), ws.numel(), rows, c,
-                                         hidden, code, L.dtype_code(w_in.dtype), L.stream_ptr()))
+        L.check(lib.kfb_feed_forward_bwd(dc.data_ptr(), xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), L.ptr(dx), L.ptr(dwi), L.ptr(dwo), ws.data_ptr(),
+                                         ws.numel(), rows, c, hidden, code, L.dtype_code(w_in.dtype), L.raw_stream(x.get_device())))
     return dx, dwi, dwo
 
 
@@ -244,16 +246,15 @@ def dropout(x: torch.Tensor, p: float, rng, shared_dim: int | None = None, resid
     shared_dim)`` with the same ``rng``, the residual's is dout.  ``shared_dim``: the mask has extent one along this dim of x, as row-wise
     (-3) and column-wise (-2) dropout of a pair tensor have it.  ``residual``, of x's shape, gives the result its dtype (float32 also for a
     bfloat16 x)."""
-    _require_cuda(x, residual)
-    _same_device("dropout", x, residual, rng if isinstance(rng, torch.Tensor) else None)
+    _one_gpu("dropout", x, residual)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout: p = {p}")
     if residual is not None and (residual.shape != x.shape or (residual.dtype != x.dtype and residual.dtype != torch.float32)):
         raise ValueError(f"dropout: residual {residual.dtype} {tuple(residual.shape)} for x {x.dtype} {tuple(x.shape)}")
     state, seed, offset = None, 0, 0
     if isinstance(rng, torch.Tensor):
-        if not rng.is_cuda or rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
-            raise ValueError("dropout: rng is a pair of integers or a contiguous int64 CUDA tensor of two")
+        if rng.get_device() != x.get_device() or rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
+            raise ValueError("dropout: rng is a pair of integers or a contiguous int64 tensor of two on x's device")
         state = rng
     else:
         seed, offset = int(rng[0]), int(rng[1])
@@ -261,16 +262,17 @@ def dropout(x: torch.Tensor, p: float, rng, shared_dim: int | None = None, resid
             raise ValueError(f"dropout: seed {seed} and offset {offset} are not in [0, 2^64)")
     outer, shared, inner = 1, 1, x.numel()
     if shared_dim is not None:
-        if not -x.dim() <= shared_dim < x.dim():
-            raise ValueError(f"dropout: dim {shared_dim} of x {tuple(x.shape)}")
-        d = shared_dim % x.dim()
-        outer, shared, inner = math.prod(x.shape[:d]), x.shape[d], math.prod(x.shape[d + 1:])
+        shape = x.shape
+        if not -len(shape) <= shared_dim < len(shape):
+            raise ValueError(f"dropout: dim {shared_dim} of x {tuple(shape)}")
+        d = shared_dim % len(shape)
+        outer, shared, inner = math.prod(shape[:d]), shape[d], math.prod(shape[d + 1:])
     xc, rc = _dense(x), None if residual is None else _dense(residual)
     out = _dense_like(x if residual is None else residual)
     scale = 1.0 / (1.0 - p) if p < 1.0 else 0.0
     with L.on_device(x.device):
-        L.check(L.lib().kfb_dropout(L.ptr(xc), L.ptr(rc), L.ptr(out), outer, shared, inner, int(p * 4294967296.0 + 0.5), scale, L.ptr(state),
-                                    _signed64(seed), _signed64(offset), L.dtype_code(x.dtype), L.dtype_code(out.dtype), L.stream_ptr()))
+        L.check(L.lib().kfb_dropout(xc.data_ptr(), L.ptr(rc), out.data_ptr(), outer, shared, inner, int(p * 4294967296.0 + 0.5), scale, L.ptr(state),
+                                    _signed64(seed), _signed64(offset), L.dtype_code(x.dtype), L.dtype_code(out.dtype), L.raw_stream(x.get_device())))
     return out
 
 

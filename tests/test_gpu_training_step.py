@@ -248,7 +248,7 @@ def test_host_threads_that_share_a_stream():
 
     def run(i):
         start.wait()
-        places.append(F._call_workspace(data[i][0].device, 1 << 16).data_ptr())
+        places.append(F._call_workspace(data[i][0].device, 1 << 16))      # (held, or a freed one's address comes again)
         for _ in range(40):
             got = step(*data[i])
             torch.cuda.current_stream().synchronize()
@@ -260,7 +260,7 @@ def test_host_threads_that_share_a_stream():
         t.start()
     for t in threads:
         t.join()
-    assert not wrong and len(set(places)) == len(data)
+    assert not wrong and len({t.data_ptr() for t in places}) == len(data)
 
 
 @pytest.mark.parametrize("rng", [(1, 2), None], ids=["numbers", "device memory"])

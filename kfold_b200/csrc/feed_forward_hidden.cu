@@ -8,7 +8,9 @@
 // shared memory for all chunks of a tile and only weights stream, 12 KB a CTA per 416 cycles of products; wider rows stream too.
 // Two S buffers of 192 columns: sixteen warps take a chunk's element-wise part while the next is multiplied.  (Eight in two groups that took the
 // chunks in turn, 32 channels at a time, waited out every latency: 3 960 cycles a chunk where its products are 1 664.)
-// What bounds it: at 128 channels the 6 bytes per row and hidden channel that it writes, at 256 that and the products alike.
+// What bounds it: at 128 channels the 6 bytes per row and hidden channel that it writes, at 256 that and the products alike.  147 456 rows of 512 hidden
+// channels, for the gradient: 107 us, 453 MB at 4.2 TB/s (writes alone reach 4), 64 without its stores.  Of 128 and 256 channels with many rows the
+// kernels that have dx too take its place; few rows: a unit is fewer chunks, so that they fill the device (331 rows of 384 channels: 10 us).
 #include "feed_forward_hidden.cuh"
 
 #include <mutex>
@@ -166,15 +168,15 @@ ffn_hidden_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         const int rs0 = rs;
         const uint32_t r_ph0 = r_ph;
         for (int c = 0; ok && c < n; ++c) {
-          ok = ptx::mbar_wait_hot(&s_free[s], s_ph, 525);
+          ok = ptx::mbar_wait(&s_free[s], s_ph, 525, ptx::kPolls);
           if (!ok) break;
           ptx::tc_fence_after_sync();
           const uint32_t d = tmem + s * kS;
           if (p.resident) { rs = rs0; r_ph = r_ph0; }
           const bool fresh_rows = !p.resident || c == 0, last_rows = !p.resident || c == n - 1;
           for (int kb = 0; kb < p.k_blocks; ++kb) {
-            if (fresh_rows) ok = ptx::mbar_wait_hot(&r_full[rs], r_ph, 526);
-            ok = ok && ptx::mbar_wait_hot(&w_full[st], ph, 527);
+            if (fresh_rows) ok = ptx::mbar_wait(&r_full[rs], r_ph, 526, ptx::kPolls);
+            ok = ok && ptx::mbar_wait(&w_full[st], ph, 527, ptx::kPolls);
             if (!ok) break;
             ptx::tc_fence_after_sync();
             const uint64_t xd = row_desc + rs * (kRowSlot >> 4), wd = w1_desc + st * (kWSlot >> 4), gd = g_desc + st * (kWSlot >> 4);

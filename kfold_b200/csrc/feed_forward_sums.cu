@@ -6,6 +6,7 @@
 // half of the columns and half of the channels.  (Products of 128 columns by 128 channels, each operand from shared memory, spend two fifths of their time
 // on reading the left one: 163 cycles for 256 x 16 values of it where its products are 128, 103 for 64.)  All operands lie across the contraction and are
 // read as they lie.
+// Measured: 147 456 rows of 1 024 hidden channels 177 us (141 at the measured burst rate; 905 MB take 138); 217 by products of 128 x 128.
 #include <mutex>
 
 #include "feed_forward_hidden.cuh"
@@ -105,7 +106,7 @@ ffn_sums_pair_kernel(const __grid_constant__ CUtensorMap tm_dab, const __grid_co
       uint32_t ph = 0;
       bool ok = true;
       for (int b = b0; b < b1; ++b) {
-        ok = ptx::mbar_wait_hot(&full[st], ph, 583);
+        ok = ptx::mbar_wait(&full[st], ph, 583, ptx::kPolls);
         if (!ok) break;
         ptx::tc_fence_after_sync();
         const uint64_t a = d0 + st * (kStage >> 4), bd = a + (2 * kAPart >> 4);

@@ -150,12 +150,12 @@ ffn_weights_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
       for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x, ++unit) {
         int t0;
         const int n = tiles_of(u, t0);
-        ok = ptx::mbar_wait_hot(w_full, unit & 1, 563);
+        ok = ptx::mbar_wait(w_full, unit & 1, 563, ptx::kPolls);
         for (int i = -1; ok && i < n; ++i) {
           const int g = round + i;                            // tile i of this unit, and the next one's slots
           const int x1 = 2 * ((g + 1) & 1), x0 = 2 * (g & 1);
           if (i + 1 < n) {
-            ok = ptx::mbar_wait_hot(s_free, (g & 1), 564) && ptx::mbar_wait_hot(&r_full[x1], ((g + 1) >> 1) & 1, 565);
+            ok = ptx::mbar_wait(s_free, (g & 1), 564, ptx::kPolls) && ptx::mbar_wait(&r_full[x1], ((g + 1) >> 1) & 1, 565, ptx::kPolls);
             if (!ok) break;
             ptx::tc_fence_after_sync();
 #pragma unroll
@@ -164,7 +164,7 @@ ffn_weights_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                               k > 0 ? 1u : 0u);
           }
           if (i + 1 < n) {
-            ok = ptx::mbar_wait_hot(&r_full[x1 + 1], ((g + 1) >> 1) & 1, 568);
+            ok = ptx::mbar_wait(&r_full[x1 + 1], ((g + 1) >> 1) & 1, 568, ptx::kPolls);
             if (!ok) break;
             ptx::tc_fence_after_sync();
 #pragma unroll
@@ -175,8 +175,8 @@ ffn_weights_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
             if (i + 2 == n) ptx::tc_commit(w_free);
           }
           if (i >= 0) {
-            if (i == 0) ok = ptx::mbar_wait_hot(o_free, (unit & 1) ^ 1, 566);
-            ok = ok && ptx::mbar_wait_hot(p_full, g & 1, 567);
+            if (i == 0) ok = ptx::mbar_wait(o_free, (unit & 1) ^ 1, 566, ptx::kPolls);
+            ok = ok && ptx::mbar_wait(p_full, g & 1, 567, ptx::kPolls);
             if (!ok) break;
             ptx::tc_fence_after_sync();
 #pragma unroll

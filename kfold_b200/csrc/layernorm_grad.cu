@@ -6,6 +6,9 @@
 // Split: a row is held by 8, 16 or 32 lanes, in 16-byte pieces where the width allows; a warp has enough rows in flight to cover the memory's
 // latency, keeps its lanes' shares of dw and db in registers from row to row, and a block leaves one row of partial sums.  A second kernel adds
 // those in the blocks' order, so that the result does not hang on which block was first: no atomics.
+//
+// Measured: 147 456 rows of 256 bf16 channels 42 us, 226 MB at 5.4 TB/s of the 6.5 that a copy has, and 5 for the second kernel.  The next rows' loads
+// have to stand before this step's stores, and the row sums of a step be interleaved: 74 us without.  49 152 rows of 505 channels 83 -> 44 us.
 #include <cuda_bf16.h>
 
 #include <mutex>

@@ -4,6 +4,9 @@
 // the products, four warps bring the accumulator from tensor memory to global memory.  Two CTAs share an SM, so that one's start and end lie
 // under the other's products.  An operand stored across k ([k][i]) is fetched as two boxes of 64 k by 64 i and read MN-major as it lies: the
 // gradients of weights contract over rows, and nothing is transposed for them.
+// What bounds it: reading the left operand from shared memory costs a product 40 cycles where its multiplications take 64, and short contractions their
+// start and end (some 3 us).  331 rows of 384 channels, 1 536 hidden ones: dx and the weights' gradients, 2.3 GFLOP, in one launch of 9 us.  Many rows of
+// the usual widths have kernels of their own.
 // fp32-accurate mode: three parts an operand, six products, x0 w0 in an accumulator of its own (the tensor core cuts off relative to the
 // accumulator at every step: the five small ones keep their small error apart).
 #include "matmul.cuh"

@@ -129,9 +129,10 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int co
 }
 
 // The wait of a thread that issues products: most of what it waits for is there, or about to be, and a suspended thread is slow to come back (a wait for a
-// barrier that has flipped costs it some 90 cycles this way, 230 to 400 otherwise; clock stamps).
-__device__ __forceinline__ bool mbar_wait_hot(uint64_t* bar, uint32_t parity, int code) {
-  for (int i = 0; i < 64; ++i)
+// barrier that has flipped costs it some 90 cycles this way, 230 to 400 otherwise; clock stamps).  It looks `polls` times before it sleeps.
+constexpr int kPolls = 64;
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int code, int polls) {
+  for (int i = 0; i < polls; ++i)
     if (mbar_test(bar, parity)) return true;
   return mbar_wait(bar, parity, code);
 }

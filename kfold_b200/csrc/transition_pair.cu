@@ -26,7 +26,7 @@
 // Measured (graph replays, three launches -> this): 589 824 rows of 128 channels 380 -> 191 us (its products: 141 at the measured burst rate; the
 // chain S - h - O through three S buffers is the rest), of 256 channels 976 -> 800 (at the power limit); 63 001 rows: 51 -> 28 and 111 -> 84.
 // With the next S behind the issue of the product before it they were 187, 749, 28 and 79.
-// The threads that issue products poll before they sleep (mbar_wait_hot): 589 824 rows 187 -> 180 and 643 -> 638 us on one device, in turn; as the
+// The threads that issue products poll before they sleep: 589 824 rows 187 -> 180 and 643 -> 638 us on one device, in turn; as the
 // gated feed-forward alone (RAW), 147 456 rows 54 -> 50 us of 128 channels (35 at the measured burst rate) and 164 -> 160 of 256 (141).
 #include <cuda_bf16.h>
 
@@ -208,16 +208,16 @@ transition_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       uint32_t par = 0, s_par = 1, a_par = 0;      // s_par: phase of v_free that the buffer's next S waits for (the first kS: none)
       bool ok = true;
       for (int it = 0; ok && it < my_tiles; ++it) {
-        ok = ptx::mbar_wait_hot(&a_norm[ab], a_par, 404) && ptx::mbar_wait_cluster(&a_peer[ab], a_par, 413);
+        ok = ptx::mbar_wait(&a_norm[ab], a_par, 404, ptx::kPolls) && ptx::mbar_wait_cluster(&a_peer[ab], a_par, 413);
         const uint64_t ad = a_desc + ab * (K::kABytes >> 4);
         for (int c = 0; ok && c < p.chunks; ++c) {
-          ok = ptx::mbar_wait_hot(&v_free[s1], s_par, 417);
+          ok = ptx::mbar_wait(&v_free[s1], s_par, 417, ptx::kPolls);
           if (!ok) break;
           ptx::tc_fence_after_sync();
           const uint32_t d = tmem_s + s1 * 128;
 #pragma unroll
           for (int u = 0; u < K::kUnits; ++u) {
-            ok = ptx::mbar_wait_hot(&full[slot], par, 403);
+            ok = ptx::mbar_wait(&full[slot], par, 403, ptx::kPolls);
             if (!ok) break;
             ptx::tc_fence_after_sync();
             const uint64_t wd = w_desc + static_cast<uint64_t>(slot * (kSlot >> 4));
@@ -246,9 +246,9 @@ transition_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       uint32_t par = 0;
       bool ok = true;
       for (int it = 0; ok && it < my_tiles; ++it) {
-        ok = ptx::mbar_wait_hot(o_empty, (it & 1) ^ 1, 405);
+        ok = ptx::mbar_wait(o_empty, (it & 1) ^ 1, 405, ptx::kPolls);
         for (int c = 0; ok && c < p.chunks; ++c) {
-          ok = ptx::mbar_wait_hot(&v_full[s2], par, 418) && ptx::mbar_wait_hot(&h_ready[s2], par, 406);
+          ok = ptx::mbar_wait(&v_full[s2], par, 418, ptx::kPolls) && ptx::mbar_wait(&h_ready[s2], par, 406, ptx::kPolls);
           if (!ok) break;
           ptx::tc_fence_after_sync();
 #pragma unroll

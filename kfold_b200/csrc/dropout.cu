@@ -5,10 +5,11 @@
 // key = seed, counter = (e / 4, offset), element e of the mask takes word e % 4 and is dropped when the word is below p 2^32.  So the mask hangs
 // on (seed, offset, element) alone: not on the launch shape, the type, or where the tensor lies.
 //
-// What bounds it: the generator, where every element draws.  Ten rounds are 20 wide multiplications and 20 three-way xors for four words; with the
-// comparisons, loads and conversions 24 instructions an element, and the integer pipe, which has the xors and comparisons, is the busiest (63 %; the issue
-// slots 65).  384 x 384 x 256 bf16 elements: 44 us with residual, where its 226 MB take 35, and 42 without, where they take 23.  (The comparison as a
-// multiply-add, to relieve that pipe: 90 us the two where they are 84; wide multiply-adds run at half the rate.)
+// What bounds it: HBM, but the generator is close where every element draws.  Ten rounds are 20 wide multiplications and 20 three-way xors for four words,
+// and the integer pipe, which has the xors and the comparisons, is the busiest: what else it had to do was taken from it (an element is added by an instruction
+// that runs or does not, instead of by a mask; 32-bit arithmetic inside a block).  384 x 384 x 256 bf16 elements: 35 us with residual, 226 MB at 6.5 TB/s
+// (a copy's rate), and 31.5 without, where HBM takes 23; they were 41.5 and 39.3 with masks.  (The comparison as a multiply-add: 90 us the two; wide
+// multiply-adds run at half the rate.)
 // A mask shared along one axis (rows or columns of the pair tensor) is computed once for the positions a thread walks along that axis, and HBM bounds it:
 // 768 x 768 x 128, columns, 130 us with residual and its gradient, 755 MB at 5.8 TB/s (a copy has 6.5).
 #include <cuda_bf16.h>
@@ -54,20 +55,23 @@ __host__ __device__ __forceinline__ void make_stream(unsigned long long seed, un
   d.a2_lo = static_cast<uint32_t>(a2);
 }
 
-__device__ __forceinline__ Words philox(unsigned long long block, const Stream& s) {
-  const uint32_t upper = static_cast<uint32_t>(block >> 32);
+// The second round's product that hangs on the block's upper half.
+struct Second {
+  uint32_t hi, lo;
+};
+__device__ __forceinline__ Second second_of(uint32_t upper, const Stream& s) {
+  if (upper == 0) return {s.a2_hi, s.a2_lo};
+  const unsigned long long a2 = static_cast<unsigned long long>(kM0) * (s.b1_hi ^ upper ^ s.key[0]);
+  return {static_cast<uint32_t>(a2 >> 32), static_cast<uint32_t>(a2)};
+}
+// The words of the block with this lower half.
+__device__ __forceinline__ Words philox(uint32_t lower, const Second& second, const Stream& s) {
   // the first two rounds
-  const unsigned long long a1 = static_cast<unsigned long long>(kM0) * static_cast<uint32_t>(block);
+  const unsigned long long a1 = static_cast<unsigned long long>(kM0) * lower;
   const uint32_t d2 = static_cast<uint32_t>(a1 >> 32) ^ s.offset_hi ^ s.key[1], d3 = static_cast<uint32_t>(a1);
-  uint32_t a2_hi = s.a2_hi, a2_lo = s.a2_lo;
-  if (upper != 0) {
-    const unsigned long long a2 = static_cast<unsigned long long>(kM0) * (s.b1_hi ^ upper ^ s.key[0]);
-    a2_hi = static_cast<uint32_t>(a2 >> 32);
-    a2_lo = static_cast<uint32_t>(a2);
-  }
   const unsigned long long b2 = static_cast<unsigned long long>(kM1) * d2;
   uint32_t c0 = static_cast<uint32_t>(b2 >> 32) ^ s.b1_lo ^ s.key[2], c1 = static_cast<uint32_t>(b2);
-  uint32_t c2 = a2_hi ^ d3 ^ s.key[3], c3 = a2_lo;
+  uint32_t c2 = second.hi ^ d3 ^ s.key[3], c3 = second.lo;
 #pragma unroll
   for (int i = 2; i < 10; ++i) {
     const unsigned long long a = static_cast<unsigned long long>(kM0) * c0, b = static_cast<unsigned long long>(kM1) * c2;
@@ -82,15 +86,13 @@ __device__ __forceinline__ Words philox(unsigned long long block, const Stream& 
 struct DropParams {
   const long long* rng;             // (seed, offset) in device memory, or null: `stream` is made of them
   Stream stream;
-  uint32_t cut;                     // kept: word > cut
-  int keep_all;                     // nothing is dropped
+  uint32_t cut;                     // kept: word >= cut
   float scale;
   long long outer, shared, inner;   // x is [outer][shared][inner], the mask [outer][inner]
   long long chunks, chunk;          // `shared` positions in `chunks` pieces of `chunk`
 };
 
-// V elements of x as they lie in memory, and the mask as words to and them with: an element that is dropped becomes a zero whatever it was, an
-// infinity or NaN too, at one instruction for two bf16 elements.
+// V elements as they lie in memory.
 template <typename TX, int V>
 struct Piece {
   static constexpr int kWords = V * sizeof(TX) < 4 ? 1 : V * static_cast<int>(sizeof(TX)) / 4;
@@ -127,84 +129,98 @@ __device__ __forceinline__ void values(const Piece<TX, V>& d, float (&v)[V]) {
   }
 }
 
-// The mask of elements e ... e + V - 1 (e a multiple of 4 unless V is 1).
-template <typename TX, int V>
-__device__ __forceinline__ void kept(const DropParams& p, const Stream& stream, long long e, Piece<TX, V>& m) {
-#pragma unroll
-  for (int i = 0; i < Piece<TX, V>::kWords; ++i) m.w[i] = 0;
+// The words of V elements from number `at` of block `lower` on: V / 4 blocks, or the one word of V = 1.
+template <int V>
+__device__ __forceinline__ void words(uint32_t lower, int at, const Second& second, const Stream& stream, uint32_t (&w)[V]) {
   if constexpr (V == 1) {
-    const Words r = philox(static_cast<unsigned long long>(e) >> 2, stream);
-    const int at = static_cast<int>(e & 3);
-    const uint32_t w = at == 0 ? r.w[0] : at == 1 ? r.w[1] : at == 2 ? r.w[2] : r.w[3];
-    m.w[0] = (w > p.cut) | p.keep_all ? 0xffffffffu : 0u;
+    const Words r = philox(lower, second, stream);
+    w[0] = at == 0 ? r.w[0] : at == 1 ? r.w[1] : at == 2 ? r.w[2] : r.w[3];
   } else {
 #pragma unroll
     for (int b = 0; b < V / 4; ++b) {
-      const Words r = philox((static_cast<unsigned long long>(e) >> 2) + b, stream);
+      const Words r = philox(lower + b, second, stream);      // (V elements start at a multiple of V: no carry into the upper half)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = 4 * b + i;
-        if constexpr (sizeof(TX) == 4) m.w[k] = r.w[i] > p.cut ? 0xffffffffu : 0u;
-        else m.w[k / 2] |= r.w[i] > p.cut ? (k & 1 ? 0xffff0000u : 0xffffu) : 0u;
-      }
-    }
-    if (p.keep_all) {
-#pragma unroll
-      for (int i = 0; i < Piece<TX, V>::kWords; ++i) m.w[i] = 0xffffffffu;
+      for (int i = 0; i < 4; ++i) w[4 * b + i] = r.w[i];
     }
   }
 }
 
-// U pieces, their loads before the first store: out may be x or resid, so the compiler keeps the order it is given.  mask(u): the piece's.
-template <int V, int U, bool RESID, typename TX, typename TR, typename Mask>
-__device__ __forceinline__ void apply(const TX* x, const TR* resid, TR* out, const long long (&at)[U], const bool (&live)[U], float scale, Mask mask) {
-  Piece<TX, V> v[U];
-  Piece<TR, V> r[U];
+// sum + (kept ? scale x : 0) and kept ? scale x : 0, as an instruction that runs or does not: no select, and an element that is dropped leaves nothing
+// behind whatever it was, an infinity or NaN too.
+__device__ __forceinline__ float add_kept(float sum, uint32_t word, uint32_t cut, float x, float scale) {
+  asm("{\n\t.reg .pred k;\n\tsetp.ge.u32 k, %1, %2;\n\t@k fma.rn.f32 %0, %3, %4, %0;\n\t}" : "+f"(sum) : "r"(word), "r"(cut), "f"(x), "f"(scale));
+  return sum;
+}
+__device__ __forceinline__ float kept(uint32_t word, uint32_t cut, float x, float scale) {
+  float f = 0.f;
+  asm("{\n\t.reg .pred k;\n\tsetp.ge.u32 k, %1, %2;\n\t@k mul.rn.f32 %0, %3, %4;\n\t}" : "+f"(f) : "r"(word), "r"(cut), "f"(x), "f"(scale));
+  return f;
+}
+
+// The words of a mask that serves many elements, as words to and x with as it lies in memory: one instruction for two bf16 elements.
+template <typename TX, int V>
+__device__ __forceinline__ void mask_of(const uint32_t (&w)[V], uint32_t cut, Piece<TX, V>& m) {
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (live[u]) {
-      load_piece<TX, V>(x + at[u], v[u]);
-      if (RESID) load_piece<TR, V>(resid + at[u], r[u]);
-    }
+  for (int i = 0; i < Piece<TX, V>::kWords; ++i) m.w[i] = 0;
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (live[u]) {
-      const Piece<TX, V> m = mask(u);
-#pragma unroll
-      for (int i = 0; i < Piece<TX, V>::kWords; ++i) v[u].w[i] &= m.w[i];
-      float f[V], add[V];
-      values<TX, V>(v[u], f);
-      if (RESID) values<TR, V>(r[u], add);
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = RESID ? fmaf(f[i], scale, add[i]) : f[i] * scale;
-      store_vec<V>(out + at[u], f);
-    }
+  for (int i = 0; i < V; ++i) {
+    if constexpr (sizeof(TX) == 4) m.w[i] = w[i] >= cut ? 0xffffffffu : 0u;
+    else m.w[i / 2] |= w[i] >= cut ? (i & 1 ? 0xffff0000u : 0xffffu) : 0u;
+  }
 }
 
 constexpr int kBlocksPerSm = 4;
+// Pieces at a time where every element draws, and the blocks (an SM) that walk them at most.  384 x 384 x 256 bf16: with residual 2 pieces 36.0 us by up to 64 blocks, 34.6 by
+// 24, 38 by 4 pieces; without 34.2 by 2 pieces, 31.5 by 4 and 64 blocks; float32 of 29.6 million elements without 39.8 and 36.2 (37.4 by 16 blocks).
+constexpr int pieces_of(bool resid) { return resid ? 2 : 4; }
+constexpr int blocks_of(bool resid) { return resid ? 24 : 64; }
 
-// Every element by itself: `inner` of them, a multiple of V.
+// Every element by itself: `inner` of them, a multiple of V.  U pieces at a time, their loads before the first store: out may be x or resid, so the
+// compiler keeps the order it is given.  A block's elements have the upper half of their counter in common, and all but the last block have every piece:
+// what is left for each element is 32-bit arithmetic.
 template <typename TX, typename TR, int V, bool RESID, bool STATE>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm) dropout_kernel(const TX* x, const TR* resid, TR* out, const DropParams p) {
-  constexpr int U = 2;
+  constexpr int U = pieces_of(RESID), kBlock = kThreads * U * V;
   grid_dependency_enter();
   Stream own;
   if (STATE) make_stream(static_cast<unsigned long long>(p.rng[0]), static_cast<unsigned long long>(p.rng[1]), own);
   const Stream& stream = STATE ? own : p.stream;
-  constexpr long long kBlock = static_cast<long long>(kThreads) * U * V;
-  for (long long base = blockIdx.x * kBlock; base < p.inner; base += gridDim.x * kBlock) {
-    long long at[U];
-    bool live[U];
+  const int first = static_cast<int>(threadIdx.x) * V;
+  for (long long base = static_cast<long long>(blockIdx.x) * kBlock; base < p.inner; base += static_cast<long long>(gridDim.x) * kBlock) {
+    const Second second = second_of(static_cast<uint32_t>(base >> 34), stream);
+    const uint32_t lower = static_cast<uint32_t>(base >> 2);
+    const int left = static_cast<int>(p.inner - base < kBlock ? p.inner - base : kBlock);
+    const TX* xb = x + base;
+    const TR* rb = RESID ? resid + base : nullptr;
+    TR* ob = out + base;
+    auto pieces = [&](auto whole) {
+      Piece<TX, V> v[U];
+      Piece<TR, V> r[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      at[u] = base + (u * kThreads + static_cast<int>(threadIdx.x)) * V;
-      live[u] = at[u] < p.inner;
-    }
-    apply<V, U, RESID>(x, resid, out, at, live, p.scale, [&](int u) {
-      Piece<TX, V> m;
-      kept<TX, V>(p, stream, at[u], m);
-      return m;
-    });
+      for (int u = 0; u < U; ++u) {
+        const int at = u * kThreads * V + first;
+        if (whole || at < left) {
+          load_piece<TX, V>(xb + at, v[u]);
+          if (RESID) load_piece<TR, V>(rb + at, r[u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = u * kThreads * V + first;
+        if (whole || at < left) {
+          uint32_t w[V];
+          words<V>(lower + (static_cast<uint32_t>(at) >> 2), at & 3, second, stream, w);
+          float f[V], o[V];
+          values<TX, V>(v[u], f);
+          if (RESID) values<TR, V>(r[u], o);
+#pragma unroll
+          for (int i = 0; i < V; ++i) o[i] = RESID ? add_kept(o[i], w[i], p.cut, f[i], p.scale) : kept(w[i], p.cut, f[i], p.scale);
+          store_vec<V>(ob + at, o);
+        }
+      }
+    };
+    if (left == kBlock) pieces(std::true_type());
+    else pieces(std::false_type());
   }
 }
 
@@ -221,21 +237,36 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) dropout_shared_kernel(
     const long long i = t % pieces * V, rest = t / pieces, o = rest / p.chunks, s0 = rest % p.chunks * p.chunk;
     // (a piece of the shared axis is short, or the threads are many: either way below 2^31 for what a GPU can hold)
     int left = static_cast<int>(s0 + p.chunk < p.shared ? p.chunk : p.shared - s0);
+    uint32_t w[V];
+    const unsigned long long e = static_cast<unsigned long long>(o * p.inner + i);
+    words<V>(static_cast<uint32_t>(e >> 2), static_cast<int>(e & 3), second_of(static_cast<uint32_t>(e >> 34), stream), stream, w);
     Piece<TX, V> m;
-    kept<TX, V>(p, stream, o * p.inner + i, m);
+    mask_of<TX, V>(w, p.cut, m);
     const long long first = (o * p.shared + s0) * p.inner + i;
     const TX* xs = x + first;
     const TR* rs = RESID ? resid + first : nullptr;
     TR* os = out + first;
     for (; left > 0; left -= U) {
-      long long at[U];
-      bool live[U];
+      Piece<TX, V> v[U];
+      Piece<TR, V> r[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        at[u] = u * p.inner;
-        live[u] = u < left;
-      }
-      apply<V, U, RESID>(xs, rs, os, at, live, p.scale, [&](int) { return m; });
+      for (int u = 0; u < U; ++u)
+        if (u < left) {
+          load_piece<TX, V>(xs + u * p.inner, v[u]);
+          if (RESID) load_piece<TR, V>(rs + u * p.inner, r[u]);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u < left) {
+#pragma unroll
+          for (int k = 0; k < Piece<TX, V>::kWords; ++k) v[u].w[k] &= m.w[k];
+          float f[V], add[V];
+          values<TX, V>(v[u], f);
+          if (RESID) values<TR, V>(r[u], add);
+#pragma unroll
+          for (int k = 0; k < V; ++k) f[k] = RESID ? fmaf(f[k], p.scale, add[k]) : f[k] * p.scale;
+          store_vec<V>(os + u * p.inner, f);
+        }
       xs += U * p.inner;
       if (RESID) rs += U * p.inner;
       os += U * p.inner;
@@ -249,8 +280,9 @@ int launch_state(cudaStream_t stream, const void* x, const void* resid, void* ou
   LaunchScope scope(stream, "dropout");
   if (p.shared == 1) {
     p.inner *= p.outer;
-    const long long blocks = (p.inner + 2ll * V * kThreads - 1) / (2ll * V * kThreads);
-    return launch_kernel(stream, dropout_kernel<TX, TR, V, RESID, STATE>, static_cast<unsigned>(blocks < sms * 64 ? blocks : sms * 64), kThreads, 0,
+    constexpr long long kBlock = static_cast<long long>(pieces_of(RESID)) * V * kThreads;
+    const long long blocks = (p.inner + kBlock - 1) / kBlock, most = sms * blocks_of(RESID);
+    return launch_kernel(stream, dropout_kernel<TX, TR, V, RESID, STATE>, static_cast<unsigned>(blocks < most ? blocks : most), kThreads, 0,
                          static_cast<const TX*>(x), static_cast<const TR*>(resid), static_cast<TR*>(out), p);
   }
   // pieces of the shared axis: as many as fill the device once
@@ -296,16 +328,21 @@ extern "C" KFB_API int kfb_dropout(const void* x, const void* residual, void* ou
                 "dropout: bad dtypes %d -> %d", x_dtype, out_dtype);
   if (outer == 0 || shared == 0 || inner == 0) return KFB_OK;
   KFB_CHECK_ARG(x != nullptr && out != nullptr, "dropout: null tensor");
+  cudaStream_t s = as_stream(stream);
+  if (drop_below == 1ll << 32) {        // nothing is kept: the kernels' comparison has no word for it
+    const size_t bytes = static_cast<size_t>(outer) * shared * inner * (out_dtype == KFB_FP32 ? 4 : 2);
+    if (residual == nullptr) KFB_CUDA(cudaMemsetAsync(out, 0, bytes, s));
+    else if (residual != out) KFB_CUDA(cudaMemcpyAsync(out, residual, bytes, cudaMemcpyDeviceToDevice, s));
+    return KFB_OK;
+  }
   DropParams d = {};
   d.rng = rng;
   make_stream(static_cast<unsigned long long>(seed), static_cast<unsigned long long>(offset), d.stream);
-  d.keep_all = drop_below == 0;
-  d.cut = drop_below == 0 ? 0u : static_cast<uint32_t>(drop_below - 1);
+  d.cut = static_cast<uint32_t>(drop_below);
   d.scale = scale;
   d.outer = outer;
   d.shared = shared;
   d.inner = inner;
-  cudaStream_t s = as_stream(stream);
   if (x_dtype == KFB_BF16)
     return out_dtype == KFB_BF16 ? dispatch<__nv_bfloat16, __nv_bfloat16>(s, x, residual, out, d) : dispatch<__nv_bfloat16, float>(s, x, residual, out, d);
   return dispatch<float, float>(s, x, residual, out, d);

@@ -14,8 +14,8 @@
 // enough; with P and dX it fills the tensor memory at 256 channels.  x and dy stay in shared memory for a tile; the next tile's come into L2 meanwhile, and
 // into the buffers as its slots fall free.
 //
-// Measured, 147 456 rows: 128 channels, 512 hidden, 84 us (59 at the measured burst rate of the products); a chunk takes 1 750 cycles, of which S is 750 and
-// dX 250, the rest the way S -> registers -> P -> dX, and a tile's end 2 200.  256 channels, 1 024 hidden, kept: 345 us, 905 MB written (3.3 TB/s with
+// Measured, 147 456 rows: 128 channels, 512 hidden, 84 us (59 at the measured burst rate of the products); a chunk takes 1 750 cycles, of which S is 800 and
+// dX 500, the rest the way from S into registers and back to the thread that issues the next (polling there changes nothing), and a tile's end 2 200.  256 channels, 1 024 hidden, kept: 345 us, 905 MB written (3.3 TB/s with
 // what is read, where writes alone reach 4; 294 without them, products 236).
 #include <mutex>
 

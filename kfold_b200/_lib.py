@@ -210,6 +210,10 @@ def raw_stream(index: int | None = None) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
+# (what torch.cuda.current_device() asks once CUDA is initialised, which a tensor on a GPU says it is)
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def stream_ptr():
     return raw_stream()
 
@@ -239,12 +243,14 @@ class on_device:
         return False
 
 
+_DTYPE_CODES = {torch.bfloat16: KFB_BF16, torch.float32: KFB_FP32}
+
+
 def dtype_code(dt: torch.dtype) -> int:
-    if dt == torch.bfloat16:
-        return KFB_BF16
-    if dt == torch.float32:
-        return KFB_FP32
-    raise ValueError(f"kfold_b200 supports bfloat16 and float32 activations, got {dt}")
+    code = _DTYPE_CODES.get(dt)
+    if code is None:
+        raise ValueError(f"kfold_b200 supports bfloat16 and float32 activations, got {dt}")
+    return code
 
 
 def device_status() -> int:

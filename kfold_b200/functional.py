@@ -8,6 +8,7 @@ and the extension must be built.
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 from threading import get_ident
 
 import torch
@@ -111,13 +112,16 @@ def _affine(t: torch.Tensor | None) -> torch.Tensor | None:
     return t.detach().float().contiguous()
 
 
+# The training calls are short: what they ask torch for is asked once, and another current device than x's is dealt with by calling again.
 def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype=None) -> torch.Tensor:
     """LayerNorm over the last dim (model/primitives/normalization.py:61-91)."""
-    _one_gpu("layer_norm", x, weight, bias)
+    at = _one_gpu("layer_norm", x, weight, bias)
+    if at != L.current_device():
+        with L.on_device(x.device):
+            return layer_norm(x, weight, bias, eps, out_dtype)
     c = x.shape[-1]
-    for t in (weight, bias):
-        if t is not None and t.numel() != c:
-            raise ValueError(f"layer_norm: weight or bias {tuple(t.shape)} for x {tuple(x.shape)}")
+    if (weight is not None and weight.numel() != c) or (bias is not None and bias.numel() != c):
+        raise ValueError(f"layer_norm: {'weight' if weight is not None and weight.numel() != c else 'bias'} of another width than x {tuple(x.shape)}")
     if x.is_contiguous():
         x2, rows, pitch = x, x.numel() // c if c else 0, c
     else:
@@ -127,20 +131,21 @@ def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype=None)
         rows, pitch = x2.shape[0], x2.stride(0)
     out = _dense_like(x, out_dtype)
     w, b = _affine(weight), _affine(bias)
-    with L.on_device(x.device):
-        L.check(L.lib().kfb_layernorm(x2.data_ptr(), out.data_ptr(), L.ptr(w), L.ptr(b), rows, c, pitch, c, eps, L.dtype_code(x.dtype),
-                                      L.dtype_code(out.dtype), L.raw_stream(x.get_device())))
+    L.check(L.lib().kfb_layernorm(x2.data_ptr(), out.data_ptr(), L.ptr(w), L.ptr(b), rows, c, pitch, c, eps, L.dtype_code(x.dtype),
+                                  L.dtype_code(out.dtype), L.raw_stream(at)))
     return out
 
 
-def _one_gpu(name: str, x: torch.Tensor, *ts: torch.Tensor | None) -> None:
-    """A kernel follows every pointer on one GPU: refuse a mixture."""
+def _one_gpu(name: str, x: torch.Tensor, *ts: torch.Tensor | None) -> int:
+    """The number of the GPU that all of them are on: a kernel follows every pointer there, so a mixture is refused."""
     at = x.get_device()
+    if at < 0:
+        _require_cuda(x)
     for t in ts:
         if t is not None and t.get_device() != at:
-            _require_cuda(x, t)
+            _require_cuda(t)
             raise ValueError(f"{name}: tensors on {x.device} and {t.device}")
-    _require_cuda(x)
+    return at
 
 
 def _call_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
@@ -158,10 +163,14 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
 
     dx is of x's dtype, dweight and dbias float32 (None without a weight or where not asked for).  Any width up to 1024.  The row's
     statistics are taken from x again, nothing has to be kept from the forward pass; sums over the rows have a fixed order."""
-    _one_gpu("layer_norm_backward", x, dy, weight)
-    c = x.shape[-1]
-    if dy.shape != x.shape or (weight is not None and weight.shape != (c,)):
-        raise ValueError(f"layer_norm_backward: dy {tuple(dy.shape)}, weight {None if weight is None else tuple(weight.shape)} for x {tuple(x.shape)}")
+    at = _one_gpu("layer_norm_backward", x, dy, weight)
+    if at != L.current_device():
+        with L.on_device(x.device):
+            return layer_norm_backward(dy, x, weight, eps, need_weight, need_bias)
+    shape = x.shape
+    c = shape[-1]
+    if dy.shape != shape or (weight is not None and weight.shape != (c,)):
+        raise ValueError(f"layer_norm_backward: dy {tuple(dy.shape)}, weight {None if weight is None else tuple(weight.shape)} for x {tuple(shape)}")
     need_weight = need_weight and weight is not None
     xc, dc, w = _dense(x), _dense(dy), _affine(weight)
     dx = _dense_like(x)
@@ -169,35 +178,45 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
     dw = param() if need_weight else None
     db = param() if need_bias else None
     lib = L.lib()
-    with L.on_device(x.device):
-        ws = _call_workspace(x.device, lib.kfb_layernorm_bwd_workspace_bytes(c)) if need_weight or need_bias else None
-        L.check(lib.kfb_layernorm_bwd(dc.data_ptr(), xc.data_ptr(), L.ptr(w), dx.data_ptr(), L.ptr(dw), L.ptr(db), L.ptr(ws),
-                                      0 if ws is None else ws.numel(), x.numel() // c if c else 0, c, eps, L.dtype_code(dy.dtype),
-                                      L.dtype_code(x.dtype), L.raw_stream(x.get_device())))
+    ws, size = None, 0
+    if need_weight or need_bias:
+        ws = _call_workspace(x.device, lib.kfb_layernorm_bwd_workspace_bytes(c))
+        size = ws.numel()
+    L.check(lib.kfb_layernorm_bwd(dc.data_ptr(), xc.data_ptr(), L.ptr(w), dx.data_ptr(), L.ptr(dw), L.ptr(db), L.ptr(ws), size,
+                                  x.numel() // c if c else 0, c, eps, L.dtype_code(dy.dtype), L.dtype_code(x.dtype), L.raw_stream(at)))
     return dx, dw, db
 
 
 def _feed_forward_operands(name: str, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, dy: torch.Tensor | None = None):
     """(rows, channels, hidden channels, kernel's dtype code; x, dy and the weights as the kernels read them)."""
-    _one_gpu(name, x, w_in, w_out, dy)
-    c = x.shape[-1] if x.dim() else 0
+    shape = x.shape
+    c = shape[-1] if shape else 0
     hidden = w_out.shape[1] if w_out.dim() == 2 else 0
     if w_out.shape != (c, hidden) or w_in.shape != (2 * hidden, c) or c % 8 or hidden % 8 or not c or not hidden:
-        raise ValueError(f"{name}: w_in {tuple(w_in.shape)}, w_out {tuple(w_out.shape)} for x {tuple(x.shape)} (channels multiples of 8)")
-    dt = x.dtype
-    if dt not in (torch.bfloat16, torch.float32) or (dy is not None and (dy.dtype != dt or dy.shape != x.shape)):
-        raise ValueError(f"{name}: x {dt} {tuple(x.shape)}" + ("" if dy is None else f", dy {dy.dtype} {tuple(dy.shape)}"))
-    if w_in.dtype != w_out.dtype or w_in.dtype not in (dt, torch.float32):
-        raise ValueError(f"{name}: weights {w_in.dtype} and {w_out.dtype} for x {dt}")
-    code = L.KFB_BF16 if dt == torch.bfloat16 else L.KFB_FP32_PRECISE
-    return x.numel() // c, c, hidden, code, _operand(x, dt), None if dy is None else _operand(dy, dt), _operand(w_in, dt), _operand(w_out, dt)
+        raise ValueError(f"{name}: w_in {tuple(w_in.shape)}, w_out {tuple(w_out.shape)} for x {tuple(shape)} (channels multiples of 8)")
+    dt, wt = x.dtype, w_in.dtype
+    if dt not in _FEED_FORWARD_CODES or (dy is not None and (dy.dtype != dt or dy.shape != shape)):
+        raise ValueError(f"{name}: x {dt} {tuple(shape)}" + ("" if dy is None else f", dy {dy.dtype} {tuple(dy.shape)}"))
+    if w_out.dtype != wt or (wt != dt and wt != torch.float32):
+        raise ValueError(f"{name}: weights {wt} and {w_out.dtype} for x {dt}")
+    return (x.numel() // c, c, hidden, _FEED_FORWARD_CODES[dt], _operand(x, dt), None if dy is None else _operand(dy, dt), _operand(w_in, dt),
+            _operand(w_out, dt))
+
+
+_FEED_FORWARD_CODES = {torch.bfloat16: L.KFB_BF16, torch.float32: L.KFB_FP32_PRECISE}
+
+
+@lru_cache(maxsize=1024)
+def _feed_forward_bytes(at: int, *sizes: int) -> int:
+    """Scratch of a call on GPU `at`, which is current."""
+    return L.lib().kfb_feed_forward_workspace_bytes(*sizes)
 
 
 def _operand(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """`t` dense, of `dtype`, starting on a 16-byte boundary."""
-    if t.dtype != dtype:
-        t = t.detach().to(dtype)
-    t = _dense(t)
+    if t.dtype == dtype and t.is_contiguous() and not t.data_ptr() & 15:
+        return t
+    t = _dense(t.detach().to(dtype))
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -207,13 +226,15 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor)
 
     x (..., C) bfloat16 (tensor-core arithmetic, float32 sums) or float32 (the fp32-accurate mode); the weights of x's dtype, or float32
     parameters that are rounded to it here.  C and hidden multiples of 8."""
+    at = _one_gpu("gated_feed_forward", x, w_in, w_out)
+    if at != L.current_device():
+        with L.on_device(x.device):
+            return gated_feed_forward(x, w_in, w_out)
     rows, c, hidden, code, xc, _, wi, wo = _feed_forward_operands("gated_feed_forward", x, w_in, w_out)
     out = _dense_like(x)
-    lib = L.lib()
-    with L.on_device(x.device):
-        ws = _call_workspace(x.device, lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, code, 0))
-        L.check(lib.kfb_feed_forward_fwd(xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(), rows, c, hidden, code,
-                                         L.raw_stream(x.get_device())))
+    ws = _call_workspace(x.device, _feed_forward_bytes(at, rows, c, hidden, code, 0))
+    L.check(L.lib().kfb_feed_forward_fwd(xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(), rows, c, hidden, code,
+                                         L.raw_stream(at)))
     return out
 
 
@@ -221,15 +242,17 @@ def gated_feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.T
                                 need_w_in: bool = True, need_w_out: bool = True):
     """Gradient of ``gated_feed_forward``: (dx, dw_in, dw_out) from dy, of x's shape and dtype; None where not asked for.  The weights'
     gradients have the weights' dtype (float32 sums either way).  The hidden channels are computed again, nothing has to be kept."""
+    at = _one_gpu("gated_feed_forward_backward", x, w_in, w_out, dy)
+    if at != L.current_device():
+        with L.on_device(x.device):
+            return gated_feed_forward_backward(dy, x, w_in, w_out, need_x, need_w_in, need_w_out)
     rows, c, hidden, code, xc, dc, wi, wo = _feed_forward_operands("gated_feed_forward_backward", x, w_in, w_out, dy)
     dx = _dense_like(x) if need_x else None
     dwi = _dense_like(w_in) if need_w_in else None
     dwo = _dense_like(w_out) if need_w_out else None
-    lib = L.lib()
-    with L.on_device(x.device):
-        ws = _call_workspace(x.device, lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, code, 1))
-        L.check(lib.kfb_feed_forward_bwd(dc.data_ptr(), xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), L.ptr(dx), L.ptr(dwi), L.ptr(dwo), ws.data_ptr(),
-                                         ws.numel(), rows, c, hidden, code, L.dtype_code(w_in.dtype), L.raw_stream(x.get_device())))
+    ws = _call_workspace(x.device, _feed_forward_bytes(at, rows, c, hidden, code, 1))
+    L.check(L.lib().kfb_feed_forward_bwd(dc.data_ptr(), xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), L.ptr(dx), L.ptr(dwi), L.ptr(dwo), ws.data_ptr(),
+                                         ws.numel(), rows, c, hidden, code, L.dtype_code(w_in.dtype), L.raw_stream(at)))
     return dx, dwi, dwo
 
 
@@ -246,14 +269,17 @@ def dropout(x: torch.Tensor, p: float, rng, shared_dim: int | None = None, resid
     shared_dim)`` with the same ``rng``, the residual's is dout.  ``shared_dim``: the mask has extent one along this dim of x, as row-wise
     (-3) and column-wise (-2) dropout of a pair tensor have it.  ``residual``, of x's shape, gives the result its dtype (float32 also for a
     bfloat16 x)."""
-    _one_gpu("dropout", x, residual)
+    at = _one_gpu("dropout", x, residual)
+    if at != L.current_device():
+        with L.on_device(x.device):
+            return dropout(x, p, rng, shared_dim, residual)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout: p = {p}")
     if residual is not None and (residual.shape != x.shape or (residual.dtype != x.dtype and residual.dtype != torch.float32)):
         raise ValueError(f"dropout: residual {residual.dtype} {tuple(residual.shape)} for x {x.dtype} {tuple(x.shape)}")
     state, seed, offset = None, 0, 0
     if isinstance(rng, torch.Tensor):
-        if rng.get_device() != x.get_device() or rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
+        if rng.get_device() != at or rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
             raise ValueError("dropout: rng is a pair of integers or a contiguous int64 tensor of two on x's device")
         state = rng
     else:
@@ -270,9 +296,8 @@ def dropout(x: torch.Tensor, p: float, rng, shared_dim: int | None = None, resid
     xc, rc = _dense(x), None if residual is None else _dense(residual)
     out = _dense_like(x if residual is None else residual)
     scale = 1.0 / (1.0 - p) if p < 1.0 else 0.0
-    with L.on_device(x.device):
-        L.check(L.lib().kfb_dropout(xc.data_ptr(), L.ptr(rc), out.data_ptr(), outer, shared, inner, int(p * 4294967296.0 + 0.5), scale, L.ptr(state),
-                                    _signed64(seed), _signed64(offset), L.dtype_code(x.dtype), L.dtype_code(out.dtype), L.raw_stream(x.get_device())))
+    L.check(L.lib().kfb_dropout(xc.data_ptr(), L.ptr(rc), out.data_ptr(), outer, shared, inner, int(p * 4294967296.0 + 0.5), scale, L.ptr(state),
+                                _signed64(seed), _signed64(offset), L.dtype_code(x.dtype), L.dtype_code(out.dtype), L.raw_stream(at)))
     return out
 
 

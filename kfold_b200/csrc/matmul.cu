@@ -259,17 +259,6 @@ __global__ void __launch_bounds__(256) split_planes_kernel(const float* x, __nv_
 
 }  // namespace
 
-int matmul_splits(int m, int n, long long k, int most) {
-  const long long tiles = static_cast<long long>(cdiv(m, kTile)) * cdiv(n, kTile), blocks = (k + kK - 1) / kK;
-  long long want = 2ll * sm_count() / tiles;
-  // (a piece of less than six blocks is start and end only: 331 rows of 384 channels and 1 536 hidden ones are fastest in one piece)
-  if (want > blocks / 6) want = blocks / 6;
-  if (want > most) want = most;
-  if (want < 1) want = 1;
-  const long long per = (blocks + want - 1) / want;
-  return static_cast<int>((blocks + per - 1) / per);
-}
-
 int launch_matmuls(cudaStream_t stream, const MatmulArgs* list, int count, const char* tag) {
   KFB_CHECK_ARG(count >= 1 && count <= kMostMatmuls, "matmul: %d products", count);
   MmBatch batch = {};

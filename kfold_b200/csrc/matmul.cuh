@@ -24,7 +24,7 @@ struct MatmulArgs {
   void* d;               // [m][ld_d], bf16 or fp32
   long long ld_d;
   int out_fp32;
-  int splits;            // fp32 D only: k in this many pieces, piece s into D + s * plane_d (matmul_splits gives a count that leaves none empty)
+  int splits;            // fp32 D only: k in this many pieces, piece s into D + s * plane_d (none of them empty)
   long long plane_d;
   int accumulate;        // fp32 D only: add to what D holds
   int precise;           // operands are three bf16 parts each
@@ -33,9 +33,6 @@ static constexpr int kMostMatmuls = 3;
 // Up to kMostMatmuls products in one launch, all of them precise or none.
 int launch_matmuls(cudaStream_t stream, const MatmulArgs* list, int count, const char* tag);
 inline int launch_matmul(cudaStream_t stream, const MatmulArgs& p, const char* tag) { return launch_matmuls(stream, &p, 1, tag); }
-
-// How many pieces (at most `most`) k is best cut into so that the tiles of an m x n product fill the device, none of them empty.
-int matmul_splits(int m, int n, long long k, int most);
 
 // out[i] = sum over s of planes[s * plane + i], i < n, in the order of s; bf16 or fp32.  Up to kMostMatmuls of them in one launch.
 struct PlaneSum {

@@ -16,8 +16,6 @@
 namespace kfb {
 namespace {
 
-constexpr int kMostPlanes = 64;
-
 // The widths that the sizes below are computed for without leaving their range.
 bool widths_ok(int c, int hidden) { return c > 0 && c % 8 == 0 && hidden > 0 && hidden % 8 == 0 && c <= 65536 && hidden <= 65536; }
 
@@ -90,22 +88,73 @@ bool nothing_kept(long long rows, int c, int hidden, int precise) {
 // 95 and 91, 20 000 171 and 159.)
 bool many_rows(long long rows) { return rows >= 64ll * sm_count(); }
 bool sums_kernel(long long piece, int c, int hidden, int precise) { return many_rows(piece) && one_kernel(c, hidden, precise) && ffn_sums_ok(c, hidden); }
-int planes_in(long long piece, int c, int hidden, int precise) {
-  return sums_kernel(piece, c, hidden, precise) ? ffn_sums_planes(piece, hidden) : matmul_splits(2 * hidden, c, piece, kMostPlanes);
+
+// How the products of a gradient that share a launch are cut along their contractions: dx (`dx_tiles` tiles of dx_k blocks of 64) and the weights' gradients
+// (`w_tiles` of w_k).  Pieces fill the device, but each starts and ends, and writes a float32 plane that is read again.  So the cheapest of these counts by
+// the time that a launch takes: its blocks, side by side on an SM, two where they fit; waves of them; planes; the launch that adds them up.  The four
+// rates are fitted to 2 300 launches (50 ... 20 000 rows of 64 ... 768 channels): on average 2 % longer than the best count of each, 9 % at most.  Each product
+// cut as if it had the device to itself was 21 % longer: 3 000 rows of 384 channels 59 us for the whole gradient, 36 by these (uncut), 4 000 of 256
+// 46 and 34, 2 000 of 768 90 and 77, 331 of 384 17 and 18.
+struct Cuts {
+  int dx, w;
+};
+Cuts best_cuts(int dx_tiles, int dx_k, bool cut_dx, int w_tiles, int w_k, int precise) {
+  static constexpr int kDx[] = {1, 2, 4, 8}, kW[] = {1, 2, 3, 4, 8, 16, 32, 64}, kLeast = 4;      // (a piece has four blocks at least)
+  const float sms = static_cast<float>(sm_count()), at_once = precise ? 1.f : 2.f;      // (the fp32-accurate mode's blocks fill an SM, and take six products for one)
+  const float per_block = precise ? 0.7f : 0.117f, per_wave = 4.7f, per_plane = 0.0205f, per_sum = 1.3f;      // us
+  Cuts best = {1, 1};
+  float least = 0.f;
+  for (int i = 0; i < (cut_dx ? 4 : 1); ++i) {
+    if (i > 0 && dx_k < kDx[i] * kLeast) break;
+    const int dx_len = cdiv(dx_k, kDx[i]), dx_n = cdiv(dx_k, dx_len);
+    for (int j = 0; j < 8; ++j) {
+      if (j > 0 && w_k < kW[j] * kLeast) break;
+      const int w_len = cdiv(w_k, kW[j]), w_n = cdiv(w_k, w_len);
+      const float d = static_cast<float>(dx_tiles) * dx_n, w = static_cast<float>(w_tiles) * w_n, n = d + w;
+      const float longest = static_cast<float>(dx_tiles > 0 && dx_len > w_len ? dx_len : w_len);
+      const float planes = (dx_n > 1 ? d : 0.f) + (w_n > 1 ? w : 0.f);
+      const float share = (d * dx_len + w * w_len) / sms, side = n / sms < 1.f ? 1.f : n / sms < at_once ? n / sms : at_once;
+      const float waves = n / (at_once * sms);
+      const float t = per_block * (share > longest * side ? share : longest * side) + per_wave * (waves > 1.f ? waves : 1.f) + per_plane * planes +
+                      (planes > 0.f ? per_sum : 0.f);
+      if ((i == 0 && j == 0) || t < least) {
+        least = t;
+        best = {dx_n, w_n};
+      }
+    }
+  }
+  return best;
 }
-int planes_out(long long piece, int c, int hidden, int precise) {
-  return sums_kernel(piece, c, hidden, precise) ? ffn_sums_planes(piece, hidden) : matmul_splits(c, hidden, piece, kMostPlanes);
+// `most` pieces of `blocks`, fewer where some would be empty.
+int pieces_of(int blocks, int most) { return cdiv(blocks, cdiv(blocks, most < blocks ? most : blocks)); }
+
+// What the gradient of these sizes does, whoever asks for which of its results.
+struct Plan {
+  long long piece;       // rows
+  bool one, sums_by_pair;
+  bool dx_here;          // dx by the launch of the weights' gradients (few rows), or by the library's own product for operands along k
+  int in, out, dx;       // float32 planes of dw_in and dw_out (1: none, where the rows come in one piece), and of dx
+};
+Plan plan_of(long long rows, int c, int hidden, int precise) {
+  Plan p = {};
+  p.one = one_kernel(c, hidden, precise);
+  p.piece = piece_rows(rows, c, hidden, precise, 1, p.one);
+  p.sums_by_pair = sums_kernel(p.piece, c, hidden, precise);
+  const bool single = rows <= p.piece;
+  const long long dx_tiles = static_cast<long long>(cdiv(static_cast<int>(p.piece), 128)) * cdiv(c, 128);
+  p.dx_here = precise || (single && dx_tiles < 2 * sm_count());
+  const int w_tiles = cdiv(c, 128) * (cdiv(2 * hidden, 128) + cdiv(hidden, 128));
+  const Cuts cuts = best_cuts(p.dx_here ? static_cast<int>(dx_tiles) : 0, cdiv(2 * hidden, 64), p.dx_here && single, p.sums_by_pair ? 0 : w_tiles,
+                              p.sums_by_pair ? 1 : cdiv(static_cast<int>(p.piece), 64), precise);
+  p.in = p.out = p.sums_by_pair ? ffn_sums_planes(p.piece, hidden) : cuts.w;
+  p.dx = cuts.dx;
+  return p;
 }
 
-// Pieces of the hidden channels of dx = [da, db] [Wa; Wb] where the rows come in one piece and their tiles do not fill the device (1 elsewhere).
-int planes_dx(long long rows, long long piece, int c, int hidden) {
-  return rows > piece ? 1 : matmul_splits(static_cast<int>(rows), c, 2ll * hidden, 16);
-}
-
-size_t carve(FfnWs& w, void* base, long long rows, int c, int hidden, int precise, int backward) {
+size_t carve(FfnWs& w, void* base, long long rows, int c, int hidden, int precise, const Plan* backward) {
   Carver cv(base);
   const bool one = one_kernel(c, hidden, precise);
-  const long long piece = piece_rows(rows, c, hidden, precise, backward, one);
+  const long long piece = backward ? backward->piece : piece_rows(rows, c, hidden, precise, 0, one);
   const size_t r = static_cast<size_t>(piece), parts = precise ? 3 : 1, cc = c, hh = hidden;
   w = {};
   if (backward && nothing_kept(rows, c, hidden, precise)) {
@@ -126,10 +175,9 @@ size_t carve(FfnWs& w, void* base, long long rows, int c, int hidden, int precis
     if (!one) w.dh = cv.take<float>(r * hh);
     if (!precise) w.wi_t = cv.take<__nv_bfloat16>(2 * hh * cc);
     w.dab = cv.take<__nv_bfloat16>(parts * r * 2 * hh);
-    w.pl_in = cv.take<float>(planes_in(piece, c, hidden, precise) * 2 * hh * cc);
-    w.pl_out = cv.take<float>(planes_out(piece, c, hidden, precise) * hh * cc);
-    const int dx_planes = planes_dx(rows, piece, c, hidden);
-    if (dx_planes > 1) w.pl_dx = cv.take<float>(dx_planes * r * cc);
+    w.pl_in = cv.take<float>(backward->in * 2 * hh * cc);
+    w.pl_out = cv.take<float>(backward->out * hh * cc);
+    if (backward->dx > 1) w.pl_dx = cv.take<float>(backward->dx * r * cc);
   }
   return cv.off;
 }
@@ -195,8 +243,10 @@ extern "C" {
 
 KFB_API size_t kfb_feed_forward_workspace_bytes(long long rows, int c, int hidden, int dtype, int backward) {
   if (rows < 1 || !widths_ok(c, hidden)) return 0;
+  const int precise = dtype == KFB_FP32_PRECISE;
+  const Plan plan = backward ? plan_of(rows, c, hidden, precise) : Plan();
   FfnWs w;
-  return carve(w, nullptr, rows, c, hidden, dtype == KFB_FP32_PRECISE, backward);
+  return carve(w, nullptr, rows, c, hidden, precise, backward ? &plan : nullptr);
 }
 
 KFB_API int kfb_feed_forward_fwd(const void* x, const void* w_in, const void* w_out, void* out, void* workspace, size_t workspace_bytes,
@@ -211,7 +261,7 @@ KFB_API int kfb_feed_forward_fwd(const void* x, const void* w_in, const void* w_
   if (!precise && feed_forward_pair_ok(rows, c, hidden) && transition_pair_is_faster(rows, c, hidden))
     return launch_feed_forward_pair(s, x, w_in, w_out, out, rows, c, hidden);
   FfnWs w;
-  carve(w, workspace, rows, c, hidden, precise, 0);
+  carve(w, workspace, rows, c, hidden, precise, nullptr);
   const long long wi_n = 2ll * hidden * c, wo_n = static_cast<long long>(hidden) * c;
   if (precise) {
     KFB_TRY(launch_split_planes(s, static_cast<const float*>(w_in), w.wi3, wi_n, wi_n));
@@ -259,10 +309,12 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
     return KFB_OK;
   }
   KFB_CHECK_ARG(dy && x && w_in && w_out, "feed_forward_bwd: null tensor");
-  KFB_TRY(check("feed_forward_bwd", workspace, workspace_bytes, kfb_feed_forward_workspace_bytes(rows, c, hidden, dtype, 1), rows, c, hidden, dtype,
+  const bool sizes = rows > 0 && rows < (1ll << 31) && widths_ok(c, hidden);
+  const Plan plan = sizes ? plan_of(rows, c, hidden, precise) : Plan();
+  FfnWs w = {};
+  KFB_TRY(check("feed_forward_bwd", workspace, workspace_bytes, sizes ? carve(w, nullptr, rows, c, hidden, precise, &plan) : 0, rows, c, hidden, dtype,
                 bits(dy) | bits(x) | bits(w_in) | bits(w_out) | bits(dx) | bits(dw_in) | bits(dw_out)));
-  FfnWs w;
-  carve(w, workspace, rows, c, hidden, precise, 1);
+  carve(w, workspace, rows, c, hidden, precise, &plan);
   if (nothing_kept(rows, c, hidden, precise)) {
     const int r = static_cast<int>(rows), planes = ffn_weights_planes(rows, hidden);
     if (dx != nullptr) KFB_TRY(launch_ffn_rows(s, x, dy, w_in, w_out, dx, nullptr, nullptr, r, c, hidden));
@@ -280,14 +332,11 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
     KFB_TRY(launch_split_planes(s, static_cast<const float*>(w_out), w.wo3, wo_n, wo_n));
   }
   const void *wi = precise ? w.wi3 : w_in, *wo = precise ? w.wo3 : w_out;
-  const bool one = one_kernel(c, hidden, precise);
-  const long long piece = piece_rows(rows, c, hidden, precise, 1, one);
-  const int most_in = planes_in(piece, c, hidden, precise), most_out = planes_out(piece, c, hidden, precise);
+  const bool one = plan.one, sums_by_pair = plan.sums_by_pair, dx_here = plan.dx_here;
+  const long long piece = plan.piece;
+  const int most_in = plan.in, most_out = plan.out, dx_planes = plan.dx;
   const int grad_fp32 = grad_dtype == KFB_FP32;
-  const bool single = rows <= piece, sums_by_pair = sums_kernel(piece, c, hidden, precise);
-  // dx of few rows: by the same launch as the weights' gradients, its hidden channels in pieces; of many: by the library's own product for operands along k
-  const int dx_planes = planes_dx(rows, piece, c, hidden);
-  const bool dx_here = precise || (single && static_cast<long long>(cdiv(static_cast<int>(rows), 128)) * cdiv(c, 128) < 2 * sm_count());
+  const bool single = rows <= piece;
   PlaneSum sums[3];
   int n_sums = 0;
   bool transposed = false;
@@ -342,11 +391,11 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
       // (one piece of the rows, of the contraction too: straight into the gradient)
       if (dw_in != nullptr) {
         if (single && most_in == 1) list[n++] = {across(mg), across(mx), 2 * hidden, c, r, dw_in, c, grad_fp32, 1, 0, 0, precise};
-        else list[n++] = {across(mg), across(mx), 2 * hidden, c, r, w.pl_in, c, 1, matmul_splits(2 * hidden, c, r, most_in), wi_n, add, precise};
+        else list[n++] = {across(mg), across(mx), 2 * hidden, c, r, w.pl_in, c, 1, pieces_of(cdiv(m, 64), most_in), wi_n, add, precise};
       }
       if (dw_out != nullptr) {
         if (single && most_out == 1) list[n++] = {across(md), across(mh), c, hidden, r, dw_out, hidden, grad_fp32, 1, 0, 0, precise};
-        else list[n++] = {across(md), across(mh), c, hidden, r, w.pl_out, hidden, 1, matmul_splits(c, hidden, r, most_out), wo_n, add, precise};
+        else list[n++] = {across(md), across(mh), c, hidden, r, w.pl_out, hidden, 1, pieces_of(cdiv(m, 64), most_out), wo_n, add, precise};
       }
     }
     if (n > 0) KFB_TRY(launch_matmuls(s, list, n, "feed_forward_products"));

@@ -77,17 +77,19 @@ struct FfnWs {
 };
 // Whether h, da and db come from the one kernel (feed_forward_hidden.cu).
 bool one_kernel(int c, int hidden, int precise) { return !precise && ffn_hidden_ok(c, hidden); }
-// Whether both gradients come from x and dy alone, nothing kept in between (feed_forward_rows.cu, feed_forward_weights.cu).  Few rows do not fill their
-// tiles of 256 rows: the kernel that spreads the hidden channels over the device, and one launch of all products, are faster (128 channels, 512 hidden, forward
-// and gradient in graph replays: 256 rows 23 us where these take 30, 6 000 36 and 38, 9 000 46 and 40).
+// Whether there are rows enough for the kernels of 256-row tiles that have dx with the hidden channels (feed_forward_rows.cu) and the weights' sums
+// (feed_forward_weights.cu, feed_forward_sums.cu).  Few do not fill them: the kernel that spreads the hidden channels over the device, and one launch of all
+// products, are faster.  Gradient alone, these and the one launch: 128 channels, 512 hidden, 4 000 rows 26 and 21 us, 7 200 29 and 25, 9 500 31 and 32, 20 000 46 and 58;
+// 256 channels, 1 024 hidden, 7 200 rows 63 and 45, 9 500 66 and 73, 20 000 117 and 154.  Fewer hidden channels shorten the one launch more: 128 and 256,
+// 16 000 rows 31 and 26, 30 000 40 and 45; 256 and 512, 12 000 rows 48 and 46, 18 900 54 and 60.
+bool many_rows(long long rows, int c, int hidden) { return rows >= 64ll * sm_count() && rows * hidden >= 64ll * sm_count() * 4 * c; }
+// Whether both gradients come from x and dy alone, nothing kept in between.
 bool nothing_kept(long long rows, int c, int hidden, int precise) {
-  return rows >= 48ll * sm_count() && !precise && ffn_weights_ok(c, hidden) && ffn_rows_ok(c, hidden);
+  return !precise && many_rows(rows, c, hidden) && ffn_weights_ok(c, hidden) && ffn_rows_ok(c, hidden);
 }
-// Pieces that the rows of a weight's gradient are summed in.
-// (256 channels: the pairs' sums from as many rows on as dx comes with the hidden channels; 1 000 rows 34 us by the one launch of products, 48 by these, 9 600
-// 95 and 91, 20 000 171 and 159.)
-bool many_rows(long long rows) { return rows >= 64ll * sm_count(); }
-bool sums_kernel(long long piece, int c, int hidden, int precise) { return many_rows(piece) && one_kernel(c, hidden, precise) && ffn_sums_ok(c, hidden); }
+bool sums_kernel(long long piece, int c, int hidden, int precise) {
+  return many_rows(piece, c, hidden) && one_kernel(c, hidden, precise) && ffn_sums_ok(c, hidden);
+}
 
 // How the products of a gradient that share a launch are cut along their contractions: dx (`dx_tiles` tiles of dx_k blocks of 64) and the weights' gradients
 // (`w_tiles` of w_k).  Pieces fill the device, but each starts and ends, and writes a float32 plane that is read again.  So the cheapest of these counts by
@@ -355,7 +357,7 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
       o.by_k = 1;
       return o;
     };
-    const bool rows_too = one && dx != nullptr && ffn_rows_ok(c, hidden) && c == 256 && many_rows(m);
+    const bool rows_too = one && dx != nullptr && ffn_rows_ok(c, hidden) && c == 256 && many_rows(m, c, hidden);
     void* dxr = static_cast<char*>(dx) + r0 * c * size;
     if (rows_too) {
       const bool keep = dw_in != nullptr || dw_out != nullptr;

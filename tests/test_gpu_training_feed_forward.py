@@ -129,6 +129,54 @@ def test_rows_behind_the_last_of_many_are_left_alone(c):
     _near(dx[:rows], want[1], want[5], BF, "dx")
 
 
+# The kernels of many rows: from 64 rows a multiprocessor on (9 472 on 148 of them), and as many more as hidden channels are fewer than 4 C.
+@pytest.mark.parametrize("rows", [9471, 9472, 9473, 9535, 9537, 9599, 9601, 18943, 18945, 19072, 19201, 37889])
+@pytest.mark.parametrize("c, hidden", [(128, 512), (256, 1024)])
+def test_rows_around_the_tiles_of_the_kernels_of_many(rows, c, hidden):
+    _check(*_case(rows, c, hidden, seed=rows))
+
+
+@pytest.mark.parametrize("rows, c, hidden", [(75777, 128, 64), (37887, 128, 128), (37889, 128, 128), (25301, 128, 192), (10901, 128, 448), (9473, 128, 576), (9473, 128, 2048),
+                                             (151601, 256, 64), (75777, 256, 128), (50601, 256, 192), (21701, 256, 448), (16901, 256, 576), (9473, 256, 2048)])
+def test_widths_of_the_kernels_of_many_rows(rows, c, hidden):
+    _check(*_case(rows, c, hidden, seed=hidden))
+
+
+@pytest.mark.parametrize("c", [128, 256])
+def test_only_some_gradients_by_the_kernels_of_many_rows(c):
+    x, w_in, w_out, dy = _case(10001, c, 4 * c)
+    want = F.gated_feed_forward_backward(dy, x, w_in, w_out)
+    for need in ((True, False, False), (False, True, False), (False, False, True), (False, True, True), (True, False, True), (False, False, False)):
+        got = F.gated_feed_forward_backward(dy, x, w_in, w_out, *need)
+        for g, w, n in zip(got, want, need):
+            assert (g is None) == (not n) and (g is None or torch.equal(g, w))
+
+
+@pytest.mark.parametrize("rows, c, hidden", [(9601, 128, 512), (9601, 256, 1024), (3001, 256, 1024), (1001, 384, 1536)])
+def test_nothing_is_written_behind_the_last_row_or_the_workspace(rows, c, hidden):
+    x, w_in, w_out, dy = _case(rows, c, hidden)
+    want = F.gated_feed_forward_backward(dy, x, w_in, w_out)
+    dx, dwi, dwo = (torch.full((n + 300, k), 7.0, dtype=BF, device=DEV) for n, k in ((rows, c), (2 * hidden, c), (c, hidden)))
+    lib = L.lib()
+    need = lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, 0, 1)
+    ws = torch.full((need + 4096,), 0xA5, dtype=torch.uint8, device=DEV)
+    L.check(lib.kfb_feed_forward_bwd(L.ptr(dy), L.ptr(x), L.ptr(w_in), L.ptr(w_out), L.ptr(dx), L.ptr(dwi), L.ptr(dwo), L.ptr(ws), need, rows, c, hidden, 0, 0,
+                                     L.stream_ptr()))
+    assert (ws[need:] == 0xA5).all()
+    for g, w in zip((dx, dwi, dwo), want):
+        assert (g[w.shape[0]:] == 7).all() and torch.equal(g[:w.shape[0]], w)
+
+
+@pytest.mark.parametrize("rows, c, hidden", [(5000, 128, 512), (10000, 128, 512), (4000, 256, 1024), (10000, 256, 1024), (1000, 384, 1536), (300, 72, 64)])
+def test_what_the_scratch_memory_holds_does_not_matter(rows, c, hidden):
+    x, w_in, w_out, dy = _case(rows, c, hidden)
+    call = lambda: (F.gated_feed_forward(x, w_in, w_out), *F.gated_feed_forward_backward(dy, x, w_in, w_out))
+    want = call()
+    for fill in (0xFF, 0x7F):
+        F._call_workspace(x.device, L.lib().kfb_feed_forward_workspace_bytes(rows, c, hidden, 0, 1)).fill_(fill)
+        assert all(torch.equal(a, b) for a, b in zip(call(), want))
+
+
 @pytest.mark.parametrize("rows, c, hidden, dtype", [(30001, 64, 8192, BF), (47000, 128, 8192, BF), (23000, 256, 8192, BF), (9000, 72, 8192, BF), (5000, 8, 8192, F32)])
 def test_rows_in_several_pieces(rows, c, hidden, dtype):
     """More rows than a workspace holds at once, the last piece a short one."""

@@ -114,3 +114,40 @@ def test_transition_keeps_its_parameters_names():
     from kfold_b200 import modules as M
     assert sorted(M.Transition(64, 2).state_dict()) == ["layernorm.bias", "layernorm.weight", "linear_out.weight", "swiglu.linear.weight"]
     assert not M.Dropout(0.1).state_dict()
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "layer_norm_backward", "gated_feed_forward", "gated_feed_forward_backward", "dropout"])
+def test_another_current_device_than_the_tensors(monkeypatch, name):
+    """The library is called with the tensors' device current, and the caller's is current again afterwards.  (CPU tensors that say they are on GPU 0.)"""
+    current, seen = [1], []
+
+    class OnDevice:
+        def __init__(self, device):
+            pass
+
+        def __enter__(self):
+            self.before, current[0] = current[0], 0
+
+        def __exit__(self, *exc):
+            current[0] = self.before
+
+    class Library:
+        def __getattr__(self, entry):
+            return lambda *args: seen.append((entry, current[0])) or (4096 if entry.endswith("bytes") else 0)
+
+    F._feed_forward_bytes.cache_clear()
+    monkeypatch.setattr(F, "_one_gpu", lambda *a: 0)
+    monkeypatch.setattr(F, "_workspace", lambda device, nbytes, *a: torch.empty(nbytes, dtype=torch.uint8))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    for what, fake in (("current_device", lambda: current[0]), ("on_device", OnDevice), ("lib", Library), ("raw_stream", lambda at=None: 7)):
+        monkeypatch.setattr(F.L, what, fake)
+    x, w, w_in, w_out = torch.zeros(4, 8), torch.zeros(8), torch.zeros(32, 8), torch.zeros(8, 16)
+    call = getattr(F, name)
+    args = {"layer_norm": (x, w, w), "layer_norm_backward": (x, x, w), "gated_feed_forward": (x, w_in, w_out),
+            "gated_feed_forward_backward": (x, x, w_in, w_out), "dropout": (x, 0.1, (1, 2))}[name]
+    for device in (1, 0):
+        current[0] = device
+        seen.clear()
+        call(*args)
+        assert seen and all(d == 0 for _, d in seen) and current[0] == device
+    F._feed_forward_bytes.cache_clear()

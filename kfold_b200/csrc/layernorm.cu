@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(256) layernorm_c128_bf16_kernel(const __nv_bfl
 
 // 256 bf16 channels, contiguous rows: layernorm_rows_kernel's lane layout, expressions and bits, with the weights kept in registers
 // and four rows in flight per warp.  That kernel, one row at a time with the weights fetched for each, took 150 us for 768 x 768
-// rows; this one 130 (92 at the memory's rate; 16-byte accesses gave 96, but another order of summation: a last-bit difference that
+// rows; this one 117 (92 at the memory's rate; 16-byte accesses gave 96, but another order of summation: a last-bit difference that
 // four blocks of bf16 rounding turn into 0.8 % of the result).
 constexpr int kC256Rows = 4;
 __global__ void __launch_bounds__(256) layernorm_c256_bf16_kernel(const __nv_bfloat16* x, __nv_bfloat16* y, const float* w, const float* b,
@@ -277,16 +277,33 @@ __global__ void __launch_bounds__(256) layernorm_c256_bf16_kernel(const __nv_bfl
   }
 }
 
-// Blocks of 256 threads that walk the rows, at most: as many as may start under the tail of the launch before (see launch_kernel).  4, 8 and 16 of
-// them an SM: 147 456 rows of 128 bf16 channels 12.6, 13.9 and 15.7 us, of 256 29.9, 31.1 and 32.5, 63 001 of 128 6.5, 7.9 and 9.7, 14 448 of 768 float32 15.8,
-// 16.6 and 17.3; behind a matrix product or a dropout the same order.  (3: 35 us where 4 are 29.9.)
+// Blocks of 256 threads that walk the rows, at most.  Four of them an SM may start under the tail of the launch before (see launch_kernel).  4, 8 and 16 an
+// SM, graph replays: 147 456 rows of 128 bf16 channels 12.6, 13.9 and 15.7 us, of 256 29.9, 31.1 and 32.5, 63 001 of 128 6.5, 7.9 and 9.7, 14 448 of 768
+// float32 15.8, 16.6 and 17.3; behind a matrix product the same order.  (3: 35 us where 4 are 29.9.)
 constexpr int kLnBlocksPerSm = 4;
+// ... of the kernel that takes the other widths and types a row at a time.  A row of few channels leaves four blocks too little on its way once the launch
+// is long, or its rows come from HBM; so do stores of 384 float32 channels.  4 and 16 an SM, rows that the launch before has left in L2 as far as they fit,
+// and the same behind a matrix product of 4 096 x 4 096 (with it), which clears L2:
+//   64 bf16 channels       16 384 rows 3.6 and 4.5 us, 89.4 and 89.2; 32 768 5.9 and 6.7, 104.5 and 103.4; 65 536 9.8 and 10.0, 104.6 and 101.8;
+//                          262 144 29.9 and 26.4; 1 048 576 174 and 113
+//   128 float32 -> bf16    16 384 4.4 and 5.5, 101.4 and 101.0; 32 768 6.6 and 7.6, 107.6 and 106.9; 65 536 11.2 and 11.7, 111.8 and 109.5;
+//                          147 456 29.9 and 25.7; 589 824 125 and 104
+//   192 bf16               49 152 11.5 and 12.6, 115.3 and 115.5; 65 536 15.0 and 15.8, 121.2 and 120.5; 147 456 35.4 and 34.8; 262 144 61.2 and 59.8
+//   384 float32            65 536 34.2 and 35.2, 131.7 and 133.2; 147 456 78.0 and 72.4; 589 824 311 and 291
+//   256 float32            65 536 24.1 and 25.0; 262 144 86.5 and 87.9
+//   768 bf16               65 536 60.4 and 64.9, 146.0 and 149.7; 147 456 123 and 126
+template <typename TO, int G>
+static long long ln_blocks_per_sm(long long rows, int c) {
+  const long long a_sm = rows / sm_count();
+  const bool many = c <= 128 ? a_sm >= 128 : (c <= 192 || (G == 6 && std::is_same<TO, float>::value)) && a_sm >= 512;
+  return many ? 16 : kLnBlocksPerSm;
+}
 template <typename TI, typename TO, int G>
 static int launch_rows(cudaStream_t stream, const void* x, void* y, const float* w, const float* b, long long rows, int c,
                        long long xs, long long ys, float eps, RowPerm perm) {
   const int warps = 8;
   long long blocks = (rows + warps - 1) / warps;
-  const long long cap = static_cast<long long>(sm_count()) * kLnBlocksPerSm;
+  const long long cap = sm_count() * ln_blocks_per_sm<TO, G>(rows, c);
   if (blocks > cap) blocks = cap;
   LaunchScope scope(stream, "layernorm_rows");
   if (perm.rows) {

@@ -32,8 +32,14 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias = ctx.saved_tensors
         dx, dw, db = F.layer_norm_backward(dy, x, weight, ctx.eps, need_weight=ctx.needs_input_grad[1], need_bias=ctx.needs_input_grad[2])
-        cast = lambda g, like: None if g is None else g if g.dtype == like.dtype else g.to(like.dtype)
-        return dx if ctx.needs_input_grad[0] else None, cast(dw, weight), cast(db, bias), None, None
+        return dx if ctx.needs_input_grad[0] else None, _as(dw, weight), _as(db, bias), None, None
+
+
+def _as(g: torch.Tensor | None, like: torch.Tensor | None) -> torch.Tensor | None:
+    """The gradient of a parameter that the forward pass took in any shape of C elements."""
+    if g is None or (g.dtype == like.dtype and g.shape == like.shape):
+        return g
+    return g.to(like.dtype).view(like.shape)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,

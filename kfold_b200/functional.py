@@ -161,22 +161,24 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
                         need_bias: bool = True):
     """Gradient of ``layer_norm(x, weight, bias, eps)``: (dx, dweight, dbias) from dy, of y's shape, bfloat16 or float32.
 
-    dx is of x's dtype, dweight and dbias float32 (None without a weight or where not asked for).  Any width up to 1024.  The row's
-    statistics are taken from x again, nothing has to be kept from the forward pass; sums over the rows have a fixed order."""
+    dx is of x's dtype; dweight, of the weight's shape, and dbias (C,) are float32 (None without a weight or where not asked for).  Any
+    width up to 1024.  The row's statistics are taken from x again, nothing has to be kept from the forward pass; sums over the rows have a
+    fixed order."""
     at = _one_gpu("layer_norm_backward", x, dy, weight)
     if at != L.current_device():
         with L.on_device(x.device):
             return layer_norm_backward(dy, x, weight, eps, need_weight, need_bias)
     shape = x.shape
     c = shape[-1]
-    if dy.shape != shape or (weight is not None and weight.shape != (c,)):
+    if dy.shape != shape or (weight is not None and weight.numel() != c):
         raise ValueError(f"layer_norm_backward: dy {tuple(dy.shape)}, weight {None if weight is None else tuple(weight.shape)} for x {tuple(shape)}")
     need_weight = need_weight and weight is not None
     xc, dc, w = _dense(x), _dense(dy), _affine(weight)
     dx = _dense_like(x)
-    param = lambda: torch.empty(c, dtype=torch.float32, device=x.device) if w is None else torch.empty_like(w)
-    dw = param() if need_weight else None
-    db = param() if need_bias else None
+    dw = torch.empty_like(w) if need_weight else None
+    db = None
+    if need_bias:
+        db = torch.empty(c, dtype=torch.float32, device=x.device) if w is None or w.dim() != 1 else torch.empty_like(w)
     lib = L.lib()
     ws, size = None, 0
     if need_weight or need_bias:

@@ -8,8 +8,10 @@ and the extension must be built.
 from __future__ import annotations
 
 import math
+import threading
+import weakref
 from functools import lru_cache
-from threading import get_ident
+from itertools import count
 
 import torch
 
@@ -154,7 +156,32 @@ def _call_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     between one another's."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return _workspace(device, nbytes, MOST_KEPT_BYTES, get_ident())
+    return _workspace(device, nbytes, MOST_KEPT_BYTES, _holder())
+
+
+class _Mark:
+    """What a thread's own storage holds: it goes when the thread ends."""
+
+
+_this_thread, _holders = threading.local(), count(1)
+
+
+def _holder() -> int:
+    """A number of the calling thread's own, under which its scratch is kept for as long as the thread lives.  (An identifier of the system's comes
+    round again, or does not: what it held would stay.)"""
+    number = getattr(_this_thread, "number", None)
+    if number is None:
+        number, _this_thread.mark = next(_holders), _Mark()
+        weakref.finalize(_this_thread.mark, _forget, number).atexit = False
+        _this_thread.number = number
+    return number
+
+
+def _forget(holder: int) -> None:
+    # (the memory goes back to the stream that it was allocated on, behind the calls that use it)
+    for key in list(_workspaces):
+        if key[2] == holder:
+            _workspaces.pop(key, None)
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-5, need_weight: bool = True,

@@ -536,9 +536,11 @@ KFB_API int kfb_layernorm(const void* x, void* y, const float* weight, const flo
  *   dtype KFB_BF16: all bf16, products with fp32 accumulation, only the operands h, da, db are rounded in between; KFB_FP32_PRECISE: all
  *   fp32 at fp32 accuracy.  grad_dtype: of dw_in and dw_out, KFB_BF16 or KFB_FP32 (always fp32 in the fp32-accurate mode).  dx, dw_in and
  *   dw_out may each be NULL (not wanted); rows == 0 gives zero gradients of the weights.  The sums over rows have an order that depends on
- *   the sizes alone.  workspace: kfb_feed_forward_workspace_bytes(..., backward) bytes; rows beyond about a
- *   gigabyte of them are taken in pieces.
+ *   the sizes alone.  workspace: kfb_feed_forward_call_bytes(..., wanted) bytes, 256-byte aligned, or NULL where that is 0; wanted is 0 for the forward
+ *   pass, else the sum of 1 (dx), 2 (dw_in) and 4 (dw_out).  Rows beyond about a gigabyte of them are taken in pieces.
+ *   kfb_feed_forward_workspace_bytes: enough for the forward pass (backward = 0) or any of the gradients (1), whatever launches these sizes take.
  */
+KFB_API size_t kfb_feed_forward_call_bytes(long long rows, int c, int hidden, int dtype, int wanted);
 KFB_API size_t kfb_feed_forward_workspace_bytes(long long rows, int c, int hidden, int dtype, int backward);
 KFB_API int kfb_feed_forward_fwd(const void* x, const void* w_in, const void* w_out, void* out, void* workspace, size_t workspace_bytes,
                                  long long rows, int c, int hidden, int dtype, void* stream);

@@ -137,6 +137,7 @@ _SIGNATURES = {
                                   c_float, c_int, c_void_p],
 }
 _SIZE_FUNCS = {
+    "kfb_feed_forward_call_bytes": [c_ll, c_int, c_int, c_int, c_int],
     "kfb_feed_forward_workspace_bytes": [c_ll, c_int, c_int, c_int, c_int],
     "kfb_layernorm_bwd_workspace_bytes": [c_int],
     "kfb_triatt_workspace_bytes_precise": [c_int, c_int, c_int, c_int],

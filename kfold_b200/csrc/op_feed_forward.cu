@@ -91,6 +91,15 @@ bool sums_kernel(long long piece, int c, int hidden, int precise) {
   return many_rows(piece, c, hidden) && one_kernel(c, hidden, precise) && ffn_sums_ok(c, hidden);
 }
 
+// What a call is asked for: its result, or some of the gradients (the entry point's `wanted`).
+constexpr int kForward = 0, kDx = 1, kDwIn = 2, kDwOut = 4, kAll = 7;
+// Whether the forward pass is the pair kernel's, which keeps nothing.
+bool forward_by_pair(long long rows, int c, int hidden, int precise) {
+  return !precise && feed_forward_pair_ok(rows, c, hidden) && transition_pair_is_faster(rows, c, hidden);
+}
+// Whether m rows of a gradient that keeps hidden channels for the weights' sums have dx from the kernel that computes them.
+bool dx_with_hidden(long long m, int c, int hidden, bool one) { return one && c == 256 && ffn_rows_ok(c, hidden) && many_rows(m, c, hidden); }
+
 // How the products of a gradient that share a launch are cut along their contractions: dx (`dx_tiles` tiles of dx_k blocks of 64) and the weights' gradients
 // (`w_tiles` of w_k).  Pieces fill the device, but each starts and ends, and writes a float32 plane that is read again.  So the cheapest of these counts by
 // the time that a launch takes: its blocks, side by side on an SM, two where they fit; waves of them; planes; the launch that adds them up.  The four
@@ -153,34 +162,55 @@ Plan plan_of(long long rows, int c, int hidden, int precise) {
   return p;
 }
 
-size_t carve(FfnWs& w, void* base, long long rows, int c, int hidden, int precise, const Plan* backward) {
+// The workspace of a gradient by `p` that is asked for `wanted`.
+size_t carve_gradient(FfnWs& w, void* base, long long rows, int c, int hidden, int precise, const Plan& p, int wanted) {
   Carver cv(base);
-  const bool one = one_kernel(c, hidden, precise);
-  const long long piece = backward ? backward->piece : piece_rows(rows, c, hidden, precise, 0, one);
-  const size_t r = static_cast<size_t>(piece), parts = precise ? 3 : 1, cc = c, hh = hidden;
+  const size_t cc = c, hh = hidden;
   w = {};
-  if (backward && nothing_kept(rows, c, hidden, precise)) {
+  if (nothing_kept(rows, c, hidden, precise)) {
     const size_t planes = ffn_weights_planes(rows, hidden);
-    w.pl_in = cv.take<float>(planes * 2 * hh * cc);
-    w.pl_out = cv.take<float>(planes * hh * cc);
+    if (wanted & kDwIn) w.pl_in = cv.take<float>(planes * 2 * hh * cc);
+    if (wanted & kDwOut) w.pl_out = cv.take<float>(planes * hh * cc);
     return cv.off;
   }
+  // Rows whose hidden channels lie in memory between launches: a piece; where dx alone is wanted and has a kernel of its own, those of a last piece
+  // that is too short for it, if any.
+  const long long last = rows % p.piece;
+  auto by_rows = [&](long long m) { return (wanted & kDx) != 0 && dx_with_hidden(m, c, hidden, p.one); };
+  auto kept = [&](long long m) { return m > 0 && ((wanted & (kDwIn | kDwOut)) != 0 || !by_rows(m)); };
+  const size_t r = static_cast<size_t>(kept(p.piece) ? p.piece : kept(last) ? last : 0), parts = precise ? 3 : 1;
+  const bool single = rows <= p.piece;
   if (precise) {
     w.x3 = cv.take<__nv_bfloat16>(3 * r * cc);
     w.wi3 = cv.take<__nv_bfloat16>(3 * 2 * hh * cc);
     w.wo3 = cv.take<__nv_bfloat16>(3 * hh * cc);
-    if (backward) w.dy3 = cv.take<__nv_bfloat16>(3 * r * cc);
+    w.dy3 = cv.take<__nv_bfloat16>(3 * r * cc);
+  }
+  if (!p.one) {
+    w.u = cv.take<float>(r * 2 * hh);
+    w.dh = cv.take<float>(r * hh);
+  }
+  w.h = cv.take<__nv_bfloat16>(parts * r * hh);
+  w.dab = cv.take<__nv_bfloat16>(parts * r * 2 * hh);
+  if ((wanted & kDx) && !p.dx_here && r > 0) w.wi_t = cv.take<__nv_bfloat16>(2 * hh * cc);
+  if ((wanted & kDwIn) && (p.sums_by_pair || !single || p.in > 1)) w.pl_in = cv.take<float>(p.in * 2 * hh * cc);
+  if ((wanted & kDwOut) && (p.sums_by_pair || !single || p.out > 1)) w.pl_out = cv.take<float>(p.out * hh * cc);
+  if ((wanted & kDx) && p.dx > 1) w.pl_dx = cv.take<float>(p.dx * r * cc);
+  return cv.off;
+}
+// ... of the forward pass by the launches that keep h.
+size_t carve_forward(FfnWs& w, void* base, long long rows, int c, int hidden, int precise) {
+  Carver cv(base);
+  const bool one = one_kernel(c, hidden, precise);
+  const size_t r = static_cast<size_t>(piece_rows(rows, c, hidden, precise, 0, one)), parts = precise ? 3 : 1, cc = c, hh = hidden;
+  w = {};
+  if (precise) {
+    w.x3 = cv.take<__nv_bfloat16>(3 * r * cc);
+    w.wi3 = cv.take<__nv_bfloat16>(3 * 2 * hh * cc);
+    w.wo3 = cv.take<__nv_bfloat16>(3 * hh * cc);
   }
   if (!one) w.u = cv.take<float>(r * 2 * hh);
   w.h = cv.take<__nv_bfloat16>(parts * r * hh);
-  if (backward) {
-    if (!one) w.dh = cv.take<float>(r * hh);
-    if (!precise) w.wi_t = cv.take<__nv_bfloat16>(2 * hh * cc);
-    w.dab = cv.take<__nv_bfloat16>(parts * r * 2 * hh);
-    w.pl_in = cv.take<float>(backward->in * 2 * hh * cc);
-    w.pl_out = cv.take<float>(backward->out * hh * cc);
-    if (backward->dx > 1) w.pl_dx = cv.take<float>(backward->dx * r * cc);
-  }
   return cv.off;
 }
 
@@ -230,7 +260,7 @@ int check(const char* name, const void* workspace, size_t workspace_bytes, size_
   KFB_CHECK_ARG(rows >= 0 && rows < (1ll << 31), "%s: rows %lld", name, rows);
   KFB_CHECK_ARG(widths_ok(c, hidden), "%s: c=%d, hidden=%d (multiples of 8 up to 65 536)", name, c, hidden);
   KFB_CHECK_ARG((tensors & 15) == 0, "%s: tensors must be 16-byte aligned", name);
-  KFB_CHECK_ARG(workspace != nullptr && workspace_bytes >= need, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
+  KFB_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need), "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
   KFB_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "%s: workspace must be 256-byte aligned", name);
   return KFB_OK;
 }
@@ -243,27 +273,34 @@ using namespace kfb;
 
 extern "C" {
 
+KFB_API size_t kfb_feed_forward_call_bytes(long long rows, int c, int hidden, int dtype, int wanted) {
+  if (rows < 1 || rows >= (1ll << 31) || !widths_ok(c, hidden) || wanted < kForward || wanted > kAll) return 0;
+  const int precise = dtype == KFB_FP32_PRECISE;
+  FfnWs w;
+  if (wanted == kForward) return forward_by_pair(rows, c, hidden, precise) ? 0 : carve_forward(w, nullptr, rows, c, hidden, precise);
+  return carve_gradient(w, nullptr, rows, c, hidden, precise, plan_of(rows, c, hidden, precise), wanted);
+}
+
 KFB_API size_t kfb_feed_forward_workspace_bytes(long long rows, int c, int hidden, int dtype, int backward) {
   if (rows < 1 || !widths_ok(c, hidden)) return 0;
   const int precise = dtype == KFB_FP32_PRECISE;
-  const Plan plan = backward ? plan_of(rows, c, hidden, precise) : Plan();
   FfnWs w;
-  return carve(w, nullptr, rows, c, hidden, precise, backward ? &plan : nullptr);
+  return backward ? carve_gradient(w, nullptr, rows, c, hidden, precise, plan_of(rows, c, hidden, precise), kAll)
+                  : carve_forward(w, nullptr, rows, c, hidden, precise);
 }
 
 KFB_API int kfb_feed_forward_fwd(const void* x, const void* w_in, const void* w_out, void* out, void* workspace, size_t workspace_bytes,
                                  long long rows, int c, int hidden, int dtype, void* stream) {
   if (rows == 0) return KFB_OK;
   KFB_CHECK_ARG(x && w_in && w_out && out, "feed_forward: null tensor");
-  KFB_TRY(check("feed_forward", workspace, workspace_bytes, kfb_feed_forward_workspace_bytes(rows, c, hidden, dtype, 0), rows, c, hidden, dtype,
+  KFB_TRY(check("feed_forward", workspace, workspace_bytes, kfb_feed_forward_call_bytes(rows, c, hidden, dtype, kForward), rows, c, hidden, dtype,
                 bits(x) | bits(w_in) | bits(w_out) | bits(out)));
   cudaStream_t s = as_stream(stream);
   const int precise = dtype == KFB_FP32_PRECISE;
   const size_t size = precise ? 4 : 2;
-  if (!precise && feed_forward_pair_ok(rows, c, hidden) && transition_pair_is_faster(rows, c, hidden))
-    return launch_feed_forward_pair(s, x, w_in, w_out, out, rows, c, hidden);
+  if (forward_by_pair(rows, c, hidden, precise)) return launch_feed_forward_pair(s, x, w_in, w_out, out, rows, c, hidden);
   FfnWs w;
-  carve(w, workspace, rows, c, hidden, precise, nullptr);
+  carve_forward(w, workspace, rows, c, hidden, precise);
   const long long wi_n = 2ll * hidden * c, wo_n = static_cast<long long>(hidden) * c;
   if (precise) {
     KFB_TRY(launch_split_planes(s, static_cast<const float*>(w_in), w.wi3, wi_n, wi_n));
@@ -313,15 +350,18 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
   KFB_CHECK_ARG(dy && x && w_in && w_out, "feed_forward_bwd: null tensor");
   const bool sizes = rows > 0 && rows < (1ll << 31) && widths_ok(c, hidden);
   const Plan plan = sizes ? plan_of(rows, c, hidden, precise) : Plan();
+  const int wanted = (dx != nullptr ? kDx : 0) | (dw_in != nullptr ? kDwIn : 0) | (dw_out != nullptr ? kDwOut : 0);
   FfnWs w = {};
-  KFB_TRY(check("feed_forward_bwd", workspace, workspace_bytes, sizes ? carve(w, nullptr, rows, c, hidden, precise, &plan) : 0, rows, c, hidden, dtype,
+  KFB_TRY(check("feed_forward_bwd", workspace, workspace_bytes,
+                sizes && wanted != 0 ? carve_gradient(w, nullptr, rows, c, hidden, precise, plan, wanted) : 0, rows, c, hidden, dtype,
                 bits(dy) | bits(x) | bits(w_in) | bits(w_out) | bits(dx) | bits(dw_in) | bits(dw_out)));
-  carve(w, workspace, rows, c, hidden, precise, &plan);
+  if (wanted == 0) return KFB_OK;
+  carve_gradient(w, workspace, rows, c, hidden, precise, plan, wanted);
   if (nothing_kept(rows, c, hidden, precise)) {
     const int r = static_cast<int>(rows), planes = ffn_weights_planes(rows, hidden);
     if (dx != nullptr) KFB_TRY(launch_ffn_rows(s, x, dy, w_in, w_out, dx, nullptr, nullptr, r, c, hidden));
     if (dw_in == nullptr && dw_out == nullptr) return KFB_OK;
-    KFB_TRY(launch_ffn_weights(s, x, dy, w_in, w_out, dw_in != nullptr ? w.pl_in : nullptr, dw_out != nullptr ? w.pl_out : nullptr, r, hidden));
+    KFB_TRY(launch_ffn_weights(s, x, dy, w_in, w_out, w.pl_in, w.pl_out, r, hidden));
     PlaneSum sums[2];
     int n = 0;
     if (dw_in != nullptr) sums[n++] = {w.pl_in, wi_n, planes, dw_in, grad_dtype == KFB_FP32, wi_n};
@@ -357,7 +397,7 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
       o.by_k = 1;
       return o;
     };
-    const bool rows_too = one && dx != nullptr && ffn_rows_ok(c, hidden) && c == 256 && many_rows(m, c, hidden);
+    const bool rows_too = dx != nullptr && dx_with_hidden(m, c, hidden, one);
     void* dxr = static_cast<char*>(dx) + r0 * c * size;
     if (rows_too) {
       const bool keep = dw_in != nullptr || dw_out != nullptr;
@@ -388,7 +428,7 @@ KFB_API int kfb_feed_forward_bwd(const void* dy, const void* x, const void* w_in
     }
     if (sums_by_pair) {
       if (dw_in != nullptr || dw_out != nullptr)
-        KFB_TRY(launch_ffn_sums(s, w.dab, xr, w.h, dr, dw_in != nullptr ? w.pl_in : nullptr, dw_out != nullptr ? w.pl_out : nullptr, most_in, add, m, hidden));
+        KFB_TRY(launch_ffn_sums(s, w.dab, xr, w.h, dr, w.pl_in, w.pl_out, most_in, add, m, hidden));
     } else {
       // (one piece of the rows, of the contraction too: straight into the gradient)
       if (dw_in != nullptr) {

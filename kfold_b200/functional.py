@@ -238,7 +238,14 @@ _FEED_FORWARD_CODES = {torch.bfloat16: L.KFB_BF16, torch.float32: L.KFB_FP32_PRE
 @lru_cache(maxsize=1024)
 def _feed_forward_bytes(at: int, *sizes: int) -> int:
     """Scratch of a call on GPU `at`, which is current."""
-    return L.lib().kfb_feed_forward_workspace_bytes(*sizes)
+    return L.lib().kfb_feed_forward_call_bytes(*sizes)
+
+
+def _feed_forward_scratch(x: torch.Tensor, *sizes: int) -> tuple:
+    """(the scratch of a call, its bytes): None and 0 where the kernels keep nothing."""
+    need = _feed_forward_bytes(x.get_device(), *sizes)
+    ws = _call_workspace(x.device, need) if need else None
+    return ws, need
 
 
 def _operand(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
@@ -261,8 +268,8 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor)
             return gated_feed_forward(x, w_in, w_out)
     rows, c, hidden, code, xc, _, wi, wo = _feed_forward_operands("gated_feed_forward", x, w_in, w_out)
     out = _dense_like(x)
-    ws = _call_workspace(x.device, _feed_forward_bytes(at, rows, c, hidden, code, 0))
-    L.check(L.lib().kfb_feed_forward_fwd(xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(), rows, c, hidden, code,
+    ws, size = _feed_forward_scratch(x, rows, c, hidden, code, 0)
+    L.check(L.lib().kfb_feed_forward_fwd(xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), out.data_ptr(), L.ptr(ws), size, rows, c, hidden, code,
                                          L.raw_stream(at)))
     return out
 
@@ -279,9 +286,10 @@ def gated_feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.T
     dx = _dense_like(x) if need_x else None
     dwi = _dense_like(w_in) if need_w_in else None
     dwo = _dense_like(w_out) if need_w_out else None
-    ws = _call_workspace(x.device, _feed_forward_bytes(at, rows, c, hidden, code, 1))
-    L.check(L.lib().kfb_feed_forward_bwd(dc.data_ptr(), xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), L.ptr(dx), L.ptr(dwi), L.ptr(dwo), ws.data_ptr(),
-                                         ws.numel(), rows, c, hidden, code, L.dtype_code(w_in.dtype), L.raw_stream(at)))
+    wanted = bool(need_x) + 2 * bool(need_w_in) + 4 * bool(need_w_out)
+    ws, size = _feed_forward_scratch(x, rows, c, hidden, code, wanted) if wanted else (None, 0)
+    L.check(L.lib().kfb_feed_forward_bwd(dc.data_ptr(), xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), L.ptr(dx), L.ptr(dwi), L.ptr(dwo), L.ptr(ws),
+                                         size, rows, c, hidden, code, L.dtype_code(w_in.dtype), L.raw_stream(at)))
     return dx, dwi, dwo
 
 

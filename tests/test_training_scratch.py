@@ -63,3 +63,18 @@ def test_released_scratch_is_taken_anew():
     assert not F._workspaces and F._call_workspace(CPU, 4096) is not first
     F.withdraw_workspaces([F._call_workspace(CPU, 4096)])
     assert not F._workspaces
+
+
+def test_sizes_of_a_call_and_of_any_call():
+    """Of widths whose launches keep their hidden channels."""
+    from kfold_b200 import _lib, build
+    build.build()
+    lib = _lib.lib()
+    for rows, c, hidden, dtype in ((1, 136, 512, 0), (5000, 72, 1024, 0), (1 << 20, 384, 1536, 0), (300, 72, 64, 2), (1 << 20, 8, 8192, 2)):
+        need = [lib.kfb_feed_forward_call_bytes(rows, c, hidden, dtype, wanted) for wanted in range(8)]
+        assert 0 < need[0] <= lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, dtype, 0)
+        assert 0 < min(need[1:]) and max(need) == max(need[0], need[7]) and need[7] == lib.kfb_feed_forward_workspace_bytes(rows, c, hidden, dtype, 1)
+        for wanted in range(1, 8):
+            assert all(need[wanted] >= need[part] for part in range(1, 8) if part & wanted == part)
+    for bad in ((0, 128, 512, 0, 1), (1 << 31, 128, 512, 0, 1), (5, 0, 512, 0, 1), (5, 12, 512, 0, 0), (5, 128, 512, 0, 8), (5, 128, 512, 0, -1)):
+        assert lib.kfb_feed_forward_call_bytes(*bad) == 0

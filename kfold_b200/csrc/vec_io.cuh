@@ -1,48 +1,10 @@
-// V neighbouring elements between global memory and float registers, in one access where V elements are 8 or 16 bytes (the address then has
-// that alignment).  Plain loads and stores: these kernels may start before the launch before them has ended (see launch_kernel).
+// V neighbouring elements from float registers to global memory, in one access where V elements are 8 or 16 bytes (the address then has that
+// alignment).
 #pragma once
 #include <cuda_bf16.h>
 #include <stdint.h>
 
 namespace kfb {
-
-template <int V>
-__device__ __forceinline__ void load_vec(const float* p, float* v) {
-  if constexpr (V % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      const float4 t = *reinterpret_cast<const float4*>(p + i);
-      v[i] = t.x;
-      v[i + 1] = t.y;
-      v[i + 2] = t.z;
-      v[i + 3] = t.w;
-    }
-  } else {
-    static_assert(V == 1, "pieces of 1 or a multiple of 4");
-    v[0] = *p;
-  }
-}
-__device__ __forceinline__ void bf16_pair(uint32_t u, float* v) {
-  v[0] = __uint_as_float(u << 16);
-  v[1] = __uint_as_float(u & 0xffff0000u);
-}
-template <int V>
-__device__ __forceinline__ void load_vec(const __nv_bfloat16* p, float* v) {
-  if constexpr (V == 8) {
-    const uint4 t = *reinterpret_cast<const uint4*>(p);
-    bf16_pair(t.x, v);
-    bf16_pair(t.y, v + 2);
-    bf16_pair(t.z, v + 4);
-    bf16_pair(t.w, v + 6);
-  } else if constexpr (V == 4) {
-    const uint2 t = *reinterpret_cast<const uint2*>(p);
-    bf16_pair(t.x, v);
-    bf16_pair(t.y, v + 2);
-  } else {
-    static_assert(V == 1, "pieces of 1, 4 or 8");
-    v[0] = __bfloat162float(*p);
-  }
-}
 
 template <int V>
 __device__ __forceinline__ void store_vec(float* p, const float* v) {

@@ -533,8 +533,8 @@ KFB_API int kfb_layernorm(const void* x, void* y, const float* weight, const flo
  * Gated feed-forward y = (silu(x Wa^T) * (x Wb^T)) Wo^T, [Wa; Wb] = w_in, and its gradient: SwiGLU and output projection of
  * Transition.forward (src/kfold/model/layers/folding/transition.py:48-68) in training, on the plain (not packed) parameters.
  *   x, out, dy, dx (rows, c), w_in, dw_in (2 hidden, c), w_out, dw_out (c, hidden), row-major, 16-byte aligned; c and hidden multiples of 8 up to 65 536.
- *   dtype KFB_BF16: all bf16, products with fp32 accumulation, only the operands h, da, db are rounded in between; KFB_FP32_PRECISE: all
- *   fp32 at fp32 accuracy.  grad_dtype: of dw_in and dw_out, KFB_BF16 or KFB_FP32 (always fp32 in the fp32-accurate mode).  dx, dw_in and
+ *   dtype KFB_BF16: all bf16, products with fp32 accumulation, only the operands h, da, db are rounded in between, and sigmoid(a) comes from the
+ *   approximate tanh: off by less than 2^-12, by some 2^-22 for a near -10 and 2^-25 near -12, of which nothing is left for a below -15.  KFB_FP32_PRECISE: all fp32 at fp32 accuracy.  grad_dtype: of dw_in and dw_out, KFB_BF16 or KFB_FP32 (always fp32 in the fp32-accurate mode).  dx, dw_in and
  *   dw_out may each be NULL (not wanted); rows == 0 gives zero gradients of the weights.  The sums over rows have an order that depends on
  *   the sizes alone.  workspace: kfb_feed_forward_call_bytes(..., wanted) bytes, 256-byte aligned, or NULL where that is 0; wanted is 0 for the forward
  *   pass, else the sum of 1 (dx), 2 (dw_in) and 4 (dw_out).  Rows beyond about a gigabyte of them are taken in pieces.

@@ -93,7 +93,14 @@ bool sums_kernel(long long piece, int c, int hidden, int precise) {
 
 // What a call is asked for: its result, or some of the gradients (the entry point's `wanted`).
 constexpr int kForward = 0, kDx = 1, kDwIn = 2, kDwOut = 4, kAll = 7;
-// Whether the forward pass is the pair kernel's, which keeps nothing.
+// Whether the forward pass is the pair kernel's, which keeps nothing, or two launches.  The rule is the Transition's, whose other form has a LayerNorm's
+// launch more.  Pair kernel and two launches, graph replays, us:
+//   128 channels, 512 hidden      64 rows 8.6 and 8.7, 1 024 9.4 and 9.4, 8 192 9.9 and 13.1, 63 001 23 and 40
+//   128 channels, 1 024 hidden    1 024 rows 13.1 and 11.9 (takes two), 2 048 13.3 and 12.9 (pair), 4 096 13.5 and 14.7, 63 001 40 and 78
+//   256 channels, 512 hidden      4 096 rows 14.1 and 12.3 (two), 5 000 14.1 and 12.6 (pair), 7 000 14.2 and 14.0, 9 600 14.7 and 18.3, 63 001 41 and 55
+//   256 channels, 1 024 hidden    8 192 rows 22.3 and 19.6 (two), 9 000 22.4 and 19.9 (pair), 9 600 22.9 and 27.5, 19 000 39 and 45, 63 001 73 and 101
+//   256 channels, 2 048 hidden    9 000 rows 38 and 31 (two), 9 600 39 and 46 (pair), 19 000 71 and 85 (two), 22 000 72 and 90 (pair)
+// So it takes the slower form by up to an eighth for 5 000 to 6 500 and 8 500 to 9 500 rows of 256 channels, and by a fifth for 19 000 to 21 000 of 2 048 hidden.
 bool forward_by_pair(long long rows, int c, int hidden, int precise) {
   return !precise && feed_forward_pair_ok(rows, c, hidden) && transition_pair_is_faster(rows, c, hidden);
 }

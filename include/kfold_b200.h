@@ -666,6 +666,69 @@ KFB_API int kfb_pair_block_fwd(const kfb_pair_block* blk, const void* z, void* z
                                const unsigned char* pair_mask, const unsigned char* mask, void* workspace, size_t workspace_bytes,
                                int batch, int n, void* stream);
 
+/*
+ * What lies between two blocks of a residual stream (training and inference): the block's output is gated and added, and the
+ * stream is normalised for the next block.
+ *   r = scale x + sigmoid(gate) u         (each of scale, gate may be NULL: one; x or u may be NULL: nothing)
+ *   y = weight LayerNorm(r) + bias        (norm 1; either may be NULL)
+ *   y = sigmoid(g) LayerNorm(r) + v       (norm 2: gate_shift rows are [g | v], 2c wide)
+ * with r as it is stored, of stream_dtype.  Output gate and adaptive norm as in
+ * src/kfold/model/layers/folding/diffusion_transformer.py:73-81 and src/kfold/model/primitives/normalization.py:117-125, the
+ * state decay as in src/kfold/model/model.py:523-529.
+ *   x, r       : (rows, c) stream_dtype;  u, y : (rows, c) compute_dtype; both bf16, both fp32, or a fp32 stream with bf16.
+ *   gate       : (rows / samples, c), rows gate_ld apart; gate_shift : (rows / samples, 2c), rows gate_shift_ld apart; compute_dtype.
+ *                Row (group, sample, token) of the stream uses row (group, token): l tokens a group, `samples` entries share.
+ *   scale, weight, bias : fp32 [c].
+ *   r          : NULL only where neither u nor scale is given (r is x then).
+ *   kept, kept_exponents : NULL, or r in 8 bits: int8 (rows, c) and bytes (rows, ceil(c / 32)), see kfb_compress.
+ * c up to 1024, rows below 2^31.
+ */
+KFB_API int kfb_residual_norm_fwd(const void* x, const void* u, const void* gate, long long gate_ld, const float* scale, const float* weight,
+                                  const float* bias, const void* gate_shift, long long gate_shift_ld, void* r, void* y, void* kept,
+                                  void* kept_exponents, long long rows, int c, int samples, int l, float eps, int norm, int stream_dtype,
+                                  int compute_dtype, void* stream);
+/*
+ * Its gradient: with z = (r - mean) rstd, m the norm's factor, s = sigmoid(gate), t = dr + rstd (m dy - mean(m dy) - z mean(m dy z)):
+ *   dx = scale t, du = s t, dgate = s (1 - s) sum(t u), dgate_shift = [m (1 - m) sum(dy z) | sum(dy)] over the samples that share a row
+ *   (compute_dtype, dense), dweight = sum(dy z), dbias = sum(dy), dscale = sum(t x) over all rows (fp32).
+ * Outputs that are NULL are not computed.  dr NULL: zero; dy is not read with norm 0.  r, u and x (u: for dgate, x: for dscale only) are the
+ * tensors, or the values of kfb_compress where their exponents are given.  The workspace is needed for dweight, dbias and dscale.
+ */
+KFB_API size_t kfb_residual_norm_bwd_workspace_bytes(int c);
+KFB_API int kfb_residual_norm_bwd(const void* dr, const void* dy, const void* r, const void* r_exponents, const void* u, const void* u_exponents,
+                                  const void* x, const void* x_exponents, const void* gate, long long gate_ld, const float* scale,
+                                  const float* weight, const void* gate_shift, long long gate_shift_ld, void* dx, void* du, void* dgate,
+                                  void* dgate_shift, float* dweight, float* dbias, float* dscale, void* workspace, size_t workspace_bytes,
+                                  long long rows, int c, int samples, int l, float eps, int norm, int stream_dtype, int compute_dtype, void* stream);
+
+/*
+ * Rows put away in 8 bits for a backward pass, and taken back.  32 neighbouring channels (the last group of a row may be shorter) share
+ * a power of two: a value is q 2^(e - 133), q a whole number of -127 ... 127 (int8), e the byte of its group: the exponent field of the
+ * group's largest magnitude as a fp32 number, one more where that magnitude would round to 128.  Off by at most half a step, 2^-7 of the
+ * group's largest.  A group with a value that is not finite comes back as NaN (e = 255); groups whose e would be below 8 (magnitudes
+ * under 2^-119) come back as zeros (e = 0), e is 254 at most.
+ *   x : (rows, c) dtype;  values : int8 (rows, c);  exponents : bytes (rows, ceil(c / 32)).  c up to 65536.
+ */
+KFB_API int kfb_compress(const void* x, void* values, void* exponents, long long rows, int c, int dtype, void* stream);
+KFB_API int kfb_expand(const void* values, const void* exponents, void* x, long long rows, int c, int dtype, void* stream);
+
+/*
+ * A linear layer with its tail, and its gradient (model/primitives/linear.py:25-107 with what follows it at its call sites):
+ *   z = x w^T + bias,  out = f(z) + residual;   dz = dy f'(z),  dx = dz w,  dw = dz^T x,  dbias = sum over rows of dz.
+ *   x : (rows, k), w : (n, k), `dtype` KFB_BF16 or KFB_FP32_PRECISE (fp32 tensors);  bias : fp32 [n] or NULL.
+ *   activation f : 0 none, 1 sigmoid, 2 silu, 3 gelu (with the error function), 4 relu.
+ *   residual, out : (rows, n) of out_dtype (KFB_BF16, or KFB_FP32: always with KFB_FP32_PRECISE);  dy : of dy_dtype likewise.
+ *   dw : (n, k) of dw_dtype, dbias : fp32; dx : (rows, k) as x.  Gradients that are NULL are not computed.
+ * k, n multiples of 8 up to 65536, tensors on 16-byte boundaries.  Workspace: `wanted` 0 for the forward pass (dy_dtype is not looked
+ * at), else the sum of 1 (dx), 2 (dw), 4 (dbias).
+ */
+KFB_API size_t kfb_fused_linear_workspace_bytes(long long rows, int k, int n, int activation, int dtype, int dy_dtype, int wanted);
+KFB_API int kfb_fused_linear_fwd(const void* x, const void* w, const float* bias, const void* residual, void* out, void* workspace,
+                                 size_t workspace_bytes, long long rows, int k, int n, int activation, int dtype, int out_dtype, void* stream);
+KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, const float* bias, void* dx, void* dw, float* dbias, void* workspace,
+                                 size_t workspace_bytes, long long rows, int k, int n, int activation, int dtype, int dy_dtype, int dw_dtype,
+                                 void* stream);
+
 #ifdef __cplusplus
 }
 #endif

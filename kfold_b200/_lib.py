@@ -132,6 +132,14 @@ _SIGNATURES = {
     "kfb_feed_forward_fwd": [c_void_p] * 5 + [ctypes.c_size_t, c_ll, c_int, c_int, c_int, c_void_p],
     "kfb_feed_forward_bwd": [c_void_p] * 8 + [ctypes.c_size_t, c_ll, c_int, c_int, c_int, c_int, c_void_p],
     "kfb_layernorm_bwd": [c_void_p] * 7 + [ctypes.c_size_t, c_ll, c_int, c_float, c_int, c_int, c_void_p],
+    "kfb_residual_norm_fwd": [c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_void_p, c_void_p,
+                              c_void_p, c_ll, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p],
+    "kfb_residual_norm_bwd": [c_void_p] * 9 + [c_ll, c_void_p, c_void_p, c_void_p, c_ll] + [c_void_p] * 8 + [ctypes.c_size_t, c_ll, c_int, c_int,
+                              c_int, c_float, c_int, c_int, c_int, c_void_p],
+    "kfb_compress": [c_void_p, c_void_p, c_void_p, c_ll, c_int, c_int, c_void_p],
+    "kfb_expand": [c_void_p, c_void_p, c_void_p, c_ll, c_int, c_int, c_void_p],
+    "kfb_fused_linear_fwd": [c_void_p] * 6 + [ctypes.c_size_t, c_ll, c_int, c_int, c_int, c_int, c_int, c_void_p],
+    "kfb_fused_linear_bwd": [c_void_p] * 8 + [ctypes.c_size_t, c_ll] + [c_int] * 6 + [c_void_p],
     "kfb_dropout": [c_void_p, c_void_p, c_void_p, c_ll, c_ll, c_ll, c_ll, c_float, c_void_p, c_ll, c_ll, c_int, c_int, c_void_p],
     "kfb_transition_fwd_static": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_int, c_int,
                                   c_float, c_int, c_void_p],
@@ -140,6 +148,8 @@ _SIZE_FUNCS = {
     "kfb_feed_forward_call_bytes": [c_ll, c_int, c_int, c_int, c_int],
     "kfb_feed_forward_workspace_bytes": [c_ll, c_int, c_int, c_int, c_int],
     "kfb_layernorm_bwd_workspace_bytes": [c_int],
+    "kfb_residual_norm_bwd_workspace_bytes": [c_int],
+    "kfb_fused_linear_workspace_bytes": [c_ll, c_int, c_int, c_int, c_int, c_int, c_int],
     "kfb_triatt_workspace_bytes_precise": [c_int, c_int, c_int, c_int],
     "kfb_apb_workspace_bytes_precise": [c_int, c_int, c_int],
     "kfb_pair_bias_workspace_bytes_precise": [c_int, c_int, c_int],

@@ -1,0 +1,91 @@
+// Rows put away in 8 bits and taken back (the format is in row_teams.cuh).
+//
+// What bounds it: HBM, 2 or 4 bytes a value one way and 33 / 32 the other.  A lane takes eight channels of a row, four lanes a group of 32; rows of any
+// width whose channels are a multiple of eight and lie on 16-byte boundaries go in whole pieces, others a value at a time.
+#include "ops_common.cuh"
+#include "row_teams.cuh"
+
+namespace kfb {
+namespace {
+
+// Pieces of eight channels, four to a group of 32: rows of `groups` groups, pieces numbered through.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) compress_kernel(const T* x, uint8_t* q, uint8_t* e, long long pieces, int c, int groups) {
+  grid_dependency_enter();
+  const long long per_row = 4ll * groups;
+  // (a warp's lanes leave the loop together: pieces beyond the end have no values)
+  for (long long first = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x / 32 * 32; first < pieces; first += gridDim.x * 256ll) {
+    const long long i = first + threadIdx.x % 32, row = i / per_row;
+    const int ch = static_cast<int>(i - row * per_row) * kPiece, n = i < pieces ? min(max(c - ch, 0), kPiece) : 0;
+    Piece<T, VEC> raw;
+    float v[kPiece];
+    raw.load(x + row * c + ch, n);
+    raw.values(v);
+    store_piece8<VEC>(q + row * c + ch, e + row * groups + ch / kGroup8, v, n, threadIdx.x % 4 == 0);
+  }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) expand_kernel(const uint8_t* q, const uint8_t* e, T* x, long long pieces, int c, int groups) {
+  grid_dependency_enter();
+  const long long per_row = 4ll * groups;
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < pieces; i += gridDim.x * 256ll) {
+    const long long row = i / per_row;
+    const int ch = static_cast<int>(i - row * per_row) * kPiece, n = min(max(c - ch, 0), kPiece);
+    Piece<float, VEC> raw;
+    float v[kPiece];
+    raw.load8(q + row * c + ch, e + row * groups + ch / kGroup8, n);
+    raw.values_of_8(v);
+    store_piece<VEC>(x + row * c + ch, v, n);
+  }
+}
+
+template <typename T>
+int compress_as(cudaStream_t s, const void* x, void* q, void* e, long long rows, int c) {
+  const long long pieces = rows * groups8(c) * 4;
+  const bool vec = c % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
+  const long long want = (pieces + 255) / 256, most = 16ll * sm_count();
+  LaunchScope scope(s, "compress");
+  return launch_kernel(s, vec ? compress_kernel<T, true> : compress_kernel<T, false>, static_cast<unsigned>(want < most ? want : most), 256, 0,
+                       static_cast<const T*>(x), static_cast<uint8_t*>(q), static_cast<uint8_t*>(e), pieces, c, groups8(c));
+}
+
+template <typename T>
+int expand_as(cudaStream_t s, const void* q, const void* e, void* x, long long rows, int c) {
+  const long long pieces = rows * groups8(c) * 4;
+  const bool vec = c % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
+  const long long want = (pieces + 255) / 256, most = 16ll * sm_count();
+  LaunchScope scope(s, "expand");
+  return launch_kernel(s, vec ? expand_kernel<T, true> : expand_kernel<T, false>, static_cast<unsigned>(want < most ? want : most), 256, 0,
+                       static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(e), static_cast<T*>(x), pieces, c, groups8(c));
+}
+
+int check(const char* name, const void* a, const void* b, const void* d, long long rows, int c, int dtype) {
+  KFB_CHECK_ARG(rows >= 0 && rows < (1ll << 40) && c > 0 && c <= 65536, "%s: rows %lld, channels %d", name, rows, c);
+  KFB_CHECK_ARG(dtype == KFB_BF16 || dtype == KFB_FP32, "%s: bad dtype %d", name, dtype);
+  KFB_CHECK_ARG(rows == 0 || (a != nullptr && b != nullptr && d != nullptr), "%s: null tensor", name);
+  return KFB_OK;
+}
+
+}  // namespace
+}  // namespace kfb
+
+using namespace kfb;
+
+extern "C" {
+
+KFB_API int kfb_compress(const void* x, void* values, void* exponents, long long rows, int c, int dtype, void* stream) {
+  KFB_TRY(check("compress", x, values, exponents, rows, c, dtype));
+  if (rows == 0) return KFB_OK;
+  cudaStream_t s = as_stream(stream);
+  return dtype == KFB_BF16 ? compress_as<__nv_bfloat16>(s, x, values, exponents, rows, c) : compress_as<float>(s, x, values, exponents, rows, c);
+}
+
+KFB_API int kfb_expand(const void* values, const void* exponents, void* x, long long rows, int c, int dtype, void* stream) {
+  KFB_TRY(check("expand", x, values, exponents, rows, c, dtype));
+  if (rows == 0) return KFB_OK;
+  cudaStream_t s = as_stream(stream);
+  return dtype == KFB_BF16 ? expand_as<__nv_bfloat16>(s, values, exponents, x, rows, c) : expand_as<float>(s, values, exponents, x, rows, c);
+}
+
+}  // extern "C"

@@ -12,6 +12,7 @@ import threading
 import weakref
 from functools import lru_cache
 from itertools import count
+from typing import NamedTuple
 
 import torch
 
@@ -184,13 +185,16 @@ def _forget(holder: int) -> None:
             _workspaces.pop(key, None)
 
 
-def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-5, need_weight: bool = True,
+def layer_norm_backward(dy: torch.Tensor, x, weight: torch.Tensor | None, eps: float = 1e-5, need_weight: bool = True,
                         need_bias: bool = True):
     """Gradient of ``layer_norm(x, weight, bias, eps)``: (dx, dweight, dbias) from dy, of y's shape, bfloat16 or float32.
 
     dx is of x's dtype; dweight, of the weight's shape, and dbias (C,) are float32 (None without a weight or where not asked for).  Any
     width up to 1024.  The row's statistics are taken from x again, nothing has to be kept from the forward pass; sums over the rows have a
-    fixed order."""
+    fixed order.  x may be ``Compressed``: dy is then of its type, or bfloat16."""
+    if type(x) is Compressed:
+        g = residual_norm_backward(None, dy, x, weight=weight, eps=eps, need_weight=need_weight, need_bias=need_bias)
+        return g.x, g.weight, g.bias
     at = _one_gpu("layer_norm_backward", x, dy, weight)
     if at != L.current_device():
         with L.on_device(x.device):
@@ -274,10 +278,12 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor)
     return out
 
 
-def gated_feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, need_x: bool = True,
+def gated_feed_forward_backward(dy: torch.Tensor, x, w_in: torch.Tensor, w_out: torch.Tensor, need_x: bool = True,
                                 need_w_in: bool = True, need_w_out: bool = True):
     """Gradient of ``gated_feed_forward``: (dx, dw_in, dw_out) from dy, of x's shape and dtype; None where not asked for.  The weights'
-    gradients have the weights' dtype (float32 sums either way).  The hidden channels are computed again, nothing has to be kept."""
+    gradients have the weights' dtype (float32 sums either way).  The hidden channels are computed again, nothing has to be kept.  x may be
+    ``Compressed``."""
+    x = _expanded(x)
     at = _one_gpu("gated_feed_forward_backward", x, w_in, w_out, dy)
     if at != L.current_device():
         with L.on_device(x.device):
@@ -336,6 +342,320 @@ def dropout(x: torch.Tensor, p: float, rng, shared_dim: int | None = None, resid
     L.check(L.lib().kfb_dropout(xc.data_ptr(), L.ptr(rc), out.data_ptr(), outer, shared, inner, int(p * 4294967296.0 + 0.5), scale, L.ptr(state),
                                 _signed64(seed), _signed64(offset), L.dtype_code(x.dtype), L.dtype_code(out.dtype), L.raw_stream(at)))
     return out
+
+
+# ---- between two blocks of a residual stream
+_NO_NORM, _AFFINE_NORM, _ADAPTIVE_NORM = 0, 1, 2
+_GROUP8 = 32                   # channels that share a power of two
+
+
+class Compressed:
+    """Rows kept in 8 bits for a backward pass (``compress``): ``values`` int8, of the rows' shape, and ``exponents`` uint8, one for 32
+    neighbouring channels (the last of a row may be fewer).  A value stands for ``values * 2 ** (exponents - 133)``, NaN where the exponent is
+    255; ``dtype`` is what the rows had and ``expand`` gives back."""
+
+    __slots__ = ("values", "exponents", "dtype")
+
+    def __init__(self, values: torch.Tensor, exponents: torch.Tensor, dtype: torch.dtype):
+        if (values.dtype != torch.int8 or exponents.dtype != torch.uint8 or not values.is_contiguous() or not exponents.is_contiguous() or not values.dim()
+                or exponents.shape != (*values.shape[:-1], (values.shape[-1] + _GROUP8 - 1) // _GROUP8) or values.device != exponents.device):
+            raise ValueError(f"Compressed: values {values.dtype} {tuple(values.shape)}, exponents {exponents.dtype} {tuple(exponents.shape)}")
+        L.dtype_code(dtype)
+        self.values, self.exponents, self.dtype = values, exponents, dtype
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.values.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.values.device
+
+    def __repr__(self) -> str:
+        return f"Compressed({tuple(self.shape)}, {self.dtype})"
+
+
+def _room8(x: torch.Tensor) -> Compressed:
+    """Room for x's rows in 8 bits."""
+    c = Compressed.__new__(Compressed)
+    c.values = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    c.exponents = torch.empty((*x.shape[:-1], (x.shape[-1] + _GROUP8 - 1) // _GROUP8), dtype=torch.uint8, device=x.device)
+    c.dtype = x.dtype
+    return c
+
+
+def compress(x: torch.Tensor) -> Compressed:
+    """x (..., C), bfloat16 or float32, in 8 bits: 33 / 32 bytes a value, each off by at most half a step of its group, 2^-7 of the group's largest
+    magnitude.  Groups with a value that is not finite come back as NaN; groups whose largest magnitude is below 2^-119 as zeros."""
+    at = _one_gpu("compress", x)
+    if at != L.current_device():
+        with L.on_device(x.device):
+            return compress(x)
+    code = L.dtype_code(x.dtype)
+    if not x.dim() or not x.shape[-1]:
+        raise ValueError(f"compress: x {tuple(x.shape)}")
+    xc, out = _dense(x), _room8(x)
+    c = x.shape[-1]
+    L.check(L.lib().kfb_compress(xc.data_ptr(), out.values.data_ptr(), out.exponents.data_ptr(), x.numel() // c, c, code, L.raw_stream(at)))
+    return out
+
+
+def expand(kept: Compressed, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """What ``kept`` stands for, of the type that its rows had or of ``dtype`` (exact in both)."""
+    values = kept.values
+    at = _one_gpu("expand", values, kept.exponents)
+    if at != L.current_device():
+        with L.on_device(values.device):
+            return expand(kept, dtype)
+    out = torch.empty(values.shape, dtype=dtype or kept.dtype, device=values.device)
+    c = values.shape[-1]
+    L.check(L.lib().kfb_expand(values.data_ptr(), kept.exponents.data_ptr(), out.data_ptr(), values.numel() // c if c else 0, c, L.dtype_code(out.dtype),
+                               L.raw_stream(at)))
+    return out
+
+
+def _expanded(x):
+    return expand(x) if type(x) is Compressed else x
+
+
+class ResidualNormGradients(NamedTuple):
+    """What ``residual_norm_backward`` gives; None where there is no such input or it was not asked for."""
+    x: torch.Tensor | None
+    u: torch.Tensor | None
+    gate: torch.Tensor | None
+    scale: torch.Tensor | None
+    weight: torch.Tensor | None
+    bias: torch.Tensor | None
+    gate_shift: torch.Tensor | None
+
+
+def _stream_operands(name: str, shape, stream: torch.dtype, compute: torch.dtype, u, gate, gate_shift, samples: int, vectors) -> tuple:
+    """(rows, channels, tokens; dtype codes of the stream and of what the blocks compute in; gate, its row stride, gate_shift, its row stride)."""
+    c = shape[-1] if shape else 0
+    if not c:
+        raise ValueError(f"{name}: rows of shape {tuple(shape)}")
+    rows = math.prod(shape[:-1])
+    if (stream, compute) not in _STREAM_CODES:
+        raise ValueError(f"{name}: a stream of {stream} with {compute} (bfloat16, float32, or float32 with bfloat16)")
+    for t in vectors:
+        if t is not None and t.numel() != c:
+            raise ValueError(f"{name}: {tuple(t.shape)} for {c} channels")
+    if u is not None and (u.shape != shape or u.dtype != compute):
+        raise ValueError(f"{name}: u {u.dtype} {tuple(u.shape)} for rows {tuple(shape)} computed in {compute}")
+    tokens = 1
+    if samples != 1:
+        if len(shape) < 2 or samples < 1 or (rows and rows % (samples * shape[-2])):
+            raise ValueError(f"{name}: {samples} samples share gates in rows {tuple(shape)}")
+        tokens = shape[-2] or 1
+    gate_ld = shift_ld = 0
+    if gate is not None:
+        if gate.shape[-1:] != (c,) or gate.numel() * samples != rows * c or gate.dtype != compute:
+            raise ValueError(f"{name}: gate {gate.dtype} {tuple(gate.shape)} for rows {tuple(shape)} of {compute}, of which {samples} entries share")
+        gate, _, gate_ld = _rows(gate, c)
+    if gate_shift is not None:
+        if gate_shift.shape[-1:] != (2 * c,) or gate_shift.numel() * samples != 2 * rows * c or gate_shift.dtype != compute:
+            raise ValueError(f"{name}: gate_shift {gate_shift.dtype} {tuple(gate_shift.shape)} for rows {tuple(shape)} of {compute}, of which {samples} "
+                             "entries share")
+        gate_shift, _, shift_ld = _rows(gate_shift, 2 * c)
+    return rows, c, tokens, *_STREAM_CODES[stream, compute], gate, gate_ld, gate_shift, shift_ld
+
+
+_STREAM_CODES = {(torch.bfloat16, torch.bfloat16): (L.KFB_BF16, L.KFB_BF16), (torch.float32, torch.float32): (L.KFB_FP32, L.KFB_FP32),
+                 (torch.float32, torch.bfloat16): (L.KFB_FP32, L.KFB_BF16)}
+
+
+def residual_norm(x: torch.Tensor | None, u: torch.Tensor | None = None, gate: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                  weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, gate_shift: torch.Tensor | None = None, samples: int = 1,
+                  eps: float = 1e-5, norm: bool = True, out_dtype: torch.dtype | None = None, compress: bool = False):
+    """What lies between two blocks of a residual stream: ``(r, y)`` with
+
+        r = scale * x + sigmoid(gate) * u                       the block's output u, gated and added (model/layers/folding/diffusion_transformer.py:73-81)
+        y = LayerNorm(r) * weight + bias                        the next block's norm, or, with gate_shift = [g | v],
+        y = sigmoid(g) * LayerNorm(r) + v                       the adaptive one (model/primitives/normalization.py:117-125)
+
+    x (..., C) is the stream and gives r its type; u and y have the type that the blocks compute in: the stream's, or bfloat16 beside a float32
+    stream.  Each of u, gate, scale (C,), weight (C,), bias (C,) may be missing, x too where u is there (r is of u's type then).  Without u and scale r is x itself; without
+    ``norm`` y is None.  What is normalised is r as it is stored.  ``gate`` (..., C) and ``gate_shift`` (..., 2 C), of u's type, have a row for
+    ``samples`` entries: x (groups * samples, L, C), flattened, takes gate (groups, L, C).  ``compress``: a third result, r in 8 bits.  Any C up to 1024."""
+    base = u if x is None else x
+    if base is None:
+        raise ValueError("residual_norm: neither x nor u")
+    at = _one_gpu("residual_norm", base, u, gate, scale, weight, bias, gate_shift)
+    if at != L.current_device():
+        with L.on_device(base.device):
+            return residual_norm(x, u, gate, scale, weight, bias, gate_shift, samples, eps, norm, out_dtype, compress)
+    compute = u.dtype if u is not None else gate_shift.dtype if gate_shift is not None else out_dtype or base.dtype
+    if norm and out_dtype is not None and out_dtype != compute:
+        raise ValueError(f"residual_norm: a result of {out_dtype} beside {compute}")
+    if (gate is not None and u is None) or (scale is not None and x is None) or (gate_shift is not None and (weight is not None or bias is not None)) or (
+            not norm and (weight is not None or bias is not None or gate_shift is not None)):
+        raise ValueError("residual_norm: a gate needs u, a scale x, parameters of the norm the norm, and gate_shift stands in for weight and bias")
+    shape = base.shape
+    rows, c, tokens, st, ct, gate, gate_ld, gs, gs_ld = _stream_operands("residual_norm", shape, base.dtype, compute, u, gate, gate_shift, samples,
+                                                                         (scale, weight, bias))
+    xc, uc = None if x is None else _dense(x), None if u is None else _dense(u)
+    r = x if u is None and scale is None else _dense_like(base)
+    y = _dense_like(base, compute) if norm else None
+    kept = _room8(base) if compress else None
+    sc, w, b = _affine(scale), _affine(weight), _affine(bias)
+    L.check(L.lib().kfb_residual_norm_fwd(L.ptr(xc), L.ptr(uc), L.ptr(gate), gate_ld, L.ptr(sc), L.ptr(w), L.ptr(b), L.ptr(gs), gs_ld,
+                                          None if r is x else r.data_ptr(), L.ptr(y), None if kept is None else kept.values.data_ptr(),
+                                          None if kept is None else kept.exponents.data_ptr(), rows, c, samples, tokens, eps,
+                                          _NO_NORM if not norm else _AFFINE_NORM if gs is None else _ADAPTIVE_NORM, st, ct, L.raw_stream(at)))
+    return (r, y, kept) if compress else (r, y)
+
+
+def _kept_or_dense(t):
+    """(tensor, address of its exponents, what holds both)."""
+    if t is None:
+        return None, None, None
+    if type(t) is Compressed:
+        return t.values.data_ptr(), t.exponents.data_ptr(), t
+    t = _dense(t)
+    return t.data_ptr(), None, t
+
+
+def _on(t):
+    return t.values if type(t) is Compressed else t
+
+
+def residual_norm_backward(dr: torch.Tensor | None, dy: torch.Tensor | None, r, u=None, gate: torch.Tensor | None = None, x=None,
+                           scale: torch.Tensor | None = None, weight: torch.Tensor | None = None, gate_shift: torch.Tensor | None = None,
+                           samples: int = 1, eps: float = 1e-5, need_x: bool = True, need_u: bool = True, need_gate: bool = True, need_scale: bool = True,
+                           need_weight: bool = True, need_bias: bool = True, need_gate_shift: bool = True) -> ResidualNormGradients:
+    """Gradient of ``residual_norm`` from dr and dy, of r's and y's shapes and types (None: nothing came back through that result).
+
+    ``r`` is the forward pass's, a tensor or ``Compressed``; ``u`` too, whose values are read for the gate's gradient only, and ``x``, for the
+    scale's only (either may be left out where that is not asked for; du is then of dy's type, or of dr's).  dx is of the stream's type, du, dgate and d gate_shift of the blocks';
+    those of scale, weight and bias are float32.  Gates that samples share get the samples' sum.  Without gate and scale dx and du of one type are one tensor."""
+    base, first = _on(r), dy if dy is not None else dr
+    if first is None:
+        raise ValueError("residual_norm_backward: neither dr nor dy")
+    name = "residual_norm_backward"
+    at = _one_gpu(name, base, dr, dy, _on(u), gate, _on(x), scale, weight, gate_shift)
+    if at != L.current_device():
+        with L.on_device(base.device):
+            return residual_norm_backward(dr, dy, r, u, gate, x, scale, weight, gate_shift, samples, eps, need_x, need_u, need_gate, need_scale, need_weight,
+                                          need_bias, need_gate_shift)
+    shape, stream = r.shape, r.dtype
+    compute = u.dtype if u is not None else gate.dtype if gate is not None else first.dtype
+    if dy is None:                                   # the norm has no part in it
+        weight = gate_shift = None
+    gate_shape, shift_shape = None if gate is None else gate.shape, None if gate_shift is None else gate_shift.shape
+    rows, c, tokens, st, ct, gate, gate_ld, gs, gs_ld = _stream_operands(name, shape, stream, compute, u, gate, gate_shift, samples, (scale, weight))
+    if (dr is not None and (dr.shape != shape or dr.dtype != stream)) or (dy is not None and (dy.shape != shape or dy.dtype != compute)) or (
+            x is not None and (x.shape != shape or x.dtype != stream)):
+        raise ValueError(f"{name}: dr {None if dr is None else (dr.dtype, tuple(dr.shape))}, dy {None if dy is None else (dy.dtype, tuple(dy.shape))}, x "
+                         f"{None if x is None else (x.dtype, tuple(x.shape))} for r {stream} {tuple(shape)} computed in {compute}")
+    need_gate, need_scale = need_gate and gate is not None, need_scale and scale is not None
+    need_u = need_u and (u is not None or gate is not None)
+    if (need_gate and u is None) or (need_scale and x is None):
+        raise ValueError(f"{name}: the gate's gradient needs u, the scale's x")
+    if gs is not None and weight is not None:
+        raise ValueError(f"{name}: gate_shift stands in for the weight")
+    affine = dy is not None and gs is None
+    need_weight, need_bias = need_weight and affine and weight is not None, need_bias and affine
+    need_gate_shift = need_gate_shift and gs is not None
+    like = first.new_empty
+    one = need_u and gate is None and scale is None and stream == compute         # du is dx
+    dx = like(shape, dtype=stream) if need_x or one else None
+    du = dx if one else like(shape, dtype=compute) if need_u else None
+    dgate = like(gate_shape, dtype=compute) if need_gate else None
+    dgs = like(shift_shape, dtype=compute) if need_gate_shift else None
+    vector = lambda need, t: torch.empty(c if t is None else t.shape, dtype=torch.float32, device=first.device) if need else None
+    dw, db, dscale = vector(need_weight, weight), vector(need_bias, weight), vector(need_scale, scale)
+    lib = L.lib()
+    ws, size = None, 0
+    if need_weight or need_bias or need_scale:
+        ws = _call_workspace(first.device, lib.kfb_residual_norm_bwd_workspace_bytes(c))
+        size = ws.numel()
+    drc, dyc = None if dr is None else _dense(dr), None if dy is None else _dense(dy)
+    (rp, re, rk), (up, ue, uk), (xp, xe, xk) = _kept_or_dense(r), _kept_or_dense(u if need_gate else None), _kept_or_dense(x if need_scale else None)
+    sc, w = _affine(scale), _affine(weight)
+    L.check(lib.kfb_residual_norm_bwd(L.ptr(drc), L.ptr(dyc), rp, re, up, ue, xp, xe, L.ptr(gate), gate_ld, L.ptr(sc), L.ptr(w), L.ptr(gs), gs_ld, L.ptr(dx),
+                                      None if one else L.ptr(du), L.ptr(dgate), L.ptr(dgs), L.ptr(dw), L.ptr(db), L.ptr(dscale), L.ptr(ws), size, rows, c,
+                                      samples, tokens, eps, _NO_NORM if dy is None else _AFFINE_NORM if gs is None else _ADAPTIVE_NORM, st, ct,
+                                      L.raw_stream(at)))
+    return ResidualNormGradients(dx if need_x else None, du, dgate, dscale, dw, db, dgs)
+
+
+# ---- a linear layer with what follows it
+_ACTIVATIONS = {None: 0, "sigmoid": 1, "silu": 2, "gelu": 3, "relu": 4}
+
+
+def _linear_operands(name: str, x, w: torch.Tensor, bias: torch.Tensor | None, activation: str | None):
+    """(rows, in and out channels, activation's number, kernel's dtype code)."""
+    shape = x.shape
+    k = shape[-1] if shape else 0
+    n = w.shape[0] if w.dim() == 2 else 0
+    if w.shape != (n, k) or not n or not k or n % 8 or k % 8 or (bias is not None and bias.numel() != n):
+        raise ValueError(f"{name}: weight {tuple(w.shape)}, bias {None if bias is None else tuple(bias.shape)} for x {tuple(shape)} (channels multiples of 8)")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"{name}: activation {activation!r} (one of {', '.join(str(a) for a in _ACTIVATIONS)})")
+    if x.dtype not in _FEED_FORWARD_CODES or (w.dtype != x.dtype and w.dtype != torch.float32):
+        raise ValueError(f"{name}: x {x.dtype}, weight {w.dtype}")
+    return math.prod(shape[:-1]), k, n, _ACTIVATIONS[activation], _FEED_FORWARD_CODES[x.dtype]
+
+
+@lru_cache(maxsize=1024)
+def _fused_linear_bytes(at: int, *sizes: int) -> int:
+    """Scratch of a call on GPU `at`, which is current."""
+    return L.lib().kfb_fused_linear_workspace_bytes(*sizes)
+
+
+def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+                 residual: torch.Tensor | None = None) -> torch.Tensor:
+    """y = f(x w^T + bias) (+ residual) on plain parameters, for training (model/primitives/linear.py:25-107 with what follows it at its call sites).
+
+    x (..., K) bfloat16 (tensor-core arithmetic, float32 sums) or float32 (the fp32-accurate mode); w (N, K) of x's type, or float32 parameters that are
+    rounded to it here; bias (N,); activation None, "sigmoid", "silu", "gelu" (with the error function) or "relu".  ``residual`` (..., N) gives the
+    result its type: x's, or float32.  K and N multiples of 8."""
+    at = _one_gpu("fused_linear", x, w, bias, residual)
+    if at != L.current_device():
+        with L.on_device(x.device):
+            return fused_linear(x, w, bias, activation, residual)
+    rows, k, n, act, code = _linear_operands("fused_linear", x, w, bias, activation)
+    shape = (*x.shape[:-1], n)
+    if residual is not None and (residual.shape != shape or (residual.dtype != x.dtype and residual.dtype != torch.float32)):
+        raise ValueError(f"fused_linear: residual {residual.dtype} {tuple(residual.shape)} for x {x.dtype} {tuple(x.shape)} and {n} channels")
+    out = x.new_empty(shape, dtype=x.dtype if residual is None else residual.dtype)
+    need = _fused_linear_bytes(at, rows, k, n, act, code, 0, 0)
+    ws = _call_workspace(x.device, need) if need else None
+    xc, wc, b = _operand(x, x.dtype), _operand(w, x.dtype), _affine(bias)
+    rc = None if residual is None else _operand(residual, residual.dtype)
+    L.check(L.lib().kfb_fused_linear_fwd(xc.data_ptr(), wc.data_ptr(), L.ptr(b), L.ptr(rc), out.data_ptr(), L.ptr(ws), need, rows, k, n, act, code,
+                                         L.dtype_code(out.dtype), L.raw_stream(at)))
+    return out
+
+
+def fused_linear_backward(dy: torch.Tensor, x, w: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None, need_x: bool = True,
+                          need_w: bool = True, need_bias: bool = True):
+    """Gradient of ``fused_linear``: (dx, dw, dbias) from dy, of y's shape and of x's type or float32; None where there is no such input or it was not
+    asked for.  The residual's gradient is dy.  ``x`` is the tensor or ``Compressed``.  dx is of x's type, dw of w's (float32 sums either way), dbias
+    float32.  What the activation was taken of is computed again."""
+    at = _one_gpu("fused_linear_backward", _on(x), w, bias, dy)
+    if at != L.current_device():
+        with L.on_device(dy.device):
+            return fused_linear_backward(dy, x, w, bias, activation, need_x, need_w, need_bias)
+    rows, k, n, act, code = _linear_operands("fused_linear_backward", x, w, bias, activation)
+    if dy.shape != (*x.shape[:-1], n) or (dy.dtype != x.dtype and dy.dtype != torch.float32):
+        raise ValueError(f"fused_linear_backward: dy {dy.dtype} {tuple(dy.shape)} for x {x.dtype} {tuple(x.shape)} and {n} channels")
+    need_bias = need_bias and bias is not None
+    wanted = bool(need_x) + 2 * bool(need_w) + 4 * need_bias
+    if not wanted:
+        return None, None, None
+    dt = x.dtype
+    dx = dy.new_empty(x.shape, dtype=dt) if need_x else None
+    dw = torch.empty(w.shape, dtype=w.dtype, device=dy.device) if need_w else None
+    db = torch.empty(bias.shape, dtype=torch.float32, device=dy.device) if need_bias else None
+    dyc, wc, b = _operand(dy, dy.dtype), _operand(w, dt), _affine(bias)
+    xc = _operand(_expanded(x), dt) if need_w or act else None
+    need = _fused_linear_bytes(at, rows, k, n, act, code, L.dtype_code(dy.dtype), wanted)
+    ws = _call_workspace(dy.device, need) if need else None
+    L.check(L.lib().kfb_fused_linear_bwd(dyc.data_ptr(), L.ptr(xc), wc.data_ptr(), L.ptr(b), L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), need, rows, k, n,
+                                         act, code, L.dtype_code(dy.dtype), L.dtype_code(w.dtype), L.raw_stream(at)))
+    return dx, dw, db
+
 
 
 def triangle_multiplication(x: torch.Tensor, mask: torch.Tensor, packed: dict, direction: str, eps: float = 1e-5,

@@ -14,8 +14,8 @@ modules they stand in for, with the CUDA kernels behind them:
 
 Conventions copied from the reference's Triton backend
 (model/primitives/triangle_multiplication.py:94-145): inference only (``RuntimeError``
-when autograd is recording or the input is not on a CUDA device; LayerNorm, Transition and
-Dropout are trained too and record their gradients), compute dtype =
+when autograd is recording or the input is not on a CUDA device; LayerNorm, Transition, Dropout,
+Linear, AdaLN and ConditionedTransitionBlock are trained too and record their gradients), compute dtype =
 autocast dtype if autocast is on else the input dtype, result returned in the input
 dtype, weights packed once per module and re-packed when a parameter's storage or
 version changes.
@@ -62,7 +62,8 @@ class LayerNorm(nn.Module):
 
 
 class Linear(nn.Module):
-    """Parameter holder for a projection; N(0, 1/fan_in) init (model/primitives/linear.py:25-107)."""
+    """A projection; N(0, 1/fan_in) init (model/primitives/linear.py:25-107); differentiable.  The blocks read its parameters; called by itself it
+    computes in the compute dtype, which is its result's.  Channels multiples of 8."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True):
         super().__init__()
@@ -71,6 +72,16 @@ class Linear(nn.Module):
             self.bias = nn.Parameter(torch.zeros(out_features))
         else:
             self.register_parameter("bias", None)
+
+    @torch.compiler.disable
+    def forward(self, x: torch.Tensor, activation: str | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
+        """f(x W^T + b) (+ residual), f one of functional.fused_linear's."""
+        cd = compute_dtype(x)
+        _is_precise(cd, type(self).__name__)
+        if not x.is_cuda:
+            raise RuntimeError("The kfold_b200 kernel backend requires CUDA tensors.")
+        with torch.autocast(x.device.type, enabled=False):
+            return (A if torch.is_grad_enabled() else F).fused_linear(x.to(cd), self.weight, self.bias, activation, residual)
 
 
 class LinearNoBias(Linear):
@@ -306,12 +317,26 @@ class AdaLN(_PackedMixin, nn.Module):
     @torch.compiler.disable
     def forward(self, a: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
         """a (B, Ns, L, c_a), s (B, 1 or Ns, L, c_s) -> (B, Ns, L, c_a): bf16 under bfloat16 compute, float32 under
-        float32 compute."""
-        _check_inference(a)
+        float32 compute.  While autograd records, gradients for a, s and all parameters."""
         precise = _is_precise(compute_dtype(a), "AdaLN")
+        if torch.is_grad_enabled():
+            with torch.autocast(a.device.type, enabled=False):
+                s, samples = _shared_conditioning(a, s)
+                return self._training(a, s, samples, torch.float32 if precise else torch.bfloat16)
+        _check_inference(a)
         with torch.autocast(a.device.type, enabled=False):
             s, samples = _shared_conditioning(a, s)
             return F.adaln(a, self.gate_shift(s, precise), samples)
+
+    def _training(self, a: torch.Tensor, s: torch.Tensor, samples: int, cd: torch.dtype) -> torch.Tensor:
+        """While autograd records: the parameters as they are; gates and shifts from one product."""
+        if not a.is_cuda:
+            raise RuntimeError("The kfold_b200 kernel backend requires CUDA tensors.")
+        ln, g = self.layernorm_s, self.linear_g
+        sn = A.layer_norm(s.to(cd) if s.dtype != torch.float32 else s, ln.weight, ln.bias, ln.eps, out_dtype=cd)
+        bias = torch.cat((g.bias, torch.zeros_like(g.bias)))
+        gs = A.fused_linear(sn, torch.cat((g.weight, self.linear_bias.weight)), bias)
+        return A.residual_norm(a if a.dtype == torch.float32 else a.to(cd), gate_shift=gs, samples=samples)[1]
 
 
 def _shared_conditioning(a: torch.Tensor, s: torch.Tensor):
@@ -512,9 +537,11 @@ class ConditionedTransitionBlock(_PackedMixin, nn.Module):
                 cond=None) -> torch.Tensor:
         """``precise`` overrides the choice made from the compute dtype (for callers that already run with autocast
         switched off).  ``cond``: (gate/shift rows, output gate logits) from a stack's conditioning tables."""
-        _check_inference(a)
         if precise is None:
             precise = _is_precise(compute_dtype(a), "ConditionedTransitionBlock")
+        if torch.is_grad_enabled() and cond is None:
+            return self._training(a, s, residual, torch.float32 if precise else torch.bfloat16)
+        _check_inference(a)
         pk = self._packed_transition(a.device, precise)
         with torch.autocast(a.device.type, enabled=False):
             s, share = _shared_conditioning(a, s)
@@ -527,6 +554,15 @@ class ConditionedTransitionBlock(_PackedMixin, nn.Module):
                 an = F.adaln(a, self.adaln.gate_shift(s), share)
                 gate = F.linear(s, pk["w_g"], pk["b_g"])
             return F.conditioned_transition(an, pk, gate, share, resid=a if residual else None, out_dtype=a.dtype)
+
+    def _training(self, a: torch.Tensor, s: torch.Tensor, residual: bool, cd: torch.dtype) -> torch.Tensor:
+        """While autograd records: the parameters as they are, gradients for all of them, a and s."""
+        with torch.autocast(a.device.type, enabled=False):
+            s, share = _shared_conditioning(a, s)
+            a_in = a if a.dtype == torch.float32 else a.to(cd)
+            u = A.gated_feed_forward(self.adaln._training(a_in, s, share, cd), self.swiglu.linear.weight, self.linear_out.weight)
+            gate = A.fused_linear(s.to(cd), self.linear_g.weight, self.linear_g.bias)
+            return A.residual_norm(a_in if residual else None, u, gate, samples=share, norm=False)[0].to(a.dtype)
 
 
 class SingleConditioning(nn.Module):

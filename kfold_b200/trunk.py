@@ -16,6 +16,7 @@ import torch
 import torch.nn.functional as tF
 from torch import nn
 
+from . import autograd as A
 from . import functional as F
 from . import packing
 from .modules import LayerNorm, Linear, LinearNoBias, Transition, _check_inference, _is_precise, compute_dtype
@@ -59,14 +60,27 @@ class ParcaeRecurrence(nn.Module):
 
     @torch.compiler.disable
     def forward(self, z: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
-        """z, u (B, N, N, C) -> a * z + Linear_b(LayerNorm(u)), same shape and dtype as z."""
-        _check_inference(z)
+        """z, u (B, N, N, C) -> a * z + Linear_b(LayerNorm(u)), same shape and dtype as z.  While autograd records, gradients for z, u and all parameters."""
         if _is_precise(compute_dtype(z), "ParcaeRecurrence"):
             raise NotImplementedError("ParcaeRecurrence: bfloat16 compute only (the trunk runs under autocast(bfloat16))")
+        if torch.is_grad_enabled():
+            return self._training(z, u)
+        _check_inference(z)
         a, b = self.dynamics(z.device)
         ln = self.layernorm_z
         with torch.autocast(z.device.type, enabled=False):
             return F.parcae_update(z, u, ln.weight, ln.bias, a, b, ln.eps)
+
+    def _training(self, z: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
+        if not z.is_cuda:
+            raise RuntimeError("The kfold_b200 kernel backend requires CUDA tensors.")
+        ln = self.layernorm_z
+        with torch.autocast(z.device.type, enabled=False):
+            delta = tF.softplus(self.parcae_log_delta.float())
+            a = torch.exp(-delta * torch.exp(self.parcae_log_a.float())).to(torch.bfloat16).float()
+            b = delta[:, None] * self.parcae_b_cont.float()
+            un = A.layer_norm(u, ln.weight, ln.bias, ln.eps, out_dtype=torch.bfloat16)
+            return A.residual_norm(z, A.fused_linear(un, b), scale=a, norm=False)[0]
 
 
 class LMToPair(nn.Module):

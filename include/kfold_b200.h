@@ -692,9 +692,10 @@ KFB_API int kfb_residual_norm_fwd(const void* x, const void* u, const void* gate
  *   dx = scale t, du = s t, dgate = s (1 - s) sum(t u), dgate_shift = [m (1 - m) sum(dy z) | sum(dy)] over the samples that share a row
  *   (compute_dtype, dense), dweight = sum(dy z), dbias = sum(dy), dscale = sum(t x) over all rows (fp32).
  * Outputs that are NULL are not computed.  dr NULL: zero; dy is not read with norm 0.  r, u and x (u: for dgate, x: for dscale only) are the
- * tensors, or the values of kfb_compress where their exponents are given.  The workspace is needed for dweight, dbias and dscale.
+ * tensors, or the values of kfb_compress where their exponents are given.  Workspace: `sums` whether dweight, dbias or dscale are wanted,
+ * `gates` whether dgate or dgate_shift are; it may be none.
  */
-KFB_API size_t kfb_residual_norm_bwd_workspace_bytes(int c);
+KFB_API size_t kfb_residual_norm_bwd_workspace_bytes(long long rows, int c, int samples, int sums, int gates);
 KFB_API int kfb_residual_norm_bwd(const void* dr, const void* dy, const void* r, const void* r_exponents, const void* u, const void* u_exponents,
                                   const void* x, const void* x_exponents, const void* gate, long long gate_ld, const float* scale,
                                   const float* weight, const void* gate_shift, long long gate_shift_ld, void* dx, void* du, void* dgate,

@@ -148,7 +148,7 @@ _SIZE_FUNCS = {
     "kfb_feed_forward_call_bytes": [c_ll, c_int, c_int, c_int, c_int],
     "kfb_feed_forward_workspace_bytes": [c_ll, c_int, c_int, c_int, c_int],
     "kfb_layernorm_bwd_workspace_bytes": [c_int],
-    "kfb_residual_norm_bwd_workspace_bytes": [c_int],
+    "kfb_residual_norm_bwd_workspace_bytes": [c_ll, c_int, c_int, c_int, c_int],
     "kfb_fused_linear_workspace_bytes": [c_ll, c_int, c_int, c_int, c_int, c_int, c_int],
     "kfb_triatt_workspace_bytes_precise": [c_int, c_int, c_int, c_int],
     "kfb_apb_workspace_bytes_precise": [c_int, c_int, c_int],

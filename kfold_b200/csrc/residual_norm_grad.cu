@@ -5,12 +5,13 @@
 //
 // What bounds it: dr, dy, r and u in, dx and du out, HBM.  Row statistics come from r again.  r, u and x may be the tensors or rows kept in 8 bits
 // (row_teams.cuh), which are taken apart in registers.
-// Split: as in residual_norm.cu a team of lanes holds a row and walks the samples that share its gates, their sums in registers; where gate rows are
-// few the teams of a block take the samples of one row between them and meet in shared memory.  Sums over all rows stay in registers from row to
-// row; a block leaves a row of partial sums, which a second kernel adds in the blocks' order.  No atomics: the order hangs on the sizes alone.
+// Split: residual_norm.cuh says how rows are walked and come in.  A team keeps the sums over the samples of a gate row in registers; where these samples are
+// cut into pieces, a piece leaves its sums in the workspace and a second kernel adds them in the pieces' order.  Sums over all rows stay in registers from row
+// to row; a block leaves a row of partial sums, added up likewise.  No atomics: the order hangs on the sizes alone.
+#include <mutex>
+
 #include "ops_common.cuh"
 #include "residual_norm.cuh"
-#include "row_teams.cuh"
 
 namespace kfb {
 namespace {
@@ -22,151 +23,154 @@ struct GradParams {
   long long gate_ld, gate_shift_ld;
   void *dx, *du, *dgate, *dgate_shift;
   float* partial;                      // [block][3][c]: sums of dy z, dy, t x
-  RowShare share;
-  unsigned sets;                       // of gate rows that a group (split: a block) takes at a time
-  int chunk, split;
+  float* pieces;                       // [unit][3][c]: a piece's sums of dy z, dy, t u; null: a gate row's samples are one piece
+  RowPlan plan;
   int c, norm;
   float eps;
+  int slots, s_dy, s_r, s_u, s_x, s_gate, s_g;    // slots of a stage, and the first of each tensor (dr: 0)
+  int words;                           // exponents come in words of four (a row's are whole words, and start on one)
 };
 
 // OWN: a row has gates of its own.
 template <typename TS, typename TC, int LANES, bool VEC, bool OWN>
-__global__ void __launch_bounds__(Teams<LANES>::kThreads) residual_norm_grad_kernel(const GradParams p) {
+__global__ void __launch_bounds__(Teams<LANES>::kThreads, 2) residual_norm_grad_kernel(const GradParams p) {
   using T = Teams<LANES>;
-  constexpr int N = kPiece;
+  constexpr int N = kPiece, kThreads = T::kThreads, kDepth = OWN ? 3 : 4;      // rows on their way for a team, the one in work among them
   __shared__ float room[2][T::kGroups][T::kWarps][2];
-  __shared__ float4 s_sum[OWN ? 1 : 3][T::kThreads * 2];
+  extern __shared__ uint4 ring_memory[];
   grid_dependency_enter();
   const int group = threadIdx.x / T::kGroupLanes, sub = threadIdx.x % LANES, team = threadIdx.x % T::kGroupLanes / LANES;
-  const int ch = sub * N, n = min(max(p.c - ch, 0), N), groups = groups8(p.c);
+  const int ch = sub * N, n = min(max(p.c - ch, 0), N), groups = groups8(p.c), e_shift = ch / kGroup8 % 4 * 8;
   const float inv_c = 1.0f / static_cast<float>(p.c);
-  const TS *dr = static_cast<const TS*>(p.dr), *r = static_cast<const TS*>(p.r), *x = static_cast<const TS*>(p.x);
-  const TC *dy = static_cast<const TC*>(p.dy), *u = static_cast<const TC*>(p.u), *gate = static_cast<const TC*>(p.gate),
-           *gs = static_cast<const TC*>(p.gate_shift);
+  const TS* dr = static_cast<const TS*>(p.dr);
+  const TC *dy = static_cast<const TC*>(p.dy), *gate = static_cast<const TC*>(p.gate), *gs = static_cast<const TC*>(p.gate_shift);
   const bool adaptive = p.norm == kAdaptiveNorm;
+  uint4* ring = ring_memory + threadIdx.x;
 
-  float m[N], open[N], a0[N], a1[N], a2[N], a3[N];
+  float m[N], open[OWN ? 1 : N], a0[N], a1[N], a2[OWN ? 1 : N], a3[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     m[i] = p.weight != nullptr && i < n ? p.weight[ch + i] : 1.f;
+    a0[i] = a1[i] = a3[i] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < (OWN ? 1 : N); ++i) {
     open[i] = 1.f;
-    a0[i] = a1[i] = a2[i] = a3[i] = 0.f;
+    a2[i] = 0.f;
   }
 
-  const unsigned step = p.split ? gridDim.x : gridDim.x * T::kGroups;
-  unsigned set = p.split ? blockIdx.x : blockIdx.x * T::kGroups + group, row = 0, cond = 0;
-  int left = 0, at = 0;
-  bool there = false;
-  Piece<TS, VEC> dr_raw, r_raw, x_raw;
-  Piece<TC, VEC> dy_raw, u_raw, gate_raw, g_raw;
-  auto enter = [&] {
-    const unsigned unit = set * T::kTeams + team;
-    there = unit < p.share.cond_rows;
-    const int first = p.split ? group * p.chunk : 0;
-    cond = there ? unit : 0;
-    left = there ? min(p.chunk, p.share.samples - first) : 0;
-    row = OWN ? cond : p.share.row(cond, first);
-  };
-  auto gates = [&] {
-    const int k = there ? n : 0;
-    if (gate != nullptr) gate_raw.load(gate + cond * p.gate_ld + ch, k);
-    if (gs != nullptr) g_raw.load(gs + cond * p.gate_shift_ld + ch, k);
-  };
-  auto fetch = [&] {
-    const int k = left > 0 ? n : 0;
-    const long long o = static_cast<long long>(row) * p.c + ch, e = static_cast<long long>(row) * groups + ch / kGroup8;
-    if (dr != nullptr) dr_raw.load(dr + o, k);
-    if (p.norm != kNoNorm) {
-      dy_raw.load(dy + o, k);
-      if (p.r_e != nullptr) r_raw.load8(static_cast<const uint8_t*>(p.r) + o, p.r_e + e, k);
-      else r_raw.load(r + o, k);
-    }
-    if (p.dgate != nullptr) {
-      if (p.u_e != nullptr) u_raw.load8(static_cast<const uint8_t*>(p.u) + o, p.u_e + e, k);
-      else u_raw.load(u + o, k);
-    }
-    if (p.x != nullptr) {
-      if (p.x_e != nullptr) x_raw.load8(static_cast<const uint8_t*>(p.x) + o, p.x_e + e, k);
-      else x_raw.load(x + o, k);
+  const unsigned step = gridDim.x * T::kGroups;
+  Walk<LANES, OWN> here, ahead;
+  here.set = blockIdx.x * T::kGroups + group;
+  if (here.set < p.plan.sets) here.enter(p.plan, team);
+  ahead = here;
+  // a tensor of the stream's or the blocks' type, or its rows in 8 bits, into its slots and out of them
+  auto copy = [&](auto tag, int slot, int stage, const void* q, const uint8_t* e, unsigned row, bool there) {
+    using E = decltype(tag);
+    uint4* to = ring + (stage * p.slots + slot) * kThreads;
+    const long long o = static_cast<long long>(row) * p.c + ch;
+    if (e == nullptr) {
+      ring_copy<E, VEC>(to, kThreads, static_cast<const E*>(q) + o, there);
+    } else {
+      copy_async<8>(to, static_cast<const uint8_t*>(q) + o, there);
+      if (p.words) copy_async<4>(reinterpret_cast<uint32_t*>(to) + 2, e + static_cast<long long>(row) * groups + (ch / kGroup8 & ~3), there);
     }
   };
-  if (set < p.sets) {
-    enter();
-    fetch();
-    if (OWN) gates();
-  }
-  int turn = 0;
-  while (set < p.sets) {
-    float t[N], v[N], d[N], z[N], slope_m[OWN ? N : 1], slope_u[OWN ? N : 1];
-    const unsigned this_row = row, this_cond = cond;
-    const int here = left > 0 ? n : 0, cond_here = there ? n : 0;
-    const bool fresh = at == 0;
-    if (fresh) {
-      if (!OWN) gates();
-      if (gate != nullptr) {
-        gate_raw.values(t);
+  auto take = [&](auto tag, int slot, int stage, const void* q, const uint8_t* e, float* v) {
+    using E = decltype(tag);
+    Piece<E, VEC> raw;
+    const int k = here.left > 0 ? n : 0;
+    [[maybe_unused]] const uint4* from = ring + (stage * p.slots + slot) * kThreads;
+    [[maybe_unused]] const long long o = static_cast<long long>(here.row) * p.c + ch;
+    const uint8_t* ep = e == nullptr ? nullptr : e + static_cast<long long>(here.row) * groups + ch / kGroup8;
+    if (e == nullptr) {
+      if constexpr (VEC) raw.take(from, kThreads);
+      else raw.load(static_cast<const E*>(q) + o, k);
+      raw.values(v);
+    } else {
+      if constexpr (VEC) {
+        raw.take8(from, e_shift);
+        if (!p.words) raw.w[2] = k > 0 ? *ep : 0u;
+      } else {
+        raw.load8(static_cast<const uint8_t*>(q) + o, ep, k);
+      }
+      raw.values_of_8(v);
+    }
+  };
+  auto fetch = [&](int stage) {
+    if (ahead.set < p.plan.sets) {
+      const bool there = ahead.left > 0 && n > 0;
+      if (dr != nullptr) copy(TS{}, 0, stage, dr, nullptr, ahead.row, there);
+      if (p.norm != kNoNorm) {
+        copy(TC{}, p.s_dy, stage, dy, nullptr, ahead.row, there);
+        copy(TS{}, p.s_r, stage, p.r, p.r_e, ahead.row, there);
+      }
+      if (p.dgate != nullptr) copy(TC{}, p.s_u, stage, p.u, p.u_e, ahead.row, there);
+      if (p.x != nullptr) copy(TS{}, p.s_x, stage, p.x, p.x_e, ahead.row, there);
+      if (OWN) {
+        if (gate != nullptr) ring_copy<TC, VEC>(ring + (stage * p.slots + p.s_gate) * kThreads, kThreads, gate + ahead.row * p.gate_ld + ch, there);
+        if (gs != nullptr) ring_copy<TC, VEC>(ring + (stage * p.slots + p.s_g) * kThreads, kThreads, gs + ahead.row * p.gate_shift_ld + ch, there);
+      }
+      ahead.next(p.plan, team, step);
+    }
+    copy_async_done();
+  };
+  // logits of this row's gate, or of the norm's
+  auto logits = [&](const TC* table, long long ld, int slot, int stage, unsigned gate_row, int k, float* v) {
+    Piece<TC, VEC> raw;
+    if (OWN && VEC) raw.take(ring + (stage * p.slots + slot) * kThreads, kThreads);
+    else raw.load(table + gate_row * ld + ch, k);
+    raw.values(v);
+  };
+  if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const Gate q = gate_at(t[i]);
-          open[i] = q.open;
-          if (OWN) slope_u[i] = q.slope;
-        }
+    for (int i = 0; i < kDepth - 1; ++i) fetch(i);
+  }
+  int stage = 0;
+  while (here.set < p.plan.sets) {
+    if constexpr (VEC) {
+      fetch(stage == 0 ? kDepth - 1 : stage - 1);
+      copy_async_wait<kDepth - 1>();
+    }
+    const int k = here.left > 0 ? n : 0;
+    const bool row_there = here.left > 0;
+    const long long o = static_cast<long long>(here.row) * p.c + ch;
+    float t[N], v[N];
+    if (!OWN && here.at == 0) {
+      const unsigned gate_row = here.gate_row(p.plan);
+      if (gate != nullptr) {
+        logits(gate, p.gate_ld, 0, 0, gate_row, k, t);
+#pragma unroll
+        for (int i = 0; i < (OWN ? 1 : N); ++i) open[i] = gate_at(t[i]).open;
       }
       if (gs != nullptr) {
-        g_raw.values(t);
+        logits(gs, p.gate_shift_ld, 0, 0, gate_row, k, t);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const Gate q = gate_at(t[i]);
-          m[i] = q.open;
-          if (OWN) slope_m[i] = q.slope;
-        }
+        for (int i = 0; i < N; ++i) m[i] = gate_at(t[i]).open;
       }
     }
+    if (OWN && gs != nullptr) {
+      logits(gs, p.gate_shift_ld, p.s_g, stage, here.row, k, t);
+#pragma unroll
+      for (int i = 0; i < N; ++i) m[i] = gate_at(t[i]).open;
+    }
     if (dr != nullptr) {
-      dr_raw.values(t);
+      take(TS{}, 0, stage, dr, nullptr, t);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) t[i] = 0.f;
     }
-    float uv[N], xv[N];
     if (p.norm != kNoNorm) {
-      dy_raw.values(d);
-      if (p.r_e != nullptr) r_raw.values_of_8(z);
-      else r_raw.values(z);
-    }
-    if (p.dgate != nullptr) {
-      if (p.u_e != nullptr) u_raw.values_of_8(uv);
-      else u_raw.values(uv);
-    }
-    if (p.x != nullptr) {
-      if (p.x_e != nullptr) x_raw.values_of_8(xv);
-      else x_raw.values(xv);
-    }
-    // on to the next row, whose loads have to stand before this one's stores
-    bool last = OWN;
-    if (OWN || ++at == p.chunk) {
-      last = true;
-      at = 0;
-      set += step;
-      if (set < p.sets) {
-        enter();
-        if (OWN) gates();
-      }
-    } else {
-      --left;
-      row += p.share.l;
-    }
-    if (set < p.sets) fetch();
-
-    if (p.norm != kNoNorm) {
+      float d[N], z[N];
+      take(TC{}, p.s_dy, stage, dy, nullptr, d);
+      take(TS{}, p.s_r, stage, p.r, p.r_e, z);
       float s[2] = {0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         s[0] += z[i];
         s[1] = fmaf(d[i], m[i], s[1]);
       }
-      team_sum<LANES>(s, room, group, turn);
-      turn ^= 1;
+      team_sum<LANES>(s, room, group, 0);
       const float mean = s[0] * inv_c, mean_g = s[1] * inv_c;
       s[0] = s[1] = 0.f;
 #pragma unroll
@@ -175,8 +179,7 @@ __global__ void __launch_bounds__(Teams<LANES>::kThreads) residual_norm_grad_ker
         s[0] = fmaf(z[i], z[i], s[0]);
         s[1] = fmaf(d[i] * m[i], z[i], s[1]);
       }
-      team_sum<LANES>(s, room, group, turn);
-      turn ^= 1;
+      team_sum<LANES>(s, room, group, 1);
       const float rstd = rsqrtf(fmaf(s[0], inv_c, p.eps)), mean_gz = s[1] * inv_c * rstd;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -185,95 +188,85 @@ __global__ void __launch_bounds__(Teams<LANES>::kThreads) residual_norm_grad_ker
       }
       if (OWN && adaptive) {
         if (p.dgate_shift != nullptr) {
+          logits(gs, p.gate_shift_ld, p.s_g, stage, here.row, k, v);
 #pragma unroll
-          for (int i = 0; i < N; ++i) v[i] = d[i] * z[i] * slope_m[i];
-          TC* o = static_cast<TC*>(p.dgate_shift) + static_cast<long long>(this_row) * 2 * p.c + ch;
-          store_piece<VEC>(o, v, here);
-          store_piece<VEC>(o + p.c, d, here);
+          for (int i = 0; i < N; ++i) v[i] = d[i] * z[i] * gate_at(v[i]).slope;
+          TC* q = static_cast<TC*>(p.dgate_shift) + static_cast<long long>(here.row) * 2 * p.c + ch;
+          store_piece<VEC>(q, v, k);
+          store_piece<VEC>(q + p.c, d, k);
         }
       } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          a0[i] = fmaf(d[i], here > 0 ? z[i] : 0.f, a0[i]);      // (z of no row is not a number where eps is zero)
+          a0[i] = fmaf(d[i], row_there ? z[i] : 0.f, a0[i]);      // (z of no row is not a number where eps is zero)
           a1[i] += d[i];
         }
       }
     }
-    const long long o = static_cast<long long>(this_row) * p.c + ch;
     if (p.dgate != nullptr) {
-      if (OWN) {
+      take(TC{}, p.s_u, stage, p.u, p.u_e, v);
+      if constexpr (OWN) {
+        float s[N];
+        logits(gate, p.gate_ld, p.s_gate, stage, here.row, k, s);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = t[i] * uv[i] * slope_u[i];
-        store_piece<VEC>(static_cast<TC*>(p.dgate) + o, v, here);
+        for (int i = 0; i < N; ++i) v[i] = t[i] * v[i] * gate_at(s[i]).slope;
+        store_piece<VEC>(static_cast<TC*>(p.dgate) + o, v, k);
       } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) a2[i] = fmaf(here > 0 ? t[i] : 0.f, uv[i], a2[i]);
+        for (int i = 0; i < N; ++i) a2[i] = fmaf(row_there ? t[i] : 0.f, v[i], a2[i]);
       }
     }
     if (p.x != nullptr) {
+      take(TS{}, p.s_x, stage, p.x, p.x_e, v);
 #pragma unroll
-      for (int i = 0; i < N; ++i) a3[i] = fmaf(here > 0 ? t[i] : 0.f, xv[i], a3[i]);
+      for (int i = 0; i < N; ++i) a3[i] = fmaf(row_there ? t[i] : 0.f, v[i], a3[i]);
     }
     if (p.du != nullptr) {
+      if (OWN && gate != nullptr) {
+        logits(gate, p.gate_ld, p.s_gate, stage, here.row, k, v);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = t[i] * open[i];
-      store_piece<VEC>(static_cast<TC*>(p.du) + o, v, here);
+        for (int i = 0; i < N; ++i) v[i] = t[i] * gate_at(v[i]).open;
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = t[i] * open[OWN ? 0 : i];
+      }
+      store_piece<VEC>(static_cast<TC*>(p.du) + o, v, k);
     }
     if (p.dx != nullptr) {
       if (p.scale != nullptr) {
 #pragma unroll
         for (int i = 0; i < N; ++i) t[i] *= i < n ? p.scale[ch + i] : 0.f;
       }
-      store_piece<VEC>(static_cast<TS*>(p.dx) + o, t, here);
+      store_piece<VEC>(static_cast<TS*>(p.dx) + o, t, k);
     }
     if constexpr (!OWN) {
-      if (last) {
-        // the gates' gradients from the sums over their samples; the logits once more, for their slopes
-        bool mine = true;
-        if (p.split) {
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            const float* a = k == 0 ? a0 : k == 1 ? a1 : a2;
-            s_sum[k][threadIdx.x * 2] = make_float4(a[0], a[1], a[2], a[3]);
-            s_sum[k][threadIdx.x * 2 + 1] = make_float4(a[4], a[5], a[6], a[7]);
+      if (here.at + 1 == p.plan.chunk) {
+        // the end of a piece: the gates' gradients from the sums over their samples, the logits once more for their slopes; or the sums for the second kernel
+        const bool there = here.unit < p.plan.units;
+        const int kk = there ? n : 0;
+        const unsigned gate_row = here.gate_row(p.plan);
+        if (p.pieces != nullptr) {
+          float* q = p.pieces + static_cast<long long>(there ? here.unit : 0) * 3 * p.c + ch;
+          if (adaptive) {
+            store_piece<VEC>(q, a0, kk);
+            store_piece<VEC>(q + p.c, a1, kk);
           }
-          __syncthreads();
-          mine = group == 0;
-          if (mine) {
+          if (p.dgate != nullptr) store_piece<VEC>(q + 2 * p.c, a2, kk);
+        } else {
+          if (adaptive && p.dgate_shift != nullptr) {
+            logits(gs, p.gate_shift_ld, 0, 0, gate_row, kk, v);
 #pragma unroll
-            for (int k = 0; k < 3; ++k) {
-              if (k < 2 && !adaptive) continue;
-              float* a = k == 0 ? a0 : k == 1 ? a1 : a2;
-              for (int q = 1; q < T::kGroups; ++q) {
-                const float4 lo = s_sum[k][(q * T::kGroupLanes + threadIdx.x) * 2], hi = s_sum[k][(q * T::kGroupLanes + threadIdx.x) * 2 + 1];
-                a[0] += lo.x;
-                a[1] += lo.y;
-                a[2] += lo.z;
-                a[3] += lo.w;
-                a[4] += hi.x;
-                a[5] += hi.y;
-                a[6] += hi.z;
-                a[7] += hi.w;
-              }
-            }
+            for (int i = 0; i < N; ++i) v[i] = a0[i] * gate_at(v[i]).slope;
+            TC* q = static_cast<TC*>(p.dgate_shift) + static_cast<long long>(gate_row) * 2 * p.c + ch;
+            store_piece<VEC>(q, v, kk);
+            store_piece<VEC>(q + p.c, a1, kk);
           }
-          __syncthreads();
-        }
-        if (mine && adaptive && p.dgate_shift != nullptr) {
-          g_raw.load(gs + this_cond * p.gate_shift_ld + ch, cond_here);
-          g_raw.values(v);
+          if (p.dgate != nullptr) {
+            logits(gate, p.gate_ld, 0, 0, gate_row, kk, v);
 #pragma unroll
-          for (int i = 0; i < N; ++i) v[i] = a0[i] * gate_at(v[i]).slope;
-          TC* q = static_cast<TC*>(p.dgate_shift) + static_cast<long long>(this_cond) * 2 * p.c + ch;
-          store_piece<VEC>(q, v, cond_here);
-          store_piece<VEC>(q + p.c, a1, cond_here);
-        }
-        if (mine && p.dgate != nullptr) {
-          gate_raw.load(gate + this_cond * p.gate_ld + ch, cond_here);
-          gate_raw.values(v);
-#pragma unroll
-          for (int i = 0; i < N; ++i) v[i] = a2[i] * gate_at(v[i]).slope;
-          store_piece<VEC>(static_cast<TC*>(p.dgate) + static_cast<long long>(this_cond) * p.c + ch, v, cond_here);
+            for (int i = 0; i < N; ++i) v[i] = a2[i] * gate_at(v[i]).slope;
+            store_piece<VEC>(static_cast<TC*>(p.dgate) + static_cast<long long>(gate_row) * p.c + ch, v, kk);
+          }
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -282,23 +275,26 @@ __global__ void __launch_bounds__(Teams<LANES>::kThreads) residual_norm_grad_ker
         }
       }
     }
+    here.next(p.plan, team, step);
+    stage = stage + 1 == kDepth ? 0 : stage + 1;
   }
 
   if (p.partial != nullptr) {
-    // the block's teams in their order
-    float* flat = reinterpret_cast<float*>(s_sum[0]);      // [team][LANES * 8]
+    // the block's teams in their order; the ring's memory, in which nothing is on its way any more
+    copy_async_wait<0>();
+    float* flat = reinterpret_cast<float*>(ring_memory);      // [team][LANES * 8]
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      const float* a = k == 0 ? a0 : k == 1 ? a1 : a3;
+    for (int j = 0; j < 3; ++j) {
+      const float* a = j == 0 ? a0 : j == 1 ? a1 : a3;
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < N; ++i) flat[(group * T::kTeams + team) * LANES * N + ch + i] = a[i];
       __syncthreads();
-      for (int i = threadIdx.x; i < p.c; i += T::kThreads) {
+      for (int i = threadIdx.x; i < p.c; i += kThreads) {
         float s = 0.f;
 #pragma unroll 4
         for (int q = 0; q < T::kGroups * T::kTeams; ++q) s += flat[q * LANES * N + i];
-        p.partial[(static_cast<long long>(blockIdx.x) * 3 + k) * p.c + i] = s;
+        p.partial[(static_cast<long long>(blockIdx.x) * 3 + j) * p.c + i] = s;
       }
     }
   }
@@ -325,32 +321,94 @@ __global__ void __launch_bounds__(1024) residual_norm_sum_kernel(const float* pa
   }
 }
 
+// The gates' gradients of rows whose samples were cut into pieces, in the order of the pieces.  A thread takes a channel of a row.
+template <typename TC>
+__global__ void __launch_bounds__(256) residual_norm_gates_kernel(const float* pieces, const TC* gate, long long gate_ld, const TC* gs, long long gs_ld, TC* dgate,
+                                                                  TC* dgs, unsigned gate_rows, int chunks, int c) {
+  grid_dependency_enter();
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < static_cast<long long>(gate_rows) * c; i += gridDim.x * 256ll) {
+    const unsigned row = static_cast<unsigned>(i / c);
+    const int ch = static_cast<int>(i - static_cast<long long>(row) * c);
+    float s[3] = {0.f, 0.f, 0.f};
+    const float* q = pieces + static_cast<long long>(row) * chunks * 3 * c + ch;
+#pragma unroll 4
+    for (int k = 0; k < chunks; ++k, q += 3ll * c) {
+      if (dgs != nullptr) {
+        s[0] += q[0];
+        s[1] += q[c];
+      }
+      if (dgate != nullptr) s[2] += q[2 * c];
+    }
+    float v;
+    if (dgs != nullptr) {
+      TC* d = dgs + static_cast<long long>(row) * 2 * c + ch;
+      v = s[0] * gate_at(static_cast<float>(gs[row * gs_ld + ch])).slope;
+      store_vec<1>(d, &v);
+      store_vec<1>(d + c, &s[1]);
+    }
+    if (dgate != nullptr) {
+      v = s[2] * gate_at(static_cast<float>(gate[row * gate_ld + ch])).slope;
+      store_vec<1>(dgate + static_cast<long long>(row) * c + ch, &v);
+    }
+  }
+}
+
 constexpr int kBlocksPerSm = 4;      // at most: the workspace's partial sums are sized by it
 constexpr int kMostSms = 160;
+constexpr int kMostRing = 216 * 1024;
+// Pieces of gate rows' samples, at most: two for each team that is at work (row_plan), of which a block has so many.
+constexpr long long most_units(int c) { return 2ll * kMostSms * kBlocksPerSm * (c <= 64 ? 32 : c <= 128 ? 16 : c <= 256 ? 8 : c <= 512 ? 4 : c <= 768 ? 3 : 2); }
 
 struct Sums {
   float *dweight, *dbias, *dscale;
 };
 
 template <typename TS, typename TC, int LANES, bool VEC, bool OWN>
-int launch(cudaStream_t stream, GradParams p, const Sums& sums) {
+int launch(cudaStream_t stream, GradParams p, const Sums& sums, long long rows, int samples, int l) {
   using T = Teams<LANES>;
-  auto kernel = residual_norm_grad_kernel<TS, TC, LANES, VEC, OWN>;
+  constexpr auto kernel = residual_norm_grad_kernel<TS, TC, LANES, VEC, OWN>;
+  constexpr int kS = sizeof(TS) / 2, kC = sizeof(TC) / 2, kDepth = OWN ? 3 : 4, kFlat = T::kThreads * kPiece * 4;
   static std::once_flag once;
   static int held = 1;
   std::call_once(once, [&] {
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, T::kThreads, 0) != cudaSuccess) cudaGetLastError();
     held = held < 1 ? 1 : held > kBlocksPerSm ? kBlocksPerSm : held;
   });
-  const unsigned most = static_cast<unsigned>(sm_count() < kMostSms ? sm_count() : kMostSms) * held;
-  const unsigned rows = p.share.cond_rows, teams = T::kGroups * T::kTeams;
-  p.split = p.share.samples > 1 && rows < most * teams;
-  p.chunk = p.split ? cdiv(p.share.samples, T::kGroups) : p.share.samples;
-  p.sets = (rows + T::kTeams - 1) / T::kTeams;
-  const unsigned want = p.split ? p.sets : (p.sets + T::kGroups - 1) / T::kGroups, blocks = want < most ? want : most;
+  // (a row in 8 bits takes one slot)
+  int slots = p.dr != nullptr ? kS : 0;
+  auto place = [&](bool there, bool small, int size) {
+    const int at = slots;
+    slots += !there ? 0 : small ? 1 : size;
+    return at;
+  };
+  p.s_dy = place(p.norm != kNoNorm, false, kC);
+  p.s_r = place(p.norm != kNoNorm, p.r_e != nullptr, kS);
+  p.s_u = place(p.dgate != nullptr, p.u_e != nullptr, kC);
+  p.s_x = place(p.x != nullptr, p.x_e != nullptr, kS);
+  p.s_gate = place(OWN && p.gate != nullptr, false, kC);
+  p.s_g = place(OWN && p.gate_shift != nullptr, false, kC);
+  p.slots = slots;
+  int smem = VEC ? kDepth * slots * T::kThreads * 16 : 0;
+  if (p.partial != nullptr && smem < kFlat) smem = kFlat;
+  KFB_TRY(allow_smem<kernel>(kMostRing));
+  const int fit = smem > 0 ? kMostRing / smem : held, blocks_per_sm = held < fit ? held : fit < 1 ? 1 : fit;
+  const long long most = static_cast<long long>(sm_count() < kMostSms ? sm_count() : kMostSms) * blocks_per_sm, teams = T::kGroups * T::kTeams;
+  p.plan = row_plan(rows, samples, l, most * teams, T::kTeams);
+  const bool gates = p.dgate != nullptr || p.dgate_shift != nullptr;
+  if (p.plan.chunks == 1 || !gates) p.pieces = nullptr;
+  else KFB_CHECK_ARG(p.plan.units <= most_units(p.c), "residual_norm_bwd: %u pieces", p.plan.units);
+  const long long want = (p.plan.sets + T::kGroups - 1) / T::kGroups;
+  const unsigned blocks = static_cast<unsigned>(want < most ? want : most);
   {
     LaunchScope scope(stream, "residual_norm_grad");
-    KFB_TRY(launch_kernel(stream, kernel, blocks, T::kThreads, 0, p));
+    KFB_TRY(launch_kernel(stream, kernel, blocks, T::kThreads, smem, p));
+  }
+  if (p.pieces != nullptr) {
+    const long long n = (static_cast<long long>(p.plan.gate_rows) * p.c + 255) / 256, grid = 4ll * sm_count();
+    LaunchScope scope(stream, "residual_norm_gates");
+    KFB_TRY(launch_kernel(stream, residual_norm_gates_kernel<TC>, static_cast<unsigned>(n < grid ? n : grid), 256, 0, const_cast<const float*>(p.pieces),
+                          static_cast<const TC*>(p.gate), p.gate_ld, static_cast<const TC*>(p.gate_shift), p.gate_shift_ld, static_cast<TC*>(p.dgate),
+                          static_cast<TC*>(p.dgate_shift), p.plan.gate_rows, p.plan.chunks, p.c));
   }
   if (p.partial != nullptr) {
     LaunchScope scope(stream, "residual_norm_sum");
@@ -361,27 +419,30 @@ int launch(cudaStream_t stream, GradParams p, const Sums& sums) {
 }
 
 template <typename TS, typename TC, int LANES, bool VEC>
-int launch_own(cudaStream_t stream, const GradParams& p, const Sums& sums) {
-  return p.share.samples == 1 ? launch<TS, TC, LANES, VEC, true>(stream, p, sums) : launch<TS, TC, LANES, VEC, false>(stream, p, sums);
+int launch_own(cudaStream_t stream, const GradParams& p, const Sums& sums, long long rows, int samples, int l) {
+  return samples == 1 ? launch<TS, TC, LANES, VEC, true>(stream, p, sums, rows, samples, l) : launch<TS, TC, LANES, VEC, false>(stream, p, sums, rows, samples, l);
 }
 
 template <typename TS, typename TC>
-int dispatch(cudaStream_t stream, const GradParams& p, const Sums& sums) {
+int dispatch(cudaStream_t stream, GradParams p, const Sums& sums, long long rows, int samples, int l) {
   auto of = [](const void* q, const uint8_t* e) { return reinterpret_cast<uintptr_t>(q) << (e != nullptr ? 1 : 0); };   // bytes: 8-byte boundaries do
   const uintptr_t at = reinterpret_cast<uintptr_t>(p.dr) | reinterpret_cast<uintptr_t>(p.dy) | of(p.r, p.r_e) | of(p.u, p.u_e) | of(p.x, p.x_e) |
                        reinterpret_cast<uintptr_t>(p.gate) | reinterpret_cast<uintptr_t>(p.gate_shift) | reinterpret_cast<uintptr_t>(p.dx) |
                        reinterpret_cast<uintptr_t>(p.du) | reinterpret_cast<uintptr_t>(p.dgate) | reinterpret_cast<uintptr_t>(p.dgate_shift) |
                        static_cast<uintptr_t>((p.gate_ld | p.gate_shift_ld) * sizeof(TC));
+  p.words = groups8(p.c) % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.r_e) | reinterpret_cast<uintptr_t>(p.u_e) | reinterpret_cast<uintptr_t>(p.x_e)) & 3) == 0;
   if (p.c % 8 == 0 && (at & 15) == 0) {
-    if (p.c <= 64) return launch_own<TS, TC, 8, true>(stream, p, sums);
-    if (p.c <= 128) return launch_own<TS, TC, 16, true>(stream, p, sums);
-    if (p.c <= 256) return launch_own<TS, TC, 32, true>(stream, p, sums);
-    if (p.c <= 512) return launch_own<TS, TC, 64, true>(stream, p, sums);
-    if (p.c <= 768) return launch_own<TS, TC, 96, true>(stream, p, sums);
-    return launch_own<TS, TC, 128, true>(stream, p, sums);
+    if (p.c <= 64) return launch_own<TS, TC, 8, true>(stream, p, sums, rows, samples, l);
+    if (p.c <= 128) return launch_own<TS, TC, 16, true>(stream, p, sums, rows, samples, l);
+    if (p.c <= 256) return launch_own<TS, TC, 32, true>(stream, p, sums, rows, samples, l);
+    if (p.c <= 512) return launch_own<TS, TC, 64, true>(stream, p, sums, rows, samples, l);
+    if (p.c <= 768) return launch_own<TS, TC, 96, true>(stream, p, sums, rows, samples, l);
+    return launch_own<TS, TC, 128, true>(stream, p, sums, rows, samples, l);
   }
-  return p.c <= 256 ? launch_own<TS, TC, 32, false>(stream, p, sums) : launch_own<TS, TC, 128, false>(stream, p, sums);
+  return p.c <= 256 ? launch_own<TS, TC, 32, false>(stream, p, sums, rows, samples, l) : launch_own<TS, TC, 128, false>(stream, p, sums, rows, samples, l);
 }
+
+size_t partial_bytes(int c) { return align_up(static_cast<size_t>(kMostSms) * kBlocksPerSm * 3 * c * sizeof(float), 256); }
 
 }  // namespace
 }  // namespace kfb
@@ -390,8 +451,10 @@ using namespace kfb;
 
 extern "C" {
 
-KFB_API size_t kfb_residual_norm_bwd_workspace_bytes(int c) {
-  return align_up(static_cast<size_t>(kMostSms) * kBlocksPerSm * 3 * (c > 0 ? c : 0) * sizeof(float), 256);
+KFB_API size_t kfb_residual_norm_bwd_workspace_bytes(long long rows, int c, int samples, int sums, int gates) {
+  if (rows <= 0 || c <= 0 || c > 1024 || samples <= 0) return 0;
+  const long long units = rows < most_units(c) ? rows : most_units(c);
+  return (sums ? partial_bytes(c) : 0) + (gates && samples > 1 ? align_up(static_cast<size_t>(units) * 3 * c * sizeof(float), 256) : 0);
 }
 
 KFB_API int kfb_residual_norm_bwd(const void* dr, const void* dy, const void* r, const void* r_exponents, const void* u, const void* u_exponents,
@@ -423,8 +486,9 @@ KFB_API int kfb_residual_norm_bwd(const void* dr, const void* dy, const void* r,
   KFB_CHECK_ARG((norm == kNoNorm || (dy != nullptr && r != nullptr)) && (norm != kNoNorm || dr != nullptr), "residual_norm_bwd: null tensor");
   KFB_CHECK_ARG(dgate == nullptr || (gate != nullptr && u != nullptr), "residual_norm_bwd: a gate's gradient needs the gate and what it multiplies");
   KFB_CHECK_ARG(dscale == nullptr || x != nullptr, "residual_norm_bwd: the scale's gradient needs x");
-  KFB_CHECK_ARG(!sums || (workspace != nullptr && workspace_bytes >= kfb_residual_norm_bwd_workspace_bytes(c)), "residual_norm_bwd: workspace %zu < %zu bytes",
-                workspace_bytes, kfb_residual_norm_bwd_workspace_bytes(c));
+  const bool gates = shared && (dgate != nullptr || dgate_shift != nullptr);
+  const size_t need = kfb_residual_norm_bwd_workspace_bytes(rows, c, samples, sums, gates);
+  KFB_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need), "residual_norm_bwd: workspace %zu < %zu bytes", workspace_bytes, need);
   KFB_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "residual_norm_bwd: workspace must be 256-byte aligned");
   GradParams p = {};
   p.dr = dr;
@@ -446,13 +510,14 @@ KFB_API int kfb_residual_norm_bwd(const void* dr, const void* dy, const void* r,
   p.dgate = dgate;
   p.dgate_shift = dgate_shift;
   p.partial = sums ? static_cast<float*>(workspace) : nullptr;
-  p.share = {static_cast<unsigned>(shared ? rows / samples : rows), static_cast<unsigned>(l), shared ? samples : 1};
+  p.pieces = gates ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (sums ? partial_bytes(c) : 0)) : nullptr;
+  const int each = shared ? samples : 1;
   p.c = c;
   p.norm = norm;
   p.eps = eps;
   const Sums to = {dweight, dbias, dscale};
-  if (stream_dtype == KFB_BF16) return dispatch<__nv_bfloat16, __nv_bfloat16>(s, p, to);
-  return compute_dtype == KFB_BF16 ? dispatch<float, __nv_bfloat16>(s, p, to) : dispatch<float, float>(s, p, to);
+  if (stream_dtype == KFB_BF16) return dispatch<__nv_bfloat16, __nv_bfloat16>(s, p, to, rows, each, l);
+  return compute_dtype == KFB_BF16 ? dispatch<float, __nv_bfloat16>(s, p, to, rows, each, l) : dispatch<float, float>(s, p, to, rows, each, l);
 }
 
 }  // extern "C"

@@ -81,6 +81,23 @@ struct Piece {
       else v[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     }
   }
+  // A piece on its way through shared memory (see Ring), and bytes with the word of exponents that theirs lies in.
+  __device__ __forceinline__ void take(const uint4* slot, int stride) {
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4) {
+      const uint4 t = slot[i / 4 * stride];
+      w[i] = t.x;
+      w[i + 1] = t.y;
+      w[i + 2] = t.z;
+      w[i + 3] = t.w;
+    }
+  }
+  __device__ __forceinline__ void take8(const uint4* slot, int shift) {
+    const uint4 t = *slot;
+    w[0] = t.x;
+    w[1] = t.y;
+    w[2] = t.z >> shift & 255u;
+  }
   // Bytes and their exponent in the same registers.
   __device__ __forceinline__ void load8(const uint8_t* p, const uint8_t* e, int n) {
     if constexpr (VEC) {
@@ -136,11 +153,25 @@ __device__ __forceinline__ void store_piece8(uint8_t* p, uint8_t* e, const float
   if (first && n > 0) *e = static_cast<uint8_t>(ex);
 }
 
+// Copies of 16, 8 or 4 bytes into shared memory that arrive while the thread goes on; zeros where `there` is false.
+__device__ __forceinline__ void copy_async16(void* to, const void* from, bool there) {
+  const int n = there ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from), "r"(n) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from, bool there) {
+  const int n = there ? BYTES : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_async_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LATER>
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory"); }
+
 // Threads of a block and teams in it.
 template <int LANES>
 struct Teams {
   static constexpr int kGroupLanes = LANES < 32 ? 32 : LANES;        // a warp of small teams, or a large team: what moves from row to row together
-  static constexpr int kThreads = 256 / kGroupLanes * kGroupLanes + (LANES == 96 ? 96 : 0);
+  static constexpr int kThreads = LANES == 96 ? 288 : 256;
   static constexpr int kGroups = kThreads / kGroupLanes, kTeams = kGroupLanes / LANES;
   static constexpr int kWarps = LANES < 32 ? 1 : LANES / 32;
 };

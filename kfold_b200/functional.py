@@ -566,9 +566,10 @@ def residual_norm_backward(dr: torch.Tensor | None, dy: torch.Tensor | None, r, 
     dw, db, dscale = vector(need_weight, weight), vector(need_bias, weight), vector(need_scale, scale)
     lib = L.lib()
     ws, size = None, 0
-    if need_weight or need_bias or need_scale:
-        ws = _call_workspace(first.device, lib.kfb_residual_norm_bwd_workspace_bytes(c))
-        size = ws.numel()
+    sums, gates = need_weight or need_bias or need_scale, samples > 1 and (need_gate or need_gate_shift)
+    if sums or gates:
+        size = lib.kfb_residual_norm_bwd_workspace_bytes(rows, c, samples, sums, gates)
+        ws = _call_workspace(first.device, size) if size else None
     drc, dyc = None if dr is None else _dense(dr), None if dy is None else _dense(dy)
     (rp, re, rk), (up, ue, uk), (xp, xe, xk) = _kept_or_dense(r), _kept_or_dense(u if need_gate else None), _kept_or_dense(x if need_scale else None)
     sc, w = _affine(scale), _affine(weight)

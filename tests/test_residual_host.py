@@ -31,7 +31,7 @@ def test_residual_norm_refuses(library):
 
 
 def test_residual_norm_gradient_refuses(library):
-    need = library.kfb_residual_norm_bwd_workspace_bytes(64)
+    need = library.kfb_residual_norm_bwd_workspace_bytes(12, 64, 2, 1, 1)
 
     def call(dr=SOME, dy=SOME, r=SOME, u=SOME, x=None, gate=SOME, gate_ld=64, w=None, gs=None, gs_ld=0, dx=SOME, du=SOME, dgate=SOME, dgs=None, dw=None, db=SOME, ds=None, ws=SOME,
              size=need, rows=12, c=64, samples=2, l=3, norm=1, st=0, ct=0):
@@ -44,7 +44,11 @@ def test_residual_norm_gradient_refuses(library):
         assert b"residual_norm_bwd" in library.kfb_last_error()
     assert call(c=1025, gate_ld=2000, size=BIG) == 2
     assert call(rows=0, db=None) == 0
-    assert library.kfb_residual_norm_bwd_workspace_bytes(0) == 0 == library.kfb_residual_norm_bwd_workspace_bytes(-3)
+    room = library.kfb_residual_norm_bwd_workspace_bytes
+    assert room(12, 0, 2, 1, 1) == room(12, -3, 2, 1, 1) == room(0, 64, 2, 1, 1) == room(12, 64, 0, 1, 1) == room(12, 64, 2, 0, 0) == room(12, 64, 1, 0, 1) == 0
+    for c in (1, 64, 128, 768, 1024):
+        sizes = [room(n, c, 4, 1, 1) for n in (4, 400, 1 << 20, (1 << 31) - 4)]
+        assert sizes == sorted(sizes) and sizes[-1] == sizes[-2] < 64 << 20
 
 
 def test_rows_in_8_bits_refuse(library):

@@ -17,11 +17,9 @@ __global__ void __launch_bounds__(256) compress_kernel(const T* x, uint8_t* q, u
   for (long long first = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x / 32 * 32; first < pieces; first += gridDim.x * 256ll) {
     const long long i = first + threadIdx.x % 32, row = i / per_row;
     const int ch = static_cast<int>(i - row * per_row) * kPiece, n = i < pieces ? min(max(c - ch, 0), kPiece) : 0;
-    Piece<T, VEC> raw;
-    float v[kPiece];
-    raw.load(x + row * c + ch, n);
-    raw.values(v);
-    store_piece8<VEC>(q + row * c + ch, e + row * groups + ch / kGroup8, v, n, threadIdx.x % 4 == 0);
+    const Pairs v = load_piece<T, VEC>(x + row * c + ch, n);
+    const uint32_t e_here = exponent8(group_top(top_of(v)));
+    store_piece8<VEC>(q + row * c + ch, e + row * groups + ch / kGroup8, v, e_here, n, threadIdx.x % 4 == 0);
   }
 }
 
@@ -32,11 +30,7 @@ __global__ void __launch_bounds__(256) expand_kernel(const uint8_t* q, const uin
   for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < pieces; i += gridDim.x * 256ll) {
     const long long row = i / per_row;
     const int ch = static_cast<int>(i - row * per_row) * kPiece, n = min(max(c - ch, 0), kPiece);
-    Piece<float, VEC> raw;
-    float v[kPiece];
-    raw.load8(q + row * c + ch, e + row * groups + ch / kGroup8, n);
-    raw.values_of_8(v);
-    store_piece<VEC>(x + row * c + ch, v, n);
+    store_piece<VEC>(x + row * c + ch, load_piece8<VEC>(q + row * c + ch, e + row * groups + ch / kGroup8, n), n);
   }
 }
 

@@ -4,15 +4,12 @@
 // What bounds it: x and u in, r and y out, HBM.  One pass: a team of lanes holds a row in registers, adds, rounds to the stream's type, and takes mean
 // and variance of what it stored (residual_norm.cuh: how rows are walked and come in).
 #include <mutex>
-#include <type_traits>
 
 #include "ops_common.cuh"
 #include "residual_norm.cuh"
 
 namespace kfb {
 namespace {
-
-constexpr int kDepth = 4;              // rows on their way for a team, the one in work among them
 
 struct Params {
   const void *x, *u, *gate, *gate_shift;
@@ -26,51 +23,55 @@ struct Params {
   int slots, s_u, s_gate, s_g;         // slots of a stage, and the first of each tensor (x: 0)
 };
 
-template <typename T>
-__device__ __forceinline__ float as_stored(float v) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) return __bfloat162float(__float2bfloat16_rn(v));
-  else return v;
-}
+template <typename TS, typename TC, int P, bool OWN>
+constexpr int depth() { return ring_depth(P * 8 * (sizeof(TS) + (OWN ? 4 : 1) * sizeof(TC))); }
 
-template <typename TS, typename TC, int LANES, bool VEC, bool OWN>
-__global__ void __launch_bounds__(Teams<LANES>::kThreads) residual_norm_kernel(const Params p) {
-  using T = Teams<LANES>;
-  constexpr int N = kPiece;
-  __shared__ float room[2][T::kGroups][T::kWarps][1];
+template <typename TS, typename TC, int LANES, int P, bool VEC, bool OWN>
+__global__ void __launch_bounds__(kRowThreads) residual_norm_kernel(const Params p) {
+  constexpr int kDepth = depth<TS, TC, P, OWN>(), kS = sizeof(TS) / 2, kC = sizeof(TC) / 2;
   extern __shared__ uint4 ring_memory[];
   grid_dependency_enter();
-  const int group = threadIdx.x / T::kGroupLanes, sub = threadIdx.x % LANES, team = threadIdx.x % T::kGroupLanes / LANES;
-  const int ch = sub * N, n = min(max(p.c - ch, 0), N);
+  const int warp = threadIdx.x / 32, sub = threadIdx.x % LANES, team = threadIdx.x % 32 / LANES;
   const float inv_c = 1.0f / static_cast<float>(p.c);
   const TS* x = static_cast<const TS*>(p.x);
   const TC *u = static_cast<const TC*>(p.u), *gate = static_cast<const TC*>(p.gate), *gs = static_cast<const TC*>(p.gate_shift);
   uint4* ring = ring_memory + threadIdx.x;
-
-  float m[N], shift[N], open[OWN ? 1 : N];
+  auto channel = [&](int q) { return (q * LANES + sub) * kPiece; };
+  auto inside = [&](int q) { return VEC ? (channel(q) < p.c ? kPiece : 0) : min(max(p.c - channel(q), 0), kPiece); };      // channels of a piece
+  auto vector = [&](const float* v, int q, float other) {
+    float f[kPiece];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    m[i] = p.weight != nullptr && i < n ? p.weight[ch + i] : 1.f;
-    shift[i] = p.bias != nullptr && i < n ? p.bias[ch + i] : 0.f;
-    if (!OWN) open[i] = 1.f;
+    for (int i = 0; i < kPiece; ++i) f[i] = v != nullptr && i < inside(q) ? v[channel(q) + i] : other;
+    return of_floats(f);
+  };
+
+  Pairs m[P], shift[P], open[OWN ? 1 : P];
+#pragma unroll
+  for (int q = 0; q < P; ++q) {
+    m[q] = vector(p.weight, q, 1.f);
+    shift[q] = vector(p.bias, q, 0.f);
   }
 
-  const unsigned step = gridDim.x * T::kGroups;
+  const unsigned step = gridDim.x * (kRowThreads / 32);
   Walk<LANES, OWN> here, ahead;
-  here.set = blockIdx.x * T::kGroups + group;
+  here.set = blockIdx.x * (kRowThreads / 32) + warp;
   if (here.set < p.plan.sets) here.enter(p.plan, team);
   ahead = here;
   auto fetch = [&](int stage) {
     if (ahead.set < p.plan.sets) {
-      uint4* q = ring + stage * p.slots * T::kThreads;
-      const bool there = ahead.left > 0 && n > 0;
-      const long long o = static_cast<long long>(ahead.row) * p.c + ch;
-      if (x != nullptr) ring_copy<TS, VEC>(q, T::kThreads, x + o, there);
-      if (u != nullptr) ring_copy<TC, VEC>(q + p.s_u * T::kThreads, T::kThreads, u + o, there);
-      if (OWN && gate != nullptr) ring_copy<TC, VEC>(q + p.s_gate * T::kThreads, T::kThreads, gate + ahead.row * p.gate_ld + ch, there);
-      if (OWN && gs != nullptr) {
-        uint4* g = q + p.s_g * T::kThreads;
-        ring_copy<TC, VEC>(g, T::kThreads, gs + ahead.row * p.gate_shift_ld + ch, there);
-        ring_copy<TC, VEC>(g + sizeof(TC) / 2 * T::kThreads, T::kThreads, gs + ahead.row * p.gate_shift_ld + p.c + ch, there);
+      const long long o = static_cast<long long>(ahead.row) * p.c;
+      uint4* s = ring + stage * p.slots * kRowThreads;
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        const int ch = channel(q);
+        const bool there = ahead.left > 0 && ch < p.c;
+        if (x != nullptr) ring_copy(s + q * kS * kRowThreads, x + o + ch, there);
+        if (u != nullptr) ring_copy(s + (p.s_u + q * kC) * kRowThreads, u + o + ch, there);
+        if (OWN && gate != nullptr) ring_copy(s + (p.s_gate + q * kC) * kRowThreads, gate + ahead.row * p.gate_ld + ch, there);
+        if (OWN && gs != nullptr) {
+          ring_copy(s + (p.s_g + q * kC) * kRowThreads, gs + ahead.row * p.gate_shift_ld + ch, there);
+          ring_copy(s + (p.s_g + (P + q) * kC) * kRowThreads, gs + ahead.row * p.gate_shift_ld + p.c + ch, there);
+        }
       }
       ahead.next(p.plan, team, step);
     }
@@ -80,120 +81,112 @@ __global__ void __launch_bounds__(Teams<LANES>::kThreads) residual_norm_kernel(c
 #pragma unroll
     for (int i = 0; i < kDepth - 1; ++i) fetch(i);
   }
-  int turn = 0, stage = 0;
+  int stage = 0;
   while (here.set < p.plan.sets) {
     if constexpr (VEC) {
       fetch(stage == 0 ? kDepth - 1 : stage - 1);
       copy_async_wait<kDepth - 1>();
     }
-    const int k = here.left > 0 ? n : 0;
-    const uint4* q = ring + stage * p.slots * T::kThreads;
-    const long long o = static_cast<long long>(here.row) * p.c + ch;
-    float r[N], t[N];
-    Piece<TC, VEC> raw;
+    const uint4* s = ring + stage * p.slots * kRowThreads;
+    const long long o = static_cast<long long>(here.row) * p.c;
+    auto channels = [&](int q) { return here.left > 0 ? inside(q) : 0; };
+    auto take = [&](auto tag, int slot, const void* from, long long at, int q) {
+      using E = decltype(tag);
+      if constexpr (VEC) return ring_take<E>(s + (slot + q * (static_cast<int>(sizeof(E)) / 2)) * kRowThreads);
+      else return load_piece<E, VEC>(static_cast<const E*>(from) + at + channel(q), channels(q));
+    };
     if (!OWN && here.at == 0) {
       const unsigned gate_row = here.gate_row(p.plan);
-      if (gate != nullptr) {
-        raw.load(gate + gate_row * p.gate_ld + ch, k);
-        raw.values(t);
 #pragma unroll
-        for (int i = 0; i < (OWN ? 1 : N); ++i) open[i] = open_exact(t[i]);
-      }
-      if (gs != nullptr) {
-        raw.load(gs + gate_row * p.gate_shift_ld + ch, k);
-        raw.values(t);
-        raw.load(gs + gate_row * p.gate_shift_ld + p.c + ch, k);
-        raw.values(shift);
-#pragma unroll
-        for (int i = 0; i < N; ++i) m[i] = gate_at(t[i]).open;
+      for (int q = 0; q < P; ++q) {
+        const int k = channels(q);
+        if (gate != nullptr) open[OWN ? 0 : q] = each(load_piece<TC, VEC>(gate + gate_row * p.gate_ld + channel(q), k), [](float a) { return open_of(exact_gate_at(a)); });
+        if (gs != nullptr) {
+          m[q] = each(load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + channel(q), k), [](float a) { return open_of(gate_at(a)); });
+          shift[q] = load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + p.c + channel(q), k);
+        }
       }
     }
-    if (x != nullptr) {
-      Piece<TS, VEC> x_raw;
-      if constexpr (VEC) x_raw.take(q, T::kThreads);
-      else x_raw.load(x + o, k);
-      x_raw.values(r);
-      if (p.scale != nullptr) {
+    Pairs r[P];
+    uint64_t sum = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) r[i] *= i < n ? p.scale[ch + i] : 0.f;
+    for (int q = 0; q < P; ++q) {
+      const int k = channels(q), ch = channel(q);
+      r[q] = x != nullptr ? take(TS{}, 0, x, o, q) : both(0.f);
+      if (p.scale != nullptr) r[q] = mul(r[q], vector(p.scale, q, 0.f));
+      if (u != nullptr) {
+        const Pairs t = take(TC{}, p.s_u, u, o, q);
+        if (gate == nullptr) r[q] = add(r[q], t);
+        else if constexpr (OWN) r[q] = fma(each(take(TC{}, p.s_gate, gate, here.row * p.gate_ld, q), [](float a) { return open_of(exact_gate_at(a)); }), t, r[q]);
+        else r[q] = fma(open[q], t, r[q]);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) r[i] = 0.f;
-    }
-    if (u != nullptr) {
-      if constexpr (VEC) raw.take(q + p.s_u * T::kThreads, T::kThreads);
-      else raw.load(u + o, k);
-      raw.values(t);
-      if (gate == nullptr) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[i] += t[i];
-      } else if constexpr (OWN) {
-        float s[N];
-        if constexpr (VEC) raw.take(q + p.s_gate * T::kThreads, T::kThreads);
-        else raw.load(gate + here.row * p.gate_ld + ch, k);
-        raw.values(s);
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[i] = fmaf(open_exact(s[i]), t[i], r[i]);
+      uint32_t top;
+      if constexpr (std::is_same<TS, __nv_bfloat16>::value) {
+        const uint4 w = to_bf16(r[q]);
+        r[q] = of_bf16(w);                          // (as it is stored)
+        top = top_of(w);
+        if constexpr (VEC) {
+          if (p.r != nullptr && k > 0) *reinterpret_cast<uint4*>(static_cast<TS*>(p.r) + o + ch) = w;
+        }
       } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[i] = fmaf(open[i], t[i], r[i]);
+        top = p.kept != nullptr ? top_of(r[q]) : 0u;
+        if constexpr (VEC) {
+          if (p.r != nullptr) store_piece<VEC>(static_cast<TS*>(p.r) + o + ch, r[q], k);
+        }
       }
+      if constexpr (!VEC) {
+        if (p.r != nullptr) store_piece<VEC>(static_cast<TS*>(p.r) + o + ch, r[q], k);
+      }
+      if (p.kept != nullptr)
+        store_piece8<VEC>(p.kept + o + ch, p.kept_e + static_cast<long long>(here.row) * groups8(p.c) + ch / kGroup8, r[q], exponent8(group_top(top)), k,
+                          sub % (kGroup8 / kPiece) == 0);
+      sum_into(sum, r[q]);
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) r[i] = as_stored<TS>(r[i]);
-    if (p.r != nullptr) store_piece<VEC>(static_cast<TS*>(p.r) + o, r, k);
-    if (p.kept != nullptr)
-      store_piece8<VEC>(p.kept + o, p.kept_e + static_cast<long long>(here.row) * groups8(p.c) + ch / kGroup8, r, k, sub % (kGroup8 / N) == 0);
     if (p.norm != kNoNorm) {
-      float s[1] = {0.f};
+      float t[1] = {total(sum)};
+      team_sum<LANES>(t);
+      const Pairs minus_mean = both(-t[0] * inv_c);
+      sum = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) s[0] += r[i];
-      team_sum<LANES>(s, room, group, turn);
-      const float mean = s[0] * inv_c;
-      s[0] = 0.f;
+      for (int q = 0; q < P; ++q) {
+        r[q] = add(r[q], minus_mean);
+        if constexpr (!VEC) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        r[i] = (VEC ? n > 0 : i < n) ? r[i] - mean : 0.f;
-        s[0] = fmaf(r[i], r[i], s[0]);
+          for (int i = 0; i < kPiece; ++i)
+            if (i >= inside(q)) r[q].v[i / 2] = i & 1 ? ptx::pack2(r[q].get(i - 1), 0.f) : ptx::pack2(0.f, 0.f);
+        }
+        if (inside(q) > 0) dot_into(sum, r[q], r[q]);
       }
-      team_sum<LANES>(s, room, group, turn ^ 1);
-      const float rstd = rsqrtf(fmaf(s[0], inv_c, p.eps));
-      if (OWN && gs != nullptr) {
-        if constexpr (VEC) raw.take(q + p.s_g * T::kThreads, T::kThreads);
-        else raw.load(gs + here.row * p.gate_shift_ld + ch, k);
-        raw.values(t);
+      t[0] = total(sum);
+      team_sum<LANES>(t);
+      const Pairs rstd = both(rsqrtf(fmaf(t[0], inv_c, p.eps)));
 #pragma unroll
-        for (int i = 0; i < N; ++i) r[i] = r[i] * rstd * gate_at(t[i]).open;
-        if constexpr (VEC) raw.take(q + (p.s_g + static_cast<int>(sizeof(TC)) / 2) * T::kThreads, T::kThreads);
-        else raw.load(gs + here.row * p.gate_shift_ld + p.c + ch, k);
-        raw.values(t);
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[i] += t[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[i] = fmaf(r[i] * rstd, m[i], shift[i]);
+      for (int q = 0; q < P; ++q) {
+        Pairs y = mul(r[q], rstd);
+        if (OWN && gs != nullptr)
+          y = fma(y, each(take(TC{}, p.s_g, gs, here.row * p.gate_shift_ld, q), [](float a) { return open_of(gate_at(a)); }),
+                  take(TC{}, p.s_g + P * kC, gs, here.row * p.gate_shift_ld + p.c, q));
+        else
+          y = fma(y, m[q], shift[q]);
+        store_piece<VEC>(static_cast<TC*>(p.y) + o + channel(q), y, channels(q));
       }
-      store_piece<VEC>(static_cast<TC*>(p.y) + o, r, k);
     }
     here.next(p.plan, team, step);
     stage = stage + 1 == kDepth ? 0 : stage + 1;
   }
 }
 
-constexpr int kMostRing = 200 * 1024;
-
-template <typename TS, typename TC, int LANES, bool VEC, bool OWN>
+template <typename TS, typename TC, int LANES, int P, bool VEC, bool OWN>
 int launch(cudaStream_t stream, Params p, long long rows, int samples, int l) {
-  using T = Teams<LANES>;
-  constexpr auto kernel = residual_norm_kernel<TS, TC, LANES, VEC, OWN>;
+  constexpr auto kernel = residual_norm_kernel<TS, TC, LANES, P, VEC, OWN>;
+  constexpr int kWarps = kRowThreads / 32, kTeams = 32 / LANES, kMostBlocks = 8;
   static std::once_flag once;
   static int held = 1;
   std::call_once(once, [&] {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, T::kThreads, 0) != cudaSuccess) cudaGetLastError();
-    held = held < 1 ? 1 : held > 4 ? 4 : held;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, kRowThreads, 0) != cudaSuccess) cudaGetLastError();
+    held = held < 1 ? 1 : held > kMostBlocks ? kMostBlocks : held;
   });
-  constexpr int kS = sizeof(TS) / 2, kC = sizeof(TC) / 2;        // slots of a piece
+  constexpr int kS = P * sizeof(TS) / 2, kC = P * sizeof(TC) / 2;        // slots of a tensor
   p.slots = p.x != nullptr ? kS : 0;
   p.s_u = p.slots;
   p.slots += p.u != nullptr ? kC : 0;
@@ -201,19 +194,19 @@ int launch(cudaStream_t stream, Params p, long long rows, int samples, int l) {
   p.slots += OWN && p.gate != nullptr ? kC : 0;
   p.s_g = p.slots;
   p.slots += OWN && p.gate_shift != nullptr ? 2 * kC : 0;
-  const int smem = VEC ? kDepth * p.slots * T::kThreads * 16 : 0;
+  const int smem = VEC ? depth<TS, TC, P, OWN>() * p.slots * kRowThreads * 16 : 0;
   if (VEC) KFB_TRY(allow_smem<kernel>(kMostRing));
   const int room = smem > 0 ? kMostRing / smem : held, blocks_per_sm = held < room ? held : room < 1 ? 1 : room;
-  const long long most = static_cast<long long>(sm_count()) * blocks_per_sm, teams = T::kGroups * T::kTeams;
-  p.plan = row_plan(rows, samples, l, most * teams, T::kTeams);
-  const long long want = (p.plan.sets + T::kGroups - 1) / T::kGroups;
+  const long long most = static_cast<long long>(sm_count()) * blocks_per_sm;
+  p.plan = row_plan(rows, samples, l, most * kWarps * kTeams, kTeams);
+  const long long want = (p.plan.sets + kWarps - 1) / kWarps;
   LaunchScope scope(stream, "residual_norm");
-  return launch_kernel(stream, kernel, static_cast<unsigned>(want < most ? want : most), T::kThreads, smem, p);
+  return launch_kernel(stream, kernel, static_cast<unsigned>(want < most ? want : most), kRowThreads, smem, p);
 }
 
-template <typename TS, typename TC, int LANES, bool VEC>
+template <typename TS, typename TC, int LANES, int P, bool VEC>
 int launch_own(cudaStream_t stream, const Params& p, long long rows, int samples, int l) {
-  return samples == 1 ? launch<TS, TC, LANES, VEC, true>(stream, p, rows, samples, l) : launch<TS, TC, LANES, VEC, false>(stream, p, rows, samples, l);
+  return samples == 1 ? launch<TS, TC, LANES, P, VEC, true>(stream, p, rows, samples, l) : launch<TS, TC, LANES, P, VEC, false>(stream, p, rows, samples, l);
 }
 
 template <typename TS, typename TC>
@@ -221,15 +214,9 @@ int dispatch(cudaStream_t stream, const Params& p, long long rows, int samples, 
   const uintptr_t at = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.u) | reinterpret_cast<uintptr_t>(p.gate) |
                        reinterpret_cast<uintptr_t>(p.gate_shift) | reinterpret_cast<uintptr_t>(p.r) | reinterpret_cast<uintptr_t>(p.y) |
                        static_cast<uintptr_t>((p.gate_ld | p.gate_shift_ld) * sizeof(TC)) | (reinterpret_cast<uintptr_t>(p.kept) & 7);
-  if (p.c % 8 == 0 && (at & 15) == 0) {
-    if (p.c <= 64) return launch_own<TS, TC, 8, true>(stream, p, rows, samples, l);
-    if (p.c <= 128) return launch_own<TS, TC, 16, true>(stream, p, rows, samples, l);
-    if (p.c <= 256) return launch_own<TS, TC, 32, true>(stream, p, rows, samples, l);
-    if (p.c <= 512) return launch_own<TS, TC, 64, true>(stream, p, rows, samples, l);
-    if (p.c <= 768) return launch_own<TS, TC, 96, true>(stream, p, rows, samples, l);
-    return launch_own<TS, TC, 128, true>(stream, p, rows, samples, l);
-  }
-  return p.c <= 256 ? launch_own<TS, TC, 32, false>(stream, p, rows, samples, l) : launch_own<TS, TC, 128, false>(stream, p, rows, samples, l);
+#define KFB_CALL(LANES, P, VEC) launch_own<TS, TC, LANES, P, VEC>(stream, p, rows, samples, l)
+  KFB_ROW_SHAPES(p.c, p.c % 8 == 0 && (at & 15) == 0, KFB_CALL);
+#undef KFB_CALL
 }
 
 }  // namespace

@@ -2,7 +2,7 @@
 //
 // Row (group, sample, token) of the stream has the gates of row (group, token).  A team takes the samples that share a gate row one after the other, so that
 // gates are read and their exponentials computed once for all of them; where gate rows are few, their samples are cut into pieces.
-// Rows come through a ring in shared memory, a slot of 16 bytes a thread and tensor: a thread copies the pieces that it will work on itself, several rows
+// Rows come through a ring in shared memory, slots of 16 bytes a thread: a thread copies the pieces that it will work on itself, several rows
 // ahead, and needs neither registers nor barriers for them.  (The same loads into registers one row ahead, at the one block of 256 threads an SM that 200
 // registers allow, moved 2.3 TB/s.)
 #pragma once
@@ -12,20 +12,22 @@ namespace kfb {
 
 enum RowNorm : int { kNoNorm = 0, kAffineNorm = 1, kAdaptiveNorm = 2 };
 
+constexpr int kRowThreads = 128;
+
 struct RowPlan {
   unsigned gate_rows, l;     // l tokens a group
   int samples;
   int chunks, chunk;         // pieces of a gate row's samples, and how many samples a piece has (the last may have fewer)
-  unsigned units, sets;      // pieces; and as groups of lanes take them
+  unsigned units, sets;      // pieces; and as warps take them
 };
 
-// OWN: every row has gates of its own.
+// The rows of one team of a warp.  OWN: every row has gates of its own.
 template <int LANES, bool OWN>
 struct Walk {
   unsigned set, row = 0, unit = 0;
-  int at = 0, left = 0;      // samples that the group has taken of this piece; that are left to this team
+  int at = 0, left = 0;      // samples that the warp has taken of this piece; that are left to this team
   __device__ __forceinline__ void enter(const RowPlan& p, int team) {
-    unit = set * Teams<LANES>::kTeams + team;
+    unit = set * (32 / LANES) + team;
     const bool there = unit < p.units;
     if (OWN) {
       row = there ? unit : 0;
@@ -49,9 +51,9 @@ struct Walk {
   __device__ __forceinline__ unsigned gate_row(const RowPlan& p) const { return OWN ? row : unit < p.units ? unit / p.chunks : 0; }
 };
 
-// A plan for `teams` teams at work at once, kTeams of them in a group of lanes: pieces that the teams finish together.  The cost of a round is its
-// samples and, for the gates and the sums, about two more.  Never more than two pieces a team.
-inline RowPlan row_plan(long long rows, int samples, int l, long long teams, int teams_in_group) {
+// A plan for `teams` teams at work at once, `in_warp` of them in a warp: pieces that the teams finish together.  The cost of a round is its samples and, for the
+// gates and the sums, about two more.  Never more than two pieces a team.
+inline RowPlan row_plan(long long rows, int samples, int l, long long teams, int in_warp) {
   RowPlan p = {};
   p.gate_rows = static_cast<unsigned>(rows / samples);
   p.l = static_cast<unsigned>(l);
@@ -69,19 +71,53 @@ inline RowPlan row_plan(long long rows, int samples, int l, long long teams, int
   p.chunk = (samples + p.chunks - 1) / p.chunks;
   p.chunks = (samples + p.chunk - 1) / p.chunk;
   p.units = p.gate_rows * p.chunks;
-  p.sets = (p.units + teams_in_group - 1) / teams_in_group;
+  p.sets = (p.units + in_warp - 1) / in_warp;
   return p;
 }
 
-// The ring: slot `s` of stage `q` of this thread at ring[(q * slots + s) * threads], a piece of float32 in two neighbouring slots.
-template <typename T, bool VEC>
-__device__ __forceinline__ void ring_copy(uint4* slot, int stride, const T* from, bool there) {
+// Sums of K values over a team's lanes, the same in all of them.
+template <int LANES, int K>
+__device__ __forceinline__ void team_sum(float (&v)[K]) {
 #pragma unroll
-  for (int i = 0; i < kPiece * static_cast<int>(sizeof(T)) / 16; ++i) copy_async16(slot + i * stride, reinterpret_cast<const uint4*>(from) + i, there);
+  for (int m = LANES / 2; m > 0; m >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], m);
 }
-__device__ __forceinline__ void ring_copy8(uint4* slot, const uint8_t* values, const uint8_t* words, bool there) {
-  copy_async<8>(slot, values, there);
-  copy_async<4>(reinterpret_cast<uint32_t*>(slot) + 2, words, there);
+
+// The ring.  Bytes that an SM's blocks have for it, and rows on their way for a team, the one in work among them: 2 to 4, as many as leave two blocks
+// of 128 threads an SM their place.
+constexpr int kMostRing = 216 * 1024;
+constexpr int ring_depth(int row_bytes) {      // of a thread and row
+  const int d = kMostRing / 2 / kRowThreads / row_bytes;
+  return d < 2 ? 2 : d > 4 ? 4 : d;
 }
+// Slot `s` of stage `q` of this thread: ring[(q * slots + s) * kRowThreads]; piece p of a tensor p * (16-byte words of a piece) slots on.
+template <typename T>
+__device__ __forceinline__ void ring_copy(uint4* slot, const T* from, bool there) {
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) copy_async16(slot + i * kRowThreads, reinterpret_cast<const uint4*>(from) + i, there);
+}
+template <typename T>
+__device__ __forceinline__ Pairs ring_take(const uint4* slot) {
+  if constexpr (sizeof(T) == 2) return of_bf16(slot[0]);
+  else return of_f32(slot[0], slot[kRowThreads]);
+}
+
+// The kernels' shapes: lanes of a team and pieces of a lane.  CALL(LANES, P, VEC) for c channels.
+#define KFB_ROW_SHAPES(c, vec, CALL)                  \
+  do {                                                \
+    if (vec) {                                        \
+      if ((c) <= 64) return CALL(8, 1, true);         \
+      if ((c) <= 128) return CALL(16, 1, true);       \
+      if ((c) <= 256) return CALL(32, 1, true);       \
+      if ((c) <= 384) return CALL(16, 3, true);       \
+      if ((c) <= 512) return CALL(32, 2, true);       \
+      if ((c) <= 768) return CALL(32, 3, true);       \
+      return CALL(32, 4, true);                       \
+    }                                                 \
+    if ((c) <= 256) return CALL(32, 1, false);        \
+    if ((c) <= 512) return CALL(32, 2, false);        \
+    return CALL(32, 4, false);                        \
+  } while (0)
 
 }  // namespace kfb

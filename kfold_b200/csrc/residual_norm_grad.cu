@@ -28,99 +28,86 @@ struct GradParams {
   int c, norm;
   float eps;
   int slots, s_dy, s_r, s_u, s_x, s_gate, s_g;    // slots of a stage, and the first of each tensor (dr: 0)
+  int s_scale;                         // behind the ring: this thread's sums of t x
   int words;                           // exponents come in words of four (a row's are whole words, and start on one)
 };
 
+template <typename TS, typename TC, int P, bool OWN>
+constexpr int depth() { return ring_depth(P * 8 * (2 * sizeof(TS) + (OWN ? 4 : 2) * sizeof(TC))); }
+
 // OWN: a row has gates of its own.
-template <typename TS, typename TC, int LANES, bool VEC, bool OWN>
-__global__ void __launch_bounds__(Teams<LANES>::kThreads, 2) residual_norm_grad_kernel(const GradParams p) {
-  using T = Teams<LANES>;
-  constexpr int N = kPiece, kThreads = T::kThreads, kDepth = OWN ? 3 : 4;      // rows on their way for a team, the one in work among them
-  __shared__ float room[2][T::kGroups][T::kWarps][2];
+template <typename TS, typename TC, int LANES, int P, bool VEC, bool OWN>
+__global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : 2) residual_norm_grad_kernel(const GradParams p) {
+  constexpr int kDepth = depth<TS, TC, P, OWN>(), kC = sizeof(TC) / 2;
   extern __shared__ uint4 ring_memory[];
   grid_dependency_enter();
-  const int group = threadIdx.x / T::kGroupLanes, sub = threadIdx.x % LANES, team = threadIdx.x % T::kGroupLanes / LANES;
-  const int ch = sub * N, n = min(max(p.c - ch, 0), N), groups = groups8(p.c), e_shift = ch / kGroup8 % 4 * 8;
+  const int warp = threadIdx.x / 32, sub = threadIdx.x % LANES, team = threadIdx.x % 32 / LANES, groups = groups8(p.c);
   const float inv_c = 1.0f / static_cast<float>(p.c);
-  const TS* dr = static_cast<const TS*>(p.dr);
-  const TC *dy = static_cast<const TC*>(p.dy), *gate = static_cast<const TC*>(p.gate), *gs = static_cast<const TC*>(p.gate_shift);
+  const TC *gate = static_cast<const TC*>(p.gate), *gs = static_cast<const TC*>(p.gate_shift);
   const bool adaptive = p.norm == kAdaptiveNorm;
   uint4* ring = ring_memory + threadIdx.x;
-
-  float m[N], open[OWN ? 1 : N], a0[N], a1[N], a2[OWN ? 1 : N], a3[N];
+  float* scale_sums = reinterpret_cast<float*>(ring_memory + p.s_scale * kRowThreads) + threadIdx.x;      // [P * 8][thread]
+  auto channel = [&](int q) { return (q * LANES + sub) * kPiece; };
+  auto inside = [&](int q) { return VEC ? (channel(q) < p.c ? kPiece : 0) : min(max(p.c - channel(q), 0), kPiece); };      // channels of a piece
+  auto vector = [&](const float* v, int q, float other) {
+    float f[kPiece];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    m[i] = p.weight != nullptr && i < n ? p.weight[ch + i] : 1.f;
-    a0[i] = a1[i] = a3[i] = 0.f;
-  }
+    for (int i = 0; i < kPiece; ++i) f[i] = v != nullptr && i < inside(q) ? v[channel(q) + i] : other;
+    return of_floats(f);
+  };
+
+  // m: what dy is multiplied by, weights or open gates; open: the output gates
+  Pairs m[P], open[OWN ? 1 : P], a0[P], a1[P], a2[OWN ? 1 : P];
 #pragma unroll
-  for (int i = 0; i < (OWN ? 1 : N); ++i) {
-    open[i] = 1.f;
-    a2[i] = 0.f;
+  for (int q = 0; q < P; ++q) {
+    m[q] = vector(p.weight, q, 1.f);
+    a0[q] = a1[q] = both(0.f);
+    if (!OWN) open[OWN ? 0 : q] = both(1.f), a2[OWN ? 0 : q] = both(0.f);
+    if (p.x != nullptr) {
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) scale_sums[(q * kPiece + i) * kRowThreads] = 0.f;
+    }
   }
 
-  const unsigned step = gridDim.x * T::kGroups;
+  const unsigned step = gridDim.x * (kRowThreads / 32);
   Walk<LANES, OWN> here, ahead;
-  here.set = blockIdx.x * T::kGroups + group;
+  here.set = blockIdx.x * (kRowThreads / 32) + warp;
   if (here.set < p.plan.sets) here.enter(p.plan, team);
   ahead = here;
-  // a tensor of the stream's or the blocks' type, or its rows in 8 bits, into its slots and out of them
-  auto copy = [&](auto tag, int slot, int stage, const void* q, const uint8_t* e, unsigned row, bool there) {
-    using E = decltype(tag);
-    uint4* to = ring + (stage * p.slots + slot) * kThreads;
-    const long long o = static_cast<long long>(row) * p.c + ch;
-    if (e == nullptr) {
-      ring_copy<E, VEC>(to, kThreads, static_cast<const E*>(q) + o, there);
-    } else {
-      copy_async<8>(to, static_cast<const uint8_t*>(q) + o, there);
-      if (p.words) copy_async<4>(reinterpret_cast<uint32_t*>(to) + 2, e + static_cast<long long>(row) * groups + (ch / kGroup8 & ~3), there);
-    }
-  };
-  auto take = [&](auto tag, int slot, int stage, const void* q, const uint8_t* e, float* v) {
-    using E = decltype(tag);
-    Piece<E, VEC> raw;
-    const int k = here.left > 0 ? n : 0;
-    [[maybe_unused]] const uint4* from = ring + (stage * p.slots + slot) * kThreads;
-    [[maybe_unused]] const long long o = static_cast<long long>(here.row) * p.c + ch;
-    const uint8_t* ep = e == nullptr ? nullptr : e + static_cast<long long>(here.row) * groups + ch / kGroup8;
-    if (e == nullptr) {
-      if constexpr (VEC) raw.take(from, kThreads);
-      else raw.load(static_cast<const E*>(q) + o, k);
-      raw.values(v);
-    } else {
-      if constexpr (VEC) {
-        raw.take8(from, e_shift);
-        if (!p.words) raw.w[2] = k > 0 ? *ep : 0u;
-      } else {
-        raw.load8(static_cast<const uint8_t*>(q) + o, ep, k);
-      }
-      raw.values_of_8(v);
-    }
-  };
   auto fetch = [&](int stage) {
     if (ahead.set < p.plan.sets) {
-      const bool there = ahead.left > 0 && n > 0;
-      if (dr != nullptr) copy(TS{}, 0, stage, dr, nullptr, ahead.row, there);
-      if (p.norm != kNoNorm) {
-        copy(TC{}, p.s_dy, stage, dy, nullptr, ahead.row, there);
-        copy(TS{}, p.s_r, stage, p.r, p.r_e, ahead.row, there);
-      }
-      if (p.dgate != nullptr) copy(TC{}, p.s_u, stage, p.u, p.u_e, ahead.row, there);
-      if (p.x != nullptr) copy(TS{}, p.s_x, stage, p.x, p.x_e, ahead.row, there);
-      if (OWN) {
-        if (gate != nullptr) ring_copy<TC, VEC>(ring + (stage * p.slots + p.s_gate) * kThreads, kThreads, gate + ahead.row * p.gate_ld + ch, there);
-        if (gs != nullptr) ring_copy<TC, VEC>(ring + (stage * p.slots + p.s_g) * kThreads, kThreads, gs + ahead.row * p.gate_shift_ld + ch, there);
+      uint4* s = ring + stage * p.slots * kRowThreads;
+      const long long o = static_cast<long long>(ahead.row) * p.c;
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        const int ch = channel(q);
+        const bool there = ahead.left > 0 && ch < p.c;
+        // a tensor, or its rows in 8 bits: the bytes, and the word of exponents that a piece's lies in
+        auto copy = [&](auto tag, int slot, const void* t, const uint8_t* e) {
+          using E = decltype(tag);
+          if (e == nullptr) {
+            ring_copy(s + (slot + q * (static_cast<int>(sizeof(E)) / 2)) * kRowThreads, static_cast<const E*>(t) + o + ch, there);
+          } else {
+            uint4* to = s + (slot + q) * kRowThreads;
+            copy_async<8>(to, static_cast<const uint8_t*>(t) + o + ch, there);
+            if (p.words) copy_async<4>(reinterpret_cast<uint32_t*>(to) + 2, e + static_cast<long long>(ahead.row) * groups + (ch / kGroup8 & ~3), there);
+          }
+        };
+        if (p.dr != nullptr) copy(TS{}, 0, p.dr, nullptr);
+        if (p.norm != kNoNorm) {
+          copy(TC{}, p.s_dy, p.dy, nullptr);
+          copy(TS{}, p.s_r, p.r, p.r_e);
+        }
+        if (p.dgate != nullptr) copy(TC{}, p.s_u, p.u, p.u_e);
+        if (p.x != nullptr) copy(TS{}, p.s_x, p.x, p.x_e);
+        if (OWN) {
+          if (gate != nullptr) ring_copy(s + (p.s_gate + q * kC) * kRowThreads, gate + ahead.row * p.gate_ld + ch, there);
+          if (gs != nullptr) ring_copy(s + (p.s_g + q * kC) * kRowThreads, gs + ahead.row * p.gate_shift_ld + ch, there);
+        }
       }
       ahead.next(p.plan, team, step);
     }
     copy_async_done();
-  };
-  // logits of this row's gate, or of the norm's
-  auto logits = [&](const TC* table, long long ld, int slot, int stage, unsigned gate_row, int k, float* v) {
-    Piece<TC, VEC> raw;
-    if (OWN && VEC) raw.take(ring + (stage * p.slots + slot) * kThreads, kThreads);
-    else raw.load(table + gate_row * ld + ch, k);
-    raw.values(v);
   };
   if constexpr (VEC) {
 #pragma unroll
@@ -132,146 +119,153 @@ __global__ void __launch_bounds__(Teams<LANES>::kThreads, 2) residual_norm_grad_
       fetch(stage == 0 ? kDepth - 1 : stage - 1);
       copy_async_wait<kDepth - 1>();
     }
-    const int k = here.left > 0 ? n : 0;
     const bool row_there = here.left > 0;
-    const long long o = static_cast<long long>(here.row) * p.c + ch;
-    float t[N], v[N];
+    const uint4* s = ring + stage * p.slots * kRowThreads;
+    const long long o = static_cast<long long>(here.row) * p.c;
+    auto channels = [&](int q) { return row_there ? inside(q) : 0; };
+    auto take = [&](auto tag, int slot, const void* t, const uint8_t* e, int q) {
+      using E = decltype(tag);
+      if (e == nullptr) {
+        if constexpr (VEC) return ring_take<E>(s + (slot + q * (static_cast<int>(sizeof(E)) / 2)) * kRowThreads);
+        else return load_piece<E, VEC>(static_cast<const E*>(t) + o + channel(q), channels(q));
+      }
+      const uint8_t* ep = e + static_cast<long long>(here.row) * groups + channel(q) / kGroup8;
+      if constexpr (VEC) {
+        const uint4 w = s[(slot + q) * kRowThreads];
+        const uint32_t ex = p.words ? w.z >> channel(q) / kGroup8 % 4 * 8 & 255u : channels(q) > 0 ? *ep : 0u;
+        return values8(make_uint2(w.x, w.y), ex);
+      } else {
+        return load_piece8<VEC>(static_cast<const uint8_t*>(t) + o + channel(q), ep, channels(q));
+      }
+    };
+    // gates (gate_at) of this row's output, or of its norm
+    auto own_gates = [&](const TC* table, long long ld, int slot, int q) {
+      Pairs t;
+      if constexpr (VEC) t = ring_take<TC>(s + (slot + q * kC) * kRowThreads);
+      else t = load_piece<TC, VEC>(table + here.row * ld + channel(q), channels(q));
+      return each(t, [](float a) { return gate_at(a); });
+    };
     if (!OWN && here.at == 0) {
       const unsigned gate_row = here.gate_row(p.plan);
-      if (gate != nullptr) {
-        logits(gate, p.gate_ld, 0, 0, gate_row, k, t);
 #pragma unroll
-        for (int i = 0; i < (OWN ? 1 : N); ++i) open[i] = gate_at(t[i]).open;
-      }
-      if (gs != nullptr) {
-        logits(gs, p.gate_shift_ld, 0, 0, gate_row, k, t);
-#pragma unroll
-        for (int i = 0; i < N; ++i) m[i] = gate_at(t[i]).open;
+      for (int q = 0; q < P; ++q) {
+        const int k = channels(q);
+        if (gate != nullptr) open[OWN ? 0 : q] = each(load_piece<TC, VEC>(gate + gate_row * p.gate_ld + channel(q), k), [](float a) { return open_of(gate_at(a)); });
+        if (gs != nullptr) m[q] = each(load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + channel(q), k), [](float a) { return open_of(gate_at(a)); });
       }
     }
-    if (OWN && gs != nullptr) {
-      logits(gs, p.gate_shift_ld, p.s_g, stage, here.row, k, t);
-#pragma unroll
-      for (int i = 0; i < N; ++i) m[i] = gate_at(t[i]).open;
-    }
-    if (dr != nullptr) {
-      take(TS{}, 0, stage, dr, nullptr, t);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) t[i] = 0.f;
-    }
+    Pairs z[P], g[P], rstd2, minus_mean_g, minus_mean_gz;
     if (p.norm != kNoNorm) {
-      float d[N], z[N];
-      take(TC{}, p.s_dy, stage, dy, nullptr, d);
-      take(TS{}, p.s_r, stage, p.r, p.r_e, z);
-      float s[2] = {0.f, 0.f};
+      uint64_t sz = 0, sg = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        s[0] += z[i];
-        s[1] = fmaf(d[i], m[i], s[1]);
-      }
-      team_sum<LANES>(s, room, group, 0);
-      const float mean = s[0] * inv_c, mean_g = s[1] * inv_c;
-      s[0] = s[1] = 0.f;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        z[i] = (VEC ? n > 0 : i < n) ? z[i] - mean : 0.f;
-        s[0] = fmaf(z[i], z[i], s[0]);
-        s[1] = fmaf(d[i] * m[i], z[i], s[1]);
-      }
-      team_sum<LANES>(s, room, group, 1);
-      const float rstd = rsqrtf(fmaf(s[0], inv_c, p.eps)), mean_gz = s[1] * inv_c * rstd;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        z[i] *= rstd;
-        t[i] = fmaf(rstd, fmaf(d[i], m[i], -mean_g) - z[i] * mean_gz, t[i]);
-      }
-      if (OWN && adaptive) {
-        if (p.dgate_shift != nullptr) {
-          logits(gs, p.gate_shift_ld, p.s_g, stage, here.row, k, v);
-#pragma unroll
-          for (int i = 0; i < N; ++i) v[i] = d[i] * z[i] * gate_at(v[i]).slope;
-          TC* q = static_cast<TC*>(p.dgate_shift) + static_cast<long long>(here.row) * 2 * p.c + ch;
-          store_piece<VEC>(q, v, k);
-          store_piece<VEC>(q + p.c, d, k);
+      for (int q = 0; q < P; ++q) {
+        z[q] = take(TS{}, p.s_r, p.r, p.r_e, q);
+        const Pairs d = take(TC{}, p.s_dy, p.dy, nullptr, q);
+        if (OWN && gs != nullptr) {
+          m[q] = own_gates(gs, p.gate_shift_ld, p.s_g, q);
+          g[q] = mul(d, each(m[q], [](float a) { return open_of(a); }));
+        } else {
+          g[q] = mul(d, m[q]);
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          a0[i] = fmaf(d[i], row_there ? z[i] : 0.f, a0[i]);      // (z of no row is not a number where eps is zero)
-          a1[i] += d[i];
-        }
+        sum_into(sz, z[q]);
+        sum_into(sg, g[q]);
       }
+      float t[2] = {total(sz), total(sg)};
+      team_sum<LANES>(t);
+      const Pairs minus_mean = both(-t[0] * inv_c);
+      minus_mean_g = both(-t[1] * inv_c);
+      sz = sg = 0;
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        z[q] = add(z[q], minus_mean);
+        if constexpr (!VEC) {
+#pragma unroll
+          for (int i = 0; i < kPiece; ++i)
+            if (i >= inside(q)) z[q].v[i / 2] = i & 1 ? ptx::pack2(z[q].get(i - 1), 0.f) : ptx::pack2(0.f, 0.f);
+        }
+        if (inside(q) > 0) dot_into(sz, z[q], z[q]);
+        dot_into(sg, g[q], z[q]);
+      }
+      t[0] = total(sz);
+      t[1] = total(sg);
+      team_sum<LANES>(t);
+      const float rstd = rsqrtf(fmaf(t[0], inv_c, p.eps));
+      rstd2 = both(rstd);
+      minus_mean_gz = both(-t[1] * inv_c * rstd);
     }
-    if (p.dgate != nullptr) {
-      take(TC{}, p.s_u, stage, p.u, p.u_e, v);
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      const int k = channels(q), ch = channel(q);
+      Pairs t = p.dr != nullptr ? take(TS{}, 0, p.dr, nullptr, q) : both(0.f);
+      if (p.norm != kNoNorm) {
+        z[q] = mul(z[q], rstd2);
+        t = fma(rstd2, fma(z[q], minus_mean_gz, add(g[q], minus_mean_g)), t);
+        const Pairs d = take(TC{}, p.s_dy, p.dy, nullptr, q);
+        if (OWN && adaptive) {
+          if (p.dgate_shift != nullptr) {
+            TC* to = static_cast<TC*>(p.dgate_shift) + static_cast<long long>(here.row) * 2 * p.c + ch;
+            store_piece<VEC>(to, mul(mul(d, z[q]), each(m[q], [](float a) { return slope_of(a); })), k);
+            store_piece<VEC>(to + p.c, d, k);
+          }
+        } else if (row_there) {                     // (z of no row is not a number where eps is zero)
+          a0[q] = fma(d, z[q], a0[q]);
+          a1[q] = add(a1[q], d);
+        }
+      }
+      Pairs u, own;
+      if (p.dgate != nullptr) u = take(TC{}, p.s_u, p.u, p.u_e, q);
       if constexpr (OWN) {
-        float s[N];
-        logits(gate, p.gate_ld, p.s_gate, stage, here.row, k, s);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = t[i] * v[i] * gate_at(s[i]).slope;
-        store_piece<VEC>(static_cast<TC*>(p.dgate) + o, v, k);
+        if (gate != nullptr) own = own_gates(gate, p.gate_ld, p.s_gate, q);
+        if (p.dgate != nullptr) store_piece<VEC>(static_cast<TC*>(p.dgate) + o + ch, mul(mul(t, u), each(own, [](float a) { return slope_of(a); })), k);
       } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) a2[i] = fmaf(row_there ? t[i] : 0.f, v[i], a2[i]);
+        if (p.dgate != nullptr && row_there) a2[OWN ? 0 : q] = fma(t, u, a2[OWN ? 0 : q]);
       }
-    }
-    if (p.x != nullptr) {
-      take(TS{}, p.s_x, stage, p.x, p.x_e, v);
-#pragma unroll
-      for (int i = 0; i < N; ++i) a3[i] = fmaf(row_there ? t[i] : 0.f, v[i], a3[i]);
-    }
-    if (p.du != nullptr) {
-      if (OWN && gate != nullptr) {
-        logits(gate, p.gate_ld, p.s_gate, stage, here.row, k, v);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = t[i] * gate_at(v[i]).open;
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = t[i] * open[OWN ? 0 : i];
+      if (p.du != nullptr) {
+        Pairs v = t;
+        if (gate != nullptr) {
+          if constexpr (OWN) v = mul(t, each(own, [](float a) { return open_of(a); }));
+          else v = mul(t, open[OWN ? 0 : q]);
+        }
+        store_piece<VEC>(static_cast<TC*>(p.du) + o + ch, v, k);
       }
-      store_piece<VEC>(static_cast<TC*>(p.du) + o, v, k);
-    }
-    if (p.dx != nullptr) {
-      if (p.scale != nullptr) {
+      if (p.x != nullptr && row_there) {
+        const Pairs v = mul(t, take(TS{}, p.s_x, p.x, p.x_e, q));
 #pragma unroll
-        for (int i = 0; i < N; ++i) t[i] *= i < n ? p.scale[ch + i] : 0.f;
+        for (int i = 0; i < kPiece; ++i) scale_sums[(q * kPiece + i) * kRowThreads] += v.get(i);
       }
-      store_piece<VEC>(static_cast<TS*>(p.dx) + o, t, k);
+      if (p.dx != nullptr) {
+        if (p.scale != nullptr) t = mul(t, vector(p.scale, q, 0.f));
+        store_piece<VEC>(static_cast<TS*>(p.dx) + o + ch, t, k);
+      }
     }
     if constexpr (!OWN) {
       if (here.at + 1 == p.plan.chunk) {
         // the end of a piece: the gates' gradients from the sums over their samples, the logits once more for their slopes; or the sums for the second kernel
         const bool there = here.unit < p.plan.units;
-        const int kk = there ? n : 0;
         const unsigned gate_row = here.gate_row(p.plan);
-        if (p.pieces != nullptr) {
-          float* q = p.pieces + static_cast<long long>(there ? here.unit : 0) * 3 * p.c + ch;
-          if (adaptive) {
-            store_piece<VEC>(q, a0, kk);
-            store_piece<VEC>(q + p.c, a1, kk);
-          }
-          if (p.dgate != nullptr) store_piece<VEC>(q + 2 * p.c, a2, kk);
-        } else {
-          if (adaptive && p.dgate_shift != nullptr) {
-            logits(gs, p.gate_shift_ld, 0, 0, gate_row, kk, v);
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = a0[i] * gate_at(v[i]).slope;
-            TC* q = static_cast<TC*>(p.dgate_shift) + static_cast<long long>(gate_row) * 2 * p.c + ch;
-            store_piece<VEC>(q, v, kk);
-            store_piece<VEC>(q + p.c, a1, kk);
+        for (int q = 0; q < P; ++q) {
+          const int k = there ? inside(q) : 0, ch = channel(q);
+          const long long to = static_cast<long long>(gate_row) * p.c + ch;
+          if (p.pieces != nullptr) {
+            float* d = p.pieces + static_cast<long long>(there ? here.unit : 0) * 3 * p.c + ch;
+            if (adaptive) {
+              store_piece<VEC>(d, a0[q], k);
+              store_piece<VEC>(d + p.c, a1[q], k);
+            }
+            if (p.dgate != nullptr) store_piece<VEC>(d + 2 * p.c, a2[OWN ? 0 : q], k);
+          } else {
+            auto slope = [](float a) { return slope_of(gate_at(a)); };
+            if (adaptive && p.dgate_shift != nullptr) {
+              TC* d = static_cast<TC*>(p.dgate_shift) + 2 * to - ch;
+              store_piece<VEC>(d, mul(a0[q], each(load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + ch, k), slope)), k);
+              store_piece<VEC>(d + p.c, a1[q], k);
+            }
+            if (p.dgate != nullptr)
+              store_piece<VEC>(static_cast<TC*>(p.dgate) + to, mul(a2[OWN ? 0 : q], each(load_piece<TC, VEC>(gate + gate_row * p.gate_ld + ch, k), slope)), k);
           }
-          if (p.dgate != nullptr) {
-            logits(gate, p.gate_ld, 0, 0, gate_row, kk, v);
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = a2[i] * gate_at(v[i]).slope;
-            store_piece<VEC>(static_cast<TC*>(p.dgate) + static_cast<long long>(gate_row) * p.c + ch, v, kk);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          a2[i] = 0.f;
-          if (adaptive) a0[i] = a1[i] = 0.f;
+          a2[OWN ? 0 : q] = both(0.f);
+          if (adaptive) a0[q] = a1[q] = both(0.f);
         }
       }
     }
@@ -282,19 +276,23 @@ __global__ void __launch_bounds__(Teams<LANES>::kThreads, 2) residual_norm_grad_
   if (p.partial != nullptr) {
     // the block's teams in their order; the ring's memory, in which nothing is on its way any more
     copy_async_wait<0>();
-    float* flat = reinterpret_cast<float*>(ring_memory);      // [team][LANES * 8]
+    constexpr int kAll = kRowThreads / LANES, kWidth = LANES * P * kPiece;
+    float* flat = reinterpret_cast<float*>(ring_memory);      // [team][kWidth]
 #pragma unroll
     for (int j = 0; j < 3; ++j) {
-      const float* a = j == 0 ? a0 : j == 1 ? a1 : a3;
+      if (j == 2 && p.x == nullptr) break;
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < N; ++i) flat[(group * T::kTeams + team) * LANES * N + ch + i] = a[i];
+      for (int q = 0; q < P; ++q)
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i)
+          flat[static_cast<int>(threadIdx.x) / LANES * kWidth + channel(q) + i] = j == 0 ? a0[q].get(i) : j == 1 ? a1[q].get(i) : scale_sums[(q * kPiece + i) * kRowThreads];
       __syncthreads();
-      for (int i = threadIdx.x; i < p.c; i += kThreads) {
-        float s = 0.f;
+      for (int i = threadIdx.x; i < p.c; i += kRowThreads) {
+        float t = 0.f;
 #pragma unroll 4
-        for (int q = 0; q < T::kGroups * T::kTeams; ++q) s += flat[q * LANES * N + i];
-        p.partial[(static_cast<long long>(blockIdx.x) * 3 + j) * p.c + i] = s;
+        for (int q = 0; q < kAll; ++q) t += flat[q * kWidth + i];
+        p.partial[(static_cast<long long>(blockIdx.x) * 3 + j) * p.c + i] = t;
       }
     }
   }
@@ -342,43 +340,42 @@ __global__ void __launch_bounds__(256) residual_norm_gates_kernel(const float* p
     float v;
     if (dgs != nullptr) {
       TC* d = dgs + static_cast<long long>(row) * 2 * c + ch;
-      v = s[0] * gate_at(static_cast<float>(gs[row * gs_ld + ch])).slope;
+      v = s[0] * slope_of(gate_at(static_cast<float>(gs[row * gs_ld + ch])));
       store_vec<1>(d, &v);
       store_vec<1>(d + c, &s[1]);
     }
     if (dgate != nullptr) {
-      v = s[2] * gate_at(static_cast<float>(gate[row * gate_ld + ch])).slope;
+      v = s[2] * slope_of(gate_at(static_cast<float>(gate[row * gate_ld + ch])));
       store_vec<1>(dgate + static_cast<long long>(row) * c + ch, &v);
     }
   }
 }
 
-constexpr int kBlocksPerSm = 4;      // at most: the workspace's partial sums are sized by it
+// Blocks of an SM, at most, and SMs: the workspace is sized by them.
+constexpr int most_blocks(int c) { return c <= 256 ? 6 : c <= 512 ? 3 : 2; }
 constexpr int kMostSms = 160;
-constexpr int kMostRing = 216 * 1024;
-// Pieces of gate rows' samples, at most: two for each team that is at work (row_plan), of which a block has so many.
-constexpr long long most_units(int c) { return 2ll * kMostSms * kBlocksPerSm * (c <= 64 ? 32 : c <= 128 ? 16 : c <= 256 ? 8 : c <= 512 ? 4 : c <= 768 ? 3 : 2); }
+// Pieces of gate rows' samples, at most: two for each team that is at work (row_plan).
+constexpr long long most_units(int c) { return 2ll * kMostSms * most_blocks(c) * (c <= 64 ? 16 : c <= 128 ? 8 : c <= 256 ? 4 : c <= 384 ? 8 : 4); }
 
 struct Sums {
   float *dweight, *dbias, *dscale;
 };
 
-template <typename TS, typename TC, int LANES, bool VEC, bool OWN>
+template <typename TS, typename TC, int LANES, int P, bool VEC, bool OWN>
 int launch(cudaStream_t stream, GradParams p, const Sums& sums, long long rows, int samples, int l) {
-  using T = Teams<LANES>;
-  constexpr auto kernel = residual_norm_grad_kernel<TS, TC, LANES, VEC, OWN>;
-  constexpr int kS = sizeof(TS) / 2, kC = sizeof(TC) / 2, kDepth = OWN ? 3 : 4, kFlat = T::kThreads * kPiece * 4;
+  constexpr auto kernel = residual_norm_grad_kernel<TS, TC, LANES, P, VEC, OWN>;
+  constexpr int kS = P * sizeof(TS) / 2, kC = P * sizeof(TC) / 2, kWarps = kRowThreads / 32, kTeams = 32 / LANES, kFlat = kRowThreads * P * kPiece * 4;
   static std::once_flag once;
   static int held = 1;
   std::call_once(once, [&] {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, T::kThreads, 0) != cudaSuccess) cudaGetLastError();
-    held = held < 1 ? 1 : held > kBlocksPerSm ? kBlocksPerSm : held;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, kRowThreads, 0) != cudaSuccess) cudaGetLastError();
+    held = held < 1 ? 1 : held;
   });
-  // (a row in 8 bits takes one slot)
+  // (a row in 8 bits takes one slot a piece)
   int slots = p.dr != nullptr ? kS : 0;
   auto place = [&](bool there, bool small, int size) {
     const int at = slots;
-    slots += !there ? 0 : small ? 1 : size;
+    slots += !there ? 0 : small ? P : size;
     return at;
   };
   p.s_dy = place(p.norm != kNoNorm, false, kC);
@@ -388,20 +385,23 @@ int launch(cudaStream_t stream, GradParams p, const Sums& sums, long long rows, 
   p.s_gate = place(OWN && p.gate != nullptr, false, kC);
   p.s_g = place(OWN && p.gate_shift != nullptr, false, kC);
   p.slots = slots;
-  int smem = VEC ? kDepth * slots * T::kThreads * 16 : 0;
+  int smem = VEC ? depth<TS, TC, P, OWN>() * slots * kRowThreads * 16 : 0;
   if (p.partial != nullptr && smem < kFlat) smem = kFlat;
+  p.s_scale = smem / 16 / kRowThreads;
+  if (p.x != nullptr) smem += kFlat;
   KFB_TRY(allow_smem<kernel>(kMostRing));
-  const int fit = smem > 0 ? kMostRing / smem : held, blocks_per_sm = held < fit ? held : fit < 1 ? 1 : fit;
-  const long long most = static_cast<long long>(sm_count() < kMostSms ? sm_count() : kMostSms) * blocks_per_sm, teams = T::kGroups * T::kTeams;
-  p.plan = row_plan(rows, samples, l, most * teams, T::kTeams);
+  KFB_CHECK_ARG(smem <= kMostRing, "residual_norm_bwd: %d bytes of shared memory", smem);
+  const int fit = smem > 0 ? kMostRing / smem : held, limit = held < most_blocks(p.c) ? held : most_blocks(p.c), blocks_per_sm = limit < fit ? limit : fit;
+  const long long most = static_cast<long long>(sm_count() < kMostSms ? sm_count() : kMostSms) * blocks_per_sm;
+  p.plan = row_plan(rows, samples, l, most * kWarps * kTeams, kTeams);
   const bool gates = p.dgate != nullptr || p.dgate_shift != nullptr;
   if (p.plan.chunks == 1 || !gates) p.pieces = nullptr;
   else KFB_CHECK_ARG(p.plan.units <= most_units(p.c), "residual_norm_bwd: %u pieces", p.plan.units);
-  const long long want = (p.plan.sets + T::kGroups - 1) / T::kGroups;
+  const long long want = (p.plan.sets + kWarps - 1) / kWarps;
   const unsigned blocks = static_cast<unsigned>(want < most ? want : most);
   {
     LaunchScope scope(stream, "residual_norm_grad");
-    KFB_TRY(launch_kernel(stream, kernel, blocks, T::kThreads, smem, p));
+    KFB_TRY(launch_kernel(stream, kernel, blocks, kRowThreads, smem, p));
   }
   if (p.pieces != nullptr) {
     const long long n = (static_cast<long long>(p.plan.gate_rows) * p.c + 255) / 256, grid = 4ll * sm_count();
@@ -412,15 +412,16 @@ int launch(cudaStream_t stream, GradParams p, const Sums& sums, long long rows, 
   }
   if (p.partial != nullptr) {
     LaunchScope scope(stream, "residual_norm_sum");
-    KFB_TRY(launch_kernel(stream, residual_norm_sum_kernel, cdiv(3 * p.c, 32), 1024, 0, const_cast<const float*>(p.partial), sums.dweight, sums.dbias,
-                          sums.dscale, static_cast<int>(blocks), p.c));
+    KFB_TRY(launch_kernel(stream, residual_norm_sum_kernel, cdiv((p.x != nullptr ? 3 : 2) * p.c, 32), 1024, 0, const_cast<const float*>(p.partial), sums.dweight,
+                          sums.dbias, sums.dscale, static_cast<int>(blocks), p.c));
   }
   return KFB_OK;
 }
 
-template <typename TS, typename TC, int LANES, bool VEC>
+template <typename TS, typename TC, int LANES, int P, bool VEC>
 int launch_own(cudaStream_t stream, const GradParams& p, const Sums& sums, long long rows, int samples, int l) {
-  return samples == 1 ? launch<TS, TC, LANES, VEC, true>(stream, p, sums, rows, samples, l) : launch<TS, TC, LANES, VEC, false>(stream, p, sums, rows, samples, l);
+  return samples == 1 ? launch<TS, TC, LANES, P, VEC, true>(stream, p, sums, rows, samples, l)
+                      : launch<TS, TC, LANES, P, VEC, false>(stream, p, sums, rows, samples, l);
 }
 
 template <typename TS, typename TC>
@@ -431,18 +432,12 @@ int dispatch(cudaStream_t stream, GradParams p, const Sums& sums, long long rows
                        reinterpret_cast<uintptr_t>(p.du) | reinterpret_cast<uintptr_t>(p.dgate) | reinterpret_cast<uintptr_t>(p.dgate_shift) |
                        static_cast<uintptr_t>((p.gate_ld | p.gate_shift_ld) * sizeof(TC));
   p.words = groups8(p.c) % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.r_e) | reinterpret_cast<uintptr_t>(p.u_e) | reinterpret_cast<uintptr_t>(p.x_e)) & 3) == 0;
-  if (p.c % 8 == 0 && (at & 15) == 0) {
-    if (p.c <= 64) return launch_own<TS, TC, 8, true>(stream, p, sums, rows, samples, l);
-    if (p.c <= 128) return launch_own<TS, TC, 16, true>(stream, p, sums, rows, samples, l);
-    if (p.c <= 256) return launch_own<TS, TC, 32, true>(stream, p, sums, rows, samples, l);
-    if (p.c <= 512) return launch_own<TS, TC, 64, true>(stream, p, sums, rows, samples, l);
-    if (p.c <= 768) return launch_own<TS, TC, 96, true>(stream, p, sums, rows, samples, l);
-    return launch_own<TS, TC, 128, true>(stream, p, sums, rows, samples, l);
-  }
-  return p.c <= 256 ? launch_own<TS, TC, 32, false>(stream, p, sums, rows, samples, l) : launch_own<TS, TC, 128, false>(stream, p, sums, rows, samples, l);
+#define KFB_CALL(LANES, P, VEC) launch_own<TS, TC, LANES, P, VEC>(stream, p, sums, rows, samples, l)
+  KFB_ROW_SHAPES(p.c, p.c % 8 == 0 && (at & 15) == 0, KFB_CALL);
+#undef KFB_CALL
 }
 
-size_t partial_bytes(int c) { return align_up(static_cast<size_t>(kMostSms) * kBlocksPerSm * 3 * c * sizeof(float), 256); }
+size_t partial_bytes(int c) { return align_up(static_cast<size_t>(kMostSms) * most_blocks(c) * 3 * c * sizeof(float), 256); }
 
 }  // namespace
 }  // namespace kfb

@@ -1,7 +1,9 @@
-// Rows of up to 1024 channels, eight a lane: what the kernels of the residual stream share (residual_norm.cu, residual_norm_grad.cu, compress.cu).
+// Rows of up to 1024 channels in the registers of up to 32 lanes: what the kernels of the residual stream share (residual_norm.cu,
+// residual_norm_grad.cu), and rows in 8 bits (compress.cu too).
 //
-// A row is held by a team of 8 ... 128 lanes, each with eight neighbouring channels; teams of up to 32 lanes share a warp, larger ones are whole
-// warps that meet at a barrier of their own.  A lane's piece is 16 or 32 bytes of bf16 or float32, or 8 bytes of a row kept in 8 bits.
+// A team of 8, 16 or 32 lanes holds a row, P pieces of eight neighbouring channels a lane; a piece is 16 or 32 bytes of bf16 or float32, or 8 bytes of a row
+// kept in 8 bits, and four pairs of float32 in registers, which the two-wide instructions take at one issue slot a pair.  (One piece a lane, and several warps
+// for a wide row, took 375 instructions a warp and row where these rows of 768 channels take a third; issue slots were what bounded them.)
 //
 // Rows in 8 bits: 32 neighbouring channels share a power of two.  A value is q 2^(e - 133), q a whole number of -127 ... 127, e a byte:
 // the exponent field of the group's largest magnitude as a float32, one more where that magnitude would round to 128.  So a value is off by at
@@ -11,15 +13,97 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
+#include "ptx.cuh"
 #include "vec_io.cuh"
 
 namespace kfb {
 
-constexpr int kPiece = 8;         // channels of a lane
+constexpr int kPiece = 8;         // channels of a piece
 constexpr int kGroup8 = 32;       // channels that share an exponent
 
 __host__ __device__ inline int groups8(int c) { return (c + kGroup8 - 1) / kGroup8; }
 
+struct Pairs {
+  uint64_t v[kPiece / 2];
+  __device__ __forceinline__ float get(int i) const {
+    const float2 f = ptx::unpack2(v[i / 2]);
+    return i & 1 ? f.y : f.x;
+  }
+};
+__device__ __forceinline__ Pairs both(float a) {
+  const uint64_t t = ptx::pack2(a, a);
+  return {{t, t, t, t}};
+}
+__device__ __forceinline__ Pairs of_floats(const float* f) {
+  Pairs r;
+#pragma unroll
+  for (int i = 0; i < kPiece / 2; ++i) r.v[i] = ptx::pack2(f[2 * i], f[2 * i + 1]);
+  return r;
+}
+__device__ __forceinline__ Pairs of_bf16(const uint4& w) {
+  const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+  Pairs r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = ptx::pack2(q[i] << 16, q[i] & 0xffff0000u);
+  return r;
+}
+__device__ __forceinline__ Pairs of_f32(const uint4& a, const uint4& b) {
+  return {{ptx::pack2(a.x, a.y), ptx::pack2(a.z, a.w), ptx::pack2(b.x, b.y), ptx::pack2(b.z, b.w)}};
+}
+__device__ __forceinline__ uint4 to_bf16(const Pairs& p) {
+  uint32_t q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = ptx::unpack2(p.v[i]);
+    q[i] = bf16_pair_of(f.x, f.y);
+  }
+  return make_uint4(q[0], q[1], q[2], q[3]);
+}
+__device__ __forceinline__ Pairs add(const Pairs& a, const Pairs& b) {
+  Pairs r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = ptx::add2(a.v[i], b.v[i]);
+  return r;
+}
+__device__ __forceinline__ Pairs mul(const Pairs& a, const Pairs& b) {
+  Pairs r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = ptx::mul2(a.v[i], b.v[i]);
+  return r;
+}
+__device__ __forceinline__ Pairs fma(const Pairs& a, const Pairs& b, const Pairs& c) {
+  Pairs r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = ptx::fma2(a.v[i], b.v[i], c.v[i]);
+  return r;
+}
+// v plus the sum of a's elements, or of a's by b's, kept in pairs
+__device__ __forceinline__ void sum_into(uint64_t& v, const Pairs& a) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v = ptx::add2(v, a.v[i]);
+}
+__device__ __forceinline__ void dot_into(uint64_t& v, const Pairs& a, const Pairs& b) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v = ptx::fma2(a.v[i], b.v[i], v);
+}
+__device__ __forceinline__ float total(uint64_t v) {
+  const float2 f = ptx::unpack2(v);
+  return f.x + f.y;
+}
+template <typename F>
+__device__ __forceinline__ Pairs each(const Pairs& a, F f) {
+  Pairs r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = ptx::unpack2(a.v[i]);
+    r.v[i] = ptx::pack2(f(t.x), f(t.y));
+  }
+  return r;
+}
+
+// ---- rows in 8 bits
 // The exponent byte of a group whose largest magnitude has these bits.
 __device__ __forceinline__ uint32_t exponent8(uint32_t top) {
   if (top >= 0x7f800000u) return 255u;
@@ -30,181 +114,138 @@ __device__ __forceinline__ float step8(uint32_t e) { return e == 255u ? __uint_a
 // What values are multiplied by before they are rounded.
 __device__ __forceinline__ float inverse_step8(uint32_t e) { return e == 255u || e == 0u ? 0.f : __uint_as_float((260u - e) << 23); }
 
-// Four whole numbers as bytes: adding 1.5 2^23 rounds to the nearest (ties to even) and leaves the number in the low byte.
-__device__ __forceinline__ uint32_t bytes8(const float* v, float inverse) {
-  uint32_t q[4];
+// Eight whole numbers as bytes: adding 1.5 2^23 rounds to the nearest (ties to even) and leaves the number in the low byte.
+__device__ __forceinline__ uint2 bytes8(const Pairs& p, uint32_t e) {
+  const float inverse = inverse_step8(e);
+  Pairs t = p;
+  if (e == 254u) t = each(p, [inverse](float v) { return fminf(fmaxf(v, -127.f / inverse), 127.f / inverse); });      // (the one that stops short)
+  t = fma(t, both(inverse), both(12582912.f));
+  uint32_t w[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float t = fminf(fmaxf(v[i] * inverse, -127.f), 127.f);
-    q[i] = __float_as_uint(t + 12582912.f);
+  for (int i = 0; i < 2; ++i) {
+    const float2 a = ptx::unpack2(t.v[2 * i]), b = ptx::unpack2(t.v[2 * i + 1]);
+    w[i] = __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
   }
-  return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+  return e == 255u ? make_uint2(0u, 0u) : make_uint2(w[0], w[1]);      // (what is not finite times zero is no number)
 }
 // ... and back: a byte with its sign turned round in the low byte of 2^23 is 2^23 + 128 + q.
-__device__ __forceinline__ void values8(uint32_t bytes, float step, float* v) {
-  const uint32_t t = bytes ^ 0x80808080u;
+__device__ __forceinline__ Pairs values8(const uint2& bytes, uint32_t e) {
+  Pairs r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (__uint_as_float(__byte_perm(t, 0x4b000000u, 0x7650 | i)) - 8388736.f) * step;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t t = (i < 2 ? bytes.x : bytes.y) ^ 0x80808080u, at = 2 * (i & 1);
+    r.v[i] = ptx::pack2(__byte_perm(t, 0x4b000000u, 0x7650 | at), __byte_perm(t, 0x4b000000u, 0x7650 | (at + 1)));
+  }
+  return mul(add(r, both(-8388736.f)), both(step8(e)));
+}
+// The bits of the largest magnitude of a piece, in float32: of values, or of bf16 words, two at a time.
+__device__ __forceinline__ uint32_t top_of(const Pairs& p) {
+  uint32_t t = 0u;
+#pragma unroll
+  for (int i = 0; i < kPiece; ++i) t = max(t, __float_as_uint(p.get(i)) & 0x7fffffffu);
+  return t;
+}
+__device__ __forceinline__ uint32_t top_of(const uint4& w) {
+  const uint32_t m = 0x7fff7fffu, t = __vmaxu2(__vmaxu2(w.x & m, w.y & m), __vmaxu2(w.z & m, w.w & m));
+  return max(t << 16, t & 0xffff0000u);
+}
+// ... of a group, which four neighbouring lanes hold.
+__device__ __forceinline__ uint32_t group_top(uint32_t t) {
+  t = max(t, __shfl_xor_sync(0xffffffffu, t, 1));
+  return max(t, __shfl_xor_sync(0xffffffffu, t, 2));
 }
 
-// A lane's eight channels as they lie in memory, of which `n` are there.  VEC: n is 0 or 8 and the address on a 16-byte boundary (8 for bytes).
+// ---- pieces in memory, of which `n` channels are there.  VEC: n is 0 or 8 and the address on a 16-byte boundary (8 for bytes).
 template <typename T, bool VEC>
-struct Piece {
-  static constexpr int kWords = kPiece * static_cast<int>(sizeof(T)) / 4;
-  uint32_t w[kWords];
-  __device__ __forceinline__ void load(const T* p, int n) {
-    if constexpr (VEC) {
-#pragma unroll
-      for (int i = 0; i < kWords; i += 4) {
-        const uint4 t = n > 0 ? reinterpret_cast<const uint4*>(p)[i / 4] : make_uint4(0, 0, 0, 0);
-        w[i] = t.x;
-        w[i + 1] = t.y;
-        w[i + 2] = t.z;
-        w[i + 3] = t.w;
-      }
-    } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < kPiece; ++i) w[i] = i < n ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
-    } else {
-      const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
-#pragma unroll
-      for (int i = 0; i < kPiece; i += 2) {
-        const uint32_t lo = i < n ? s[i] : 0u, hi = i + 1 < n ? s[i + 1] : 0u;
-        w[i / 2] = lo | hi << 16;
-      }
-    }
-  }
-  __device__ __forceinline__ void values(float* v) const {
+__device__ __forceinline__ Pairs load_piece(const T* p, int n) {
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  if constexpr (VEC) {
+    const uint4* q = reinterpret_cast<const uint4*>(p);
+    if constexpr (sizeof(T) == 2) return of_bf16(n > 0 ? q[0] : zero);
+    else return of_f32(n > 0 ? q[0] : zero, n > 0 ? q[1] : zero);
+  } else {
+    float f[kPiece];
 #pragma unroll
     for (int i = 0; i < kPiece; ++i) {
-      if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
-      else v[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+      if constexpr (sizeof(T) == 2) f[i] = i < n ? __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(p)[i]) << 16) : 0.f;
+      else f[i] = i < n ? p[i] : 0.f;
     }
-  }
-  // A piece on its way through shared memory (see Ring), and bytes with the word of exponents that theirs lies in.
-  __device__ __forceinline__ void take(const uint4* slot, int stride) {
-#pragma unroll
-    for (int i = 0; i < kWords; i += 4) {
-      const uint4 t = slot[i / 4 * stride];
-      w[i] = t.x;
-      w[i + 1] = t.y;
-      w[i + 2] = t.z;
-      w[i + 3] = t.w;
-    }
-  }
-  __device__ __forceinline__ void take8(const uint4* slot, int shift) {
-    const uint4 t = *slot;
-    w[0] = t.x;
-    w[1] = t.y;
-    w[2] = t.z >> shift & 255u;
-  }
-  // Bytes and their exponent in the same registers.
-  __device__ __forceinline__ void load8(const uint8_t* p, const uint8_t* e, int n) {
-    if constexpr (VEC) {
-      const uint2 t = n > 0 ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
-      w[0] = t.x;
-      w[1] = t.y;
-    } else {
-      w[0] = w[1] = 0u;
-#pragma unroll
-      for (int i = 0; i < kPiece; ++i)
-        if (i < n) w[i / 4] |= static_cast<uint32_t>(p[i]) << 8 * (i & 3);
-    }
-    w[2] = n > 0 ? *e : 0u;
-  }
-  __device__ __forceinline__ void values_of_8(float* v) const {
-    const float step = step8(w[2]);
-    values8(w[0], step, v);
-    values8(w[1], step, v + 4);
-  }
-};
-
-// The first n of eight values to memory.
-template <bool VEC, typename T>
-__device__ __forceinline__ void store_piece(T* p, const float* v, int n) {
-  if constexpr (VEC) {
-    if (n > 0) store_vec<kPiece>(p, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPiece; ++i)
-      if (i < n) store_vec<1>(p + i, v + i);
+    return of_floats(f);
   }
 }
-
-// A lane's eight values (zeros where the row has ended) into bytes and, by the first lane of a group, its exponent.  Four neighbouring lanes hold a group.
 template <bool VEC>
-__device__ __forceinline__ void store_piece8(uint8_t* p, uint8_t* e, const float* v, int n, bool first) {
-  uint32_t top = 0u;
-#pragma unroll
-  for (int i = 0; i < kPiece; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  const uint32_t ex = exponent8(top);
-  const float inverse = inverse_step8(ex);
-  uint32_t q[2] = {bytes8(v, inverse), bytes8(v + 4, inverse)};
-  if (ex == 255u) q[0] = q[1] = 0u;      // (what is not finite times zero is no number)
+__device__ __forceinline__ Pairs load_piece8(const uint8_t* p, const uint8_t* e, int n) {
+  uint2 b = make_uint2(0, 0);
   if constexpr (VEC) {
-    if (n > 0) *reinterpret_cast<uint2*>(p) = make_uint2(q[0], q[1]);
+    if (n > 0) b = *reinterpret_cast<const uint2*>(p);
   } else {
 #pragma unroll
     for (int i = 0; i < kPiece; ++i)
-      if (i < n) p[i] = static_cast<uint8_t>(q[i / 4] >> 8 * (i & 3));
+      if (i < n) (i < 4 ? b.x : b.y) |= static_cast<uint32_t>(p[i]) << 8 * (i & 3);
+  }
+  return values8(b, n > 0 ? *e : 0u);
+}
+template <bool VEC, typename T>
+__device__ __forceinline__ void store_piece(T* p, const Pairs& v, int n) {
+  if constexpr (VEC) {
+    if (n <= 0) return;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(p) = to_bf16(v);
+    } else {
+      ulonglong2* q = reinterpret_cast<ulonglong2*>(p);
+      q[0] = make_ulonglong2(v.v[0], v.v[1]);
+      q[1] = make_ulonglong2(v.v[2], v.v[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) {
+      const float f = v.get(i);
+      if (i < n) store_vec<1>(p + i, &f);
+    }
+  }
+}
+// Bytes, and by the first lane of a group its exponent.
+template <bool VEC>
+__device__ __forceinline__ void store_piece8(uint8_t* p, uint8_t* e, const Pairs& v, uint32_t ex, int n, bool first) {
+  const uint2 q = bytes8(v, ex);
+  if constexpr (VEC) {
+    if (n > 0) *reinterpret_cast<uint2*>(p) = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i)
+      if (i < n) p[i] = static_cast<uint8_t>((i < 4 ? q.x : q.y) >> 8 * (i & 3));
   }
   if (first && n > 0) *e = static_cast<uint8_t>(ex);
 }
 
-// Copies of 16, 8 or 4 bytes into shared memory that arrive while the thread goes on; zeros where `there` is false.
+// ---- copies of 16, 8 or 4 bytes into shared memory that arrive while the thread goes on; zeros where `there` is false
 __device__ __forceinline__ void copy_async16(void* to, const void* from, bool there) {
   const int n = there ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from), "r"(n) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(to)), "l"(from), "r"(n) : "memory");
 }
 template <int BYTES>
 __device__ __forceinline__ void copy_async(void* to, const void* from, bool there) {
   const int n = there ? BYTES : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from), "n"(BYTES), "r"(n) : "memory");
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(ptx::smem_u32(to)), "l"(from), "n"(BYTES), "r"(n) : "memory");
 }
 __device__ __forceinline__ void copy_async_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LATER>
 __device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory"); }
 
-// Threads of a block and teams in it.
-template <int LANES>
-struct Teams {
-  static constexpr int kGroupLanes = LANES < 32 ? 32 : LANES;        // a warp of small teams, or a large team: what moves from row to row together
-  static constexpr int kThreads = LANES == 96 ? 288 : 256;
-  static constexpr int kGroups = kThreads / kGroupLanes, kTeams = kGroupLanes / LANES;
-  static constexpr int kWarps = LANES < 32 ? 1 : LANES / 32;
-};
-
-// Sums of K values over a team's lanes, the same in all of them and in the same order each time.  `turn` alternates from call to call: a buffer is
-// written again only behind the barrier of the call between, which every reader of it has passed.
-template <int LANES, int K>
-__device__ __forceinline__ void team_sum(float (&v)[K], float (*room)[Teams<LANES>::kGroups][Teams<LANES>::kWarps][K], int group, int turn) {
-#pragma unroll
-  for (int m = (LANES < 32 ? LANES : 32) / 2; m > 0; m >>= 1)
-#pragma unroll
-    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], m);
-  if constexpr (LANES > 32) {
-    const int in_team = static_cast<int>(threadIdx.x) % LANES, warp = in_team / 32;
-    if (in_team % 32 == 0) {
-#pragma unroll
-      for (int k = 0; k < K; ++k) room[turn][group][warp][k] = v[k];
-    }
-    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(LANES) : "memory");
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      float t = room[turn][group][0][k];
-#pragma unroll
-      for (int w = 1; w < LANES / 32; ++w) t += room[turn][group][w][k];
-      v[k] = t;
-    }
-  }
+// ---- gates
+// A gate with logit a as one number: sigmoid(-|a|), with a's sign.  Both sigmoid(a) and its slope come from it without the subtraction that would
+// lose the slope of an open gate.
+__device__ __forceinline__ float gate_at(float a) {
+  const float e = __expf(-fabsf(a));
+  return copysignf(__fdividef(e, 1.f + e), a);
 }
+__device__ __forceinline__ float open_of(float q) { return __float_as_int(q) < 0 ? -q : 1.f - q; }
+__device__ __forceinline__ float slope_of(float q) { return fmaf(-q, q, fabsf(q)); }
 
-// sigmoid(a) to float32's own rounding, for sums that are stored and then put away in 8 bits: where the sum lies near a border between two stored values, an
+// The same to float32's own rounding, for sums that are stored and then put away in 8 bits: where the sum lies near a border between two stored values, an
 // error of the fast exponential (some 2^-21) decides ten times as often as rounding does.  exp(y) by its Taylor series to y^7 / 7! for |y| <= ln 2 / 2
-// (the rest is below 2^-27), the powers of two apart.
-__device__ __forceinline__ float open_exact(float a) {
+// (the rest is below 2^-27), the powers of two apart; one step of Newton's iteration for the reciprocal.
+__device__ __forceinline__ float exact_gate_at(float a) {
   const float x = -fabsf(a), k = rintf(x * 1.44269504f);
   const float y = fmaf(k, -3.19461849e-5f, fmaf(k, -0.693115234375f, x));      // x - k ln 2, ln 2 in two parts, the first of 12 bits
   float t = 1.f / 5040.f;
@@ -215,18 +256,9 @@ __device__ __forceinline__ float open_exact(float a) {
   t = fmaf(t, y, 0.5f);
   t = fmaf(t, y, 1.f);
   t = fmaf(t, y, 1.f);
-  const float e = x < -87.f ? 0.f : t * __uint_as_float(static_cast<uint32_t>(static_cast<int>(k) + 127) << 23);
-  const float d = __frcp_rn(1.f + e);
-  return a < 0.f ? e * d : d;
-}
-
-// sigmoid(a) and its slope, from exp(-|a|): 1 - sigmoid(a) by subtraction would lose the slope of an open gate.
-struct Gate {
-  float open, slope;
-};
-__device__ __forceinline__ Gate gate_at(float a) {
-  const float e = __expf(-fabsf(a)), d = __fdividef(1.f, 1.f + e);
-  return {a < 0.f ? e * d : d, e * d * d};
+  const float e = x < -87.f ? 0.f : __int_as_float(__float_as_int(t) + (static_cast<int>(k) << 23));
+  const float w = 1.f + e, d = __fdividef(1.f, w);
+  return copysignf(e * fmaf(d, fmaf(-w, d, 1.f), d), a);
 }
 
 }  // namespace kfb

@@ -28,20 +28,24 @@ constexpr int depth() { return ring_depth(P * 8 * (sizeof(TS) + (OWN ? 4 : 1) * 
 
 template <typename TS, typename TC, int LANES, int P, bool VEC, bool OWN>
 __global__ void __launch_bounds__(kRowThreads) residual_norm_kernel(const Params p) {
-  constexpr int kDepth = depth<TS, TC, P, OWN>(), kS = sizeof(TS) / 2, kC = sizeof(TC) / 2;
+  constexpr int kDepth = depth<TS, TC, P, OWN>(), kC = sizeof(TC) / 2;
+  constexpr int kStep = LANES * kPiece;      // channels from a lane's piece to its next
   extern __shared__ uint4 ring_memory[];
   grid_dependency_enter();
-  const int warp = threadIdx.x / 32, sub = threadIdx.x % LANES, team = threadIdx.x % 32 / LANES;
+  const int warp = threadIdx.x / 32, ch = threadIdx.x % LANES * kPiece, team = threadIdx.x % 32 / LANES;
   const float inv_c = 1.0f / static_cast<float>(p.c);
-  const TS* x = static_cast<const TS*>(p.x);
-  const TC *u = static_cast<const TC*>(p.u), *gate = static_cast<const TC*>(p.gate), *gs = static_cast<const TC*>(p.gate_shift);
-  uint4* ring = ring_memory + threadIdx.x;
-  auto channel = [&](int q) { return (q * LANES + sub) * kPiece; };
-  auto inside = [&](int q) { return VEC ? (channel(q) < p.c ? kPiece : 0) : min(max(p.c - channel(q), 0), kPiece); };      // channels of a piece
+  const TS* x = static_cast<const TS*>(p.x) + ch;
+  const TC *u = static_cast<const TC*>(p.u) + ch, *gate = static_cast<const TC*>(p.gate) + ch, *gs = static_cast<const TC*>(p.gate_shift) + ch;
+  const bool has_x = p.x != nullptr, has_u = p.u != nullptr, gated = p.gate != nullptr, adaptive = p.gate_shift != nullptr;
+  const uint4* ring = ring_memory + threadIdx.x;
+  const uint32_t ring_at = ptx::smem_u32(ring);
+  int inside[P];                             // channels of a piece
+#pragma unroll
+  for (int q = 0; q < P; ++q) inside[q] = min(max(p.c - ch - q * kStep, 0), kPiece);
   auto vector = [&](const float* v, int q, float other) {
     float f[kPiece];
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) f[i] = v != nullptr && i < inside(q) ? v[channel(q) + i] : other;
+    for (int i = 0; i < kPiece; ++i) f[i] = v != nullptr && i < inside[q] ? v[ch + q * kStep + i] : other;
     return of_floats(f);
   };
 
@@ -50,6 +54,7 @@ __global__ void __launch_bounds__(kRowThreads) residual_norm_kernel(const Params
   for (int q = 0; q < P; ++q) {
     m[q] = vector(p.weight, q, 1.f);
     shift[q] = vector(p.bias, q, 0.f);
+    if (!OWN) open[OWN ? 0 : q] = both(1.f);
   }
 
   const unsigned step = gridDim.x * (kRowThreads / 32);
@@ -60,18 +65,16 @@ __global__ void __launch_bounds__(kRowThreads) residual_norm_kernel(const Params
   auto fetch = [&](int stage) {
     if (ahead.set < p.plan.sets) {
       const long long o = static_cast<long long>(ahead.row) * p.c;
-      uint4* s = ring + stage * p.slots * kRowThreads;
+      const uint32_t s = ring_at + stage * p.slots * kRowThreads * 16;
+      bool there[P];
 #pragma unroll
-      for (int q = 0; q < P; ++q) {
-        const int ch = channel(q);
-        const bool there = ahead.left > 0 && ch < p.c;
-        if (x != nullptr) ring_copy(s + q * kS * kRowThreads, x + o + ch, there);
-        if (u != nullptr) ring_copy(s + (p.s_u + q * kC) * kRowThreads, u + o + ch, there);
-        if (OWN && gate != nullptr) ring_copy(s + (p.s_gate + q * kC) * kRowThreads, gate + ahead.row * p.gate_ld + ch, there);
-        if (OWN && gs != nullptr) {
-          ring_copy(s + (p.s_g + q * kC) * kRowThreads, gs + ahead.row * p.gate_shift_ld + ch, there);
-          ring_copy(s + (p.s_g + (P + q) * kC) * kRowThreads, gs + ahead.row * p.gate_shift_ld + p.c + ch, there);
-        }
+      for (int q = 0; q < P; ++q) there[q] = ahead.left > 0 && inside[q] > 0;
+      if (has_x) ring_copy<TS, P, kStep>(s, x + o, there);
+      if (has_u) ring_copy<TC, P, kStep>(s + p.s_u * kRowThreads * 16, u + o, there);
+      if (OWN && gated) ring_copy<TC, P, kStep>(s + p.s_gate * kRowThreads * 16, gate + ahead.row * p.gate_ld, there);
+      if (OWN && adaptive) {
+        ring_copy<TC, P, kStep>(s + p.s_g * kRowThreads * 16, gs + ahead.row * p.gate_shift_ld, there);
+        ring_copy<TC, P, kStep>(s + (p.s_g + P * kC) * kRowThreads * 16, gs + ahead.row * p.gate_shift_ld + p.c, there);
       }
       ahead.next(p.plan, team, step);
     }
@@ -88,88 +91,121 @@ __global__ void __launch_bounds__(kRowThreads) residual_norm_kernel(const Params
       copy_async_wait<kDepth - 1>();
     }
     const uint4* s = ring + stage * p.slots * kRowThreads;
-    const long long o = static_cast<long long>(here.row) * p.c;
-    auto channels = [&](int q) { return here.left > 0 ? inside(q) : 0; };
-    auto take = [&](auto tag, int slot, const void* from, long long at, int q) {
+    const long long o = static_cast<long long>(here.row) * p.c + ch;
+    int k[P];                                // channels that are there
+#pragma unroll
+    for (int q = 0; q < P; ++q) k[q] = here.left > 0 ? inside[q] : 0;
+    // (from: this lane's first piece)
+    auto take = [&](auto tag, int slot, const auto* from, int q) {
       using E = decltype(tag);
       if constexpr (VEC) return ring_take<E>(s + (slot + q * (static_cast<int>(sizeof(E)) / 2)) * kRowThreads);
-      else return load_piece<E, VEC>(static_cast<const E*>(from) + at + channel(q), channels(q));
+      else return load_piece<E, VEC>(from + q * kStep, k[q]);
     };
     if (!OWN && here.at == 0) {
       const unsigned gate_row = here.gate_row(p.plan);
+      if (gated) {
 #pragma unroll
-      for (int q = 0; q < P; ++q) {
-        const int k = channels(q);
-        if (gate != nullptr) open[OWN ? 0 : q] = each(load_piece<TC, VEC>(gate + gate_row * p.gate_ld + channel(q), k), [](float a) { return open_of(exact_gate_at(a)); });
-        if (gs != nullptr) {
-          m[q] = each(load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + channel(q), k), [](float a) { return open_of(gate_at(a)); });
-          shift[q] = load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + p.c + channel(q), k);
+        for (int q = 0; q < P; ++q)
+          open[OWN ? 0 : q] = each(load_piece<TC, VEC>(gate + gate_row * p.gate_ld + q * kStep, k[q]), [](float a) { return open_of(exact_gate_at(a)); });
+      }
+      if (adaptive) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          m[q] = each(load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + q * kStep, k[q]), [](float a) { return open_of(gate_at(a)); });
+          shift[q] = load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + p.c + q * kStep, k[q]);
         }
       }
     }
+    // (a question that is the same for all pieces is asked once: the pieces' instructions then lie side by side)
     Pairs r[P];
-    uint64_t sum = 0;
+    if (has_x) {
 #pragma unroll
-    for (int q = 0; q < P; ++q) {
-      const int k = channels(q), ch = channel(q);
-      r[q] = x != nullptr ? take(TS{}, 0, x, o, q) : both(0.f);
-      if (p.scale != nullptr) r[q] = mul(r[q], vector(p.scale, q, 0.f));
-      if (u != nullptr) {
-        const Pairs t = take(TC{}, p.s_u, u, o, q);
-        if (gate == nullptr) r[q] = add(r[q], t);
-        else if constexpr (OWN) r[q] = fma(each(take(TC{}, p.s_gate, gate, here.row * p.gate_ld, q), [](float a) { return open_of(exact_gate_at(a)); }), t, r[q]);
-        else r[q] = fma(open[q], t, r[q]);
+      for (int q = 0; q < P; ++q) r[q] = take(TS{}, 0, x + (o - ch), q);
+      if (p.scale != nullptr) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) r[q] = mul(r[q], vector(p.scale, q, 0.f));
       }
-      uint32_t top;
-      if constexpr (std::is_same<TS, __nv_bfloat16>::value) {
-        const uint4 w = to_bf16(r[q]);
-        r[q] = of_bf16(w);                          // (as it is stored)
-        top = top_of(w);
-        if constexpr (VEC) {
-          if (p.r != nullptr && k > 0) *reinterpret_cast<uint4*>(static_cast<TS*>(p.r) + o + ch) = w;
-        }
+    } else {
+#pragma unroll
+      for (int q = 0; q < P; ++q) r[q] = both(0.f);
+    }
+    if (has_u) {
+      if (OWN && gated) {
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+          r[q] = fma(each(take(TC{}, p.s_gate, gate + here.row * p.gate_ld, q), [](float a) { return open_of(exact_gate_at(a)); }), take(TC{}, p.s_u, u + (o - ch), q), r[q]);
       } else {
-        top = p.kept != nullptr ? top_of(r[q]) : 0u;
-        if constexpr (VEC) {
-          if (p.r != nullptr) store_piece<VEC>(static_cast<TS*>(p.r) + o + ch, r[q], k);
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          const Pairs t = take(TC{}, p.s_u, u + (o - ch), q);
+          r[q] = OWN ? add(r[q], t) : fma(open[OWN ? 0 : q], t, r[q]);
         }
       }
-      if constexpr (!VEC) {
-        if (p.r != nullptr) store_piece<VEC>(static_cast<TS*>(p.r) + o + ch, r[q], k);
+    }
+    // as it is stored
+    TS* to = static_cast<TS*>(p.r) + o;
+    uint32_t top[P];
+    if constexpr (std::is_same<TS, __nv_bfloat16>::value) {
+      uint4 w[P];
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        w[q] = to_bf16(r[q]);
+        r[q] = of_bf16(w[q]);
+        top[q] = top_of(w[q]);
       }
-      if (p.kept != nullptr)
-        store_piece8<VEC>(p.kept + o + ch, p.kept_e + static_cast<long long>(here.row) * groups8(p.c) + ch / kGroup8, r[q], exponent8(group_top(top)), k,
-                          sub % (kGroup8 / kPiece) == 0);
-      sum_into(sum, r[q]);
+      if constexpr (VEC) {
+        if (p.r != nullptr) {
+#pragma unroll
+          for (int q = 0; q < P; ++q)
+            if (k[q] > 0) *reinterpret_cast<uint4*>(to + q * kStep) = w[q];
+        }
+      }
+    }
+    if (!(VEC && std::is_same<TS, __nv_bfloat16>::value) && p.r != nullptr) {
+#pragma unroll
+      for (int q = 0; q < P; ++q) store_piece<VEC>(to + q * kStep, r[q], k[q]);
+    }
+    if (p.kept != nullptr) {
+      uint8_t *bytes = p.kept + o, *e = p.kept_e + static_cast<long long>(here.row) * groups8(p.c) + ch / kGroup8;
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        if constexpr (!std::is_same<TS, __nv_bfloat16>::value) top[q] = top_of(r[q]);
+        store_piece8<VEC>(bytes + q * kStep, e + q * (kStep / kGroup8), r[q], exponent8(group_top(top[q])), k[q], ch % kGroup8 == 0);
+      }
     }
     if (p.norm != kNoNorm) {
+      Pairs sum = r[0];
+#pragma unroll
+      for (int q = 1; q < P; ++q) sum = add(sum, r[q]);
       float t[1] = {total(sum)};
       team_sum<LANES>(t);
-      const Pairs minus_mean = both(-t[0] * inv_c);
-      sum = 0;
+      const float mean = t[0] * inv_c;
+      sum = both(0.f);
 #pragma unroll
       for (int q = 0; q < P; ++q) {
-        r[q] = add(r[q], minus_mean);
+        r[q] = add(r[q], both(inside[q] > 0 ? -mean : 0.f));      // (nothing stays nothing)
         if constexpr (!VEC) {
 #pragma unroll
           for (int i = 0; i < kPiece; ++i)
-            if (i >= inside(q)) r[q].v[i / 2] = i & 1 ? ptx::pack2(r[q].get(i - 1), 0.f) : ptx::pack2(0.f, 0.f);
+            if (i >= inside[q]) r[q].v[i / 2] = i & 1 ? ptx::pack2(r[q].get(i - 1), 0.f) : ptx::pack2(0.f, 0.f);
         }
-        if (inside(q) > 0) dot_into(sum, r[q], r[q]);
+        sum = fma(r[q], r[q], sum);
       }
       t[0] = total(sum);
       team_sum<LANES>(t);
       const Pairs rstd = both(rsqrtf(fmaf(t[0], inv_c, p.eps)));
+      if (OWN && adaptive) {
 #pragma unroll
-      for (int q = 0; q < P; ++q) {
-        Pairs y = mul(r[q], rstd);
-        if (OWN && gs != nullptr)
-          y = fma(y, each(take(TC{}, p.s_g, gs, here.row * p.gate_shift_ld, q), [](float a) { return open_of(gate_at(a)); }),
-                  take(TC{}, p.s_g + P * kC, gs, here.row * p.gate_shift_ld + p.c, q));
-        else
-          y = fma(y, m[q], shift[q]);
-        store_piece<VEC>(static_cast<TC*>(p.y) + o + channel(q), y, channels(q));
+        for (int q = 0; q < P; ++q)
+          r[q] = fma(mul(r[q], rstd), each(take(TC{}, p.s_g, gs + here.row * p.gate_shift_ld, q), [](float a) { return open_of(gate_at(a)); }),
+                     take(TC{}, p.s_g + P * kC, gs + here.row * p.gate_shift_ld + p.c, q));
+      } else {
+#pragma unroll
+        for (int q = 0; q < P; ++q) r[q] = fma(mul(r[q], rstd), m[q], shift[q]);
       }
+      TC* y = static_cast<TC*>(p.y) + o;
+#pragma unroll
+      for (int q = 0; q < P; ++q) store_piece<VEC>(y + q * kStep, r[q], k[q]);
     }
     here.next(p.plan, team, step);
     stage = stage + 1 == kDepth ? 0 : stage + 1;

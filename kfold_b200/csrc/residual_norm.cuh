@@ -91,11 +91,24 @@ constexpr int ring_depth(int row_bytes) {      // of a thread and row
   const int d = kMostRing / 2 / kRowThreads / row_bytes;
   return d < 2 ? 2 : d > 4 ? 4 : d;
 }
-// Slot `s` of stage `q` of this thread: ring[(q * slots + s) * kRowThreads]; piece p of a tensor p * (16-byte words of a piece) slots on.
-template <typename T>
-__device__ __forceinline__ void ring_copy(uint4* slot, const T* from, bool there) {
+// Slot `s` of stage `q` of this thread: ring + ((q * slots + s) * kRowThreads + thread) * 16 bytes; piece p of a tensor p * (16-byte words of a piece) slots on.
+// `from`: this lane's first piece of a row, the others STEP elements apart; there: P flags, which pieces there are.
+template <typename T, int P, int STEP>
+__device__ __forceinline__ void ring_copy(uint32_t slot, const T* from, const bool (&there)[P]) {
+  constexpr int kWords = sizeof(T) / 2;
 #pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) copy_async16(slot + i * kRowThreads, reinterpret_cast<const uint4*>(from) + i, there);
+  for (int q = 0; q < P; ++q)
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) copy_async<16>(slot + (q * kWords + i) * kRowThreads * 16, reinterpret_cast<const uint4*>(from + q * STEP) + i, there[q]);
+}
+// Rows in 8 bits: the bytes, and where `words` says so the words of exponents that the pieces' lie in (`exponents`: a row's).
+template <int P, int STEP>
+__device__ __forceinline__ void ring_copy8(uint32_t slot, const uint8_t* from, const uint8_t* exponents, int channel, bool words, const bool (&there)[P]) {
+#pragma unroll
+  for (int q = 0; q < P; ++q) {
+    copy_async<8>(slot + q * kRowThreads * 16, from + q * STEP, there[q]);
+    if (words) copy_async<4>(slot + q * kRowThreads * 16 + 8, exponents + ((channel + q * STEP) / kGroup8 & ~3), there[q]);
+  }
 }
 template <typename T>
 __device__ __forceinline__ Pairs ring_take(const uint4* slot) {

@@ -39,20 +39,23 @@ constexpr int depth() { return ring_depth(P * 8 * (2 * sizeof(TS) + (OWN ? 4 : 2
 template <typename TS, typename TC, int LANES, int P, bool VEC, bool OWN>
 __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : 2) residual_norm_grad_kernel(const GradParams p) {
   constexpr int kDepth = depth<TS, TC, P, OWN>(), kC = sizeof(TC) / 2;
+  constexpr int kStep = LANES * kPiece;      // channels from a lane's piece to its next
   extern __shared__ uint4 ring_memory[];
   grid_dependency_enter();
-  const int warp = threadIdx.x / 32, sub = threadIdx.x % LANES, team = threadIdx.x % 32 / LANES, groups = groups8(p.c);
+  const int warp = threadIdx.x / 32, ch = threadIdx.x % LANES * kPiece, team = threadIdx.x % 32 / LANES, groups = groups8(p.c);
   const float inv_c = 1.0f / static_cast<float>(p.c);
-  const TC *gate = static_cast<const TC*>(p.gate), *gs = static_cast<const TC*>(p.gate_shift);
-  const bool adaptive = p.norm == kAdaptiveNorm;
-  uint4* ring = ring_memory + threadIdx.x;
+  const TC *gate = static_cast<const TC*>(p.gate) + ch, *gs = static_cast<const TC*>(p.gate_shift) + ch;
+  const bool gated = p.gate != nullptr, adaptive = p.norm == kAdaptiveNorm;
+  const uint4* ring = ring_memory + threadIdx.x;
+  const uint32_t ring_at = ptx::smem_u32(ring);
   float* scale_sums = reinterpret_cast<float*>(ring_memory + p.s_scale * kRowThreads) + threadIdx.x;      // [P * 8][thread]
-  auto channel = [&](int q) { return (q * LANES + sub) * kPiece; };
-  auto inside = [&](int q) { return VEC ? (channel(q) < p.c ? kPiece : 0) : min(max(p.c - channel(q), 0), kPiece); };      // channels of a piece
+  int inside[P];                             // channels of a piece
+#pragma unroll
+  for (int q = 0; q < P; ++q) inside[q] = min(max(p.c - ch - q * kStep, 0), kPiece);
   auto vector = [&](const float* v, int q, float other) {
     float f[kPiece];
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) f[i] = v != nullptr && i < inside(q) ? v[channel(q) + i] : other;
+    for (int i = 0; i < kPiece; ++i) f[i] = v != nullptr && i < inside[q] ? v[ch + q * kStep + i] : other;
     return of_floats(f);
   };
 
@@ -76,35 +79,26 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : 2) residual_norm_gra
   ahead = here;
   auto fetch = [&](int stage) {
     if (ahead.set < p.plan.sets) {
-      uint4* s = ring + stage * p.slots * kRowThreads;
-      const long long o = static_cast<long long>(ahead.row) * p.c;
+      const uint32_t s = ring_at + stage * p.slots * kRowThreads * 16;
+      const long long o = static_cast<long long>(ahead.row) * p.c + ch, e = static_cast<long long>(ahead.row) * groups;
+      bool there[P];
 #pragma unroll
-      for (int q = 0; q < P; ++q) {
-        const int ch = channel(q);
-        const bool there = ahead.left > 0 && ch < p.c;
-        // a tensor, or its rows in 8 bits: the bytes, and the word of exponents that a piece's lies in
-        auto copy = [&](auto tag, int slot, const void* t, const uint8_t* e) {
-          using E = decltype(tag);
-          if (e == nullptr) {
-            ring_copy(s + (slot + q * (static_cast<int>(sizeof(E)) / 2)) * kRowThreads, static_cast<const E*>(t) + o + ch, there);
-          } else {
-            uint4* to = s + (slot + q) * kRowThreads;
-            copy_async<8>(to, static_cast<const uint8_t*>(t) + o + ch, there);
-            if (p.words) copy_async<4>(reinterpret_cast<uint32_t*>(to) + 2, e + static_cast<long long>(ahead.row) * groups + (ch / kGroup8 & ~3), there);
-          }
-        };
-        if (p.dr != nullptr) copy(TS{}, 0, p.dr, nullptr);
-        if (p.norm != kNoNorm) {
-          copy(TC{}, p.s_dy, p.dy, nullptr);
-          copy(TS{}, p.s_r, p.r, p.r_e);
-        }
-        if (p.dgate != nullptr) copy(TC{}, p.s_u, p.u, p.u_e);
-        if (p.x != nullptr) copy(TS{}, p.s_x, p.x, p.x_e);
-        if (OWN) {
-          if (gate != nullptr) ring_copy(s + (p.s_gate + q * kC) * kRowThreads, gate + ahead.row * p.gate_ld + ch, there);
-          if (gs != nullptr) ring_copy(s + (p.s_g + q * kC) * kRowThreads, gs + ahead.row * p.gate_shift_ld + ch, there);
-        }
+      for (int q = 0; q < P; ++q) there[q] = ahead.left > 0 && inside[q] > 0;
+      auto copy = [&](auto tag, int slot, const void* t, const uint8_t* exponents) {
+        using E = decltype(tag);
+        const uint32_t to = s + slot * kRowThreads * 16;
+        if (exponents == nullptr) ring_copy<E, P, kStep>(to, static_cast<const E*>(t) + o, there);
+        else ring_copy8<P, kStep>(to, static_cast<const uint8_t*>(t) + o, exponents + e, ch, p.words, there);
+      };
+      if (p.dr != nullptr) copy(TS{}, 0, p.dr, nullptr);
+      if (p.norm != kNoNorm) {
+        copy(TC{}, p.s_dy, p.dy, nullptr);
+        copy(TS{}, p.s_r, p.r, p.r_e);
       }
+      if (p.dgate != nullptr) copy(TC{}, p.s_u, p.u, p.u_e);
+      if (p.x != nullptr) copy(TS{}, p.s_x, p.x, p.x_e);
+      if (OWN && gated) ring_copy<TC, P, kStep>(s + p.s_gate * kRowThreads * 16, gate + ahead.row * p.gate_ld, there);
+      if (OWN && adaptive) ring_copy<TC, P, kStep>(s + p.s_g * kRowThreads * 16, gs + ahead.row * p.gate_shift_ld, there);
       ahead.next(p.plan, team, step);
     }
     copy_async_done();
@@ -121,149 +115,200 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : 2) residual_norm_gra
     }
     const bool row_there = here.left > 0;
     const uint4* s = ring + stage * p.slots * kRowThreads;
-    const long long o = static_cast<long long>(here.row) * p.c;
-    auto channels = [&](int q) { return row_there ? inside(q) : 0; };
-    auto take = [&](auto tag, int slot, const void* t, const uint8_t* e, int q) {
+    const long long o = static_cast<long long>(here.row) * p.c + ch, e = static_cast<long long>(here.row) * groups;
+    int k[P];                                // channels that are there
+#pragma unroll
+    for (int q = 0; q < P; ++q) k[q] = row_there ? inside[q] : 0;
+    // All pieces of a tensor, or of its rows in 8 bits.  (A question that is the same for all pieces is asked once: the pieces' instructions then lie side by side.)
+    auto take = [&](auto tag, int slot, const void* t, const uint8_t* exponents, Pairs (&v)[P]) {
       using E = decltype(tag);
-      if (e == nullptr) {
-        if constexpr (VEC) return ring_take<E>(s + (slot + q * (static_cast<int>(sizeof(E)) / 2)) * kRowThreads);
-        else return load_piece<E, VEC>(static_cast<const E*>(t) + o + channel(q), channels(q));
-      }
-      const uint8_t* ep = e + static_cast<long long>(here.row) * groups + channel(q) / kGroup8;
-      if constexpr (VEC) {
-        const uint4 w = s[(slot + q) * kRowThreads];
-        const uint32_t ex = p.words ? w.z >> channel(q) / kGroup8 % 4 * 8 & 255u : channels(q) > 0 ? *ep : 0u;
-        return values8(make_uint2(w.x, w.y), ex);
+      if (exponents == nullptr) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          if constexpr (VEC) v[q] = ring_take<E>(s + (slot + q * (static_cast<int>(sizeof(E)) / 2)) * kRowThreads);
+          else v[q] = load_piece<E, VEC>(static_cast<const E*>(t) + o + q * kStep, k[q]);
+        }
+      } else if (VEC && p.words) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          const uint4 w = s[(slot + q) * kRowThreads];
+          v[q] = values8(make_uint2(w.x, w.y), w.z >> (ch + q * kStep) / kGroup8 % 4 * 8 & 255u);
+        }
       } else {
-        return load_piece8<VEC>(static_cast<const uint8_t*>(t) + o + channel(q), ep, channels(q));
+#pragma unroll
+        for (int q = 0; q < P; ++q) v[q] = load_piece8<VEC>(static_cast<const uint8_t*>(t) + o + q * kStep, exponents + e + (ch + q * kStep) / kGroup8, k[q]);
       }
     };
     // gates (gate_at) of this row's output, or of its norm
-    auto own_gates = [&](const TC* table, long long ld, int slot, int q) {
+    auto own_gates = [&](const TC* row, int slot, int q) {
       Pairs t;
       if constexpr (VEC) t = ring_take<TC>(s + (slot + q * kC) * kRowThreads);
-      else t = load_piece<TC, VEC>(table + here.row * ld + channel(q), channels(q));
+      else t = load_piece<TC, VEC>(row + q * kStep, k[q]);
       return each(t, [](float a) { return gate_at(a); });
     };
     if (!OWN && here.at == 0) {
       const unsigned gate_row = here.gate_row(p.plan);
+      auto opened = [](float a) { return open_of(gate_at(a)); };
+      if (gated) {
 #pragma unroll
-      for (int q = 0; q < P; ++q) {
-        const int k = channels(q);
-        if (gate != nullptr) open[OWN ? 0 : q] = each(load_piece<TC, VEC>(gate + gate_row * p.gate_ld + channel(q), k), [](float a) { return open_of(gate_at(a)); });
-        if (gs != nullptr) m[q] = each(load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + channel(q), k), [](float a) { return open_of(gate_at(a)); });
+        for (int q = 0; q < P; ++q) open[OWN ? 0 : q] = each(load_piece<TC, VEC>(gate + gate_row * p.gate_ld + q * kStep, k[q]), opened);
+      }
+      if (adaptive) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) m[q] = each(load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + q * kStep, k[q]), opened);
       }
     }
-    Pairs z[P], g[P], rstd2, minus_mean_g, minus_mean_gz;
+    Pairs t[P];
     if (p.norm != kNoNorm) {
-      uint64_t sz = 0, sg = 0;
+      Pairs z[P], g[P], d[P];
+      take(TS{}, p.s_r, p.r, p.r_e, z);
+      take(TC{}, p.s_dy, p.dy, nullptr, d);
+      if (OWN && adaptive) {
 #pragma unroll
-      for (int q = 0; q < P; ++q) {
-        z[q] = take(TS{}, p.s_r, p.r, p.r_e, q);
-        const Pairs d = take(TC{}, p.s_dy, p.dy, nullptr, q);
-        if (OWN && gs != nullptr) {
-          m[q] = own_gates(gs, p.gate_shift_ld, p.s_g, q);
-          g[q] = mul(d, each(m[q], [](float a) { return open_of(a); }));
-        } else {
-          g[q] = mul(d, m[q]);
+        for (int q = 0; q < P; ++q) {
+          m[q] = own_gates(gs + here.row * p.gate_shift_ld, p.s_g, q);
+          g[q] = mul(d[q], each(m[q], [](float a) { return open_of(a); }));
         }
-        sum_into(sz, z[q]);
-        sum_into(sg, g[q]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < P; ++q) g[q] = mul(d[q], m[q]);
       }
-      float t[2] = {total(sz), total(sg)};
-      team_sum<LANES>(t);
-      const Pairs minus_mean = both(-t[0] * inv_c);
-      minus_mean_g = both(-t[1] * inv_c);
-      sz = sg = 0;
+      Pairs sz = z[0], sg = g[0];
+#pragma unroll
+      for (int q = 1; q < P; ++q) {
+        sz = add(sz, z[q]);
+        sg = add(sg, g[q]);
+      }
+      float sums[2] = {total(sz), total(sg)};
+      team_sum<LANES>(sums);
+      const float mean = sums[0] * inv_c;
+      const Pairs minus_mean_g = both(-sums[1] * inv_c);
+      sz = sg = both(0.f);
 #pragma unroll
       for (int q = 0; q < P; ++q) {
-        z[q] = add(z[q], minus_mean);
+        z[q] = add(z[q], both(inside[q] > 0 ? -mean : 0.f));      // (nothing stays nothing)
         if constexpr (!VEC) {
 #pragma unroll
           for (int i = 0; i < kPiece; ++i)
-            if (i >= inside(q)) z[q].v[i / 2] = i & 1 ? ptx::pack2(z[q].get(i - 1), 0.f) : ptx::pack2(0.f, 0.f);
+            if (i >= inside[q]) z[q].v[i / 2] = i & 1 ? ptx::pack2(z[q].get(i - 1), 0.f) : ptx::pack2(0.f, 0.f);
         }
-        if (inside(q) > 0) dot_into(sz, z[q], z[q]);
-        dot_into(sg, g[q], z[q]);
+        sz = fma(z[q], z[q], sz);
+        sg = fma(g[q], z[q], sg);
       }
-      t[0] = total(sz);
-      t[1] = total(sg);
-      team_sum<LANES>(t);
-      const float rstd = rsqrtf(fmaf(t[0], inv_c, p.eps));
-      rstd2 = both(rstd);
-      minus_mean_gz = both(-t[1] * inv_c * rstd);
-    }
+      sums[0] = total(sz);
+      sums[1] = total(sg);
+      team_sum<LANES>(sums);
+      const float rstd = row_there ? rsqrtf(fmaf(sums[0], inv_c, p.eps)) : 0.f;      // (no row: no number where eps is zero)
+      const Pairs rstd2 = both(rstd), minus_mean_gz = both(-sums[1] * inv_c * rstd);
 #pragma unroll
-    for (int q = 0; q < P; ++q) {
-      const int k = channels(q), ch = channel(q);
-      Pairs t = p.dr != nullptr ? take(TS{}, 0, p.dr, nullptr, q) : both(0.f);
-      if (p.norm != kNoNorm) {
+      for (int q = 0; q < P; ++q) {
         z[q] = mul(z[q], rstd2);
-        t = fma(rstd2, fma(z[q], minus_mean_gz, add(g[q], minus_mean_g)), t);
-        const Pairs d = take(TC{}, p.s_dy, p.dy, nullptr, q);
-        if (OWN && adaptive) {
-          if (p.dgate_shift != nullptr) {
-            TC* to = static_cast<TC*>(p.dgate_shift) + static_cast<long long>(here.row) * 2 * p.c + ch;
-            store_piece<VEC>(to, mul(mul(d, z[q]), each(m[q], [](float a) { return slope_of(a); })), k);
-            store_piece<VEC>(to + p.c, d, k);
+        t[q] = mul(rstd2, fma(z[q], minus_mean_gz, add(g[q], minus_mean_g)));
+      }
+      if constexpr (VEC && P > 1) take(TC{}, p.s_dy, p.dy, nullptr, d);               // (read again: it frees the registers meanwhile)
+      if (OWN && adaptive) {
+        if (p.dgate_shift != nullptr) {
+          TC* to = static_cast<TC*>(p.dgate_shift) + 2 * (o - ch) + ch;
+#pragma unroll
+          for (int q = 0; q < P; ++q) {
+            store_piece<VEC>(to + q * kStep, mul(mul(d[q], z[q]), each(m[q], [](float a) { return slope_of(a); })), k[q]);
+            store_piece<VEC>(to + p.c + q * kStep, d[q], k[q]);
           }
-        } else if (row_there) {                     // (z of no row is not a number where eps is zero)
-          a0[q] = fma(d, z[q], a0[q]);
-          a1[q] = add(a1[q], d);
         }
-      }
-      Pairs u, own;
-      if (p.dgate != nullptr) u = take(TC{}, p.s_u, p.u, p.u_e, q);
-      if constexpr (OWN) {
-        if (gate != nullptr) own = own_gates(gate, p.gate_ld, p.s_gate, q);
-        if (p.dgate != nullptr) store_piece<VEC>(static_cast<TC*>(p.dgate) + o + ch, mul(mul(t, u), each(own, [](float a) { return slope_of(a); })), k);
       } else {
-        if (p.dgate != nullptr && row_there) a2[OWN ? 0 : q] = fma(t, u, a2[OWN ? 0 : q]);
-      }
-      if (p.du != nullptr) {
-        Pairs v = t;
-        if (gate != nullptr) {
-          if constexpr (OWN) v = mul(t, each(own, [](float a) { return open_of(a); }));
-          else v = mul(t, open[OWN ? 0 : q]);
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          a0[q] = fma(d[q], z[q], a0[q]);
+          a1[q] = add(a1[q], d[q]);
         }
-        store_piece<VEC>(static_cast<TC*>(p.du) + o + ch, v, k);
       }
-      if (p.x != nullptr && row_there) {
-        const Pairs v = mul(t, take(TS{}, p.s_x, p.x, p.x_e, q));
+      if (p.dr != nullptr) {
+        take(TS{}, 0, p.dr, nullptr, z);
+#pragma unroll
+        for (int q = 0; q < P; ++q) t[q] = add(t[q], z[q]);
+      }
+    } else {
+      take(TS{}, 0, p.dr, nullptr, t);
+    }
+    if (p.dgate != nullptr) {
+      Pairs u[P];
+      take(TC{}, p.s_u, p.u, p.u_e, u);
+      if constexpr (OWN) {
+        TC* to = static_cast<TC*>(p.dgate) + o;
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          const Pairs own = own_gates(gate + here.row * p.gate_ld, p.s_gate, q);
+          store_piece<VEC>(to + q * kStep, mul(mul(t[q], u[q]), each(own, [](float a) { return slope_of(a); })), k[q]);
+          if (p.du != nullptr) store_piece<VEC>(static_cast<TC*>(p.du) + o + q * kStep, mul(t[q], each(own, [](float a) { return open_of(a); })), k[q]);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < P; ++q) a2[OWN ? 0 : q] = fma(t[q], u[q], a2[OWN ? 0 : q]);
+      }
+    }
+    if (p.du != nullptr && !(OWN && p.dgate != nullptr)) {
+      TC* to = static_cast<TC*>(p.du) + o;
+      if (OWN && gated) {
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+          store_piece<VEC>(to + q * kStep, mul(t[q], each(own_gates(gate + here.row * p.gate_ld, p.s_gate, q), [](float a) { return open_of(a); })), k[q]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < P; ++q) store_piece<VEC>(to + q * kStep, OWN ? t[q] : mul(t[q], open[OWN ? 0 : q]), k[q]);
+      }
+    }
+    if (p.x != nullptr) {
+      Pairs x[P];
+      take(TS{}, p.s_x, p.x, p.x_e, x);
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        const Pairs v = mul(t[q], x[q]);
 #pragma unroll
         for (int i = 0; i < kPiece; ++i) scale_sums[(q * kPiece + i) * kRowThreads] += v.get(i);
       }
-      if (p.dx != nullptr) {
-        if (p.scale != nullptr) t = mul(t, vector(p.scale, q, 0.f));
-        store_piece<VEC>(static_cast<TS*>(p.dx) + o + ch, t, k);
+    }
+    if (p.dx != nullptr) {
+      if (p.scale != nullptr) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) t[q] = mul(t[q], vector(p.scale, q, 0.f));
       }
+      TS* to = static_cast<TS*>(p.dx) + o;
+#pragma unroll
+      for (int q = 0; q < P; ++q) store_piece<VEC>(to + q * kStep, t[q], k[q]);
     }
     if constexpr (!OWN) {
       if (here.at + 1 == p.plan.chunk) {
         // the end of a piece: the gates' gradients from the sums over their samples, the logits once more for their slopes; or the sums for the second kernel
         const bool there = here.unit < p.plan.units;
         const unsigned gate_row = here.gate_row(p.plan);
+        auto slope = [](float a) { return slope_of(gate_at(a)); };
+#pragma unroll 1
+        for (int which = 0; which < 2; ++which) {
+          // the norm's gates and shifts, the output gate
+          if (which == 0 ? !adaptive : p.dgate == nullptr) continue;
+#pragma unroll
+          for (int q = 0; q < P; ++q) {
+            const int n = there ? inside[q] : 0;
+            if (p.pieces != nullptr) {
+              float* d = p.pieces + static_cast<long long>(there ? here.unit : 0) * 3 * p.c + ch + q * kStep;
+              if (which == 0) {
+                store_piece<VEC>(d, a0[q], n);
+                store_piece<VEC>(d + p.c, a1[q], n);
+              } else {
+                store_piece<VEC>(d + 2 * p.c, a2[OWN ? 0 : q], n);
+              }
+            } else if (which == 1) {
+              store_piece<VEC>(static_cast<TC*>(p.dgate) + static_cast<long long>(gate_row) * p.c + ch + q * kStep,
+                               mul(a2[OWN ? 0 : q], each(load_piece<TC, VEC>(gate + gate_row * p.gate_ld + q * kStep, n), slope)), n);
+            } else if (p.dgate_shift != nullptr) {
+              TC* d = static_cast<TC*>(p.dgate_shift) + static_cast<long long>(gate_row) * 2 * p.c + ch + q * kStep;
+              store_piece<VEC>(d, mul(a0[q], each(load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + q * kStep, n), slope)), n);
+              store_piece<VEC>(d + p.c, a1[q], n);
+            }
+          }
+        }
 #pragma unroll
         for (int q = 0; q < P; ++q) {
-          const int k = there ? inside(q) : 0, ch = channel(q);
-          const long long to = static_cast<long long>(gate_row) * p.c + ch;
-          if (p.pieces != nullptr) {
-            float* d = p.pieces + static_cast<long long>(there ? here.unit : 0) * 3 * p.c + ch;
-            if (adaptive) {
-              store_piece<VEC>(d, a0[q], k);
-              store_piece<VEC>(d + p.c, a1[q], k);
-            }
-            if (p.dgate != nullptr) store_piece<VEC>(d + 2 * p.c, a2[OWN ? 0 : q], k);
-          } else {
-            auto slope = [](float a) { return slope_of(gate_at(a)); };
-            if (adaptive && p.dgate_shift != nullptr) {
-              TC* d = static_cast<TC*>(p.dgate_shift) + 2 * to - ch;
-              store_piece<VEC>(d, mul(a0[q], each(load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + ch, k), slope)), k);
-              store_piece<VEC>(d + p.c, a1[q], k);
-            }
-            if (p.dgate != nullptr)
-              store_piece<VEC>(static_cast<TC*>(p.dgate) + to, mul(a2[OWN ? 0 : q], each(load_piece<TC, VEC>(gate + gate_row * p.gate_ld + ch, k), slope)), k);
-          }
           a2[OWN ? 0 : q] = both(0.f);
           if (adaptive) a0[q] = a1[q] = both(0.f);
         }
@@ -286,7 +331,7 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : 2) residual_norm_gra
       for (int q = 0; q < P; ++q)
 #pragma unroll
         for (int i = 0; i < kPiece; ++i)
-          flat[static_cast<int>(threadIdx.x) / LANES * kWidth + channel(q) + i] = j == 0 ? a0[q].get(i) : j == 1 ? a1[q].get(i) : scale_sums[(q * kPiece + i) * kRowThreads];
+          flat[static_cast<int>(threadIdx.x) / LANES * kWidth + ch + q * kStep + i] = j == 0 ? a0[q].get(i) : j == 1 ? a1[q].get(i) : scale_sums[(q * kPiece + i) * kRowThreads];
       __syncthreads();
       for (int i = threadIdx.x; i < p.c; i += kRowThreads) {
         float t = 0.f;

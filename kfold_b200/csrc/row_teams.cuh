@@ -79,17 +79,9 @@ __device__ __forceinline__ Pairs fma(const Pairs& a, const Pairs& b, const Pairs
   for (int i = 0; i < 4; ++i) r.v[i] = ptx::fma2(a.v[i], b.v[i], c.v[i]);
   return r;
 }
-// v plus the sum of a's elements, or of a's by b's, kept in pairs
-__device__ __forceinline__ void sum_into(uint64_t& v, const Pairs& a) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v = ptx::add2(v, a.v[i]);
-}
-__device__ __forceinline__ void dot_into(uint64_t& v, const Pairs& a, const Pairs& b) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v = ptx::fma2(a.v[i], b.v[i], v);
-}
-__device__ __forceinline__ float total(uint64_t v) {
-  const float2 f = ptx::unpack2(v);
+// The sum of the elements: of pairs that were added up side by side, so that no addition waits for the one before it.
+__device__ __forceinline__ float total(const Pairs& a) {
+  const float2 f = ptx::unpack2(ptx::add2(ptx::add2(a.v[0], a.v[1]), ptx::add2(a.v[2], a.v[3])));
   return f.x + f.y;
 }
 template <typename F>
@@ -219,14 +211,11 @@ __device__ __forceinline__ void store_piece8(uint8_t* p, uint8_t* e, const Pairs
 }
 
 // ---- copies of 16, 8 or 4 bytes into shared memory that arrive while the thread goes on; zeros where `there` is false
-__device__ __forceinline__ void copy_async16(void* to, const void* from, bool there) {
-  const int n = there ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(to)), "l"(from), "r"(n) : "memory");
-}
 template <int BYTES>
-__device__ __forceinline__ void copy_async(void* to, const void* from, bool there) {
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, bool there) {
   const int n = there ? BYTES : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(ptx::smem_u32(to)), "l"(from), "n"(BYTES), "r"(n) : "memory");
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(n) : "memory");
 }
 __device__ __forceinline__ void copy_async_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LATER>

@@ -720,10 +720,10 @@ KFB_API int kfb_expand(const void* values, const void* exponents, void* x, long 
  *   activation f : 0 none, 1 sigmoid, 2 silu, 3 gelu (with the error function), 4 relu.
  *   residual, out : (rows, n) of out_dtype (KFB_BF16, or KFB_FP32: always with KFB_FP32_PRECISE);  dy : of dy_dtype likewise.
  *   dw : (n, k) of dw_dtype, dbias : fp32; dx : (rows, k) as x.  Gradients that are NULL are not computed.
- * k, n multiples of 8 up to 65536, tensors on 16-byte boundaries.  Workspace: `wanted` 0 for the forward pass (dy_dtype is not looked
- * at), else the sum of 1 (dx), 2 (dw), 4 (dbias).
+ * k, n multiples of 8 up to 65536, tensors on 16-byte boundaries.  Workspace: `wanted` 0 for the forward pass, else the sum of 1 (dx),
+ * 2 (dw), 4 (dbias); out_dtype: the result's, or dy's; it may be none.  Another device may need another size.
  */
-KFB_API size_t kfb_fused_linear_workspace_bytes(long long rows, int k, int n, int activation, int dtype, int dy_dtype, int wanted);
+KFB_API size_t kfb_fused_linear_workspace_bytes(long long rows, int k, int n, int activation, int dtype, int out_dtype, int wanted);
 KFB_API int kfb_fused_linear_fwd(const void* x, const void* w, const float* bias, const void* residual, void* out, void* workspace,
                                  size_t workspace_bytes, long long rows, int k, int n, int activation, int dtype, int out_dtype, void* stream);
 KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, const float* bias, void* dx, void* dw, float* dbias, void* workspace,

@@ -116,22 +116,22 @@ __global__ void __launch_bounds__(32 * kTailWarps) linear_tail_kernel(const Tail
   }
 }
 
-// out[c] (+)= sum over blocks of partial[b][c], in the order of the blocks.
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* partial, float* out, int blocks, int n, int add) {
-  __shared__ float s[8][33];
+// out[c] (+)= sum over rows of partial[row][c], in an order of their number alone.
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* partial, float* out, int rows, int n, int add) {
+  __shared__ float s[32][33];
   grid_dependency_enter();
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
   float t = 0.f;
   if (col < n) {
-#pragma unroll 4
-    for (int b = part; b < blocks; b += 8) t += partial[static_cast<long long>(b) * n + col];
+#pragma unroll 8
+    for (int b = part; b < rows; b += 32) t += partial[static_cast<long long>(b) * n + col];
   }
   s[part][lane] = t;
   __syncthreads();
   if (part == 0 && col < n) {
     t = add ? out[col] : 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) t += s[k][lane];
+    for (int k = 0; k < 32; ++k) t += s[k][lane];
     out[col] = t;
   }
 }
@@ -156,9 +156,22 @@ int launch_tail(cudaStream_t stream, TailParams p, int act, int* row_blocks) {
 
 bool widths_ok(int k, int n) { return k > 0 && k % 8 == 0 && n > 0 && n % 8 == 0 && k <= 65536 && n <= 65536; }
 
+// Which kernels a call takes: many bf16 rows those for CTA pairs, which keep nothing but dz; others products into float32 and the tail by itself.
+struct Ways {
+  bool z, dx, dw;          // the products with what follows them, those for dx, those for dW
+};
+Ways ways(long long rows, int k, int n, int act, int precise, int wide, int wanted) {
+  Ways w = {};
+  if (precise) return w;
+  w.z = !wide && (wanted == 0 || act != kIdentity) && linear_pair_ok(rows, n, k);
+  w.dx = (wanted & 1) && linear_pair_ok(rows, k, n);
+  w.dw = (wanted & 2) && linear_weights_ok(n, k);
+  return w;
+}
+
 // Rows of a piece: as many as keep what a row needs below half a gigabyte.
-long long piece_rows(long long rows, int k, int n, int precise) {
-  const long long per_row = 6ll * n + (precise ? 6ll * (k + n) : 0), most = ((1ll << 29) / per_row + 127) / 128 * 128;
+long long piece_rows(long long rows, int k, int n, int precise, bool z) {
+  const long long per_row = 2ll * n + (z ? 4ll * n : 0) + (precise ? 6ll * (k + n) : 0), most = ((1ll << 29) / per_row + 127) / 128 * 128;
   return rows < most ? rows : most;
 }
 
@@ -172,24 +185,35 @@ int blocks_per_plane(long long piece, int k, int n) {
 int weight_splits(long long rows, int per) { return static_cast<int>(((rows + 63) / 64 + per - 1) / per); }
 
 struct Room {
+  Ways way;
+  long long piece;
+  int per_plane, splits;
   float* z;
   __nv_bfloat16 *dz, *x3, *w3;
   float *planes, *partial;
   size_t bytes;
 };
 
-// wanted: 0 forward, else a sum of 1 dx, 2 dW, 4 db; round: dy is wider than an operand
-Room carve(void* base, long long rows, int k, int n, int act, int precise, int round, int wanted) {
+// wanted: 0 forward, else a sum of 1 dx, 2 dW, 4 db; wide: the result or its gradient is float32 beside bf16
+Room carve(void* base, long long rows, int k, int n, int act, int precise, int wide, int wanted) {
   Carver c(base);
   Room r = {};
-  const long long piece = piece_rows(rows, k, n, precise);
-  const bool z = wanted == 0 || act != kIdentity;
-  if (z) r.z = c.take<float>(piece * n);
-  if ((wanted & 3) != 0 && (precise || round || act != kIdentity)) r.dz = c.take<__nv_bfloat16>(piece * n * (precise ? 3 : 1));
-  if (precise && (z || (wanted & 2))) r.x3 = c.take<__nv_bfloat16>(piece * k * 3);
+  r.way = ways(rows, k, n, act, precise, wide, wanted);
+  const bool z = (wanted == 0 || act != kIdentity) && !r.way.z;
+  r.piece = wanted == 0 && r.way.z ? rows : piece_rows(rows, k, n, precise, z);
+  if (z) r.z = c.take<float>(r.piece * n);
+  if (wanted != 0 && (r.way.z || ((wanted & 3) != 0 && (precise || wide || act != kIdentity)))) r.dz = c.take<__nv_bfloat16>(r.piece * n * (precise ? 3 : 1));
+  if (precise && (z || (wanted & 2))) r.x3 = c.take<__nv_bfloat16>(r.piece * k * 3);
   if (precise && (z || (wanted & 1))) r.w3 = c.take<__nv_bfloat16>(3ll * n * k);
-  if (wanted & 2) r.planes = c.take<float>(static_cast<size_t>(weight_splits(piece, blocks_per_plane(piece, k, n))) * n * k);
-  if (wanted & 4) r.partial = c.take<float>(static_cast<size_t>(kMostRowBlocks) * n);
+  if (wanted & 2) {
+    r.per_plane = blocks_per_plane(r.piece, k, n);
+    r.splits = r.way.dw ? linear_weights_splits(r.piece, n, k) : weight_splits(r.piece, r.per_plane);
+    r.planes = c.take<float>(static_cast<size_t>(r.splits) * n * k);
+  }
+  if (wanted & 4) {
+    const int pairs = r.way.z ? linear_pair_partials(r.piece, n, k) : 0;
+    r.partial = c.take<float>(static_cast<size_t>(pairs > kMostRowBlocks ? pairs : kMostRowBlocks) * n);
+  }
   r.bytes = c.off;
   return r;
 }
@@ -211,10 +235,10 @@ using namespace kfb;
 
 extern "C" {
 
-KFB_API size_t kfb_fused_linear_workspace_bytes(long long rows, int k, int n, int activation, int dtype, int dy_dtype, int wanted) {
+KFB_API size_t kfb_fused_linear_workspace_bytes(long long rows, int k, int n, int activation, int dtype, int out_dtype, int wanted) {
   if (rows <= 0 || rows >= (1ll << 31) || !widths_ok(k, n)) return 0;
   const int precise = dtype == KFB_FP32_PRECISE;
-  return carve(nullptr, rows, k, n, activation, precise, dy_dtype != KFB_BF16, wanted).bytes;
+  return carve(nullptr, rows, k, n, activation, precise, !precise && out_dtype != KFB_BF16, wanted).bytes;
 }
 
 KFB_API int kfb_fused_linear_fwd(const void* x, const void* w, const float* bias, const void* residual, void* out, void* workspace,
@@ -225,11 +249,15 @@ KFB_API int kfb_fused_linear_fwd(const void* x, const void* w, const float* bias
   const int precise = dtype == KFB_FP32_PRECISE;
   KFB_CHECK_ARG(x != nullptr && w != nullptr && out != nullptr, "fused_linear: null tensor");
   KFB_CHECK_ARG(!off16(x) && !off16(w) && !off16(out) && !off16(residual), "fused_linear: tensors start on 16-byte boundaries");
-  const Room m = carve(workspace, rows, k, n, activation, precise, 0, 0);
+  const Room m = carve(workspace, rows, k, n, activation, precise, !precise && out_dtype != KFB_BF16, 0);
+  cudaStream_t s = as_stream(stream);
+  if (m.way.z) {
+    const LinearPair p = {kForwardTail, x, w, 0, bias, activation, residual, out, nullptr, rows, n, k};
+    return launch_linear_pair(s, p, "fused_linear");
+  }
   KFB_CHECK_ARG(workspace != nullptr && workspace_bytes >= m.bytes, "fused_linear: workspace %zu < %zu bytes", workspace_bytes, m.bytes);
   KFB_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "fused_linear: workspace must be 256-byte aligned");
-  cudaStream_t s = as_stream(stream);
-  const long long piece = piece_rows(rows, k, n, precise);
+  const long long piece = m.piece;
   const size_t out_size = out_dtype == KFB_FP32 ? 4 : 2;
   if (precise) KFB_TRY(launch_split_planes(s, static_cast<const float*>(w), m.w3, static_cast<long long>(n) * k, static_cast<long long>(n) * k));
   for (long long r0 = 0; r0 < rows; r0 += piece) {
@@ -280,14 +308,13 @@ KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, c
   const bool f = activation != kIdentity, need_z = f;
   KFB_CHECK_ARG(dy != nullptr && (!(dw != nullptr || f) || x != nullptr) && (!(dx != nullptr || f) || w != nullptr), "fused_linear_bwd: null tensor");
   KFB_CHECK_ARG(!off16(dy) && !off16(x) && !off16(w) && !off16(dx) && !off16(dw), "fused_linear_bwd: tensors start on 16-byte boundaries");
-  const Room m = carve(workspace, rows, k, n, activation, precise, dy_dtype != KFB_BF16, wanted);
+  const Room m = carve(workspace, rows, k, n, activation, precise, !precise && dy_dtype != KFB_BF16, wanted);
   KFB_CHECK_ARG(workspace != nullptr || m.bytes == 0, "fused_linear_bwd: null workspace");
   KFB_CHECK_ARG(workspace_bytes >= m.bytes, "fused_linear_bwd: workspace %zu < %zu bytes", workspace_bytes, m.bytes);
   KFB_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "fused_linear_bwd: workspace must be 256-byte aligned");
-  const long long piece = piece_rows(rows, k, n, precise), nk = static_cast<long long>(n) * k;
+  const long long piece = m.piece, nk = static_cast<long long>(n) * k;
   const size_t dy_size = dy_dtype == KFB_FP32 ? 4 : 2, x_size = precise ? 4 : 2;
   if (m.w3 != nullptr) KFB_TRY(launch_split_planes(s, static_cast<const float*>(w), m.w3, nk, nk));
-  const int per_plane = blocks_per_plane(piece, k, n);
   for (long long r0 = 0; r0 < rows; r0 += piece) {
     const long long count = rows - r0 < piece ? rows - r0 : piece;
     const uint8_t *xp = static_cast<const uint8_t*>(x) + (x != nullptr ? r0 * k * x_size : 0), *dyp = static_cast<const uint8_t*>(dy) + r0 * n * dy_size;
@@ -296,7 +323,12 @@ KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, c
     MatmulArgs a = {};
     a.splits = 1;
     a.precise = precise;
-    if (need_z) {
+    int blocks = 0;
+    if (m.way.z) {
+      blocks = linear_pair_partials(count, n, k);
+      const LinearPair q = {kBackwardTail, xp, w, 0, bias, activation, dyp, m.dz, m.partial, count, n, k};
+      KFB_TRY(launch_linear_pair(s, q, "fused_linear_dz"));
+    } else if (need_z) {
       a.a = xo;
       a.b = wo;
       a.m = static_cast<int>(count);
@@ -307,7 +339,7 @@ KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, c
       a.out_fp32 = 1;
       KFB_TRY(launch_matmul(s, a, "fused_linear_z"));
     }
-    if (m.dz != nullptr || dbias != nullptr) {
+    if (!m.way.z && (m.dz != nullptr || dbias != nullptr)) {
       TailParams t = {};
       t.z = need_z ? m.z : nullptr;
       t.bias = bias;
@@ -319,15 +351,17 @@ KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, c
       t.partial = m.partial;
       t.rows = count;
       t.n = n;
-      int blocks;
       KFB_TRY(launch_tail<true>(s, t, activation, &blocks));
-      if (dbias != nullptr) {
-        LaunchScope scope(s, "linear_bias_sum");
-        KFB_TRY(launch_kernel(s, column_sum_kernel, cdiv(n, 32), 256, 0, const_cast<const float*>(m.partial), dbias, blocks, n, r0 > 0 ? 1 : 0));
-      }
+    }
+    if (dbias != nullptr) {
+      LaunchScope scope(s, "linear_bias_sum");
+      KFB_TRY(launch_kernel(s, column_sum_kernel, cdiv(n, 32), 1024, 0, const_cast<const float*>(m.partial), dbias, blocks, n, r0 > 0 ? 1 : 0));
     }
     MatOperand dz = operand(m.dz != nullptr ? static_cast<const void*>(m.dz) : dyp, n, 0, count * n);
-    if (dx != nullptr) {
+    if (dx != nullptr && m.way.dx) {
+      const LinearPair q = {kPlainTail, dz.ptr, w, 1, nullptr, kIdentity, nullptr, static_cast<uint8_t*>(dx) + r0 * k * x_size, nullptr, count, k, n};
+      KFB_TRY(launch_linear_pair(s, q, "fused_linear_dx"));
+    } else if (dx != nullptr) {
       a.a = dz;
       a.b = wo;
       a.b.by_k = 1;
@@ -339,7 +373,9 @@ KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, c
       a.out_fp32 = precise;
       KFB_TRY(launch_matmul(s, a, "fused_linear_dx"));
     }
-    if (dw != nullptr) {
+    if (dw != nullptr && m.way.dw) {
+      KFB_TRY(launch_linear_weights(s, dz.ptr, xp, m.planes, m.splits, r0 > 0 ? 1 : 0, count, n, k));
+    } else if (dw != nullptr) {
       a.a = dz;
       a.a.by_k = 1;
       a.b = xo;
@@ -350,14 +386,14 @@ KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, c
       a.d = m.planes;
       a.ld_d = k;
       a.out_fp32 = 1;
-      a.splits = weight_splits(count, per_plane);
+      a.splits = weight_splits(count, m.per_plane);
       a.plane_d = nk;
       a.accumulate = r0 > 0;
       KFB_TRY(launch_matmul(s, a, "fused_linear_dw"));
     }
   }
   if (dw != nullptr) {
-    const PlaneSum q = {m.planes, nk, weight_splits(piece, per_plane), dw, dw_dtype == KFB_FP32, nk};
+    const PlaneSum q = {m.planes, nk, m.splits, dw, dw_dtype == KFB_FP32, nk};
     KFB_TRY(launch_sum_planes(s, &q, 1));
   }
   return KFB_OK;

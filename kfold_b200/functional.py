@@ -620,7 +620,7 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     if residual is not None and (residual.shape != shape or (residual.dtype != x.dtype and residual.dtype != torch.float32)):
         raise ValueError(f"fused_linear: residual {residual.dtype} {tuple(residual.shape)} for x {x.dtype} {tuple(x.shape)} and {n} channels")
     out = x.new_empty(shape, dtype=x.dtype if residual is None else residual.dtype)
-    need = _fused_linear_bytes(at, rows, k, n, act, code, 0, 0)
+    need = _fused_linear_bytes(at, rows, k, n, act, code, L.dtype_code(out.dtype), 0)
     ws = _call_workspace(x.device, need) if need else None
     xc, wc, b = _operand(x, x.dtype), _operand(w, x.dtype), _affine(bias)
     rc = None if residual is None else _operand(residual, residual.dtype)

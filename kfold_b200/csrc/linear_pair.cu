@@ -24,11 +24,14 @@ constexpr int kThreads = 32 * (kTailWarp + 2 * kGroupWarps);
 
 template <int BN>
 struct Cfg {
-  static constexpr int kBStage = BN / 2 * 128, kStage = kBox + kBStage;
-  static constexpr int kTile = BN / 64 * kBox;       // a group's buffer
-  static constexpr int kStages = BN == 256 ? 3 : 6;
-  static constexpr int kSmem = kStages * kStage + 2 * kTile + 512 + 1024;
-  static constexpr int kChunks = BN / 64;            // 32-column chunks of a warp: half of the tile's columns
+  static constexpr int kBBoxes = (BN / 2 + 63) / 64;                  // of 64 columns, across k
+  static constexpr int kBStage = kBBoxes * kRowsBox, kStage = kBox + kBStage;
+  static constexpr int kBBytes = BN / 2 * 128;       // along k: what comes
+  static constexpr int kPasses = BN / 64;            // a group has 64 columns in a buffer at a time, of which a warp has 32
+  static constexpr int kFit = (232448 - 1536 - 4 * kBox) / kStage, kStages = kFit < 6 ? kFit : 6;
+  static constexpr int kTmem = BN == 128 ? 256 : 512;
+  static constexpr int kSmem = kStages * kStage + 4 * kBox + 512 + 1024;
+  static_assert(BN % 64 == 0 && kStages >= 3, "tiles of 128, 192 or 256 columns");
   static_assert(kSmem <= 232448, "shared memory");
 };
 
@@ -39,20 +42,6 @@ struct PairParams {
   float* partial;
 };
 
-// Sums over a warp's rows (lanes) of eight columns: lane l has column 4 (l >> 4 & 1) + 2 (l >> 3 & 1) + (l >> 2 & 1) at the end.  (Half of the columns change hands
-// at each of the first three steps.)
-__device__ __forceinline__ float sum_rows(const float (&v)[8], int lane) {
-  float a[4], b[2];
-  const bool h4 = lane & 16, h3 = lane & 8, h2 = lane & 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) a[i] = (h4 ? v[4 + i] : v[i]) + __shfl_xor_sync(0xffffffffu, h4 ? v[i] : v[4 + i], 16);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) b[i] = (h3 ? a[2 + i] : a[i]) + __shfl_xor_sync(0xffffffffu, h3 ? a[i] : a[2 + i], 8);
-  float c = (h2 ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, h2 ? b[0] : b[1], 4);
-  c += __shfl_xor_sync(0xffffffffu, c, 2);
-  return c + __shfl_xor_sync(0xffffffffu, c, 1);
-}
-
 template <int BN, int TAIL, bool BY_K>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_aux,
@@ -61,13 +50,13 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* tiles = ring + K::kStages * K::kStage;
-  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + 2 * K::kTile);      // in the leader: both CTAs' copies
+  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + 4 * kBox);          // in the leader: both CTAs' copies
   uint64_t* empty = full + K::kStages;
   uint64_t* acc_full = empty + K::kStages;           // [2]
   uint64_t* acc_empty = acc_full + 2;                // [2], in the leader: the group's warps in both CTAs
-  uint64_t* ready = acc_empty + 2;                   // [2] the group's buffer: aux has come, or it is free
-  uint64_t* done = ready + 2;                        // [2] the group's warps have written it
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 2);
+  uint64_t* ready = acc_empty + 2;                   // [group][buffer] aux has come, or the buffer is free
+  uint64_t* done = ready + 4;                        // [group][buffer] the group's warps have written it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(ptx::cluster_ctarank());
@@ -86,13 +75,15 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&acc_full[i], 1);
       ptx::mbar_init(&acc_empty[i], 2 * kGroupWarps);
+    }
+    for (int i = 0; i < 4; ++i) {
       ptx::mbar_init(&ready[i], 1);
       ptx::mbar_init(&done[i], kGroupWarps);
     }
     ptx::fence_barrier_init();
   }
   if (warp == 1) {
-    ptx::tmem_alloc_pair(tmem_slot, 2 * BN);
+    ptx::tmem_alloc_pair(tmem_slot, K::kTmem);
     ptx::tmem_relinquish_pair();
   }
   ptx::tc_fence_before_sync();
@@ -111,13 +102,13 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         for (int kb = 0; kb < p.blocks; ++kb) {
           ok = ptx::mbar_wait(&empty[st], ph ^ 1, 701);
           if (!ok) break;
-          if (rank == 0) ptx::mbar_expect_tx(&full[st], 2 * K::kStage);
+          if (rank == 0) ptx::mbar_expect_tx(&full[st], 2 * (kBox + (BY_K ? K::kBStage : K::kBBytes)));
           const uint32_t bar = ptx::leader_addr(&full[st]);
           uint8_t *a = ring + st * K::kStage, *b = a + kBox;
           ptx::tma_load_4d_pair(a, &tm_a, bar, kb * 64, row0_of(i), 0, 0);
           if constexpr (BY_K) {
 #pragma unroll
-            for (int q = 0; q < BN / 128; ++q) ptx::tma_load_4d_pair(b + q * kRowsBox, &tm_b, bar, n0 + rank * (BN / 2) + q * 64, kb * 64, 0, 0);
+            for (int q = 0; q < K::kBBoxes; ++q) ptx::tma_load_4d_pair(b + q * kRowsBox, &tm_b, bar, n0 + rank * (BN / 2) + q * 64, kb * 64, 0, 0);
           } else {
             ptx::tma_load_4d_pair(b, &tm_b, bar, kb * 64, n0 + rank * (BN / 2), 0, 0);
           }
@@ -162,51 +153,60 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     // ---------------------------------------------------------------- a group's buffer: aux in, the tile out
     if (ptx::elect_one()) {
       const int g = warp - 2;
-      uint8_t* tile = tiles + g * K::kTile;
-      for (int i = g; i < my_tiles; i += 2) {
-        const int row0 = row0_of(i);
+      const int count = (my_tiles - g + 1) / 2 * K::kPasses;      // passes of the group's tiles
+      auto row0_at = [&](int q) { return row0_of(g + q / K::kPasses * 2); };
+      auto arm = [&](int q) {
+        uint64_t* bar = &ready[2 * g + (q & 1)];
         if (TAIL != kPlainTail && p.has_aux) {
-          ptx::mbar_expect_tx(&ready[g], K::kTile);
-#pragma unroll
-          for (int q = 0; q < BN / 64; ++q) ptx::tma_load_4d(tile + q * kBox, &tm_aux, &ready[g], n0 + q * 64, row0, 0, 0);
+          ptx::mbar_expect_tx(bar, kBox);
+          ptx::tma_load_4d(tiles + (2 * g + (q & 1)) * kBox, &tm_aux, bar, n0 + q % K::kPasses * 64, row0_at(q), 0, 0);
         } else {
-          ptx::mbar_arrive(&ready[g]);
+          ptx::mbar_arrive(bar);
         }
-        if (!ptx::mbar_wait(&done[g], i >> 1 & 1, 705)) break;
-        if (row0 < p.rows) {
-          for (int q = 0; q < BN / 64 && n0 + q * 64 < p.n; ++q) ptx::tma_store_4d(&tm_out, tile + q * kBox, n0 + q * 64, row0, 0, 0);
+      };
+      for (int q = 0; q < 2 && q < count; ++q) arm(q);
+      for (int q = 0; q < count; ++q) {
+        if (!ptx::mbar_wait(&done[2 * g + (q & 1)], q >> 1 & 1, 705)) break;
+        const int col = n0 + q % K::kPasses * 64;
+        if (row0_at(q) < p.rows && col < p.n) {
+          ptx::tma_store_4d(&tm_out, tiles + (2 * g + (q & 1)) * kBox, col, row0_at(q), 0, 0);
           ptx::tma_store_commit();
         }
-        ptx::tma_store_wait_read();
+        if (q + 2 < count) {
+          ptx::tma_store_wait_read();                // (the group has the other buffer meanwhile)
+          arm(q + 2);
+        }
       }
       ptx::tma_store_wait_all();
     }
   } else {
     // ---------------------------------------------------------------- the tail: a warp has 32 rows (tensor-memory lanes) of half of the columns
-    const int g = (warp - kTailWarp) / kGroupWarps, quad = warp & 3, col0 = (warp - kTailWarp) / 4 % 2 * (BN / 2), r = quad * 32 + lane;
-    const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16) + g * BN + col0;
-    uint8_t* tile = tiles + g * K::kTile + r * 128;
-    float sums[K::kChunks];                          // of column 8 (lane & 3) + what sum_rows gives, of each chunk
+    const int g = (warp - kTailWarp) / kGroupWarps, quad = warp & 3, half = (warp - kTailWarp) / 4 % 2, r = quad * 32 + lane;
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16) + g * BN + half * 32;
+    uint8_t* row = tiles + 2 * g * kBox + r * 128;
+    float sums[K::kPasses];                          // of column 8 (lane & 3) + what sum_rows8 gives, of each pass
 #pragma unroll
-    for (int j = 0; j < K::kChunks; ++j) sums[j] = 0.f;
-    for (int i = g; i < my_tiles; i += 2) {
-      const uint32_t ph = i >> 1 & 1;
-      if (!__all_sync(0xffffffffu, ptx::mbar_wait(&ready[g], ph, 706))) break;
-      if (!__all_sync(0xffffffffu, ptx::mbar_wait(&acc_full[g], ph, 707))) break;
+    for (int j = 0; j < K::kPasses; ++j) sums[j] = 0.f;
+    bool ok = true;
+    int at_pass = 0;
+    for (int i = g; ok && i < my_tiles; i += 2) {
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&acc_full[g], i >> 1 & 1, 707)) != 0;
+      if (!ok) break;
       ptx::tc_fence_after_sync();
-#pragma unroll(TAIL == kBackwardTail ? K::kChunks : 1)
-      for (int j = 0; j < K::kChunks; ++j) {
+#pragma unroll(TAIL == kBackwardTail ? K::kPasses : 1)
+      for (int pass = 0; pass < K::kPasses; ++pass, ++at_pass) {
+        const int buffer = at_pass & 1, col = pass * 64 + half * 32;
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&ready[2 * g + buffer], at_pass >> 1 & 1, 706)) != 0;
+        if (!ok) break;
         uint32_t raw[32];
-        ptx::tmem_ld_32x32b_x32(t_row + j * 32, raw);
+        ptx::tmem_ld_32x32b_x32(t_row + pass * 64, raw);
         ptx::tmem_ld_wait();
-        if (j + 1 == K::kChunks) {
+        if (pass + 1 == K::kPasses) {
           ptx::tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive_cluster(ptx::leader_addr(&acc_empty[g]));
         }
-        const int col = col0 + j * 32;
-        uint8_t* row = tile + col / 64 * kBox;
-        auto cell_at = [&](int c) { return reinterpret_cast<uint4*>(row + (((col / 8 + c) & 7) ^ (r & 7)) * 16); };
+        auto cell_at = [&](int c) { return reinterpret_cast<uint4*>(row + buffer * kBox + ((half * 4 + c) ^ (r & 7)) * 16); };
         if constexpr (TAIL == kPlainTail) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -221,54 +221,54 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const int at = n0 + col + 8 * c;
-              float v[8];
+              uint64_t v[4], x[4];
 #pragma unroll
-              for (int q = 0; q < 8; ++q) v[q] = __uint_as_float(raw[8 * c + q]);
+              for (int q = 0; q < 4; ++q) v[q] = ptx::pack2(raw[8 * c + 2 * q], raw[8 * c + 2 * q + 1]);
               if (p.bias != nullptr && at < p.n) {          // (n is a multiple of 8)
-                const float4 lo = *reinterpret_cast<const float4*>(p.bias + at), hi = *reinterpret_cast<const float4*>(p.bias + at + 4);
-                v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w, v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+                const ulonglong2* b = reinterpret_cast<const ulonglong2*>(p.bias + at);
+                const ulonglong2 lo = b[0], hi = b[1];
+                v[0] = ptx::add2(v[0], lo.x), v[1] = ptx::add2(v[1], lo.y), v[2] = ptx::add2(v[2], hi.x), v[3] = ptx::add2(v[3], hi.y);
               }
               uint4* cell = cell_at(c);
-              float x[8];
               if (TAIL == kBackwardTail || p.has_aux) {
                 const uint4 a = *cell;
                 const uint32_t aw[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-                for (int q = 0; q < 8; ++q) x[q] = __uint_as_float(q & 1 ? aw[q / 2] & 0xffff0000u : aw[q / 2] << 16);
+                for (int q = 0; q < 4; ++q) x[q] = ptx::pack2(aw[q] << 16, aw[q] & 0xffff0000u);
               }
               if constexpr (TAIL == kForwardTail) {
 #pragma unroll
-                for (int q = 0; q < 8; ++q) v[q] = activation<ACT>(v[q]);
+                for (int q = 0; q < 4; ++q) v[q] = activation<ACT>(v[q]);
                 if (p.has_aux) {
 #pragma unroll
-                  for (int q = 0; q < 8; ++q) v[q] += x[q];
+                  for (int q = 0; q < 4; ++q) v[q] = ptx::add2(v[q], x[q]);
                 }
               } else {
 #pragma unroll
-                for (int q = 0; q < 8; ++q) v[q] = x[q] * slope<ACT>(v[q]);
+                for (int q = 0; q < 4; ++q) v[q] = ptx::mul2(x[q], slope<ACT>(v[q]));
                 if (p.partial != nullptr) {
-                  const float s = sum_rows(v, lane);
-                  if ((lane & 3) == c) sums[j] += s;
+                  const float s = sum_rows8(v, lane);
+                  if ((lane & 3) == c) sums[pass] += s;
                 }
               }
               uint32_t w[4];
 #pragma unroll
-              for (int q = 0; q < 4; ++q) w[q] = pack_bf16x2(v[2 * q], v[2 * q + 1]);
+              for (int q = 0; q < 4; ++q) w[q] = pack_bf16x2(v[q]);
               *cell = make_uint4(w[0], w[1], w[2], w[3]);
             }
           });
         }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&done[2 * g + buffer]);
       }
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&done[g]);
     }
     if (TAIL == kBackwardTail && p.partial != nullptr) {
       // a row of partial sums for each pair of a column tile, group, CTA and quadrant
       float* row = p.partial + static_cast<long long>(((first * 2 + g) * 2 + rank) * 4 + quad) * p.n;
 #pragma unroll
-      for (int j = 0; j < K::kChunks; ++j) {
-        const int at = n0 + col0 + j * 32 + 8 * (lane & 3) + 4 * (lane >> 4 & 1) + 2 * (lane >> 3 & 1) + (lane >> 2 & 1);
+      for (int j = 0; j < K::kPasses; ++j) {
+        const int at = n0 + j * 64 + half * 32 + 8 * (lane & 3) + 4 * (lane >> 4 & 1) + 2 * (lane >> 3 & 1) + (lane >> 2 & 1);
         if (at < p.n) row[at] = sums[j];
       }
     }
@@ -279,7 +279,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   ptx::cluster_sync();      // neither CTA leaves while the other may still read its operands or reach its barriers
   if (warp == 1) {
     ptx::tc_fence_after_sync();
-    ptx::tmem_dealloc_pair(tmem, 2 * BN);
+    ptx::tmem_dealloc_pair(tmem, K::kTmem);
   }
 }
 
@@ -296,8 +296,13 @@ int pairs_held() {
   return held[dev & 63];
 }
 
-// A tile's columns: 256, or 128 where these leave fewer of them unused.
-int tile_width(int n) { return (n + 255) / 256 * 256 - n >= 128 ? 128 : 256; }
+// A tile's columns: 256, or 192 or 128 where these leave fewer of them unused.
+int tile_width(int n) {
+  int best = 256;
+  for (int w : {192, 128})
+    if (cdiv(n, w) * w < cdiv(n, best) * best) best = w;
+  return best;
+}
 
 struct Grid {
   int bn, n_tiles, row_blocks, groups;
@@ -353,7 +358,10 @@ int launch_width(cudaStream_t stream, const LinearPair& q, const char* tag) {
   return launch_as<BN, kPlainTail, true>(stream, q, tag);
 }
 
-int backward_pairs(int n) { return tile_width(n) == 256 ? pairs_held<256, kBackwardTail, false>() : pairs_held<128, kBackwardTail, false>(); }
+int backward_pairs(int n) {
+  const int w = tile_width(n);
+  return w == 256 ? pairs_held<256, kBackwardTail, false>() : w == 192 ? pairs_held<192, kBackwardTail, false>() : pairs_held<128, kBackwardTail, false>();
+}
 
 }  // namespace
 
@@ -368,7 +376,8 @@ int linear_pair_partials(long long rows, int n, int k) { return grid_of(rows, n,
 
 int launch_linear_pair(cudaStream_t stream, const LinearPair& p, const char* tag) {
   KFB_CHECK_ARG((p.tail == kPlainTail) == (p.by_k != 0), "linear: tail %d with an operand %s k", p.tail, p.by_k ? "across" : "along");
-  return tile_width(p.n) == 256 ? launch_width<256>(stream, p, tag) : launch_width<128>(stream, p, tag);
+  const int w = tile_width(p.n);
+  return w == 256 ? launch_width<256>(stream, p, tag) : w == 192 ? launch_width<192>(stream, p, tag) : launch_width<128>(stream, p, tag);
 }
 
 }  // namespace kfb

@@ -5,54 +5,109 @@
 #include <type_traits>
 
 #include "common.cuh"
+#ifdef __CUDACC__
+#include "ptx.cuh"
+#endif
 
 namespace kfb {
 
 enum Activation : int { kIdentity = 0, kSigmoid = 1, kSilu = 2, kGelu = 3, kRelu = 4 };
 
 #ifdef __CUDACC__
-// The complementary error function for x >= 0 by the Chebyshev fit of Press, Teukolsky, Vetterling and Flannery, "Numerical Recipes in C" (1992), 6.2,
-// whose relative error is below 1.2e-7 everywhere: Phi(z) keeps its digits where it is small.
-__device__ __forceinline__ float erfc_positive(float x) {
-  const float t = __fdividef(1.f, fmaf(0.5f, x, 1.f));
-  float q = 0.17087277f;
-  q = fmaf(q, t, -0.82215223f);
-  q = fmaf(q, t, 1.48851587f);
-  q = fmaf(q, t, -1.13520398f);
-  q = fmaf(q, t, 0.27886807f);
-  q = fmaf(q, t, -0.18628806f);
-  q = fmaf(q, t, 0.09678418f);
-  q = fmaf(q, t, 0.37409196f);
-  q = fmaf(q, t, 1.00002368f);
-  q = fmaf(q, t, -1.26551223f);
-  return t * __expf(fmaf(-x, x, q));
+// The activations work on pairs of float32, which the two-wide instructions take at one issue slot a pair: an element's tail, not its products, is what a tile's time
+// would be otherwise.
+__device__ __forceinline__ uint64_t pair_of(float a) { return ptx::pack2(a, a); }
+template <typename F>
+__device__ __forceinline__ uint64_t each_of(uint64_t v, F f) {
+  const float2 t = ptx::unpack2(v);
+  return ptx::pack2(f(t.x), f(t.y));
 }
-__device__ __forceinline__ float normal_cdf(float z) {
-  const float t = 0.5f * erfc_positive(0.70710678f * fabsf(z));
-  return z < 0.f ? t : 1.f - t;
+__device__ __forceinline__ uint64_t magnitude(uint64_t v) { return v & 0x7fffffff7fffffffull; }
+__device__ __forceinline__ uint64_t reciprocal(uint64_t v) {
+  return each_of(v, [](float a) { return __fdividef(1.f, a); });
+}
+// 2^v
+__device__ __forceinline__ uint64_t power(uint64_t v) {
+  return each_of(v, [](float a) { return exp2f(a); });
+}
+// low where z is negative, high elsewhere
+__device__ __forceinline__ uint64_t by_sign(uint64_t z, uint64_t low, uint64_t high) {
+  const float2 a = ptx::unpack2(z), l = ptx::unpack2(low), h = ptx::unpack2(high);
+  return ptx::pack2(a.x < 0.f ? l.x : h.x, a.y < 0.f ? l.y : h.y);
 }
 
-// f(z) and f'(z).  sigmoid's slope comes from exp(-|z|), so that it stays exact where the gate is open; gelu is z Phi(z).
+// exp(-z^2 / 2), and Phi(z) from it: Phi(-|z|) = exp(-z^2 / 2) t P(t), t = 1 / (1 + 0.30052 |z|), P of degree 7 fitted to erfcx by least squares with weights that level
+// the relative error, 1.2e-7 at most for |z| < 13.4, where exp(-z^2 / 2) ends: Phi keeps its digits where it is small.
+__device__ __forceinline__ uint64_t normal_cdf(uint64_t z, uint64_t& density) {
+  density = power(ptx::mul2(ptx::mul2(z, z), pair_of(-0.72134752f)));
+  const uint64_t t = reciprocal(ptx::fma2(magnitude(z), pair_of(0.3005204f), pair_of(1.f)));
+  uint64_t p = pair_of(0.036092564f);
+  p = ptx::fma2(p, t, pair_of(-0.15805097f));
+  p = ptx::fma2(p, t, pair_of(0.20634612f));
+  p = ptx::fma2(p, t, pair_of(-0.053961266f));
+  p = ptx::fma2(p, t, pair_of(0.12877955f));
+  p = ptx::fma2(p, t, pair_of(0.099978104f));
+  p = ptx::fma2(p, t, pair_of(0.12098045f));
+  p = ptx::fma2(p, t, pair_of(0.119835384f));
+  const uint64_t low = ptx::mul2(ptx::mul2(p, t), density);
+  return by_sign(z, low, ptx::fma2(low, pair_of(-1.f), pair_of(1.f)));
+}
+// sigmoid(z), and its slope from exp(-|z|), so that this stays exact where the gate is open.
+__device__ __forceinline__ uint64_t sigmoid_of(uint64_t z, uint64_t& slope) {
+  const uint64_t e = power(ptx::mul2(magnitude(z), pair_of(-1.44269504f))), d = reciprocal(ptx::add2(e, pair_of(1.f))), low = ptx::mul2(e, d);
+  slope = ptx::mul2(low, d);
+  return by_sign(z, low, d);
+}
+
+// f(z) and f'(z); gelu is z Phi(z).
 template <int ACT>
-__device__ __forceinline__ float activation(float z) {
-  if constexpr (ACT == kRelu) return z > 0.f || z != z ? z : 0.f;
-  if constexpr (ACT == kGelu) return z * normal_cdf(z);
-  if constexpr (ACT == kSigmoid || ACT == kSilu) {
-    const float e = __expf(-fabsf(z)), d = __fdividef(1.f, 1.f + e), s = z < 0.f ? e * d : d;
-    return ACT == kSigmoid ? s : z * s;
-  }
+__device__ __forceinline__ uint64_t activation(uint64_t z) {
+  uint64_t other;
+  if constexpr (ACT == kRelu) return each_of(z, [](float a) { return a > 0.f || a != a ? a : 0.f; });
+  if constexpr (ACT == kGelu) return ptx::mul2(z, normal_cdf(z, other));
+  if constexpr (ACT == kSigmoid) return sigmoid_of(z, other);
+  if constexpr (ACT == kSilu) return ptx::mul2(z, sigmoid_of(z, other));
   return z;
 }
 template <int ACT>
-__device__ __forceinline__ float slope(float z) {
-  if constexpr (ACT == kRelu) return z > 0.f ? 1.f : 0.f;
-  if constexpr (ACT == kGelu) return fmaf(z * 0.39894228f, __expf(-0.5f * z * z), normal_cdf(z));
-  if constexpr (ACT == kSigmoid || ACT == kSilu) {
-    const float e = __expf(-fabsf(z)), d = __fdividef(1.f, 1.f + e), s = z < 0.f ? e * d : d, ss = e * d * d;
-    return ACT == kSigmoid ? ss : fmaf(z, ss, s);
+__device__ __forceinline__ uint64_t slope(uint64_t z) {
+  uint64_t other;
+  if constexpr (ACT == kRelu) return each_of(z, [](float a) { return a > 0.f ? 1.f : 0.f; });
+  if constexpr (ACT == kGelu) {
+    const uint64_t cdf = normal_cdf(z, other);
+    return ptx::fma2(ptx::mul2(z, pair_of(0.39894228f)), other, cdf);
   }
-  return 1.f;
+  if constexpr (ACT == kSigmoid) {
+    sigmoid_of(z, other);
+    return other;
+  }
+  if constexpr (ACT == kSilu) {
+    const uint64_t s = sigmoid_of(z, other);
+    return ptx::fma2(z, other, s);
+  }
+  return pair_of(1.f);
 }
+
+// Sums over a warp's rows (lanes) of eight columns: lane l has column 4 (l >> 4 & 1) + 2 (l >> 3 & 1) + (l >> 2 & 1) at the end.  (Half of the columns change hands
+// at each of the first three steps.)
+__device__ __forceinline__ float sum_rows8(const uint64_t (&pairs)[4], int lane) {
+  float v[8], a[4], b[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = ptx::unpack2(pairs[i]);
+    v[2 * i] = t.x;
+    v[2 * i + 1] = t.y;
+  }
+  const bool h4 = lane & 16, h3 = lane & 8, h2 = lane & 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] = (h4 ? v[4 + i] : v[i]) + __shfl_xor_sync(0xffffffffu, h4 ? v[i] : v[4 + i], 16);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) b[i] = (h3 ? a[2 + i] : a[i]) + __shfl_xor_sync(0xffffffffu, h3 ? a[i] : a[2 + i], 8);
+  float c = (h2 ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, h2 ? b[0] : b[1], 4);
+  c += __shfl_xor_sync(0xffffffffu, c, 2);
+  return c + __shfl_xor_sync(0xffffffffu, c, 1);
+}
+
 // A call with the activation as a constant.
 template <typename F>
 __device__ __forceinline__ void with_activation(int act, F f) {
@@ -86,8 +141,10 @@ int linear_pair_partials(long long rows, int n, int k);       // rows of partial
 int launch_linear_pair(cudaStream_t stream, const LinearPair& p, const char* tag);
 
 // dW planes: plane[s][n][k] = sum over a piece of the rows of dz^T x (linear_weights.cu).
-bool linear_weights_ok(int n, int k);
+// bias_planes: null, or [s][n] sums of dz over the same pieces.
+bool linear_weights_ok(long long rows, int n, int k);
 int linear_weights_splits(long long rows, int n, int k);
-int launch_linear_weights(cudaStream_t stream, const void* dz, const void* x, float* planes, int splits, int add, long long rows, int n, int k);
+int launch_linear_weights(cudaStream_t stream, const void* dz, const void* x, float* planes, float* bias_planes, int splits, int add, long long rows, int n,
+                          int k);
 
 }  // namespace kfb

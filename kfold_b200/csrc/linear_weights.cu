@@ -1,7 +1,8 @@
 // The gradient of a linear layer's weights: plane[s][n][k] = sum over piece s of the rows of dz(r, n) x(r, k), bf16 operands, float32 planes.
 //
 // What bounds it: dz and x in, HBM, and their trips through shared memory.  A CTA pair (cta_group::2) multiplies 256 columns of dz by 256 of x over its piece
-// of the rows, so that each operand is read by few pairs; all operands lie across the contraction and are read as they lie.
+// of the rows, so that each operand is read by few pairs; all operands lie across the contraction and are read as they lie.  The bias's gradient, where dz is the
+// gradient itself, is one more product with columns of ones: a pass over dz and a launch less.
 #include <mutex>
 
 #include "gemm.cuh"   // st_global_v8
@@ -17,11 +18,13 @@ constexpr int kOperand = 2 * kBox, kStage = 2 * kOperand, kStages = 6;      // 1
 constexpr int kTile = 256;
 constexpr int kTailWarp = 4, kTailWarps = 8;
 constexpr int kThreads = 32 * (kTailWarp + kTailWarps);
-constexpr int kSmem = kStages * kStage + 512 + 1024;
+constexpr int kOnes = 4096;                          // bytes of ones: the operand whose product with dz is its sums over rows, whatever its layout
+constexpr int kOnesColumns = 32;                     // of the pair
+constexpr int kSmem = kStages * kStage + kOnes + 512 + 1024;
 
 struct WeightParams {
   int n, k, blocks, splits, n_tiles, tiles, add;     // blocks of 64 rows
-  float* planes;
+  float *planes, *bias_planes;
 };
 
 __device__ __forceinline__ uint64_t across_desc(uint32_t addr) {   // rows of 128 bytes, one per row of the operand; the next 64 columns a box further
@@ -33,7 +36,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 linear_weights_kernel(const __grid_constant__ CUtensorMap tm_dz, const __grid_constant__ CUtensorMap tm_x, const WeightParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * kStage);     // in the leader: both CTAs' copies
+  uint8_t* ones = ring + kStages * kStage;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ones + kOnes);                // in the leader: both CTAs' copies
   uint64_t* empty = full + kStages;
   uint64_t* done = empty + kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
@@ -55,8 +59,11 @@ linear_weights_kernel(const __grid_constant__ CUtensorMap tm_dz, const __grid_co
     ptx::mbar_init(done, 1);
     ptx::fence_barrier_init();
   }
+  const bool bias = p.bias_planes != nullptr && k0 == 0;
+  for (int i = threadIdx.x; i < kOnes / 4; i += kThreads) reinterpret_cast<uint32_t*>(ones)[i] = 0x3f803f80u;
+  ptx::fence_proxy_async_smem();
   if (warp == 1) {
-    ptx::tmem_alloc_pair(tmem_slot, kTile);
+    ptx::tmem_alloc_pair(tmem_slot, 512);
     ptx::tmem_relinquish_pair();
   }
   ptx::tc_fence_before_sync();
@@ -92,7 +99,8 @@ linear_weights_kernel(const __grid_constant__ CUtensorMap tm_dz, const __grid_co
   } else if (warp == 1) {
     if (rank == 0 && ptx::elect_one()) {
       constexpr uint32_t idesc = ptx::make_idesc(256, kTile, 1) | (1u << 15) | (1u << 16);
-      const uint64_t d0 = across_desc(ptx::smem_u32(ring));
+      constexpr uint32_t ones_idesc = ptx::make_idesc(256, kOnesColumns, 1) | (1u << 15);
+      const uint64_t d0 = across_desc(ptx::smem_u32(ring)), ones_desc = ptx::make_kmajor_desc<128>(ptx::smem_u32(ones));
       int st = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -103,6 +111,10 @@ linear_weights_kernel(const __grid_constant__ CUtensorMap tm_dz, const __grid_co
         const uint64_t a = d0 + st * (kStage >> 4), x = a + (kOperand >> 4);
 #pragma unroll
         for (int k = 0; k < 4; ++k) ptx::mma_f16_ss_pair(tmem, a + k * (2048 >> 4), x + k * (2048 >> 4), idesc, b > b0 || k > 0 ? 1u : 0u);
+        if (bias) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) ptx::mma_f16_ss_pair(tmem + kTile, a + k * (2048 >> 4), ones_desc, ones_idesc, b > b0 || k > 0 ? 1u : 0u);
+        }
         ptx::tc_commit_pair(&empty[st]);
         if (++st == kStages) { st = 0; ph ^= 1u; }
       }
@@ -115,6 +127,15 @@ linear_weights_kernel(const __grid_constant__ CUtensorMap tm_dz, const __grid_co
     const bool ok = __all_sync(0xffffffffu, ptx::mbar_wait(done, 0, 724)) != 0;
     ptx::tc_fence_after_sync();
     if (ok) {
+      if (bias && c0 == 0) {
+        uint32_t v[8];
+        ptx::tmem_ld_32x32b_x8(t_row + kTile, v);
+        ptx::tmem_ld_wait();
+        if (n < p.n) {
+          float* d = p.bias_planes + static_cast<long long>(split) * p.n + n;
+          *d = __uint_as_float(v[0]) + (p.add ? *d : 0.f);
+        }
+      }
       float* d = p.planes + (static_cast<long long>(split) * p.n + n) * p.k + k0;
 #pragma unroll 1
       for (int c = c0; c < c0 + kTile / 2; c += 32) {
@@ -140,7 +161,7 @@ linear_weights_kernel(const __grid_constant__ CUtensorMap tm_dz, const __grid_co
   ptx::cluster_sync();      // neither CTA leaves while the other may still read its operands or reach its barriers
   if (warp == 1) {
     ptx::tc_fence_after_sync();
-    ptx::tmem_dealloc_pair(tmem, kTile);
+    ptx::tmem_dealloc_pair(tmem, 512);
   }
 }
 
@@ -166,14 +187,16 @@ int tiles_of(int n, int k) { return cdiv(n, kTile) * cdiv(k, kTile); }
 
 }  // namespace
 
-bool linear_weights_ok(int n, int k) { return n >= 256 && k >= 256 && tiles_of(n, k) <= pairs_held(); }
+// Many rows: below some thousand a pair's start and end, and the planes, cost more than tiles of 128 x 128 do (matmul.cu).
+bool linear_weights_ok(long long rows, int n, int k) { return rows >= 4096 && n >= 256 && k >= 256 && tiles_of(n, k) <= pairs_held(); }
 
 int linear_weights_splits(long long rows, int n, int k) {
   const long long blocks = (rows + kK - 1) / kK, most = pairs_held() / tiles_of(n, k);
   return static_cast<int>(most < 1 ? 1 : most < blocks ? most : blocks);
 }
 
-int launch_linear_weights(cudaStream_t stream, const void* dz, const void* x, float* planes, int splits, int add, long long rows, int n, int k) {
+int launch_linear_weights(cudaStream_t stream, const void* dz, const void* x, float* planes, float* bias_planes, int splits, int add, long long rows, int n,
+                          int k) {
   CUtensorMap ta, tb;
   KFB_TRY(matrix_map(&ta, dz, rows, n));
   KFB_TRY(matrix_map(&tb, x, rows, k));
@@ -187,6 +210,7 @@ int launch_linear_weights(cudaStream_t stream, const void* dz, const void* x, fl
   p.tiles = tiles_of(n, k);
   p.add = add;
   p.planes = planes;
+  p.bias_planes = bias_planes;
   LaunchScope scope(stream, "linear_weights");
   return launch_kernel_clustered(stream, linear_weights_kernel, 2, 2 * p.tiles * p.splits, kThreads, kSmem, ta, tb, p);
 }

@@ -12,6 +12,7 @@
 #include "matmul.cuh"
 
 #include "gemm.cuh"   // split3, epi_store_chunk
+#include "linear_tail.cuh"
 #include "ops_common.cuh"
 #include "ptx.cuh"
 
@@ -34,6 +35,7 @@ struct MmParams {
 struct MmBatch {
   CUtensorMap a[kMostMatmuls], b[kMostMatmuls];
   MmParams p[kMostMatmuls];
+  MatmulTail tail;                                 // of a launch of one product
   int end[kMostMatmuls];                           // blocks of the grid up to and with each product
 };
 
@@ -48,9 +50,75 @@ __device__ __forceinline__ uint64_t by_k_desc(uint32_t addr) {
          (1ull << 46) | (2ull << 61);
 }
 
-template <int PARTS>
-__global__ void __launch_bounds__(kThreads, PARTS == 3 ? 1 : 2) matmul_kernel(const __grid_constant__ MmBatch batch) {
-  constexpr int kStages = stages<PARTS>();
+// The launches with a tail have tiles of 64 columns and twice the warps for them: few rows make few tiles, and a tile's tail is the longer part.
+template <bool TAIL>
+constexpr int tile_columns() { return TAIL ? 64 : kTile; }
+template <bool TAIL>
+constexpr int threads() { return TAIL ? kThreads + 128 : kThreads; }
+
+// A tail's tensor at eight neighbouring columns, as pairs of float32.
+__device__ __forceinline__ void tail_load(const void* p, long long o, int fp32, uint64_t (&v)[4]) {
+  if (fp32) {
+    const ulonglong2* q = reinterpret_cast<const ulonglong2*>(static_cast<const float*>(p) + o);
+    const ulonglong2 a = q[0], b = q[1];
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + o);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = ptx::pack2(w[i] << 16, w[i] & 0xffff0000u);
+  }
+}
+
+// 32 columns of a row through the tail.  x: aux there, zeros where there is none.  (Columns end at a multiple of 8, the tensors' rows start on 16-byte boundaries.)
+__device__ __forceinline__ void tail_chunk(const MatmulTail& t, const EpiSeg& out, long long plane, long long row_off, int row_group, int col, int n, const float (&v)[32],
+                                           const uint64_t (&x)[4][4], bool there, int lane) {
+  with_activation(t.act, [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int at = col + 8 * c;
+      if (at >= n) break;
+      uint64_t z[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] = ptx::pack2(v[8 * c + 2 * i], v[8 * c + 2 * i + 1]);
+      if (t.bias != nullptr) {
+        tail_load(t.bias, at, 1, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] = ptx::add2(z[i], b[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] = t.backward ? ptx::mul2(x[c][i], slope<ACT>(z[i])) : ptx::add2(activation<ACT>(z[i]), x[c][i]);
+      if (t.partial != nullptr) {
+        const float s = sum_rows8(z, lane);
+        if ((lane & 3) == 0) t.partial[static_cast<long long>(row_group) * n + at + 4 * (lane >> 4 & 1) + 2 * (lane >> 3 & 1) + (lane >> 2 & 1)] = s;
+      }
+      if (!there) continue;
+      if (t.parts == 3) {
+        __nv_bfloat16 q[3][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = ptx::unpack2(z[i]);
+          split3(f.x, q[0][2 * i], q[1][2 * i], q[2][2 * i]);
+          split3(f.y, q[0][2 * i + 1], q[1][2 * i + 1], q[2][2 * i + 1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out.dst) + k * plane + row_off + at) = *reinterpret_cast<const uint4*>(q[k]);
+      } else if (out.out_fp32) {
+        ulonglong2* d = reinterpret_cast<ulonglong2*>(static_cast<float*>(out.dst) + row_off + at);
+        d[0] = make_ulonglong2(z[0], z[1]);
+        d[1] = make_ulonglong2(z[2], z[3]);
+      } else {
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out.dst) + row_off + at) = make_uint4(pack_bf16x2(z[0]), pack_bf16x2(z[1]), pack_bf16x2(z[2]), pack_bf16x2(z[3]));
+      }
+    }
+  });
+}
+
+template <int PARTS, bool TAIL>
+__global__ void __launch_bounds__(threads<TAIL>(), PARTS == 3 ? 1 : 2) matmul_kernel(const __grid_constant__ MmBatch batch) {
+  constexpr int kStages = stages<PARTS>(), kTileN = tile_columns<TAIL>(), kBytes = kOperand + kTileN * kK * 2;
   constexpr uint32_t kCols = PARTS == 3 ? 256 : 128;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -100,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, PARTS == 3 ? 1 : 2) matmul_kernel(co
         for (int part = 0; part < PARTS; ++part) {
           ok = ptx::mbar_wait(&empty[st], ph ^ 1, 501);
           if (!ok) break;
-          ptx::mbar_expect_tx(&full[st], kStage);
+          ptx::mbar_expect_tx(&full[st], kBytes);
           uint8_t *a = ring + st * kStage, *b = a + kOperand;
           if (p.a_by_k) {
             ptx::tma_load_3d(a, &tm_a, &full[st], m_tile * kTile, kb * kK, part);
@@ -108,18 +176,18 @@ __global__ void __launch_bounds__(kThreads, PARTS == 3 ? 1 : 2) matmul_kernel(co
           } else {
             ptx::tma_load_3d(a, &tm_a, &full[st], kb * kK, m_tile * kTile, part);
           }
-          if (p.b_by_k) {
-            ptx::tma_load_3d(b, &tm_b, &full[st], n_tile * kTile, kb * kK, part);
-            ptx::tma_load_3d(b + kOperand / 2, &tm_b, &full[st], n_tile * kTile + 64, kb * kK, part);
+          if (p.b_by_k) {                            // (never with a tail)
+            ptx::tma_load_3d(b, &tm_b, &full[st], n_tile * kTileN, kb * kK, part);
+            ptx::tma_load_3d(b + kOperand / 2, &tm_b, &full[st], n_tile * kTileN + 64, kb * kK, part);
           } else {
-            ptx::tma_load_3d(b, &tm_b, &full[st], kb * kK, n_tile * kTile, part);
+            ptx::tma_load_3d(b, &tm_b, &full[st], kb * kK, n_tile * kTileN, part);
           }
           if (++st == kStages) { st = 0; ph ^= 1u; }
         }
     }
   } else if (warp == 1) {
     if (ptx::elect_one()) {
-      const uint32_t idesc = ptx::make_idesc(kTile, kTile, 1) | (p.a_by_k ? 1u << 15 : 0u) | (p.b_by_k ? 1u << 16 : 0u);
+      const uint32_t idesc = ptx::make_idesc(kTile, kTileN, 1) | (p.a_by_k ? 1u << 15 : 0u) | (p.b_by_k ? 1u << 16 : 0u);
       const uint32_t a_step = p.a_by_k ? 2048 >> 4 : 2, b_step = p.b_by_k ? 2048 >> 4 : 2;     // of 16 k
       int st = 0;
       uint32_t ph = 0;
@@ -158,13 +226,25 @@ __global__ void __launch_bounds__(kThreads, PARTS == 3 ? 1 : 2) matmul_kernel(co
   } else {
     const int quad = warp & 3, row = m_tile * kTile + quad * 32 + lane;
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const long long row_off = static_cast<long long>(row) * p.out.s_n + (TAIL ? 0 : split * p.plane_d);
+    // a tail's warp has 32 columns; what is added or multiplied comes while the products are made
+    const int c_first = TAIL ? (warp - 2) / 4 * 32 : 0, c_end = TAIL ? c_first + 32 : kTile;
+    uint64_t x[4][4];
+    if constexpr (TAIL) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int at = n_tile * kTileN + c_first + 8 * c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[c][i] = 0;
+        if (batch.tail.aux != nullptr && row < p.m && at < p.n) tail_load(batch.tail.aux, row_off + at, batch.tail.aux_fp32, x[c]);
+      }
+    }
     const bool ok = __all_sync(0xffffffffu, ptx::mbar_wait(done, 0, 503)) != 0;
     ptx::tc_fence_after_sync();
     if (ok) {
-      const long long row_off = static_cast<long long>(row) * p.out.s_n + split * p.plane_d;
 #pragma unroll 1
-      for (int c = 0; c < kTile; c += 32) {
-        const int col = n_tile * kTile + c;
+      for (int c = c_first; c < c_end; c += 32) {
+        const int col = n_tile * kTileN + c;
         if (col >= p.n) break;
         uint32_t raw[32];
         float v[32];
@@ -177,6 +257,10 @@ __global__ void __launch_bounds__(kThreads, PARTS == 3 ? 1 : 2) matmul_kernel(co
           ptx::tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(raw[i]);
+        }
+        if constexpr (TAIL) {
+          tail_chunk(batch.tail, p.out, p.plane_d, row_off, m_tile * 4 + quad, col, p.n, v, x, row < p.m, lane);
+          continue;
         }
         if (p.accumulate && row < p.m) {
           const float* d = static_cast<const float*>(p.out.dst) + row_off + col;
@@ -207,10 +291,10 @@ __global__ void __launch_bounds__(kThreads, PARTS == 3 ? 1 : 2) matmul_kernel(co
   }
 }
 
-int operand_map(CUtensorMap* map, const MatOperand& o, int extent, long long k, int parts) {
+int operand_map(CUtensorMap* map, const MatOperand& o, int extent, long long k, int parts, int tile) {
   const uint64_t dims[3] = {static_cast<uint64_t>(o.by_k ? extent : k), static_cast<uint64_t>(o.by_k ? k : extent), static_cast<uint64_t>(parts)};
   const uint64_t str[2] = {static_cast<uint64_t>(o.ld) * 2, static_cast<uint64_t>(parts > 1 ? o.plane : o.ld) * 2};
-  const uint32_t box[3] = {64, o.by_k ? 64u : static_cast<uint32_t>(kTile), 1};
+  const uint32_t box[3] = {64, o.by_k ? 64u : static_cast<uint32_t>(tile), 1};
   return make_tmap(map, o.ptr, 2, 3, dims, str, box, 128);
 }
 
@@ -272,7 +356,8 @@ int launch_matmuls(cudaStream_t stream, const MatmulArgs* list, int count, const
     p.m = a.m;
     p.n = a.n;
     p.m_tiles = cdiv(a.m, kTile);
-    p.n_tiles = cdiv(a.n, kTile);
+    const int columns = a.tail != nullptr ? tile_columns<true>() : tile_columns<false>();
+    p.n_tiles = cdiv(a.n, columns);
     p.splits = a.splits;
     p.blocks = static_cast<int>((a.k + kK - 1) / kK);
     p.per_split = cdiv(p.blocks, a.splits);
@@ -281,10 +366,15 @@ int launch_matmuls(cudaStream_t stream, const MatmulArgs* list, int count, const
     p.b_by_k = a.b.by_k;
     p.out = row_major_seg(a.d, a.n, a.ld_d, 0, 0, a.out_fp32);
     if (a.splits > 1 && a.plane_d % 4 != 0) p.out.vec = 0;
+    if (a.tail != nullptr) {
+      KFB_CHECK_ARG(count == 1 && a.splits == 1 && !a.accumulate && !a.b.by_k && a.n % 8 == 0 && a.ld_d % 8 == 0 && a.plane_d % 8 == 0, "matmul: a tail of %d products, %d pieces, %d columns",
+                    count, a.splits, a.n);
+      batch.tail = *a.tail;
+    }
     p.plane_d = a.plane_d;
     p.accumulate = a.accumulate;
-    KFB_TRY(operand_map(&batch.a[i], a.a, a.m, a.k, a.precise ? 3 : 1));
-    KFB_TRY(operand_map(&batch.b[i], a.b, a.n, a.k, a.precise ? 3 : 1));
+    KFB_TRY(operand_map(&batch.a[i], a.a, a.m, a.k, a.precise ? 3 : 1, kTile));
+    KFB_TRY(operand_map(&batch.b[i], a.b, a.n, a.k, a.precise ? 3 : 1, columns));
     const long long add = static_cast<long long>(p.m_tiles) * p.n_tiles * p.splits;
     KFB_CHECK_ARG(add + blocks < (1ll << 31), "matmul: %lld tiles", add);
     blocks += static_cast<int>(add);
@@ -292,12 +382,21 @@ int launch_matmuls(cudaStream_t stream, const MatmulArgs* list, int count, const
   }
   for (int i = count; i < kMostMatmuls; ++i) batch.end[i] = blocks;
   LaunchScope scope(stream, tag);
+  auto run = [&](auto kernel_of, int smem) { return launch_kernel(stream, kernel_of, blocks, list[0].tail != nullptr ? threads<true>() : threads<false>(), smem, batch); };
   if (list[0].precise) {
-    KFB_TRY(allow_smem<matmul_kernel<3>>(smem_bytes<3>()));
-    return launch_kernel(stream, matmul_kernel<3>, blocks, kThreads, smem_bytes<3>(), batch);
+    if (list[0].tail != nullptr) {
+      KFB_TRY((allow_smem<matmul_kernel<3, true>>(smem_bytes<3>())));
+      return run(matmul_kernel<3, true>, smem_bytes<3>());
+    }
+    KFB_TRY((allow_smem<matmul_kernel<3, false>>(smem_bytes<3>())));
+    return run(matmul_kernel<3, false>, smem_bytes<3>());
   }
-  KFB_TRY(allow_smem<matmul_kernel<1>>(smem_bytes<1>()));
-  return launch_kernel(stream, matmul_kernel<1>, blocks, kThreads, smem_bytes<1>(), batch);
+  if (list[0].tail != nullptr) {
+    KFB_TRY((allow_smem<matmul_kernel<1, true>>(smem_bytes<1>())));
+    return run(matmul_kernel<1, true>, smem_bytes<1>());
+  }
+  KFB_TRY((allow_smem<matmul_kernel<1, false>>(smem_bytes<1>())));
+  return run(matmul_kernel<1, false>, smem_bytes<1>());
 }
 
 int launch_sum_planes(cudaStream_t stream, const PlaneSum* list, int count) {

@@ -16,6 +16,17 @@ struct MatOperand {
   long long plane;
 };
 
+// What becomes of a product z instead of being written as it is (a linear layer's tail, linear_tail.cuh); all products of a launch have one or none.
+struct MatmulTail {
+  int backward;          // 0: d = f(z + bias) + aux;  1: d = aux f'(z + bias), and its sums over rows
+  int act;
+  const float* bias;
+  const void* aux;       // [m][ld_d], may be null in the forward direction
+  int aux_fp32;
+  int parts;             // 3: d is bf16 in three parts, plane_d apart; 1: bf16 or fp32 as out_fp32 says
+  float* partial;        // backward, or null: [4 per 128 rows][n] sums of d before it is rounded
+};
+
 // D[m][n] = sum over k of A(m, k) B(n, k), accumulated in fp32.
 struct MatmulArgs {
   MatOperand a, b;
@@ -28,6 +39,7 @@ struct MatmulArgs {
   long long plane_d;
   int accumulate;        // fp32 D only: add to what D holds
   int precise;           // operands are three bf16 parts each
+  const MatmulTail* tail;
 };
 static constexpr int kMostMatmuls = 3;
 // Up to kMostMatmuls products in one launch, all of them precise or none.

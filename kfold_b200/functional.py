@@ -622,7 +622,7 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     out = x.new_empty(shape, dtype=x.dtype if residual is None else residual.dtype)
     need = _fused_linear_bytes(at, rows, k, n, act, code, L.dtype_code(out.dtype), 0)
     ws = _call_workspace(x.device, need) if need else None
-    xc, wc, b = _operand(x, x.dtype), _operand(w, x.dtype), _affine(bias)
+    xc, wc, b = _operand(x, x.dtype), _operand(w, x.dtype), None if bias is None else _operand(bias, torch.float32)
     rc = None if residual is None else _operand(residual, residual.dtype)
     L.check(L.lib().kfb_fused_linear_fwd(xc.data_ptr(), wc.data_ptr(), L.ptr(b), L.ptr(rc), out.data_ptr(), L.ptr(ws), need, rows, k, n, act, code,
                                          L.dtype_code(out.dtype), L.raw_stream(at)))
@@ -649,7 +649,7 @@ def fused_linear_backward(dy: torch.Tensor, x, w: torch.Tensor, bias: torch.Tens
     dx = dy.new_empty(x.shape, dtype=dt) if need_x else None
     dw = torch.empty(w.shape, dtype=w.dtype, device=dy.device) if need_w else None
     db = torch.empty(bias.shape, dtype=torch.float32, device=dy.device) if need_bias else None
-    dyc, wc, b = _operand(dy, dy.dtype), _operand(w, dt), _affine(bias)
+    dyc, wc, b = _operand(dy, dy.dtype), _operand(w, dt), None if bias is None else _operand(bias, torch.float32)
     xc = _operand(_expanded(x), dt) if need_w or act else None
     need = _fused_linear_bytes(at, rows, k, n, act, code, L.dtype_code(dy.dtype), wanted)
     ws = _call_workspace(dy.device, need) if need else None

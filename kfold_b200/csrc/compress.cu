@@ -1,7 +1,8 @@
 // Rows put away in 8 bits and taken back (the format is in row_teams.cuh).
 //
 // What bounds it: HBM, 2 or 4 bytes a value one way and 33 / 32 the other.  A lane takes eight channels of a row, four lanes a group of 32; rows of any
-// width whose channels are a multiple of eight and lie on 16-byte boundaries go in whole pieces, others a value at a time.
+// width whose channels are a multiple of eight and lie on 16-byte boundaries go in whole pieces, others a value at a time.  Rows of whole groups have no ends: their
+// pieces are numbered through, and a thread has four of them on their way.
 #include "ops_common.cuh"
 #include "row_teams.cuh"
 
@@ -34,24 +35,66 @@ __global__ void __launch_bounds__(256) expand_kernel(const uint8_t* q, const uin
   }
 }
 
+constexpr int kAhead = 4;
+template <typename T>
+__global__ void __launch_bounds__(256) compress_whole_kernel(const T* x, uint8_t* q, uint8_t* e, long long pieces) {
+  grid_dependency_enter();
+  const long long step = 256ll * kAhead;
+  for (long long first = blockIdx.x * step; first < pieces; first += gridDim.x * step) {
+    Pairs v[kAhead];
+    long long i[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      i[k] = first + k * 256 + threadIdx.x;
+      v[k] = load_piece<T, true>(x + i[k] * kPiece, i[k] < pieces ? kPiece : 0);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      store_piece8<true>(q + i[k] * kPiece, e + i[k] / 4, v[k], exponent8(group_top(top_of(v[k]))), i[k] < pieces ? kPiece : 0, threadIdx.x % 4 == 0);
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) expand_whole_kernel(const uint8_t* q, const uint8_t* e, T* x, long long pieces) {
+  grid_dependency_enter();
+  const long long step = 256ll * kAhead;
+  for (long long first = blockIdx.x * step; first < pieces; first += gridDim.x * step) {
+    uint2 b[kAhead];
+    uint32_t ex[kAhead];
+    long long i[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      i[k] = first + k * 256 + threadIdx.x;
+      const bool there = i[k] < pieces;
+      b[k] = there ? *reinterpret_cast<const uint2*>(q + i[k] * kPiece) : make_uint2(0, 0);
+      ex[k] = there ? e[i[k] / 4] : 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) store_piece<true>(x + i[k] * kPiece, values8(b[k], ex[k]), i[k] < pieces ? kPiece : 0);
+  }
+}
+
 template <typename T>
 int compress_as(cudaStream_t s, const void* x, void* q, void* e, long long rows, int c) {
   const long long pieces = rows * groups8(c) * 4;
-  const bool vec = c % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
-  const long long want = (pieces + 255) / 256, most = 16ll * sm_count();
+  const bool vec = c % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0, whole = vec && c % kGroup8 == 0;
+  const long long block = whole ? 256 * kAhead : 256, want = (pieces + block - 1) / block, most = (whole ? 8ll : 16ll) * sm_count();
+  const unsigned blocks = static_cast<unsigned>(want < most ? want : most);
   LaunchScope scope(s, "compress");
-  return launch_kernel(s, vec ? compress_kernel<T, true> : compress_kernel<T, false>, static_cast<unsigned>(want < most ? want : most), 256, 0,
-                       static_cast<const T*>(x), static_cast<uint8_t*>(q), static_cast<uint8_t*>(e), pieces, c, groups8(c));
+  if (whole) return launch_kernel(s, compress_whole_kernel<T>, blocks, 256, 0, static_cast<const T*>(x), static_cast<uint8_t*>(q), static_cast<uint8_t*>(e), pieces);
+  return launch_kernel(s, vec ? compress_kernel<T, true> : compress_kernel<T, false>, blocks, 256, 0, static_cast<const T*>(x), static_cast<uint8_t*>(q),
+                       static_cast<uint8_t*>(e), pieces, c, groups8(c));
 }
 
 template <typename T>
 int expand_as(cudaStream_t s, const void* q, const void* e, void* x, long long rows, int c) {
   const long long pieces = rows * groups8(c) * 4;
-  const bool vec = c % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
-  const long long want = (pieces + 255) / 256, most = 16ll * sm_count();
+  const bool vec = c % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0, whole = vec && c % kGroup8 == 0;
+  const long long block = whole ? 256 * kAhead : 256, want = (pieces + block - 1) / block, most = (whole ? 8ll : 16ll) * sm_count();
+  const unsigned blocks = static_cast<unsigned>(want < most ? want : most);
   LaunchScope scope(s, "expand");
-  return launch_kernel(s, vec ? expand_kernel<T, true> : expand_kernel<T, false>, static_cast<unsigned>(want < most ? want : most), 256, 0,
-                       static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(e), static_cast<T*>(x), pieces, c, groups8(c));
+  if (whole) return launch_kernel(s, expand_whole_kernel<T>, blocks, 256, 0, static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(e), static_cast<T*>(x), pieces);
+  return launch_kernel(s, vec ? expand_kernel<T, true> : expand_kernel<T, false>, blocks, 256, 0, static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(e),
+                       static_cast<T*>(x), pieces, c, groups8(c));
 }
 
 int check(const char* name, const void* a, const void* b, const void* d, long long rows, int c, int dtype) {

@@ -193,7 +193,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       ok = __all_sync(0xffffffffu, ptx::mbar_wait(&acc_full[g], i >> 1 & 1, 707)) != 0;
       if (!ok) break;
       ptx::tc_fence_after_sync();
-#pragma unroll(TAIL == kBackwardTail ? K::kPasses : 1)
+#pragma unroll 1                                      // (unrolled, the code of four passes does not stay in the instruction caches)
       for (int pass = 0; pass < K::kPasses; ++pass, ++at_pass) {
         const int buffer = at_pass & 1, col = pass * 64 + half * 32;
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(&ready[2 * g + buffer], at_pass >> 1 & 1, 706)) != 0;
@@ -216,6 +216,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
             *cell_at(c) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         } else {
+          float mine = 0.f;
           with_activation(p.act, [&](auto act) {
             constexpr int ACT = decltype(act)::value;
 #pragma unroll
@@ -248,7 +249,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
                 for (int q = 0; q < 4; ++q) v[q] = ptx::mul2(x[q], slope<ACT>(v[q]));
                 if (p.partial != nullptr) {
                   const float s = sum_rows8(v, lane);
-                  if ((lane & 3) == c) sums[pass] += s;
+                  if ((lane & 3) == c) mine = s;
                 }
               }
               uint32_t w[4];
@@ -257,6 +258,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
               *cell = make_uint4(w[0], w[1], w[2], w[3]);
             }
           });
+#pragma unroll
+          for (int j = 0; j < K::kPasses; ++j) sums[j] += j == pass ? mine : 0.f;
         }
         ptx::fence_proxy_async_smem();
         __syncwarp();

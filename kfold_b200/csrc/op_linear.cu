@@ -194,11 +194,11 @@ long long piece_rows(long long rows, long long per_row) {
   return rows < most ? rows : most;
 }
 
-// Blocks of 64 rows that a plane of dW takes from a piece: two tiles an SM.
+// Blocks of 64 rows that a plane of dW takes from a piece: two tiles an SM, but eight blocks at least: below that a plane costs more than it saves.
 int blocks_per_plane(long long piece, int k, int n) {
   const long long tiles = static_cast<long long>(cdiv(n, 128)) * cdiv(k, 128), blocks = (piece + 63) / 64, want = 2 * 148 / tiles;
-  const long long s = want < 1 ? 1 : want < blocks ? want : blocks;
-  return static_cast<int>((blocks + s - 1) / s);
+  const long long per = want < 1 ? blocks : (blocks + want - 1) / want;
+  return static_cast<int>(per > 8 ? per : blocks < 8 ? blocks : 8);
 }
 // (a shorter last piece has no more planes than a full one)
 int weight_splits(long long rows, int per) { return static_cast<int>(((rows + 63) / 64 + per - 1) / per); }
@@ -206,7 +206,7 @@ int weight_splits(long long rows, int per) { return static_cast<int>(((rows + 63
 // How a call goes, and its workspace.  wanted: 0 forward, else a sum of 1 dx, 2 dW, 4 db; wide: the result or its gradient is float32 beside bf16.
 struct Plan {
   bool z, again;               // products with a tail: by pairs; at all
-  bool dx, dw, ones;           // dx by pairs, dW by pairs, db by dW's kernel
+  bool dx, dw, ones, whole;    // dx by pairs, dW by pairs, db by dW's kernel, dW in one piece
   long long piece;
   int per_plane, splits;
   __nv_bfloat16 *dz, *x3, *w3;
@@ -230,7 +230,8 @@ Plan plan_of(void* base, long long rows, int k, int n, int act, int precise, int
   if (wanted & 2) {
     p.per_plane = blocks_per_plane(p.piece, k, n);
     p.splits = p.dw ? linear_weights_splits(p.piece, n, k) : weight_splits(p.piece, p.per_plane);
-    p.planes = c.take<float>(static_cast<size_t>(p.splits) * n * k);
+    p.whole = !p.dw && p.splits == 1 && p.piece == rows;
+    if (!p.whole) p.planes = c.take<float>(static_cast<size_t>(p.splits) * n * k);
   }
   if (wanted & 4) {
     const long long lines = p.ones ? p.splits : p.z ? linear_pair_partials(p.piece, n, k) : p.again ? 4 * ((p.piece + 127) / 128) : kMostRowBlocks;
@@ -400,16 +401,16 @@ KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, c
       a.m = n;
       a.n = k;
       a.k = count;
-      a.d = m.planes;
+      a.d = m.whole ? dw : m.planes;
       a.ld_d = k;
-      a.out_fp32 = 1;
+      a.out_fp32 = !m.whole || dw_dtype == KFB_FP32;
       a.splits = weight_splits(count, m.per_plane);
       a.plane_d = nk;
       a.accumulate = r0 > 0;
       a.precise = precise;
     }
     if (products > 0) KFB_TRY(launch_matmuls(s, list, products, "fused_linear_grads"));
-    Sum of_w = {m.planes, m.splits, nk, last ? dw : nullptr, dw_dtype == KFB_FP32, 0, 1};
+    Sum of_w = {m.planes, m.splits, nk, last && !m.whole ? dw : nullptr, dw_dtype == KFB_FP32, 0, 1};
     // (planes of pieces before are in dW's planes; of db's the ones of the last piece hold all, others are a piece's own)
     Sum of_b = {m.partial, lines, n, !m.ones || last ? dbias : nullptr, 1, !m.ones && r0 > 0, 1};
     KFB_TRY(launch_sums(s, of_w, of_b));

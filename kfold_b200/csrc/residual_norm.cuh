@@ -121,8 +121,8 @@ __device__ __forceinline__ Pairs ring_take(const uint4* slot) {
   do {                                                \
     if (vec) {                                        \
       if ((c) <= 64) return CALL(8, 1, true);         \
-      if ((c) <= 128) return CALL(16, 1, true);       \
-      if ((c) <= 256) return CALL(32, 1, true);       \
+      if ((c) <= 128) return CALL(8, 2, true);        \
+      if ((c) <= 256) return CALL(16, 2, true);       \
       if ((c) <= 384) return CALL(16, 3, true);       \
       if ((c) <= 512) return CALL(32, 2, true);       \
       if ((c) <= 768) return CALL(32, 3, true);       \

@@ -37,7 +37,7 @@ constexpr int depth() { return ring_depth(P * 8 * (2 * sizeof(TS) + (OWN ? 4 : 2
 
 // OWN: a row has gates of its own.
 template <typename TS, typename TC, int LANES, int P, bool VEC, bool OWN>
-__global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : 2) residual_norm_grad_kernel(const GradParams p) {
+__global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 ? 3 : 2) residual_norm_grad_kernel(const GradParams p) {
   constexpr int kDepth = depth<TS, TC, P, OWN>(), kC = sizeof(TC) / 2;
   constexpr int kStep = LANES * kPiece;      // channels from a lane's piece to its next
   extern __shared__ uint4 ring_memory[];
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(256) residual_norm_gates_kernel(const float* p
 constexpr int most_blocks(int c) { return c <= 256 ? 6 : c <= 512 ? 3 : 2; }
 constexpr int kMostSms = 160;
 // Pieces of gate rows' samples, at most: two for each team that is at work (row_plan).
-constexpr long long most_units(int c) { return 2ll * kMostSms * most_blocks(c) * (c <= 64 ? 16 : c <= 128 ? 8 : c <= 256 ? 4 : c <= 384 ? 8 : 4); }
+constexpr long long most_units(int c) { return 2ll * kMostSms * most_blocks(c) * (c <= 128 ? 16 : c <= 384 ? 8 : 4); }
 
 struct Sums {
   float *dweight, *dbias, *dscale;

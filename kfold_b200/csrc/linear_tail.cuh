@@ -24,7 +24,11 @@ __device__ __forceinline__ uint64_t each_of(uint64_t v, F f) {
 }
 __device__ __forceinline__ uint64_t magnitude(uint64_t v) { return v & 0x7fffffff7fffffffull; }
 __device__ __forceinline__ uint64_t reciprocal(uint64_t v) {
-  return each_of(v, [](float a) { return __fdividef(1.f, a); });
+  return each_of(v, [](float a) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
+    return r;
+  });
 }
 // 2^v
 __device__ __forceinline__ uint64_t power(uint64_t v) {
@@ -36,21 +40,19 @@ __device__ __forceinline__ uint64_t by_sign(uint64_t z, uint64_t low, uint64_t h
   return ptx::pack2(a.x < 0.f ? l.x : h.x, a.y < 0.f ? l.y : h.y);
 }
 
-// exp(-z^2 / 2), and Phi(z) from it: Phi(-|z|) = exp(-z^2 / 2) t P(t), t = 1 / (1 + 0.30052 |z|), P of degree 7 fitted to erfcx by least squares with weights that level
-// the relative error, 1.2e-7 at most for |z| < 13.4, where exp(-z^2 / 2) ends: Phi keeps its digits where it is small.
-__device__ __forceinline__ uint64_t normal_cdf(uint64_t z, uint64_t& density) {
+// Phi(-|z|) and exp(-z^2 / 2) for gelu = z Phi(z):  Phi(-|z|) = exp(-z^2 / 2) t P(t), t = 1 / (1 + 0.26517 |z|), P of degree 6 fitted to erfcx by least squares with weights
+// that level the relative error, 7e-7 at most for |z| < 13.4, where exp(-z^2 / 2) ends: it keeps its digits where it is small.
+__device__ __forceinline__ uint64_t normal_tail(uint64_t z, uint64_t& density) {
   density = power(ptx::mul2(ptx::mul2(z, z), pair_of(-0.72134752f)));
-  const uint64_t t = reciprocal(ptx::fma2(magnitude(z), pair_of(0.3005204f), pair_of(1.f)));
-  uint64_t p = pair_of(0.036092564f);
-  p = ptx::fma2(p, t, pair_of(-0.15805097f));
-  p = ptx::fma2(p, t, pair_of(0.20634612f));
-  p = ptx::fma2(p, t, pair_of(-0.053961266f));
-  p = ptx::fma2(p, t, pair_of(0.12877955f));
-  p = ptx::fma2(p, t, pair_of(0.099978104f));
-  p = ptx::fma2(p, t, pair_of(0.12098045f));
-  p = ptx::fma2(p, t, pair_of(0.119835384f));
-  const uint64_t low = ptx::mul2(ptx::mul2(p, t), density);
-  return by_sign(z, low, ptx::fma2(low, pair_of(-1.f), pair_of(1.f)));
+  const uint64_t t = reciprocal(ptx::fma2(magnitude(z), pair_of(0.26516503f), pair_of(1.f)));
+  uint64_t p = pair_of(-0.067547895f);
+  p = ptx::fma2(p, t, pair_of(0.19396849f));
+  p = ptx::fma2(p, t, pair_of(-0.064797565f));
+  p = ptx::fma2(p, t, pair_of(0.14152952f));
+  p = ptx::fma2(p, t, pair_of(0.08333303f));
+  p = ptx::fma2(p, t, pair_of(0.107844375f));
+  p = ptx::fma2(p, t, pair_of(0.10566975f));
+  return ptx::mul2(ptx::mul2(p, t), density);
 }
 // sigmoid(z), and its slope from exp(-|z|), so that this stays exact where the gate is open.
 __device__ __forceinline__ uint64_t sigmoid_of(uint64_t z, uint64_t& slope) {
@@ -64,7 +66,10 @@ template <int ACT>
 __device__ __forceinline__ uint64_t activation(uint64_t z) {
   uint64_t other;
   if constexpr (ACT == kRelu) return each_of(z, [](float a) { return a > 0.f || a != a ? a : 0.f; });
-  if constexpr (ACT == kGelu) return ptx::mul2(z, normal_cdf(z, other));
+  if constexpr (ACT == kGelu) {                      // max(z, 0) - |z| Phi(-|z|)
+    const uint64_t low = normal_tail(z, other);
+    return ptx::fma2(magnitude(z) | 0x8000000080000000ull, low, each_of(z, [](float a) { return fmaxf(a, 0.f); }));
+  }
   if constexpr (ACT == kSigmoid) return sigmoid_of(z, other);
   if constexpr (ACT == kSilu) return ptx::mul2(z, sigmoid_of(z, other));
   return z;
@@ -74,8 +79,9 @@ __device__ __forceinline__ uint64_t slope(uint64_t z) {
   uint64_t other;
   if constexpr (ACT == kRelu) return each_of(z, [](float a) { return a > 0.f ? 1.f : 0.f; });
   if constexpr (ACT == kGelu) {
-    const uint64_t cdf = normal_cdf(z, other);
-    return ptx::fma2(ptx::mul2(z, pair_of(0.39894228f)), other, cdf);
+    const uint64_t low = normal_tail(z, other);      // at -|z|: Phi - |z| phi; the slope at |z| is one less that
+    const uint64_t v = ptx::fma2(ptx::mul2(magnitude(z), pair_of(-0.39894228f)), other, low);
+    return by_sign(z, v, ptx::fma2(v, pair_of(-1.f), pair_of(1.f)));
   }
   if constexpr (ACT == kSigmoid) {
     sigmoid_of(z, other);
@@ -141,9 +147,10 @@ int linear_pair_partials(long long rows, int n, int k);       // rows of partial
 int launch_linear_pair(cudaStream_t stream, const LinearPair& p, const char* tag);
 
 // dW planes: plane[s][n][k] = sum over a piece of the rows of dz^T x (linear_weights.cu).
-// bias_planes: null, or [s][n] sums of dz over the same pieces.
+// bias_planes: null, or [linear_weights_bias_planes][n] sums of dz, over rows that are divided between them.
 bool linear_weights_ok(long long rows, int n, int k);
 int linear_weights_splits(long long rows, int n, int k);
+int linear_weights_bias_planes(int splits, int k);
 int launch_linear_weights(cudaStream_t stream, const void* dz, const void* x, float* planes, float* bias_planes, int splits, int add, long long rows, int n,
                           int k);
 

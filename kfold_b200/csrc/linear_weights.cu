@@ -59,7 +59,10 @@ linear_weights_kernel(const __grid_constant__ CUtensorMap tm_dz, const __grid_co
     ptx::mbar_init(done, 1);
     ptx::fence_barrier_init();
   }
-  const bool bias = p.bias_planes != nullptr && k0 == 0;
+  // (the tiles that share these columns of dz share this work: a block of rows is one's)
+  const bool bias = p.bias_planes != nullptr;
+  const int k_tiles = p.tiles / p.n_tiles, turn = tile / p.n_tiles;
+  int first_bias = b0 + (turn - b0 % k_tiles + k_tiles) % k_tiles;      // the first block of this tile's
   for (int i = threadIdx.x; i < kOnes / 4; i += kThreads) reinterpret_cast<uint32_t*>(ones)[i] = 0x3f803f80u;
   ptx::fence_proxy_async_smem();
   if (warp == 1) {
@@ -111,9 +114,9 @@ linear_weights_kernel(const __grid_constant__ CUtensorMap tm_dz, const __grid_co
         const uint64_t a = d0 + st * (kStage >> 4), x = a + (kOperand >> 4);
 #pragma unroll
         for (int k = 0; k < 4; ++k) ptx::mma_f16_ss_pair(tmem, a + k * (2048 >> 4), x + k * (2048 >> 4), idesc, b > b0 || k > 0 ? 1u : 0u);
-        if (bias) {
+        if (bias && b % k_tiles == turn) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) ptx::mma_f16_ss_pair(tmem + kTile, a + k * (2048 >> 4), ones_desc, ones_idesc, b > b0 || k > 0 ? 1u : 0u);
+          for (int k = 0; k < 4; ++k) ptx::mma_f16_ss_pair(tmem + kTile, a + k * (2048 >> 4), ones_desc, ones_idesc, b > first_bias || k > 0 ? 1u : 0u);
         }
         ptx::tc_commit_pair(&empty[st]);
         if (++st == kStages) { st = 0; ph ^= 1u; }
@@ -132,8 +135,8 @@ linear_weights_kernel(const __grid_constant__ CUtensorMap tm_dz, const __grid_co
         ptx::tmem_ld_32x32b_x8(t_row + kTile, v);
         ptx::tmem_ld_wait();
         if (n < p.n) {
-          float* d = p.bias_planes + static_cast<long long>(split) * p.n + n;
-          *d = __uint_as_float(v[0]) + (p.add ? *d : 0.f);
+          float* d = p.bias_planes + (static_cast<long long>(split) * k_tiles + turn) * p.n + n;
+          *d = (first_bias < b1 ? __uint_as_float(v[0]) : 0.f) + (p.add ? *d : 0.f);
         }
       }
       float* d = p.planes + (static_cast<long long>(split) * p.n + n) * p.k + k0;
@@ -189,6 +192,8 @@ int tiles_of(int n, int k) { return cdiv(n, kTile) * cdiv(k, kTile); }
 
 // Many rows: below some thousand a pair's start and end, and the planes, cost more than tiles of 128 x 128 do (matmul.cu).
 bool linear_weights_ok(long long rows, int n, int k) { return rows >= 4096 && n >= 256 && k >= 256 && tiles_of(n, k) <= pairs_held(); }
+
+int linear_weights_bias_planes(int splits, int k) { return splits * cdiv(k, kTile); }
 
 int linear_weights_splits(long long rows, int n, int k) {
   const long long blocks = (rows + kK - 1) / kK, most = pairs_held() / tiles_of(n, k);

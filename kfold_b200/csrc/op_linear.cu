@@ -234,7 +234,7 @@ Plan plan_of(void* base, long long rows, int k, int n, int act, int precise, int
     if (!p.whole) p.planes = c.take<float>(static_cast<size_t>(p.splits) * n * k);
   }
   if (wanted & 4) {
-    const long long lines = p.ones ? p.splits : p.z ? linear_pair_partials(p.piece, n, k) : p.again ? 4 * ((p.piece + 127) / 128) : kMostRowBlocks;
+    const long long lines = p.ones ? linear_weights_bias_planes(p.splits, k) : p.z ? linear_pair_partials(p.piece, n, k) : p.again ? 4 * ((p.piece + 127) / 128) : kMostRowBlocks;
     p.partial = c.take<float>(static_cast<size_t>(lines) * n);
   }
   p.bytes = c.off;
@@ -391,7 +391,7 @@ KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, c
     }
     if (dw != nullptr && m.dw) {
       KFB_TRY(launch_linear_weights(s, dz.ptr, xp, m.planes, m.ones ? m.partial : nullptr, m.splits, r0 > 0 ? 1 : 0, count, n, k));
-      if (m.ones) lines = m.splits;
+      if (m.ones) lines = linear_weights_bias_planes(m.splits, k);
     } else if (dw != nullptr) {
       MatmulArgs& a = list[products++];
       a.a = dz;

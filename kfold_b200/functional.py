@@ -103,8 +103,8 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
 
 def _dense_like(x: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
     """A dense tensor of x's shape, of `dtype` or x's.  (empty_like costs the host 1.4 us where empty with its arguments costs 3.3.)"""
-    if x.is_contiguous() and (dtype is None or dtype == x.dtype):
-        return torch.empty_like(x)
+    if x.is_contiguous():
+        return torch.empty_like(x) if dtype is None or dtype == x.dtype else torch.empty_like(x, dtype=dtype)
     return torch.empty(x.shape, dtype=dtype or x.dtype, device=x.device)
 
 
@@ -378,8 +378,9 @@ class Compressed:
 def _room8(x: torch.Tensor) -> Compressed:
     """Room for x's rows in 8 bits."""
     c = Compressed.__new__(Compressed)
-    c.values = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    c.exponents = torch.empty((*x.shape[:-1], (x.shape[-1] + _GROUP8 - 1) // _GROUP8), dtype=torch.uint8, device=x.device)
+    shape = x.shape
+    c.values = _dense_like(x, torch.int8)
+    c.exponents = x.new_empty((*shape[:-1], (shape[-1] + _GROUP8 - 1) // _GROUP8), dtype=torch.uint8)
     c.dtype = x.dtype
     return c
 
@@ -429,35 +430,46 @@ class ResidualNormGradients(NamedTuple):
     gate_shift: torch.Tensor | None
 
 
-def _stream_operands(name: str, shape, stream: torch.dtype, compute: torch.dtype, u, gate, gate_shift, samples: int, vectors) -> tuple:
-    """(rows, channels, tokens; dtype codes of the stream and of what the blocks compute in; gate, its row stride, gate_shift, its row stride)."""
+@lru_cache(maxsize=1024)
+def _stream_sizes(name: str, shape, stream: torch.dtype, compute: torch.dtype, u, gate, gate_shift, samples: int) -> tuple:
+    """(rows, channels, tokens; dtype codes of the stream and of what the blocks compute in) for tensors of these shapes, u, gate and gate_shift with their types."""
     c = shape[-1] if shape else 0
     if not c:
         raise ValueError(f"{name}: rows of shape {tuple(shape)}")
     rows = math.prod(shape[:-1])
     if (stream, compute) not in _STREAM_CODES:
         raise ValueError(f"{name}: a stream of {stream} with {compute} (bfloat16, float32, or float32 with bfloat16)")
-    for t in vectors:
-        if t is not None and t.numel() != c:
-            raise ValueError(f"{name}: {tuple(t.shape)} for {c} channels")
-    if u is not None and (u.shape != shape or u.dtype != compute):
-        raise ValueError(f"{name}: u {u.dtype} {tuple(u.shape)} for rows {tuple(shape)} computed in {compute}")
+    if u is not None and u != (shape, compute):
+        raise ValueError(f"{name}: u {u[1]} {tuple(u[0])} for rows {tuple(shape)} computed in {compute}")
     tokens = 1
     if samples != 1:
         if len(shape) < 2 or samples < 1 or (rows and rows % (samples * shape[-2])):
             raise ValueError(f"{name}: {samples} samples share gates in rows {tuple(shape)}")
         tokens = shape[-2] or 1
-    gate_ld = shift_ld = 0
-    if gate is not None:
-        if gate.shape[-1:] != (c,) or gate.numel() * samples != rows * c or gate.dtype != compute:
-            raise ValueError(f"{name}: gate {gate.dtype} {tuple(gate.shape)} for rows {tuple(shape)} of {compute}, of which {samples} entries share")
-        gate, _, gate_ld = _rows(gate, c)
-    if gate_shift is not None:
-        if gate_shift.shape[-1:] != (2 * c,) or gate_shift.numel() * samples != 2 * rows * c or gate_shift.dtype != compute:
-            raise ValueError(f"{name}: gate_shift {gate_shift.dtype} {tuple(gate_shift.shape)} for rows {tuple(shape)} of {compute}, of which {samples} "
-                             "entries share")
-        gate_shift, _, shift_ld = _rows(gate_shift, 2 * c)
-    return rows, c, tokens, *_STREAM_CODES[stream, compute], gate, gate_ld, gate_shift, shift_ld
+    for what, t, width in (("gate", gate, c), ("gate_shift", gate_shift, 2 * c)):
+        if t is not None and (t[0][-1:] != (width,) or math.prod(t[0]) * samples != rows * width or t[1] != compute):
+            raise ValueError(f"{name}: {what} {t[1]} {tuple(t[0])} for rows {tuple(shape)} of {compute}, of which {samples} entries share")
+    return rows, c, tokens, *_STREAM_CODES[stream, compute]
+
+
+def _of(t) -> tuple | None:
+    return None if t is None else (t.shape, t.dtype)
+
+
+def _table(t: torch.Tensor | None, c: int) -> tuple:
+    """(gate rows as the kernels read them, elements from one to the next)."""
+    if t is None:
+        return None, 0
+    if t.is_contiguous() and not t.data_ptr() & 15:
+        return t, c
+    t, _, ld = _rows(t, c)
+    return t, ld
+
+
+def _vector_of(name: str, c: int, *ts: torch.Tensor | None) -> None:
+    for t in ts:
+        if t is not None and t.numel() != c:
+            raise ValueError(f"{name}: {tuple(t.shape)} for {c} channels")
 
 
 _STREAM_CODES = {(torch.bfloat16, torch.bfloat16): (L.KFB_BF16, L.KFB_BF16), (torch.float32, torch.float32): (L.KFB_FP32, L.KFB_FP32),
@@ -490,9 +502,10 @@ def residual_norm(x: torch.Tensor | None, u: torch.Tensor | None = None, gate: t
     if (gate is not None and u is None) or (scale is not None and x is None) or (gate_shift is not None and (weight is not None or bias is not None)) or (
             not norm and (weight is not None or bias is not None or gate_shift is not None)):
         raise ValueError("residual_norm: a gate needs u, a scale x, parameters of the norm the norm, and gate_shift stands in for weight and bias")
-    shape = base.shape
-    rows, c, tokens, st, ct, gate, gate_ld, gs, gs_ld = _stream_operands("residual_norm", shape, base.dtype, compute, u, gate, gate_shift, samples,
-                                                                         (scale, weight, bias))
+    rows, c, tokens, st, ct = _stream_sizes("residual_norm", base.shape, base.dtype, compute, _of(u), _of(gate), _of(gate_shift), samples)
+    if scale is not None or weight is not None or bias is not None:
+        _vector_of("residual_norm", c, scale, weight, bias)
+    (gate, gate_ld), (gs, gs_ld) = _table(gate, c), _table(gate_shift, 2 * c)
     xc, uc = None if x is None else _dense(x), None if u is None else _dense(u)
     r = x if u is None and scale is None else _dense_like(base)
     y = _dense_like(base, compute) if norm else None
@@ -541,8 +554,10 @@ def residual_norm_backward(dr: torch.Tensor | None, dy: torch.Tensor | None, r, 
     compute = u.dtype if u is not None else gate.dtype if gate is not None else first.dtype
     if dy is None:                                   # the norm has no part in it
         weight = gate_shift = None
-    gate_shape, shift_shape = None if gate is None else gate.shape, None if gate_shift is None else gate_shift.shape
-    rows, c, tokens, st, ct, gate, gate_ld, gs, gs_ld = _stream_operands(name, shape, stream, compute, u, gate, gate_shift, samples, (scale, weight))
+    rows, c, tokens, st, ct = _stream_sizes(name, shape, stream, compute, _of(u), _of(gate), _of(gate_shift), samples)
+    if scale is not None or weight is not None:
+        _vector_of(name, c, scale, weight)
+    (gt, gate_ld), (gs, gs_ld) = _table(gate, c), _table(gate_shift, 2 * c)
     if (dr is not None and (dr.shape != shape or dr.dtype != stream)) or (dy is not None and (dy.shape != shape or dy.dtype != compute)) or (
             x is not None and (x.shape != shape or x.dtype != stream)):
         raise ValueError(f"{name}: dr {None if dr is None else (dr.dtype, tuple(dr.shape))}, dy {None if dy is None else (dy.dtype, tuple(dy.shape))}, x "
@@ -556,14 +571,16 @@ def residual_norm_backward(dr: torch.Tensor | None, dy: torch.Tensor | None, r, 
     affine = dy is not None and gs is None
     need_weight, need_bias = need_weight and affine and weight is not None, need_bias and affine
     need_gate_shift = need_gate_shift and gs is not None
-    like = first.new_empty
     one = need_u and gate is None and scale is None and stream == compute         # du is dx
-    dx = like(shape, dtype=stream) if need_x or one else None
-    du = dx if one else like(shape, dtype=compute) if need_u else None
-    dgate = like(gate_shape, dtype=compute) if need_gate else None
-    dgs = like(shift_shape, dtype=compute) if need_gate_shift else None
-    vector = lambda need, t: torch.empty(c if t is None else t.shape, dtype=torch.float32, device=first.device) if need else None
-    dw, db, dscale = vector(need_weight, weight), vector(need_bias, weight), vector(need_scale, scale)
+    dx = _dense_like(first, stream) if need_x or one else None
+    du = dx if one else _dense_like(first, compute) if need_u else None
+    dgate = _dense_like(gate) if need_gate else None
+    dgs = _dense_like(gate_shift) if need_gate_shift else None
+    dw = _dense_like(weight, torch.float32) if need_weight else None
+    db = None
+    if need_bias:
+        db = _dense_like(weight, torch.float32) if weight is not None else torch.empty(c, dtype=torch.float32, device=first.device)
+    dscale = _dense_like(scale, torch.float32) if need_scale else None
     lib = L.lib()
     ws, size = None, 0
     sums, gates = need_weight or need_bias or need_scale, samples > 1 and (need_gate or need_gate_shift)
@@ -573,7 +590,7 @@ def residual_norm_backward(dr: torch.Tensor | None, dy: torch.Tensor | None, r, 
     drc, dyc = None if dr is None else _dense(dr), None if dy is None else _dense(dy)
     (rp, re, rk), (up, ue, uk), (xp, xe, xk) = _kept_or_dense(r), _kept_or_dense(u if need_gate else None), _kept_or_dense(x if need_scale else None)
     sc, w = _affine(scale), _affine(weight)
-    L.check(lib.kfb_residual_norm_bwd(L.ptr(drc), L.ptr(dyc), rp, re, up, ue, xp, xe, L.ptr(gate), gate_ld, L.ptr(sc), L.ptr(w), L.ptr(gs), gs_ld, L.ptr(dx),
+    L.check(lib.kfb_residual_norm_bwd(L.ptr(drc), L.ptr(dyc), rp, re, up, ue, xp, xe, L.ptr(gt), gate_ld, L.ptr(sc), L.ptr(w), L.ptr(gs), gs_ld, L.ptr(dx),
                                       None if one else L.ptr(du), L.ptr(dgate), L.ptr(dgs), L.ptr(dw), L.ptr(db), L.ptr(dscale), L.ptr(ws), size, rows, c,
                                       samples, tokens, eps, _NO_NORM if dy is None else _AFFINE_NORM if gs is None else _ADAPTIVE_NORM, st, ct,
                                       L.raw_stream(at)))
@@ -619,7 +636,7 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     shape = (*x.shape[:-1], n)
     if residual is not None and (residual.shape != shape or (residual.dtype != x.dtype and residual.dtype != torch.float32)):
         raise ValueError(f"fused_linear: residual {residual.dtype} {tuple(residual.shape)} for x {x.dtype} {tuple(x.shape)} and {n} channels")
-    out = x.new_empty(shape, dtype=x.dtype if residual is None else residual.dtype)
+    out = x.new_empty(shape) if residual is None else _dense_like(residual)
     need = _fused_linear_bytes(at, rows, k, n, act, code, L.dtype_code(out.dtype), 0)
     ws = _call_workspace(x.device, need) if need else None
     xc, wc, b = _operand(x, x.dtype), _operand(w, x.dtype), None if bias is None else _operand(bias, torch.float32)
@@ -646,9 +663,11 @@ def fused_linear_backward(dy: torch.Tensor, x, w: torch.Tensor, bias: torch.Tens
     if not wanted:
         return None, None, None
     dt = x.dtype
-    dx = dy.new_empty(x.shape, dtype=dt) if need_x else None
-    dw = torch.empty(w.shape, dtype=w.dtype, device=dy.device) if need_w else None
-    db = torch.empty(bias.shape, dtype=torch.float32, device=dy.device) if need_bias else None
+    dx = None
+    if need_x:
+        dx = dy.new_empty(x.shape, dtype=dt) if type(x) is Compressed else _dense_like(x)
+    dw = _dense_like(w) if need_w else None
+    db = _dense_like(bias, torch.float32) if need_bias else None
     dyc, wc, b = _operand(dy, dy.dtype), _operand(w, dt), None if bias is None else _operand(bias, torch.float32)
     xc = _operand(_expanded(x), dt) if need_w or act else None
     need = _fused_linear_bytes(at, rows, k, n, act, code, L.dtype_code(dy.dtype), wanted)

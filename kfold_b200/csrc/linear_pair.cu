@@ -28,9 +28,9 @@ struct Cfg {
   static constexpr int kBStage = kBBoxes * kRowsBox, kStage = kBox + kBStage;
   static constexpr int kBBytes = BN / 2 * 128;       // along k: what comes
   static constexpr int kPasses = BN / 64;            // a group has 64 columns in a buffer at a time, of which a warp has 32
-  static constexpr int kFit = (232448 - 1536 - 4 * kBox) / kStage, kStages = kFit < 6 ? kFit : 6;
+  static constexpr int kFit = (232448 - 1536 - BN * 4 - 4 * kBox) / kStage, kStages = kFit < 6 ? kFit : 6;
   static constexpr int kTmem = BN == 128 ? 256 : 512;
-  static constexpr int kSmem = kStages * kStage + 4 * kBox + 512 + 1024;
+  static constexpr int kSmem = kStages * kStage + 4 * kBox + BN * 4 + 512 + 1024;
   static_assert(BN % 64 == 0 && kStages >= 3, "tiles of 128, 192 or 256 columns");
   static_assert(kSmem <= 232448, "shared memory");
 };
@@ -42,6 +42,9 @@ struct PairParams {
   float* partial;
 };
 
+// The warps of both groups.
+__device__ __forceinline__ void tail_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(64 * kGroupWarps) : "memory"); }
+
 template <int BN, int TAIL, bool BY_K>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_aux,
@@ -50,7 +53,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* tiles = ring + K::kStages * K::kStage;
-  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + 4 * kBox);          // in the leader: both CTAs' copies
+  float* s_bias = reinterpret_cast<float*>(tiles + 4 * kBox);              // of the tile's columns
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_bias + BN);               // in the leader: both CTAs' copies
   uint64_t* empty = full + K::kStages;
   uint64_t* acc_full = empty + K::kStages;           // [2]
   uint64_t* acc_empty = acc_full + 2;                // [2], in the leader: the group's warps in both CTAs
@@ -187,6 +191,10 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     float sums[K::kPasses];                          // of column 8 (lane & 3) + what sum_rows8 gives, of each pass
 #pragma unroll
     for (int j = 0; j < K::kPasses; ++j) sums[j] = 0.f;
+    if constexpr (TAIL != kPlainTail) {
+      for (int c = threadIdx.x - 32 * kTailWarp; c < BN; c += 64 * kGroupWarps) s_bias[c] = p.bias != nullptr && n0 + c < p.n ? p.bias[n0 + c] : 0.f;
+      tail_barrier();
+    }
     bool ok = true;
     int at_pass = 0;
     for (int i = g; ok && i < my_tiles; i += 2) {
@@ -221,15 +229,12 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
             constexpr int ACT = decltype(act)::value;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              const int at = n0 + col + 8 * c;
               uint64_t v[4], x[4];
 #pragma unroll
               for (int q = 0; q < 4; ++q) v[q] = ptx::pack2(raw[8 * c + 2 * q], raw[8 * c + 2 * q + 1]);
-              if (p.bias != nullptr && at < p.n) {          // (n is a multiple of 8)
-                const ulonglong2* b = reinterpret_cast<const ulonglong2*>(p.bias + at);
-                const ulonglong2 lo = b[0], hi = b[1];
-                v[0] = ptx::add2(v[0], lo.x), v[1] = ptx::add2(v[1], lo.y), v[2] = ptx::add2(v[2], hi.x), v[3] = ptx::add2(v[3], hi.y);
-              }
+              const ulonglong2* b = reinterpret_cast<const ulonglong2*>(s_bias + col + 8 * c);
+              const ulonglong2 lo = b[0], hi = b[1];
+              v[0] = ptx::add2(v[0], lo.x), v[1] = ptx::add2(v[1], lo.y), v[2] = ptx::add2(v[2], hi.x), v[3] = ptx::add2(v[3], hi.y);
               uint4* cell = cell_at(c);
               if (TAIL == kBackwardTail || p.has_aux) {
                 const uint4 a = *cell;
@@ -267,12 +272,19 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       }
     }
     if (TAIL == kBackwardTail && p.partial != nullptr) {
-      // a row of partial sums for each pair of a column tile, group, CTA and quadrant
-      float* row = p.partial + static_cast<long long>(((first * 2 + g) * 2 + rank) * 4 + quad) * p.n;
+      // a row of partial sums for each CTA of a column tile: its warps' through the ring, whose operands the last product has read
+      float* warps = reinterpret_cast<float*>(ring);      // [group, quadrant][BN]
+      tail_barrier();
 #pragma unroll
-      for (int j = 0; j < K::kPasses; ++j) {
-        const int at = n0 + j * 64 + half * 32 + 8 * (lane & 3) + 4 * (lane >> 4 & 1) + 2 * (lane >> 3 & 1) + (lane >> 2 & 1);
-        if (at < p.n) row[at] = sums[j];
+      for (int j = 0; j < K::kPasses; ++j)
+        warps[(g * 4 + quad) * BN + j * 64 + half * 32 + 8 * (lane & 3) + 4 * (lane >> 4 & 1) + 2 * (lane >> 3 & 1) + (lane >> 2 & 1)] = sums[j];
+      tail_barrier();
+      const int c = threadIdx.x - 32 * kTailWarp;
+      if (c < BN && n0 + c < p.n) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s += warps[w * BN + c];
+        p.partial[static_cast<long long>(first * 2 + rank) * p.n + n0 + c] = s;
       }
     }
   }
@@ -375,7 +387,7 @@ bool linear_pair_ok(long long rows, int n, int k) {
   return g.groups > 0 && 4 * g.groups * g.n_tiles >= 3 * held;      // (three quarters of the pairs at least have a tile)
 }
 
-int linear_pair_partials(long long rows, int n, int k) { return grid_of(rows, n, backward_pairs(n)).groups * 16; }
+int linear_pair_partials(long long rows, int n, int k) { return grid_of(rows, n, backward_pairs(n)).groups * 2; }
 
 int launch_linear_pair(cudaStream_t stream, const LinearPair& p, const char* tag) {
   KFB_CHECK_ARG((p.tail == kPlainTail) == (p.by_k != 0), "linear: tail %d with an operand %s k", p.tail, p.by_k ? "across" : "along");

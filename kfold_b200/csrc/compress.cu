@@ -1,36 +1,42 @@
 // Rows put away in 8 bits and taken back (the format is in row_teams.cuh).
 //
-// What bounds it: HBM, 2 or 4 bytes a value one way and 33 / 32 the other.  A lane takes eight channels of a row, four lanes a group of 32; rows of any
-// width whose channels are a multiple of eight and lie on 16-byte boundaries go in whole pieces, others a value at a time.  Rows of whole groups have no ends: their
-// pieces are numbered through, and a thread has four of them on their way.
+// What bounds it: HBM, 2 or 4 bytes a value one way and 33 / 32 the other.  A lane takes eight neighbouring channels of a row where they are a multiple of eight and lie
+// on 16-byte boundaries, four lanes then hold a group of 32; else every 32nd channel, a group being a warp's.  Rows of whole groups have no ends: their pieces are
+// numbered through, and a thread has four of them on their way.
 #include "ops_common.cuh"
 #include "row_teams.cuh"
 
 namespace kfb {
 namespace {
 
-// Pieces of eight channels, four to a group of 32: rows of `groups` groups, pieces numbered through.
+// Rows of `groups` groups of 32.  VEC: four pieces of eight neighbouring channels a group, numbered through.  Otherwise pieces of eight groups, a warp's: a lane has
+// every 32nd channel.
+template <bool VEC>
+__device__ __forceinline__ long long pieces_of_row(int groups) { return VEC ? 4ll * groups : (groups + kPiece - 1) / kPiece * 32ll; }
+// (first channel of a lane's piece number i of a row)
+template <bool VEC>
+__device__ __forceinline__ int first_channel(int i) { return VEC ? i * kPiece : i / 32 * (32 * kPiece) + i % 32; }
+
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) compress_kernel(const T* x, uint8_t* q, uint8_t* e, long long pieces, int c, int groups) {
+__global__ void __launch_bounds__(256) compress_kernel(const T* x, uint8_t* q, uint8_t* e, long long rows, int c, int groups) {
   grid_dependency_enter();
-  const long long per_row = 4ll * groups;
+  const long long per_row = pieces_of_row<VEC>(groups), pieces = rows * per_row;
   // (a warp's lanes leave the loop together: pieces beyond the end have no values)
   for (long long first = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x / 32 * 32; first < pieces; first += gridDim.x * 256ll) {
     const long long i = first + threadIdx.x % 32, row = i / per_row;
-    const int ch = static_cast<int>(i - row * per_row) * kPiece, n = i < pieces ? min(max(c - ch, 0), kPiece) : 0;
+    const int ch = first_channel<VEC>(static_cast<int>(i - row * per_row)), n = i < pieces ? channels_of<VEC>(c, ch) : 0;
     const Pairs v = load_piece<T, VEC>(x + row * c + ch, n);
-    const uint32_t e_here = exponent8(group_top(top_of(v)));
-    store_piece8<VEC>(q + row * c + ch, e + row * groups + ch / kGroup8, v, e_here, n, threadIdx.x % 4 == 0);
+    store_piece8<VEC>(q + row * c + ch, e + row * groups + ch / kGroup8, v, top_of(v), n, threadIdx.x % 32);
   }
 }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) expand_kernel(const uint8_t* q, const uint8_t* e, T* x, long long pieces, int c, int groups) {
+__global__ void __launch_bounds__(256) expand_kernel(const uint8_t* q, const uint8_t* e, T* x, long long rows, int c, int groups) {
   grid_dependency_enter();
-  const long long per_row = 4ll * groups;
+  const long long per_row = pieces_of_row<VEC>(groups), pieces = rows * per_row;
   for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < pieces; i += gridDim.x * 256ll) {
     const long long row = i / per_row;
-    const int ch = static_cast<int>(i - row * per_row) * kPiece, n = min(max(c - ch, 0), kPiece);
+    const int ch = first_channel<VEC>(static_cast<int>(i - row * per_row)), n = channels_of<VEC>(c, ch);
     store_piece<VEC>(x + row * c + ch, load_piece8<VEC>(q + row * c + ch, e + row * groups + ch / kGroup8, n), n);
   }
 }
@@ -50,7 +56,7 @@ __global__ void __launch_bounds__(256) compress_whole_kernel(const T* x, uint8_t
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      store_piece8<true>(q + i[k] * kPiece, e + i[k] / 4, v[k], exponent8(group_top(top_of(v[k]))), i[k] < pieces ? kPiece : 0, threadIdx.x % 4 == 0);
+      store_piece8<true>(q + i[k] * kPiece, e + i[k] / 4, v[k], top_of(v[k]), i[k] < pieces ? kPiece : 0, threadIdx.x % 32);
   }
 }
 template <typename T>
@@ -82,7 +88,7 @@ int compress_as(cudaStream_t s, const void* x, void* q, void* e, long long rows,
   LaunchScope scope(s, "compress");
   if (whole) return launch_kernel(s, compress_whole_kernel<T>, blocks, 256, 0, static_cast<const T*>(x), static_cast<uint8_t*>(q), static_cast<uint8_t*>(e), pieces);
   return launch_kernel(s, vec ? compress_kernel<T, true> : compress_kernel<T, false>, blocks, 256, 0, static_cast<const T*>(x), static_cast<uint8_t*>(q),
-                       static_cast<uint8_t*>(e), pieces, c, groups8(c));
+                       static_cast<uint8_t*>(e), rows, c, groups8(c));
 }
 
 template <typename T>
@@ -94,7 +100,7 @@ int expand_as(cudaStream_t s, const void* q, const void* e, void* x, long long r
   LaunchScope scope(s, "expand");
   if (whole) return launch_kernel(s, expand_whole_kernel<T>, blocks, 256, 0, static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(e), static_cast<T*>(x), pieces);
   return launch_kernel(s, vec ? expand_kernel<T, true> : expand_kernel<T, false>, blocks, 256, 0, static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(e),
-                       static_cast<T*>(x), pieces, c, groups8(c));
+                       static_cast<T*>(x), rows, c, groups8(c));
 }
 
 int check(const char* name, const void* a, const void* b, const void* d, long long rows, int c, int dtype) {

@@ -24,36 +24,36 @@ struct Params {
 };
 
 template <typename TS, typename TC, int P, bool OWN>
-constexpr int depth() { return ring_depth(P * 8 * (sizeof(TS) + (OWN ? 4 : 1) * sizeof(TC))); }
+constexpr int depth() { return ring_depth(P * 8 * (sizeof(TS) + (OWN ? 4 : 1) * sizeof(TC)), OWN ? 3 : 2); }
 
-template <typename TS, typename TC, int LANES, int P, bool VEC, bool OWN>
+template <typename TS, typename TC, int LANES, int P, bool VEC, int GATES>
 __global__ void __launch_bounds__(kRowThreads) residual_norm_kernel(const Params p) {
+  constexpr bool OWN = GATES != kSharedGates, kVectors = GATES != kOwnAdaptive;
   constexpr int kDepth = depth<TS, TC, P, OWN>(), kC = sizeof(TC) / 2;
   constexpr int kStep = LANES * kPiece;      // channels from a lane's piece to its next
   extern __shared__ uint4 ring_memory[];
   grid_dependency_enter();
-  const int warp = threadIdx.x / 32, ch = threadIdx.x % LANES * kPiece, team = threadIdx.x % 32 / LANES;
+  const int warp = threadIdx.x / 32, ch = threadIdx.x % LANES * (VEC ? kPiece : 1), team = threadIdx.x % 32 / LANES;
   const float inv_c = 1.0f / static_cast<float>(p.c);
   const TS* x = static_cast<const TS*>(p.x) + ch;
   const TC *u = static_cast<const TC*>(p.u) + ch, *gate = static_cast<const TC*>(p.gate) + ch, *gs = static_cast<const TC*>(p.gate_shift) + ch;
-  const bool has_x = p.x != nullptr, has_u = p.u != nullptr, gated = p.gate != nullptr, adaptive = p.gate_shift != nullptr;
+  const bool has_x = p.x != nullptr, has_u = p.u != nullptr, gated = p.gate != nullptr, adaptive = GATES == kOwnAdaptive || (GATES == kSharedGates && p.gate_shift != nullptr);
   const uint4* ring = ring_memory + threadIdx.x;
   const uint32_t ring_at = ptx::smem_u32(ring);
   int inside[P];                             // channels of a piece
 #pragma unroll
-  for (int q = 0; q < P; ++q) inside[q] = min(max(p.c - ch - q * kStep, 0), kPiece);
+  for (int q = 0; q < P; ++q) inside[q] = channels_of<VEC>(p.c, ch + q * kStep);
   auto vector = [&](const float* v, int q, float other) {
     float f[kPiece];
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) f[i] = v != nullptr && i < inside[q] ? v[ch + q * kStep + i] : other;
+    for (int i = 0; i < kPiece; ++i) f[i] = v != nullptr && i < inside[q] ? v[ch + q * kStep + i * channel_step<VEC>()] : other;
     return of_floats(f);
   };
 
-  Pairs m[P], shift[P], open[OWN ? 1 : P];
+  Pairs m[kVectors ? P : 1], shift[kVectors ? P : 1], open[OWN ? 1 : P];
 #pragma unroll
   for (int q = 0; q < P; ++q) {
-    m[q] = vector(p.weight, q, 1.f);
-    shift[q] = vector(p.bias, q, 0.f);
+    if (kVectors) m[kVectors ? q : 0] = vector(p.weight, q, 1.f), shift[kVectors ? q : 0] = vector(p.bias, q, 0.f);
     if (!OWN) open[OWN ? 0 : q] = both(1.f);
   }
 
@@ -111,8 +111,8 @@ __global__ void __launch_bounds__(kRowThreads) residual_norm_kernel(const Params
       if (adaptive) {
 #pragma unroll
         for (int q = 0; q < P; ++q) {
-          m[q] = each(load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + q * kStep, k[q]), [](float a) { return open_of(gate_at(a)); });
-          shift[q] = load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + p.c + q * kStep, k[q]);
+          m[kVectors ? q : 0] = each(load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + q * kStep, k[q]), [](float a) { return open_of(gate_at(a)); });
+          shift[kVectors ? q : 0] = load_piece<TC, VEC>(gs + gate_row * p.gate_shift_ld + p.c + q * kStep, k[q]);
         }
       }
     }
@@ -166,11 +166,11 @@ __global__ void __launch_bounds__(kRowThreads) residual_norm_kernel(const Params
       for (int q = 0; q < P; ++q) store_piece<VEC>(to + q * kStep, r[q], k[q]);
     }
     if (p.kept != nullptr) {
-      uint8_t *bytes = p.kept + o, *e = p.kept_e + static_cast<long long>(here.row) * groups8(p.c) + ch / kGroup8;
+      uint8_t *bytes = p.kept + o, *e = p.kept_e + static_cast<long long>(here.row) * groups8(p.c);
 #pragma unroll
       for (int q = 0; q < P; ++q) {
         if constexpr (!std::is_same<TS, __nv_bfloat16>::value) top[q] = top_of(r[q]);
-        store_piece8<VEC>(bytes + q * kStep, e + q * (kStep / kGroup8), r[q], exponent8(group_top(top[q])), k[q], ch % kGroup8 == 0);
+        store_piece8<VEC>(bytes + q * kStep, e + (ch + q * kStep) / kGroup8, r[q], top[q], k[q], threadIdx.x % 32);
       }
     }
     if (p.norm != kNoNorm) {
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kRowThreads) residual_norm_kernel(const Params
                      take(TC{}, p.s_g + P * kC, gs + here.row * p.gate_shift_ld + p.c, q));
       } else {
 #pragma unroll
-        for (int q = 0; q < P; ++q) r[q] = fma(mul(r[q], rstd), m[q], shift[q]);
+        for (int q = 0; q < P; ++q) r[q] = fma(mul(r[q], rstd), m[kVectors ? q : 0], shift[kVectors ? q : 0]);
       }
       TC* y = static_cast<TC*>(p.y) + o;
 #pragma unroll
@@ -212,9 +212,10 @@ __global__ void __launch_bounds__(kRowThreads) residual_norm_kernel(const Params
   }
 }
 
-template <typename TS, typename TC, int LANES, int P, bool VEC, bool OWN>
+template <typename TS, typename TC, int LANES, int P, bool VEC, int GATES>
 int launch(cudaStream_t stream, Params p, long long rows, int samples, int l) {
-  constexpr auto kernel = residual_norm_kernel<TS, TC, LANES, P, VEC, OWN>;
+  constexpr bool OWN = GATES != kSharedGates;
+  constexpr auto kernel = residual_norm_kernel<TS, TC, LANES, P, VEC, GATES>;
   constexpr int kWarps = kRowThreads / 32, kTeams = 32 / LANES, kMostBlocks = 8;
   static std::once_flag once;
   static int held = 1;
@@ -234,7 +235,7 @@ int launch(cudaStream_t stream, Params p, long long rows, int samples, int l) {
   if (VEC) KFB_TRY(allow_smem<kernel>(kMostRing));
   const int room = smem > 0 ? kMostRing / smem : held, blocks_per_sm = held < room ? held : room < 1 ? 1 : room;
   const long long most = static_cast<long long>(sm_count()) * blocks_per_sm;
-  p.plan = row_plan(rows, samples, l, most * kWarps * kTeams, kTeams);
+  p.plan = row_plan(rows, samples, l, most * kWarps * kTeams, kTeams, 0);
   const long long want = (p.plan.sets + kWarps - 1) / kWarps;
   LaunchScope scope(stream, "residual_norm");
   return launch_kernel(stream, kernel, static_cast<unsigned>(want < most ? want : most), kRowThreads, smem, p);
@@ -242,7 +243,9 @@ int launch(cudaStream_t stream, Params p, long long rows, int samples, int l) {
 
 template <typename TS, typename TC, int LANES, int P, bool VEC>
 int launch_own(cudaStream_t stream, const Params& p, long long rows, int samples, int l) {
-  return samples == 1 ? launch<TS, TC, LANES, P, VEC, true>(stream, p, rows, samples, l) : launch<TS, TC, LANES, P, VEC, false>(stream, p, rows, samples, l);
+  if (samples > 1) return launch<TS, TC, LANES, P, VEC, kSharedGates>(stream, p, rows, samples, l);
+  return p.norm == kAdaptiveNorm ? launch<TS, TC, LANES, P, VEC, kOwnAdaptive>(stream, p, rows, samples, l)
+                                 : launch<TS, TC, LANES, P, VEC, kOwnGates>(stream, p, rows, samples, l);
 }
 
 template <typename TS, typename TC>

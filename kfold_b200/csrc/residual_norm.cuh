@@ -12,6 +12,10 @@ namespace kfb {
 
 enum RowNorm : int { kNoNorm = 0, kAffineNorm = 1, kAdaptiveNorm = 2 };
 
+// What a kernel is made for: gates that samples share (of the output, the norm or both), gates of a row's own with a norm without them, and with the adaptive
+// one.  Each keeps other things in registers from row to row.
+enum RowGates : int { kSharedGates = 0, kOwnGates = 1, kOwnAdaptive = 2 };
+
 constexpr int kRowThreads = 128;
 
 struct RowPlan {
@@ -52,8 +56,8 @@ struct Walk {
 };
 
 // A plan for `teams` teams at work at once, `in_warp` of them in a warp: pieces that the teams finish together.  The cost of a round is its samples and, for the
-// gates and the sums, about two more.  Never more than two pieces a team.
-inline RowPlan row_plan(long long rows, int samples, int l, long long teams, int in_warp) {
+// gates and the sums, about two more; `join` for pieces that a second kernel has to join.  Never more than two pieces a team.
+inline RowPlan row_plan(long long rows, int samples, int l, long long teams, int in_warp, int join) {
   RowPlan p = {};
   p.gate_rows = static_cast<unsigned>(rows / samples);
   p.l = static_cast<unsigned>(l);
@@ -61,7 +65,7 @@ inline RowPlan row_plan(long long rows, int samples, int l, long long teams, int
   p.chunks = 1;
   long long best = -1;
   for (int k = 1; k <= samples; ++k) {
-    const long long units = static_cast<long long>(p.gate_rows) * k, cost = (units + teams - 1) / teams * ((samples + k - 1) / k + 2);
+    const long long units = static_cast<long long>(p.gate_rows) * k, cost = (units + teams - 1) / teams * ((samples + k - 1) / k + 2) + (k > 1 ? join : 0);
     if (k > 1 && units > 2 * teams) break;
     if (best < 0 || cost < best) {
       best = cost;
@@ -84,11 +88,11 @@ __device__ __forceinline__ void team_sum(float (&v)[K]) {
     for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], m);
 }
 
-// The ring.  Bytes that an SM's blocks have for it, and rows on their way for a team, the one in work among them: 2 to 4, as many as leave two blocks
-// of 128 threads an SM their place.
+// The ring.  Bytes that an SM's blocks have for it, and rows on their way for a team, the one in work among them: 2 to 4, as many as leave `blocks`
+// of 128 threads an SM their place.  (Gates of a row's own leave registers for three, and their exponentials want the warps more than a third row on its way.)
 constexpr int kMostRing = 216 * 1024;
-constexpr int ring_depth(int row_bytes) {      // of a thread and row
-  const int d = kMostRing / 2 / kRowThreads / row_bytes;
+constexpr int ring_depth(int row_bytes, int blocks) {      // of a thread and row
+  const int d = kMostRing / blocks / kRowThreads / row_bytes;
   return d < 2 ? 2 : d > 4 ? 4 : d;
 }
 // Slot `s` of stage `q` of this thread: ring + ((q * slots + s) * kRowThreads + thread) * 16 bytes; piece p of a tensor p * (16-byte words of a piece) slots on.

@@ -33,38 +33,38 @@ struct GradParams {
 };
 
 template <typename TS, typename TC, int P, bool OWN>
-constexpr int depth() { return ring_depth(P * 8 * (2 * sizeof(TS) + (OWN ? 4 : 2) * sizeof(TC))); }
+constexpr int depth() { return ring_depth(P * 8 * (2 * sizeof(TS) + (OWN ? 4 : 2) * sizeof(TC)), OWN ? 3 : 2); }
 
-// OWN: a row has gates of its own.
-template <typename TS, typename TC, int LANES, int P, bool VEC, bool OWN>
-__global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 ? 3 : 2) residual_norm_grad_kernel(const GradParams p) {
+template <typename TS, typename TC, int LANES, int P, bool VEC, int GATES>
+__global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 || (P == 3 && GATES == kOwnAdaptive) ? 3 : 2) residual_norm_grad_kernel(const GradParams p) {
+  constexpr bool OWN = GATES != kSharedGates, kSums = GATES != kOwnAdaptive;      // (sums from row to row)
   constexpr int kDepth = depth<TS, TC, P, OWN>(), kC = sizeof(TC) / 2;
   constexpr int kStep = LANES * kPiece;      // channels from a lane's piece to its next
   extern __shared__ uint4 ring_memory[];
   grid_dependency_enter();
-  const int warp = threadIdx.x / 32, ch = threadIdx.x % LANES * kPiece, team = threadIdx.x % 32 / LANES, groups = groups8(p.c);
+  const int warp = threadIdx.x / 32, ch = threadIdx.x % LANES * (VEC ? kPiece : 1), team = threadIdx.x % 32 / LANES, groups = groups8(p.c);
   const float inv_c = 1.0f / static_cast<float>(p.c);
   const TC *gate = static_cast<const TC*>(p.gate) + ch, *gs = static_cast<const TC*>(p.gate_shift) + ch;
-  const bool gated = p.gate != nullptr, adaptive = p.norm == kAdaptiveNorm;
+  const bool gated = p.gate != nullptr, adaptive = GATES == kOwnAdaptive || (GATES == kSharedGates && p.norm == kAdaptiveNorm);
   const uint4* ring = ring_memory + threadIdx.x;
   const uint32_t ring_at = ptx::smem_u32(ring);
   float* scale_sums = reinterpret_cast<float*>(ring_memory + p.s_scale * kRowThreads) + threadIdx.x;      // [P * 8][thread]
   int inside[P];                             // channels of a piece
 #pragma unroll
-  for (int q = 0; q < P; ++q) inside[q] = min(max(p.c - ch - q * kStep, 0), kPiece);
+  for (int q = 0; q < P; ++q) inside[q] = channels_of<VEC>(p.c, ch + q * kStep);
   auto vector = [&](const float* v, int q, float other) {
     float f[kPiece];
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) f[i] = v != nullptr && i < inside[q] ? v[ch + q * kStep + i] : other;
+    for (int i = 0; i < kPiece; ++i) f[i] = v != nullptr && i < inside[q] ? v[ch + q * kStep + i * channel_step<VEC>()] : other;
     return of_floats(f);
   };
 
   // m: what dy is multiplied by, weights or open gates; open: the output gates
-  Pairs m[P], open[OWN ? 1 : P], a0[P], a1[P], a2[OWN ? 1 : P];
+  Pairs m[P], open[OWN ? 1 : P], a0[kSums ? P : 1], a1[kSums ? P : 1], a2[OWN ? 1 : P];
 #pragma unroll
   for (int q = 0; q < P; ++q) {
     m[q] = vector(p.weight, q, 1.f);
-    a0[q] = a1[q] = both(0.f);
+    if (kSums) a0[kSums ? q : 0] = a1[kSums ? q : 0] = both(0.f);
     if (!OWN) open[OWN ? 0 : q] = both(1.f), a2[OWN ? 0 : q] = both(0.f);
     if (p.x != nullptr) {
 #pragma unroll
@@ -109,11 +109,17 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 ? 3 : 2) resi
   }
   int stage = 0;
   while (here.set < p.plan.sets) {
+    const bool row_there = here.left > 0;
+    uint32_t r_ex[P];                        // r's exponents where they come in no words: asked for before the wait
     if constexpr (VEC) {
       fetch(stage == 0 ? kDepth - 1 : stage - 1);
+      if (p.r_e != nullptr && !p.words) {
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+          r_ex[q] = row_there && inside[q] > 0 ? p.r_e[static_cast<long long>(here.row) * groups + (ch + q * kStep) / kGroup8] : 0u;
+      }
       copy_async_wait<kDepth - 1>();
     }
-    const bool row_there = here.left > 0;
     const uint4* s = ring + stage * p.slots * kRowThreads;
     const long long o = static_cast<long long>(here.row) * p.c + ch, e = static_cast<long long>(here.row) * groups;
     int k[P];                                // channels that are there
@@ -128,11 +134,11 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 ? 3 : 2) resi
           if constexpr (VEC) v[q] = ring_take<E>(s + (slot + q * (static_cast<int>(sizeof(E)) / 2)) * kRowThreads);
           else v[q] = load_piece<E, VEC>(static_cast<const E*>(t) + o + q * kStep, k[q]);
         }
-      } else if (VEC && p.words) {
+      } else if (VEC && (p.words || exponents == p.r_e)) {
 #pragma unroll
         for (int q = 0; q < P; ++q) {
           const uint4 w = s[(slot + q) * kRowThreads];
-          v[q] = values8(make_uint2(w.x, w.y), w.z >> (ch + q * kStep) / kGroup8 % 4 * 8 & 255u);
+          v[q] = values8(make_uint2(w.x, w.y), p.words ? w.z >> (ch + q * kStep) / kGroup8 % 4 * 8 & 255u : r_ex[q]);
         }
       } else {
 #pragma unroll
@@ -218,8 +224,8 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 ? 3 : 2) resi
       } else {
 #pragma unroll
         for (int q = 0; q < P; ++q) {
-          a0[q] = fma(d[q], z[q], a0[q]);
-          a1[q] = add(a1[q], d[q]);
+          a0[kSums ? q : 0] = fma(d[q], z[q], a0[kSums ? q : 0]);
+          a1[kSums ? q : 0] = add(a1[kSums ? q : 0], d[q]);
         }
       }
       if (p.dr != nullptr) {
@@ -331,7 +337,8 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 ? 3 : 2) resi
       for (int q = 0; q < P; ++q)
 #pragma unroll
         for (int i = 0; i < kPiece; ++i)
-          flat[static_cast<int>(threadIdx.x) / LANES * kWidth + ch + q * kStep + i] = j == 0 ? a0[q].get(i) : j == 1 ? a1[q].get(i) : scale_sums[(q * kPiece + i) * kRowThreads];
+          flat[static_cast<int>(threadIdx.x) / LANES * kWidth + ch + q * kStep + i * channel_step<VEC>()] =
+              j == 2 ? scale_sums[(q * kPiece + i) * kRowThreads] : !kSums ? 0.f : (j == 0 ? a0 : a1)[kSums ? q : 0].get(i);
       __syncthreads();
       for (int i = threadIdx.x; i < p.c; i += kRowThreads) {
         float t = 0.f;
@@ -397,7 +404,7 @@ __global__ void __launch_bounds__(256) residual_norm_gates_kernel(const float* p
 }
 
 // Blocks of an SM, at most, and SMs: the workspace is sized by them.
-constexpr int most_blocks(int c) { return c <= 256 ? 6 : c <= 512 ? 3 : 2; }
+constexpr int most_blocks(int c) { return c <= 256 ? 6 : 3; }
 constexpr int kMostSms = 160;
 // Pieces of gate rows' samples, at most: two for each team that is at work (row_plan).
 constexpr long long most_units(int c) { return 2ll * kMostSms * most_blocks(c) * (c <= 128 ? 16 : c <= 384 ? 8 : 4); }
@@ -406,9 +413,10 @@ struct Sums {
   float *dweight, *dbias, *dscale;
 };
 
-template <typename TS, typename TC, int LANES, int P, bool VEC, bool OWN>
+template <typename TS, typename TC, int LANES, int P, bool VEC, int GATES>
 int launch(cudaStream_t stream, GradParams p, const Sums& sums, long long rows, int samples, int l) {
-  constexpr auto kernel = residual_norm_grad_kernel<TS, TC, LANES, P, VEC, OWN>;
+  constexpr bool OWN = GATES != kSharedGates;
+  constexpr auto kernel = residual_norm_grad_kernel<TS, TC, LANES, P, VEC, GATES>;
   constexpr int kS = P * sizeof(TS) / 2, kC = P * sizeof(TC) / 2, kWarps = kRowThreads / 32, kTeams = 32 / LANES, kFlat = kRowThreads * P * kPiece * 4;
   static std::once_flag once;
   static int held = 1;
@@ -438,8 +446,8 @@ int launch(cudaStream_t stream, GradParams p, const Sums& sums, long long rows, 
   KFB_CHECK_ARG(smem <= kMostRing, "residual_norm_bwd: %d bytes of shared memory", smem);
   const int fit = smem > 0 ? kMostRing / smem : held, limit = held < most_blocks(p.c) ? held : most_blocks(p.c), blocks_per_sm = limit < fit ? limit : fit;
   const long long most = static_cast<long long>(sm_count() < kMostSms ? sm_count() : kMostSms) * blocks_per_sm;
-  p.plan = row_plan(rows, samples, l, most * kWarps * kTeams, kTeams);
   const bool gates = p.dgate != nullptr || p.dgate_shift != nullptr;
+  p.plan = row_plan(rows, samples, l, most * kWarps * kTeams, kTeams, gates ? 4 : 0);      // (the second launch: 301 gate rows of 5 samples 13.4 -> 10 us in one piece)
   if (p.plan.chunks == 1 || !gates) p.pieces = nullptr;
   else KFB_CHECK_ARG(p.plan.units <= most_units(p.c), "residual_norm_bwd: %u pieces", p.plan.units);
   const long long want = (p.plan.sets + kWarps - 1) / kWarps;
@@ -465,8 +473,9 @@ int launch(cudaStream_t stream, GradParams p, const Sums& sums, long long rows, 
 
 template <typename TS, typename TC, int LANES, int P, bool VEC>
 int launch_own(cudaStream_t stream, const GradParams& p, const Sums& sums, long long rows, int samples, int l) {
-  return samples == 1 ? launch<TS, TC, LANES, P, VEC, true>(stream, p, sums, rows, samples, l)
-                      : launch<TS, TC, LANES, P, VEC, false>(stream, p, sums, rows, samples, l);
+  if (samples > 1) return launch<TS, TC, LANES, P, VEC, kSharedGates>(stream, p, sums, rows, samples, l);
+  return p.norm == kAdaptiveNorm ? launch<TS, TC, LANES, P, VEC, kOwnAdaptive>(stream, p, sums, rows, samples, l)
+                                 : launch<TS, TC, LANES, P, VEC, kOwnGates>(stream, p, sums, rows, samples, l);
 }
 
 template <typename TS, typename TC>

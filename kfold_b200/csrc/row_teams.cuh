@@ -147,7 +147,16 @@ __device__ __forceinline__ uint32_t group_top(uint32_t t) {
   return max(t, __shfl_xor_sync(0xffffffffu, t, 2));
 }
 
-// ---- pieces in memory, of which `n` channels are there.  VEC: n is 0 or 8 and the address on a 16-byte boundary (8 for bytes).
+// ---- pieces in memory, of which the first `n` channels are there.  VEC: eight neighbouring channels, n is 0 or 8 and the address on a 16-byte boundary (8 for bytes).
+// Otherwise (any width, any address) a lane has every 32nd channel, so that a warp's accesses lie side by side and a group of 32 is the warp's: p, and e of bytes, are
+// then those of the lane's first channel; all lanes of a warp come to the bytes together, with one piece of one row.
+constexpr int kSpread = 32;
+template <bool VEC>
+__host__ __device__ constexpr int channel_step() { return VEC ? 1 : kSpread; }
+// Channels of a piece that a row of c has, and its first channel.
+template <bool VEC>
+__device__ __forceinline__ int channels_of(int c, int first) { return min(max(VEC ? c - first : (c - first + kSpread - 1) / kSpread, 0), kPiece); }
+
 template <typename T, bool VEC>
 __device__ __forceinline__ Pairs load_piece(const T* p, int n) {
   const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -159,23 +168,28 @@ __device__ __forceinline__ Pairs load_piece(const T* p, int n) {
     float f[kPiece];
 #pragma unroll
     for (int i = 0; i < kPiece; ++i) {
-      if constexpr (sizeof(T) == 2) f[i] = i < n ? __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(p)[i]) << 16) : 0.f;
-      else f[i] = i < n ? p[i] : 0.f;
+      if constexpr (sizeof(T) == 2) f[i] = i < n ? __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(p)[i * kSpread]) << 16) : 0.f;
+      else f[i] = i < n ? p[i * kSpread] : 0.f;
     }
     return of_floats(f);
   }
 }
 template <bool VEC>
 __device__ __forceinline__ Pairs load_piece8(const uint8_t* p, const uint8_t* e, int n) {
-  uint2 b = make_uint2(0, 0);
   if constexpr (VEC) {
-    if (n > 0) b = *reinterpret_cast<const uint2*>(p);
+    return values8(n > 0 ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0), n > 0 ? *e : 0u);
   } else {
+    // (lane i takes the exponent of group i for all)
+    uint32_t b[kPiece];
+    const int lane = threadIdx.x % 32, most = __shfl_sync(0xffffffffu, n, 0);
+    const float step = lane < most && lane < kPiece ? step8(e[lane]) : 0.f;
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i)
-      if (i < n) (i < 4 ? b.x : b.y) |= static_cast<uint32_t>(p[i]) << 8 * (i & 3);
+    for (int i = 0; i < kPiece; ++i) b[i] = i < n ? p[i * kSpread] : 0u;
+    float f[kPiece];
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) f[i] = static_cast<float>(static_cast<int8_t>(b[i])) * __shfl_sync(0xffffffffu, step, i);
+    return of_floats(f);
   }
-  return values8(b, n > 0 ? *e : 0u);
 }
 template <bool VEC, typename T>
 __device__ __forceinline__ void store_piece(T* p, const Pairs& v, int n) {
@@ -192,22 +206,38 @@ __device__ __forceinline__ void store_piece(T* p, const Pairs& v, int n) {
 #pragma unroll
     for (int i = 0; i < kPiece; ++i) {
       const float f = v.get(i);
-      if (i < n) store_vec<1>(p + i, &f);
+      if (i < n) store_vec<1>(p + i * kSpread, &f);
     }
   }
 }
-// Bytes, and by the first lane of a group its exponent.
+// Values into bytes, and by the first lane of a group its exponent.  `top`: of the piece (VEC).  All lanes of a warp come here together.
 template <bool VEC>
-__device__ __forceinline__ void store_piece8(uint8_t* p, uint8_t* e, const Pairs& v, uint32_t ex, int n, bool first) {
-  const uint2 q = bytes8(v, ex);
+__device__ __forceinline__ void store_piece8(uint8_t* p, uint8_t* e, const Pairs& v, uint32_t top, int n, int lane) {
   if constexpr (VEC) {
-    if (n > 0) *reinterpret_cast<uint2*>(p) = q;
+    const uint32_t ex = exponent8(group_top(top));
+    const uint2 q = bytes8(v, ex);
+    if (n <= 0) return;
+    *reinterpret_cast<uint2*>(p) = q;
+    if (lane % (kGroup8 / kPiece) == 0) *e = static_cast<uint8_t>(ex);
   } else {
+    // (lane i works out the exponent of group i for all; the first lane has a channel of every group that is there)
+    const int lane32 = threadIdx.x % 32, most = __shfl_sync(0xffffffffu, n, 0);
+    uint32_t mine = 0u;
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i)
-      if (i < n) p[i] = static_cast<uint8_t>((i < 4 ? q.x : q.y) >> 8 * (i & 3));
+    for (int i = 0; i < kPiece; ++i) {
+      const uint32_t t = __reduce_max_sync(0xffffffffu, __float_as_uint(v.get(i)) & 0x7fffffffu);
+      if (lane32 == i) mine = t;
+    }
+    const uint32_t ex = exponent8(mine);
+    const float inverse = inverse_step8(ex);
+    const uint32_t bad = __ballot_sync(0xffffffffu, ex == 255u);
+    if (lane32 < most && lane32 < kPiece) e[lane32] = static_cast<uint8_t>(ex);
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) {
+      const float t = fminf(fmaxf(v.get(i) * __shfl_sync(0xffffffffu, inverse, i), -127.f), 127.f) + 12582912.f;
+      if (i < n) p[i * kSpread] = bad >> i & 1u ? 0 : static_cast<uint8_t>(__float_as_uint(t));
+    }
   }
-  if (first && n > 0) *e = static_cast<uint8_t>(ex);
 }
 
 // ---- copies of 16, 8 or 4 bytes into shared memory that arrive while the thread goes on; zeros where `there` is false

@@ -66,7 +66,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, out_dtype):
         ctx.eps = eps
-        if _compressing() and (x.dtype, out_dtype or x.dtype) in F._STREAM_CODES and x.shape[-1] <= 1024:
+        if _compressing() and any(ctx.needs_input_grad) and (x.dtype, out_dtype or x.dtype) in F._STREAM_CODES and x.shape[-1] <= 1024:
             _, y, kept = F.residual_norm(x, weight=weight, bias=bias, eps=eps, out_dtype=out_dtype, compress=True)
             _keep(ctx, [kept], weight, bias)
             return y
@@ -97,7 +97,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
 class _GatedFeedForward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_in, w_out):
-        _keep(ctx, [F.compress(x) if _compressing() else x], w_in, w_out)
+        _keep(ctx, [F.compress(x) if _compressing() and any(ctx.needs_input_grad) else x], w_in, w_out)
         return F.gated_feed_forward(x, w_in, w_out)
 
     @staticmethod

@@ -41,10 +41,14 @@ __device__ __forceinline__ uint64_t by_sign(uint64_t z, uint64_t low, uint64_t h
 }
 
 // Phi(-|z|) and exp(-z^2 / 2) for gelu = z Phi(z):  Phi(-|z|) = exp(-z^2 / 2) t P(t), t = 1 / (1 + 0.26517 |z|), P of degree 6 fitted to erfcx by least squares with weights
-// that level the relative error, 7e-7 at most for |z| < 13.4, where exp(-z^2 / 2) ends: it keeps its digits where it is small.
-__device__ __forceinline__ uint64_t normal_tail(uint64_t z, uint64_t& density) {
+// that level the relative error, 7e-7 at most for |z| < 13.4, where exp(-z^2 / 2) ends: it keeps its digits where it is small.  size: |z|, finite, so that nothing
+// times it is nothing.
+__device__ __forceinline__ uint64_t finite_size(uint64_t z) {
+  return each_of(magnitude(z), [](float a) { return a > 1e30f ? 1e30f : a; });      // (what is no number stays none)
+}
+__device__ __forceinline__ uint64_t normal_tail(uint64_t z, uint64_t size, uint64_t& density) {
   density = power(ptx::mul2(ptx::mul2(z, z), pair_of(-0.72134752f)));
-  const uint64_t t = reciprocal(ptx::fma2(magnitude(z), pair_of(0.26516503f), pair_of(1.f)));
+  const uint64_t t = reciprocal(ptx::fma2(size, pair_of(0.26516503f), pair_of(1.f)));
   uint64_t p = pair_of(-0.067547895f);
   p = ptx::fma2(p, t, pair_of(0.19396849f));
   p = ptx::fma2(p, t, pair_of(-0.064797565f));
@@ -67,8 +71,8 @@ __device__ __forceinline__ uint64_t activation(uint64_t z) {
   uint64_t other;
   if constexpr (ACT == kRelu) return each_of(z, [](float a) { return a > 0.f || a != a ? a : 0.f; });
   if constexpr (ACT == kGelu) {                      // max(z, 0) - |z| Phi(-|z|)
-    const uint64_t low = normal_tail(z, other);
-    return ptx::fma2(magnitude(z) | 0x8000000080000000ull, low, each_of(z, [](float a) { return fmaxf(a, 0.f); }));
+    const uint64_t size = finite_size(z), low = normal_tail(z, size, other);
+    return ptx::fma2(size | 0x8000000080000000ull, low, each_of(z, [](float a) { return fmaxf(a, 0.f); }));
   }
   if constexpr (ACT == kSigmoid) return sigmoid_of(z, other);
   if constexpr (ACT == kSilu) return ptx::mul2(z, sigmoid_of(z, other));
@@ -79,8 +83,8 @@ __device__ __forceinline__ uint64_t slope(uint64_t z) {
   uint64_t other;
   if constexpr (ACT == kRelu) return each_of(z, [](float a) { return a > 0.f ? 1.f : 0.f; });
   if constexpr (ACT == kGelu) {
-    const uint64_t low = normal_tail(z, other);      // at -|z|: Phi - |z| phi; the slope at |z| is one less that
-    const uint64_t v = ptx::fma2(ptx::mul2(magnitude(z), pair_of(-0.39894228f)), other, low);
+    const uint64_t size = finite_size(z), low = normal_tail(z, size, other);
+    const uint64_t v = ptx::fma2(ptx::mul2(size, pair_of(-0.39894228f)), other, low);      // at -|z|: Phi - |z| phi; the slope at |z| is one less that
     return by_sign(z, v, ptx::fma2(v, pair_of(-1.f), pair_of(1.f)));
   }
   if constexpr (ACT == kSigmoid) {

@@ -89,6 +89,16 @@ __global__ void __launch_bounds__(kRowThreads) residual_norm_kernel(const Params
     if constexpr (VEC) {
       fetch(stage == 0 ? kDepth - 1 : stage - 1);
       copy_async_wait<kDepth - 1>();
+    } else {
+      ahead.next(p.plan, team, step);
+      if (ahead.set < p.plan.sets && ahead.left > 0) {
+        const int lane = threadIdx.x % 32;
+        const long long o = static_cast<long long>(ahead.row) * p.c - ch;
+        if (has_x) prefetch_row(x + o, p.c, lane);
+        if (has_u) prefetch_row(u + o, p.c, lane);
+        if (OWN && gated) prefetch_row(gate - ch + ahead.row * p.gate_ld, p.c, lane);
+        if (OWN && adaptive) prefetch_row(gs - ch + ahead.row * p.gate_shift_ld, 2 * p.c, lane);
+      }
     }
     const uint4* s = ring + stage * p.slots * kRowThreads;
     const long long o = static_cast<long long>(here.row) * p.c + ch;

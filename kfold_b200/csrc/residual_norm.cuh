@@ -114,6 +114,13 @@ __device__ __forceinline__ void ring_copy8(uint32_t slot, const uint8_t* from, c
     if (words) copy_async<4>(slot + q * kRowThreads * 16 + 8, exponents + ((channel + q * STEP) / kGroup8 & ~3), there[q]);
   }
 }
+// Rows of other widths or addresses are read as they lie; a warp asks for the next one's lines ahead.
+template <typename T>
+__device__ __forceinline__ void prefetch_row(const T* row, int c, int lane) {
+  for (int i = lane * (128 / static_cast<int>(sizeof(T))); i < c; i += 32 * (128 / static_cast<int>(sizeof(T))))
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(row + i));
+}
+
 template <typename T>
 __device__ __forceinline__ Pairs ring_take(const uint4* slot) {
   if constexpr (sizeof(T) == 2) return of_bf16(slot[0]);

@@ -119,6 +119,21 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 || (P == 3 &&
           r_ex[q] = row_there && inside[q] > 0 ? p.r_e[static_cast<long long>(here.row) * groups + (ch + q * kStep) / kGroup8] : 0u;
       }
       copy_async_wait<kDepth - 1>();
+    } else {
+      ahead.next(p.plan, team, step);
+      if (ahead.set < p.plan.sets && ahead.left > 0) {
+        const int lane = threadIdx.x % 32;
+        const long long o = static_cast<long long>(ahead.row) * p.c;
+        if (p.dr != nullptr) prefetch_row(static_cast<const TS*>(p.dr) + o, p.c, lane);
+        if (p.norm != kNoNorm) {
+          prefetch_row(static_cast<const TC*>(p.dy) + o, p.c, lane);
+          if (p.r_e != nullptr) prefetch_row(static_cast<const uint8_t*>(p.r) + o, p.c, lane);
+          else prefetch_row(static_cast<const TS*>(p.r) + o, p.c, lane);
+        }
+        if (p.dgate != nullptr && p.u_e == nullptr) prefetch_row(static_cast<const TC*>(p.u) + o, p.c, lane);
+        if (OWN && gated) prefetch_row(gate - ch + ahead.row * p.gate_ld, p.c, lane);
+        if (OWN && adaptive) prefetch_row(gs - ch + ahead.row * p.gate_shift_ld, p.c, lane);
+      }
     }
     const uint4* s = ring + stage * p.slots * kRowThreads;
     const long long o = static_cast<long long>(here.row) * p.c + ch, e = static_cast<long long>(here.row) * groups;
@@ -134,7 +149,7 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 || (P == 3 &&
           if constexpr (VEC) v[q] = ring_take<E>(s + (slot + q * (static_cast<int>(sizeof(E)) / 2)) * kRowThreads);
           else v[q] = load_piece<E, VEC>(static_cast<const E*>(t) + o + q * kStep, k[q]);
         }
-      } else if (VEC && (p.words || exponents == p.r_e)) {
+      } else if (VEC && (p.words || slot == p.s_r)) {
 #pragma unroll
         for (int q = 0; q < P; ++q) {
           const uint4 w = s[(slot + q) * kRowThreads];

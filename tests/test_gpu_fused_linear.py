@@ -131,10 +131,74 @@ def test_many_rows(rows, k, n, act):
     _check(*_case(rows, k, n, residual=act is None, seed=9), act)
 
 
-@pytest.mark.parametrize("rows", [30000, 700001])
+@pytest.mark.parametrize("rows", [30000, 900001])
 def test_pieces_of_rows_in_float32(rows):
+    """What a row keeps in the workspace is 6 (k + n) bytes, of which half a gigabyte is one piece."""
     k, n = (256, 384) if rows < 100000 else (40, 72)
     _check(*_case(rows, k, n, F32, residual=True, seed=4), "silu")
+
+
+@pytest.mark.parametrize("rows, k, n, out", [(150001, 64, 2048, BF), (300001, 256, 1024, BF), (150001, 64, 2048, F32), (5000001, 8, 64, BF)])
+def test_pieces_of_rows_in_bf16(rows, k, n, out):
+    """2 n bytes a row; both ways of the products."""
+    x, w, b, _, dy = _case(rows, k, n, seed=6, out=out)
+    dx, dw, db = F.fused_linear_backward(dy, x, w, b, "silu")
+    parts = [slice(i, min(i + 65536, rows)) for i in range(0, rows, 65536)]
+    rw, rb, wsize, bsize = (torch.zeros(s, dtype=torch.float64, device=DEV) for s in ((n, k), (n,), (n, k), (n,)))
+    for p in parts:
+        (_, px, pw, pb), z = R.linear(x[p], w, b, "silu", None, dy[p])
+        rw, rb = rw + pw, rb + pb
+        dz = (dy[p].double() * R.slope(z, "silu")).abs()
+        wsize, bsize = wsize + dz.t() @ x[p].double().abs(), bsize + dz.sum(0)
+        room = 2.0 ** -7 * (dz @ w.double().abs())
+        assert ((dx[p].double() - px).abs() <= P.HALF_STEP[BF] * px.abs() + room).all()
+    assert ((dw.double() - rw).abs() <= P.HALF_STEP[BF] * rw.abs() + 2.0 ** -7 * wsize).all()
+    assert ((db.double() - rb).abs() <= (2.0 ** -16 + rows * P.U32) * bsize).all()
+
+
+def test_more_than_2_to_31_elements():
+    """Element numbers that pass 32 bits: rows at the start, across the border and at the end as they are alone."""
+    rows, k, n = (1 << 20) + 300, 64, 2048
+    x, w = torch.empty(rows, k, dtype=BF, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(1)), _randn(2, n, k, dtype=BF, scale=0.1)
+    y = F.fused_linear(x, w, None, "relu")
+    dx = F.fused_linear_backward(y, x, w, None, None, True, False, False)[0]
+    for p in (slice(0, 256), slice((1 << 20) - 256, (1 << 20) + 256), slice(rows - 256, rows)):
+        assert torch.equal(y[p], F.fused_linear(x[p], w, None, "relu"))
+        ref = y[p].double() @ w.double()
+        assert ((dx[p].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + (8 + n / 16) * 2.0 ** -23 * (y[p].double().abs() @ w.double().abs())).all()
+
+
+@pytest.mark.parametrize("rows, k, n", [(300, 64, 72), (20000, 256, 264)])
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_what_lies_behind_the_rows_stays(rows, k, n, act):
+    """The entry points write the rows they are given, of buffers that go on."""
+    x, w, b, r, dy = _case(rows, k, n, residual=True)
+    more = lambda c, rows=rows, dtype=BF: torch.full((rows + 200, c), 7.0, dtype=dtype, device=DEV)
+    y, dx, dw, db = more(n), more(k), more(k, n), more(1, n, F32).view(-1)
+    code, lib, stream = {None: 0, "gelu": 3}[act], L.lib(), L.raw_stream()
+    size = max(lib.kfb_fused_linear_workspace_bytes(rows, k, n, code, 0, 0, wanted) for wanted in (0, 7))
+    ws = torch.full((size + 4096,), 3, dtype=torch.uint8, device=DEV)
+    L.check(lib.kfb_fused_linear_fwd(x.data_ptr(), w.data_ptr(), b.data_ptr(), r.data_ptr(), y.data_ptr(), ws.data_ptr(), size, rows, k, n, code, 0, 0, stream))
+    L.check(lib.kfb_fused_linear_bwd(dy.data_ptr(), x.data_ptr(), w.data_ptr(), b.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), size, rows, k, n,
+                                     code, 0, 0, 0, stream))
+    assert torch.equal(y[:rows], F.fused_linear(x, w, b, act, r))
+    for t, ref in zip((dx[:rows], dw[:n], db[:n]), F.fused_linear_backward(dy, x, w, b, act)):
+        assert torch.equal(t, ref)
+    assert (y[rows:] == 7).all() and (dx[rows:] == 7).all() and (dw[n:] == 7).all() and (db[n:] == 7).all() and (ws[size:] == 3).all()
+
+
+@pytest.mark.parametrize("rows", [5, 30000])
+def test_infinities_before_the_activation(rows):
+    inf, nan = float("inf"), float("nan")
+    x = torch.zeros(rows, 128, device=DEV, dtype=BF)
+    x[0, 0], x[1, 0], x[2, 0], x[3, 0] = inf, -inf, nan, 1e30
+    w = torch.zeros(128, 128, device=DEV, dtype=BF)
+    w[0, 0] = 1
+    zero = torch.zeros(rows, 128, device=DEV, dtype=BF)
+    for act, want in (("relu", [inf, 0, nan, 1e30]), ("sigmoid", [1, 0, nan, 1]), ("gelu", [inf, 0, nan, 1e30]), ("silu", [inf, nan, nan, 1e30])):
+        got = F.fused_linear(x, w, None, act)[:4, 0]
+        assert torch.equal(torch.nan_to_num(got.float(), nan=-5.0), torch.nan_to_num(torch.tensor(want, device=DEV).to(BF).float(), nan=-5.0)), act
+        assert torch.equal(F.fused_linear(x, w, None, act)[4:], F.fused_linear(zero, w, None, act)[4:])
 
 
 def test_no_rows():

@@ -163,6 +163,29 @@ def test_kept_branch_and_stream(samples):
         assert (a is None and b is None) or torch.equal(a, b)
 
 
+@pytest.mark.parametrize("c", [64, 100, 128, 136, 505])
+def test_the_same_kept_rows_in_two_places(c):
+    d, dr, dy = _case(2, 3, 21, c, scale=True)
+    d["u"] = d["x"].clone()
+    kept = F.residual_norm(**d, samples=3, compress=True)[2]
+    at = F.expand(kept)
+    for gates in (3, 1):
+        gate, gs = (t if gates == 3 else t.repeat_interleave(3, 0) for t in (d["gate"], d["gate_shift"]))
+        g = F.residual_norm_backward(dr, dy, kept, kept, gate, kept, d["scale"], None, gs, gates)
+        h = F.residual_norm_backward(dr, dy, at, at, gate, at, d["scale"], None, gs, gates)
+        for a, b in zip(g, h):
+            assert (a is None and b is None) or torch.equal(a, b)
+
+
+def test_wide_rows_of_every_tensor_in_float32():
+    """The widest rows with everything that they can bring: what does not fit the shared memory is read as it lies."""
+    for c in (1023, 1021):
+        for samples in (1, 2):
+            d, dr, dy = _case(2, samples, 5, c, "f32", scale=True, seed=c)
+            _check(d, dr, dy, samples)
+            _check(d, dr, dy, samples, compress=True)
+
+
 def test_nothing_to_do():
     for groups, l in ((0, 5), (3, 0)):
         d, dr, dy = _case(max(groups, 1), 1, max(l, 1), 64, norm="affine", scale=True)
@@ -243,6 +266,31 @@ def test_no_epsilon():
     _check(d, dr, dy, 1, eps=0.0)
     d, dr, dy = _case(1, 5, 3, 60, "f32", scale=True)                # (lanes and teams without a row)
     _check(d, dr, dy, 5, eps=0.0)
+
+
+@pytest.mark.parametrize("c", [128, 99])
+@pytest.mark.parametrize("samples", [1, 5])
+def test_what_lies_behind_the_rows_stays(c, samples):
+    """The entry points write the rows they are given, of buffers that go on."""
+    l, rows, g = 7, 7 * samples, c + 31 & ~31
+    d, dr, dy = _case(1, samples, l, c)
+    more = lambda n, c, dtype=BF: torch.full((n + 40, c), 7, dtype=dtype, device=DEV)
+    r, y, kept, e = more(rows, c), more(rows, c), more(rows, c, torch.int8), more(rows, g // 32, torch.uint8)
+    dx, du, dgate, dgs = more(rows, c), more(rows, c), more(l, c), more(l, 2 * c)
+    lib, stream, p = L.lib(), L.raw_stream(), lambda t: t.data_ptr()
+    L.check(lib.kfb_residual_norm_fwd(p(d["x"]), p(d["u"]), p(d["gate"]), c, None, None, None, p(d["gate_shift"]), 2 * c, p(r), p(y), p(kept), p(e), rows, c, samples, l, 1e-5, 2,
+                                      0, 0, stream))
+    size = lib.kfb_residual_norm_bwd_workspace_bytes(rows, c, samples, 0, 1)
+    ws = torch.full((size + 4096,), 3, dtype=torch.uint8, device=DEV)
+    L.check(lib.kfb_residual_norm_bwd(p(dr), p(dy), p(kept), p(e), p(d["u"]), None, None, None, p(d["gate"]), c, None, None, p(d["gate_shift"]), 2 * c, p(dx), p(du), p(dgate), p(dgs),
+                                      None, None, None, p(ws), size, rows, c, samples, l, 1e-5, 2, 0, 0, stream))
+    about = dict(gate=d["gate"], gate_shift=d["gate_shift"], samples=samples)
+    want = F.residual_norm(d["x"], d["u"], compress=True, **about)
+    grads = F.residual_norm_backward(dr, dy, want[2], d["u"], **about)
+    for t, ref, n in ((r, want[0], rows), (y, want[1], rows), (kept, want[2].values, rows), (e, want[2].exponents, rows), (dx, grads.x, rows), (du, grads.u, rows),
+                      (dgate, grads.gate, l), (dgs, grads.gate_shift, l)):
+        assert torch.equal(t[:n], ref.reshape(n, -1)) and (t[n:] == 7).all()
+    assert (ws[size:] == 3).all()
 
 
 def test_long_rows_of_samples_same_bits_every_time():

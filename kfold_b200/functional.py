@@ -601,18 +601,19 @@ def residual_norm_backward(dr: torch.Tensor | None, dy: torch.Tensor | None, r, 
 _ACTIVATIONS = {None: 0, "sigmoid": 1, "silu": 2, "gelu": 3, "relu": 4}
 
 
-def _linear_operands(name: str, x, w: torch.Tensor, bias: torch.Tensor | None, activation: str | None):
-    """(rows, in and out channels, activation's number, kernel's dtype code)."""
-    shape = x.shape
+@lru_cache(maxsize=1024)
+def _linear_sizes(name: str, x: tuple, w: tuple, bias, activation: str | None):
+    """(rows, in and out channels, activation's number, kernel's dtype code) for x and a weight of these shapes and types, and a bias of this shape."""
+    (shape, dtype), (w_shape, w_dtype) = x, w
     k = shape[-1] if shape else 0
-    n = w.shape[0] if w.dim() == 2 else 0
-    if w.shape != (n, k) or not n or not k or n % 8 or k % 8 or (bias is not None and bias.numel() != n):
-        raise ValueError(f"{name}: weight {tuple(w.shape)}, bias {None if bias is None else tuple(bias.shape)} for x {tuple(shape)} (channels multiples of 8)")
+    n = w_shape[0] if len(w_shape) == 2 else 0
+    if w_shape != (n, k) or not n or not k or n % 8 or k % 8 or (bias is not None and math.prod(bias) != n):
+        raise ValueError(f"{name}: weight {tuple(w_shape)}, bias {None if bias is None else tuple(bias)} for x {tuple(shape)} (channels multiples of 8)")
     if activation not in _ACTIVATIONS:
         raise ValueError(f"{name}: activation {activation!r} (one of {', '.join(str(a) for a in _ACTIVATIONS)})")
-    if x.dtype not in _FEED_FORWARD_CODES or (w.dtype != x.dtype and w.dtype != torch.float32):
-        raise ValueError(f"{name}: x {x.dtype}, weight {w.dtype}")
-    return math.prod(shape[:-1]), k, n, _ACTIVATIONS[activation], _FEED_FORWARD_CODES[x.dtype]
+    if dtype not in _FEED_FORWARD_CODES or (w_dtype != dtype and w_dtype != torch.float32):
+        raise ValueError(f"{name}: x {dtype}, weight {w_dtype}")
+    return math.prod(shape[:-1]), k, n, _ACTIVATIONS[activation], _FEED_FORWARD_CODES[dtype]
 
 
 @lru_cache(maxsize=1024)
@@ -632,14 +633,15 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     if at != L.current_device():
         with L.on_device(x.device):
             return fused_linear(x, w, bias, activation, residual)
-    rows, k, n, act, code = _linear_operands("fused_linear", x, w, bias, activation)
+    dt = x.dtype
+    rows, k, n, act, code = _linear_sizes("fused_linear", (x.shape, dt), (w.shape, w.dtype), None if bias is None else bias.shape, activation)
     shape = (*x.shape[:-1], n)
     if residual is not None and (residual.shape != shape or (residual.dtype != x.dtype and residual.dtype != torch.float32)):
         raise ValueError(f"fused_linear: residual {residual.dtype} {tuple(residual.shape)} for x {x.dtype} {tuple(x.shape)} and {n} channels")
     out = x.new_empty(shape) if residual is None else _dense_like(residual)
     need = _fused_linear_bytes(at, rows, k, n, act, code, L.dtype_code(out.dtype), 0)
     ws = _call_workspace(x.device, need) if need else None
-    xc, wc, b = _operand(x, x.dtype), _operand(w, x.dtype), None if bias is None else _operand(bias, torch.float32)
+    xc, wc, b = _operand(x, dt), _operand(w, dt), None if bias is None else _operand(bias, torch.float32)
     rc = None if residual is None else _operand(residual, residual.dtype)
     L.check(L.lib().kfb_fused_linear_fwd(xc.data_ptr(), wc.data_ptr(), L.ptr(b), L.ptr(rc), out.data_ptr(), L.ptr(ws), need, rows, k, n, act, code,
                                          L.dtype_code(out.dtype), L.raw_stream(at)))
@@ -655,7 +657,7 @@ def fused_linear_backward(dy: torch.Tensor, x, w: torch.Tensor, bias: torch.Tens
     if at != L.current_device():
         with L.on_device(dy.device):
             return fused_linear_backward(dy, x, w, bias, activation, need_x, need_w, need_bias)
-    rows, k, n, act, code = _linear_operands("fused_linear_backward", x, w, bias, activation)
+    rows, k, n, act, code = _linear_sizes("fused_linear_backward", (x.shape, x.dtype), (w.shape, w.dtype), None if bias is None else bias.shape, activation)
     if dy.shape != (*x.shape[:-1], n) or (dy.dtype != x.dtype and dy.dtype != torch.float32):
         raise ValueError(f"fused_linear_backward: dy {dy.dtype} {tuple(dy.shape)} for x {x.dtype} {tuple(x.shape)} and {n} channels")
     need_bias = need_bias and bias is not None

@@ -170,7 +170,7 @@ class _ResidualNorm(torch.autograd.Function):
         if r is None:
             r = dr                       # (of its shape and type)
         if u is None and ctx.u_dtype is not None:
-            u = dr if dr is not None and dr.dtype == ctx.u_dtype else dy if dy is not None else dr.to(ctx.u_dtype)
+            u = dr if dr is not None and dr.dtype == ctx.u_dtype else dy if dy is not None else dr.new_empty((), dtype=ctx.u_dtype).expand(dr.shape)
         g = F.residual_norm_backward(dr, dy, r, u, gate, x, scale, weight, gate_shift, ctx.samples, ctx.eps, need[0], need[1], need[2] and gate is not None,
                                      need[3] and scale is not None, need[4], need[5], need[6])
         return (None if ctx.x_missing else g.x, g.u, g.gate, _as(g.scale, scale), _as(g.weight, weight), _as(g.bias, bias), g.gate_shift, None, None, None, None)

@@ -27,7 +27,7 @@ struct GradParams {
   RowPlan plan;
   int c, norm;
   float eps;
-  int slots, s_dy, s_r, s_u, s_x, s_gate, s_g;    // slots of a stage, and the first of each tensor (dr: 0)
+  int slots, s_dy, s_r, s_u, s_x, s_gate, s_g;    // slots of a stage, and the first of each tensor (dr: 0; s_x below zero: x is read as it lies)
   int s_scale;                         // behind the ring: this thread's sums of t x
   int words;                           // exponents come in words of four (a row's are whole words, and start on one)
 };
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 || (P == 3 &&
         copy(TS{}, p.s_r, p.r, p.r_e);
       }
       if (p.dgate != nullptr) copy(TC{}, p.s_u, p.u, p.u_e);
-      if (p.x != nullptr) copy(TS{}, p.s_x, p.x, p.x_e);
+      if (p.x != nullptr && p.s_x >= 0) copy(TS{}, p.s_x, p.x, p.x_e);
       if (OWN && gated) ring_copy<TC, P, kStep>(s + p.s_gate * kRowThreads * 16, gate + ahead.row * p.gate_ld, there);
       if (OWN && adaptive) ring_copy<TC, P, kStep>(s + p.s_g * kRowThreads * 16, gs + ahead.row * p.gate_shift_ld, there);
       ahead.next(p.plan, team, step);
@@ -280,7 +280,14 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 || (P == 3 &&
     }
     if (p.x != nullptr) {
       Pairs x[P];
-      take(TS{}, p.s_x, p.x, p.x_e, x);
+      if (VEC && GATES == kOwnAdaptive && P == 4 && sizeof(TC) == 4 && p.s_x < 0) {
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+          x[q] = p.x_e != nullptr ? load_piece8<VEC>(static_cast<const uint8_t*>(p.x) + o + q * kStep, p.x_e + e + (ch + q * kStep) / kGroup8, k[q])
+                                  : load_piece<TS, VEC>(static_cast<const TS*>(p.x) + o + q * kStep, k[q]);
+      } else {
+        take(TS{}, p.s_x, p.x, p.x_e, x);
+      }
 #pragma unroll
       for (int q = 0; q < P; ++q) {
         const Pairs v = mul(t[q], x[q]);
@@ -449,11 +456,13 @@ int launch(cudaStream_t stream, GradParams p, const Sums& sums, long long rows, 
   p.s_dy = place(p.norm != kNoNorm, false, kC);
   p.s_r = place(p.norm != kNoNorm, p.r_e != nullptr, kS);
   p.s_u = place(p.dgate != nullptr, p.u_e != nullptr, kC);
-  p.s_x = place(p.x != nullptr, p.x_e != nullptr, kS);
   p.s_gate = place(OWN && p.gate != nullptr, false, kC);
   p.s_g = place(OWN && p.gate_shift != nullptr, false, kC);
+  // (seven float32 tensors of more than 768 channels, or six and x in 8 bits, are more than the ring holds)
+  constexpr int kStage = VEC ? depth<TS, TC, P, OWN>() * kRowThreads * 16 : 0;
+  p.s_x = p.x != nullptr && (slots + (p.x_e != nullptr ? P : kS)) * kStage + kFlat > kMostRing ? -1 : place(p.x != nullptr, p.x_e != nullptr, kS);
   p.slots = slots;
-  int smem = VEC ? depth<TS, TC, P, OWN>() * slots * kRowThreads * 16 : 0;
+  int smem = slots * kStage;
   if (p.partial != nullptr && smem < kFlat) smem = kFlat;
   p.s_scale = smem / 16 / kRowThreads;
   if (p.x != nullptr) smem += kFlat;

@@ -186,6 +186,20 @@ def test_wide_rows_of_every_tensor_in_float32():
             _check(d, dr, dy, samples, compress=True)
 
 
+@pytest.mark.parametrize("c", [1016, 1024])
+def test_wide_rows_of_seven_float32_tensors(c):
+    """dr, dy, r, u, x, gate and the norm's gates, a row's own: more than a ring of two rows holds, with x as a tensor or in 8 bits."""
+    d, dr, dy = _case(2, 1, 700, c, "f32", scale=True, seed=c)
+    _check(d, dr, dy, 1)
+    _check(d, dr, dy, 1, compress=True)
+    r, y = F.residual_norm(**d)
+    about = dict(scale=d["scale"], gate_shift=d["gate_shift"])
+    x8 = F.compress(d["x"])
+    a = F.residual_norm_backward(dr, dy, r, d["u"], d["gate"], x8, **about)
+    b = F.residual_norm_backward(dr, dy, r, d["u"], d["gate"], F.expand(x8), **about)
+    assert all((s is None and t is None) or torch.equal(s, t) for s, t in zip(a, b))
+
+
 def test_nothing_to_do():
     for groups, l in ((0, 5), (3, 0)):
         d, dr, dy = _case(max(groups, 1), 1, max(l, 1), 64, norm="affine", scale=True)

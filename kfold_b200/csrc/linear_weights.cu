@@ -3,6 +3,7 @@
 // What bounds it: dz and x in, HBM, and their trips through shared memory.  A CTA pair (cta_group::2) multiplies 256 columns of dz by 256 of x over its piece
 // of the rows, so that each operand is read by few pairs; all operands lie across the contraction and are read as they lie.  The bias's gradient, where dz is the
 // gradient itself, is one more product with columns of ones: a pass over dz and a launch less.
+// 147 456 rows, 512 x 256: 44 us (0.87 PFLOP/s, 5.1 TB/s) and 8 for the planes; 18 432 rows, 384 x 1 536: 25 us (0.87 PFLOP/s) and 7.
 #include <mutex>
 
 #include "gemm.cuh"   // st_global_v8
@@ -143,6 +144,7 @@ linear_weights_kernel(const __grid_constant__ CUtensorMap tm_dz, const __grid_co
 #pragma unroll 1
       for (int c = c0; c < c0 + kTile / 2; c += 32) {
         uint32_t v[32];
+        __syncwarp();
         ptx::tmem_ld_32x32b_x32(t_row + c, v);
         ptx::tmem_ld_wait();
         if (n >= p.n) continue;
@@ -190,8 +192,14 @@ int tiles_of(int n, int k) { return cdiv(n, kTile) * cdiv(k, kTile); }
 
 }  // namespace
 
-// Many rows: below some thousand a pair's start and end, and the planes, cost more than tiles of 128 x 128 do (matmul.cu).
-bool linear_weights_ok(long long rows, int n, int k) { return rows >= 4096 && n >= 256 && k >= 256 && tiles_of(n, k) <= pairs_held(); }
+// Many rows: a pair's start and end, and the planes of all pairs, cost more than tiles of 128 x 128 do (matmul.cu) until the products take some microseconds, half
+// as many where a pass over dz for the bias's gradient goes with it.  By pairs and by tiles, bf16: 768 x 768, 4 096 rows 24 and 24 us, 24 576 rows 34 and 40;
+// 512 x 256, 8 192 rows 19 and 12, 49 152 rows 30 and 30; with the bias's gradient 19 and 17, 30 and 38;
+// 63 001 rows of 128 x 128 (half of a tile unused) 15 and 13.
+bool linear_weights_ok(long long rows, int n, int k, bool with_bias) {
+  const double products = static_cast<double>(rows) * n * k;
+  return rows >= 4096 && n >= 256 && k >= 256 && products >= (with_bias ? 2.5e9 : 5e9) && tiles_of(n, k) <= pairs_held();
+}
 
 int linear_weights_bias_planes(int splits, int k) { return splits * cdiv(k, kTile); }
 

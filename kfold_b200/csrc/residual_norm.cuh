@@ -56,18 +56,22 @@ struct Walk {
 };
 
 // A plan for `teams` teams at work at once, `in_warp` of them in a warp: pieces that the teams finish together.  The cost of a round is its samples and, for the
-// gates and the sums, about two more; `join` for pieces that a second kernel has to join.  Never more than two pieces a team.
-inline RowPlan row_plan(long long rows, int samples, int l, long long teams, int in_warp, int join) {
+// gates and the sums, about two more; where a second kernel has to join pieces of `unit_bytes`, written and read, its launch costs 1.3 and seven megabytes one
+// (the gradient of 301 gate rows of five samples of 768 channels: whole 12.9 us, cut 14.4; of 64: 12.4 and 8.9).
+// Never more than two pieces a team.
+inline RowPlan row_plan(long long rows, int samples, int l, long long teams, int in_warp, int unit_bytes) {
   RowPlan p = {};
   p.gate_rows = static_cast<unsigned>(rows / samples);
   p.l = static_cast<unsigned>(l);
   p.samples = samples;
   p.chunks = 1;
-  long long best = -1;
+  double best = 0.;
   for (int k = 1; k <= samples; ++k) {
-    const long long units = static_cast<long long>(p.gate_rows) * k, cost = (units + teams - 1) / teams * ((samples + k - 1) / k + 2) + (k > 1 ? join : 0);
+    const long long units = static_cast<long long>(p.gate_rows) * k;
     if (k > 1 && units > 2 * teams) break;
-    if (best < 0 || cost < best) {
+    const double join = k > 1 && unit_bytes > 0 ? 1.3 + 1.5e-7 * units * unit_bytes : 0.;
+    const double cost = static_cast<double>((units + teams - 1) / teams * ((samples + k - 1) / k + 2)) + join;
+    if (k == 1 || cost < best) {
       best = cost;
       p.chunks = k;
     }
@@ -127,7 +131,8 @@ __device__ __forceinline__ Pairs ring_take(const uint4* slot) {
   else return of_f32(slot[0], slot[kRowThreads]);
 }
 
-// The kernels' shapes: lanes of a team and pieces of a lane.  CALL(LANES, P, VEC) for c channels.
+// The kernels' shapes: lanes of a team and pieces of a lane, two at least where there are, for fewer instructions a row (the gradient of 384 x 384 rows of 128 channels 32 us,
+// 41 with 16 lanes of one).  CALL(LANES, P, VEC) for c channels.
 #define KFB_ROW_SHAPES(c, vec, CALL)                  \
   do {                                                \
     if (vec) {                                        \

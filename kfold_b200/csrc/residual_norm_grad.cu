@@ -7,7 +7,9 @@
 // (row_teams.cuh), which are taken apart in registers.
 // Split: residual_norm.cuh says how rows are walked and come in.  A team keeps the sums over the samples of a gate row in registers; where these samples are
 // cut into pieces, a piece leaves its sums in the workspace and a second kernel adds them in the pieces' order.  Sums over all rows stay in registers from row
-// to row; a block leaves a row of partial sums, added up likewise.  No atomics: the order hangs on the sizes alone.
+// to row; a block leaves a row of partial sums, added up likewise.  No atomics: the order hangs on the sizes alone.  The rows of residual_norm.cu, r from 8 bits where it was kept so:
+//   shared gates   40 us, 3.9 TB/s: 254 registers, the sums of a gate row among them, leave eight warps an SM, whose sums over a row wait on one another
+//   gates of their own, float32 stream   79 us, 5.0 TB/s          128 channels   31 us, 4.3 TB/s, of which 4 are the sums over the blocks
 #include <mutex>
 
 #include "ops_common.cuh"
@@ -471,7 +473,7 @@ int launch(cudaStream_t stream, GradParams p, const Sums& sums, long long rows, 
   const int fit = smem > 0 ? kMostRing / smem : held, limit = held < most_blocks(p.c) ? held : most_blocks(p.c), blocks_per_sm = limit < fit ? limit : fit;
   const long long most = static_cast<long long>(sm_count() < kMostSms ? sm_count() : kMostSms) * blocks_per_sm;
   const bool gates = p.dgate != nullptr || p.dgate_shift != nullptr;
-  p.plan = row_plan(rows, samples, l, most * kWarps * kTeams, kTeams, gates ? 4 : 0);      // (the second launch: 301 gate rows of 5 samples 13.4 -> 10 us in one piece)
+  p.plan = row_plan(rows, samples, l, most * kWarps * kTeams, kTeams, gates ? 2 * 3 * 4 * p.c : 0);
   if (p.plan.chunks == 1 || !gates) p.pieces = nullptr;
   else KFB_CHECK_ARG(p.plan.units <= most_units(p.c), "residual_norm_bwd: %u pieces", p.plan.units);
   const long long want = (p.plan.sets + kWarps - 1) / kWarps;

@@ -131,6 +131,19 @@ def test_many_rows(rows, k, n, act):
     _check(*_case(rows, k, n, residual=act is None, seed=9), act)
 
 
+@pytest.mark.parametrize("rows, k, n", [(30001, 264, 648), (20001, 776, 328), (5001, 1000, 1024), (4100, 2048, 2304), (10001, 512, 520), (9600, 512, 512), (19100, 512, 512)])
+@pytest.mark.parametrize("act", [None, "silu"])
+def test_weights_of_many_rows_and_odd_widths(rows, k, n, act):
+    """Tiles of 256 columns that end inside, one piece of the rows and many, and both sides of where these tiles begin."""
+    _check(*_case(rows, k, n, seed=k), act)
+
+
+@pytest.mark.parametrize("rows, k, n", [(1999, 384, 1536), (4700, 512, 512), (4900, 512, 512), (2300, 768, 1000)])
+def test_both_sides_of_where_pairs_begin(rows, k, n):
+    """Half of the pairs of multiprocessors have a tile, or a few less."""
+    _check(*_case(rows, k, n, residual=True, seed=n), "silu")
+
+
 @pytest.mark.parametrize("rows", [30000, 900001])
 def test_pieces_of_rows_in_float32(rows):
     """What a row keeps in the workspace is 6 (k + n) bytes, of which half a gigabyte is one piece."""
@@ -168,7 +181,7 @@ def test_more_than_2_to_31_elements():
         assert ((dx[p].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + (8 + n / 16) * 2.0 ** -23 * (y[p].double().abs() @ w.double().abs())).all()
 
 
-@pytest.mark.parametrize("rows, k, n", [(300, 64, 72), (20000, 256, 264)])
+@pytest.mark.parametrize("rows, k, n", [(300, 64, 72), (20000, 256, 264), (37000, 264, 520)])
 @pytest.mark.parametrize("act", [None, "gelu"])
 def test_what_lies_behind_the_rows_stays(rows, k, n, act):
     """The entry points write the rows they are given, of buffers that go on."""

@@ -3,7 +3,7 @@
 // What bounds it: dz and x in, HBM, and their trips through shared memory.  A CTA pair (cta_group::2) multiplies 256 columns of dz by 256 of x over its piece
 // of the rows, so that each operand is read by few pairs; all operands lie across the contraction and are read as they lie.  The bias's gradient, where dz is the
 // gradient itself, is one more product with columns of ones: a pass over dz and a launch less.
-// 147 456 rows, 512 x 256: 44 us (0.87 PFLOP/s, 5.1 TB/s) and 8 for the planes; 18 432 rows, 384 x 1 536: 25 us (0.87 PFLOP/s) and 7.
+// 147 456 rows, 512 x 256: 44 us (0.87 PFLOP/s, 5.1 TB/s) and 8 for the planes; 18 432 rows, 384 x 1 536: 25 us (0.87 PFLOP/s) and 6.
 #include <mutex>
 
 #include "gemm.cuh"   // st_global_v8

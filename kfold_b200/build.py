@@ -24,6 +24,9 @@ FLAGS = [
     "--use_fast_math", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
     "--expt-relaxed-constexpr", "-rdc=true",
 ]
+# Where results are to be those of elementary float32 operations bit for bit: what --use_fast_math says but for the fast exponential.
+EXACT_EXP = {"residual_norm.cu"}
+EXACT_EXP_FLAGS = ["-ftz=true", "-prec-div=false", "-prec-sqrt=false"]
 
 
 def _sources():
@@ -45,7 +48,8 @@ def build(verbose: bool = False, force: bool = False) -> str:
         o = os.path.join(OUT_DIR, src[:-3] + ".o")
         objs.append(o)
         if force or not os.path.exists(o) or os.path.getmtime(o) < max(os.path.getmtime(s), hdr_m):
-            cmd = [NVCC, *FLAGS, "-c", s, "-o", o]
+            flags = [f for f in FLAGS if f != "--use_fast_math"] + EXACT_EXP_FLAGS if src in EXACT_EXP else FLAGS
+            cmd = [NVCC, *flags, "-c", s, "-o", o]
             if verbose:
                 cmd.insert(1, "-Xptxas")
                 cmd.insert(2, "-v")

@@ -110,7 +110,7 @@ __device__ __forceinline__ float inverse_step8(uint32_t e) { return e == 255u ||
 __device__ __forceinline__ uint2 bytes8(const Pairs& p, uint32_t e) {
   const float inverse = inverse_step8(e);
   Pairs t = p;
-  if (e == 254u) t = each(p, [inverse](float v) { return fminf(fmaxf(v, -127.f / inverse), 127.f / inverse); });      // (the one that stops short)
+  if (e == 254u) t = each(p, [](float v) { return fminf(fmaxf(v, __uint_as_float(0xff7e0000u)), __uint_as_float(0x7f7e0000u)); });      // (the one that stops short, at 127 2^121)
   t = fma(t, both(inverse), both(12582912.f));
   uint32_t w[2];
 #pragma unroll
@@ -260,24 +260,5 @@ __device__ __forceinline__ float gate_at(float a) {
 }
 __device__ __forceinline__ float open_of(float q) { return __float_as_int(q) < 0 ? -q : 1.f - q; }
 __device__ __forceinline__ float slope_of(float q) { return fmaf(-q, q, fabsf(q)); }
-
-// The same to float32's own rounding, for sums that are stored and then put away in 8 bits: where the sum lies near a border between two stored values, an
-// error of the fast exponential (some 2^-21) decides ten times as often as rounding does.  exp(y) by its Taylor series to y^7 / 7! for |y| <= ln 2 / 2
-// (the rest is below 2^-27), the powers of two apart; one step of Newton's iteration for the reciprocal.
-__device__ __forceinline__ float exact_gate_at(float a) {
-  const float x = -fabsf(a), k = rintf(x * 1.44269504f);
-  const float y = fmaf(k, -3.19461849e-5f, fmaf(k, -0.693115234375f, x));      // x - k ln 2, ln 2 in two parts, the first of 12 bits
-  float t = 1.f / 5040.f;
-  t = fmaf(t, y, 1.f / 720.f);
-  t = fmaf(t, y, 1.f / 120.f);
-  t = fmaf(t, y, 1.f / 24.f);
-  t = fmaf(t, y, 1.f / 6.f);
-  t = fmaf(t, y, 0.5f);
-  t = fmaf(t, y, 1.f);
-  t = fmaf(t, y, 1.f);
-  const float e = x < -87.f ? 0.f : __int_as_float(__float_as_int(t) + (static_cast<int>(k) << 23));
-  const float w = 1.f + e, d = __fdividef(1.f, w);
-  return copysignf(e * fmaf(d, fmaf(-w, d, 1.f), d), a);
-}
 
 }  // namespace kfb

@@ -200,6 +200,22 @@ def test_wide_rows_of_seven_float32_tensors(c):
     assert all((s is None and t is None) or torch.equal(s, t) for s, t in zip(a, b))
 
 
+@pytest.mark.parametrize("samples", [1, 4])
+@pytest.mark.parametrize("c", [128, 100, 768])
+@pytest.mark.parametrize("types", list(TYPES))
+def test_the_stream_is_that_of_elementary_operations(samples, c, types):
+    """Bit for bit, gates of every size among them; so are the rows in 8 bits."""
+    d, _, _ = _case(2, samples, 500, c, types, norm=None, scale=types == "f32")
+    d["gate"] = (d["gate"].float() * torch.linspace(0.1, 40, c, device=DEV)).to(d["gate"].dtype)
+    r, _, kept = F.residual_norm(**d, samples=samples, compress=True)
+    gate = 1.0 / (1.0 + torch.exp(-d["gate"].float())).repeat_interleave(samples, 0)
+    x = d["x"].float() if d["scale"] is None else d["x"].float() * d["scale"]
+    want = (x + gate * d["u"].float()).to(r.dtype)
+    assert torch.equal(r, want)
+    again = F.compress(want)
+    assert torch.equal(kept.values, again.values) and torch.equal(kept.exponents, again.exponents)
+
+
 def test_nothing_to_do():
     for groups, l in ((0, 5), (3, 0)):
         d, dr, dy = _case(max(groups, 1), 1, max(l, 1), 64, norm="affine", scale=True)

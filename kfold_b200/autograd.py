@@ -32,7 +32,8 @@ _this_thread = threading.local()
 def compressed(enabled: bool = True):
     """``with compressed():`` -- calls of this thread keep rows for the backward pass in 8 bits (``functional.compress``: 33 / 32 bytes a value, off by
     at most 2^-7 of the largest of 32 neighbours): the inputs of layer_norm, gated_feed_forward and fused_linear, the stream and the block's
-    output of residual_norm.  Results of the forward pass stay what they are; gradients are those at the kept values."""
+    output of residual_norm.  Results of the forward pass stay what they are, but for the last bit of layer_norm, which residual_norm's kernel then
+    computes; gradients are those at the kept values."""
     before = _compressing()
     _this_thread.compressed = enabled
     try:

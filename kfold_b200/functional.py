@@ -487,7 +487,7 @@ def residual_norm(x: torch.Tensor | None, u: torch.Tensor | None = None, gate: t
 
     x (..., C) is the stream and gives r its type; u and y have the type that the blocks compute in: the stream's, or bfloat16 beside a float32
     stream.  Each of u, gate, scale (C,), weight (C,), bias (C,) may be missing, x too where u is there (r is of u's type then).  Without u and scale r is x itself; without
-    ``norm`` y is None.  What is normalised is r as it is stored.  ``gate`` (..., C) and ``gate_shift`` (..., 2 C), of u's type, have a row for
+    ``norm`` y is None.  r is what elementary float32 operations give, sigmoid as 1 / (1 + exp(-gate)), rounded once; what is normalised is r as it is stored.  ``gate`` (..., C) and ``gate_shift`` (..., 2 C), of u's type, have a row for
     ``samples`` entries: x (groups * samples, L, C), flattened, takes gate (groups, L, C).  ``compress``: a third result, r in 8 bits.  Any C up to 1024."""
     base = u if x is None else x
     if base is None:

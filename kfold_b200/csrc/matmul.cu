@@ -8,7 +8,8 @@
 // start and end (some 3 us).  331 rows of 384 channels, 1 536 hidden ones: dx and the weights' gradients, 2.3 GFLOP, in one launch of 9 us.  Many rows of
 // the usual widths have kernels of their own.
 // fp32-accurate mode: three parts an operand, six products, x0 w0 in an accumulator of its own (the tensor core cuts off relative to the
-// accumulator at every step: the five small ones keep their small error apart).
+// accumulator at every step: the five small ones keep their small error apart).  That cut goes with the length of the contraction, 1e-6 of the result after 1 024: `turns`
+// accumulators that take the blocks of k in turn are smaller and are cut a third as often each (3e-7; float32 sums one after the other 6e-7).  A CTA has an SM, and its tensor memory, to itself.
 #include "matmul.cuh"
 
 #include "gemm.cuh"   // split3, epi_store_chunk
@@ -36,6 +37,7 @@ struct MmBatch {
   CUtensorMap a[kMostMatmuls], b[kMostMatmuls];
   MmParams p[kMostMatmuls];
   MatmulTail tail;                                 // of a launch of one product
+  int turns;                                       // PARTS = 3
   int end[kMostMatmuls];                           // blocks of the grid up to and with each product
 };
 
@@ -119,7 +121,9 @@ __device__ __forceinline__ void tail_chunk(const MatmulTail& t, const EpiSeg& ou
 template <int PARTS, bool TAIL>
 __global__ void __launch_bounds__(threads<TAIL>(), PARTS == 3 ? 1 : 2) matmul_kernel(const __grid_constant__ MmBatch batch) {
   constexpr int kStages = stages<PARTS>(), kTileN = tile_columns<TAIL>(), kBytes = kOperand + kTileN * kK * 2;
-  constexpr uint32_t kCols = PARTS == 3 ? 256 : 128;
+  // columns of the large products' accumulators, and behind the first of the small ones'
+  constexpr uint32_t kCols = PARTS == 3 ? 512 : 128;
+  auto large = [](int turn) { return static_cast<uint32_t>(turn == 0 ? 0 : 128 + 128 * turn); };
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * kStage);
@@ -210,7 +214,8 @@ __global__ void __launch_bounds__(threads<TAIL>(), PARTS == 3 ? 1 : 2) matmul_ke
           used[i] = st;
           if (++st == kStages) { st = 0; ph ^= 1u; }
           if (i == 0) {
-            product(0, 0, tmem, kb == first);
+            if (PARTS == 3) product(0, 0, tmem + large((kb - first) % batch.turns), kb - first < batch.turns);
+            else product(0, 0, tmem, kb == first);
           } else {
             product(0, i, tmem + 128, kb == first && i == 1);
             product(i, 0, tmem + 128, false);
@@ -253,6 +258,12 @@ __global__ void __launch_bounds__(threads<TAIL>(), PARTS == 3 ? 1 : 2) matmul_ke
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
         if (PARTS == 3) {
+          for (int turn = 1; turn < batch.turns && turn < last - first; ++turn) {
+            ptx::tmem_ld_32x32b_x32(t_row + large(turn) + c, raw);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(raw[i]);
+          }
           ptx::tmem_ld_32x32b_x32(t_row + 128 + c, raw);
           ptx::tmem_ld_wait();
 #pragma unroll
@@ -351,7 +362,7 @@ int launch_matmuls(cudaStream_t stream, const MatmulArgs* list, int count, const
     const MatmulArgs& a = list[i];
     KFB_CHECK_ARG(a.m > 0 && a.n > 0 && a.k > 0 && a.k < (1ll << 31) && a.splits >= 1, "matmul: m %d n %d k %lld, %d pieces", a.m, a.n, a.k, a.splits);
     KFB_CHECK_ARG(a.out_fp32 || (a.splits == 1 && !a.accumulate), "matmul: pieces and sums need an fp32 result");
-    KFB_CHECK_ARG(a.precise == list[0].precise, "matmul: products of both modes in one launch");
+    KFB_CHECK_ARG(a.precise == list[0].precise && a.turns == list[0].turns && a.turns >= 0 && a.turns <= kMostTurns, "matmul: products of both modes in one launch, or %d turns", a.turns);
     MmParams& p = batch.p[i];
     p.m = a.m;
     p.n = a.n;
@@ -381,6 +392,7 @@ int launch_matmuls(cudaStream_t stream, const MatmulArgs* list, int count, const
     batch.end[i] = blocks;
   }
   for (int i = count; i < kMostMatmuls; ++i) batch.end[i] = blocks;
+  batch.turns = list[0].turns > 0 ? list[0].turns : 1;
   LaunchScope scope(stream, tag);
   auto run = [&](auto kernel_of, int smem) { return launch_kernel(stream, kernel_of, blocks, list[0].tail != nullptr ? threads<true>() : threads<false>(), smem, batch); };
   if (list[0].precise) {

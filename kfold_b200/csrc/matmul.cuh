@@ -40,7 +40,9 @@ struct MatmulArgs {
   int accumulate;        // fp32 D only: add to what D holds
   int precise;           // operands are three bf16 parts each
   const MatmulTail* tail;
+  int turns;             // fp32-accurate mode: accumulators that the large products' blocks of k go to in turn (matmul.cu), up to kMostTurns; 0 is one
 };
+static constexpr int kMostTurns = 3;
 static constexpr int kMostMatmuls = 3;
 // Up to kMostMatmuls products in one launch, all of them precise or none.
 int launch_matmuls(cudaStream_t stream, const MatmulArgs* list, int count, const char* tag);

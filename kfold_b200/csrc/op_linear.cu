@@ -282,6 +282,7 @@ int launch_tail(cudaStream_t s, const MatOperand& x, const MatOperand& w, const 
   a.splits = 1;
   a.plane_d = plane;
   a.precise = precise;
+  a.turns = kMostTurns;
   a.tail = &tail;
   return launch_matmul(s, a, tag);
 }
@@ -399,6 +400,7 @@ KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, c
       a.out_fp32 = precise;
       a.splits = 1;
       a.precise = precise;
+      a.turns = kMostTurns;
     }
     if (dw != nullptr && m.dw) {
       KFB_TRY(launch_linear_weights(s, dz.ptr, xp, m.planes, m.ones ? m.partial : nullptr, m.splits, r0 > 0 ? 1 : 0, count, n, k));
@@ -419,6 +421,7 @@ KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, c
       a.plane_d = nk;
       a.accumulate = r0 > 0;
       a.precise = precise;
+      a.turns = kMostTurns;
     }
     if (products > 0) KFB_TRY(launch_matmuls(s, list, products, "fused_linear_grads"));
     Sum of_w = {m.planes, m.splits, nk, last && !m.whole ? dw : nullptr, dw_dtype == KFB_FP32, 0, 1};

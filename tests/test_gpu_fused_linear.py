@@ -138,6 +138,19 @@ def test_weights_of_many_rows_and_odd_widths(rows, k, n, act):
     _check(*_case(rows, k, n, seed=k), act)
 
 
+@pytest.mark.parametrize("rows, k, n", [(331, 256, 1024), (331, 2048, 64), (3000, 64, 64), (70, 24, 8)])
+def test_the_float32_mode_is_float32(rows, k, n):
+    """Root mean square of the errors: what is cut off at a step of the contraction is at most 2^-23 of an accumulator, 2^-24 on average, at k / 16 / 3 steps for each of
+    three accumulators whose squares add up to the result's: 2^-24 k / 48 of it, and float32's own rounding and parts that are left out, 2^-23 together, twice over."""
+    x, w, _, _, dy = _case(rows, k, n, F32, bias=False, seed=3)
+    off = lambda got, ref: ((got.double() - ref).square().mean() / ref.square().mean()).sqrt().item()
+    room = lambda terms: 2 * (2.0 ** -24 * terms / 48 + 2.0 ** -23)
+    dx, dw, _ = F.fused_linear_backward(dy, x, w)
+    assert off(F.fused_linear(x, w), x.double() @ w.double().t()) <= room(k)
+    assert off(dx, dy.double() @ w.double()) <= room(n)
+    assert off(dw, dy.double().t() @ x.double()) <= room(rows)
+
+
 @pytest.mark.parametrize("rows, k, n", [(1999, 384, 1536), (4700, 512, 512), (4900, 512, 512), (2300, 768, 1000)])
 def test_both_sides_of_where_pairs_begin(rows, k, n):
     """Half of the pairs of multiprocessors have a tile, or a few less."""

@@ -99,7 +99,7 @@ def test_widths_and_types(c, types):
     _check(*_case(2, 1, 11, c, types, norm="affine", gate=False, scale=True, seed=c), 1, compress=True)
 
 
-@pytest.mark.parametrize("groups, samples, l", [(1, 1, 1), (1, 5, 1), (1, 2, 3), (3, 4, 5), (1, 48, 2), (1, 48, 37), (7, 1, 33), (1, 5, 301), (2, 7, 130), (1, 3, 5000), (5, 1, 4000)])
+@pytest.mark.parametrize("groups, samples, l", [(1, 1, 1), (1, 5, 1), (1, 2, 3), (3, 4, 5), (1, 48, 2), (1, 48, 37), (7, 1, 33), (1, 5, 301), (2, 7, 130), (1, 3, 5000), (5, 1, 4000), (1, 3001, 2)])
 @pytest.mark.parametrize("c", [64, 128, 768])
 def test_rows_and_samples(groups, samples, l, c):
     """Gate rows that outnumber the teams, and too few of them: both ways of dividing the samples."""

@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 || (P == 3 &&
   int stage = 0;
   while (here.set < p.plan.sets) {
     const bool row_there = here.left > 0;
-    uint32_t r_ex[P];                        // r's exponents where they come in no words: asked for before the wait
+    uint32_t r_ex[P];                        // r's exponents where they come in no words: asked for before the wait; nothing without a norm
     if constexpr (VEC) {
       fetch(stage == 0 ? kDepth - 1 : stage - 1);
       if (p.r_e != nullptr && !p.words) {
@@ -142,20 +142,24 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 || (P == 3 &&
     int k[P];                                // channels that are there
 #pragma unroll
     for (int q = 0; q < P; ++q) k[q] = row_there ? inside[q] : 0;
-    // All pieces of a tensor, or of its rows in 8 bits.  (A question that is the same for all pieces is asked once: the pieces' instructions then lie side by side.)
-    auto take = [&](auto tag, int slot, const void* t, const uint8_t* exponents, Pairs (&v)[P]) {
+    // All pieces of a tensor, or of its rows in 8 bits.  is_r: it is r, whose exponents are in r_ex; others read theirs.  (Slots do not tell r from others: what is not there
+    // takes none.)  (A question that is the same for all pieces is asked once: the pieces' instructions then lie side by side.)
+    auto take = [&](auto tag, auto is_r, int slot, const void* t, const uint8_t* exponents, Pairs (&v)[P]) {
       using E = decltype(tag);
+      constexpr bool kIsR = decltype(is_r)::value;
       if (exponents == nullptr) {
 #pragma unroll
         for (int q = 0; q < P; ++q) {
           if constexpr (VEC) v[q] = ring_take<E>(s + (slot + q * (static_cast<int>(sizeof(E)) / 2)) * kRowThreads);
           else v[q] = load_piece<E, VEC>(static_cast<const E*>(t) + o + q * kStep, k[q]);
         }
-      } else if (VEC && (p.words || slot == p.s_r)) {
+      } else if (VEC && (kIsR || p.words)) {
 #pragma unroll
         for (int q = 0; q < P; ++q) {
           const uint4 w = s[(slot + q) * kRowThreads];
-          v[q] = values8(make_uint2(w.x, w.y), p.words ? w.z >> (ch + q * kStep) / kGroup8 % 4 * 8 & 255u : r_ex[q]);
+          uint32_t ex = w.z >> (ch + q * kStep) / kGroup8 % 4 * 8 & 255u;
+          if constexpr (kIsR) ex = p.words ? ex : r_ex[q];
+          v[q] = values8(make_uint2(w.x, w.y), ex);
         }
       } else {
 #pragma unroll
@@ -184,8 +188,8 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 || (P == 3 &&
     Pairs t[P];
     if (p.norm != kNoNorm) {
       Pairs z[P], g[P], d[P];
-      take(TS{}, p.s_r, p.r, p.r_e, z);
-      take(TC{}, p.s_dy, p.dy, nullptr, d);
+      take(TS{}, std::true_type{}, p.s_r, p.r, p.r_e, z);
+      take(TC{}, std::false_type{}, p.s_dy, p.dy, nullptr, d);
       if (OWN && adaptive) {
 #pragma unroll
         for (int q = 0; q < P; ++q) {
@@ -228,7 +232,7 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 || (P == 3 &&
         z[q] = mul(z[q], rstd2);
         t[q] = mul(rstd2, fma(z[q], minus_mean_gz, add(g[q], minus_mean_g)));
       }
-      if constexpr (VEC && P > 1) take(TC{}, p.s_dy, p.dy, nullptr, d);               // (read again: it frees the registers meanwhile)
+      if constexpr (VEC && P > 1) take(TC{}, std::false_type{}, p.s_dy, p.dy, nullptr, d);               // (read again: it frees the registers meanwhile)
       if (OWN && adaptive) {
         if (p.dgate_shift != nullptr) {
           TC* to = static_cast<TC*>(p.dgate_shift) + 2 * (o - ch) + ch;
@@ -246,16 +250,16 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 || (P == 3 &&
         }
       }
       if (p.dr != nullptr) {
-        take(TS{}, 0, p.dr, nullptr, z);
+        take(TS{}, std::false_type{}, 0, p.dr, nullptr, z);
 #pragma unroll
         for (int q = 0; q < P; ++q) t[q] = add(t[q], z[q]);
       }
     } else {
-      take(TS{}, 0, p.dr, nullptr, t);
+      take(TS{}, std::false_type{}, 0, p.dr, nullptr, t);
     }
     if (p.dgate != nullptr) {
       Pairs u[P];
-      take(TC{}, p.s_u, p.u, p.u_e, u);
+      take(TC{}, std::false_type{}, p.s_u, p.u, p.u_e, u);
       if constexpr (OWN) {
         TC* to = static_cast<TC*>(p.dgate) + o;
 #pragma unroll
@@ -288,7 +292,7 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 || (P == 3 &&
           x[q] = p.x_e != nullptr ? load_piece8<VEC>(static_cast<const uint8_t*>(p.x) + o + q * kStep, p.x_e + e + (ch + q * kStep) / kGroup8, k[q])
                                   : load_piece<TS, VEC>(static_cast<const TS*>(p.x) + o + q * kStep, k[q]);
       } else {
-        take(TS{}, p.s_x, p.x, p.x_e, x);
+        take(TS{}, std::false_type{}, p.s_x, p.x, p.x_e, x);
       }
 #pragma unroll
       for (int q = 0; q < P; ++q) {

@@ -16,30 +16,45 @@ refused.  The calls are CUDA only, as everything here.
 from __future__ import annotations
 
 import threading
-from contextlib import contextmanager
+from contextlib import ContextDecorator
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import functional as F
 
-__all__ = ["layer_norm", "gated_feed_forward", "dropout", "residual_norm", "fused_linear", "compressed"]
+__all__ = ["layer_norm", "gated_feed_forward", "dropout", "residual_norm", "fused_linear", "compressed", "checkpoint_contexts"]
 
 _this_thread = threading.local()
 
 
-@contextmanager
-def compressed(enabled: bool = True):
+class compressed(ContextDecorator):
     """``with compressed():`` -- calls of this thread keep rows for the backward pass in 8 bits (``functional.compress``: 33 / 32 bytes a value, off by
     at most 2^-7 of the largest of 32 neighbours): the inputs of layer_norm, gated_feed_forward and fused_linear, the stream and the block's
     output of residual_norm.  Results of the forward pass stay what they are, but for the last bit of layer_norm, which residual_norm's kernel then
-    computes; gradients are those at the kept values."""
-    before = _compressing()
-    _this_thread.compressed = enabled
-    try:
-        yield
-    finally:
-        _this_thread.compressed = before
+    computes; gradients are those at the kept values.
+
+    A checkpoint repeats the forward pass on a thread of autograd's own, where this one's choice does not hold: the ``with`` stands inside the function that is
+    checkpointed, or the checkpoint is given ``checkpoint_contexts``."""
+
+    def __init__(self, enabled: bool = True):
+        self.enabled = enabled
+
+    def __enter__(self) -> None:
+        if not hasattr(_this_thread, "before"):
+            _this_thread.before = []
+        _this_thread.before.append(_compressing())
+        _this_thread.compressed = self.enabled
+
+    def __exit__(self, *exc) -> None:
+        _this_thread.compressed = _this_thread.before.pop()
+
+
+def checkpoint_contexts() -> tuple:
+    """``checkpoint(block, x, use_reentrant=False, context_fn=checkpoint_contexts)`` (torch.utils.checkpoint): the pass that is repeated keeps rows as the first
+    one does, which is as this thread keeps them now (``compressed``)."""
+    as_now = compressed(_compressing())
+    return as_now, as_now
 
 
 def _compressing() -> bool:

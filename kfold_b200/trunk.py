@@ -77,7 +77,10 @@ class ParcaeRecurrence(nn.Module):
         ln = self.layernorm_z
         with torch.autocast(z.device.type, enabled=False):
             delta = tF.softplus(self.parcae_log_delta.float())
-            a = torch.exp(-delta * torch.exp(self.parcae_log_a.float())).to(torch.bfloat16).float()
+            a = torch.exp(-delta * torch.exp(self.parcae_log_a.float()))
+            # its value is rounded as in inference, its gradient, a float32 sum over all rows, is not (the difference of a number and what it rounds to is
+            # exact, and so is the sum)
+            a = a + (a.detach().to(torch.bfloat16).float() - a.detach())
             b = delta[:, None] * self.parcae_b_cont.float()
             un = A.layer_norm(u, ln.weight, ln.bias, ln.eps, out_dtype=torch.bfloat16)
             return A.residual_norm(z, A.fused_linear(un, b), scale=a, norm=False)[0]

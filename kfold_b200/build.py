@@ -24,8 +24,8 @@ FLAGS = [
     "--use_fast_math", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
     "--expt-relaxed-constexpr", "-rdc=true",
 ]
-# Where results are to be those of elementary float32 operations bit for bit: what --use_fast_math says but for the fast exponential.
-EXACT_EXP = {"residual_norm.cu"}
+# Where gates of float32 logits are to be those of elementary float32 operations: what --use_fast_math says but for the fast exponential.
+EXACT_EXP = {"residual_norm.cu", "residual_norm_grad.cu"}
 EXACT_EXP_FLAGS = ["-ftz=true", "-prec-div=false", "-prec-sqrt=false"]
 
 

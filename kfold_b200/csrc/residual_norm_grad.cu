@@ -171,11 +171,11 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 || (P == 3 &&
       Pairs t;
       if constexpr (VEC) t = ring_take<TC>(s + (slot + q * kC) * kRowThreads);
       else t = load_piece<TC, VEC>(row + q * kStep, k[q]);
-      return each(t, [](float a) { return gate_at(a); });
+      return each(t, [](float a) { return gate_at<TC>(a); });
     };
     if (!OWN && here.at == 0) {
       const unsigned gate_row = here.gate_row(p.plan);
-      auto opened = [](float a) { return open_of(gate_at(a)); };
+      auto opened = [](float a) { return open_of(gate_at<TC>(a)); };
       if (gated) {
 #pragma unroll
         for (int q = 0; q < P; ++q) open[OWN ? 0 : q] = each(load_piece<TC, VEC>(gate + gate_row * p.gate_ld + q * kStep, k[q]), opened);
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kRowThreads, P == 1 ? 4 : P == 2 || (P == 3 &&
         // the end of a piece: the gates' gradients from the sums over their samples, the logits once more for their slopes; or the sums for the second kernel
         const bool there = here.unit < p.plan.units;
         const unsigned gate_row = here.gate_row(p.plan);
-        auto slope = [](float a) { return slope_of(gate_at(a)); };
+        auto slope = [](float a) { return slope_of(gate_at<TC>(a)); };
 #pragma unroll 1
         for (int which = 0; which < 2; ++which) {
           // the norm's gates and shifts, the output gate
@@ -420,12 +420,12 @@ __global__ void __launch_bounds__(256) residual_norm_gates_kernel(const float* p
     float v;
     if (dgs != nullptr) {
       TC* d = dgs + static_cast<long long>(row) * 2 * c + ch;
-      v = s[0] * slope_of(gate_at(static_cast<float>(gs[row * gs_ld + ch])));
+      v = s[0] * slope_of(gate_at<TC>(static_cast<float>(gs[row * gs_ld + ch])));
       store_vec<1>(d, &v);
       store_vec<1>(d + c, &s[1]);
     }
     if (dgate != nullptr) {
-      v = s[2] * slope_of(gate_at(static_cast<float>(gate[row * gate_ld + ch])));
+      v = s[2] * slope_of(gate_at<TC>(static_cast<float>(gate[row * gate_ld + ch])));
       store_vec<1>(dgate + static_cast<long long>(row) * c + ch, &v);
     }
   }

@@ -252,11 +252,23 @@ template <int LATER>
 __device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory"); }
 
 // ---- gates
+// A reciprocal of 1 ... 10^38, rounded correctly by Markstein's step (IBM J. Res. Dev. 34, 1990) from one within a unit.
+__device__ __forceinline__ float reciprocal_of(float w) {
+  const float d = __fdividef(1.f, w);
+  return fmaf(fmaf(-w, d, 1.f), d, d);
+}
 // A gate with logit a as one number: sigmoid(-|a|), with a's sign.  Both sigmoid(a) and its slope come from it without the subtraction that would
-// lose the slope of an open gate.
+// lose the slope of an open gate.  T: the logits' type.  What bf16 logits open or shut is bf16 too (y and u, or dy, though dx may be
+// float32), 2^-9, beside which the fast exponential's 2^-21 is nothing; float32 logits take the exact one, in files that are built with it, and the reciprocal above.
+template <typename T>
 __device__ __forceinline__ float gate_at(float a) {
-  const float e = __expf(-fabsf(a));
-  return copysignf(__fdividef(e, 1.f + e), a);
+  if constexpr (sizeof(T) == 2) {
+    const float e = __expf(-fabsf(a));
+    return copysignf(__fdividef(e, 1.f + e), a);
+  } else {
+    const float e = expf(-fabsf(a));
+    return copysignf(e * reciprocal_of(1.f + e), a);
+  }
 }
 __device__ __forceinline__ float open_of(float q) { return __float_as_int(q) < 0 ? -q : 1.f - q; }
 __device__ __forceinline__ float slope_of(float q) { return fmaf(-q, q, fabsf(q)); }

@@ -4,7 +4,7 @@
 
 Each .cu file is compiled to an object with nvcc (in parallel) and linked into one
 shared library that exports the C ABI declared in include/kfold_b200.h.  Objects are
-rebuilt only when a source or header is newer.
+rebuilt only when a source, a header or this file, which has their flags, is newer.
 """
 from __future__ import annotations
 
@@ -33,21 +33,22 @@ def _sources():
     return sorted(f for f in os.listdir(CSRC) if f.endswith(".cu"))
 
 
-def _headers_mtime() -> float:
-    hs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
-    hs.append(os.path.join(os.path.dirname(PKG), "include", "kfold_b200.h"))
-    return max(os.path.getmtime(h) for h in hs)
+def _shared_mtime() -> float:
+    """Of what every object hangs on."""
+    shared = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
+    shared += [os.path.join(os.path.dirname(PKG), "include", "kfold_b200.h"), os.path.abspath(__file__)]
+    return max(os.path.getmtime(f) for f in shared)
 
 
 def build(verbose: bool = False, force: bool = False) -> str:
     os.makedirs(OUT_DIR, exist_ok=True)
-    hdr_m = _headers_mtime()
+    shared_m = _shared_mtime()
     jobs, objs = [], []
     for src in _sources():
         s = os.path.join(CSRC, src)
         o = os.path.join(OUT_DIR, src[:-3] + ".o")
         objs.append(o)
-        if force or not os.path.exists(o) or os.path.getmtime(o) < max(os.path.getmtime(s), hdr_m):
+        if force or not os.path.exists(o) or os.path.getmtime(o) < max(os.path.getmtime(s), shared_m):
             flags = [f for f in FLAGS if f != "--use_fast_math"] + EXACT_EXP_FLAGS if src in EXACT_EXP else FLAGS
             cmd = [NVCC, *flags, "-c", s, "-o", o]
             if verbose:

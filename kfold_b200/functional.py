@@ -189,7 +189,7 @@ def layer_norm_backward(dy: torch.Tensor, x, weight: torch.Tensor | None, eps: f
                         need_bias: bool = True):
     """Gradient of ``layer_norm(x, weight, bias, eps)``: (dx, dweight, dbias) from dy, of y's shape, bfloat16 or float32.
 
-    dx is of x's dtype; dweight, of the weight's shape, and dbias (C,) are float32 (None without a weight or where not asked for).  Any
+    dx is of x's dtype; dweight, of the weight's shape (None without a weight), and dbias (C,) are float32, None where not asked for.  Any
     width up to 1024.  The row's statistics are taken from x again, nothing has to be kept from the forward pass; sums over the rows have a
     fixed order.  x may be ``Compressed``: dy is then of its type, or bfloat16."""
     if type(x) is Compressed:
@@ -540,7 +540,7 @@ def residual_norm_backward(dr: torch.Tensor | None, dy: torch.Tensor | None, r, 
 
     ``r`` is the forward pass's, a tensor or ``Compressed``; ``u`` too, whose values are read for the gate's gradient only, and ``x``, for the
     scale's only (either may be left out where that is not asked for; du is then of dy's type, or of dr's).  dx is of the stream's type, du, dgate and d gate_shift of the blocks';
-    those of scale, weight and bias are float32.  Gates that samples share get the samples' sum.  Without gate and scale dx and du of one type are one tensor."""
+    those of scale and weight, of their shapes, and bias (C,) are float32.  Gates that samples share get the samples' sum.  Without gate and scale dx and du of one type are one tensor."""
     base, first = _on(r), dy if dy is not None else dr
     if first is None:
         raise ValueError("residual_norm_backward: neither dr nor dy")
@@ -579,7 +579,7 @@ def residual_norm_backward(dr: torch.Tensor | None, dy: torch.Tensor | None, r, 
     dw = _dense_like(weight, torch.float32) if need_weight else None
     db = None
     if need_bias:
-        db = _dense_like(weight, torch.float32) if weight is not None else torch.empty(c, dtype=torch.float32, device=first.device)
+        db = _dense_like(weight, torch.float32) if weight is not None and weight.dim() == 1 else torch.empty(c, dtype=torch.float32, device=first.device)
     dscale = _dense_like(scale, torch.float32) if need_scale else None
     lib = L.lib()
     ws, size = None, 0

@@ -196,10 +196,9 @@ int launch_sums(cudaStream_t stream, const Sum& a, const Sum& b) {
 // ------------------------------------------------------------------------------------------------ sizes
 bool widths_ok(int k, int n) { return k > 0 && k % 8 == 0 && n > 0 && n % 8 == 0 && k <= 65536 && n <= 65536; }
 
-// Rows of a piece: as many as keep what a row needs in the workspace below half a gigabyte.
+// Rows of a piece: as many as keep what a row needs in the workspace below half a gigabyte, and 2^30 at most, so that its rows and tiles are counted in 32 bits.
 long long piece_rows(long long rows, long long per_row) {
-  if (per_row == 0) return rows;
-  const long long most = ((1ll << 29) / per_row + 127) / 128 * 128;
+  const long long most = per_row == 0 ? 1ll << 30 : ((1ll << 29) / per_row + 127) / 128 * 128;
   return rows < most ? rows : most;
 }
 

@@ -151,7 +151,7 @@ int linear_pair_partials(long long rows, int n, int k);       // rows of partial
 int launch_linear_pair(cudaStream_t stream, const LinearPair& p, const char* tag);
 
 // dW planes: plane[s][n][k] = sum over a piece of the rows of dz^T x (linear_weights.cu).
-// bias_planes: null, or [linear_weights_bias_planes][n] sums of dz, over rows that are divided between them.
+// add: to what the planes hold.  bias_planes: null, or [linear_weights_bias_planes][n] sums of dz, over rows that are divided between them (not with add).
 bool linear_weights_ok(long long rows, int n, int k, bool with_bias);
 int linear_weights_splits(long long rows, int n, int k);
 int linear_weights_bias_planes(int splits, int k);

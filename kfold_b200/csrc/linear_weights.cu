@@ -137,7 +137,7 @@ linear_weights_kernel(const __grid_constant__ CUtensorMap tm_dz, const __grid_co
         ptx::tmem_ld_wait();
         if (n < p.n) {
           float* d = p.bias_planes + (static_cast<long long>(split) * k_tiles + turn) * p.n + n;
-          *d = (first_bias < b1 ? __uint_as_float(v[0]) : 0.f) + (p.add ? *d : 0.f);
+          *d = first_bias < b1 ? __uint_as_float(v[0]) : 0.f;
         }
       }
       float* d = p.planes + (static_cast<long long>(split) * p.n + n) * p.k + k0;
@@ -214,6 +214,7 @@ int launch_linear_weights(cudaStream_t stream, const void* dz, const void* x, fl
   KFB_TRY(matrix_map(&ta, dz, rows, n));
   KFB_TRY(matrix_map(&tb, x, rows, k));
   KFB_CHECK_ARG(pairs_held() > 0, "linear: the device holds no pair of this kernel");
+  KFB_CHECK_ARG(bias_planes == nullptr || !add, "linear: sums of dz over one piece of the rows only");
   WeightParams p = {};
   p.n = n;
   p.k = k;

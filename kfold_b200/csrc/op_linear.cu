@@ -228,12 +228,12 @@ Plan plan_of(void* base, long long rows, int k, int n, int act, int precise, int
   p.again = wanted == 0 || act != kIdentity;
   p.z = p.again && !precise && !wide && linear_pair_ok(rows, n, k);
   p.dx = (wanted & 1) && !precise && linear_pair_ok(rows, k, n);
-  const bool ones = (wanted & 4) && !p.again && !wide;
-  p.dw = (wanted & 2) && !precise && linear_weights_ok(rows, n, k, ones);
-  p.ones = p.dw && ones;
   const bool dz = wanted != 0 && (p.again || ((wanted & 3) != 0 && (precise || wide)));
   const bool x3 = precise && (p.again || (wanted & 2)), w3 = precise && (p.again || (wanted & 1));
   p.piece = piece_rows(rows, (dz ? (precise ? 6ll : 2ll) * n : 0) + (x3 ? 6ll * k : 0));
+  const bool ones = (wanted & 4) && !p.again && !wide && p.piece == rows;      // (dW's kernel sums up dy over one piece)
+  p.dw = (wanted & 2) && !precise && linear_weights_ok(rows, n, k, ones);
+  p.ones = p.dw && ones;
   if (dz) p.dz = c.take<__nv_bfloat16>(p.piece * n * (precise ? 3 : 1));
   if (x3) p.x3 = c.take<__nv_bfloat16>(p.piece * k * 3);
   if (w3) p.w3 = c.take<__nv_bfloat16>(3ll * n * k);
@@ -424,8 +424,8 @@ KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, c
     }
     if (products > 0) KFB_TRY(launch_matmuls(s, list, products, "fused_linear_grads"));
     Sum of_w = {m.planes, m.splits, nk, last && !m.whole ? dw : nullptr, dw_dtype == KFB_FP32, 0, 1};
-    // (planes of pieces before are in dW's planes; of db's the ones of the last piece hold all, others are a piece's own)
-    Sum of_b = {m.partial, lines, n, !m.ones || last ? dbias : nullptr, 1, !m.ones && r0 > 0, 1};
+    // (dW's planes hold the pieces before, db's are a piece's own)
+    Sum of_b = {m.partial, lines, n, dbias, 1, r0 > 0, 1};
     KFB_TRY(launch_sums(s, of_w, of_b));
   }
   return KFB_OK;

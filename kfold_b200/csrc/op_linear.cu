@@ -183,7 +183,7 @@ int launch_sums(cudaStream_t stream, const Sum& a, const Sum& b) {
   // thread; of 147 456 rows, 512 -> 256: 54.9 -> 52.4 against four blocks an SM)
   for (Sum& q : p.s) {
     q.parts = 1;
-    while (q.parts < 64 && q.n * q.parts < kSumThreads * 4 * 148 && q.count > 8 * q.parts) q.parts *= 2;
+    while (q.parts < 64 && q.n * q.parts < kSumThreads * 4 * sm_count() && q.count > 8 * q.parts) q.parts *= 2;
   }
   auto blocks = [](const Sum& q) { return q.out == nullptr ? 0u : static_cast<unsigned>((q.n + sum_elements(q.parts) - 1) / sum_elements(q.parts)); };
   p.end = blocks(p.s[0]);
@@ -205,7 +205,7 @@ long long piece_rows(long long rows, long long per_row) {
 // Blocks of 64 rows that a plane of dW takes from a piece: two tiles an SM, but eight blocks at least: below that a plane costs more than it saves
 // (1 024 rows, 384 -> 1 536: 10 us, 15 with two blocks; 8 192 rows of 128 -> 128, where planes are small: 8.5 and 7.9).
 int blocks_per_plane(long long piece, int k, int n) {
-  const long long tiles = static_cast<long long>(cdiv(n, 128)) * cdiv(k, 128), blocks = (piece + 63) / 64, want = 2 * 148 / tiles;
+  const long long tiles = static_cast<long long>(cdiv(n, 128)) * cdiv(k, 128), blocks = (piece + 63) / 64, want = 2 * sm_count() / tiles;
   const long long per = want < 1 ? blocks : (blocks + want - 1) / want;
   return static_cast<int>(per > 8 ? per : blocks < 8 ? blocks : 8);
 }

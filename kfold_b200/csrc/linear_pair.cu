@@ -391,7 +391,7 @@ bool linear_pair_ok(long long rows, int n, int k) {
   return g.groups > 0 && 2 * g.groups * g.n_tiles >= held;
 }
 
-int linear_pair_partials(long long rows, int n, int k) { return grid_of(rows, n, backward_pairs(n)).groups * 2; }
+int linear_pair_partials(long long rows, int n) { return grid_of(rows, n, backward_pairs(n)).groups * 2; }
 
 int launch_linear_pair(cudaStream_t stream, const LinearPair& p, const char* tag) {
   KFB_CHECK_ARG((p.tail == kPlainTail) == (p.by_k != 0), "linear: tail %d with an operand %s k", p.tail, p.by_k ? "across" : "along");

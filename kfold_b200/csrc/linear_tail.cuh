@@ -147,7 +147,7 @@ struct LinearPair {
   int n, k;
 };
 bool linear_pair_ok(long long rows, int n, int k);
-int linear_pair_partials(long long rows, int n, int k);       // rows of partial sums
+int linear_pair_partials(long long rows, int n);       // rows of partial sums
 int launch_linear_pair(cudaStream_t stream, const LinearPair& p, const char* tag);
 
 // dW planes: plane[s][n][k] = sum over a piece of the rows of dz^T x (linear_weights.cu).

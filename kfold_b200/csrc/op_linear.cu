@@ -3,7 +3,7 @@
 //
 // z is computed again where f' needs it: 2 of then 8 operations per row and weight, where keeping it is 2 bytes a row and output.  z stays float32;
 // dz is rounded to bf16 once, as an operand, and db is summed before that.
-// The tail goes with the products: many bf16 rows by CTA pairs (linear_pair.cu), others and the fp32-accurate mode by tiles of 128 x 128 (matmul.cu), dx and dW then
+// The tail goes with the products: many bf16 rows by CTA pairs (linear_pair.cu), others and the fp32-accurate mode by tiles of 128 x 64 (matmul.cu; those without a tail 128 x 128), dx and dW then
 // in one launch.  Rows are taken in pieces, so that the workspace does not grow with them; dW is summed over pieces of rows in float32 planes and added up at the
 // end, in an order that depends on the sizes alone.
 #include "linear_tail.cuh"
@@ -244,7 +244,7 @@ Plan plan_of(void* base, long long rows, int k, int n, int act, int precise, int
     if (!p.whole) p.planes = c.take<float>(static_cast<size_t>(p.splits) * n * k);
   }
   if (wanted & 4) {
-    const long long lines = p.ones ? linear_weights_bias_planes(p.splits, k) : p.z ? linear_pair_partials(p.piece, n, k) : p.again ? 4 * ((p.piece + 127) / 128) : kMostRowBlocks;
+    const long long lines = p.ones ? linear_weights_bias_planes(p.splits, k) : p.z ? linear_pair_partials(p.piece, n) : p.again ? 4 * ((p.piece + 127) / 128) : kMostRowBlocks;
     p.partial = c.take<float>(static_cast<size_t>(lines) * n);
   }
   p.bytes = c.off;
@@ -266,7 +266,7 @@ int check_room(const char* name, const Plan& m, const void* workspace, size_t by
 }
 bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
-// z = x W^T with a tail, by tiles of 128 x 128.
+// z = x W^T with a tail, by tiles of 128 x 64.
 int launch_tail(cudaStream_t s, const MatOperand& x, const MatOperand& w, const MatmulTail& tail, void* d, int out_fp32, long long plane, long long rows, int k, int n,
                 int precise, const char* tag) {
   MatmulArgs a = {};
@@ -361,7 +361,7 @@ KFB_API int kfb_fused_linear_bwd(const void* dy, const void* x, const void* w, c
     int lines = 0;                                   // of partial sums
     if (m.z) {
       const LinearPair q = {kBackwardTail, xp, w, 0, bias, activation, dyp, m.dz, partial, count, n, k};
-      lines = linear_pair_partials(count, n, k);
+      lines = linear_pair_partials(count, n);
       KFB_TRY(launch_linear_pair(s, q, "fused_linear_dz"));
     } else if (m.again) {
       const MatmulTail tail = {1, activation, bias, dyp, wide, precise ? 3 : 1, partial};

@@ -672,7 +672,7 @@ KFB_API int kfb_pair_block_fwd(const kfb_pair_block* blk, const void* z, void* z
  *   r = scale x + sigmoid(gate) u         (each of scale, gate may be NULL: one; x or u may be NULL: nothing)
  *   y = weight LayerNorm(r) + bias        (norm 1; either may be NULL)
  *   y = sigmoid(g) LayerNorm(r) + v       (norm 2: gate_shift rows are [g | v], 2c wide)
- * with r as it is stored, of stream_dtype.  Output gate and adaptive norm as in
+ * with r as it is stored, of stream_dtype (numbers below 2^-126 are zeros).  Output gate and adaptive norm as in
  * src/kfold/model/layers/folding/diffusion_transformer.py:73-81 and src/kfold/model/primitives/normalization.py:117-125, the
  * state decay as in src/kfold/model/model.py:523-529.
  *   x, r       : (rows, c) stream_dtype;  u, y : (rows, c) compute_dtype; both bf16, both fp32, or a fp32 stream with bf16.
@@ -720,6 +720,7 @@ KFB_API int kfb_expand(const void* values, const void* exponents, void* x, long 
  *   activation f : 0 none, 1 sigmoid, 2 silu, 3 gelu (with the error function), 4 relu.
  *   residual, out : (rows, n) of out_dtype (KFB_BF16, or KFB_FP32: always with KFB_FP32_PRECISE);  dy : of dy_dtype likewise.
  *   dw : (n, k) of dw_dtype, dbias : fp32; dx : (rows, k) as x.  Gradients that are NULL are not computed.
+ * With KFB_BF16 dz is rounded to bf16 as an operand of dx and dw, not in dbias.
  * k, n multiples of 8 up to 65536, tensors on 16-byte boundaries.  Workspace: `wanted` 0 for the forward pass, else the sum of 1 (dx),
  * 2 (dw), 4 (dbias); out_dtype: the result's, or dy's; it may be none.  Another device may need another size.
  */

@@ -10,6 +10,7 @@
 // to row; a block leaves a row of partial sums, added up likewise.  No atomics: the order hangs on the sizes alone.  The rows of residual_norm.cu, r from 8 bits where it was kept so:
 //   shared gates   40 us, 3.9 TB/s: 254 registers, the sums of a gate row among them, leave eight warps an SM, whose sums over a row wait on one another
 //   gates of their own, float32 stream   79 us, 5.0 TB/s          128 channels   31 us, 4.3 TB/s, of which 4 are the sums over the blocks
+//   768 float32 channels, gates of their own   148 us, 4.6 TB/s                   shared   101 us, 3.4 TB/s
 #include <mutex>
 
 #include "ops_common.cuh"
